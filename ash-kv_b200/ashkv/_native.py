@@ -76,6 +76,14 @@ SIGNATURES: dict[str, tuple] = {
     "ashkv_migrate_pages": (_I32, [_P, _P, _P, _P, _P, _I64, _P, _P, _P, _I32, _P, _P, _I32, _I32, _I32, _I64, _P,
                                    _F32, _U64, _I32, _P, _P, _P]),
     "ashkv_release_slots": (_I32, [_P, _P, _I32, _P, _P, _P]),
+    "ashkv_decode_scratch_floats": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "ashkv_decode_attention": (_I32, [_P, _P, _I64, _I64, _I32, _I32, _P, _I64, _I32, _P, _P, _P, _I32, _F32, _P,
+                                      _I64, _F32, _P, _P, _P, _P, _P]),
+    "ashkv_page_bounds": (_I32, [_P, _P, _P, _I32, _P, _P, _P, _P, _P]),
+    "ashkv_select_scratch_floats": (_I64, [_I32, _I32, _I32]),
+    "ashkv_select_pages": (_I32, [_P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _I64, _P, _I64, _I32, _P, _I32,
+                                  _I32, _I32, _I32, _P, _P, _P, _P, _P]),
+    "ashkv_evict_pages": (_I32, [_P, _I64, _P, _I64, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P]),
 }
 
 
@@ -534,3 +542,72 @@ def release_slots(released, count, max_entries: int, stores, status=None) -> Non
     _require_cuda(released, count, status)
     check(lib().ashkv_release_slots(released.data_ptr(), count.data_ptr(), max_entries, ctypes.addressof(stores),
                                     _ptr(status), stream_handle(released.device)), "release_slots")
+
+
+# --------------------------------------------------------------------------- paged attention
+class PagedKVDesc(ctypes.Structure):
+    """ashkv_paged_kv_t."""
+    _fields_ = [("d_tier", ctypes.c_void_p), ("d_layer_id", ctypes.c_void_p), ("d_token_start", ctypes.c_void_p),
+                ("d_page_slot", ctypes.c_void_p), ("n_pages", ctypes.c_int64), ("d_layer_k", ctypes.c_void_p),
+                ("d_layer_v", ctypes.c_void_p), ("pool_tokens", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("n_layers", ctypes.c_int32), ("tokens_per_page", ctypes.c_int32), ("heads_kv", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("outlier_cap", ctypes.c_int32), ("stores", ctypes.c_void_p)]
+
+
+def _check_text(status: int, what: str) -> None:
+    """``check`` with the library's own words for a refused argument."""
+    if status == BAD_ARGUMENT:
+        raise KernelError(what, status, f"{status_string(status)} ({lib().ashkv_last_error().decode()})")
+    check(status, what)
+
+
+def decode_scratch_floats(n_seqs: int, heads_q: int, heads_kv: int, head_dim: int, pages_per_list: int,
+                          with_mass: bool) -> int:
+    return int(lib().ashkv_decode_scratch_floats(n_seqs, heads_q, heads_kv, head_dim, pages_per_list, int(with_mass)))
+
+
+def decode_attention(desc: PagedKVDesc, q: torch.Tensor, page_ids: torch.Tensor, lengths: torch.Tensor,
+                     selected: Optional[torch.Tensor], selected_count: Optional[torch.Tensor], scale: float,
+                     page_mass: Optional[torch.Tensor], decay: float, out: torch.Tensor,
+                     lse: Optional[torch.Tensor], scratch: torch.Tensor, status: Optional[torch.Tensor]) -> None:
+    """q [n_seqs, heads_q, head_dim] bf16 (unit inner stride) over the pages of ``desc`` -> out, lse, page_mass."""
+    n_seqs, heads_q = q.shape[0], q.shape[1]
+    _check_text(lib().ashkv_decode_attention(
+        ctypes.addressof(desc), q.data_ptr(), q.stride(0), q.stride(1), n_seqs, heads_q, page_ids.data_ptr(),
+        page_ids.stride(0), page_ids.shape[1], lengths.data_ptr(), _ptr(selected), _ptr(selected_count),
+        0 if selected is None else selected.shape[2], scale, _ptr(page_mass),
+        0 if page_mass is None else page_mass.stride(0), decay, out.data_ptr(), _ptr(lse), scratch.data_ptr(),
+        _ptr(status), stream_handle(q.device)), "decode_attention")
+
+
+def page_bounds(desc: PagedKVDesc, pages: torch.Tensor, count: Optional[torch.Tensor], valid: Optional[torch.Tensor],
+                codes: torch.Tensor, exponents: torch.Tensor, status: Optional[torch.Tensor]) -> None:
+    _check_text(lib().ashkv_page_bounds(
+        ctypes.addressof(desc), pages.data_ptr(), _ptr(count), pages.numel(), _ptr(valid), codes.data_ptr(),
+        exponents.data_ptr(), _ptr(status), stream_handle(pages.device)), "page_bounds")
+
+
+def select_scratch_floats(n_seqs: int, heads_kv: int, max_pages: int) -> int:
+    return int(lib().ashkv_select_scratch_floats(n_seqs, heads_kv, max_pages))
+
+
+def select_pages(q: torch.Tensor, codes: torch.Tensor, exponents: torch.Tensor, page_ids: torch.Tensor,
+                 lengths: torch.Tensor, tokens_per_page: int, budget: int, sink: int, recent: int,
+                 selected: torch.Tensor, count: torch.Tensor, scratch: torch.Tensor,
+                 status: Optional[torch.Tensor]) -> None:
+    n_seqs, heads_q, head_dim = q.shape
+    _check_text(lib().ashkv_select_pages(
+        q.data_ptr(), q.stride(0), q.stride(1), n_seqs, heads_q, codes.shape[1], head_dim, codes.data_ptr(),
+        exponents.data_ptr(), codes.shape[0], page_ids.data_ptr(), page_ids.stride(0), page_ids.shape[1],
+        lengths.data_ptr(), tokens_per_page, budget, sink, recent, selected.data_ptr(), count.data_ptr(),
+        scratch.data_ptr(), _ptr(status), stream_handle(q.device)), "select_pages")
+
+
+def evict_pages(page_mass: torch.Tensor, page_ids: torch.Tensor, lengths: torch.Tensor, tokens_per_page: int,
+                budget: int, sink: int, recent: int, out_ids: torch.Tensor, out_mass: torch.Tensor,
+                out_lengths: torch.Tensor, evicted: torch.Tensor, evicted_count: torch.Tensor) -> None:
+    _check_text(lib().ashkv_evict_pages(
+        page_mass.data_ptr(), page_mass.stride(0), page_ids.data_ptr(), page_ids.stride(0), lengths.data_ptr(),
+        page_ids.shape[0], page_ids.shape[1], tokens_per_page, budget, sink, recent, out_ids.data_ptr(),
+        out_mass.data_ptr(), out_lengths.data_ptr(), evicted.data_ptr(), evicted_count.data_ptr(),
+        stream_handle(page_ids.device)), "evict_pages")

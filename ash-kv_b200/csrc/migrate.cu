@@ -44,6 +44,7 @@
 #include "fp8_conv.cuh"
 #include "int4_group.cuh"
 #include "nbit_group.cuh"
+#include "page_layout.cuh"
 
 namespace ashkv {
 namespace {
@@ -55,20 +56,10 @@ constexpr int kWarps = kThreads / 32;
 #define kNT int(blockDim.x)
 #define kNW int(blockDim.x >> 5)
 __host__ __device__ constexpr int block_threads(int row) { return row >= 1024 ? 256 : row / 4; }
-constexpr int kTiers = 6;
 constexpr int kBatch = 32;
 constexpr int kMaxElems = 65536;  // 128 KiB of staging; outlier indices fit in 16 bits
 constexpr int kDirectBlocks = 3;  // CTAs per SM of the direct pass (registers <= 85)
 constexpr int kStagedBlocks = 3;  // CTAs per SM of the staged pass (registers <= 85, 3 x 68 KiB)
-
-struct Store {
-  uint8_t* data;
-  int64_t slot_bytes;
-  int32_t n_slots;
-  int32_t format;
-  int32_t* free_stack;
-  int32_t* free_top;
-};
 
 struct MigParams {
   int8_t* tier;
@@ -100,20 +91,6 @@ struct Entry {
   uint64_t kbase, vbase;  // K / V row of the page's first token in the pool
   int32_t page, cur, tgt, layer, ts, old_slot, new_slot, status;
 };
-
-__host__ __device__ __forceinline__ int64_t int8_codes_offset(int T) { return (4 * int64_t(T) + 15) / 16 * 16; }
-
-// Slot layouts (E elements, offsets in bytes):
-//   INT8   [2T fp16 scales | pad to 16 | E int8 codes]           (the hooks' per-token layout)
-//   FP8    [E e4m3fn bytes]
-//   INT4   [E/64 bf16 scales | E/2 nibble bytes]                 (INT4Codec, group 64)
-//   NBIT*  [u32 n_out, 3 x u32 0 | E/32 bf16 delta | E*bits/8 codes | cap x u32 outliers]
-//          outlier entry = (element index in the page << 16) | bf16 bits, ascending
-__host__ __device__ __forceinline__ int64_t nbit_delta_off() { return 16; }
-__host__ __device__ __forceinline__ int64_t nbit_codes_off(int64_t E) { return 16 + E / 16; }
-__host__ __device__ __forceinline__ int64_t nbit_entries_off(int64_t E, int bits) {
-  return nbit_codes_off(E) + E * bits / 8;
-}
 
 int64_t slot_bytes_for(int32_t format, int64_t E, int32_t cap) {
   int64_t b = -1;
@@ -166,12 +143,6 @@ __device__ __forceinline__ uint16_t* pool_chunk(const MigParams& p, const Entry&
   return pool_row(p, en, k / CPR) + (k % CPR) * 8;
 }
 
-// 16-byte asynchronous global -> shared copy: no register staging, so every
-// chunk of a page can be in flight at once; cp.async.wait_all completes them.
-__device__ __forceinline__ void cp_async16(uint32_t smem_addr, const void* gptr) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_addr), "l"(gptr) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ uint2 ld_nc_v2(const void* p) {
   uint2 r;
   asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
@@ -1015,23 +986,6 @@ ashkv_status_t launch_migrate(const MigParams& p, bool xcode_direct, size_t raw_
   const int64_t gs = std::min<int64_t>(p.max_entries, int64_t(sms) * kStagedBlocks * CTA_SCALE);
   migrate_pages_kernel<ROW, kStaged><<<unsigned(gs > 0 ? gs : 1), NT, stage_smem, st>>>(p);
   return check_launch("migrate_pages (staged pass)");
-}
-
-bool copy_stores(const ashkv_tier_store_t* stores, Store (&out)[kTiers], bool need_data) {
-  if (!stores) return false;
-  for (int t = 0; t < kTiers; ++t) {
-    const ashkv_tier_store_t& s = stores[t];
-    out[t] = Store{static_cast<uint8_t*>(s.d_data), s.slot_bytes, s.n_slots, s.format, s.d_free_stack, s.d_free_top};
-    if (t == 0) {
-      if (s.format != ASHKV_PAGE_BF16) return false;
-      continue;
-    }
-    if (s.format == ASHKV_PAGE_NONE) continue;
-    if (s.format < ASHKV_PAGE_INT8 || s.format > ASHKV_PAGE_NBIT2) return false;
-    if (s.n_slots < 0 || s.n_slots > 0xFFFFFF || !s.d_free_stack || !s.d_free_top) return false;
-    if (need_data && (!s.d_data || !aligned(s.d_data, 16) || s.slot_bytes % 16)) return false;
-  }
-  return true;
 }
 
 }  // namespace

@@ -480,6 +480,132 @@ ASHKV_API ashkv_status_t ashkv_page_features(const float* d_token_saliency, cons
                                              int64_t n_k, int32_t tokens_per_page, float* d_s_raw, float* d_S,
                                              float* d_N, void* stream);
 
+/* ========================================================================
+ * Attention of one new token per sequence over tiered, paged KV.  No
+ * counterpart in the reference, whose engine promotes a compressed page
+ * before it attends it (ashkv/runtime/migrate.py:35-191): here every page is
+ * read where its tier keeps it, so a demoted page costs its compressed bytes.
+ *
+ * ashkv_paged_kv_t (a host struct, read during the call) describes the pages
+ * as ashkv_migrate_pages does: page p is tokens_per_page tokens of heads_kv *
+ * head_dim channels; in the BF16 tier its rows are at token d_token_start[p]
+ * of layer d_layer_id[p] (K at d_layer_k[l] + token * row_stride elements, V
+ * likewise, pool_tokens rows each), else it is slot d_page_slot[p] of
+ * stores[d_tier[p]].  Sequence b's token t is token t % tokens_per_page of
+ * page d_page_ids[b * page_ids_stride + t / tokens_per_page].
+ *
+ * For t < d_lengths[b] and query head h (key head h / (heads_q / heads_kv)):
+ *   s[h,t] = scale * q[b,h] . K[t],  P[h,:] = softmax(s[h,:]),
+ *   out[b,h] = sum_t P[h,t] V[t]  (bf16),  lse[b,h] = log sum_t exp s[h,t].
+ * K and V are the numbers the page's codes stand for: the bf16 values, INT8
+ * code * scale / 127, INT4 (nibble - 8) * scale / 7, FP8 the e4m3 number,
+ * none rounded to bf16, and for the dithered formats the bf16 values that
+ * their decoder gives.  Sums and softmax statistics are fp32.  A sequence
+ * without tokens gives 0 and -inf.  Tokens past the length are not used,
+ * whatever their page holds.
+ *   d_selected (may be NULL): [n_seqs, heads_kv, max_selected] page positions;
+ *   key head h then attends only positions d_selected[b,h,i], i <
+ *   d_selected_count[b,h] (as ashkv_select_pages writes them).
+ *   d_page_mass (may be NULL, not with d_selected): fp32 [n_seqs, max_pages]
+ *   with row stride mass_stride; for each page position j that holds tokens
+ *   mass[b,j] = decay * mass[b,j] + sum over h and the page's tokens of P[h,t].
+ * A page that does not exist (id, tier, layer, slot or token range outside
+ * its table) is left out and sets ASHKV_FLAG_INDEX_RANGE in *d_status (if
+ * given), as does a length or count beyond max_pages / max_selected, which is
+ * cut there.  d_q: bf16 with unit element stride and the given strides (in
+ * elements); d_out: contiguous bf16; d_lse (may be NULL): fp32 [n_seqs,
+ * heads_q].  head_dim is 64 or 128; with stores, heads_kv * head_dim and
+ * tokens_per_page have the limits of ashkv_migrate_pages.  n_seqs * heads_q
+ * is at most 2^24.  d_scratch: ashkv_decode_scratch_floats(...) floats
+ * (pages_per_list = max_selected with d_selected, else max_pages), 16-byte
+ * aligned, used by this call alone until it has run.
+ * ======================================================================== */
+typedef struct {
+  const int8_t* d_tier;          /* [n_pages] */
+  const int32_t* d_layer_id;     /* [n_pages] */
+  const int32_t* d_token_start;  /* [n_pages] */
+  const int32_t* d_page_slot;    /* [n_pages] */
+  int64_t n_pages;
+  const uint64_t* d_layer_k;     /* [n_layers] device addresses, 16-byte aligned */
+  const uint64_t* d_layer_v;
+  int64_t pool_tokens;           /* rows of each layer's K and V */
+  int64_t row_stride;            /* elements, a multiple of 8 */
+  int32_t n_layers;
+  int32_t tokens_per_page;
+  int32_t heads_kv;
+  int32_t head_dim;
+  int32_t outlier_cap;           /* of the dithered stores */
+  const ashkv_tier_store_t* stores; /* host array of six */
+} ashkv_paged_kv_t;
+
+ASHKV_API int64_t ashkv_decode_scratch_floats(int32_t n_seqs, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+                                              int32_t pages_per_list, int32_t with_mass);
+ASHKV_API ashkv_status_t ashkv_decode_attention(
+    const ashkv_paged_kv_t* kv, const void* d_q, int64_t q_seq_stride, int64_t q_head_stride, int32_t n_seqs,
+    int32_t heads_q, const int32_t* d_page_ids, int64_t page_ids_stride, int32_t max_pages, const int32_t* d_lengths,
+    const int32_t* d_selected, const int32_t* d_selected_count, int32_t max_selected, float scale, float* d_page_mass,
+    int64_t mass_stride, float decay, void* d_out, float* d_lse, float* d_scratch, uint32_t* d_status, void* stream);
+
+/* ========================================================================
+ * Page selection by key bounds.  No counterpart in the reference.
+ * ashkv_page_bounds writes, for each entry i < (d_count ? min(*d_count,
+ * max_entries) : max_entries) of d_list (page p in the BF16 tier, its first
+ * d_valid[i] tokens, all of them without d_valid) and each key head:
+ *   e = the smallest integer >= -100 with max |k| <= 127 * 2^e,
+ *   d_codes[p, head, 0, d] = floor(min_t k[t,d] / 2^e),
+ *   d_codes[p, head, 1, d] = ceil(max_t k[t,d] / 2^e)       (int8),
+ *   d_exponents[p, head] = e                                (int8),
+ * so that the codes bound every key of the page.  NaN keys are ignored,
+ * infinite ones count as the largest finite bf16; a channel without a number
+ * (and a page without tokens) gives 0.  A page outside the table or in
+ * another tier is skipped and sets ASHKV_FLAG_INDEX_RANGE.
+ * ashkv_select_pages scores the pages of each sequence for each key head:
+ *   q8 = rint(q / 2^f), f the exponent of the query head as above (elements
+ *        that are not finite count as 0),
+ *   score[b, head, j] = max over the head's query heads of
+ *        2^(f + e) * sum_d max(q8[d] * lo[d], q8[d] * hi[d])      (lo <= hi)
+ * -- whole numbers times a power of two, so the scores, and with them the
+ * selection, are exact -- and writes to d_selected[b, head, 0 .. budget) the
+ * positions, ascending, of the first `sink` pages, the last `recent` pages
+ * and the highest scores up to `budget` (all pages where there are no more;
+ * of equal scores the lower position), then -1, and their number to
+ * d_selected_count.  A page id outside the bounds table scores -inf and sets
+ * ASHKV_FLAG_INDEX_RANGE.  sink + recent <= budget, budget >= 1.
+ * d_scratch: ashkv_select_scratch_floats(...) floats.
+ * ======================================================================== */
+ASHKV_API ashkv_status_t ashkv_page_bounds(const ashkv_paged_kv_t* kv, const int32_t* d_list, const int32_t* d_count,
+                                           int32_t max_entries, const int32_t* d_valid, int8_t* d_codes,
+                                           int8_t* d_exponents, uint32_t* d_status, void* stream);
+ASHKV_API int64_t ashkv_select_scratch_floats(int32_t n_seqs, int32_t heads_kv, int32_t max_pages);
+ASHKV_API ashkv_status_t ashkv_select_pages(const void* d_q, int64_t q_seq_stride, int64_t q_head_stride,
+                                            int32_t n_seqs, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+                                            const int8_t* d_codes, const int8_t* d_exponents, int64_t n_pages,
+                                            const int32_t* d_page_ids, int64_t page_ids_stride, int32_t max_pages,
+                                            const int32_t* d_lengths, int32_t tokens_per_page, int32_t budget,
+                                            int32_t sink, int32_t recent, int32_t* d_selected,
+                                            int32_t* d_selected_count, float* d_scratch, uint32_t* d_status,
+                                            void* stream);
+
+/* ========================================================================
+ * Eviction by accumulated attention (the mass that ashkv_decode_attention
+ * keeps).  No counterpart in the reference.  A sequence with more than
+ * `budget` pages keeps its first `sink` pages, its last `recent` pages and,
+ * up to budget, the pages of greatest mass (of equal mass the lower position;
+ * NaN counts as the least); the others leave it:
+ *   d_out_page_ids, d_out_mass [n_seqs, max_pages]: the kept pages in their
+ *       order, then -1 / 0;  d_out_lengths[b]: the tokens left;
+ *   d_evicted [n_seqs, max_pages]: the pages that left, in their order, then
+ *       -1;  d_evicted_count[b].
+ * 1 <= recent, sink + recent <= budget.  Outputs are contiguous and must not
+ * overlap the inputs.  A length beyond max_pages pages is cut there.
+ * ======================================================================== */
+ASHKV_API ashkv_status_t ashkv_evict_pages(const float* d_page_mass, int64_t mass_stride, const int32_t* d_page_ids,
+                                           int64_t page_ids_stride, const int32_t* d_lengths, int32_t n_seqs,
+                                           int32_t max_pages, int32_t tokens_per_page, int32_t budget, int32_t sink,
+                                           int32_t recent, int32_t* d_out_page_ids, float* d_out_mass,
+                                           int32_t* d_out_lengths, int32_t* d_evicted, int32_t* d_evicted_count,
+                                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,611 @@
+"""GPU tests of the paged serving operators against float64.
+
+Tolerances, from the arithmetic and not from runs.  With u = 2^-24:
+  a score is an fp32 sum of dim exact products, scaled by a few factors:
+      |ds| <= (dim + 16) * u * size,  size = max_t scale * sum_d |q_d k_d|, plus
+      4 u |s| for the scale and 2^-22 of a weight for exp2;
+  a weight is then off by a factor of at most 1 + dp, dp = 2 max|ds| + 2^-20;
+  weights are rounded once before the product with V: 2^-11 (fp16) or, in two
+      bf16 parts, 2^-16; the product accumulates in fp32 over the tokens;
+  the result is rounded to bf16: 2^-8 of its value.
+So |out - exact| <= 2^-8 |exact| + (2^-11 + 2 dp + n u) * sum_t P |v|.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import oracle
+from oracle import attention as O
+
+from ashkv import _native as N
+from ashkv.runtime import attention as A
+from ashkv.runtime.batch import DevicePageTable, KVLayers, TierStore
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+CAP = 512
+TIER = {N.PAGE_BF16: 0, N.PAGE_INT8: 1, N.PAGE_FP8: 1, N.PAGE_INT4: 2, N.PAGE_NBIT4: 2, N.PAGE_NBIT2: 3}
+
+
+def bits(t: torch.Tensor) -> np.ndarray:
+    return t.cpu().contiguous().view(torch.int16).numpy().view(np.uint16)
+
+
+class Cache:
+    """A page table over ``layers`` pool layers with each page in a random place of its format's tier."""
+
+    def __init__(self, dev, formats, T, heads, dim, seed=0, layers=2, std=1.0, pool_bits=None):
+        g = np.random.default_rng(seed)
+        self.T, self.heads, self.dim, self.formats = T, heads, dim, list(formats)
+        n, row = len(self.formats), heads * dim
+        fill = torch.Generator().manual_seed(seed)
+        pages = (torch.randn(n, 2 * T * row, generator=fill) * std)
+        pages[:, ::701] *= 6.0
+        self.bits = bits(pages.to(torch.bfloat16)) if pool_bits is None else pool_bits
+        spots = g.permutation(layers * n)[:n]
+        layer, start = spots % layers, spots // layers * T
+        pool = np.zeros((2, layers, n * T, row), np.uint16)
+        pool[:] = 0x7FC0  # NaN wherever no page of the BF16 tier lives
+        tier, slot = np.zeros(n, np.int8), np.full(n, -1, np.int32)
+        self.values, stores = [], {}
+        for fmt in sorted(set(self.formats) - {N.PAGE_BF16}):
+            stores[TIER[fmt]] = TierStore(fmt, n, dev, T, row, CAP if fmt in (N.PAGE_NBIT4, N.PAGE_NBIT2) else 0)
+        slots = {t: np.full((n, s.slot_bytes), 0xFF, np.uint8) for t, s in stores.items()}
+        free = {t: list(g.permutation(n)) for t in stores}
+        for i, fmt in enumerate(self.formats):
+            x = self.bits[i]
+            if fmt == N.PAGE_BF16:
+                pool[0, layer[i], start[i]:start[i] + T] = x[:T * row].reshape(T, row)
+                pool[1, layer[i], start[i]:start[i] + T] = x[T * row:].reshape(T, row)
+                self.values.append(O.page_values(fmt, x, T, heads, dim))
+                continue
+            data, _, n_out = oracle.page_encode(fmt, x, T, row, page_id=i, outlier_cap=CAP)
+            assert n_out <= CAP
+            tier[i], slot[i] = TIER[fmt], free[TIER[fmt]].pop()
+            slots[TIER[fmt]][slot[i], :len(data)] = data
+            self.values.append(O.page_values(fmt, data, T, heads, dim, CAP))
+        for t, s in stores.items():
+            s.data[:n * s.slot_bytes].copy_(torch.from_numpy(slots[t].reshape(-1)))
+        up = lambda a: torch.from_numpy(a).to(dev)  # noqa: E731
+        z = torch.zeros(n, device=dev)
+        self.table = DevicePageTable(z, z, z, z, up(tier), up(np.zeros(n, np.int32)), up(layer.astype(np.int32)),
+                                     up(start.astype(np.int32)), up(slot))
+        tens = [[up(pool[i, l].view(np.int16)).view(torch.bfloat16).view(n * T, heads, dim) for l in range(layers)]
+                for i in range(2)]
+        self.kv = KVLayers(tens[0], tens[1])
+        self.stores = stores
+
+    def lists(self, page_ids, lengths):
+        T = self.T
+        return [[[(j, self.values[page_ids[b][j]]) for j in range(-(-int(lengths[b]) // T))]] * self.heads
+                for b in range(len(lengths))]
+
+
+def queries(n, hq, dim, seed, std=1.0):
+    g = torch.Generator().manual_seed(1000 + seed)
+    return (torch.randn(n, hq, dim, generator=g) * std).to(torch.bfloat16)
+
+
+def check(got, lse, want, dim, n_tokens, mass=None, acc=None, decay=1.0):
+    out = got.double().cpu().numpy()
+    ds = (dim + 20) * U * want["size"]
+    dp = 2 * ds + 2.0 ** -20
+    tol = 2.0 ** -8 * np.abs(want["out"]) + (2.0 ** -11 + 2 * dp + n_tokens * U)[..., None] * want["reach"] + 1e-37
+    assert np.isfinite(out).all()
+    worst = np.max(np.abs(out - want["out"]) / tol) if out.size else 0.0
+    assert worst <= 1.0, f"result off by {worst} of its tolerance"
+    l = lse.double().cpu().numpy()
+    none = np.isneginf(want["lse"])
+    assert (np.isneginf(l) == none).all()
+    t = (ds + 2.0 ** -19 + 8 * U * np.abs(want["lse"], where=~none, out=np.zeros_like(l)))[~none]
+    assert (np.abs(l[~none] - want["lse"][~none]) <= t).all()
+    if mass is not None:
+        m = mass.double().cpu().numpy()
+        drawn = want["mass"] - np.where(want["mass"] != acc, decay * acc, want["mass"])
+        tm = (2 * dp.max() + 2.0 ** -19 + n_tokens * U) * np.abs(drawn) + 8 * U * (np.abs(acc) + np.abs(want["mass"]))
+        assert (np.abs(m - want["mass"]) <= tm).all(), np.max(np.abs(m - want["mass"]) / (tm + 1e-300))
+
+
+FORMATS = {"bf16": [N.PAGE_BF16], "int8": [N.PAGE_INT8], "fp8": [N.PAGE_FP8], "int4": [N.PAGE_INT4],
+           "nbit4": [N.PAGE_NBIT4], "nbit2": [N.PAGE_NBIT2],
+           "mixed": [N.PAGE_BF16, N.PAGE_INT8, N.PAGE_INT4, N.PAGE_NBIT2],
+           "mixed8": [N.PAGE_FP8, N.PAGE_NBIT4, N.PAGE_BF16, N.PAGE_NBIT2]}
+
+
+def run_case(dev, tiers, T, heads_q, heads, dim, lengths, seed, with_mass=True, decay=0.75, std=1.0):
+    P = max(1, max(-(-x // T) for x in lengths))
+    n = len(lengths) * P
+    g = np.random.default_rng(seed)
+    kinds = FORMATS[tiers]
+    c = Cache(dev, [kinds[i] for i in g.integers(0, len(kinds), n)], T, heads, dim, seed, std=std)
+    ids = g.permutation(n).astype(np.int32).reshape(len(lengths), P)
+    q = queries(len(lengths), heads_q, dim, seed, 2.0)
+    acc = g.random((len(lengths), P), dtype=np.float32)
+    mass = torch.from_numpy(acc.copy()).to(dev) if with_mass else None
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    L = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    out, lse = A.decode_attention(q.to(dev), c.table, c.kv, c.stores, torch.from_numpy(ids).to(dev), L,
+                                  tokens_per_page=T, page_mass=mass, decay=decay, return_lse=True, status=status)
+    want = O.decode_attention(q.double().numpy(), c.lists(ids, lengths), lengths, T, dim ** -0.5, acc, decay)
+    assert int(status) == 0
+    check(out, lse, want, dim, max(lengths) + 1, mass, acc, decay)
+    return c, ids, q, out, lse, mass
+
+
+@pytest.mark.parametrize("tiers", list(FORMATS))
+@pytest.mark.parametrize("heads_q,heads,dim", [(8, 2, 128), (3, 1, 128), (4, 4, 64), (16, 2, 64)])
+def test_decode_formats(cuda, tiers, heads_q, heads, dim):
+    run_case(cuda, tiers, 16, heads_q, heads, dim, [70, 0, 1, 16, 33, 257], 1)
+
+
+@pytest.mark.parametrize("tiers", ["bf16", "mixed", "int4"])
+@pytest.mark.parametrize("heads_q,heads", [(8, 8), (7, 1), (8, 1), (9, 1), (16, 1), (17, 1), (40, 2)])
+def test_decode_head_layouts(cuda, tiers, heads_q, heads):
+    run_case(cuda, tiers, 16, heads_q, heads, 128, [50, 131], 2)
+
+
+@pytest.mark.parametrize("T,tiers", [(1, "bf16"), (5, "bf16"), (7, "bf16"), (24, "bf16"), (8, "mixed"), (12, "int8"),
+                                     (20, "int4"), (32, "mixed8"), (40, "mixed"), (64, "int8")])
+def test_decode_page_sizes(cuda, T, tiers):
+    run_case(cuda, tiers, T, 4, 2, 128, [1, T, T + 1, 3 * T - 1, 150], 3)
+
+
+@pytest.mark.parametrize("tiers", ["bf16", "int8", "int4"])
+def test_decode_many_sequences_and_one_long(cuda, tiers):
+    run_case(cuda, tiers, 16, 4, 2, 64, [(37 * i) % 90 for i in range(150)], 4)
+    run_case(cuda, tiers, 16, 4, 2, 64, [4001], 5)
+
+
+@pytest.mark.parametrize("tiers", ["bf16", "int8", "mixed"])
+@pytest.mark.parametrize("std", [1e-3, 30.0])
+def test_decode_value_ranges(cuda, tiers, std):
+    """Small values, and scores in the hundreds (one token takes the whole row)."""
+    run_case(cuda, tiers, 16, 4, 2, 128, [100, 17], 6, std=std)
+
+
+def test_decode_no_tokens_and_no_sequences(cuda):
+    c = Cache(cuda, [N.PAGE_BF16] * 4, 16, 2, 64)
+    ids = torch.arange(4, dtype=torch.int32, device=cuda).view(2, 2)
+    q = queries(2, 4, 64, 0).to(cuda)
+    zero = torch.zeros(2, dtype=torch.int32, device=cuda)
+    mass = torch.ones(2, 2, device=cuda)
+    out, lse = A.decode_attention(q, c.table, c.kv, None, ids, zero, page_mass=mass, decay=0.5, return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all() and (mass == 1).all()
+    out, lse = A.decode_attention(q, c.table, c.kv, None, ids[:, :0], zero, return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    assert A.decode_attention(q[:0], c.table, c.kv, None, ids[:0], zero[:0]).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("fmt", [N.PAGE_BF16, N.PAGE_FP8, N.PAGE_INT8, N.PAGE_INT4, N.PAGE_NBIT2])
+def test_tokens_past_the_length_do_not_count(cuda, fmt):
+    """A page that ends inside its last tile may hold anything behind its last token."""
+    T, heads, dim, length = 16, 2, 128, 21
+    a = Cache(cuda, [fmt, fmt], T, heads, dim, 7)
+    page = np.concatenate([a.bits[1].reshape(2, T, -1)], 0).copy()
+    ids = torch.arange(2, dtype=torch.int32, device=cuda).view(1, 2)
+    L = torch.tensor([length], dtype=torch.int32, device=cuda)
+    q = queries(1, 8, dim, 7).to(cuda)
+    ref = A.decode_attention(q, a.table, a.kv, a.stores, ids, L)
+    if fmt == N.PAGE_BF16:
+        l, s = int(a.table.layer[1]), int(a.table.token_start[1])
+        for t, junk in enumerate((float("nan"), float("inf"), -float("inf"), 3e38)):
+            for x in (a.kv.k[l], a.kv.v[l]):
+                x[s + length - T + t::T][:1] = junk
+                x[s + length - T + 4:s + T] = float("nan")
+    else:
+        st = a.stores[TIER[fmt]]
+        slot = st.slot_view()[int(a.table.slot[1])]
+        row = heads * dim
+        if fmt == N.PAGE_INT8:  # scales and codes of the unused rows
+            for r in list(range(5, T)) + list(range(T + 5, 2 * T)):
+                slot[2 * r:2 * r + 2] = torch.tensor([0xFF, 0x7F], dtype=torch.uint8)
+        elif fmt == N.PAGE_FP8:
+            for r in list(range(5, T)) + list(range(T + 5, 2 * T)):
+                slot[r * row:(r + 1) * row] = 0x7F
+        elif fmt == N.PAGE_INT4:
+            for r in list(range(5, T)) + list(range(T + 5, 2 * T)):
+                slot[r * row // 32:(r + 1) * row // 32] = 0xFF
+        else:
+            for r in list(range(5, T)) + list(range(T + 5, 2 * T)):
+                slot[16 + r * row // 16:16 + (r + 1) * row // 16] = 0xFF
+    got = A.decode_attention(q, a.table, a.kv, a.stores, ids, L)
+    assert torch.isfinite(got).all() and torch.equal(got, ref)
+    assert page.size
+
+
+def test_decode_nan_and_inf_in_use_come_through(cuda):
+    c = Cache(cuda, [N.PAGE_BF16] * 2, 16, 1, 64, 8)
+    ids = torch.arange(2, dtype=torch.int32, device=cuda).view(1, 2)
+    L = torch.tensor([32], dtype=torch.int32, device=cuda)
+    q = queries(1, 2, 64, 8).to(cuda)
+    l, s = int(c.table.layer[0]), int(c.table.token_start[0])
+    c.kv.v[l][s + 3, 0, 5] = float("nan")
+    out = A.decode_attention(q, c.table, c.kv, None, ids, L)
+    assert torch.isnan(out[..., 5]).all() and torch.isfinite(out[..., :5]).all()
+    c.kv.k[l][s + 3, 0, 5] = float("nan")
+    out, lse = A.decode_attention(q, c.table, c.kv, None, ids, L, return_lse=True)
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
+
+
+def test_all_scores_minus_infinity(cuda):
+    c = Cache(cuda, [N.PAGE_BF16], 16, 1, 64, 9)
+    l, s = int(c.table.layer[0]), int(c.table.token_start[0])
+    c.kv.k[l][s:s + 16] = -float("inf")
+    out, lse = A.decode_attention(torch.ones(1, 1, 64, dtype=torch.bfloat16, device=cuda), c.table, c.kv, None,
+                                  torch.zeros(1, 1, dtype=torch.int32, device=cuda),
+                                  torch.tensor([16], dtype=torch.int32, device=cuda), return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+def test_decode_strides_shared_pages_and_out(cuda):
+    """A query cut out of a fused projection, a block table with spare columns, one page in two rows."""
+    T, heads, dim = 16, 2, 128
+    c = Cache(cuda, [N.PAGE_INT8, N.PAGE_BF16, N.PAGE_INT8, N.PAGE_BF16], T, heads, dim, 10)
+    ids = torch.full((3, 9), 77, dtype=torch.int32, device=cuda)
+    ids[:, :3] = torch.tensor([[0, 1, 2], [0, 1, 3], [0, 0, 1]], dtype=torch.int32)
+    L = torch.tensor([40, 48, 33], dtype=torch.int32, device=cuda)
+    fused = torch.randn(3, 12 * dim + 6, device=cuda).bfloat16()
+    q = fused[:, 3:3 + 8 * dim].unflatten(1, (8, dim))
+    mass = torch.zeros(3, 11, device=cuda)
+    out = torch.full((3, 8, dim), 7.0, dtype=torch.bfloat16, device=cuda)
+    back, lse = A.decode_attention(q, c.table, c.kv, c.stores, ids[:, :3], L, page_mass=mass[:, 4:7], out=out,
+                                   return_lse=True)
+    assert back is out and (mass[:, :4] == 0).all() and (mass[:, 7:] == 0).all()
+    want = O.decode_attention(q.double().cpu().numpy(), c.lists(ids.cpu().numpy(), L.cpu().numpy()), L.cpu().numpy(),
+                              T, dim ** -0.5, np.zeros((3, 3)), 1.0)
+    check(out, lse, want, dim, 49, mass[:, 4:7].contiguous(), np.zeros((3, 3)))
+    swapped = q.transpose(0, 1).contiguous().transpose(0, 1)  # heads outermost
+    assert torch.equal(A.decode_attention(swapped, c.table, c.kv, c.stores, ids[:, :3], L), out)
+
+
+def test_decode_bad_pages_are_left_out_and_flagged(cuda):
+    T, heads, dim = 16, 2, 64
+    fmts = [N.PAGE_BF16, N.PAGE_INT8, N.PAGE_BF16, N.PAGE_INT8, N.PAGE_BF16, N.PAGE_BF16]
+    c = Cache(cuda, fmts, T, heads, dim, 11)
+    q = queries(1, 4, dim, 11).to(cuda)
+    full = torch.tensor([6 * T], dtype=torch.int32, device=cuda)
+    ids = torch.arange(6, dtype=torch.int32, device=cuda).view(1, 6)
+    good = {name: getattr(c.table, name).clone() for name in ("tier", "slot", "layer", "token_start")}
+
+    def status_of(ids_, L):
+        st = torch.zeros(1, dtype=torch.int32, device=cuda)
+        out, lse = A.decode_attention(q, c.table, c.kv, c.stores, ids_, L, return_lse=True, status=st)
+        return out, lse, int(st)
+
+    without = O.decode_attention(q.double().cpu().numpy(), [[[(j, c.values[j]) for j in (0, 2, 3, 4, 5)]] * heads],
+                                 [6 * T], T, dim ** -0.5)
+    for name, value in (("tier", 3), ("tier", -1), ("tier", 6), ("slot", -1), ("slot", 6)):
+        getattr(c.table, name)[1] = value
+        out, lse, st = status_of(ids, full)
+        assert st == N.FLAG_INDEX_RANGE, name
+        check(out, lse, without, dim, 6 * T)
+        getattr(c.table, name).copy_(good[name])
+    without = O.decode_attention(q.double().cpu().numpy(), [[[(j, c.values[j]) for j in (0, 1, 3, 4, 5)]] * heads],
+                                 [6 * T], T, dim ** -0.5)
+    for name, value in (("layer", -1), ("layer", 2), ("token_start", -1), ("token_start", 6 * T - T + 1)):
+        getattr(c.table, name)[2] = value
+        out, lse, st = status_of(ids, full)
+        assert st == N.FLAG_INDEX_RANGE, name
+        check(out, lse, without, dim, 6 * T)
+        getattr(c.table, name).copy_(good[name])
+    for bad in (-1, 6, 2 ** 31 - 1):
+        ids2 = ids.clone()
+        ids2[0, 2] = bad
+        out, lse, st = status_of(ids2, full)
+        assert st == N.FLAG_INDEX_RANGE
+        check(out, lse, without, dim, 6 * T)
+    # a length beyond the list is cut there, a negative one is none
+    ref = status_of(ids, full)
+    out, lse, st = status_of(ids, full + 5)
+    assert st == N.FLAG_INDEX_RANGE and torch.equal(out, ref[0]) and torch.equal(lse, ref[1])
+    out, lse, st = status_of(ids, torch.full_like(full, -3))
+    assert st == N.FLAG_INDEX_RANGE and (out == 0).all()
+
+
+def test_decode_offsets_beyond_32_bits(cuda):
+    """Pool rows and slots that lie more than 2^32 bytes from their base."""
+    T, heads, dim = 16, 8, 128
+    tokens = (1 << 32) // (heads * dim * 2) + 4 * T
+    k = torch.empty(tokens, heads, dim, dtype=torch.bfloat16, device=cuda)
+    v = torch.empty(tokens, heads, dim, dtype=torch.bfloat16, device=cuda)
+    far = tokens - T
+    g = torch.Generator().manual_seed(12)
+    kp, vp = (torch.randn(T, heads, dim, generator=g).bfloat16() for _ in range(2))
+    k[far:], v[far:] = kp.to(cuda), vp.to(cuda)
+    row = heads * dim
+    n_slots = (1 << 32) // N.page_slot_bytes(N.PAGE_INT8, T, row) + 3
+    store = TierStore(N.PAGE_INT8, n_slots, cuda, T, row)
+    page = bits((torch.randn(2 * T * row, generator=g)).bfloat16())
+    data = oracle.page_encode(N.PAGE_INT8, page, T, row)[0]
+    store.slot_view()[n_slots - 1, :len(data)] = torch.from_numpy(data).to(cuda)
+    z, i32 = torch.zeros(2, device=cuda), lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    table = DevicePageTable(z, z, z, z, torch.tensor([0, 1], dtype=torch.int8, device=cuda), i32(0, 0), i32(0, 0),
+                            i32(far, 0), i32(-1, n_slots - 1))
+    q = queries(1, 16, dim, 12)
+    out, lse = A.decode_attention(q.to(cuda), table, KVLayers([k], [v]), {1: store}, i32(0, 1).view(1, 2), i32(30),
+                                  return_lse=True)
+    vals = [(kp.double().numpy(), vp.double().numpy()), O.page_values(N.PAGE_INT8, data, T, heads, dim)]
+    want = O.decode_attention(q.double().numpy(), [[list(enumerate(vals))] * heads], [30], T, dim ** -0.5)
+    check(out, lse, want, dim, 30)
+    bounds = A.PageBounds.empty(2, heads, dim, cuda)
+    bounds.update(table, KVLayers([k], [v]), i32(0))
+    codes, exps = O.page_bounds(vals[0][0], T)
+    assert np.array_equal(bounds.codes[0].cpu().numpy(), codes) and np.array_equal(bounds.exponents[0].cpu().numpy(), exps)
+
+
+def test_decode_streams_and_graphs(cuda):
+    """The same call on two side streams at once, and two captured graphs replayed together."""
+    c = Cache(cuda, [N.PAGE_BF16, N.PAGE_INT8, N.PAGE_INT4, N.PAGE_NBIT2] * 8, 16, 2, 128, 13)
+    ids = torch.randperm(32, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(2, 16).to(cuda)
+    L = torch.tensor([250, 101], dtype=torch.int32, device=cuda)
+    qs = [queries(2, 8, 128, 20 + i).to(cuda) for i in range(2)]
+    want = [A.decode_attention(q, c.table, c.kv, c.stores, ids, L) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = []
+    for q, s in zip(qs, streams):
+        with torch.cuda.stream(s):
+            got.append(A.decode_attention(q, c.table, c.kv, c.stores, ids, L))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs, ins, masses = [], [], [], []
+    for q in qs:
+        ins.append(q.clone())
+        masses.append(torch.zeros(2, 16, device=cuda))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(A.decode_attention(ins[-1], c.table, c.kv, c.stores, ids, L, page_mass=masses[-1], decay=0.5))
+        graphs.append(g)
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    # three replays of decay 0.5: 1 + 1/2 + 1/4 of a step's mass
+    once = torch.zeros(2, 16, device=cuda)
+    A.decode_attention(qs[0], c.table, c.kv, c.stores, ids, L, page_mass=once, decay=0.5)
+    assert torch.allclose(masses[0], 1.75 * once, rtol=8 * 2.0 ** -23)
+    ins[0].copy_(qs[1])  # a graph reads its inputs anew
+    L.fill_(60)
+    graphs[0].replay()
+    assert torch.equal(outs[0], A.decode_attention(qs[1], c.table, c.kv, c.stores, ids, L))
+
+
+# ----------------------------------------------------------------------------- bounds
+@pytest.mark.parametrize("heads,dim,T", [(2, 128, 16), (8, 64, 16), (1, 128, 5), (3, 64, 40)])
+def test_page_bounds(cuda, heads, dim, T):
+    n = 12
+    c = Cache(cuda, [N.PAGE_BF16] * n, T, heads, dim, 30, layers=2)
+    special = [0.0, -0.0, float("inf"), -float("inf"), float("nan"), 1e-38, -1e-38, 3e38, 127.0, 127.5, 2.0 ** -130]
+    g = np.random.default_rng(3)
+    for i in range(n // 2):  # half of the pages get special values
+        l, s = int(c.table.layer[i]), int(c.table.token_start[i])
+        for x in special:
+            c.kv.k[l][s + int(g.integers(T)), int(g.integers(heads)), int(g.integers(dim))] = x
+    l, s = int(c.table.layer[0]), int(c.table.token_start[0])
+    c.kv.k[l][s:s + T, 0] = 0.0
+    c.kv.k[l][s:s + T, 0, 3] = float("nan")
+    b = A.PageBounds.empty(n, heads, dim, cuda)
+    b.codes.fill_(55), b.exponents.fill_(9)
+    pages = torch.tensor([0, 1, 2, 3, 7, 8, 9], dtype=torch.int32, device=cuda)
+    valid = [T, T - 1, 1, 0, T, max(1, T // 2), T + 9]
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    b.update(c.table, c.kv, pages, valid=torch.tensor(valid, dtype=torch.int32, device=cuda), tokens_per_page=T,
+             status=status)
+    assert int(status) == 0
+    listed = dict(zip(pages.tolist(), valid))
+    for p in range(n):
+        if p not in listed:
+            assert (b.codes[p] == 55).all() and (b.exponents[p] == 9).all()
+            continue
+        l, s = int(c.table.layer[p]), int(c.table.token_start[p])
+        codes, exps = O.page_bounds(c.kv.k[l][s:s + T].double().cpu().numpy(), min(listed[p], T))
+        assert np.array_equal(b.exponents[p].cpu().numpy(), exps), p
+        assert np.array_equal(b.codes[p].cpu().numpy(), codes), p
+
+
+def test_page_bounds_count_and_bad_pages(cuda):
+    c = Cache(cuda, [N.PAGE_BF16, N.PAGE_INT8, N.PAGE_BF16, N.PAGE_BF16], 16, 2, 64, 31)
+    b = A.PageBounds.empty(4, 2, 64, cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    pages = torch.tensor([0, 2, 3], dtype=torch.int32, device=cuda)
+    b.update(c.table, c.kv, pages, count=torch.tensor([2], dtype=torch.int32, device=cuda), status=status)
+    assert int(status) == 0 and (b.codes[3] == 0).all() and (b.codes[2] != 0).any()
+    was = b.codes.clone()
+    for bad in (1, -1, 4):  # a compressed page, ids outside the table
+        status.zero_()
+        b.update(c.table, c.kv, torch.tensor([bad], dtype=torch.int32, device=cuda), status=status)
+        assert int(status) == N.FLAG_INDEX_RANGE and torch.equal(b.codes, was)
+    c.table.token_start[3] = 4 * 16 - 15
+    status.zero_()
+    b.update(c.table, c.kv, pages, status=status)
+    assert int(status) == N.FLAG_INDEX_RANGE and torch.equal(b.codes, was)
+    b.update(c.table, c.kv, pages[:0])
+
+
+# ----------------------------------------------------------------------------- selection
+def select_want(q, b, ids, lengths, T, budget, sink, recent):
+    codes, exps = b.codes.cpu().numpy(), b.exponents.cpu().numpy()
+    group = q.shape[1] // codes.shape[1]
+    want = []
+    for i in range(len(lengths)):
+        row = []
+        for h in range(codes.shape[1]):
+            pages = ids[i][:max(0, -(-int(lengths[i]) // T))]
+            score = O.page_scores(q[i, h * group:(h + 1) * group].double().numpy(), codes[pages, h], exps[pages, h])
+            row.append(O.keep_highest(score, budget, sink, recent))
+        want.append(row)
+    return want
+
+
+def check_selected(sel, cnt, want):
+    sel, cnt = sel.cpu().numpy(), cnt.cpu().numpy()
+    for i, row in enumerate(want):
+        for h, keep in enumerate(row):
+            assert cnt[i, h] == len(keep)
+            assert sel[i, h, :len(keep)].tolist() == keep, (i, h)
+            assert (sel[i, h, len(keep):] == -1).all()
+
+
+@pytest.mark.parametrize("heads_q,heads,dim", [(8, 2, 128), (4, 4, 64), (6, 1, 128), (40, 2, 64)])
+@pytest.mark.parametrize("budget,sink,recent", [(1, 0, 0), (3, 1, 2), (10, 0, 1), (40, 4, 4), (500, 1, 1)])
+def test_select_pages(cuda, heads_q, heads, dim, budget, sink, recent):
+    T, lengths = 16, [0, 1, 16, 900, 2000, 305]
+    P = 130
+    g = torch.Generator().manual_seed(40)
+    n = P * 3
+    b = A.PageBounds.empty(n, heads, dim, cuda)
+    lo = torch.randint(-127, 60, (n, heads, dim), generator=g)
+    hi = (lo + torch.randint(0, 60, (n, heads, dim), generator=g)).clamp_max(127)
+    b.codes.copy_(torch.stack((lo, hi), 2).to(torch.int8))
+    b.exponents.copy_(torch.randint(-3, 3, (n, heads), generator=g).to(torch.int8))
+    ids = torch.randint(0, n, (len(lengths), P + 5), generator=g).to(torch.int32)  # pages repeat: ties
+    q = queries(len(lengths), heads_q, dim, 41)
+    q[3, 0, :4] = torch.tensor([float("nan"), float("inf"), -float("inf"), 1e-38])
+    q[4] = 0.0  # every score alike
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    sel, cnt = A.select_pages(q.to(cuda), b, ids.to(cuda)[:, :P], torch.tensor(lengths, dtype=torch.int32, device=cuda),
+                              budget, sink=sink, recent=recent, tokens_per_page=T, status=status)
+    assert int(status) == 0
+    check_selected(sel, cnt, select_want(q, b, ids[:, :P].numpy(), lengths, T, budget, sink, recent))
+
+
+def test_select_long_row_and_bad_ids(cuda):
+    T, n = 16, 5000
+    g = torch.Generator().manual_seed(42)
+    b = A.PageBounds.empty(n, 1, 64, cuda)
+    b.codes.copy_(torch.randint(-127, 128, b.codes.shape, generator=g).sort(2).values.to(torch.int8))  # lo <= hi
+    ids = torch.randperm(n, generator=g).to(torch.int32).view(1, n)
+    q = queries(1, 2, 64, 43)
+    L = torch.tensor([n * T - 3], dtype=torch.int32, device=cuda)
+    sel, cnt = A.select_pages(q.to(cuda), b, ids.to(cuda), L, 700, sink=2, recent=3)
+    check_selected(sel, cnt, select_want(q, b, ids.numpy(), [n * T - 3], T, 700, 2, 3))
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    bad = ids.clone()
+    bad[0, 100] = -5
+    bad[0, 200] = n
+    sel, cnt = A.select_pages(q.to(cuda), b, bad.to(cuda), L, n - 2, sink=0, recent=0, status=status)
+    assert int(status) == N.FLAG_INDEX_RANGE and int(cnt) == n - 2
+    assert not ({100, 200} & set(sel[0, 0].tolist()))  # the two that do not exist come last
+    status.zero_()
+    A.select_pages(q.to(cuda), b, ids.to(cuda), L + 100, 5, status=status)
+    assert int(status) == N.FLAG_INDEX_RANGE
+
+
+def test_selected_attention(cuda):
+    """Each key head attends its own pages; padding, wrong positions and an empty list."""
+    T, heads, dim, P = 16, 2, 128, 12
+    kinds = [N.PAGE_BF16, N.PAGE_INT8, N.PAGE_INT4, N.PAGE_NBIT2]
+    c = Cache(cuda, [kinds[i % 4] for i in range(2 * P)], T, heads, dim, 44)
+    ids = np.random.default_rng(5).permutation(2 * P).astype(np.int32).reshape(2, P)
+    lengths = [P * T - 7, 100]
+    q = queries(2, 8, dim, 44)
+    sel = torch.full((2, heads, 6), -1, dtype=torch.int32)
+    rows = {(0, 0): [0, 3, 11], (0, 1): [1, 2, 5, 7, 8, 11], (1, 0): [], (1, 1): [6]}
+    cnt = torch.zeros(2, heads, dtype=torch.int32)
+    for (b, h), r in rows.items():
+        sel[b, h, :len(r)] = torch.tensor(r, dtype=torch.int32)
+        cnt[b, h] = len(r)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    args = (q.to(cuda), c.table, c.kv, c.stores, torch.from_numpy(ids).to(cuda),
+            torch.tensor(lengths, dtype=torch.int32, device=cuda))
+    out, lse = A.decode_attention(*args, selected=sel.to(cuda), selected_count=cnt.to(cuda), return_lse=True,
+                                  status=status)
+    lists = [[[(j, c.values[ids[b, j]]) for j in rows[b, h]] for h in range(heads)] for b in range(2)]
+    want = O.decode_attention(q.double().numpy(), lists, lengths, T, dim ** -0.5)
+    assert int(status) == 0
+    check(out, lse, want, dim, 12 * T)
+    sel[0, 0, 1] = 40  # a position that the sequence does not have
+    lists[0][0] = [e for e in lists[0][0] if e[0] != 3]
+    cnt[1, 1] = 9      # more than the list holds: cut, its padding left out
+    out, lse = A.decode_attention(*args, selected=sel.to(cuda), selected_count=cnt.to(cuda), return_lse=True,
+                                  status=status)
+    assert int(status) == N.FLAG_INDEX_RANGE
+    check(out, lse, O.decode_attention(q.double().numpy(), lists, lengths, T, dim ** -0.5), dim, 12 * T)
+
+
+# ----------------------------------------------------------------------------- eviction
+@pytest.mark.parametrize("budget,sink,recent", [(1, 0, 1), (4, 1, 3), (9, 2, 1), (64, 1, 1), (2000, 3, 5)])
+def test_evict_pages(cuda, budget, sink, recent):
+    T, P = 16, 1500
+    lengths = [0, 5, 16 * 9, 16 * 9 + 1, 16 * 1500, 23001, 16 * 64]
+    g = torch.Generator().manual_seed(50)
+    mass = torch.rand(len(lengths), P + 3, generator=g)
+    mass[4, ::2] = 0.25                      # ties
+    mass[5, 3::5] = float("nan")
+    mass[5, 4::50] = -0.0
+    mass[5, 7::50] = 0.0
+    mass[5, 8::50] = -1.0
+    mass[5, 9::50] = float("inf")
+    mass[6] = 0.0
+    ids = torch.randint(0, 1 << 30, (len(lengths), P + 9), generator=g).to(torch.int32)
+    m, i = mass.to(cuda)[:, :P], ids.to(cuda)[:, 2:2 + P]
+    L = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    got = A.evict_pages(m, i, L, budget, sink=sink, recent=recent, tokens_per_page=T)
+    ids, mass = ids[:, 2:2 + P].numpy(), mass[:, :P].numpy()
+    for b, n in enumerate(lengths):
+        pages = -(-n // T)
+        keep = O.keep_highest(mass[b, :pages].astype(np.float64), budget, sink, recent)
+        gone = sorted(set(range(pages)) - set(keep))
+        assert got.page_ids[b, :len(keep)].tolist() == ids[b, keep].tolist()
+        assert (got.page_ids[b, len(keep):] == -1).all() and (got.page_mass[b, len(keep):] == 0).all()
+        assert np.array_equal(got.page_mass[b, :len(keep)].cpu().numpy(), mass[b, keep], equal_nan=True)
+        assert got.evicted[b, :len(gone)].tolist() == ids[b, gone].tolist() and (got.evicted[b, len(gone):] == -1).all()
+        assert int(got.n_evicted[b]) == len(gone) and int(got.lengths[b]) == n - T * len(gone)
+
+
+def test_refusals(cuda):
+    c = Cache(cuda, [N.PAGE_BF16, N.PAGE_INT8], 16, 2, 64, 60)
+    ids = torch.zeros(1, 2, dtype=torch.int32, device=cuda)
+    L = torch.tensor([16], dtype=torch.int32, device=cuda)
+    q = queries(1, 4, 64, 60).to(cuda)
+    mass = torch.zeros(1, 2, device=cuda)
+    sel, cnt = torch.zeros(1, 2, 1, dtype=torch.int32, device=cuda), torch.ones(1, 2, dtype=torch.int32, device=cuda)
+
+    def no(exc, fn, *a, **k):
+        with pytest.raises(exc):
+            fn(*a, **k)
+
+    D = A.decode_attention
+    no(TypeError, D, q.half(), c.table, c.kv, c.stores, ids, L)
+    no(ValueError, D, q[:, :3], c.table, c.kv, c.stores, ids, L)
+    no(ValueError, D, q[..., ::2], c.table, c.kv, c.stores, ids, L)
+    no(ValueError, D, q.repeat(1, 1, 2), c.table, c.kv, c.stores, ids, L, out=q)
+    no(ValueError, D, q, c.table, c.kv, c.stores, ids[0], L)
+    no(TypeError, D, q, c.table, c.kv, c.stores, ids.long(), L)
+    no(ValueError, D, q, c.table, c.kv, c.stores, ids.cpu(), L)
+    no(ValueError, D, q, c.table, c.kv, c.stores, ids, L.repeat(2))
+    no(ValueError, D, q, c.table, c.kv, c.stores, ids, L, tokens_per_page=0)
+    no(N.KernelError, D, q, c.table, c.kv, c.stores, ids, L, tokens_per_page=17)
+    no(N.KernelError, D, q, c.table, c.kv, c.stores, ids, L, tokens_per_page=32)
+    no(ValueError, D, q, c.table, c.kv, {0: c.stores[1]}, ids, L)
+    no(ValueError, D, q, c.table, c.kv, {6: c.stores[1]}, ids, L)
+    no(ValueError, D, q, c.table, c.kv, c.stores, ids, L, selected=sel)
+    no(ValueError, D, q, c.table, c.kv, c.stores, ids, L, selected=sel, selected_count=cnt, page_mass=mass)
+    no(ValueError, D, q, c.table, c.kv, c.stores, ids, L, selected=sel[..., :0], selected_count=cnt)
+    no(ValueError, D, q, c.table, c.kv, c.stores, ids, L, selected=sel[:, :1], selected_count=cnt)
+    no(ValueError, D, q, c.table, c.kv, c.stores, ids, L, page_mass=mass[:, :1])
+    no(ValueError, D, q, c.table, c.kv, c.stores, ids.expand(2, 2), L.repeat(2),
+       page_mass=mass.expand(2, 2))
+    no(TypeError, D, q, c.table, c.kv, c.stores, ids, L, status=mass[0, :1])
+    b = A.PageBounds.empty(2, 2, 64, cuda)
+    S = A.select_pages
+    no(ValueError, S, q, b, ids, L, 0)
+    no(ValueError, S, q, b, ids, L, 2, sink=2, recent=1)
+    no(ValueError, S, q, b, ids, L, 2, sink=-1)
+    no(ValueError, S, q[:, :3], b, ids, L, 2)
+    no(ValueError, S, torch.zeros(1, 4, 128, dtype=torch.bfloat16, device=cuda), b, ids, L, 2)
+    no(ValueError, A.PageBounds, b.codes[..., :32].contiguous(), b.exponents)
+    no(ValueError, A.PageBounds, b.codes, b.exponents[:1])
+    no(ValueError, A.PageBounds.empty(3, 2, 64, cuda).update, c.table, c.kv, ids[0])
+    no(ValueError, A.PageBounds.empty(2, 1, 64, cuda).update, c.table, c.kv, ids[0])
+    no(ValueError, b.update, c.table, c.kv, ids[0], valid=L)
+    E = A.evict_pages
+    no(ValueError, E, mass, ids, L, 2, recent=0)
+    no(ValueError, E, mass, ids, L, 2, sink=2, recent=1)
+    no(ValueError, E, mass[:, :1], ids, L, 2)
+    no(TypeError, E, mass.double(), ids, L, 2)
