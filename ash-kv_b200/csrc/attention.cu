@@ -13,7 +13,7 @@
 #include <cstdio>
 
 #include "common.cuh"
-#include "fp8_conv.cuh"
+#include "nbit_group.cuh"
 #include "page_layout.cuh"
 
 namespace ashkv {
@@ -21,7 +21,6 @@ namespace {
 
 constexpr int kWarpsA = 4;          // warps of a CTA, each a worker of its own
 constexpr int kWorkersPerSm = 12;   // resident worker warps per SM
-constexpr int kQ = 8;               // query heads of one worker
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kJoinThreads = 128;
@@ -129,80 +128,697 @@ __device__ PageRef resolve(const AttnParams& p, int b, int hk, int i) {
   return r;
 }
 
-// N neighbouring values (columns c .. c + N - 1) of row r of a page (its K rows, then its V rows).
-template <int N, int BITS>
-__device__ __forceinline__ void nbit_values(const AttnParams& p, const uint8_t* slot, int64_t e, float (&x)[N]) {
-  const int64_t E = 2 * int64_t(p.T) * p.row_len;
-  const float delta = bf16_to_f32(reinterpret_cast<const uint16_t*>(slot + nbit_delta_off())[e / 32]);
-  const uint8_t* codes = slot + nbit_codes_off(E);
-  constexpr float half = float((1 << BITS) - 1) * 0.5f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int64_t bit = (e + i) * BITS;
-    const int c = (codes[bit >> 3] >> (8 - BITS - int(bit & 7))) & ((1 << BITS) - 1);
-    x[i] = bf16_to_f32(f32_to_bf16(__fmul_rn(float(c) - half, delta)));
-  }
-  const uint32_t* ent = reinterpret_cast<const uint32_t*>(slot + nbit_entries_off(E, BITS));
-  uint32_t lo = 0, n = min(*reinterpret_cast<const uint32_t*>(slot), uint32_t(p.outlier_cap));
-  for (uint32_t hi = n; lo < hi;) {  // first entry at element e or later
-    const uint32_t mid = (lo + hi) / 2;
-    if ((ent[mid] >> 16) < uint32_t(e)) lo = mid + 1;
-    else hi = mid;
-  }
-  for (; lo < n && (ent[lo] >> 16) < uint32_t(e) + N; ++lo)
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if ((ent[lo] >> 16) == uint32_t(e) + i) x[i] = bf16_to_f32(uint16_t(ent[lo] & 0xFFFFu));
+// ---------------------------------------------------------------- tensor-core pieces
+// D (16 x 8, fp32) += A (16 x 16, row) * B (16 x 8, col).  Lane (g, t) = (lane / 4,
+// lane % 4) holds A rows g and g + 8, k = 2t, 2t + 1, 2t + 8, 2t + 9 (a0 .. a3: row
+// g, row g + 8, then the same for the upper k), B column g at the same k (b0, b1),
+// and D rows g, g + 8 at columns 2t, 2t + 1.
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Transpose of an 8 x 8 matrix of 16-bit values spread over the warp (row g, columns 2t, 2t + 1).
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t f32x2_to_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t r;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// 16 bytes global -> shared; zeros instead when `real` is false (nothing is read then).
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
-__device__ void page_values(const AttnParams& p, const PageRef& pg, int r, int c, float (&x)[N]) {
-  const int64_t e = int64_t(r) * p.row_len + c, E = 2 * int64_t(p.T) * p.row_len;
-  switch (pg.format) {
-    case ASHKV_PAGE_BF16: {
-      const bool isv = r >= p.T;
-      const uint16_t* row = reinterpret_cast<const uint16_t*>(isv ? pg.v : pg.k) + int64_t(isv ? r - p.T : r) * p.row_stride + c;
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = bf16_to_f32(row[i]);
-      break;
-    }
-    case ASHKV_PAGE_INT8: {
-      const float s = f16_to_f32(reinterpret_cast<const uint16_t*>(pg.k)[r]) * (1.0f / 127.0f);
-      const int8_t* q = reinterpret_cast<const int8_t*>(pg.k) + int8_codes_offset(p.T) + e;
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = float(q[i]) * s;
-      break;
-    }
-    case ASHKV_PAGE_FP8: {
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = bf16lo(bf16x2_from_fp8x2(pg.k[e + i]));
-      break;
-    }
-    case ASHKV_PAGE_INT4: {
-      const float s = bf16_to_f32(reinterpret_cast<const uint16_t*>(pg.k)[e / 64]) * (1.0f / 7.0f);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint8_t w = pg.k[E / 32 + (e + i) / 2];
-        x[i] = float(int((e + i) & 1 ? w & 15 : w >> 4) - 8) * s;
-      }
-      break;
-    }
-    case ASHKV_PAGE_NBIT4: nbit_values<N, 4>(p, pg.k, e, x); break;
-    default: nbit_values<N, 2>(p, pg.k, e, x); break;
-  }
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
+// Codes as exact fp16 pairs, by putting them into the low bits of 1024.0 (0x6400)
+// and subtracting what that adds.
+// Bytes (0, 1) or (2, 3) of an int8 word with its sign bits flipped (code + 128):
+__device__ __forceinline__ uint32_t int8_pair(uint32_t flipped, uint32_t sel) {
+  return add_f16x2(__byte_perm(flipped, 0x64646464u, sel), 0xE480E480u);  // - 1152
+}
+// Nibbles at bits 0-3 and 16-19, or at bits 4-7 and 20-23, less 8:
+__device__ __forceinline__ uint32_t nibble_lo(uint32_t w) { return add_f16x2((w & 0x000F000Fu) | 0x64006400u, 0xE408E408u); }
+__device__ __forceinline__ uint32_t nibble_hi(uint32_t w) {  // (1024 + 16 n) / 16 - 72
+  return fma_f16x2((w & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+}
+__device__ __forceinline__ uint32_t fp8_pair(uint32_t c16) {  // two e4m3 bytes -> fp16 pair, exact
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(c16)));
+  return h;
 }
 
-// A warp per (range of pages, key head, up to kQ of its query heads).  Lane l
-// holds channels l * D/32 .. of the queries and of the results.
+// Where row r (token of a tile), 16-byte chunk c of a K or V tile of RB bytes a
+// row sits in shared memory.  The rows a warp reads together (K: tokens g; V:
+// tokens 2t, 2t + 1 and those + 8) fall into different banks.
+template <int RB>
+__device__ __forceinline__ uint32_t k_off(uint32_t r, uint32_t c) {
+  if constexpr (RB >= 128) return r * RB + ((c ^ ((r & 1u) << 2)) << 4);
+  else if constexpr (RB == 64) return r * RB + ((c ^ (r & 2u)) << 4);
+  else return r * RB + (c << 4);
+}
+template <int RB>
+__device__ __forceinline__ uint32_t v_off(uint32_t r, uint32_t c) {
+  if constexpr (RB >= 128) return r * RB + ((c ^ (r & 6u)) << 4);
+  const uint32_t q = (r >> 1) | ((r & 1u) << 3);
+  if constexpr (RB == 64) return q * RB + ((c ^ (q & 2u)) << 4);
+  return q * RB + (c << 4);
+}
+
+// ---------------------------------------------------------------- the pages of a worker
+constexpr int kRing = 3;  // units in shared memory per warp: one in use, two on their way
+
+// A unit is 16 tokens of a page for one key head: the K or the V rows of a BF16
+// page (16 x D bf16), or the codes of both of a compressed page (K first).
+struct Unit {
+  int32_t format;  // BF16, INT8, FP8, INT4; NONE past the end
+  int32_t rows;    // tokens in use
+  int32_t pos;     // page position in the sequence
+  bool is_v, last; // BF16: the V rows; the page's last unit
+  uint32_t scale;  // lane l: scale bits of K row l (l < 16) or V row l - 16
+};
+
 template <int D>
-__global__ void __launch_bounds__(kWarpsA * 32) decode_partials_kernel(const AttnParams p) {
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int w = int(blockIdx.x) * kWarpsA + int(threadIdx.x >> 5);
+struct Feeder {
+  static constexpr int kUnitBytes = 16 * D * 2;
+  const AttnParams& p;
+  int b, hk, i, i1;       // next list entry, end of the segment
+  int64_t tokens;
+  uint32_t ring;          // shared address of the warp's ring
+  int slot, tile;
+  bool second;            // BF16: the V unit of (page, tile) is next
+  PageRef batch;          // lane l: list entry batch0 + l
+  int batch0;
+  PageRef page;           // current page
+  int page_rows;          // its tokens in use
+
+  __device__ __forceinline__ Feeder(const AttnParams& p_, int hk_, uint32_t ring_) : p(p_), hk(hk_), ring(ring_), slot(0) {}
+  __device__ __forceinline__ void start(int b_, int i0, int i1_) {
+    b = b_; i = i0; i1 = i1_; tokens = seq_tokens(p, b); batch0 = i0 - 32; tile = 0; second = false;
+    next_page();
+  }
+  // Makes list entry i, or the next one with tokens, the current page.
+  __device__ void next_page() {
+    const int lane = threadIdx.x & 31;
+    for (; i < i1; ++i) {
+      if (i >= batch0 + 32) {
+        batch0 = i;
+        if (i + lane < i1) batch = resolve(p, b, hk, i + lane);
+      }
+      const int src = i - batch0;
+      page.k = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(batch.k), src));
+      page.v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(batch.v), src));
+      page.format = __shfl_sync(0xFFFFFFFFu, batch.format, src);
+      page.pos = __shfl_sync(0xFFFFFFFFu, batch.pos, src);
+      if (page.format == ASHKV_PAGE_NONE) {
+        if (p.mass)
+          for (int g = lane; g < p.group; g += 32)
+            p.page_lse2[(int64_t(b) * p.max_pages + page.pos) * p.heads_q + hk * p.group + g] = -INFINITY;
+        continue;
+      }
+      page_rows = int(min(int64_t(p.T), tokens - int64_t(page.pos) * p.T));
+      return;
+    }
+    page.format = ASHKV_PAGE_NONE;
+  }
+
+  // Rows of RB bytes: row r of the tile at src + r * stride.
+  template <int RB, bool V>
+  __device__ __forceinline__ void copy_rows(const uint8_t* src, int64_t stride, int rows, uint32_t dst) const {
+    const int lane = threadIdx.x & 31;
+    constexpr int CPR = RB / 16;
+#pragma unroll
+    for (int j = 0; j < CPR / 2; ++j) {
+      const int c = lane + 32 * j, r = c / CPR, col = c % CPR;
+      const bool real = r < rows;
+      cp_async16_or_zero(dst + (V ? v_off<RB>(r, col) : k_off<RB>(r, col)), src + (real ? r * stride + col * 16 : 0), real);
+    }
+  }
+  // Decodes the K or V rows of a dithered page into a BF16 unit.
+  template <int BITS>
+  __device__ void stage_nbit(bool v, int t0, int rows, uint32_t dst) const {
+    const int lane = threadIdx.x & 31;
+    const int64_t E = 2 * int64_t(p.T) * p.row_len;
+    const uint16_t* delta = reinterpret_cast<const uint16_t*>(page.k + nbit_delta_off());
+    const uint8_t* codes = page.k + nbit_codes_off(E);
+    constexpr float half = float((1 << BITS) - 1) * 0.5f;
+    constexpr int GPR = D / 32, RB = D * 2;
+    const int row0 = (v ? p.T : 0) + t0;
+#pragma unroll
+    for (int j = 0; j < GPR / 2; ++j) {
+      const int n = lane + 32 * j, r = n / GPR, k = n % GPR;
+      uint32_t o[16];
+      if (r < rows) {
+        GroupCodes<BITS> gc;
+        load_group<BITS>(delta, codes, (int64_t(row0 + r) * p.row_len + hk * D) / 32 + k, gc);
+        group_bf16<BITS>(gc, half, o);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) o[c] = 0;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        sts128(dst + (v ? v_off<RB>(r, 4 * k + c) : k_off<RB>(r, 4 * k + c)),
+               make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]));
+    }
+    __syncwarp();  // dense values first, then the outliers overwrite theirs
+    const uint32_t n_out = min(*reinterpret_cast<const uint32_t*>(page.k), uint32_t(p.outlier_cap));
+    const uint32_t* ent = reinterpret_cast<const uint32_t*>(page.k + nbit_entries_off(E, BITS));
+    for (uint32_t j = lane; j < n_out; j += 32) {
+      const uint32_t e = ent[j];
+      const uint32_t r = (e >> 16) / uint32_t(p.row_len) - uint32_t(row0);
+      const uint32_t c = (e >> 16) % uint32_t(p.row_len) - uint32_t(hk * D);
+      if (r < uint32_t(rows) && c < uint32_t(D)) {
+        const uint32_t at = dst + (v ? v_off<RB>(r, c >> 3) : k_off<RB>(r, c >> 3)) + (c & 7u) * 2u;
+        asm volatile("st.shared.u16 [%0], %1;" :: "r"(at), "h"(static_cast<uint16_t>(e)) : "memory");
+      }
+    }
+  }
+
+  // Sends the next unit on its way (always one cp.async group) and describes it.
+  __device__ Unit issue() {
+    Unit u{page.format, 0, page.pos, second, true, 0u};
+    if (page.format != ASHKV_PAGE_NONE) {
+      const int lane = threadIdx.x & 31;
+      const int t0 = tile * 16;
+      u.rows = min(16, page_rows - t0);
+      const uint32_t dst = ring + slot * kUnitBytes;
+      bool done = true;  // with this tile
+      if (page.format == ASHKV_PAGE_BF16) {
+        const uint8_t* src = (second ? page.v : page.k) + (int64_t(t0) * p.row_stride + hk * D) * 2;
+        if (second) copy_rows<D * 2, true>(src, p.row_stride * 2, u.rows, dst);
+        else copy_rows<D * 2, false>(src, p.row_stride * 2, u.rows, dst);
+        done = second;
+        second = !second;
+      } else if (page.format >= ASHKV_PAGE_NBIT4) {
+        u.format = ASHKV_PAGE_BF16;
+        if (page.format == ASHKV_PAGE_NBIT4) stage_nbit<4>(second, t0, u.rows, dst);
+        else stage_nbit<2>(second, t0, u.rows, dst);
+        done = second;
+        second = !second;
+      } else {
+        const int64_t row = p.row_len, kr = t0, vr = p.T + t0;
+        const bool mine = (lane & 15) < u.rows;
+        const int64_t srow = (lane < 16 ? kr : vr) + (lane & 15);
+        if (page.format == ASHKV_PAGE_INT4) {
+          const uint8_t* codes = page.k + p.T * row / 16 + hk * (D / 2);  // past E/32 bytes of scales
+          copy_rows<D / 2, false>(codes + kr * (row / 2), row / 2, u.rows, dst);
+          copy_rows<D / 2, true>(codes + vr * (row / 2), row / 2, u.rows, dst + 8 * D);
+          const uint8_t* sc = page.k + (srow * row + hk * D) / 32;
+          if (mine) u.scale = D == 128 ? *reinterpret_cast<const uint32_t*>(sc) : uint32_t(*reinterpret_cast<const uint16_t*>(sc));
+        } else {
+          const bool i8 = page.format == ASHKV_PAGE_INT8;
+          const uint8_t* codes = page.k + (i8 ? int8_codes_offset(p.T) : 0) + hk * D;
+          copy_rows<D, false>(codes + kr * row, row, u.rows, dst);
+          copy_rows<D, true>(codes + vr * row, row, u.rows, dst + 16 * D);
+          if (i8 && mine) u.scale = reinterpret_cast<const uint16_t*>(page.k)[srow];
+        }
+      }
+      u.last = done && t0 + 16 >= page_rows;
+      if (done) {
+        if (u.last) {
+          tile = 0;
+          ++i;
+          next_page();
+        } else {
+          ++tile;
+        }
+      }
+      slot = slot == kRing - 1 ? 0 : slot + 1;
+    }
+    cp_async_commit();
+    return u;
+  }
+};
+
+// ---------------------------------------------------------------- the worker
+// A warp per (range of pages, key head, up to 8 * NT of its query heads).
+//   S (tokens x queries) = K Q^T, then O^T (channels x queries) += V^T P^T: the
+//   tokens and channels fill the 16 rows of the tensor-core tile and the few
+//   queries its 8 columns, so no row is spent on padding.  P leaves the first
+//   product with tokens as rows and enters the second with tokens as k: an 8 x
+//   8 transpose per half tile.
+// Per query (this lane: 2t and 2t + 1) m is the reference of the weights 2^(s -
+// m).  It follows the running maximum only when a score lies more than 2^8 above
+// it, which is rare after the first tiles, so most tiles reduce nothing across
+// the lanes.  acc holds sum_t 2^(s - m) * c * v.  The scale of a compressed V row
+// rides on its weight and its codes enter the product as whole numbers; the power
+// of two c keeps weight * scale inside the fp16 range: c * (largest scale so far)
+// lies in [2^6, 2^7], a weight below 2^8, so the operand stays below 2^15 and is
+// off by at most 2^-25 / c where fp16 runs out of digits, 2^-31 of a largest value.
+template <int D, int NT>
+struct Worker {
+  static constexpr int MT = D / 16;  // channel tiles of 16
+  const AttnParams& p;
+  float acc[NT][MT][4];
+  float m[NT][2], thr[NT][2], l[NT][2], ps[NT][2];  // ps: the page's own sum
+  float c;
+  float qs_b, qs_h[NT][2];  // factors from a raw dot product to a log2 score: bf16 and fp16 queries
+  uint32_t qb, qh;          // the queries in shared memory as bf16 and as fp16 (scaled by a power of two)
+  int lane, g, t;
+  bool fresh;               // no scale was seen yet
+
+  __device__ __forceinline__ Worker(const AttnParams& p_, uint32_t q_smem)
+      : p(p_), qb(q_smem), qh(q_smem + NT * 8 * D * 2), lane(threadIdx.x & 31), g(lane >> 2), t(lane & 3) {}
+
+  // 16-byte chunk k of query row n: rows 2n and 2n + 1 in different halves of the banks, as they are read together.
+  static __device__ __forceinline__ uint32_t qb_off(uint32_t n, uint32_t k) { return n * (D * 2) + ((k ^ ((n & 1u) << 2)) << 4); }
+  static __device__ __forceinline__ uint32_t qh_off(uint32_t n, uint32_t k) { return n * (D * 2) + ((k ^ (n & 1u)) << 4); }
+
+  __device__ void start(int b, int hq0, int nq) {
+    constexpr int N = D / 32;  // channels of a lane here
+    qs_b = p.scale2;
+#pragma unroll
+    for (int half = 0; half < NT; ++half)
+#pragma unroll 2
+    for (int n = 8 * half; n < 8 * half + 8; ++n) {
+      uint16_t x[N];
+      float amax = 0.0f;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        x[k] = n < nq ? p.q[b * p.q_seq_stride + int64_t(hq0 + n) * p.q_head_stride + lane * N + k] : uint16_t(0);
+        const float a = fabsf(bf16_to_f32(x[k]));
+        if (a < INFINITY) amax = fmaxf(amax, a);
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, off));
+      // the largest query value to [2^14, 2^15): fp16 then keeps all 8 bits of every value
+      // down to 2^-31 of it, exactly
+      const int e = min(112, max(-112, int(__float_as_uint(amax) >> 23) - 127 - 14));
+      const float down = __uint_as_float(uint32_t(127 - e) << 23), up = __uint_as_float(uint32_t(127 + e) << 23);
+      if ((n & 7) == 2 * t) qs_h[half][0] = p.scale2 * up;
+      if ((n & 7) == 2 * t + 1) qs_h[half][1] = p.scale2 * up;
+      const uint32_t kb = uint32_t(lane * N) >> 3, in = (uint32_t(lane * N) & 7u) * 2u;
+      if constexpr (N == 4) {
+        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(qb + qb_off(n, kb) + in),
+                     "r"(uint32_t(x[0]) | (uint32_t(x[1]) << 16)), "r"(uint32_t(x[2]) | (uint32_t(x[3]) << 16)) : "memory");
+        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(qh + qh_off(n, kb) + in),
+                     "r"(f32x2_to_f16x2(bf16_to_f32(x[0]) * down, bf16_to_f32(x[1]) * down)),
+                     "r"(f32x2_to_f16x2(bf16_to_f32(x[2]) * down, bf16_to_f32(x[3]) * down)) : "memory");
+      } else {
+        asm volatile("st.shared.u32 [%0], %1;" :: "r"(qb + qb_off(n, kb) + in), "r"(uint32_t(x[0]) | (uint32_t(x[1]) << 16)) : "memory");
+        asm volatile("st.shared.u32 [%0], %1;" :: "r"(qh + qh_off(n, kb) + in),
+                     "r"(f32x2_to_f16x2(bf16_to_f32(x[0]) * down, bf16_to_f32(x[1]) * down)) : "memory");
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        m[n][j] = 0.0f; thr[n][j] = -INFINITY; l[n][j] = 0.0f; ps[n][j] = 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < MT; ++k)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[n][k][x] = 0.0f;
+    }
+    c = 0x1p-8f;  // weights reach 2^8: with bf16 pages alone the sums hold any mean of bf16 values
+    fresh = true;
+    __syncwarp();
+  }
+
+  __device__ __forceinline__ void scale_acc(int n, float f0, float f1) {
+#pragma unroll
+    for (int k = 0; k < MT; ++k) {
+      acc[n][k][0] *= f0; acc[n][k][1] *= f1; acc[n][k][2] *= f0; acc[n][k][3] *= f1;
+    }
+  }
+  static __device__ __forceinline__ float max_over_tokens(float x) {  // over the lanes of the same queries
+    x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
+    x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
+    return fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
+  }
+
+  // log2 scores (token g: s[0], s[1]; token g + 8: s[2], s[3]) -> weights 2^(s - m), added up.
+  __device__ __forceinline__ void weights(float (&s)[NT][4], int rows) {
+    if (rows < 16) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (g >= rows) s[n][0] = s[n][1] = -INFINITY;
+        if (g + 8 >= rows) s[n][2] = s[n][3] = -INFINITY;
+      }
+    }
+    bool over = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      over |= fmaxf(s[n][0], s[n][2]) > thr[n][0] || fmaxf(s[n][1], s[n][3]) > thr[n][1];
+    if (__any_sync(0xFFFFFFFFu, over)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float f[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float top = max_over_tokens(fmaxf(s[n][j], s[n][j + 2]));
+          f[j] = 1.0f;
+          if (top > thr[n][j]) {
+            if (thr[n][j] != -INFINITY) f[j] = ex2(m[n][j] - top);
+            m[n][j] = top;
+            thr[n][j] = top + 8.0f;
+            l[n][j] *= f[j];
+            ps[n][j] *= f[j];
+          }
+        }
+        scale_acc(n, f[0], f[1]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[n][x] = ex2(s[n][x] - m[n][x & 1]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float sum = s[n][j] + s[n][j + 2];
+        l[n][j] += sum;
+        ps[n][j] += sum;
+      }
+    }
+  }
+
+  // Makes room for V rows of scale x (this lane's, 0 where it holds none; K of them).
+  __device__ __forceinline__ void fit_scale(float x) {
+    if (!__any_sync(0xFFFFFFFFu, fresh || x * c > 128.0f)) return;
+    const float top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, x > 0.0f ? __float_as_uint(x) : 0u));
+    if (top > 0x1p-100f && top < 0x1p100f) {  // c * top to [2^6, 2^7)
+      const float next = __uint_as_float(uint32_t(254 + 6 - int(__float_as_uint(top) >> 23)) << 23);
+      const float f = next / c;  // a power of two
+#pragma unroll
+      for (int n = 0; n < NT; ++n) scale_acc(n, f, f);
+      c = next;
+      fresh = false;
+    }
+  }
+  // Weights times c and a row scale, as the fp16 operand of the product with V: b[k][n][0] tokens
+  // 0-7, b[k][n][1] tokens 8-15.  w[k] = scale of row g, of row g + 8 for scale group k.
+  template <int K>
+  __device__ __forceinline__ void fp16_weights(const float (&s)[NT][4], const float (&w)[K][2], uint32_t (&b)[K][NT][2]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float w0 = w[k][0] * c, w1 = w[k][1] * c;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        b[k][n][0] = transpose8(f32x2_to_f16x2(s[n][0] * w0, s[n][1] * w0));
+        b[k][n][1] = transpose8(f32x2_to_f16x2(s[n][2] * w1, s[n][3] * w1));
+      }
+    }
+  }
+
+  // Scores of a tile of BF16 keys.
+  __device__ __forceinline__ void bf16_scores(uint32_t tile, int rows, float (&s)[NT][4]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const uint4 ka = lds128(tile + k_off<D * 2>(g, 4 * i + t)), kb = lds128(tile + k_off<D * 2>(g + 8, 4 * i + t));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint4 q = lds128(qb + qb_off(8 * n + g, 4 * i + t));
+        mma16816<true>(s[n], ka.x, kb.x, ka.y, kb.y, q.x, q.y);
+        mma16816<true>(s[n], ka.z, kb.z, ka.w, kb.w, q.z, q.w);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[n][x] *= qs_b;
+    weights(s, rows);
+  }
+  // Adds a tile of BF16 values: the weights in two bf16 parts (8 + 8 bits), as a single one would
+  // cost as much accuracy as the rounding of the result.
+  __device__ __forceinline__ void bf16_values(uint32_t tile, const float (&s)[NT][4]) {
+    uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x0 = s[n][2 * h] * c, x1 = s[n][2 * h + 1] * c;
+        const uint32_t top = f32x2_to_bf16x2(x0, x1);
+        hi[n][h] = transpose8(top);
+        lo[n][h] = transpose8(f32x2_to_bf16x2(x0 - bf16lo(top), x1 - bf16hi(top)));
+      }
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      uint32_t v[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 x = lds128(tile + v_off<D * 2>(2 * t + (k & 1) + 8 * (k >> 1), g + 8 * i));
+        v[k][0] = x.x; v[k][1] = x.y; v[k][2] = x.z; v[k][3] = x.w;
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5410), a1 = __byte_perm(v[0][w], v[1][w], 0x7632);
+        const uint32_t a2 = __byte_perm(v[2][w], v[3][w], 0x5410), a3 = __byte_perm(v[2][w], v[3][w], 0x7632);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma16816<true>(acc[n][4 * i + w], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+          mma16816<true>(acc[n][4 * i + w], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+        }
+      }
+    }
+  }
+
+  // A tile of a page of 8-bit codes, K then V.
+  template <bool INT8>
+  __device__ __forceinline__ void tile8(uint32_t tile, const Unit& u) {
+    float ks0 = 1.0f, ks1 = 1.0f;
+    float vs[1][2] = {{1.0f, 1.0f}};
+    if constexpr (INT8) {
+      const float x = f16_to_f32(uint16_t(u.scale)) * (1.0f / 127.0f);
+      ks0 = __shfl_sync(0xFFFFFFFFu, x, g);
+      ks1 = __shfl_sync(0xFFFFFFFFu, x, g + 8);
+      vs[0][0] = __shfl_sync(0xFFFFFFFFu, x, g + 16);
+      vs[0][1] = __shfl_sync(0xFFFFFFFFu, x, g + 24);
+      fit_scale(lane < 16 ? 0.0f : x);
+    } else {
+      fit_scale(1.0f);
+    }
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const uint4 xa = lds128(tile + k_off<D>(g, 4 * i + t)), xb = lds128(tile + k_off<D>(g + 8, 4 * i + t));
+      const uint32_t ka[4] = {xa.x, xa.y, xa.z, xa.w}, kb[4] = {xb.x, xb.y, xb.z, xb.w};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 q[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) q[n] = lds128(qh + qh_off(8 * n + g, 2 * (4 * i + t) + h));
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint32_t a0, a1, a2, a3;
+          if constexpr (INT8) {
+            const uint32_t fa = ka[2 * h + w] ^ 0x80808080u, fb = kb[2 * h + w] ^ 0x80808080u;
+            a0 = int8_pair(fa, 0x4140); a1 = int8_pair(fb, 0x4140);
+            a2 = int8_pair(fa, 0x4342); a3 = int8_pair(fb, 0x4342);
+          } else {
+            a0 = fp8_pair(ka[2 * h + w]); a1 = fp8_pair(kb[2 * h + w]);
+            a2 = fp8_pair(ka[2 * h + w] >> 16); a3 = fp8_pair(kb[2 * h + w] >> 16);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<false>(s[n], a0, a1, a2, a3, w ? q[n].z : q[n].x, w ? q[n].w : q[n].y);
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[n][x] *= qs_h[n][x & 1] * (x < 2 ? ks0 : ks1);
+    weights(s, u.rows);
+    uint32_t b[1][NT][2];
+    fp16_weights<1>(s, vs, b);
+    tile += 16 * D;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      uint32_t v[4][2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint2 x = lds64(tile + v_off<D>(2 * t + (k & 1) + 8 * (k >> 1), 4 * i + (g >> 1)) + (g & 1) * 8);
+        v[k][0] = INT8 ? x.x ^ 0x80808080u : x.x;
+        v[k][1] = INT8 ? x.y ^ 0x80808080u : x.y;
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // channels 4w + 2h, + 1: (token, next token) bytes side by side
+          const uint32_t lo = __byte_perm(v[0][w], v[1][w], h ? 0x7362 : 0x5140);
+          const uint32_t hi = __byte_perm(v[2][w], v[3][w], h ? 0x7362 : 0x5140);
+          uint32_t a0, a1, a2, a3;
+          if constexpr (INT8) {
+            a0 = int8_pair(lo, 0x4140); a1 = int8_pair(lo, 0x4342);
+            a2 = int8_pair(hi, 0x4140); a3 = int8_pair(hi, 0x4342);
+          } else {
+            a0 = fp8_pair(lo); a1 = fp8_pair(lo >> 16);
+            a2 = fp8_pair(hi); a3 = fp8_pair(hi >> 16);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<false>(acc[n][4 * i + 2 * w + h], a0, a1, a2, a3, b[0][n][0], b[0][n][1]);
+        }
+    }
+  }
+
+  // A tile of an INT4 page (scales per 64 channels), K then V.
+  __device__ __forceinline__ void tile4(uint32_t tile, const Unit& u) {
+    constexpr int K = D / 64;
+    float s[NT][4], vs[K][2], x_max = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float x = (k ? bf16hi(u.scale) : bf16lo(u.scale)) * (1.0f / 7.0f);
+      const float ks0 = __shfl_sync(0xFFFFFFFFu, x, g), ks1 = __shfl_sync(0xFFFFFFFFu, x, g + 8);
+      vs[k][0] = __shfl_sync(0xFFFFFFFFu, x, g + 16);
+      vs[k][1] = __shfl_sync(0xFFFFFFFFu, x, g + 24);
+      x_max = fmaxf(x_max, x);
+      const uint2 xa = lds64(tile + k_off<D / 2>(g, 2 * k + (t >> 1)) + (t & 1) * 8);
+      const uint2 xb = lds64(tile + k_off<D / 2>(g + 8, 2 * k + (t >> 1)) + (t & 1) * 8);
+      float d[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {  // eight channels: byte j = (channel 2j, channel 2j + 1), the first in the high nibble
+        const uint32_t ka = w ? xa.y : xa.x, kb = w ? xb.y : xb.x, ka8 = ka >> 8, kb8 = kb >> 8;
+        const uint32_t a04 = nibble_hi(ka), b04 = nibble_hi(kb), a15 = nibble_lo(ka), b15 = nibble_lo(kb);
+        const uint32_t a26 = nibble_hi(ka8), b26 = nibble_hi(kb8), a37 = nibble_lo(ka8), b37 = nibble_lo(kb8);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4 q = lds128(qh + qh_off(8 * n + g, 2 * (4 * k + t) + w));
+          mma16816<false>(d[n], a04, b04, a15, b15, __byte_perm(q.x, q.z, 0x5410), __byte_perm(q.x, q.z, 0x7632));
+          mma16816<false>(d[n], a26, b26, a37, b37, __byte_perm(q.y, q.w, 0x5410), __byte_perm(q.y, q.w, 0x7632));
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) s[n][y] = fmaf(d[n][y], y < 2 ? ks0 : ks1, s[n][y]);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) s[n][y] *= qs_h[n][y & 1];
+    fit_scale(lane < 16 ? 0.0f : x_max);
+    weights(s, u.rows);
+    uint32_t b[K][NT][2];
+    fp16_weights<K>(s, vs, b);
+    tile += 8 * D;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      uint32_t v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = lds32(tile + v_off<D / 2>(2 * t + (j & 1) + 8 * (j >> 1), 2 * k + (g >> 2)) + (g & 3) * 4);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // bytes 2h, 2h + 1 of both tokens: four channels
+        uint32_t lo = __byte_perm(v[0], v[1], h ? 0x7632 : 0x5410), hi = __byte_perm(v[2], v[3], h ? 0x7632 : 0x5410);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t a0 = nibble_hi(lo), a1 = nibble_lo(lo), a2 = nibble_hi(hi), a3 = nibble_lo(hi);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<false>(acc[n][4 * k + 2 * h + w], a0, a1, a2, a3, b[k][n][0], b[k][n][1]);
+          lo >>= 8;
+          hi >>= 8;
+        }
+      }
+    }
+  }
+
+  static __device__ __forceinline__ float sum_over_tokens(float x) {
+    x += __shfl_xor_sync(0xFFFFFFFFu, x, 4);
+    x += __shfl_xor_sync(0xFFFFFFFFu, x, 8);
+    return x + __shfl_xor_sync(0xFFFFFFFFu, x, 16);
+  }
+  // The log2-sum of the page that just ended, for its mass.
+  __device__ __forceinline__ void page_sum(int b, int pos, int hq0, int nq) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float sum = sum_over_tokens(ps[n][j]);
+        const int q = 8 * n + 2 * t + j;
+        if (g == 0 && q < nq)
+          p.page_lse2[(int64_t(b) * p.max_pages + pos) * p.heads_q + hq0 + q] = m[n][j] + log2f(sum);
+        ps[n][j] = 0.0f;
+      }
+  }
+  // The segment's partial result.
+  __device__ void finish(int64_t row0, int nq) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float sum = sum_over_tokens(l[n][j]);
+        const float inv = sum == 0.0f ? 0.0f : (1.0f / sum) * (1.0f / c);
+        const int q = 8 * n + 2 * t + j;
+        if (q >= nq) continue;
+        if (g == 0) p.part_lse2[row0 + q] = m[n][j] + log2f(sum);
+        float* o = p.part_o + (row0 + q) * D;
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          float x[8];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            x[2 * w] = acc[n][4 * i + w][j] * inv;
+            x[2 * w + 1] = acc[n][4 * i + w][2 + j] * inv;
+          }
+          float4* at = reinterpret_cast<float4*>(o + 64 * i + 8 * g);
+          at[0] = make_float4(x[0], x[1], x[2], x[3]);
+          at[1] = make_float4(x[4], x[5], x[6], x[7]);
+        }
+      }
+  }
+};
+
+template <int D, int NT>
+constexpr int warp_smem() { return kRing * Feeder<D>::kUnitBytes + 2 * NT * 8 * D * 2; }
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarpsA * 32, NT == 1 ? 3 : 2) decode_partials_kernel(const __grid_constant__ AttnParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5;
+  const int w = int(blockIdx.x) * kWarpsA + warp;
   const int cells = p.heads_kv * p.q_chunks;
   const int range = w / cells, cell = w % cells;
   if (range >= p.ranges) return;
-  const int hk = cell % p.heads_kv, q0 = (cell / p.heads_kv) * kQ;
-  const int nq = min(kQ, p.group - q0), hq0 = hk * p.group + q0;
+  const int hk = cell % p.heads_kv, q0 = (cell / p.heads_kv) * (8 * NT);
+  const int nq = min(8 * NT, p.group - q0), hq0 = hk * p.group + q0;
   const int total = lists_before(p, p.n_seqs, hk), len = range_len(p, total);
   int64_t pos = int64_t(range) * len;
   const int64_t end = min(pos + len, int64_t(total));
@@ -213,55 +829,46 @@ __global__ void __launch_bounds__(kWarpsA * 32) decode_partials_kernel(const Att
     if (before + n > pos) break;
     before += n;
   }
+  const uint32_t ring = smem_u32(smem) + uint32_t(warp * warp_smem<D, NT>());
+  Feeder<D> feed(p, hk, ring);
+  Worker<D, NT> work(p, ring + kRing * Feeder<D>::kUnitBytes);
   for (; pos < end; ++b) {
     const int n = list_len(p, b, hk);
     if (n == 0) continue;
     const int i0 = int(pos - before), i1 = int(min(int64_t(n), end - before));
-    float q[kQ][N], o[kQ][N], m[kQ], l[kQ];
-    const int64_t tokens = seq_tokens(p, b);
-    for (int g = 0; g < kQ; ++g) {
-      m[g] = -INFINITY;
-      l[g] = 0.0f;
-      for (int i = 0; i < N; ++i) {
-        o[g][i] = 0.0f;
-        q[g][i] = g < nq ? bf16_to_f32(p.q[b * p.q_seq_stride + (hq0 + g) * p.q_head_stride + lane * N + i]) : 0.0f;
+    feed.slot = 0;
+    feed.start(b, i0, i1);
+    Unit next[kRing];
+#pragma unroll
+    for (int k = 0; k < kRing; ++k) next[k] = feed.issue();
+    work.start(b, hq0, nq);
+    float s[NT][4];  // weights of a BF16 tile between its K and its V unit
+    int slot = 0;
+    while (next[0].format != ASHKV_PAGE_NONE) {
+      cp_async_wait<kRing - 1>();
+      __syncwarp();
+      const Unit u = next[0];
+      const uint32_t tile = ring + slot * Feeder<D>::kUnitBytes;
+      if (u.format == ASHKV_PAGE_BF16) {
+        if (u.is_v) work.bf16_values(tile, s);
+        else work.bf16_scores(tile, u.rows, s);
+      } else if (u.format == ASHKV_PAGE_INT8) {
+        work.template tile8<true>(tile, u);
+      } else if (u.format == ASHKV_PAGE_FP8) {
+        work.template tile8<false>(tile, u);
+      } else {
+        work.tile4(tile, u);
       }
+      __syncwarp();  // every lane has read the unit
+#pragma unroll
+      for (int k = 0; k + 1 < kRing; ++k) next[k] = next[k + 1];
+      next[kRing - 1] = feed.issue();
+      slot = slot == kRing - 1 ? 0 : slot + 1;
+      if (p.mass && u.last) work.page_sum(b, u.pos, hq0, nq);
     }
-    for (int i = i0; i < i1; ++i) {
-      const PageRef pg = resolve(p, b, hk, i);
-      const int nt = pg.format == ASHKV_PAGE_NONE ? 0 : int(min(int64_t(p.T), tokens - int64_t(pg.pos) * p.T));
-      float pm[kQ], pl[kQ];  // the page's own maximum and sum
-      for (int g = 0; g < kQ; ++g) { pm[g] = -INFINITY; pl[g] = 0.0f; }
-      for (int t = 0; t < nt; ++t) {
-        float k[N], v[N];
-        page_values<N>(p, pg, t, hk * D + lane * N, k);
-        page_values<N>(p, pg, p.T + t, hk * D + lane * N, v);
-        for (int g = 0; g < kQ; ++g) {
-          float s = 0.0f;
-          for (int c = 0; c < N; ++c) s = fmaf(q[g][c], k[c], s);
-          for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, off);
-          s *= p.scale2;
-          const float mn = fmaxf(m[g], s), ref = mn == -INFINITY ? 0.0f : mn;
-          const float a = exp2f(m[g] - ref), e = exp2f(s - ref);
-          l[g] = l[g] * a + e;
-          for (int c = 0; c < N; ++c) o[g][c] = fmaf(e, v[c], o[g][c] * a);
-          m[g] = mn;
-          const float pn = fmaxf(pm[g], s), pref = pn == -INFINITY ? 0.0f : pn;
-          pl[g] = pl[g] * exp2f(pm[g] - pref) + exp2f(s - pref);
-          pm[g] = pn;
-        }
-      }
-      if (p.mass && lane == 0)
-        for (int g = 0; g < nq; ++g)
-          p.page_lse2[(int64_t(b) * p.max_pages + pg.pos) * p.heads_q + hq0 + g] =
-              nt > 0 ? (pm[g] == -INFINITY ? 0.0f : pm[g]) + log2f(pl[g]) : -INFINITY;
-    }
-    const int64_t slot = int64_t(range + b) * p.heads_q + hq0;
-    for (int g = 0; g < nq; ++g) {
-      const float inv = l[g] == 0.0f ? 0.0f : 1.0f / l[g];
-      for (int c = 0; c < N; ++c) p.part_o[(slot + g) * D + lane * N + c] = o[g][c] * inv;
-      if (lane == 0) p.part_lse2[slot + g] = (m[g] == -INFINITY ? 0.0f : m[g]) + log2f(l[g]);
-    }
+    cp_async_wait<0>();
+    __syncwarp();
+    work.finish(int64_t(range + b) * p.heads_q + hq0, nq);
     pos = before + i1;
     before += n;
   }
@@ -352,7 +959,12 @@ int ranges_for(int64_t n_seqs, int heads_kv, int q_chunks, int64_t pages_per_lis
   const int64_t fit = std::max<int64_t>(1, int64_t(sms) * kWorkersPerSm / (int64_t(heads_kv) * q_chunks));
   return int(std::max<int64_t>(1, std::min<int64_t>(fit, n_seqs * pages_per_list)));
 }
-int q_chunks_for(int heads_q, int heads_kv) { return (heads_q / heads_kv + kQ - 1) / kQ; }
+// Query heads of one worker: one or two column tiles.
+int worker_queries(int group) { return group <= 8 ? 8 : 16; }
+int q_chunks_for(int heads_q, int heads_kv) {
+  const int group = heads_q / heads_kv, n = worker_queries(group);
+  return (group + n - 1) / n;
+}
 
 bool row_ok(int64_t row) { return row == 128 || row == 256 || row == 512 || row == 1024 || row == 2048; }
 
@@ -393,10 +1005,16 @@ ashkv_status_t refuse(const char* what, const char* why) {
   return ASHKV_BAD_ARGUMENT;
 }
 
-template <int D>
+template <int D, int NT>
 ashkv_status_t launch_decode(const AttnParams& p, cudaStream_t st) {
   const int64_t workers = int64_t(p.ranges) * p.heads_kv * p.q_chunks;
-  decode_partials_kernel<D><<<unsigned((workers + kWarpsA - 1) / kWarpsA), kWarpsA * 32, 0, st>>>(p);
+  constexpr int smem = kWarpsA * warp_smem<D, NT>();
+  const cudaError_t e = cudaFuncSetAttribute(decode_partials_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) {
+    set_error("ashkv_decode_attention (shared memory attribute)", e);
+    return ASHKV_LAUNCH_ERROR;
+  }
+  decode_partials_kernel<D, NT><<<unsigned((workers + kWarpsA - 1) / kWarpsA), kWarpsA * 32, smem, st>>>(p);
   int64_t blocks = int64_t(p.n_seqs) * p.heads_q;
   if (p.mass) blocks += int64_t(p.n_seqs) * ((p.max_pages + kJoinThreads - 1) / kJoinThreads);
   decode_join_kernel<D><<<unsigned(blocks), kJoinThreads, p.mass ? size_t(p.heads_q) * 4 : 0, st>>>(p);
@@ -451,5 +1069,7 @@ extern "C" ashkv_status_t ashkv_decode_attention(
   p.part_o = d_scratch;
   p.part_lse2 = p.part_o + rows * kv->head_dim;
   p.page_lse2 = p.part_lse2 + rows;
-  return kv->head_dim == 64 ? launch_decode<64>(p, as_stream(stream)) : launch_decode<128>(p, as_stream(stream));
+  cudaStream_t st = as_stream(stream);
+  if (worker_queries(p.group) == 8) return kv->head_dim == 64 ? launch_decode<64, 1>(p, st) : launch_decode<128, 1>(p, st);
+  return kv->head_dim == 64 ? launch_decode<64, 2>(p, st) : launch_decode<128, 2>(p, st);
 }

@@ -40,12 +40,12 @@ def page_values(fmt: int, data: np.ndarray, T: int, heads: int, dim: int, outlie
 def decode_attention(q, lists, lengths, T, scale, page_mass=None, decay=1.0):
     """q float64 [n, heads_q, dim]; ``lists[b][hk]`` = [(position, (K, V)), ...] of key head hk.
 
-    Returns dicts of arrays: out, lse, mass, and for tolerances ``reach`` = sum_t P |v| per result
-    element and ``size`` = max_t scale * sum |q||k| per query head (0 where nothing is attended)."""
+    Returns arrays: out, lse, mass, and for tolerances ``reach`` = sum_t P |v| per result element,
+    ``size`` = max_t scale * sum |q||k| and ``largest`` = max |v| per query head (0 without tokens)."""
     n, hq, d = q.shape
     hkv = len(lists[0])
     out, reach = np.zeros_like(q), np.zeros_like(q)
-    lse, size = np.full((n, hq), -np.inf), np.zeros((n, hq))
+    lse, size, largest = np.full((n, hq), -np.inf), np.zeros((n, hq)), np.zeros((n, hq))
     mass = None if page_mass is None else page_mass.astype(np.float64).copy()
     for b in range(n):
         if mass is not None:
@@ -66,12 +66,13 @@ def decode_attention(q, lists, lengths, T, scale, page_mass=None, decay=1.0):
             p = p / p.sum() if p.sum() != 0 else p
             out[b, h], reach[b, h] = p @ V, p @ np.abs(V)
             size[b, h] = (abs(scale) * (np.abs(K) @ np.abs(q[b, h]))).max()
+            largest[b, h] = np.abs(V).max()
             if mass is not None:
                 at = 0
                 for pos, k, _ in entries:
                     mass[b, pos] += p[at:at + len(k)].sum()
                     at += len(k)
-    return {"out": out, "lse": lse, "mass": mass, "reach": reach, "size": size}
+    return {"out": out, "lse": lse, "mass": mass, "reach": reach, "size": size, "largest": largest}
 
 
 def exponent(amax: float) -> int:
