@@ -59,6 +59,8 @@ struct AttnParams {
   float* part_o;      // [ranges + n_seqs][heads_q][D], each divided by its sum
   float* part_lse2;   // [ranges + n_seqs][heads_q]
   float* page_lse2;   // [n_seqs][max_pages][heads_q], with mass only
+  int32_t warp_smem;  // bytes of shared memory of a worker
+  int32_t fp8_pages, int_pages;  // whether a store holds FP8, or INT8 or INT4 pages
   uint32_t* status;
 };
 
@@ -142,6 +144,12 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same with int8 operands and k = 32: A and B registers hold k = 4t .. 4t + 3, the upper ones 16 more.
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Transpose of an 8 x 8 matrix of 16-bit values spread over the warp (row g, columns 2t, 2t + 1).
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -237,6 +245,49 @@ struct Unit {
   uint32_t scale;  // lane l: scale bits of K row l (l < 16) or V row l - 16
 };
 
+  // Decodes the K or V rows of a dithered page into a BF16 unit.
+  // (Out of line: a call costs little beside the decode, and the loop of the other formats stays short.)
+template <int D, int BITS>
+__device__ __noinline__ void stage_nbit(const uint8_t* slot, int T, int row_len, int cap, int hk, bool v, int t0, int rows,
+                                        uint32_t dst) {
+    const int lane = threadIdx.x & 31;
+    const int64_t E = 2 * int64_t(T) * row_len;
+    const uint16_t* delta = reinterpret_cast<const uint16_t*>(slot + nbit_delta_off());
+    const uint8_t* codes = slot + nbit_codes_off(E);
+    constexpr float half = float((1 << BITS) - 1) * 0.5f;
+    constexpr int GPR = D / 32, RB = D * 2;
+    const int row0 = (v ? T : 0) + t0;
+#pragma unroll
+    for (int j = 0; j < GPR / 2; ++j) {
+      const int n = lane + 32 * j, r = n / GPR, k = n % GPR;
+      uint32_t o[16];
+      if (r < rows) {
+        GroupCodes<BITS> gc;
+        load_group<BITS>(delta, codes, (int64_t(row0 + r) * row_len + hk * D) / 32 + k, gc);
+        group_bf16<BITS>(gc, half, o);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) o[c] = 0;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        sts128(dst + (v ? v_off<RB>(r, 4 * k + c) : k_off<RB>(r, 4 * k + c)),
+               make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]));
+    }
+    __syncwarp();  // dense values first, then the outliers overwrite theirs
+    const uint32_t n_out = min(*reinterpret_cast<const uint32_t*>(slot), uint32_t(cap));
+    const uint32_t* ent = reinterpret_cast<const uint32_t*>(slot + nbit_entries_off(E, BITS));
+    for (uint32_t j = lane; j < n_out; j += 32) {
+      const uint32_t e = ent[j];
+      const uint32_t r = (e >> 16) / uint32_t(row_len) - uint32_t(row0);
+      const uint32_t c = (e >> 16) % uint32_t(row_len) - uint32_t(hk * D);
+      if (r < uint32_t(rows) && c < uint32_t(D)) {
+        const uint32_t at = dst + (v ? v_off<RB>(r, c >> 3) : k_off<RB>(r, c >> 3)) + (c & 7u) * 2u;
+        asm volatile("st.shared.u16 [%0], %1;" :: "r"(at), "h"(static_cast<uint16_t>(e)) : "memory");
+      }
+    }
+  }
+
 template <int D>
 struct Feeder {
   static constexpr int kUnitBytes = 16 * D * 2;
@@ -285,55 +336,24 @@ struct Feeder {
   template <int RB, bool V>
   __device__ __forceinline__ void copy_rows(const uint8_t* src, int64_t stride, int rows, uint32_t dst) const {
     const int lane = threadIdx.x & 31;
-    constexpr int CPR = RB / 16;
+    constexpr int CPR = RB / 16, RPI = 32 / CPR;  // chunks of a row, rows of one instruction
+    const int r0 = lane / CPR, col = lane % CPR;
+    if (rows == 16) {
+      src += r0 * stride + col * 16;
 #pragma unroll
-    for (int j = 0; j < CPR / 2; ++j) {
-      const int c = lane + 32 * j, r = c / CPR, col = c % CPR;
+      for (int j = 0; j < 16 / RPI; ++j) {
+        cp_async16(dst + (V ? v_off<RB>(r0 + RPI * j, col) : k_off<RB>(r0 + RPI * j, col)), src);
+        src += RPI * stride;
+      }
+      return;
+    }
+#pragma unroll 1
+    for (int j = 0; j < 16 / RPI; ++j) {
+      const int r = r0 + RPI * j;
       const bool real = r < rows;
       cp_async16_or_zero(dst + (V ? v_off<RB>(r, col) : k_off<RB>(r, col)), src + (real ? r * stride + col * 16 : 0), real);
     }
   }
-  // Decodes the K or V rows of a dithered page into a BF16 unit.
-  template <int BITS>
-  __device__ void stage_nbit(bool v, int t0, int rows, uint32_t dst) const {
-    const int lane = threadIdx.x & 31;
-    const int64_t E = 2 * int64_t(p.T) * p.row_len;
-    const uint16_t* delta = reinterpret_cast<const uint16_t*>(page.k + nbit_delta_off());
-    const uint8_t* codes = page.k + nbit_codes_off(E);
-    constexpr float half = float((1 << BITS) - 1) * 0.5f;
-    constexpr int GPR = D / 32, RB = D * 2;
-    const int row0 = (v ? p.T : 0) + t0;
-#pragma unroll
-    for (int j = 0; j < GPR / 2; ++j) {
-      const int n = lane + 32 * j, r = n / GPR, k = n % GPR;
-      uint32_t o[16];
-      if (r < rows) {
-        GroupCodes<BITS> gc;
-        load_group<BITS>(delta, codes, (int64_t(row0 + r) * p.row_len + hk * D) / 32 + k, gc);
-        group_bf16<BITS>(gc, half, o);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 16; ++c) o[c] = 0;
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        sts128(dst + (v ? v_off<RB>(r, 4 * k + c) : k_off<RB>(r, 4 * k + c)),
-               make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]));
-    }
-    __syncwarp();  // dense values first, then the outliers overwrite theirs
-    const uint32_t n_out = min(*reinterpret_cast<const uint32_t*>(page.k), uint32_t(p.outlier_cap));
-    const uint32_t* ent = reinterpret_cast<const uint32_t*>(page.k + nbit_entries_off(E, BITS));
-    for (uint32_t j = lane; j < n_out; j += 32) {
-      const uint32_t e = ent[j];
-      const uint32_t r = (e >> 16) / uint32_t(p.row_len) - uint32_t(row0);
-      const uint32_t c = (e >> 16) % uint32_t(p.row_len) - uint32_t(hk * D);
-      if (r < uint32_t(rows) && c < uint32_t(D)) {
-        const uint32_t at = dst + (v ? v_off<RB>(r, c >> 3) : k_off<RB>(r, c >> 3)) + (c & 7u) * 2u;
-        asm volatile("st.shared.u16 [%0], %1;" :: "r"(at), "h"(static_cast<uint16_t>(e)) : "memory");
-      }
-    }
-  }
-
   // Sends the next unit on its way (always one cp.async group) and describes it.
   __device__ Unit issue() {
     Unit u{page.format, 0, page.pos, second, true, 0u};
@@ -351,8 +371,8 @@ struct Feeder {
         second = !second;
       } else if (page.format >= ASHKV_PAGE_NBIT4) {
         u.format = ASHKV_PAGE_BF16;
-        if (page.format == ASHKV_PAGE_NBIT4) stage_nbit<4>(second, t0, u.rows, dst);
-        else stage_nbit<2>(second, t0, u.rows, dst);
+        if (page.format == ASHKV_PAGE_NBIT4) stage_nbit<D, 4>(page.k, p.T, p.row_len, p.outlier_cap, hk, second, t0, u.rows, dst);
+        else stage_nbit<D, 2>(page.k, p.T, p.row_len, p.outlier_cap, hk, second, t0, u.rows, dst);
         done = second;
         second = !second;
       } else {
@@ -412,52 +432,87 @@ struct Worker {
   float acc[NT][MT][4];
   float m[NT][2], thr[NT][2], l[NT][2], ps[NT][2];  // ps: the page's own sum
   float c;
-  float qs_b, qs_h[NT][2];  // factors from a raw dot product to a log2 score: bf16 and fp16 queries
-  uint32_t qb, qh;          // the queries in shared memory as bf16 and as fp16 (scaled by a power of two)
+  float qs_h[NT][2], qs_i[NT][2];  // factors from a dot product with the fp16 / whole-number queries to a log2 score
+  // The queries in shared memory, [8 NT][D] each: bf16; fp16, scaled by a power of two (FP8
+  // stores only); three int8 digits of whole numbers (INT8 and INT4 stores only).
+  uint32_t qb, qh, qi;
   int lane, g, t;
   bool fresh;               // no scale was seen yet
 
   __device__ __forceinline__ Worker(const AttnParams& p_, uint32_t q_smem)
-      : p(p_), qb(q_smem), qh(q_smem + NT * 8 * D * 2), lane(threadIdx.x & 31), g(lane >> 2), t(lane & 3) {}
+      : p(p_), qb(q_smem), qh(q_smem + NT * 8 * D * 2), qi(qh + (p_.fp8_pages ? NT * 8 * D * 2 : 0)),
+        lane(threadIdx.x & 31), g(lane >> 2), t(lane & 3) {}
 
   // 16-byte chunk k of query row n: rows 2n and 2n + 1 in different halves of the banks, as they are read together.
   static __device__ __forceinline__ uint32_t qb_off(uint32_t n, uint32_t k) { return n * (D * 2) + ((k ^ ((n & 1u) << 2)) << 4); }
   static __device__ __forceinline__ uint32_t qh_off(uint32_t n, uint32_t k) { return n * (D * 2) + ((k ^ (n & 1u)) << 4); }
+  static __device__ __forceinline__ uint32_t qi_off(uint32_t n, uint32_t k) { return n * D + ((k ^ ((n & 1u) << 2)) & (D / 16 - 1)) * 16; }
 
   __device__ void start(int b, int hq0, int nq) {
     constexpr int N = D / 32;  // channels of a lane here
-    qs_b = p.scale2;
 #pragma unroll
     for (int half = 0; half < NT; ++half)
 #pragma unroll 2
     for (int n = 8 * half; n < 8 * half + 8; ++n) {
       uint16_t x[N];
       float amax = 0.0f;
+      bool whole = true;
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         x[k] = n < nq ? p.q[b * p.q_seq_stride + int64_t(hq0 + n) * p.q_head_stride + lane * N + k] : uint16_t(0);
         const float a = fabsf(bf16_to_f32(x[k]));
         if (a < INFINITY) amax = fmaxf(amax, a);
+        else whole = false;
       }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, off));
-      // the largest query value to [2^14, 2^15): fp16 then keeps all 8 bits of every value
-      // down to 2^-31 of it, exactly
-      const int e = min(112, max(-112, int(__float_as_uint(amax) >> 23) - 127 - 14));
-      const float down = __uint_as_float(uint32_t(127 - e) << 23), up = __uint_as_float(uint32_t(127 + e) << 23);
-      if ((n & 7) == 2 * t) qs_h[half][0] = p.scale2 * up;
-      if ((n & 7) == 2 * t + 1) qs_h[half][1] = p.scale2 * up;
+      amax = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(amax)));
+      whole = __all_sync(0xFFFFFFFFu, whole);
       const uint32_t kb = uint32_t(lane * N) >> 3, in = (uint32_t(lane * N) & 7u) * 2u;
-      if constexpr (N == 4) {
+      if constexpr (N == 4)
         asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(qb + qb_off(n, kb) + in),
                      "r"(uint32_t(x[0]) | (uint32_t(x[1]) << 16)), "r"(uint32_t(x[2]) | (uint32_t(x[3]) << 16)) : "memory");
-        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(qh + qh_off(n, kb) + in),
-                     "r"(f32x2_to_f16x2(bf16_to_f32(x[0]) * down, bf16_to_f32(x[1]) * down)),
-                     "r"(f32x2_to_f16x2(bf16_to_f32(x[2]) * down, bf16_to_f32(x[3]) * down)) : "memory");
-      } else {
+      else
         asm volatile("st.shared.u32 [%0], %1;" :: "r"(qb + qb_off(n, kb) + in), "r"(uint32_t(x[0]) | (uint32_t(x[1]) << 16)) : "memory");
-        asm volatile("st.shared.u32 [%0], %1;" :: "r"(qh + qh_off(n, kb) + in),
-                     "r"(f32x2_to_f16x2(bf16_to_f32(x[0]) * down, bf16_to_f32(x[1]) * down)) : "memory");
+      // the exponent of the largest value, kept where 2^+-(e + 23) are normal numbers
+      const int e = min(100, max(-100, int(__float_as_uint(amax) >> 23) - 127));
+      const float unit = __uint_as_float(uint32_t(127 + e) << 23), inv = __uint_as_float(uint32_t(127 - e) << 23);
+      const bool mine0 = (n & 7) == 2 * t, mine1 = (n & 7) == 2 * t + 1;
+      if (p.fp8_pages) {
+        // the largest value to [2^14, 2^15): fp16 then keeps all 8 bits of every value down to
+        // 2^-31 of it, exactly
+        const float up = p.scale2 * unit * 0x1p-14f, down = inv * 0x1p14f;
+        if (mine0) qs_h[half][0] = up;
+        if (mine1) qs_h[half][1] = up;
+#pragma unroll
+        for (int k = 0; k < N; k += 2)
+          asm volatile("st.shared.u32 [%0], %1;" :: "r"(qh + qh_off(n, kb) + in + 2 * k),
+                       "r"(f32x2_to_f16x2(bf16_to_f32(x[k]) * down, bf16_to_f32(x[k + 1]) * down)) : "memory");
+      }
+      if (p.int_pages) {
+        // whole numbers of 23 bits with sign, as digits of base 256 in [-128, 127]: exact down to
+        // 2^-15 of the largest value, off by at most 2^-24 of it below
+        const float up = whole ? p.scale2 * unit * 0x1p-22f : NAN;
+        if (mine0) qs_i[half][0] = up;
+        if (mine1) qs_i[half][1] = up;
+        uint32_t d0 = 0, d1 = 0, d2 = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int v = __float2int_rn(bf16_to_f32(x[k]) * (inv * 0x1p22f));
+          const int v1 = (v + 128) >> 8, v2 = (v1 + 128) >> 8;
+          d0 |= uint32_t(v & 255) << (8 * k);
+          d1 |= uint32_t(v1 & 255) << (8 * k);
+          d2 |= uint32_t(v2 & 255) << (8 * k);
+        }
+        const uint32_t at = qi + qi_off(n, uint32_t(lane * N) >> 4) + (uint32_t(lane * N) & 15u);
+        constexpr uint32_t kDigit = NT * 8 * D;
+        if constexpr (N == 4) {
+          asm volatile("st.shared.u32 [%0], %1;" :: "r"(at), "r"(d2) : "memory");
+          asm volatile("st.shared.u32 [%0], %1;" :: "r"(at + kDigit), "r"(d1) : "memory");
+          asm volatile("st.shared.u32 [%0], %1;" :: "r"(at + 2 * kDigit), "r"(d0) : "memory");
+        } else {
+          asm volatile("st.shared.u16 [%0], %1;" :: "r"(at), "h"(uint16_t(d2)) : "memory");
+          asm volatile("st.shared.u16 [%0], %1;" :: "r"(at + kDigit), "h"(uint16_t(d1)) : "memory");
+          asm volatile("st.shared.u16 [%0], %1;" :: "r"(at + 2 * kDigit), "h"(uint16_t(d0)) : "memory");
+        }
       }
     }
 #pragma unroll
@@ -578,7 +633,7 @@ struct Worker {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) s[n][x] *= qs_b;
+      for (int x = 0; x < 4; ++x) s[n][x] *= p.scale2;
     weights(s, rows);
   }
   // Adds a tile of BF16 values: the weights in two bf16 parts (8 + 8 bits), as a single one would
@@ -615,6 +670,28 @@ struct Worker {
     }
   }
 
+  // Products of int8 keys with the three digits of the queries: 64 channels i, thread t's 16 in
+  // ka (token g) and kb (token g + 8).  Whole numbers below 2^21 each, exact.
+  static __device__ __forceinline__ void zero_digits(int (&d)[3][NT][4]) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) d[k][n][0] = d[k][n][1] = d[k][n][2] = d[k][n][3] = 0;
+  }
+  __device__ __forceinline__ void add_digits(int (&d)[3][NT][4], const uint4& ka, const uint4& kb, int i) const {
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint4 q = lds128(qi + k * (NT * 8 * D) + qi_off(8 * n + g, 4 * i + t));
+        mma16832(d[k][n], ka.x, kb.x, ka.y, kb.y, q.x, q.y);
+        mma16832(d[k][n], ka.z, kb.z, ka.w, kb.w, q.z, q.w);
+      }
+  }
+  static __device__ __forceinline__ float digits_value(const int (&d)[3][NT][4], int n, int x) {
+    return fmaf(float(d[0][n][x] * 256 + d[1][n][x]), 256.0f, float(d[2][n][x]));
+  }
+
   // A tile of a page of 8-bit codes, K then V.
   template <bool INT8>
   __device__ __forceinline__ void tile8(uint32_t tile, const Unit& u) {
@@ -631,37 +708,44 @@ struct Worker {
       fit_scale(1.0f);
     }
     float s[NT][4];
+    if constexpr (INT8) {
+      int d[3][NT][4];
+      zero_digits(d);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+      for (int i = 0; i < D / 64; ++i) {
+        const uint4 ka = lds128(tile + k_off<D>(g, 4 * i + t)), kb = lds128(tile + k_off<D>(g + 8, 4 * i + t));
+        add_digits(d, ka, kb, i);
+      }
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      const uint4 xa = lds128(tile + k_off<D>(g, 4 * i + t)), xb = lds128(tile + k_off<D>(g + 8, 4 * i + t));
-      const uint32_t ka[4] = {xa.x, xa.y, xa.z, xa.w}, kb[4] = {xb.x, xb.y, xb.z, xb.w};
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4 q[NT];
+        for (int x = 0; x < 4; ++x) s[n][x] = digits_value(d, n, x) * (qs_i[n][x & 1] * (x < 2 ? ks0 : ks1));
+    } else {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) q[n] = lds128(qh + qh_off(8 * n + g, 2 * (4 * i + t) + h));
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          uint32_t a0, a1, a2, a3;
-          if constexpr (INT8) {
-            const uint32_t fa = ka[2 * h + w] ^ 0x80808080u, fb = kb[2 * h + w] ^ 0x80808080u;
-            a0 = int8_pair(fa, 0x4140); a1 = int8_pair(fb, 0x4140);
-            a2 = int8_pair(fa, 0x4342); a3 = int8_pair(fb, 0x4342);
-          } else {
-            a0 = fp8_pair(ka[2 * h + w]); a1 = fp8_pair(kb[2 * h + w]);
-            a2 = fp8_pair(ka[2 * h + w] >> 16); a3 = fp8_pair(kb[2 * h + w] >> 16);
+      for (int i = 0; i < D / 64; ++i) {
+        const uint4 xa = lds128(tile + k_off<D>(g, 4 * i + t)), xb = lds128(tile + k_off<D>(g + 8, 4 * i + t));
+        const uint32_t ka[4] = {xa.x, xa.y, xa.z, xa.w}, kb[4] = {xb.x, xb.y, xb.z, xb.w};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint4 q[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) q[n] = lds128(qh + qh_off(8 * n + g, 2 * (4 * i + t) + h));
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t a0 = fp8_pair(ka[2 * h + w]), a1 = fp8_pair(kb[2 * h + w]);
+            const uint32_t a2 = fp8_pair(ka[2 * h + w] >> 16), a3 = fp8_pair(kb[2 * h + w] >> 16);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816<false>(s[n], a0, a1, a2, a3, w ? q[n].z : q[n].x, w ? q[n].w : q[n].y);
           }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816<false>(s[n], a0, a1, a2, a3, w ? q[n].z : q[n].x, w ? q[n].w : q[n].y);
         }
       }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[n][x] *= qs_h[n][x & 1];
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) s[n][x] *= qs_h[n][x & 1] * (x < 2 ? ks0 : ks1);
     weights(s, u.rows);
     uint32_t b[1][NT][2];
     fp16_weights<1>(s, vs, b);
@@ -695,6 +779,15 @@ struct Worker {
     }
   }
 
+  // Sixteen nibbles (8 bytes: byte j = channel 2j in the high nibble, 2j + 1) as int8 16 * (nibble -
+  // 8) in channel order: a nibble in the upper half of a byte with its top bit flipped.
+  static __device__ __forceinline__ uint4 nibbles_x16(uint2 w) {
+    const uint32_t e0 = (w.x & 0xF0F0F0F0u) ^ 0x80808080u, o0 = ((w.x << 4) & 0xF0F0F0F0u) ^ 0x80808080u;
+    const uint32_t e1 = (w.y & 0xF0F0F0F0u) ^ 0x80808080u, o1 = ((w.y << 4) & 0xF0F0F0F0u) ^ 0x80808080u;
+    return make_uint4(__byte_perm(e0, o0, 0x5140), __byte_perm(e0, o0, 0x7362), __byte_perm(e1, o1, 0x5140),
+                      __byte_perm(e1, o1, 0x7362));
+  }
+
   // A tile of an INT4 page (scales per 64 channels), K then V.
   __device__ __forceinline__ void tile4(uint32_t tile, const Unit& u) {
     constexpr int K = D / 64;
@@ -710,30 +803,18 @@ struct Worker {
       x_max = fmaxf(x_max, x);
       const uint2 xa = lds64(tile + k_off<D / 2>(g, 2 * k + (t >> 1)) + (t & 1) * 8);
       const uint2 xb = lds64(tile + k_off<D / 2>(g + 8, 2 * k + (t >> 1)) + (t & 1) * 8);
-      float d[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.0f;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {  // eight channels: byte j = (channel 2j, channel 2j + 1), the first in the high nibble
-        const uint32_t ka = w ? xa.y : xa.x, kb = w ? xb.y : xb.x, ka8 = ka >> 8, kb8 = kb >> 8;
-        const uint32_t a04 = nibble_hi(ka), b04 = nibble_hi(kb), a15 = nibble_lo(ka), b15 = nibble_lo(kb);
-        const uint32_t a26 = nibble_hi(ka8), b26 = nibble_hi(kb8), a37 = nibble_lo(ka8), b37 = nibble_lo(kb8);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint4 q = lds128(qh + qh_off(8 * n + g, 2 * (4 * k + t) + w));
-          mma16816<false>(d[n], a04, b04, a15, b15, __byte_perm(q.x, q.z, 0x5410), __byte_perm(q.x, q.z, 0x7632));
-          mma16816<false>(d[n], a26, b26, a37, b37, __byte_perm(q.y, q.w, 0x5410), __byte_perm(q.y, q.w, 0x7632));
-        }
-      }
+      int d[3][NT][4];
+      zero_digits(d);
+      add_digits(d, nibbles_x16(xa), nibbles_x16(xb), k);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) s[n][y] = fmaf(d[n][y], y < 2 ? ks0 : ks1, s[n][y]);
+        for (int y = 0; y < 4; ++y) s[n][y] = fmaf(digits_value(d, n, y), y < 2 ? ks0 : ks1, s[n][y]);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int y = 0; y < 4; ++y) s[n][y] *= qs_h[n][y & 1];
+      for (int y = 0; y < 4; ++y) s[n][y] *= qs_i[n][y & 1] * 0.0625f;
     fit_scale(lane < 16 ? 0.0f : x_max);
     weights(s, u.rows);
     uint32_t b[K][NT][2];
@@ -806,8 +887,6 @@ struct Worker {
   }
 };
 
-template <int D, int NT>
-constexpr int warp_smem() { return kRing * Feeder<D>::kUnitBytes + 2 * NT * 8 * D * 2; }
 
 template <int D, int NT>
 __global__ void __launch_bounds__(kWarpsA * 32, NT == 1 ? 3 : 2) decode_partials_kernel(const __grid_constant__ AttnParams p) {
@@ -829,7 +908,7 @@ __global__ void __launch_bounds__(kWarpsA * 32, NT == 1 ? 3 : 2) decode_partials
     if (before + n > pos) break;
     before += n;
   }
-  const uint32_t ring = smem_u32(smem) + uint32_t(warp * warp_smem<D, NT>());
+  const uint32_t ring = smem_u32(smem) + uint32_t(warp * p.warp_smem);
   Feeder<D> feed(p, hk, ring);
   Worker<D, NT> work(p, ring + kRing * Feeder<D>::kUnitBytes);
   for (; pos < end; ++b) {
@@ -838,16 +917,22 @@ __global__ void __launch_bounds__(kWarpsA * 32, NT == 1 ? 3 : 2) decode_partials
     const int i0 = int(pos - before), i1 = int(min(int64_t(n), end - before));
     feed.slot = 0;
     feed.start(b, i0, i1);
-    Unit next[kRing];
-#pragma unroll
-    for (int k = 0; k < kRing; ++k) next[k] = feed.issue();
     work.start(b, hq0, nq);
+    Unit next[kRing];
     float s[NT][4];  // weights of a BF16 tile between its K and its V unit
     int slot = 0;
-    while (next[0].format != ASHKV_PAGE_NONE) {
+    for (int ahead = 0;;) {
+#pragma unroll
+      for (int k = 0; k + 1 < kRing; ++k) next[k] = next[k + 1];
+      next[kRing - 1] = feed.issue();
+      if (ahead < kRing - 1) {
+        ++ahead;
+        continue;
+      }
+      const Unit u = next[0];
+      if (u.format == ASHKV_PAGE_NONE) break;
       cp_async_wait<kRing - 1>();
       __syncwarp();
-      const Unit u = next[0];
       const uint32_t tile = ring + slot * Feeder<D>::kUnitBytes;
       if (u.format == ASHKV_PAGE_BF16) {
         if (u.is_v) work.bf16_values(tile, s);
@@ -859,12 +944,9 @@ __global__ void __launch_bounds__(kWarpsA * 32, NT == 1 ? 3 : 2) decode_partials
       } else {
         work.tile4(tile, u);
       }
-      __syncwarp();  // every lane has read the unit
-#pragma unroll
-      for (int k = 0; k + 1 < kRing; ++k) next[k] = next[k + 1];
-      next[kRing - 1] = feed.issue();
-      slot = slot == kRing - 1 ? 0 : slot + 1;
       if (p.mass && u.last) work.page_sum(b, u.pos, hq0, nq);
+      slot = slot == kRing - 1 ? 0 : slot + 1;
+      __syncwarp();  // every lane has read the unit
     }
     cp_async_wait<0>();
     __syncwarp();
@@ -1006,9 +1088,10 @@ ashkv_status_t refuse(const char* what, const char* why) {
 }
 
 template <int D, int NT>
-ashkv_status_t launch_decode(const AttnParams& p, cudaStream_t st) {
+ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
   const int64_t workers = int64_t(p.ranges) * p.heads_kv * p.q_chunks;
-  constexpr int smem = kWarpsA * warp_smem<D, NT>();
+  p.warp_smem = kRing * Feeder<D>::kUnitBytes + NT * 8 * D * (2 + (p.fp8_pages ? 2 : 0) + (p.int_pages ? 3 : 0));
+  const int smem = kWarpsA * p.warp_smem;
   const cudaError_t e = cudaFuncSetAttribute(decode_partials_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     set_error("ashkv_decode_attention (shared memory attribute)", e);
@@ -1069,6 +1152,10 @@ extern "C" ashkv_status_t ashkv_decode_attention(
   p.part_o = d_scratch;
   p.part_lse2 = p.part_o + rows * kv->head_dim;
   p.page_lse2 = p.part_lse2 + rows;
+  for (int t = 1; t < kTiers; ++t) {
+    p.fp8_pages |= p.store[t].format == ASHKV_PAGE_FP8;
+    p.int_pages |= p.store[t].format == ASHKV_PAGE_INT8 || p.store[t].format == ASHKV_PAGE_INT4;
+  }
   cudaStream_t st = as_stream(stream);
   if (worker_queries(p.group) == 8) return kv->head_dim == 64 ? launch_decode<64, 1>(p, st) : launch_decode<128, 1>(p, st);
   return kv->head_dim == 64 ? launch_decode<64, 2>(p, st) : launch_decode<128, 2>(p, st);
