@@ -91,18 +91,19 @@ __device__ int lists_before(const AttnParams& p, int b, int hk) {
 // Pages per range; every range but the last of the row has as many.
 __device__ __forceinline__ int range_len(const AttnParams& p, int total) { return max(1, (total + p.ranges - 1) / p.ranges); }
 
-// The page behind list entry i of (sequence b, key head hk).
+// The page behind list entry i of (sequence b, key head hk), as the copies need it.
 struct PageRef {
-  const uint8_t* k;   // BF16: the K row of the page's first token; else the slot
-  const uint8_t* v;   // BF16: the V row
-  int32_t format;     // ASHKV_PAGE_*, ASHKV_PAGE_NONE for a page to leave out
+  const uint8_t* k;   // BF16: K channel 0 of the head at the page's first token; codes: the same; dithered: the slot
+  const uint8_t* v;   // BF16: the same of V; codes: the slot
+  uint32_t meta;      // format | tokens in use << 8; no tokens: a page to leave out
   int32_t pos;        // position in the sequence
 };
-__device__ PageRef resolve(const AttnParams& p, int b, int hk, int i) {
-  PageRef r{nullptr, nullptr, ASHKV_PAGE_NONE, i};
+template <int D>
+__device__ PageRef resolve(const AttnParams& p, int b, int hk, int i, int64_t tokens) {
+  PageRef r{nullptr, nullptr, 0, i};
   if (p.selected) {
     r.pos = p.selected[(int64_t(b) * p.heads_kv + hk) * p.max_selected + i];
-    if (r.pos < 0 || int64_t(r.pos) * p.T >= seq_tokens(p, b)) {
+    if (r.pos < 0 || int64_t(r.pos) * p.T >= tokens) {
       flag(p.status, ASHKV_FLAG_INDEX_RANGE);
       r.pos = 0;
       return r;
@@ -116,16 +117,23 @@ __device__ PageRef resolve(const AttnParams& p, int b, int hk, int i) {
     const int32_t l = p.layer_id[id], ts = p.token_start[id];
     ok = l >= 0 && l < p.n_layers && ts >= 0 && int64_t(ts) + p.T <= p.pool_tokens;
     if (ok) {
-      const int64_t off = int64_t(ts) * p.row_stride * 2;
+      const int64_t off = (int64_t(ts) * p.row_stride + hk * D) * 2;
       r.k = reinterpret_cast<const uint8_t*>(p.layer_k[l]) + off;
       r.v = reinterpret_cast<const uint8_t*>(p.layer_v[l]) + off;
+      r.meta = ASHKV_PAGE_BF16;
     }
   } else if (ok) {
     const int32_t s = p.page_slot[id];
     ok = s >= 0 && s < p.store[t].n_slots;
-    if (ok) r.k = p.store[t].data + int64_t(s) * p.store[t].slot_bytes;
+    if (ok) {
+      r.v = r.k = p.store[t].data + int64_t(s) * p.store[t].slot_bytes;
+      r.meta = uint32_t(p.store[t].format);
+      if (r.meta == ASHKV_PAGE_INT8) r.k += int8_codes_offset(p.T) + hk * D;
+      if (r.meta == ASHKV_PAGE_FP8) r.k += hk * D;
+      if (r.meta == ASHKV_PAGE_INT4) r.k += p.T * p.row_len / 16 + hk * (D / 2);  // past E / 32 bytes of scales
+    }
   }
-  if (ok) r.format = t == 0 ? ASHKV_PAGE_BF16 : p.store[t].format;
+  if (ok) r.meta |= uint32_t(min(int64_t(p.T), tokens - int64_t(r.pos) * p.T)) << 8;
   else flag(p.status, ASHKV_FLAG_INDEX_RANGE);
   return r;
 }
@@ -238,14 +246,15 @@ constexpr int kRing = 3;  // units in shared memory per warp: one in use, two on
 // A unit is 16 tokens of a page for one key head: the K or the V rows of a BF16
 // page (16 x D bf16), or the codes of both of a compressed page (K first).
 struct Unit {
-  int32_t format;  // BF16, INT8, FP8, INT4; NONE past the end
-  int32_t rows;    // tokens in use
+  uint32_t meta;   // format | kIsV (BF16: the V rows) | kLast (the page's last unit) | tokens in use << 16; 0: none
   int32_t pos;     // page position in the sequence
-  bool is_v, last; // BF16: the V rows; the page's last unit
   uint32_t scale;  // lane l: scale bits of K row l (l < 16) or V row l - 16
+  static constexpr uint32_t kIsV = 0x100u, kLast = 0x200u;
+  __device__ __forceinline__ uint32_t format() const { return meta & 0xFFu; }
+  __device__ __forceinline__ int rows() const { return int(meta >> 16); }
 };
 
-  // Decodes the K or V rows of a dithered page into a BF16 unit.
+// Decodes the K or V rows of a dithered page into a BF16 unit.
   // (Out of line: a call costs little beside the decode, and the loop of the other formats stays short.)
 template <int D, int BITS>
 __device__ __noinline__ void stage_nbit(const uint8_t* slot, int T, int row_len, int cap, int hk, bool v, int t0, int rows,
@@ -294,116 +303,118 @@ struct Feeder {
   const AttnParams& p;
   int b, hk, i, i1;       // next list entry, end of the segment
   int64_t tokens;
-  uint32_t ring;          // shared address of the warp's ring
-  int slot, tile;
-  bool second;            // BF16: the V unit of (page, tile) is next
+  uint32_t ring, dst;     // shared addresses of the warp's ring and of the next unit
+  int t0;                 // first token of the next unit in its page
+  bool second;            // BF16: the V unit of (page, t0) is next
   PageRef batch;          // lane l: list entry batch0 + l
   int batch0;
-  PageRef page;           // current page
-  int page_rows;          // its tokens in use
+  PageRef page;           // current page; no tokens in use: none
 
-  __device__ __forceinline__ Feeder(const AttnParams& p_, int hk_, uint32_t ring_) : p(p_), hk(hk_), ring(ring_), slot(0) {}
+  __device__ __forceinline__ Feeder(const AttnParams& p_, int hk_, uint32_t ring_) : p(p_), hk(hk_), ring(ring_) {}
   __device__ __forceinline__ void start(int b_, int i0, int i1_) {
-    b = b_; i = i0; i1 = i1_; tokens = seq_tokens(p, b); batch0 = i0 - 32; tile = 0; second = false;
+    b = b_; i = i0; i1 = i1_; tokens = seq_tokens(p, b); batch0 = i0 - 32; t0 = 0; second = false; dst = ring;
     next_page();
   }
   // Makes list entry i, or the next one with tokens, the current page.
-  __device__ void next_page() {
-    const int lane = threadIdx.x & 31;
+  __device__ __forceinline__ void next_page() {
     for (; i < i1; ++i) {
-      if (i >= batch0 + 32) {
-        batch0 = i;
-        if (i + lane < i1) batch = resolve(p, b, hk, i + lane);
-      }
+      if (i >= batch0 + 32) next_batch();
       const int src = i - batch0;
-      page.k = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(batch.k), src));
-      page.v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(batch.v), src));
-      page.format = __shfl_sync(0xFFFFFFFFu, batch.format, src);
+      page.meta = __shfl_sync(0xFFFFFFFFu, batch.meta, src);
       page.pos = __shfl_sync(0xFFFFFFFFu, batch.pos, src);
-      if (page.format == ASHKV_PAGE_NONE) {
-        if (p.mass)
-          for (int g = lane; g < p.group; g += 32)
-            p.page_lse2[(int64_t(b) * p.max_pages + page.pos) * p.heads_q + hk * p.group + g] = -INFINITY;
-        continue;
+      if (page.meta >> 8) {
+        page.k = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(batch.k), src));
+        page.v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(batch.v), src));
+        return;
       }
-      page_rows = int(min(int64_t(p.T), tokens - int64_t(page.pos) * p.T));
-      return;
     }
-    page.format = ASHKV_PAGE_NONE;
+    page.meta = 0;
+  }
+  __device__ __forceinline__ void next_batch() {
+    const int lane = threadIdx.x & 31;
+    batch0 = i;
+    if (i + lane < i1) {
+      batch = resolve<D>(p, b, hk, i + lane, tokens);
+      if (p.mass && !(batch.meta >> 8))  // a page that is left out draws nothing
+        for (int g = 0; g < p.group; ++g)
+          p.page_lse2[(int64_t(b) * p.max_pages + batch.pos) * p.heads_q + hk * p.group + g] = -INFINITY;
+    }
   }
 
-  // Rows of RB bytes: row r of the tile at src + r * stride.
+  // 16 rows of RB bytes, `step` bytes apart from src on, into a tile; rows behind `rows` become zeros.
   template <int RB, bool V>
-  __device__ __forceinline__ void copy_rows(const uint8_t* src, int64_t stride, int rows, uint32_t dst) const {
-    const int lane = threadIdx.x & 31;
-    constexpr int CPR = RB / 16, RPI = 32 / CPR;  // chunks of a row, rows of one instruction
-    const int r0 = lane / CPR, col = lane % CPR;
+  __device__ __forceinline__ void copy_rows(const uint8_t* src, uint32_t step, int rows, uint32_t tile) const {
+    const uint32_t lane = threadIdx.x & 31u;
+    constexpr uint32_t CPR = RB / 16, RPI = 32 / CPR;  // chunks of a row, rows of one instruction
+    const uint32_t r0 = lane / CPR, col = lane % CPR;
+    src += r0 * step + col * 16u;
     if (rows == 16) {
-      src += r0 * stride + col * 16;
 #pragma unroll
-      for (int j = 0; j < 16 / RPI; ++j) {
-        cp_async16(dst + (V ? v_off<RB>(r0 + RPI * j, col) : k_off<RB>(r0 + RPI * j, col)), src);
-        src += RPI * stride;
-      }
+      for (uint32_t j = 0; j < 16 / RPI; ++j)
+        cp_async16(tile + (V ? v_off<RB>(r0 + RPI * j, col) : k_off<RB>(r0 + RPI * j, col)), src + uint64_t(step) * (RPI * j));
       return;
     }
 #pragma unroll 1
-    for (int j = 0; j < 16 / RPI; ++j) {
-      const int r = r0 + RPI * j;
-      const bool real = r < rows;
-      cp_async16_or_zero(dst + (V ? v_off<RB>(r, col) : k_off<RB>(r, col)), src + (real ? r * stride + col * 16 : 0), real);
+    for (uint32_t j = 0; j < 16 / RPI; ++j) {
+      const uint32_t r = r0 + RPI * j;
+      const bool real = r < uint32_t(rows);
+      cp_async16_or_zero(tile + (V ? v_off<RB>(r, col) : k_off<RB>(r, col)), real ? src + uint64_t(step) * (RPI * j) : page.k, real);
     }
   }
+
   // Sends the next unit on its way (always one cp.async group) and describes it.
-  __device__ Unit issue() {
-    Unit u{page.format, 0, page.pos, second, true, 0u};
-    if (page.format != ASHKV_PAGE_NONE) {
-      const int lane = threadIdx.x & 31;
-      const int t0 = tile * 16;
-      u.rows = min(16, page_rows - t0);
-      const uint32_t dst = ring + slot * kUnitBytes;
-      bool done = true;  // with this tile
-      if (page.format == ASHKV_PAGE_BF16) {
-        const uint8_t* src = (second ? page.v : page.k) + (int64_t(t0) * p.row_stride + hk * D) * 2;
-        if (second) copy_rows<D * 2, true>(src, p.row_stride * 2, u.rows, dst);
-        else copy_rows<D * 2, false>(src, p.row_stride * 2, u.rows, dst);
+  __device__ __forceinline__ Unit issue() {
+    Unit u{0u, page.pos, 0u};
+    if (page.meta) {
+      const uint32_t lane = threadIdx.x & 31u;
+      const uint32_t format = page.meta & 0xFFu;
+      const int left = int(page.meta >> 8) - t0, rows = min(16, left);
+      u.meta = format | uint32_t(rows) << 16;
+      const uint32_t row = uint32_t(p.row_len);
+      bool done = true;  // with these tokens
+      if (format == ASHKV_PAGE_BF16) {
+        const uint32_t step = uint32_t(p.row_stride) * 2u;
+        if (second) {
+          u.meta |= Unit::kIsV;
+          copy_rows<D * 2, true>(page.v + uint32_t(t0) * step, step, rows, dst);
+        } else {
+          copy_rows<D * 2, false>(page.k + uint32_t(t0) * step, step, rows, dst);
+        }
         done = second;
         second = !second;
-      } else if (page.format >= ASHKV_PAGE_NBIT4) {
-        u.format = ASHKV_PAGE_BF16;
-        if (page.format == ASHKV_PAGE_NBIT4) stage_nbit<D, 4>(page.k, p.T, p.row_len, p.outlier_cap, hk, second, t0, u.rows, dst);
-        else stage_nbit<D, 2>(page.k, p.T, p.row_len, p.outlier_cap, hk, second, t0, u.rows, dst);
+      } else if (format >= ASHKV_PAGE_NBIT4) {
+        u.meta = ASHKV_PAGE_BF16 | uint32_t(rows) << 16 | (second ? Unit::kIsV : 0u);
+        if (format == ASHKV_PAGE_NBIT4) stage_nbit<D, 4>(page.k, p.T, p.row_len, p.outlier_cap, hk, second, t0, rows, dst);
+        else stage_nbit<D, 2>(page.k, p.T, p.row_len, p.outlier_cap, hk, second, t0, rows, dst);
         done = second;
         second = !second;
       } else {
-        const int64_t row = p.row_len, kr = t0, vr = p.T + t0;
-        const bool mine = (lane & 15) < u.rows;
-        const int64_t srow = (lane < 16 ? kr : vr) + (lane & 15);
-        if (page.format == ASHKV_PAGE_INT4) {
-          const uint8_t* codes = page.k + p.T * row / 16 + hk * (D / 2);  // past E/32 bytes of scales
-          copy_rows<D / 2, false>(codes + kr * (row / 2), row / 2, u.rows, dst);
-          copy_rows<D / 2, true>(codes + vr * (row / 2), row / 2, u.rows, dst + 8 * D);
-          const uint8_t* sc = page.k + (srow * row + hk * D) / 32;
-          if (mine) u.scale = D == 128 ? *reinterpret_cast<const uint32_t*>(sc) : uint32_t(*reinterpret_cast<const uint16_t*>(sc));
+        const uint32_t sr = uint32_t(t0) + (lane & 15u) + (lane & 16u ? uint32_t(p.T) : 0u);  // this lane's scale row
+        const bool mine = int(lane & 15u) < rows;
+        if (format == ASHKV_PAGE_INT4) {
+          const uint32_t step = row / 2;
+          const uint8_t* codes = page.k + uint32_t(t0) * step;
+          copy_rows<D / 2, false>(codes, step, rows, dst);
+          copy_rows<D / 2, true>(codes + uint32_t(p.T) * step, step, rows, dst + 8 * D);
+          const uint8_t* sc = page.v + (sr * row + hk * D) / 32u;
+          if (mine) u.scale = D == 128 ? __ldg(reinterpret_cast<const uint32_t*>(sc)) : uint32_t(__ldg(reinterpret_cast<const uint16_t*>(sc)));
         } else {
-          const bool i8 = page.format == ASHKV_PAGE_INT8;
-          const uint8_t* codes = page.k + (i8 ? int8_codes_offset(p.T) : 0) + hk * D;
-          copy_rows<D, false>(codes + kr * row, row, u.rows, dst);
-          copy_rows<D, true>(codes + vr * row, row, u.rows, dst + 16 * D);
-          if (i8 && mine) u.scale = reinterpret_cast<const uint16_t*>(page.k)[srow];
+          const uint8_t* codes = page.k + uint32_t(t0) * row;
+          copy_rows<D, false>(codes, row, rows, dst);
+          copy_rows<D, true>(codes + uint32_t(p.T) * row, row, rows, dst + 16 * D);
+          if (format == ASHKV_PAGE_INT8 && mine) u.scale = __ldg(reinterpret_cast<const uint16_t*>(page.v) + sr);
         }
       }
-      u.last = done && t0 + 16 >= page_rows;
       if (done) {
-        if (u.last) {
-          tile = 0;
+        t0 += 16;
+        if (left <= 16) {
+          u.meta |= Unit::kLast;
+          t0 = 0;
           ++i;
           next_page();
-        } else {
-          ++tile;
         }
       }
-      slot = slot == kRing - 1 ? 0 : slot + 1;
+      dst = dst == ring + (kRing - 1) * kUnitBytes ? ring : dst + kUnitBytes;
     }
     cp_async_commit();
     return u;
@@ -746,7 +757,7 @@ struct Worker {
 #pragma unroll
         for (int x = 0; x < 4; ++x) s[n][x] *= qs_h[n][x & 1];
     }
-    weights(s, u.rows);
+    weights(s, u.rows());
     uint32_t b[1][NT][2];
     fp16_weights<1>(s, vs, b);
     tile += 16 * D;
@@ -816,7 +827,7 @@ struct Worker {
 #pragma unroll
       for (int y = 0; y < 4; ++y) s[n][y] *= qs_i[n][y & 1] * 0.0625f;
     fit_scale(lane < 16 ? 0.0f : x_max);
-    weights(s, u.rows);
+    weights(s, u.rows());
     uint32_t b[K][NT][2];
     fp16_weights<K>(s, vs, b);
     tile += 8 * D;
@@ -915,37 +926,32 @@ __global__ void __launch_bounds__(kWarpsA * 32, NT == 1 ? 3 : 2) decode_partials
     const int n = list_len(p, b, hk);
     if (n == 0) continue;
     const int i0 = int(pos - before), i1 = int(min(int64_t(n), end - before));
-    feed.slot = 0;
     feed.start(b, i0, i1);
     work.start(b, hq0, nq);
-    Unit next[kRing];
+    Unit next[kRing] = {};
     float s[NT][4];  // weights of a BF16 tile between its K and its V unit
-    int slot = 0;
-    for (int ahead = 0;;) {
+    uint32_t tile = ring;
+    for (int ahead = 0;; ++ahead) {
 #pragma unroll
       for (int k = 0; k + 1 < kRing; ++k) next[k] = next[k + 1];
       next[kRing - 1] = feed.issue();
-      if (ahead < kRing - 1) {
-        ++ahead;
-        continue;
-      }
+      if (ahead < kRing - 1) continue;
       const Unit u = next[0];
-      if (u.format == ASHKV_PAGE_NONE) break;
+      if (!u.meta) break;
       cp_async_wait<kRing - 1>();
       __syncwarp();
-      const uint32_t tile = ring + slot * Feeder<D>::kUnitBytes;
-      if (u.format == ASHKV_PAGE_BF16) {
-        if (u.is_v) work.bf16_values(tile, s);
-        else work.bf16_scores(tile, u.rows, s);
-      } else if (u.format == ASHKV_PAGE_INT8) {
+      if (u.format() == ASHKV_PAGE_BF16) {
+        if (u.meta & Unit::kIsV) work.bf16_values(tile, s);
+        else work.bf16_scores(tile, u.rows(), s);
+      } else if (u.format() == ASHKV_PAGE_INT8) {
         work.template tile8<true>(tile, u);
-      } else if (u.format == ASHKV_PAGE_FP8) {
+      } else if (u.format() == ASHKV_PAGE_FP8) {
         work.template tile8<false>(tile, u);
       } else {
         work.tile4(tile, u);
       }
-      if (p.mass && u.last) work.page_sum(b, u.pos, hq0, nq);
-      slot = slot == kRing - 1 ? 0 : slot + 1;
+      if (p.mass && (u.meta & Unit::kLast)) work.page_sum(b, u.pos, hq0, nq);
+      tile = tile == ring + (kRing - 1) * Feeder<D>::kUnitBytes ? ring : tile + Feeder<D>::kUnitBytes;
       __syncwarp();  // every lane has read the unit
     }
     cp_async_wait<0>();
@@ -1058,6 +1064,8 @@ const char* copy_pages(const ashkv_paged_kv_t* kv, AttnParams& p) {
       kv->outlier_cap < 0 || kv->tokens_per_page > 65536 || kv->heads_kv > 65536)
     return "heads_kv, tokens_per_page and n_layers must be positive, sizes not negative";
   const int64_t row = int64_t(kv->heads_kv) * kv->head_dim;
+  if (row > 0x7FFFFFFF || kv->row_stride > 0x3FFFFFFF || kv->tokens_per_page * kv->row_stride > 0x3FFFFFFF)
+    return "a page must span less than 2^31 bytes";
   if (kv->row_stride < row || kv->row_stride % 8) return "row_stride must be a multiple of 8 and at least heads_kv * head_dim";
   if (!kv->d_tier || !kv->d_layer_id || !kv->d_token_start || !kv->d_page_slot || !kv->d_layer_k || !kv->d_layer_v)
     return "null device pointer";
