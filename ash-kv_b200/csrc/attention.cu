@@ -139,31 +139,38 @@ __device__ PageRef resolve(const AttnParams& p, int b, int hk, int i, int64_t to
 }
 
 // ---------------------------------------------------------------- tensor-core pieces
-// D (16 x 8, fp32) += A (16 x 16, row) * B (16 x 8, col).  Lane (g, t) = (lane / 4,
-// lane % 4) holds A rows g and g + 8, k = 2t, 2t + 1, 2t + 8, 2t + 9 (a0 .. a3: row
-// g, row g + 8, then the same for the upper k), B column g at the same k (b0, b1),
-// and D rows g, g + 8 at columns 2t, 2t + 1.
+// D (16 x 8, fp32) = A (16 x 16, row) * B (16 x 8, col) + (first ? 0 : D).  Lane (g,
+// t) = (lane / 4, lane % 4) holds A rows g and g + 8, k = 2t, 2t + 1, 2t + 8, 2t +
+// 9 (a.x .. a.w: row g, row g + 8, then the same for the upper k), B column g at
+// the same k (b0, b1), and D rows g, g + 8 at columns 2t, 2t + 1.
+#define ASHKV_MMA(KIND, C, ...) \
+  asm volatile("mma.sync.aligned." KIND " {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, " C ";" __VA_ARGS__)
 template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  if constexpr (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1, bool first = false) {
+  if (first) {
+    if constexpr (BF16)
+      ASHKV_MMA("m16n8k16.row.col.f32.bf16.bf16.f32", "{%10,%10,%10,%10}", : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+      ASHKV_MMA("m16n8k16.row.col.f32.f16.f16.f32", "{%10,%10,%10,%10}", : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
+  } else {
+    if constexpr (BF16)
+      ASHKV_MMA("m16n8k16.row.col.f32.bf16.bf16.f32", "{%0,%1,%2,%3}", : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+    else
+      ASHKV_MMA("m16n8k16.row.col.f32.f16.f16.f32", "{%0,%1,%2,%3}", : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+  }
 }
 // The same with int8 operands and k = 32: A and B registers hold k = 4t .. 4t + 3, the upper ones 16 more.
-__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// Transpose of an 8 x 8 matrix of 16-bit values spread over the warp (row g, columns 2t, 2t + 1).
-__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-  return r;
+__device__ __forceinline__ void mma16832(int (&d)[4], const uint4& a, uint32_t b0, uint32_t b1, bool first) {
+  if (first)
+    ASHKV_MMA("m16n8k32.row.col.s32.s8.s8.s32", "{%10,%10,%10,%10}", : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+              : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(0));
+  else
+    ASHKV_MMA("m16n8k32.row.col.s32.s8.s8.s32", "{%0,%1,%2,%3}", : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+              : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -201,6 +208,9 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 // 16 bytes global -> shared; zeros instead when `real` is false (nothing is read then).
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -244,11 +254,13 @@ __device__ __forceinline__ uint32_t v_off(uint32_t r, uint32_t c) {
 constexpr int kRing = 3;  // units in shared memory per warp: one in use, two on their way
 
 // A unit is 16 tokens of a page for one key head: the K or the V rows of a BF16
-// page (16 x D bf16), or the codes of both of a compressed page (K first).
+// page (16 x D bf16), or the codes of both of a compressed page (K first), and
+// behind them the scales of those rows: INT8: fp16, K then V, the V rows from the
+// last 4-byte boundary on; INT4: a word per row, K then V (D = 64: the row's scale
+// for this head is the word's upper half for an odd head).
 struct Unit {
   uint32_t meta;   // format | kIsV (BF16: the V rows) | kLast (the page's last unit) | tokens in use << 16; 0: none
   int32_t pos;     // page position in the sequence
-  uint32_t scale;  // lane l: scale bits of K row l (l < 16) or V row l - 16
   static constexpr uint32_t kIsV = 0x100u, kLast = 0x200u;
   __device__ __forceinline__ uint32_t format() const { return meta & 0xFFu; }
   __device__ __forceinline__ int rows() const { return int(meta >> 16); }
@@ -299,7 +311,8 @@ __device__ __noinline__ void stage_nbit(const uint8_t* slot, int T, int row_len,
 
 template <int D>
 struct Feeder {
-  static constexpr int kUnitBytes = 16 * D * 2;
+  static constexpr int kScales = 16 * D * 2;           // byte offset of the scales
+  static constexpr int kUnitBytes = kScales + 128;
   const AttnParams& p;
   int b, hk, i, i1;       // next list entry, end of the segment
   int64_t tokens;
@@ -364,7 +377,7 @@ struct Feeder {
 
   // Sends the next unit on its way (always one cp.async group) and describes it.
   __device__ __forceinline__ Unit issue() {
-    Unit u{0u, page.pos, 0u};
+    Unit u{0u, page.pos};
     if (page.meta) {
       const uint32_t lane = threadIdx.x & 31u;
       const uint32_t format = page.meta & 0xFFu;
@@ -389,20 +402,22 @@ struct Feeder {
         done = second;
         second = !second;
       } else {
-        const uint32_t sr = uint32_t(t0) + (lane & 15u) + (lane & 16u ? uint32_t(p.T) : 0u);  // this lane's scale row
-        const bool mine = int(lane & 15u) < rows;
         if (format == ASHKV_PAGE_INT4) {
           const uint32_t step = row / 2;
           const uint8_t* codes = page.k + uint32_t(t0) * step;
           copy_rows<D / 2, false>(codes, step, rows, dst);
           copy_rows<D / 2, true>(codes + uint32_t(p.T) * step, step, rows, dst + 8 * D);
-          const uint8_t* sc = page.v + (sr * row + hk * D) / 32u;
-          if (mine) u.scale = D == 128 ? __ldg(reinterpret_cast<const uint32_t*>(sc)) : uint32_t(__ldg(reinterpret_cast<const uint16_t*>(sc)));
+          const uint32_t sr = min(uint32_t(t0) + (lane & 15u), uint32_t(p.T) - 1u) + (lane & 16u ? uint32_t(p.T) : 0u);
+          cp_async4(dst + kScales + lane * 4u, page.v + ((sr * row + hk * D) / 32u & ~3u));
         } else {
           const uint8_t* codes = page.k + uint32_t(t0) * row;
           copy_rows<D, false>(codes, row, rows, dst);
           copy_rows<D, true>(codes + uint32_t(p.T) * row, row, rows, dst + 16 * D);
-          if (format == ASHKV_PAGE_INT8 && mine) u.scale = __ldg(reinterpret_cast<const uint16_t*>(page.v) + sr);
+          if (format == ASHKV_PAGE_INT8 && lane < 17u) {
+            // 8 words of K scales, 9 of V scales (all inside the slot: codes follow them)
+            const uint32_t at = lane < 8u ? uint32_t(t0) * 2u + lane * 4u : (uint32_t(p.T + t0) * 2u & ~3u) + (lane - 8u) * 4u;
+            cp_async4(dst + kScales + lane * 4u, page.v + at);
+          }
         }
       }
       if (done) {
@@ -423,41 +438,67 @@ struct Feeder {
 
 // ---------------------------------------------------------------- the worker
 // A warp per (range of pages, key head, up to 8 * NT of its query heads).
-//   S (tokens x queries) = K Q^T, then O^T (channels x queries) += V^T P^T: the
-//   tokens and channels fill the 16 rows of the tensor-core tile and the few
-//   queries its 8 columns, so no row is spent on padding.  P leaves the first
-//   product with tokens as rows and enters the second with tokens as k: an 8 x
-//   8 transpose per half tile.
-// Per query (this lane: 2t and 2t + 1) m is the reference of the weights 2^(s -
-// m).  It follows the running maximum only when a score lies more than 2^8 above
-// it, which is rare after the first tiles, so most tiles reduce nothing across
-// the lanes.  acc holds sum_t 2^(s - m) * c * v.  The scale of a compressed V row
-// rides on its weight and its codes enter the product as whole numbers; the power
-// of two c keeps weight * scale inside the fp16 range: c * (largest scale so far)
-// lies in [2^6, 2^7], a weight below 2^8, so the operand stays below 2^15 and is
-// off by at most 2^-25 / c where fp16 runs out of digits, 2^-31 of a largest value.
+//   S (queries x tokens) = Q K^T, then O^T (channels x queries) += V^T P^T.  K rows
+// enter the first product as its B operand and the weights leave it laid out as
+// the B operand of the second, so nothing is exchanged between lanes; the 16
+// rows of A are the channels in the second product.  In the first they hold up
+// to 16 queries (NT = 2); for 8 (NT = 1) the upper 8 rows do not idle but hold
+// the same queries' next 16 channels (or their next digit, see below), and each
+// half of D is read from the product whose B operand matches it.
+//   Lane (g, t) owns the scores of query g (and g + 8) and tokens 2t, 2t + 1, 2t +
+// 8, 2t + 9 of a tile.  m is the reference of the weights 2^(s - m).  It follows
+// the running maximum only when a score lies more than 2^8 above it, which is
+// rare after the first tiles, so most tiles reduce nothing across the lanes.
+// acc holds sum_t 2^(s - m) * c * v.  The scale of a compressed V row rides on its
+// weight and its codes enter the product as whole numbers; the power of two c
+// keeps weight * scale inside the fp16 range: c * (largest scale so far) lies in
+// [2^6, 2^7], a weight below 2^8, so the operand stays below 2^15 and is off by at
+// most 2^-25 / c where fp16 runs out of digits, 2^-31 of a largest value.
 template <int D, int NT>
 struct Worker {
   static constexpr int MT = D / 16;  // channel tiles of 16
   const AttnParams& p;
-  float acc[NT][MT][4];
-  float m[NT][2], thr[NT][2], l[NT][2], ps[NT][2];  // ps: the page's own sum
+  float acc[NT][MT][4];              // [queries 8 n ..][channel tile]: rows g, g + 8, columns (queries) 2t, 2t + 1
+  float m[NT], thr[NT], l[NT], ps[NT];  // of query 8 n + g; ps: the page's own sum
   float c;
-  float qs_h[NT][2], qs_i[NT][2];  // factors from a dot product with the fp16 / whole-number queries to a log2 score
-  // The queries in shared memory, [8 NT][D] each: bf16; fp16, scaled by a power of two (FP8
-  // stores only); three int8 digits of whole numbers (INT8 and INT4 stores only).
+  float qs_h[NT], qs_i[NT];  // factors from a dot product with the fp16 / whole-number queries to a log2 score
+  // The queries in shared memory as A operands: bf16; fp16, scaled by a power of two (FP8 stores
+  // only); three int8 digits of whole numbers (INT8 and INT4 stores only).
   uint32_t qb, qh, qi;
   int lane, g, t;
   bool fresh;               // no scale was seen yet
+  bool odd_head;
 
-  __device__ __forceinline__ Worker(const AttnParams& p_, uint32_t q_smem)
+  __device__ __forceinline__ Worker(const AttnParams& p_, uint32_t q_smem, int hk)
       : p(p_), qb(q_smem), qh(q_smem + NT * 8 * D * 2), qi(qh + (p_.fp8_pages ? NT * 8 * D * 2 : 0)),
-        lane(threadIdx.x & 31), g(lane >> 2), t(lane & 3) {}
+        lane(threadIdx.x & 31), g(lane >> 2), t(lane & 3), odd_head(hk & 1) {}
 
-  // 16-byte chunk k of query row n: rows 2n and 2n + 1 in different halves of the banks, as they are read together.
-  static __device__ __forceinline__ uint32_t qb_off(uint32_t n, uint32_t k) { return n * (D * 2) + ((k ^ ((n & 1u) << 2)) << 4); }
-  static __device__ __forceinline__ uint32_t qh_off(uint32_t n, uint32_t k) { return n * (D * 2) + ((k ^ (n & 1u)) << 4); }
-  static __device__ __forceinline__ uint32_t qi_off(uint32_t n, uint32_t k) { return n * D + ((k ^ ((n & 1u) << 2)) & (D / 16 - 1)) * 16; }
+  // 16-bit queries.  Channels 8 k .. 8 k + 7 (words w = 0 .. 3 of two) serve two products of 16
+  // channels, words 0, 1 the first.  NT = 1: one operand (0, 2, 1, 3), the second product's words in
+  // rows 8-15; NT = 2: two operands (row g, row g + 8).  Neighbouring rows go to other banks.
+  static __device__ __forceinline__ uint32_t q_chunk(uint32_t row, uint32_t chunk, bool wide) {
+    return row * (NT * D * 2) + ((chunk ^ (NT == 1 && !wide ? (row & 1u) << 2 : row & 1u)) << 4);
+  }
+  static __device__ __forceinline__ uint32_t q_word(uint32_t n, uint32_t k, uint32_t w, bool wide) {
+    if constexpr (NT == 1) return q_chunk(n, k, wide) + (((w & 1u) << 1) | (w >> 1)) * 4u;
+    return q_chunk(n & 7u, 2u * k + (w >> 1), true) + ((w & 1u) * 2u + (n >> 3)) * 4u;
+  }
+  // Digits.  Channels 16 k .. 16 k + 15 (words of four) serve two products of 32 channels.  NT = 1: the
+  // two higher digits as the two halves of the rows, two operands; the lowest like 16-bit words above.
+  // NT = 2: two operands for each digit.
+  static constexpr uint32_t kLowDigit = 8 * D * 2;
+  static __device__ __forceinline__ uint32_t digit_chunk(uint32_t row, uint32_t chunk) { return row * (D * 2) + ((chunk ^ (row & 1u)) << 4); }
+  static __device__ __forceinline__ uint32_t low_chunk(uint32_t row, uint32_t chunk) {
+    return kLowDigit + row * D + (((chunk ^ ((row & 1u) << 2)) & (D / 16 - 1)) << 4);
+  }
+  static __device__ __forceinline__ uint32_t digit_word(uint32_t digit, uint32_t n, uint32_t k, uint32_t w) {  // digit 0: the highest
+    if constexpr (NT == 1) {
+      if (digit == 2) return low_chunk(n, k) + (((w & 1u) << 1) | (w >> 1)) * 4u;
+      return digit_chunk(n, 2u * k + (w >> 1)) + ((w & 1u) * 2u + digit) * 4u;
+    }
+    return digit * (16 * D) + digit_chunk(n & 7u, 2u * k + (w >> 1)) + ((w & 1u) * 2u + (n >> 3)) * 4u;
+  }
+  static __device__ __forceinline__ void sts32(uint32_t a, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" :: "r"(a), "r"(v) : "memory"); }
 
   __device__ void start(int b, int hq0, int nq) {
     constexpr int N = D / 32;  // channels of a lane here
@@ -477,61 +518,47 @@ struct Worker {
       }
       amax = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(amax)));
       whole = __all_sync(0xFFFFFFFFu, whole);
-      const uint32_t kb = uint32_t(lane * N) >> 3, in = (uint32_t(lane * N) & 7u) * 2u;
-      if constexpr (N == 4)
-        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(qb + qb_off(n, kb) + in),
-                     "r"(uint32_t(x[0]) | (uint32_t(x[1]) << 16)), "r"(uint32_t(x[2]) | (uint32_t(x[3]) << 16)) : "memory");
-      else
-        asm volatile("st.shared.u32 [%0], %1;" :: "r"(qb + qb_off(n, kb) + in), "r"(uint32_t(x[0]) | (uint32_t(x[1]) << 16)) : "memory");
+      const uint32_t k8 = uint32_t(lane * N) >> 3, w8 = (uint32_t(lane * N) & 7u) >> 1;
+#pragma unroll
+      for (int k = 0; k < N; k += 2) sts32(qb + q_word(n, k8, w8 + k / 2, false), uint32_t(x[k]) | (uint32_t(x[k + 1]) << 16));
       // the exponent of the largest value, kept where 2^+-(e + 23) are normal numbers
       const int e = min(100, max(-100, int(__float_as_uint(amax) >> 23) - 127));
       const float unit = __uint_as_float(uint32_t(127 + e) << 23), inv = __uint_as_float(uint32_t(127 - e) << 23);
-      const bool mine0 = (n & 7) == 2 * t, mine1 = (n & 7) == 2 * t + 1;
+      const bool mine = (n & 7) == g;
       if (p.fp8_pages) {
         // the largest value to [2^14, 2^15): fp16 then keeps all 8 bits of every value down to
         // 2^-31 of it, exactly
-        const float up = p.scale2 * unit * 0x1p-14f, down = inv * 0x1p14f;
-        if (mine0) qs_h[half][0] = up;
-        if (mine1) qs_h[half][1] = up;
+        if (mine) qs_h[half] = p.scale2 * unit * 0x1p-14f;
+        const float down = inv * 0x1p14f;
 #pragma unroll
         for (int k = 0; k < N; k += 2)
-          asm volatile("st.shared.u32 [%0], %1;" :: "r"(qh + qh_off(n, kb) + in + 2 * k),
-                       "r"(f32x2_to_f16x2(bf16_to_f32(x[k]) * down, bf16_to_f32(x[k + 1]) * down)) : "memory");
+          sts32(qh + q_word(n, k8, w8 + k / 2, true), f32x2_to_f16x2(bf16_to_f32(x[k]) * down, bf16_to_f32(x[k + 1]) * down));
       }
       if (p.int_pages) {
         // whole numbers of 23 bits with sign, as digits of base 256 in [-128, 127]: exact down to
         // 2^-15 of the largest value, off by at most 2^-24 of it below
-        const float up = whole ? p.scale2 * unit * 0x1p-22f : NAN;
-        if (mine0) qs_i[half][0] = up;
-        if (mine1) qs_i[half][1] = up;
-        uint32_t d0 = 0, d1 = 0, d2 = 0;
+        if (mine) qs_i[half] = whole ? p.scale2 * unit * 0x1p-22f : NAN;
+        uint32_t d[3] = {0, 0, 0};
 #pragma unroll
         for (int k = 0; k < N; ++k) {
           const int v = __float2int_rn(bf16_to_f32(x[k]) * (inv * 0x1p22f));
           const int v1 = (v + 128) >> 8, v2 = (v1 + 128) >> 8;
-          d0 |= uint32_t(v & 255) << (8 * k);
-          d1 |= uint32_t(v1 & 255) << (8 * k);
-          d2 |= uint32_t(v2 & 255) << (8 * k);
+          d[0] |= uint32_t(v2 & 255) << (8 * k);
+          d[1] |= uint32_t(v1 & 255) << (8 * k);
+          d[2] |= uint32_t(v & 255) << (8 * k);
         }
-        const uint32_t at = qi + qi_off(n, uint32_t(lane * N) >> 4) + (uint32_t(lane * N) & 15u);
-        constexpr uint32_t kDigit = NT * 8 * D;
-        if constexpr (N == 4) {
-          asm volatile("st.shared.u32 [%0], %1;" :: "r"(at), "r"(d2) : "memory");
-          asm volatile("st.shared.u32 [%0], %1;" :: "r"(at + kDigit), "r"(d1) : "memory");
-          asm volatile("st.shared.u32 [%0], %1;" :: "r"(at + 2 * kDigit), "r"(d0) : "memory");
-        } else {
-          asm volatile("st.shared.u16 [%0], %1;" :: "r"(at), "h"(uint16_t(d2)) : "memory");
-          asm volatile("st.shared.u16 [%0], %1;" :: "r"(at + kDigit), "h"(uint16_t(d1)) : "memory");
-          asm volatile("st.shared.u16 [%0], %1;" :: "r"(at + 2 * kDigit), "h"(uint16_t(d0)) : "memory");
+        const uint32_t k16 = uint32_t(lane * N) >> 4, w16 = (uint32_t(lane * N) & 15u) >> 2;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          const uint32_t at = qi + digit_word(k, n, k16, w16);
+          if constexpr (N == 4) sts32(at, d[k]);
+          else asm volatile("st.shared.u16 [%0], %1;" :: "r"(at + (lane & 1) * 2), "h"(uint16_t(d[k])) : "memory");
         }
       }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        m[n][j] = 0.0f; thr[n][j] = -INFINITY; l[n][j] = 0.0f; ps[n][j] = 0.0f;
-      }
+      m[n] = 0.0f; thr[n] = -INFINITY; l[n] = 0.0f; ps[n] = 0.0f;
 #pragma unroll
       for (int k = 0; k < MT; ++k)
 #pragma unroll
@@ -548,58 +575,59 @@ struct Worker {
       acc[n][k][0] *= f0; acc[n][k][1] *= f1; acc[n][k][2] *= f0; acc[n][k][3] *= f1;
     }
   }
-  static __device__ __forceinline__ float max_over_tokens(float x) {  // over the lanes of the same queries
-    x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
-    x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
-    return fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
+  // Query 8 n + 2t + j's value of x, which is spread over the owners (8 n + g) of the queries.
+  __device__ __forceinline__ float of_column(float x, int j) const { return __shfl_sync(0xFFFFFFFFu, x, 8 * t + 4 * j); }
+  static __device__ __forceinline__ float max_over_tokens(float x) {
+    x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 1));
+    return fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
+  }
+  static __device__ __forceinline__ float sum_over_tokens(float x) {
+    x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
+    return x + __shfl_xor_sync(0xFFFFFFFFu, x, 2);
   }
 
-  // log2 scores (token g: s[0], s[1]; token g + 8: s[2], s[3]) -> weights 2^(s - m), added up.
+  // log2 scores of tokens 2t, 2t + 1, 2t + 8, 2t + 9 -> weights 2^(s - m), added up.
   __device__ __forceinline__ void weights(float (&s)[NT][4], int rows) {
     if (rows < 16) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (g >= rows) s[n][0] = s[n][1] = -INFINITY;
-        if (g + 8 >= rows) s[n][2] = s[n][3] = -INFINITY;
-      }
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (2 * t + (x & 1) + 8 * (x >> 1) >= rows) s[n][x] = -INFINITY;
     }
     bool over = false;
+    float top[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      over |= fmaxf(s[n][0], s[n][2]) > thr[n][0] || fmaxf(s[n][1], s[n][3]) > thr[n][1];
+    for (int n = 0; n < NT; ++n) {
+      top[n] = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3]));
+      over |= top[n] > thr[n];
+    }
     if (__any_sync(0xFFFFFFFFu, over)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float f[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float top = max_over_tokens(fmaxf(s[n][j], s[n][j + 2]));
-          f[j] = 1.0f;
-          if (top > thr[n][j]) {
-            if (thr[n][j] != -INFINITY) f[j] = ex2(m[n][j] - top);
-            m[n][j] = top;
-            thr[n][j] = top + 8.0f;
-            l[n][j] *= f[j];
-            ps[n][j] *= f[j];
-          }
+        const float x = max_over_tokens(top[n]);
+        float f = 1.0f;
+        if (x > thr[n]) {
+          if (thr[n] != -INFINITY) f = ex2(m[n] - x);
+          m[n] = x;
+          thr[n] = x + 8.0f;
+          l[n] *= f;
+          ps[n] *= f;
         }
-        scale_acc(n, f[0], f[1]);
+        scale_acc(n, of_column(f, 0), of_column(f, 1));
       }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) s[n][x] = ex2(s[n][x] - m[n][x & 1]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float sum = s[n][j] + s[n][j + 2];
-        l[n][j] += sum;
-        ps[n][j] += sum;
-      }
+      for (int x = 0; x < 4; ++x) s[n][x] = ex2(s[n][x] - m[n]);
+      const float sum = (s[n][0] + s[n][1]) + (s[n][2] + s[n][3]);
+      l[n] += sum;
+      ps[n] += sum;
     }
   }
 
-  // Makes room for V rows of scale x (this lane's, 0 where it holds none; K of them).
+  // Makes room for V rows of scale x (this lane's, 0 where it holds none).
   __device__ __forceinline__ void fit_scale(float x) {
     if (!__any_sync(0xFFFFFFFFu, fresh || x * c > 128.0f)) return;
     const float top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, x > 0.0f ? __float_as_uint(x) : 0u));
@@ -612,35 +640,54 @@ struct Worker {
       fresh = false;
     }
   }
-  // Weights times c and a row scale, as the fp16 operand of the product with V: b[k][n][0] tokens
-  // 0-7, b[k][n][1] tokens 8-15.  w[k] = scale of row g, of row g + 8 for scale group k.
-  template <int K>
-  __device__ __forceinline__ void fp16_weights(const float (&s)[NT][4], const float (&w)[K][2], uint32_t (&b)[K][NT][2]) {
+  // Weights times c and the scales w of the rows of this lane's tokens, as the fp16 operand of the
+  // product with V.
+  __device__ __forceinline__ void fp16_weights(const float (&s)[NT][4], const float (&w)[4], uint32_t (&b)[NT][2]) {
+    float wc[4];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const float w0 = w[k][0] * c, w1 = w[k][1] * c;
+    for (int x = 0; x < 4; ++x) wc[x] = w[x] * c;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        b[k][n][0] = transpose8(f32x2_to_f16x2(s[n][0] * w0, s[n][1] * w0));
-        b[k][n][1] = transpose8(f32x2_to_f16x2(s[n][2] * w1, s[n][3] * w1));
-      }
+    for (int n = 0; n < NT; ++n) {
+      b[n][0] = f32x2_to_f16x2(s[n][0] * wc[0], s[n][1] * wc[1]);
+      b[n][1] = f32x2_to_f16x2(s[n][2] * wc[2], s[n][3] * wc[3]);
     }
   }
 
-  // Scores of a tile of BF16 keys.
-  __device__ __forceinline__ void bf16_scores(uint32_t tile, int rows, float (&s)[NT][4]) {
+  // Dot products with the 16-bit queries at q (8-channel chunk k) of 16 channels each, keys (b0, b1)
+  // and (b2, b3) of one token half: d takes the first or, with NT = 2, both; e the second with NT = 1.
+  template <bool BF16>
+  static __device__ __forceinline__ void dot16(float (&d)[4], float (&e)[4], const uint4 (&q)[NT], uint32_t b0, uint32_t b1,
+                                               uint32_t b2, uint32_t b3, bool first) {
+    mma16816<BF16>(d, q[0], b0, b1, first);
+    if constexpr (NT == 1) mma16816<BF16>(e, q[0], b2, b3, first);
+    else mma16816<BF16>(d, q[1], b2, b3);
+  }
+  static __device__ __forceinline__ void gather16(float (&s)[NT][4], const float (&d)[2][4], const float (&e)[2][4]) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+    for (int x = 0; x < 4; ++x) {
+      if constexpr (NT == 1) s[0][x] = d[x >> 1][x & 1] + e[x >> 1][2 + (x & 1)];
+      else { s[0][x] = d[x >> 1][x & 1]; s[1][x] = d[x >> 1][2 + (x & 1)]; }
+    }
+  }
+  __device__ __forceinline__ void load_q16(uint4 (&q)[NT], uint32_t base, uint32_t k, bool wide) const {
+    if constexpr (NT == 1) q[0] = lds128(base + q_chunk(g, k, wide));
+    else { q[0] = lds128(base + q_chunk(g, 2 * k, true)); q[1] = lds128(base + q_chunk(g, 2 * k + 1, true)); }
+  }
+
+  // Weights of a tile of BF16 keys.
+  __device__ __forceinline__ void bf16_scores(uint32_t tile, int rows, float (&s)[NT][4]) {
+    float d[2][4], e[2][4];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
-      const uint4 ka = lds128(tile + k_off<D * 2>(g, 4 * i + t)), kb = lds128(tile + k_off<D * 2>(g + 8, 4 * i + t));
+      uint4 q[NT];
+      load_q16(q, qb, 4 * i + t, false);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint4 q = lds128(qb + qb_off(8 * n + g, 4 * i + t));
-        mma16816<true>(s[n], ka.x, kb.x, ka.y, kb.y, q.x, q.y);
-        mma16816<true>(s[n], ka.z, kb.z, ka.w, kb.w, q.z, q.w);
+      for (int h = 0; h < 2; ++h) {
+        const uint4 k = lds128(tile + k_off<D * 2>(g + 8 * h, 4 * i + t));
+        dot16<true>(d[h], e[h], q, k.x, k.y, k.z, k.w, i == 0);
       }
     }
+    gather16(s, d, e);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -656,9 +703,8 @@ struct Worker {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float x0 = s[n][2 * h] * c, x1 = s[n][2 * h + 1] * c;
-        const uint32_t top = f32x2_to_bf16x2(x0, x1);
-        hi[n][h] = transpose8(top);
-        lo[n][h] = transpose8(f32x2_to_bf16x2(x0 - bf16lo(top), x1 - bf16hi(top)));
+        hi[n][h] = f32x2_to_bf16x2(x0, x1);
+        lo[n][h] = f32x2_to_bf16x2(x0 - bf16lo(hi[n][h]), x1 - bf16hi(hi[n][h]));
       }
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
@@ -670,96 +716,117 @@ struct Worker {
       }
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5410), a1 = __byte_perm(v[0][w], v[1][w], 0x7632);
-        const uint32_t a2 = __byte_perm(v[2][w], v[3][w], 0x5410), a3 = __byte_perm(v[2][w], v[3][w], 0x7632);
+        const uint4 a = make_uint4(__byte_perm(v[0][w], v[1][w], 0x5410), __byte_perm(v[0][w], v[1][w], 0x7632),
+                                   __byte_perm(v[2][w], v[3][w], 0x5410), __byte_perm(v[2][w], v[3][w], 0x7632));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma16816<true>(acc[n][4 * i + w], a0, a1, a2, a3, hi[n][0], hi[n][1]);
-          mma16816<true>(acc[n][4 * i + w], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+          mma16816<true>(acc[n][4 * i + w], a, hi[n][0], hi[n][1]);
+          mma16816<true>(acc[n][4 * i + w], a, lo[n][0], lo[n][1]);
         }
       }
     }
   }
 
-  // Products of int8 keys with the three digits of the queries: 64 channels i, thread t's 16 in
-  // ka (token g) and kb (token g + 8).  Whole numbers below 2^21 each, exact.
-  static __device__ __forceinline__ void zero_digits(int (&d)[3][NT][4]) {
+  // Dot products of int8 keys (64 channels i, this thread's 16 of tokens g and g + 8 in k[0], k[1])
+  // with the three digits of the queries: whole numbers below 2^21 each, exact.
+  struct Dots {
+    int d[3][2][4];  // NT = 1: the higher two digits, the lowest of the first 32 channels, of the second; NT = 2: a digit each
+  };
+  __device__ __forceinline__ void add_digits(Dots& a, const uint4 (&k)[2], int i, bool first) const {
+    if constexpr (NT == 1) {
+      const uint4 q0 = lds128(qi + digit_chunk(g, 2 * (4 * i + t))), q1 = lds128(qi + digit_chunk(g, 2 * (4 * i + t) + 1));
+      const uint4 ql = lds128(qi + low_chunk(g, 4 * i + t));
 #pragma unroll
-    for (int k = 0; k < 3; ++k)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) d[k][n][0] = d[k][n][1] = d[k][n][2] = d[k][n][3] = 0;
-  }
-  __device__ __forceinline__ void add_digits(int (&d)[3][NT][4], const uint4& ka, const uint4& kb, int i) const {
-#pragma unroll
-    for (int k = 0; k < 3; ++k)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint4 q = lds128(qi + k * (NT * 8 * D) + qi_off(8 * n + g, 4 * i + t));
-        mma16832(d[k][n], ka.x, kb.x, ka.y, kb.y, q.x, q.y);
-        mma16832(d[k][n], ka.z, kb.z, ka.w, kb.w, q.z, q.w);
+      for (int h = 0; h < 2; ++h) {
+        mma16832(a.d[0][h], q0, k[h].x, k[h].y, first);
+        mma16832(a.d[0][h], q1, k[h].z, k[h].w, false);
+        mma16832(a.d[1][h], ql, k[h].x, k[h].y, first);
+        mma16832(a.d[2][h], ql, k[h].z, k[h].w, first);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        const uint4 q0 = lds128(qi + j * (16 * D) + digit_chunk(g, 2 * (4 * i + t)));
+        const uint4 q1 = lds128(qi + j * (16 * D) + digit_chunk(g, 2 * (4 * i + t) + 1));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mma16832(a.d[j][h], q0, k[h].x, k[h].y, first);
+          mma16832(a.d[j][h], q1, k[h].z, k[h].w, false);
+        }
+      }
+    }
   }
-  static __device__ __forceinline__ float digits_value(const int (&d)[3][NT][4], int n, int x) {
-    return fmaf(float(d[0][n][x] * 256 + d[1][n][x]), 256.0f, float(d[2][n][x]));
+  static __device__ __forceinline__ float dot_value(const Dots& a, int n, int x) {
+    const int h = x >> 1, j = x & 1;
+    if constexpr (NT == 1)
+      return fmaf(float(a.d[0][h][j] * 256 + a.d[0][h][2 + j]), 256.0f, float(a.d[1][h][j] + a.d[2][h][2 + j]));
+    return fmaf(float(a.d[0][h][2 * n + j] * 256 + a.d[1][h][2 * n + j]), 256.0f, float(a.d[2][h][2 * n + j]));
+  }
+  // A tile's row scales of this lane's tokens 2t, 2t + 1, 2t + 8, 2t + 9; 0 for rows not in use.
+  __device__ __forceinline__ void zero_unused(float (&x)[4], int rows) const {
+    if (rows < 16) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (2 * t + (k & 1) + 8 * (k >> 1) >= rows) x[k] = 0.0f;
+    }
+  }
+  static __device__ __forceinline__ void fp16_pairs(uint32_t a, uint32_t b, float (&x)[4]) {
+    x[0] = f16_to_f32(uint16_t(a)) * (1.0f / 127.0f); x[1] = f16_to_f32(uint16_t(a >> 16)) * (1.0f / 127.0f);
+    x[2] = f16_to_f32(uint16_t(b)) * (1.0f / 127.0f); x[3] = f16_to_f32(uint16_t(b >> 16)) * (1.0f / 127.0f);
+  }
+  __device__ __forceinline__ void int8_scales(uint32_t at, int rows, float (&ks)[4], float (&vs)[4]) const {
+    fp16_pairs(lds32(at + 4 * t), lds32(at + 4 * t + 16), ks);
+    at += 32 + 4 * t;
+    if (p.T & 1)  // the V rows start in the upper half of a word
+      fp16_pairs(__byte_perm(lds32(at), lds32(at + 4), 0x5432), __byte_perm(lds32(at + 16), lds32(at + 20), 0x5432), vs);
+    else
+      fp16_pairs(lds32(at), lds32(at + 16), vs);
+    zero_unused(ks, rows);
+    zero_unused(vs, rows);
   }
 
   // A tile of a page of 8-bit codes, K then V.
   template <bool INT8>
   __device__ __forceinline__ void tile8(uint32_t tile, const Unit& u) {
-    float ks0 = 1.0f, ks1 = 1.0f;
-    float vs[1][2] = {{1.0f, 1.0f}};
+    float s[NT][4], vs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
     if constexpr (INT8) {
-      const float x = f16_to_f32(uint16_t(u.scale)) * (1.0f / 127.0f);
-      ks0 = __shfl_sync(0xFFFFFFFFu, x, g);
-      ks1 = __shfl_sync(0xFFFFFFFFu, x, g + 8);
-      vs[0][0] = __shfl_sync(0xFFFFFFFFu, x, g + 16);
-      vs[0][1] = __shfl_sync(0xFFFFFFFFu, x, g + 24);
-      fit_scale(lane < 16 ? 0.0f : x);
+      float ks[4];
+      int8_scales(tile + Feeder<D>::kScales, u.rows(), ks, vs);
+      fit_scale(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
+      Dots a;
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        const uint4 k[2] = {lds128(tile + k_off<D>(g, 4 * i + t)), lds128(tile + k_off<D>(g + 8, 4 * i + t))};
+        add_digits(a, k, i, i == 0);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][x] = dot_value(a, n, x) * (qs_i[n] * ks[x]);
     } else {
       fit_scale(1.0f);
-    }
-    float s[NT][4];
-    if constexpr (INT8) {
-      int d[3][NT][4];
-      zero_digits(d);
+      float d[2][4], e[2][4];
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
-        const uint4 ka = lds128(tile + k_off<D>(g, 4 * i + t)), kb = lds128(tile + k_off<D>(g + 8, 4 * i + t));
-        add_digits(d, ka, kb, i);
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s[n][x] = digits_value(d, n, x) * (qs_i[n][x & 1] * (x < 2 ? ks0 : ks1));
-    } else {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        const uint4 xa = lds128(tile + k_off<D>(g, 4 * i + t)), xb = lds128(tile + k_off<D>(g + 8, 4 * i + t));
-        const uint32_t ka[4] = {xa.x, xa.y, xa.z, xa.w}, kb[4] = {xb.x, xb.y, xb.z, xb.w};
+        uint4 q[2][NT];
+        load_q16(q[0], qh, 2 * (4 * i + t), true);
+        load_q16(q[1], qh, 2 * (4 * i + t) + 1, true);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint4 q[NT];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) q[n] = lds128(qh + qh_off(8 * n + g, 2 * (4 * i + t) + h));
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const uint32_t a0 = fp8_pair(ka[2 * h + w]), a1 = fp8_pair(kb[2 * h + w]);
-            const uint32_t a2 = fp8_pair(ka[2 * h + w] >> 16), a3 = fp8_pair(kb[2 * h + w] >> 16);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816<false>(s[n], a0, a1, a2, a3, w ? q[n].z : q[n].x, w ? q[n].w : q[n].y);
-          }
+          const uint4 k = lds128(tile + k_off<D>(g + 8 * h, 4 * i + t));
+          dot16<false>(d[h], e[h], q[0], fp8_pair(k.x), fp8_pair(k.x >> 16), fp8_pair(k.y), fp8_pair(k.y >> 16), i == 0);
+          dot16<false>(d[h], e[h], q[1], fp8_pair(k.z), fp8_pair(k.z >> 16), fp8_pair(k.w), fp8_pair(k.w >> 16), false);
         }
       }
+      gather16(s, d, e);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) s[n][x] *= qs_h[n][x & 1];
+        for (int x = 0; x < 4; ++x) s[n][x] *= qs_h[n];
     }
     weights(s, u.rows());
-    uint32_t b[1][NT][2];
-    fp16_weights<1>(s, vs, b);
+    uint32_t b[NT][2];
+    fp16_weights(s, vs, b);
     tile += 16 * D;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
@@ -776,16 +843,13 @@ struct Worker {
         for (int h = 0; h < 2; ++h) {  // channels 4w + 2h, + 1: (token, next token) bytes side by side
           const uint32_t lo = __byte_perm(v[0][w], v[1][w], h ? 0x7362 : 0x5140);
           const uint32_t hi = __byte_perm(v[2][w], v[3][w], h ? 0x7362 : 0x5140);
-          uint32_t a0, a1, a2, a3;
-          if constexpr (INT8) {
-            a0 = int8_pair(lo, 0x4140); a1 = int8_pair(lo, 0x4342);
-            a2 = int8_pair(hi, 0x4140); a3 = int8_pair(hi, 0x4342);
-          } else {
-            a0 = fp8_pair(lo); a1 = fp8_pair(lo >> 16);
-            a2 = fp8_pair(hi); a3 = fp8_pair(hi >> 16);
-          }
+          uint4 a;
+          if constexpr (INT8)
+            a = make_uint4(int8_pair(lo, 0x4140), int8_pair(lo, 0x4342), int8_pair(hi, 0x4140), int8_pair(hi, 0x4342));
+          else
+            a = make_uint4(fp8_pair(lo), fp8_pair(lo >> 16), fp8_pair(hi), fp8_pair(hi >> 16));
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816<false>(acc[n][4 * i + 2 * w + h], a0, a1, a2, a3, b[0][n][0], b[0][n][1]);
+          for (int n = 0; n < NT; ++n) mma16816<false>(acc[n][4 * i + 2 * w + h], a, b[n][0], b[n][1]);
         }
     }
   }
@@ -799,41 +863,57 @@ struct Worker {
                       __byte_perm(e1, o1, 0x7362));
   }
 
+  __device__ __forceinline__ void int4_scales(uint32_t at, int rows, float (&x)[D / 64][4]) const {
+    const uint2 a = lds64(at), b = lds64(at + 32);
+    const uint32_t w[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      if constexpr (D == 128) {
+        x[0][y] = bf16lo(w[y]) * (1.0f / 7.0f);
+        x[1][y] = bf16hi(w[y]) * (1.0f / 7.0f);
+      } else {
+        x[0][y] = (odd_head ? bf16hi(w[y]) : bf16lo(w[y])) * (1.0f / 7.0f);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) zero_unused(x[k], rows);
+  }
+
   // A tile of an INT4 page (scales per 64 channels), K then V.
   __device__ __forceinline__ void tile4(uint32_t tile, const Unit& u) {
     constexpr int K = D / 64;
-    float s[NT][4], vs[K][2], x_max = 0.0f;
+    float ks[K][4], vs[K][4];
+    int4_scales(tile + Feeder<D>::kScales + 8 * t, u.rows(), ks);
+    int4_scales(tile + Feeder<D>::kScales + 8 * t + 64, u.rows(), vs);
+    float top = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+    for (int k = 0; k < K; ++k) top = fmaxf(top, fmaxf(fmaxf(vs[k][0], vs[k][1]), fmaxf(vs[k][2], vs[k][3])));
+    fit_scale(top);
+    float s[NT][4];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const float x = (k ? bf16hi(u.scale) : bf16lo(u.scale)) * (1.0f / 7.0f);
-      const float ks0 = __shfl_sync(0xFFFFFFFFu, x, g), ks1 = __shfl_sync(0xFFFFFFFFu, x, g + 8);
-      vs[k][0] = __shfl_sync(0xFFFFFFFFu, x, g + 16);
-      vs[k][1] = __shfl_sync(0xFFFFFFFFu, x, g + 24);
-      x_max = fmaxf(x_max, x);
-      const uint2 xa = lds64(tile + k_off<D / 2>(g, 2 * k + (t >> 1)) + (t & 1) * 8);
-      const uint2 xb = lds64(tile + k_off<D / 2>(g + 8, 2 * k + (t >> 1)) + (t & 1) * 8);
-      int d[3][NT][4];
-      zero_digits(d);
-      add_digits(d, nibbles_x16(xa), nibbles_x16(xb), k);
+      const uint4 x[2] = {nibbles_x16(lds64(tile + k_off<D / 2>(g, 2 * k + (t >> 1)) + (t & 1) * 8)),
+                          nibbles_x16(lds64(tile + k_off<D / 2>(g + 8, 2 * k + (t >> 1)) + (t & 1) * 8))};
+      Dots a;
+      add_digits(a, x, k, true);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) s[n][y] = fmaf(digits_value(d, n, y), y < 2 ? ks0 : ks1, s[n][y]);
+        for (int y = 0; y < 4; ++y) {
+          const float z = dot_value(a, n, y);
+          s[n][y] = k ? fmaf(z, ks[k][y], s[n][y]) : z * ks[k][y];
+        }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int y = 0; y < 4; ++y) s[n][y] *= qs_i[n][y & 1] * 0.0625f;
-    fit_scale(lane < 16 ? 0.0f : x_max);
+      for (int y = 0; y < 4; ++y) s[n][y] *= qs_i[n] * 0.0625f;
     weights(s, u.rows());
-    uint32_t b[K][NT][2];
-    fp16_weights<K>(s, vs, b);
     tile += 8 * D;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      uint32_t v[4];
+      uint32_t b[NT][2], v[4];
+      fp16_weights(s, vs[k], b);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         v[j] = lds32(tile + v_off<D / 2>(2 * t + (j & 1) + 8 * (j >> 1), 2 * k + (g >> 2)) + (g & 3) * 4);
@@ -842,9 +922,9 @@ struct Worker {
         uint32_t lo = __byte_perm(v[0], v[1], h ? 0x7632 : 0x5410), hi = __byte_perm(v[2], v[3], h ? 0x7632 : 0x5410);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const uint32_t a0 = nibble_hi(lo), a1 = nibble_lo(lo), a2 = nibble_hi(hi), a3 = nibble_lo(hi);
+          const uint4 a = make_uint4(nibble_hi(lo), nibble_lo(lo), nibble_hi(hi), nibble_lo(hi));
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816<false>(acc[n][4 * k + 2 * h + w], a0, a1, a2, a3, b[k][n][0], b[k][n][1]);
+          for (int n = 0; n < NT; ++n) mma16816<false>(acc[n][4 * k + 2 * h + w], a, b[n][0], b[n][1]);
           lo >>= 8;
           hi >>= 8;
         }
@@ -852,35 +932,28 @@ struct Worker {
     }
   }
 
-  static __device__ __forceinline__ float sum_over_tokens(float x) {
-    x += __shfl_xor_sync(0xFFFFFFFFu, x, 4);
-    x += __shfl_xor_sync(0xFFFFFFFFu, x, 8);
-    return x + __shfl_xor_sync(0xFFFFFFFFu, x, 16);
-  }
   // The log2-sum of the page that just ended, for its mass.
   __device__ __forceinline__ void page_sum(int b, int pos, int hq0, int nq) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float sum = sum_over_tokens(ps[n][j]);
-        const int q = 8 * n + 2 * t + j;
-        if (g == 0 && q < nq)
-          p.page_lse2[(int64_t(b) * p.max_pages + pos) * p.heads_q + hq0 + q] = m[n][j] + log2f(sum);
-        ps[n][j] = 0.0f;
-      }
+    for (int n = 0; n < NT; ++n) {
+      const float sum = sum_over_tokens(ps[n]);
+      if (t == 0 && 8 * n + g < nq)
+        p.page_lse2[(int64_t(b) * p.max_pages + pos) * p.heads_q + hq0 + 8 * n + g] = m[n] + __log2f(sum);
+      ps[n] = 0.0f;
+    }
   }
   // The segment's partial result.
   __device__ void finish(int64_t row0, int nq) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+      const float sum = sum_over_tokens(l[n]);
+      if (t == 0 && 8 * n + g < nq) p.part_lse2[row0 + 8 * n + g] = m[n] + log2f(sum);
+      const float own = sum == 0.0f ? 0.0f : (1.0f / sum) * (1.0f / c);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float sum = sum_over_tokens(l[n][j]);
-        const float inv = sum == 0.0f ? 0.0f : (1.0f / sum) * (1.0f / c);
+        const float inv = of_column(own, j);
         const int q = 8 * n + 2 * t + j;
         if (q >= nq) continue;
-        if (g == 0) p.part_lse2[row0 + q] = m[n][j] + log2f(sum);
         float* o = p.part_o + (row0 + q) * D;
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
@@ -895,9 +968,9 @@ struct Worker {
           at[1] = make_float4(x[4], x[5], x[6], x[7]);
         }
       }
+    }
   }
 };
-
 
 template <int D, int NT>
 __global__ void __launch_bounds__(kWarpsA * 32, NT == 1 ? 3 : 2) decode_partials_kernel(const __grid_constant__ AttnParams p) {
@@ -921,7 +994,7 @@ __global__ void __launch_bounds__(kWarpsA * 32, NT == 1 ? 3 : 2) decode_partials
   }
   const uint32_t ring = smem_u32(smem) + uint32_t(warp * p.warp_smem);
   Feeder<D> feed(p, hk, ring);
-  Worker<D, NT> work(p, ring + kRing * Feeder<D>::kUnitBytes);
+  Worker<D, NT> work(p, ring + kRing * Feeder<D>::kUnitBytes, hk);
   for (; pos < end; ++b) {
     const int n = list_len(p, b, hk);
     if (n == 0) continue;
