@@ -11,6 +11,7 @@
 // weighs the partials of each sequence by 2^(their log2-sum - the total).
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 #include "common.cuh"
 #include "nbit_group.cuh"
@@ -90,53 +91,6 @@ __device__ int lists_before(const AttnParams& p, int b, int hk) {
 }
 // Pages per range; every range but the last of the row has as many.
 __device__ __forceinline__ int range_len(const AttnParams& p, int total) { return max(1, (total + p.ranges - 1) / p.ranges); }
-
-// The page behind list entry i of (sequence b, key head hk), as the copies need it.
-struct PageRef {
-  const uint8_t* k;   // BF16: K channel 0 of the head at the page's first token; codes: the same; dithered: the slot
-  const uint8_t* v;   // BF16: the same of V; codes: the slot
-  uint32_t meta;      // format | tokens in use << 8; no tokens: a page to leave out
-  int32_t pos;        // position in the sequence
-};
-template <int D>
-__device__ PageRef resolve(const AttnParams& p, int b, int hk, int i, int64_t tokens) {
-  PageRef r{nullptr, nullptr, 0, i};
-  if (p.selected) {
-    r.pos = p.selected[(int64_t(b) * p.heads_kv + hk) * p.max_selected + i];
-    if (r.pos < 0 || int64_t(r.pos) * p.T >= tokens) {
-      flag(p.status, ASHKV_FLAG_INDEX_RANGE);
-      r.pos = 0;
-      return r;
-    }
-  }
-  const int32_t id = p.page_ids[int64_t(b) * p.page_ids_stride + r.pos];
-  bool ok = id >= 0 && id < p.n_pages;
-  const int t = ok ? p.tier[id] : -1;
-  ok = ok && t >= 0 && t < kTiers && (t == 0 || p.store[t].format != ASHKV_PAGE_NONE);
-  if (ok && t == 0) {
-    const int32_t l = p.layer_id[id], ts = p.token_start[id];
-    ok = l >= 0 && l < p.n_layers && ts >= 0 && int64_t(ts) + p.T <= p.pool_tokens;
-    if (ok) {
-      const int64_t off = (int64_t(ts) * p.row_stride + hk * D) * 2;
-      r.k = reinterpret_cast<const uint8_t*>(p.layer_k[l]) + off;
-      r.v = reinterpret_cast<const uint8_t*>(p.layer_v[l]) + off;
-      r.meta = ASHKV_PAGE_BF16;
-    }
-  } else if (ok) {
-    const int32_t s = p.page_slot[id];
-    ok = s >= 0 && s < p.store[t].n_slots;
-    if (ok) {
-      r.v = r.k = p.store[t].data + int64_t(s) * p.store[t].slot_bytes;
-      r.meta = uint32_t(p.store[t].format);
-      if (r.meta == ASHKV_PAGE_INT8) r.k += int8_codes_offset(p.T) + hk * D;
-      if (r.meta == ASHKV_PAGE_FP8) r.k += hk * D;
-      if (r.meta == ASHKV_PAGE_INT4) r.k += p.T * p.row_len / 16 + hk * (D / 2);  // past E / 32 bytes of scales
-    }
-  }
-  if (ok) r.meta |= uint32_t(min(int64_t(p.T), tokens - int64_t(r.pos) * p.T)) << 8;
-  else flag(p.status, ASHKV_FLAG_INDEX_RANGE);
-  return r;
-}
 
 // ---------------------------------------------------------------- tensor-core pieces
 // D (16 x 8, fp32) = A (16 x 16, row) * B (16 x 8, col) + (first ? 0 : D).  Lane (g,
@@ -257,13 +211,37 @@ constexpr int kRing = 3;  // units in shared memory per warp: one in use, two on
 // page (16 x D bf16), or the codes of both of a compressed page (K first), and
 // behind them the scales of those rows: INT8: fp16, K then V, the V rows from the
 // last 4-byte boundary on; INT4: a word per row, K then V (D = 64: the row's scale
-// for this head is the word's upper half for an odd head).
-struct Unit {
-  uint32_t meta;   // format | kIsV (BF16: the V rows) | kLast (the page's last unit) | tokens in use << 16; 0: none
-  int32_t pos;     // page position in the sequence
-  static constexpr uint32_t kIsV = 0x100u, kLast = 0x200u;
+// for this head is the word's upper half for an odd head).  A page to leave out
+// takes a unit that nothing is copied to.
+//
+// The list entries of a segment are looked up 16 at a time, a lane each, in four
+// steps a few pages apart (position, page id, page-table columns, layer address),
+// so that no step waits for the loads of the one before it; the result, where to
+// copy from, goes to a ring of 32 references in shared memory that both ends of
+// the unit ring read.
+constexpr int kRefs = 32, kLook = 16;
+constexpr int kRefBytes = kRefs * 24;  // {k, meta, pos} of every entry, then v
+// k: BF16: K channel 0 of the head at the page's first token; codes: the same; dithered: the slot.
+// v: BF16: the same of V; INT8, INT4: where the slot's scales start.
+// meta: format | tokens in use << 8 (none: a page to leave out); pos: position in the sequence.
+struct PageRef {
+  const uint8_t* k;
+  uint32_t meta;
+  int32_t pos;
   __device__ __forceinline__ uint32_t format() const { return meta & 0xFFu; }
-  __device__ __forceinline__ int rows() const { return int(meta >> 16); }
+  __device__ __forceinline__ int tokens() const { return int(meta >> 8); }
+};
+
+__device__ __forceinline__ const uint8_t* address(uint32_t lo, uint32_t hi) {
+  return reinterpret_cast<const uint8_t*>(uint64_t(lo) | uint64_t(hi) << 32);
+}
+
+// A place in the units of a segment.
+struct Cursor {
+  int i;         // list entry
+  int t0;        // first token in its page (pages of at most 16 tokens: 0)
+  bool second;   // BF16: the V rows
+  uint32_t unit; // shared address of the unit
 };
 
 // Decodes the K or V rows of a dithered page into a BF16 unit.
@@ -309,130 +287,192 @@ __device__ __noinline__ void stage_nbit(const uint8_t* slot, int T, int row_len,
     }
   }
 
-template <int D>
+// T16: pages have 16 tokens (the library's default), one tile each.
+template <int D, bool T16>
 struct Feeder {
   static constexpr int kScales = 16 * D * 2;           // byte offset of the scales
   static constexpr int kUnitBytes = kScales + 128;
   const AttnParams& p;
-  int b, hk, i, i1;       // next list entry, end of the segment
+  int b, hk, i1;          // sequence, key head, end of the segment's entries
   int64_t tokens;
-  uint32_t ring, dst;     // shared addresses of the warp's ring and of the next unit
-  int t0;                 // first token of the next unit in its page
-  bool second;            // BF16: the V unit of (page, t0) is next
-  PageRef batch;          // lane l: list entry batch0 + l
-  int batch0;
-  PageRef page;           // current page; no tokens in use: none
+  uint32_t ring, refs;    // shared addresses of the units and of the references
+  Cursor at;              // the next unit to send
+  PageRef page;           // its page
+  const uint8_t* page_v;
+  int look, step;         // first entry being looked up, next step
+  int pos, id, tier, layer, start_or_slot;
+  uint32_t lane16, lane8, lane4;  // byte offset of this lane's first chunk in rows of 16-, 8- and 4-bit elements
 
-  __device__ __forceinline__ Feeder(const AttnParams& p_, int hk_, uint32_t ring_) : p(p_), hk(hk_), ring(ring_) {}
+  __device__ __forceinline__ Feeder(const AttnParams& p_, int hk_, uint32_t ring_)
+      : p(p_), hk(hk_), ring(ring_), refs(ring_ + kRing * kUnitBytes) {
+    const uint32_t lane = threadIdx.x & 31u, row = uint32_t(p.row_len);
+    lane16 = lane / (D / 8) * uint32_t(p.row_stride) * 2u + lane % (D / 8) * 16u;
+    lane8 = lane / (D / 16) * row + lane % (D / 16) * 16u;
+    lane4 = lane / (D / 32) * (row / 2) + lane % (D / 32) * 16u;
+  }
+  __device__ __forceinline__ int page_tokens() const { return T16 ? 16 : p.T; }
+
   __device__ __forceinline__ void start(int b_, int i0, int i1_) {
-    b = b_; i = i0; i1 = i1_; tokens = seq_tokens(p, b); batch0 = i0 - 32; t0 = 0; second = false; dst = ring;
-    next_page();
+    b = b_; i1 = i1_; tokens = seq_tokens(p, b);
+    at = Cursor{i0, 0, false, ring};
+    look = i0;
+    for (step = 0; step < 4; ++step) look_up();
+    look = i0 + kLook;
+    step = 0;
   }
-  // Makes list entry i, or the next one with tokens, the current page.
-  __device__ __forceinline__ void next_page() {
-    for (; i < i1; ++i) {
-      if (i >= batch0 + 32) next_batch();
-      const int src = i - batch0;
-      page.meta = __shfl_sync(0xFFFFFFFFu, batch.meta, src);
-      page.pos = __shfl_sync(0xFFFFFFFFu, batch.pos, src);
-      if (page.meta >> 8) {
-        page.k = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(batch.k), src));
-        page.v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(batch.v), src));
-        return;
+  // One step of the look-up of entries look .. look + 15 (lane l: look + l).
+  __device__ __forceinline__ void look_up() {
+    const int lane = threadIdx.x & 31, i = look + lane;
+    const bool mine = lane < kLook && i < i1;
+    if (step == 0) {
+      pos = mine && p.selected ? p.selected[(int64_t(b) * p.heads_kv + hk) * p.max_selected + i] : i;
+    } else if (step == 1) {
+      const bool ok = mine && pos >= 0 && int64_t(pos) * page_tokens() < tokens;
+      id = ok ? p.page_ids[int64_t(b) * p.page_ids_stride + pos] : -1;
+      if (!ok) pos = 0;
+    } else if (step == 2) {
+      const bool ok = id >= 0 && id < p.n_pages;
+      tier = ok ? p.tier[id] : -1;
+      layer = ok ? p.layer_id[id] : 0;
+      start_or_slot = ok ? p.token_start[id] : 0;
+      const int slot = ok ? p.page_slot[id] : 0;
+      if (tier != 0) start_or_slot = slot;
+    } else if (mine) {
+      const uint8_t *k = nullptr, *v = nullptr;
+      uint32_t meta = 0;
+      bool ok = tier >= 0 && tier < kTiers;
+      if (ok && tier == 0) {
+        ok = layer >= 0 && layer < p.n_layers && start_or_slot >= 0 &&
+             int64_t(start_or_slot) + page_tokens() <= p.pool_tokens;
+        if (ok) {
+          const int64_t off = (int64_t(start_or_slot) * p.row_stride + hk * D) * 2;
+          k = reinterpret_cast<const uint8_t*>(p.layer_k[layer]) + off;
+          v = reinterpret_cast<const uint8_t*>(p.layer_v[layer]) + off;
+          meta = ASHKV_PAGE_BF16;
+        }
+      } else if (ok) {
+        const Store& st = p.store[tier];
+        ok = st.format != ASHKV_PAGE_NONE && start_or_slot >= 0 && start_or_slot < st.n_slots;
+        if (ok) {
+          v = k = st.data + int64_t(start_or_slot) * st.slot_bytes;
+          meta = uint32_t(st.format);
+          if (meta == ASHKV_PAGE_INT8) k += int8_codes_offset(page_tokens()) + hk * D;
+          if (meta == ASHKV_PAGE_FP8) k += hk * D;
+          if (meta == ASHKV_PAGE_INT4) {
+            k += page_tokens() * p.row_len / 16 + hk * (D / 2);  // past E / 32 bytes of scales
+            v += hk * D / 32 & ~3;
+          }
+        }
       }
+      if (ok) {
+        meta |= uint32_t(min(int64_t(page_tokens()), tokens - int64_t(pos) * page_tokens())) << 8;
+      } else {
+        flag(p.status, ASHKV_FLAG_INDEX_RANGE);
+        if (p.mass)  // a page that is left out draws nothing
+          for (int g = 0; g < p.group; ++g)
+            p.page_lse2[(int64_t(b) * p.max_pages + pos) * p.heads_q + hk * p.group + g] = -INFINITY;
+      }
+      const uint32_t e = uint32_t(i) & (kRefs - 1);
+      const uint64_t ka = reinterpret_cast<uint64_t>(k), va = reinterpret_cast<uint64_t>(v);
+      sts128(refs + e * 16, make_uint4(uint32_t(ka), uint32_t(ka >> 32), meta, uint32_t(pos)));
+      asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(refs + kRefs * 16 + e * 8), "r"(uint32_t(va)), "r"(uint32_t(va >> 32)) : "memory");
     }
-    page.meta = 0;
+    if (step == 3) __syncwarp();
   }
-  __device__ __forceinline__ void next_batch() {
-    const int lane = threadIdx.x & 31;
-    batch0 = i;
-    if (i + lane < i1) {
-      batch = resolve<D>(p, b, hk, i + lane, tokens);
-      if (p.mass && !(batch.meta >> 8))  // a page that is left out draws nothing
-        for (int g = 0; g < p.group; ++g)
-          p.page_lse2[(int64_t(b) * p.max_pages + batch.pos) * p.heads_q + hk * p.group + g] = -INFINITY;
-    }
+  __device__ __forceinline__ PageRef ref(int i) const {
+    const uint4 x = lds128(refs + (uint32_t(i) & (kRefs - 1)) * 16);
+    return PageRef{address(x.x, x.y), x.z, int32_t(x.w)};
   }
 
-  // 16 rows of RB bytes, `step` bytes apart from src on, into a tile; rows behind `rows` become zeros.
+  // Moves a cursor behind its unit; true where that ends the page.
+  static __device__ __forceinline__ bool advance(Cursor& c, const PageRef& page, uint32_t ring) {
+    c.unit = c.unit == ring + (kRing - 1) * kUnitBytes ? ring : c.unit + kUnitBytes;
+    const bool two = page.format() == ASHKV_PAGE_BF16 || page.format() >= ASHKV_PAGE_NBIT4;
+    if (two && !c.second && page.tokens()) {
+      c.second = true;
+      return false;
+    }
+    c.second = false;
+    if constexpr (!T16) {
+      c.t0 += 16;
+      if (c.t0 < page.tokens()) return false;
+      c.t0 = 0;
+    }
+    ++c.i;
+    return true;
+  }
+
+  // 16 rows of RB bytes, `step` bytes apart, into a tile, src being this lane's first chunk; rows
+  // behind `rows` become zeros.
   template <int RB, bool V>
-  __device__ __forceinline__ void copy_rows(const uint8_t* src, uint32_t step, int rows, uint32_t tile) const {
+  __device__ __forceinline__ void copy_rows(const uint8_t* src, uint32_t step_bytes, int rows, uint32_t tile) const {
     const uint32_t lane = threadIdx.x & 31u;
     constexpr uint32_t CPR = RB / 16, RPI = 32 / CPR;  // chunks of a row, rows of one instruction
     const uint32_t r0 = lane / CPR, col = lane % CPR;
-    src += r0 * step + col * 16u;
-    if (rows == 16) {
+    step_bytes *= RPI;
+    if (rows >= 16) {
 #pragma unroll
-      for (uint32_t j = 0; j < 16 / RPI; ++j)
-        cp_async16(tile + (V ? v_off<RB>(r0 + RPI * j, col) : k_off<RB>(r0 + RPI * j, col)), src + uint64_t(step) * (RPI * j));
+      for (uint32_t j = 0; j < 16 / RPI; ++j) {
+        cp_async16(tile + (V ? v_off<RB>(r0 + RPI * j, col) : k_off<RB>(r0 + RPI * j, col)), src);
+        src += step_bytes;
+      }
       return;
     }
 #pragma unroll 1
     for (uint32_t j = 0; j < 16 / RPI; ++j) {
       const uint32_t r = r0 + RPI * j;
       const bool real = r < uint32_t(rows);
-      cp_async16_or_zero(tile + (V ? v_off<RB>(r, col) : k_off<RB>(r, col)), real ? src + uint64_t(step) * (RPI * j) : page.k, real);
+      cp_async16_or_zero(tile + (V ? v_off<RB>(r, col) : k_off<RB>(r, col)), real ? src + uint64_t(step_bytes) * j : page.k, real);
     }
   }
 
-  // Sends the next unit on its way (always one cp.async group) and describes it.
-  __device__ __forceinline__ Unit issue() {
-    Unit u{0u, page.pos};
-    if (page.meta) {
-      const uint32_t lane = threadIdx.x & 31u;
-      const uint32_t format = page.meta & 0xFFu;
-      const int left = int(page.meta >> 8) - t0, rows = min(16, left);
-      u.meta = format | uint32_t(rows) << 16;
-      const uint32_t row = uint32_t(p.row_len);
-      bool done = true;  // with these tokens
-      if (format == ASHKV_PAGE_BF16) {
-        const uint32_t step = uint32_t(p.row_stride) * 2u;
-        if (second) {
-          u.meta |= Unit::kIsV;
-          copy_rows<D * 2, true>(page.v + uint32_t(t0) * step, step, rows, dst);
-        } else {
-          copy_rows<D * 2, false>(page.k + uint32_t(t0) * step, step, rows, dst);
-        }
-        done = second;
-        second = !second;
-      } else if (format >= ASHKV_PAGE_NBIT4) {
-        u.meta = ASHKV_PAGE_BF16 | uint32_t(rows) << 16 | (second ? Unit::kIsV : 0u);
-        if (format == ASHKV_PAGE_NBIT4) stage_nbit<D, 4>(page.k, p.T, p.row_len, p.outlier_cap, hk, second, t0, rows, dst);
-        else stage_nbit<D, 2>(page.k, p.T, p.row_len, p.outlier_cap, hk, second, t0, rows, dst);
-        done = second;
-        second = !second;
-      } else {
-        if (format == ASHKV_PAGE_INT4) {
-          const uint32_t step = row / 2;
-          const uint8_t* codes = page.k + uint32_t(t0) * step;
-          copy_rows<D / 2, false>(codes, step, rows, dst);
-          copy_rows<D / 2, true>(codes + uint32_t(p.T) * step, step, rows, dst + 8 * D);
-          const uint32_t sr = min(uint32_t(t0) + (lane & 15u), uint32_t(p.T) - 1u) + (lane & 16u ? uint32_t(p.T) : 0u);
-          cp_async4(dst + kScales + lane * 4u, page.v + ((sr * row + hk * D) / 32u & ~3u));
-        } else {
-          const uint8_t* codes = page.k + uint32_t(t0) * row;
-          copy_rows<D, false>(codes, row, rows, dst);
-          copy_rows<D, true>(codes + uint32_t(p.T) * row, row, rows, dst + 16 * D);
-          if (format == ASHKV_PAGE_INT8 && lane < 17u) {
-            // 8 words of K scales, 9 of V scales (all inside the slot: codes follow them)
-            const uint32_t at = lane < 8u ? uint32_t(t0) * 2u + lane * 4u : (uint32_t(p.T + t0) * 2u & ~3u) + (lane - 8u) * 4u;
-            cp_async4(dst + kScales + lane * 4u, page.v + at);
+  // Sends the next unit on its way (always one cp.async group).
+  __device__ __forceinline__ void issue() {
+    if (at.i < i1) {
+      if (!at.second && (T16 || at.t0 == 0)) {  // the next page
+        if (!((at.i - look) & 3)) {  // every four pages a step for the next 16 entries
+          if (at.i == look) {        // their first is due: the look-up is done
+            look += kLook;
+            step = 0;
           }
+          look_up();
+          ++step;
         }
+        page = ref(at.i);
+        const uint2 x = lds64(refs + kRefs * 16 + (uint32_t(at.i) & (kRefs - 1)) * 8);
+        page_v = address(x.x, x.y);
       }
-      if (done) {
-        t0 += 16;
-        if (left <= 16) {
-          u.meta |= Unit::kLast;
-          t0 = 0;
-          ++i;
-          next_page();
+      const uint32_t lane = threadIdx.x & 31u, format = page.format(), row = uint32_t(p.row_len), dst = at.unit;
+      const uint32_t t0 = T16 ? 0u : uint32_t(at.t0), T = uint32_t(page_tokens());
+      const int left = page.tokens() - int(t0);
+      if (left <= 0) {
+      } else if (format == ASHKV_PAGE_BF16) {
+        const uint32_t step_bytes = uint32_t(p.row_stride) * 2u;
+        if (at.second) copy_rows<D * 2, true>(page_v + (lane16 + t0 * step_bytes), step_bytes, left, dst);
+        else copy_rows<D * 2, false>(page.k + (lane16 + t0 * step_bytes), step_bytes, left, dst);
+      } else if (format == ASHKV_PAGE_INT4) {
+        const uint8_t* codes = page.k + (lane4 + t0 * (row / 2));
+        copy_rows<D / 2, false>(codes, row / 2, left, dst);
+        copy_rows<D / 2, true>(codes + T * (row / 2), row / 2, left, dst + 8 * D);
+        const uint32_t sr = T16 ? lane : min(t0 + (lane & 15u), T - 1u) + (lane & 16u ? T : 0u);
+        cp_async4(dst + kScales + lane * 4u, page_v + sr * (row / 32u));
+      } else if (format < ASHKV_PAGE_NBIT4) {
+        const uint8_t* codes = page.k + (lane8 + t0 * row);
+        copy_rows<D, false>(codes, row, left, dst);
+        copy_rows<D, true>(codes + T * row, row, left, dst + 16 * D);
+        if (format == ASHKV_PAGE_INT8 && lane < 17u) {
+          // 8 words of K scales, 9 of V scales (all inside the slot: codes follow them)
+          const uint32_t o = lane < 8u ? t0 * 2u + lane * 4u : ((T + t0) * 2u & ~3u) + (lane - 8u) * 4u;
+          cp_async4(dst + kScales + lane * 4u, page_v + o);
         }
+      } else if (format == ASHKV_PAGE_NBIT4) {
+        stage_nbit<D, 4>(page.k, p.T, p.row_len, p.outlier_cap, hk, at.second, int(t0), min(left, 16), dst);
+      } else {
+        stage_nbit<D, 2>(page.k, p.T, p.row_len, p.outlier_cap, hk, at.second, int(t0), min(left, 16), dst);
       }
-      dst = dst == ring + (kRing - 1) * kUnitBytes ? ring : dst + kUnitBytes;
+      advance(at, page, ring);
     }
     cp_async_commit();
-    return u;
   }
 };
 
@@ -467,11 +507,11 @@ struct Worker {
   uint32_t qb, qh, qi;
   int lane, g, t;
   bool fresh;               // no scale was seen yet
-  bool odd_head;
+  bool odd_head, odd_pages;
 
   __device__ __forceinline__ Worker(const AttnParams& p_, uint32_t q_smem, int hk)
       : p(p_), qb(q_smem), qh(q_smem + NT * 8 * D * 2), qi(qh + (p_.fp8_pages ? NT * 8 * D * 2 : 0)),
-        lane(threadIdx.x & 31), g(lane >> 2), t(lane & 3), odd_head(hk & 1) {}
+        lane(threadIdx.x & 31), g(lane >> 2), t(lane & 3), odd_head(hk & 1), odd_pages(p_.T & 1) {}
 
   // 16-bit queries.  Channels 8 k .. 8 k + 7 (words w = 0 .. 3 of two) serve two products of 16
   // channels, words 0, 1 the first.  NT = 1: one operand (0, 2, 1, 3), the second product's words in
@@ -777,7 +817,7 @@ struct Worker {
   __device__ __forceinline__ void int8_scales(uint32_t at, int rows, float (&ks)[4], float (&vs)[4]) const {
     fp16_pairs(lds32(at + 4 * t), lds32(at + 4 * t + 16), ks);
     at += 32 + 4 * t;
-    if (p.T & 1)  // the V rows start in the upper half of a word
+    if (odd_pages)  // the V rows start in the upper half of a word
       fp16_pairs(__byte_perm(lds32(at), lds32(at + 4), 0x5432), __byte_perm(lds32(at + 16), lds32(at + 20), 0x5432), vs);
     else
       fp16_pairs(lds32(at), lds32(at + 16), vs);
@@ -787,11 +827,11 @@ struct Worker {
 
   // A tile of a page of 8-bit codes, K then V.
   template <bool INT8>
-  __device__ __forceinline__ void tile8(uint32_t tile, const Unit& u) {
+  __device__ __forceinline__ void tile8(uint32_t tile, int rows) {
     float s[NT][4], vs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
     if constexpr (INT8) {
       float ks[4];
-      int8_scales(tile + Feeder<D>::kScales, u.rows(), ks, vs);
+      int8_scales(tile + 16 * D * 2, rows, ks, vs);
       fit_scale(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
       Dots a;
 #pragma unroll
@@ -824,7 +864,7 @@ struct Worker {
 #pragma unroll
         for (int x = 0; x < 4; ++x) s[n][x] *= qs_h[n];
     }
-    weights(s, u.rows());
+    weights(s, rows);
     uint32_t b[NT][2];
     fp16_weights(s, vs, b);
     tile += 16 * D;
@@ -880,11 +920,11 @@ struct Worker {
   }
 
   // A tile of an INT4 page (scales per 64 channels), K then V.
-  __device__ __forceinline__ void tile4(uint32_t tile, const Unit& u) {
+  __device__ __forceinline__ void tile4(uint32_t tile, int rows) {
     constexpr int K = D / 64;
     float ks[K][4], vs[K][4];
-    int4_scales(tile + Feeder<D>::kScales + 8 * t, u.rows(), ks);
-    int4_scales(tile + Feeder<D>::kScales + 8 * t + 64, u.rows(), vs);
+    int4_scales(tile + 16 * D * 2 + 8 * t, rows, ks);
+    int4_scales(tile + 16 * D * 2 + 8 * t + 64, rows, vs);
     float top = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) top = fmaxf(top, fmaxf(fmaxf(vs[k][0], vs[k][1]), fmaxf(vs[k][2], vs[k][3])));
@@ -908,7 +948,7 @@ struct Worker {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int y = 0; y < 4; ++y) s[n][y] *= qs_i[n] * 0.0625f;
-    weights(s, u.rows());
+    weights(s, rows);
     tile += 8 * D;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -972,7 +1012,7 @@ struct Worker {
   }
 };
 
-template <int D, int NT>
+template <int D, int NT, bool T16>
 __global__ void __launch_bounds__(kWarpsA * 32, NT == 1 ? 3 : 2) decode_partials_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5;
@@ -993,38 +1033,37 @@ __global__ void __launch_bounds__(kWarpsA * 32, NT == 1 ? 3 : 2) decode_partials
     before += n;
   }
   const uint32_t ring = smem_u32(smem) + uint32_t(warp * p.warp_smem);
-  Feeder<D> feed(p, hk, ring);
-  Worker<D, NT> work(p, ring + kRing * Feeder<D>::kUnitBytes, hk);
+  Feeder<D, T16> feed(p, hk, ring);
+  Worker<D, NT> work(p, ring + kRing * Feeder<D, T16>::kUnitBytes + kRefBytes, hk);
   for (; pos < end; ++b) {
     const int n = list_len(p, b, hk);
     if (n == 0) continue;
     const int i0 = int(pos - before), i1 = int(min(int64_t(n), end - before));
     feed.start(b, i0, i1);
     work.start(b, hq0, nq);
-    Unit next[kRing] = {};
     float s[NT][4];  // weights of a BF16 tile between its K and its V unit
-    uint32_t tile = ring;
-    for (int ahead = 0;; ++ahead) {
-#pragma unroll
-      for (int k = 0; k + 1 < kRing; ++k) next[k] = next[k + 1];
-      next[kRing - 1] = feed.issue();
+    Cursor at{i0, 0, false, ring};
+    for (int ahead = 0; at.i < i1; ++ahead) {
+      feed.issue();
       if (ahead < kRing - 1) continue;
-      const Unit u = next[0];
-      if (!u.meta) break;
+      const PageRef page = feed.ref(at.i);
+      const int left = page.tokens() - at.t0;
       cp_async_wait<kRing - 1>();
       __syncwarp();
-      if (u.format() == ASHKV_PAGE_BF16) {
-        if (u.meta & Unit::kIsV) work.bf16_values(tile, s);
-        else work.bf16_scores(tile, u.rows(), s);
-      } else if (u.format() == ASHKV_PAGE_INT8) {
-        work.template tile8<true>(tile, u);
-      } else if (u.format() == ASHKV_PAGE_FP8) {
-        work.template tile8<false>(tile, u);
+      if (left <= 0) {
+      } else if (page.format() == ASHKV_PAGE_INT8) {
+        work.template tile8<true>(at.unit, left);
+      } else if (page.format() == ASHKV_PAGE_FP8) {
+        work.template tile8<false>(at.unit, left);
+      } else if (page.format() == ASHKV_PAGE_INT4) {
+        work.tile4(at.unit, left);
+      } else if (at.second) {
+        work.bf16_values(at.unit, s);
       } else {
-        work.tile4(tile, u);
+        work.bf16_scores(at.unit, left, s);
       }
-      if (p.mass && (u.meta & Unit::kLast)) work.page_sum(b, u.pos, hq0, nq);
-      tile = tile == ring + (kRing - 1) * Feeder<D>::kUnitBytes ? ring : tile + Feeder<D>::kUnitBytes;
+      const bool done = Feeder<D, T16>::advance(at, page, ring);
+      if (p.mass && done && left > 0) work.page_sum(b, page.pos, hq0, nq);
       __syncwarp();  // every lane has read the unit
     }
     cp_async_wait<0>();
@@ -1168,17 +1207,17 @@ ashkv_status_t refuse(const char* what, const char* why) {
   return ASHKV_BAD_ARGUMENT;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool T16>
 ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
   const int64_t workers = int64_t(p.ranges) * p.heads_kv * p.q_chunks;
-  p.warp_smem = kRing * Feeder<D>::kUnitBytes + NT * 8 * D * (2 + (p.fp8_pages ? 2 : 0) + (p.int_pages ? 3 : 0));
+  p.warp_smem = kRing * Feeder<D, T16>::kUnitBytes + kRefBytes + NT * 8 * D * (2 + (p.fp8_pages ? 2 : 0) + (p.int_pages ? 3 : 0));
   const int smem = kWarpsA * p.warp_smem;
-  const cudaError_t e = cudaFuncSetAttribute(decode_partials_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = cudaFuncSetAttribute(decode_partials_kernel<D, NT, T16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     set_error("ashkv_decode_attention (shared memory attribute)", e);
     return ASHKV_LAUNCH_ERROR;
   }
-  decode_partials_kernel<D, NT><<<unsigned((workers + kWarpsA - 1) / kWarpsA), kWarpsA * 32, smem, st>>>(p);
+  decode_partials_kernel<D, NT, T16><<<unsigned((workers + kWarpsA - 1) / kWarpsA), kWarpsA * 32, smem, st>>>(p);
   int64_t blocks = int64_t(p.n_seqs) * p.heads_q;
   if (p.mass) blocks += int64_t(p.n_seqs) * ((p.max_pages + kJoinThreads - 1) / kJoinThreads);
   decode_join_kernel<D><<<unsigned(blocks), kJoinThreads, p.mass ? size_t(p.heads_q) * 4 : 0, st>>>(p);
@@ -1238,6 +1277,14 @@ extern "C" ashkv_status_t ashkv_decode_attention(
     p.int_pages |= p.store[t].format == ASHKV_PAGE_INT8 || p.store[t].format == ASHKV_PAGE_INT4;
   }
   cudaStream_t st = as_stream(stream);
-  if (worker_queries(p.group) == 8) return kv->head_dim == 64 ? launch_decode<64, 1>(p, st) : launch_decode<128, 1>(p, st);
-  return kv->head_dim == 64 ? launch_decode<64, 2>(p, st) : launch_decode<128, 2>(p, st);
+  const auto launch = [&](auto dim, auto tiles) {
+    constexpr int D = decltype(dim)::value, NT = decltype(tiles)::value;
+    return p.T == 16 ? launch_decode<D, NT, true>(p, st) : launch_decode<D, NT, false>(p, st);
+  };
+  using std::integral_constant;
+  if (worker_queries(p.group) == 8)
+    return kv->head_dim == 64 ? launch(integral_constant<int, 64>{}, integral_constant<int, 1>{})
+                              : launch(integral_constant<int, 128>{}, integral_constant<int, 1>{});
+  return kv->head_dim == 64 ? launch(integral_constant<int, 64>{}, integral_constant<int, 2>{})
+                            : launch(integral_constant<int, 128>{}, integral_constant<int, 2>{});
 }
