@@ -11,7 +11,6 @@
 // weighs the partials of each sequence by 2^(their log2-sum - the total).
 #include <algorithm>
 #include <cstdio>
-#include <type_traits>
 
 #include "common.cuh"
 #include "nbit_group.cuh"
@@ -20,8 +19,10 @@
 namespace ashkv {
 namespace {
 
-constexpr int kWarpsA = 4;          // warps of a CTA, each a worker of its own
+constexpr int kWarpsA = 4;          // worker warps of a CTA; a fifth warp feeds them
+constexpr int kThreadsA = (kWarpsA + 1) * 32;
 constexpr int kWorkersPerSm = 12;   // resident worker warps per SM
+constexpr uint32_t kPolls = 1u << 24;  // bounded mbarrier waits
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kJoinThreads = 128;
@@ -166,10 +167,6 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
-
 // Codes as exact fp16 pairs, by putting them into the low bits of 1024.0 (0x6400)
 // and subtracting what that adds.
 // Bytes (0, 1) or (2, 3) of an int8 word with its sign bits flipped (code + 128):
@@ -205,43 +202,26 @@ __device__ __forceinline__ uint32_t v_off(uint32_t r, uint32_t c) {
 }
 
 // ---------------------------------------------------------------- the pages of a worker
-constexpr int kRing = 3;  // units in shared memory per warp: one in use, two on their way
+constexpr int kRing = 3;  // units in shared memory per worker: one in use, two on their way
 
 // A unit is 16 tokens of a page for one key head: the K or the V rows of a BF16
 // page (16 x D bf16), or the codes of both of a compressed page (K first), and
 // behind them the scales of those rows: INT8: fp16, K then V, the V rows from the
 // last 4-byte boundary on; INT4: a word per row, K then V (D = 64: the row's scale
-// for this head is the word's upper half for an odd head).  A page to leave out
-// takes a unit that nothing is copied to.
-//
-// The list entries of a segment are looked up 16 at a time, a lane each, in four
-// steps a few pages apart (position, page id, page-table columns, layer address),
-// so that no step waits for the loads of the one before it; the result, where to
-// copy from, goes to a ring of 32 references in shared memory that both ends of
-// the unit ring read.
-constexpr int kRefs = 32, kLook = 16;
-constexpr int kRefBytes = kRefs * 24;  // {k, meta, pos} of every entry, then v
-// k: BF16: K channel 0 of the head at the page's first token; codes: the same; dithered: the slot.
-// v: BF16: the same of V; INT8, INT4: where the slot's scales start.
-// meta: format | tokens in use << 8 (none: a page to leave out); pos: position in the sequence.
-struct PageRef {
-  const uint8_t* k;
-  uint32_t meta;
-  int32_t pos;
-  __device__ __forceinline__ uint32_t format() const { return meta & 0xFFu; }
-  __device__ __forceinline__ int tokens() const { return int(meta >> 8); }
+// for this head is the word's upper half for an odd head).  A dithered page, and
+// one to leave out, takes a unit that nothing is copied to.  A header says what
+// the unit is.
+template <int D>
+struct UnitLayout {
+  static constexpr int kScales = 16 * D * 2, kHeader = kScales + 128, kBytes = kHeader + 16;
 };
-
-__device__ __forceinline__ const uint8_t* address(uint32_t lo, uint32_t hi) {
-  return reinterpret_cast<const uint8_t*>(uint64_t(lo) | uint64_t(hi) << 32);
-}
-
-// A place in the units of a segment.
-struct Cursor {
-  int i;         // list entry
-  int t0;        // first token in its page (pages of at most 16 tokens: 0)
-  bool second;   // BF16: the V rows
-  uint32_t unit; // shared address of the unit
+struct Header {
+  const uint8_t* slot;  // dithered pages
+  uint32_t meta;        // format | rows in use << 8 | flags | first token / 16 << 20
+  int32_t pos;          // page position in the sequence
+  static constexpr uint32_t kIsV = 1u << 16, kPageEnd = 1u << 17, kSegmentEnd = 1u << 18;
+  __device__ __forceinline__ uint32_t format() const { return meta & 0xFFu; }
+  __device__ __forceinline__ int rows() const { return int(meta >> 8) & 0xFF; }
 };
 
 // Decodes the K or V rows of a dithered page into a BF16 unit.
@@ -287,134 +267,144 @@ __device__ __noinline__ void stage_nbit(const uint8_t* slot, int T, int row_len,
     }
   }
 
-// T16: pages have 16 tokens (the library's default), one tile each.
-template <int D, bool T16>
-struct Feeder {
-  static constexpr int kScales = 16 * D * 2;           // byte offset of the scales
-  static constexpr int kUnitBytes = kScales + 128;
+// Where a worker's pages begin: sequence b, of whose list `before` entries of the row lie ahead.
+struct Share {
+  int b, before, pos, end;  // row positions [pos, end)
+};
+
+// The producer warp of a CTA sends the units of its four workers, eight lanes for
+// each, so that the instructions that find pages and copy rows serve four
+// workers at once (they mostly hold four heads of the same pages).  List entries
+// are looked up eight at a time, a lane each, in four steps two pages apart
+// (position, page id, page-table columns, layer address), so that no step waits
+// for the loads of the one before it.
+template <int D>
+struct Producer {
+  using Layout = UnitLayout<D>;
+  static constexpr int kLook = 8;
   const AttnParams& p;
-  int b, hk, i1;          // sequence, key head, end of the segment's entries
+  const int hk, sub;      // this lane's worker's key head; lane within the worker's eight
+  int b, i, i0, i1;       // its sequence, next list entry, the segment's entries
   int64_t tokens;
-  uint32_t ring, refs;    // shared addresses of the units and of the references
-  Cursor at;              // the next unit to send
-  PageRef page;           // its page
-  const uint8_t* page_v;
-  int look, step;         // first entry being looked up, next step
-  int pos, id, tier, layer, start_or_slot;
-  uint32_t lane16, lane8, lane4;  // byte offset of this lane's first chunk in rows of 16-, 8- and 4-bit elements
+  int row_pos, row_end, before;
+  bool active;
+  int t0;                 // first token of the next unit in its page
+  bool second;            // BF16: the V rows are next
+  uint32_t unit, slot, phase;
+  const uint32_t ring, bars;  // shared addresses: the units; full[kRing], empty[kRing]
+  // entry batch0 + sub of the segment, and the one being looked up for the next batch
+  const uint8_t *k, *v;
+  uint32_t meta;
+  int pos, batch0;
+  int n_pos, n_id, n_tier, n_layer, n_where;
+  uint64_t n_k, n_v;
 
-  __device__ __forceinline__ Feeder(const AttnParams& p_, int hk_, uint32_t ring_)
-      : p(p_), hk(hk_), ring(ring_), refs(ring_ + kRing * kUnitBytes) {
-    const uint32_t lane = threadIdx.x & 31u, row = uint32_t(p.row_len);
-    lane16 = lane / (D / 8) * uint32_t(p.row_stride) * 2u + lane % (D / 8) * 16u;
-    lane8 = lane / (D / 16) * row + lane % (D / 16) * 16u;
-    lane4 = lane / (D / 32) * (row / 2) + lane % (D / 32) * 16u;
+  __device__ __forceinline__ Producer(const AttnParams& p_, int hk_, const Share& s, uint32_t ring_, uint32_t bars_)
+      : p(p_), hk(hk_), sub(int(threadIdx.x & 7u)), unit(ring_), slot(0), phase(0), ring(ring_), bars(bars_) {
+    b = s.b; before = s.before; row_pos = s.pos; row_end = s.end;
+    active = row_pos < row_end;
   }
-  __device__ __forceinline__ int page_tokens() const { return T16 ? 16 : p.T; }
 
-  __device__ __forceinline__ void start(int b_, int i0, int i1_) {
-    b = b_; i1 = i1_; tokens = seq_tokens(p, b);
-    at = Cursor{i0, 0, false, ring};
-    look = i0;
-    for (step = 0; step < 4; ++step) look_up();
-    look = i0 + kLook;
-    step = 0;
+  // A segment is the part of the worker's pages that lies in one sequence.
+  __device__ void open_segment() {
+    int n = 0;
+    for (; active; ++b) {
+      n = list_len(p, b, hk);
+      if (before + n > row_pos) break;
+      before += n;
+    }
+    if (active) {
+      i0 = i = row_pos - before;
+      i1 = min(n, row_end - before);
+      tokens = seq_tokens(p, b);
+    } else {
+      i0 = i = i1 = 0;
+      tokens = 0;
+    }
+    t0 = 0;
+    second = false;
+    batch0 = i0 - kLook;
+    for (int step = 0; step < 4; ++step) look_up(step);
+    take_batch();
   }
-  // One step of the look-up of entries look .. look + 15 (lane l: look + l).
-  __device__ __forceinline__ void look_up() {
-    const int lane = threadIdx.x & 31, i = look + lane;
-    const bool mine = lane < kLook && i < i1;
+  // Steps of the look-up of entry batch0 + kLook + sub.
+  __device__ __forceinline__ void look_up(int step) {
+    const int e = batch0 + kLook + sub;
+    const bool mine = e < i1;
     if (step == 0) {
-      pos = mine && p.selected ? p.selected[(int64_t(b) * p.heads_kv + hk) * p.max_selected + i] : i;
+      n_pos = mine && p.selected ? p.selected[(int64_t(b) * p.heads_kv + hk) * p.max_selected + e] : e;
     } else if (step == 1) {
-      const bool ok = mine && pos >= 0 && int64_t(pos) * page_tokens() < tokens;
-      id = ok ? p.page_ids[int64_t(b) * p.page_ids_stride + pos] : -1;
-      if (!ok) pos = 0;
+      const bool ok = mine && n_pos >= 0 && int64_t(n_pos) * p.T < tokens;
+      n_id = ok ? p.page_ids[int64_t(b) * p.page_ids_stride + n_pos] : -1;
+      if (!ok) n_pos = 0;
     } else if (step == 2) {
-      const bool ok = id >= 0 && id < p.n_pages;
-      tier = ok ? p.tier[id] : -1;
-      layer = ok ? p.layer_id[id] : 0;
-      start_or_slot = ok ? p.token_start[id] : 0;
-      const int slot = ok ? p.page_slot[id] : 0;
-      if (tier != 0) start_or_slot = slot;
-    } else if (mine) {
-      const uint8_t *k = nullptr, *v = nullptr;
-      uint32_t meta = 0;
-      bool ok = tier >= 0 && tier < kTiers;
-      if (ok && tier == 0) {
-        ok = layer >= 0 && layer < p.n_layers && start_or_slot >= 0 &&
-             int64_t(start_or_slot) + page_tokens() <= p.pool_tokens;
-        if (ok) {
-          const int64_t off = (int64_t(start_or_slot) * p.row_stride + hk * D) * 2;
-          k = reinterpret_cast<const uint8_t*>(p.layer_k[layer]) + off;
-          v = reinterpret_cast<const uint8_t*>(p.layer_v[layer]) + off;
-          meta = ASHKV_PAGE_BF16;
-        }
-      } else if (ok) {
-        const Store& st = p.store[tier];
-        ok = st.format != ASHKV_PAGE_NONE && start_or_slot >= 0 && start_or_slot < st.n_slots;
-        if (ok) {
-          v = k = st.data + int64_t(start_or_slot) * st.slot_bytes;
-          meta = uint32_t(st.format);
-          if (meta == ASHKV_PAGE_INT8) k += int8_codes_offset(page_tokens()) + hk * D;
-          if (meta == ASHKV_PAGE_FP8) k += hk * D;
-          if (meta == ASHKV_PAGE_INT4) {
-            k += page_tokens() * p.row_len / 16 + hk * (D / 2);  // past E / 32 bytes of scales
-            v += hk * D / 32 & ~3;
-          }
-        }
-      }
+      const bool ok = n_id >= 0 && n_id < p.n_pages;
+      n_tier = ok ? p.tier[n_id] : -1;
+      n_layer = ok ? p.layer_id[n_id] : 0;
+      n_where = ok ? p.token_start[n_id] : 0;
+      const int s = ok ? p.page_slot[n_id] : 0;
+      if (n_tier != 0) n_where = s;
+    } else {
+      const bool ok = n_tier == 0 && n_layer >= 0 && n_layer < p.n_layers;
+      n_k = ok ? p.layer_k[n_layer] : 0;
+      n_v = ok ? p.layer_v[n_layer] : 0;
+    }
+  }
+  // Makes the entry looked up this lane's entry of the current batch (the last step).
+  __device__ __forceinline__ void take_batch() {
+    batch0 += kLook;
+    k = v = nullptr;
+    meta = 0;
+    pos = n_pos;
+    if (batch0 + sub >= i1) return;
+    bool ok = n_tier >= 0 && n_tier < kTiers && n_where >= 0;
+    if (ok && n_tier == 0) {
+      ok = n_layer >= 0 && n_layer < p.n_layers && int64_t(n_where) + p.T <= p.pool_tokens;
       if (ok) {
-        meta |= uint32_t(min(int64_t(page_tokens()), tokens - int64_t(pos) * page_tokens())) << 8;
-      } else {
-        flag(p.status, ASHKV_FLAG_INDEX_RANGE);
-        if (p.mass)  // a page that is left out draws nothing
-          for (int g = 0; g < p.group; ++g)
-            p.page_lse2[(int64_t(b) * p.max_pages + pos) * p.heads_q + hk * p.group + g] = -INFINITY;
+        const int64_t off = (int64_t(n_where) * p.row_stride + hk * D) * 2;
+        k = reinterpret_cast<const uint8_t*>(n_k) + off;
+        v = reinterpret_cast<const uint8_t*>(n_v) + off;
+        meta = ASHKV_PAGE_BF16;
       }
-      const uint32_t e = uint32_t(i) & (kRefs - 1);
-      const uint64_t ka = reinterpret_cast<uint64_t>(k), va = reinterpret_cast<uint64_t>(v);
-      sts128(refs + e * 16, make_uint4(uint32_t(ka), uint32_t(ka >> 32), meta, uint32_t(pos)));
-      asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(refs + kRefs * 16 + e * 8), "r"(uint32_t(va)), "r"(uint32_t(va >> 32)) : "memory");
+    } else if (ok) {
+      const Store& st = p.store[n_tier];
+      ok = st.format != ASHKV_PAGE_NONE && n_where < st.n_slots;
+      if (ok) {
+        v = k = st.data + int64_t(n_where) * st.slot_bytes;
+        meta = uint32_t(st.format);
+        if (meta == ASHKV_PAGE_INT8) k += int8_codes_offset(p.T) + hk * D;
+        if (meta == ASHKV_PAGE_FP8) k += hk * D;
+        if (meta == ASHKV_PAGE_INT4) {
+          k += p.T * p.row_len / 16 + hk * (D / 2);  // past E / 32 bytes of scales
+          v += hk * D / 32 & ~3;
+        }
+      }
     }
-    if (step == 3) __syncwarp();
-  }
-  __device__ __forceinline__ PageRef ref(int i) const {
-    const uint4 x = lds128(refs + (uint32_t(i) & (kRefs - 1)) * 16);
-    return PageRef{address(x.x, x.y), x.z, int32_t(x.w)};
-  }
-
-  // Moves a cursor behind its unit; true where that ends the page.
-  static __device__ __forceinline__ bool advance(Cursor& c, const PageRef& page, uint32_t ring) {
-    c.unit = c.unit == ring + (kRing - 1) * kUnitBytes ? ring : c.unit + kUnitBytes;
-    const bool two = page.format() == ASHKV_PAGE_BF16 || page.format() >= ASHKV_PAGE_NBIT4;
-    if (two && !c.second && page.tokens()) {
-      c.second = true;
-      return false;
+    if (ok) {
+      meta |= uint32_t(min(int64_t(p.T), tokens - int64_t(pos) * p.T)) << 8;
+    } else {
+      flag(p.status, ASHKV_FLAG_INDEX_RANGE);
+      if (p.mass)  // a page that is left out draws nothing
+        for (int g = 0; g < p.group; ++g)
+          p.page_lse2[(int64_t(b) * p.max_pages + pos) * p.heads_q + hk * p.group + g] = -INFINITY;
     }
-    c.second = false;
-    if constexpr (!T16) {
-      c.t0 += 16;
-      if (c.t0 < page.tokens()) return false;
-      c.t0 = 0;
-    }
-    ++c.i;
-    return true;
   }
 
-  // 16 rows of RB bytes, `step` bytes apart, into a tile, src being this lane's first chunk; rows
-  // behind `rows` become zeros.
+  // 16 rows of RB bytes, `step` bytes apart from src on, into a tile by the worker's eight lanes;
+  // rows behind `rows` become zeros.
   template <int RB, bool V>
-  __device__ __forceinline__ void copy_rows(const uint8_t* src, uint32_t step_bytes, int rows, uint32_t tile) const {
-    const uint32_t lane = threadIdx.x & 31u;
-    constexpr uint32_t CPR = RB / 16, RPI = 32 / CPR;  // chunks of a row, rows of one instruction
-    const uint32_t r0 = lane / CPR, col = lane % CPR;
-    step_bytes *= RPI;
+  __device__ __forceinline__ void copy_rows(const uint8_t* src, uint32_t step, int rows, uint32_t tile) const {
+    constexpr uint32_t CPR = RB / 16;                     // chunks of a row
+    constexpr uint32_t LPR = CPR < 8 ? CPR : 8, RPI = 8 / LPR;  // lanes of a row, rows of one instruction
+    const uint32_t r0 = uint32_t(sub) / LPR, c0 = uint32_t(sub) % LPR;
+    src += r0 * step + c0 * 16u;
     if (rows >= 16) {
 #pragma unroll
       for (uint32_t j = 0; j < 16 / RPI; ++j) {
-        cp_async16(tile + (V ? v_off<RB>(r0 + RPI * j, col) : k_off<RB>(r0 + RPI * j, col)), src);
-        src += step_bytes;
+#pragma unroll
+        for (uint32_t c = 0; c < CPR; c += LPR)
+          cp_async16(tile + (V ? v_off<RB>(r0 + RPI * j, c0 + c) : k_off<RB>(r0 + RPI * j, c0 + c)), src + c * 16);
+        src += RPI * step;
       }
       return;
     }
@@ -422,57 +412,113 @@ struct Feeder {
     for (uint32_t j = 0; j < 16 / RPI; ++j) {
       const uint32_t r = r0 + RPI * j;
       const bool real = r < uint32_t(rows);
-      cp_async16_or_zero(tile + (V ? v_off<RB>(r, col) : k_off<RB>(r, col)), real ? src + uint64_t(step_bytes) * j : page.k, real);
+#pragma unroll
+      for (uint32_t c = 0; c < CPR; c += LPR)
+        cp_async16_or_zero(tile + (V ? v_off<RB>(r, c0 + c) : k_off<RB>(r, c0 + c)),
+                           real ? src + uint64_t(RPI * step) * j + c * 16 : k, real);
     }
   }
 
-  // Sends the next unit on its way (always one cp.async group).
-  __device__ __forceinline__ void issue() {
-    if (at.i < i1) {
-      if (!at.second && (T16 || at.t0 == 0)) {  // the next page
-        if (!((at.i - look) & 3)) {  // every four pages a step for the next 16 entries
-          if (at.i == look) {        // their first is due: the look-up is done
-            look += kLook;
-            step = 0;
+  __device__ void run() {
+    open_segment();
+    const uint32_t group = threadIdx.x & 24u;  // first lane of the worker's eight
+    for (uint32_t sent = 0; __any_sync(0xFFFFFFFFu, active); ++sent) {
+      const bool page_start = active && !second && t0 == 0;
+      // two pages apart, a step for the next eight entries
+      if (page_start && !((i - batch0) & 1)) {
+        if (i - batch0 == kLook) take_batch();
+        look_up((i - batch0) >> 1);
+      }
+      __syncwarp();
+      const int src = int(group) + ((i - batch0) & (kLook - 1));
+      const uint8_t* pk = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(k), src));
+      const uint8_t* pv = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(v), src));
+      const uint32_t pm = __shfl_sync(0xFFFFFFFFu, meta, src);
+      const int pp = __shfl_sync(0xFFFFFFFFu, pos, src);
+      bool ok = true;
+      if (active && sent >= kRing) ok = wait_bar(bars + (kRing + slot) * 8, phase ^ 1u);
+      if (!__all_sync(0xFFFFFFFFu, ok)) {
+        flag(p.status, ASHKV_FLAG_TIMEOUT);
+        break;
+      }
+      if (active) {
+        const uint32_t format = pm & 0xFFu, T = uint32_t(p.T), row = uint32_t(p.row_len);
+        const int page_tokens = int(pm >> 8), left = page_tokens - t0;
+        uint32_t h = format | uint32_t(max(0, min(left, 16))) << 8 | uint32_t(t0) << 16;
+        bool done = true;  // with these tokens
+        if (left <= 0) {
+        } else if (format == ASHKV_PAGE_BF16) {
+          const uint32_t step = uint32_t(p.row_stride) * 2u;
+          if (second) copy_rows<D * 2, true>(pv + uint32_t(t0) * step, step, left, unit);
+          else copy_rows<D * 2, false>(pk + uint32_t(t0) * step, step, left, unit);
+          if (second) h |= Header::kIsV;
+          done = second;
+          second = !second;
+        } else if (format == ASHKV_PAGE_INT4) {
+          const uint8_t* codes = pk + uint32_t(t0) * (row / 2);
+          copy_rows<D / 2, false>(codes, row / 2, left, unit);
+          copy_rows<D / 2, true>(codes + T * (row / 2), row / 2, left, unit + 8 * D);
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t r = sub + 8u * (j & 1u);
+            cp_async4(unit + Layout::kScales + (16u * (j >> 1) + r) * 4u,
+                      pv + (min(uint32_t(t0) + r, T - 1u) + (j >> 1) * T) * (row / 32u));
           }
-          look_up();
-          ++step;
+        } else if (format < ASHKV_PAGE_NBIT4) {
+          const uint8_t* codes = pk + uint32_t(t0) * row;
+          copy_rows<D, false>(codes, row, left, unit);
+          copy_rows<D, true>(codes + T * row, row, left, unit + 16 * D);
+          if (format == ASHKV_PAGE_INT8) {
+            // 8 words of K scales, 9 of V scales (all inside the slot: codes follow them)
+            const uint8_t* vs = pv + ((T + uint32_t(t0)) * 2u & ~3u);
+            cp_async4(unit + Layout::kScales + sub * 4u, pv + t0 * 2 + sub * 4);
+            cp_async4(unit + Layout::kScales + 32u + sub * 4u, vs + sub * 4);
+            if (sub == 0) cp_async4(unit + Layout::kScales + 64u, vs + 32);
+          }
         }
-        page = ref(at.i);
-        const uint2 x = lds64(refs + kRefs * 16 + (uint32_t(at.i) & (kRefs - 1)) * 8);
-        page_v = address(x.x, x.y);
-      }
-      const uint32_t lane = threadIdx.x & 31u, format = page.format(), row = uint32_t(p.row_len), dst = at.unit;
-      const uint32_t t0 = T16 ? 0u : uint32_t(at.t0), T = uint32_t(page_tokens());
-      const int left = page.tokens() - int(t0);
-      if (left <= 0) {
-      } else if (format == ASHKV_PAGE_BF16) {
-        const uint32_t step_bytes = uint32_t(p.row_stride) * 2u;
-        if (at.second) copy_rows<D * 2, true>(page_v + (lane16 + t0 * step_bytes), step_bytes, left, dst);
-        else copy_rows<D * 2, false>(page.k + (lane16 + t0 * step_bytes), step_bytes, left, dst);
-      } else if (format == ASHKV_PAGE_INT4) {
-        const uint8_t* codes = page.k + (lane4 + t0 * (row / 2));
-        copy_rows<D / 2, false>(codes, row / 2, left, dst);
-        copy_rows<D / 2, true>(codes + T * (row / 2), row / 2, left, dst + 8 * D);
-        const uint32_t sr = T16 ? lane : min(t0 + (lane & 15u), T - 1u) + (lane & 16u ? T : 0u);
-        cp_async4(dst + kScales + lane * 4u, page_v + sr * (row / 32u));
-      } else if (format < ASHKV_PAGE_NBIT4) {
-        const uint8_t* codes = page.k + (lane8 + t0 * row);
-        copy_rows<D, false>(codes, row, left, dst);
-        copy_rows<D, true>(codes + T * row, row, left, dst + 16 * D);
-        if (format == ASHKV_PAGE_INT8 && lane < 17u) {
-          // 8 words of K scales, 9 of V scales (all inside the slot: codes follow them)
-          const uint32_t o = lane < 8u ? t0 * 2u + lane * 4u : ((T + t0) * 2u & ~3u) + (lane - 8u) * 4u;
-          cp_async4(dst + kScales + lane * 4u, page_v + o);
+        if (done) {
+          t0 += 16;
+          if (left <= 16) {
+            h |= Header::kPageEnd;
+            t0 = 0;
+            if (++i == i1) h |= Header::kSegmentEnd;
+          }
         }
-      } else if (format == ASHKV_PAGE_NBIT4) {
-        stage_nbit<D, 4>(page.k, p.T, p.row_len, p.outlier_cap, hk, at.second, int(t0), min(left, 16), dst);
-      } else {
-        stage_nbit<D, 2>(page.k, p.T, p.row_len, p.outlier_cap, hk, at.second, int(t0), min(left, 16), dst);
+        const uint32_t full = bars + slot * 8;
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(full) : "memory");
+        if (sub == 0) {
+          const uint64_t a = reinterpret_cast<uint64_t>(pk);
+          sts128(unit + Layout::kHeader, make_uint4(uint32_t(a), uint32_t(a >> 32), h, uint32_t(pp)));
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(full) : "memory");
+        }
+        if (++slot == kRing) {
+          slot = 0;
+          phase ^= 1u;
+          unit = ring;
+        } else {
+          unit += Layout::kBytes;
+        }
       }
-      advance(at, page, ring);
+      const bool ended = active && i == i1;
+      if (__any_sync(0xFFFFFFFFu, ended)) {
+        if (ended) {
+          row_pos = before + i1;
+          active = row_pos < row_end;
+          open_segment();
+        }
+        __syncwarp();
+      }
     }
-    cp_async_commit();
+    cp_async_wait_all();
+  }
+  static __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
+    for (uint32_t n = 0; n < kPolls; ++n) {
+      uint32_t done;
+      asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                   : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+      if (done) return true;
+    }
+    return false;
   }
 };
 
@@ -1012,65 +1058,115 @@ struct Worker {
   }
 };
 
-template <int D, int NT, bool T16>
-__global__ void __launch_bounds__(kWarpsA * 32, NT == 1 ? 3 : 2) decode_partials_kernel(const __grid_constant__ AttnParams p) {
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_kernel(const __grid_constant__ AttnParams p) {
+  using Layout = UnitLayout<D>;
   extern __shared__ __align__(128) uint8_t smem[];
-  const int warp = threadIdx.x >> 5;
-  const int w = int(blockIdx.x) * kWarpsA + warp;
+  __shared__ Share s_share[kWarpsA];
+  __shared__ __align__(8) uint64_t s_bars[kWarpsA][2 * kRing];  // full, empty
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cells = p.heads_kv * p.q_chunks;
+  // the worker of this warp, or of this lane of the producer
+  const int mine = warp < kWarpsA ? warp : lane >> 3;
+  const int w = int(blockIdx.x) * kWarpsA + mine;
   const int range = w / cells, cell = w % cells;
-  if (range >= p.ranges) return;
   const int hk = cell % p.heads_kv, q0 = (cell / p.heads_kv) * (8 * NT);
-  const int nq = min(8 * NT, p.group - q0), hq0 = hk * p.group + q0;
-  const int total = lists_before(p, p.n_seqs, hk), len = range_len(p, total);
-  int64_t pos = int64_t(range) * len;
-  const int64_t end = min(pos + len, int64_t(total));
-  if (pos >= end) return;
-  int b = 0, before = 0;
-  for (;; ++b) {  // the sequence that the range starts in
-    const int n = list_len(p, b, hk);
-    if (before + n > pos) break;
-    before += n;
+  const uint32_t ring = smem_u32(smem) + uint32_t(mine * p.warp_smem), bars = smem_u32(s_bars[mine]);
+  if (warp < kWarpsA) {
+    Share sh{0, 0, 0, 0};
+    if (range < p.ranges) {
+      const int total = lists_before(p, p.n_seqs, hk), len = range_len(p, total);
+      const int64_t at = int64_t(range) * len;
+      sh.pos = int(min(at, int64_t(total)));
+      sh.end = int(min(at + len, int64_t(total)));
+      if (sh.pos < sh.end) {  // the sequence that the range starts in
+        for (int b0 = 0;; b0 += 32) {
+          const int n = b0 + lane < p.n_seqs ? list_len(p, b0 + lane, hk) : 0;
+          int upto = n;
+#pragma unroll
+          for (int off = 1; off < 32; off <<= 1) {
+            const int x = __shfl_up_sync(0xFFFFFFFFu, upto, off);
+            if (lane >= off) upto += x;
+          }
+          const unsigned past = __ballot_sync(0xFFFFFFFFu, sh.before + upto > sh.pos);
+          if (past || b0 + 32 >= p.n_seqs) {
+            const int l = past ? __ffs(past) - 1 : 31;
+            sh.b = b0 + l;
+            sh.before += __shfl_sync(0xFFFFFFFFu, upto - n, l);
+            break;
+          }
+          sh.before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+        }
+      }
+    }
+    if (lane == 0) {
+      s_share[warp] = sh;
+      for (int k = 0; k < kRing; ++k) {
+        mbar_init(&s_bars[warp][k], 9);          // eight lanes' copies and the header
+        mbar_init(&s_bars[warp][kRing + k], 1);
+      }
+      mbar_init_fence();
+    }
   }
-  const uint32_t ring = smem_u32(smem) + uint32_t(warp * p.warp_smem);
-  Feeder<D, T16> feed(p, hk, ring);
-  Worker<D, NT> work(p, ring + kRing * Feeder<D, T16>::kUnitBytes + kRefBytes, hk);
+  __syncthreads();
+  if (warp == kWarpsA) {
+    Producer<D>(p, hk, s_share[mine], ring, bars).run();
+    return;
+  }
+  Worker<D, NT> work(p, ring + kRing * Layout::kBytes, hk);
+  const int nq = min(8 * NT, p.group - q0), hq0 = hk * p.group + q0;
+  int b = s_share[warp].b, before = s_share[warp].before, pos = s_share[warp].pos;
+  const int end = s_share[warp].end;
+  uint32_t unit = ring, slot = 0, phase = 0;
   for (; pos < end; ++b) {
     const int n = list_len(p, b, hk);
     if (n == 0) continue;
-    const int i0 = int(pos - before), i1 = int(min(int64_t(n), end - before));
-    feed.start(b, i0, i1);
     work.start(b, hq0, nq);
     float s[NT][4];  // weights of a BF16 tile between its K and its V unit
-    Cursor at{i0, 0, false, ring};
-    for (int ahead = 0; at.i < i1; ++ahead) {
-      feed.issue();
-      if (ahead < kRing - 1) continue;
-      const PageRef page = feed.ref(at.i);
-      const int left = page.tokens() - at.t0;
-      cp_async_wait<kRing - 1>();
-      __syncwarp();
-      if (left <= 0) {
-      } else if (page.format() == ASHKV_PAGE_INT8) {
-        work.template tile8<true>(at.unit, left);
-      } else if (page.format() == ASHKV_PAGE_FP8) {
-        work.template tile8<false>(at.unit, left);
-      } else if (page.format() == ASHKV_PAGE_INT4) {
-        work.tile4(at.unit, left);
-      } else if (at.second) {
-        work.bf16_values(at.unit, s);
-      } else {
-        work.bf16_scores(at.unit, left, s);
+    for (bool last = false; !last;) {
+      if (!Producer<D>::wait_bar(bars + slot * 8, phase)) {
+        flag(p.status, ASHKV_FLAG_TIMEOUT);
+        return;
       }
-      const bool done = Feeder<D, T16>::advance(at, page, ring);
-      if (p.mass && done && left > 0) work.page_sum(b, page.pos, hq0, nq);
+      const uint4 h4 = lds128(unit + Layout::kHeader);
+      const Header h{reinterpret_cast<const uint8_t*>(uint64_t(h4.x) | uint64_t(h4.y) << 32), h4.z, int32_t(h4.w)};
+      if (h.rows() == 0) {
+      } else if (h.format() == ASHKV_PAGE_INT8) {
+        work.template tile8<true>(unit, h.rows());
+      } else if (h.format() == ASHKV_PAGE_FP8) {
+        work.template tile8<false>(unit, h.rows());
+      } else if (h.format() == ASHKV_PAGE_INT4) {
+        work.tile4(unit, h.rows());
+      } else if (h.format() >= ASHKV_PAGE_NBIT4) {
+        const int t0 = int(h.meta >> 20) * 16;
+        for (int half = 0; half < 2; ++half) {
+          if (h.format() == ASHKV_PAGE_NBIT4) stage_nbit<D, 4>(h.slot, p.T, p.row_len, p.outlier_cap, hk, half, t0, h.rows(), unit);
+          else stage_nbit<D, 2>(h.slot, p.T, p.row_len, p.outlier_cap, hk, half, t0, h.rows(), unit);
+          __syncwarp();
+          if (half) work.bf16_values(unit, s);
+          else work.bf16_scores(unit, h.rows(), s);
+          __syncwarp();
+        }
+      } else if (h.meta & Header::kIsV) {
+        work.bf16_values(unit, s);
+      } else {
+        work.bf16_scores(unit, h.rows(), s);
+      }
+      if (p.mass && (h.meta & Header::kPageEnd) && h.rows()) work.page_sum(b, h.pos, hq0, nq);
+      last = h.meta & Header::kSegmentEnd;
       __syncwarp();  // every lane has read the unit
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bars + (kRing + slot) * 8) : "memory");
+      if (++slot == kRing) {
+        slot = 0;
+        phase ^= 1u;
+        unit = ring;
+      } else {
+        unit += Layout::kBytes;
+      }
     }
-    cp_async_wait<0>();
-    __syncwarp();
     work.finish(int64_t(range + b) * p.heads_q + hq0, nq);
-    pos = before + i1;
     before += n;
+    pos = before;
   }
 }
 
@@ -1207,17 +1303,17 @@ ashkv_status_t refuse(const char* what, const char* why) {
   return ASHKV_BAD_ARGUMENT;
 }
 
-template <int D, int NT, bool T16>
+template <int D, int NT>
 ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
   const int64_t workers = int64_t(p.ranges) * p.heads_kv * p.q_chunks;
-  p.warp_smem = kRing * Feeder<D, T16>::kUnitBytes + kRefBytes + NT * 8 * D * (2 + (p.fp8_pages ? 2 : 0) + (p.int_pages ? 3 : 0));
+  p.warp_smem = kRing * UnitLayout<D>::kBytes + NT * 8 * D * (2 + (p.fp8_pages ? 2 : 0) + (p.int_pages ? 3 : 0));
   const int smem = kWarpsA * p.warp_smem;
-  const cudaError_t e = cudaFuncSetAttribute(decode_partials_kernel<D, NT, T16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = cudaFuncSetAttribute(decode_partials_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     set_error("ashkv_decode_attention (shared memory attribute)", e);
     return ASHKV_LAUNCH_ERROR;
   }
-  decode_partials_kernel<D, NT, T16><<<unsigned((workers + kWarpsA - 1) / kWarpsA), kWarpsA * 32, smem, st>>>(p);
+  decode_partials_kernel<D, NT><<<unsigned((workers + kWarpsA - 1) / kWarpsA), kThreadsA, smem, st>>>(p);
   int64_t blocks = int64_t(p.n_seqs) * p.heads_q;
   if (p.mass) blocks += int64_t(p.n_seqs) * ((p.max_pages + kJoinThreads - 1) / kJoinThreads);
   decode_join_kernel<D><<<unsigned(blocks), kJoinThreads, p.mass ? size_t(p.heads_q) * 4 : 0, st>>>(p);
@@ -1277,14 +1373,6 @@ extern "C" ashkv_status_t ashkv_decode_attention(
     p.int_pages |= p.store[t].format == ASHKV_PAGE_INT8 || p.store[t].format == ASHKV_PAGE_INT4;
   }
   cudaStream_t st = as_stream(stream);
-  const auto launch = [&](auto dim, auto tiles) {
-    constexpr int D = decltype(dim)::value, NT = decltype(tiles)::value;
-    return p.T == 16 ? launch_decode<D, NT, true>(p, st) : launch_decode<D, NT, false>(p, st);
-  };
-  using std::integral_constant;
-  if (worker_queries(p.group) == 8)
-    return kv->head_dim == 64 ? launch(integral_constant<int, 64>{}, integral_constant<int, 1>{})
-                              : launch(integral_constant<int, 128>{}, integral_constant<int, 1>{});
-  return kv->head_dim == 64 ? launch(integral_constant<int, 64>{}, integral_constant<int, 2>{})
-                            : launch(integral_constant<int, 128>{}, integral_constant<int, 2>{});
+  if (worker_queries(p.group) == 8) return kv->head_dim == 64 ? launch_decode<64, 1>(p, st) : launch_decode<128, 1>(p, st);
+  return kv->head_dim == 64 ? launch_decode<64, 2>(p, st) : launch_decode<128, 2>(p, st);
 }
