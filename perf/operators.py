@@ -257,8 +257,9 @@ def _inputs(case, seed):
 
 def prepare(case, seed):
     s = _inputs(case, seed)
-    if own and case["kind"] != "evict":
-        s["handle"] = _handle(s)
+    if own:
+        s["library"] = _library()
+        s["handle"] = _handle(s) if case["kind"] != "evict" else None
     return s
 
 
@@ -275,7 +276,7 @@ def _library():
 
 def _handle(s):
     """The page table, the pool, the stores and the bounds as a user's program keeps them."""
-    PageBounds = _library().PageBounds
+    PageBounds = s["library"].PageBounds
     from ashkv.runtime.batch import DevicePageTable, KVLayers, TierStore
     case, dev = s["case"], s["q"].device
     f = s["mass"].reshape(-1) if s["case"]["mass"] else s["zeros"].float()
@@ -472,7 +473,7 @@ def run(s):
     case = s["case"]
     if not own:
         return {"decode": _decode, "sparse": _sparse, "bounds": _bounds, "evict": _evict}[case["kind"]](s)
-    A = _library()
+    A = s["library"]
     if case["kind"] == "evict":
         got = A.evict_pages(s["mass"], s["page_ids"], s["lengths"], case["budget"], sink=case["sink"],
                             recent=case["recent"], tokens_per_page=T)
