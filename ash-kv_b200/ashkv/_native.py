@@ -136,6 +136,11 @@ def stream_handle(device: Optional[torch.device] = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(t: torch.Tensor) -> int:
+    """The current stream of ``t``'s device (``stream_handle`` without a Stream object: 0.1 us, not 2)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -577,14 +582,14 @@ def decode_attention(desc: PagedKVDesc, q: torch.Tensor, page_ids: torch.Tensor,
         page_ids.stride(0), page_ids.shape[1], lengths.data_ptr(), _ptr(selected), _ptr(selected_count),
         0 if selected is None else selected.shape[2], scale, _ptr(page_mass),
         0 if page_mass is None else page_mass.stride(0), decay, out.data_ptr(), _ptr(lse), scratch.data_ptr(),
-        _ptr(status), stream_handle(q.device)), "decode_attention")
+        _ptr(status), raw_stream(q)), "decode_attention")
 
 
 def page_bounds(desc: PagedKVDesc, pages: torch.Tensor, count: Optional[torch.Tensor], valid: Optional[torch.Tensor],
                 codes: torch.Tensor, exponents: torch.Tensor, status: Optional[torch.Tensor]) -> None:
     _check_text(lib().ashkv_page_bounds(
         ctypes.addressof(desc), pages.data_ptr(), _ptr(count), pages.numel(), _ptr(valid), codes.data_ptr(),
-        exponents.data_ptr(), _ptr(status), stream_handle(pages.device)), "page_bounds")
+        exponents.data_ptr(), _ptr(status), raw_stream(pages)), "page_bounds")
 
 
 def select_scratch_floats(n_seqs: int, heads_kv: int, max_pages: int) -> int:
@@ -600,7 +605,7 @@ def select_pages(q: torch.Tensor, codes: torch.Tensor, exponents: torch.Tensor, 
         q.data_ptr(), q.stride(0), q.stride(1), n_seqs, heads_q, codes.shape[1], head_dim, codes.data_ptr(),
         exponents.data_ptr(), codes.shape[0], page_ids.data_ptr(), page_ids.stride(0), page_ids.shape[1],
         lengths.data_ptr(), tokens_per_page, budget, sink, recent, selected.data_ptr(), count.data_ptr(),
-        scratch.data_ptr(), _ptr(status), stream_handle(q.device)), "select_pages")
+        scratch.data_ptr(), _ptr(status), raw_stream(q)), "select_pages")
 
 
 def evict_pages(page_mass: torch.Tensor, page_ids: torch.Tensor, lengths: torch.Tensor, tokens_per_page: int,
@@ -610,4 +615,4 @@ def evict_pages(page_mass: torch.Tensor, page_ids: torch.Tensor, lengths: torch.
         page_mass.data_ptr(), page_mass.stride(0), page_ids.data_ptr(), page_ids.stride(0), lengths.data_ptr(),
         page_ids.shape[0], page_ids.shape[1], tokens_per_page, budget, sink, recent, out_ids.data_ptr(),
         out_mass.data_ptr(), out_lengths.data_ptr(), evicted.data_ptr(), evicted_count.data_ptr(),
-        stream_handle(page_ids.device)), "evict_pages")
+        raw_stream(page_ids)), "evict_pages")

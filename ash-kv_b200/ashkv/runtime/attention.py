@@ -38,33 +38,38 @@ from .batch import NUM_TIERS, DevicePageTable, KVLayers, TierStore
 
 def _on(device: torch.device):
     """Make ``device`` current for a call, if it is not already."""
-    same = device.index is None or device.index == torch.cuda.current_device()
-    return nullcontext() if same else torch.cuda.device(device)
+    return _SAME if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
-def _require(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
-    """A CUDA tensor of ``dtype`` and ``shape`` on ``device`` whose last dimension is dense."""
+_SAME = nullcontext()
+
+
+def _refuse(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
+    """Says what keeps ``t`` from being a tensor of ``dtype`` and ``shape`` on ``device``."""
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
-    if shape and shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name} must be dense in its last dimension")
 
 
 def _require_rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
-    """``_require`` for [rows, width] with any row stride that keeps rows apart."""
-    _require(t, name, dtype, shape, device)
-    if shape[0] > 1 and t.stride(0) < shape[1]:
-        raise ValueError(f"{name} rows overlap")
+    """[rows, width], dense in its width, with any row stride that keeps rows apart."""
+    if not (t.is_cuda and t.dtype == dtype and t.shape == shape and t.device == device):
+        _refuse(t, name, dtype, shape, device)
+    if not t.is_contiguous():
+        if shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"{name} must be dense in its last dimension")
+        if shape[0] > 1 and t.stride(0) < shape[1]:
+            raise ValueError(f"{name} rows overlap")
 
 
 def _require_dense(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
-    _require(t, name, dtype, shape, device)
+    if not (t.is_cuda and t.dtype == dtype and t.shape == shape and t.device == device):
+        _refuse(t, name, dtype, shape, device)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
 
@@ -72,9 +77,12 @@ def _require_dense(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple,
 def _require_query(q: torch.Tensor) -> None:
     if q.dim() != 3:
         raise ValueError("q must be [n_seqs, heads_q, head_dim]")
-    _require(q, "q", torch.bfloat16, tuple(q.shape), q.device)
+    if not q.is_cuda or q.dtype != torch.bfloat16:
+        _refuse(q, "q", torch.bfloat16, q.shape, q.device)
     if q.shape[2] not in (64, 128):
         raise ValueError("head_dim must be 64 or 128")
+    if q.stride(2) != 1:
+        raise ValueError("q must be dense in its last dimension")
     if q.shape[1] == 0:
         raise ValueError("q has no heads")
 
@@ -91,6 +99,11 @@ def _row_stride(t: torch.Tensor) -> torch.Tensor:
     return t if t.shape[0] != 1 or t.stride(0) >= t.shape[1] else t.as_strided(t.shape, (max(t.shape[1], 1), 1))
 
 
+_StoreDescs = _native.TierStoreDesc * NUM_TIERS
+_NO_STORES = bytes(_StoreDescs(*(_native.TierStoreDesc(
+    None, 0, 0, _native.PAGE_NONE if t else _native.PAGE_BF16, None, None) for t in range(NUM_TIERS))))
+
+
 def _pages_desc(table: DevicePageTable, kv: KVLayers, stores: Optional[Mapping[int, TierStore]], head_dim: int,
                 tokens_per_page: int, device: torch.device):
     """The ashkv_paged_kv_t of a table, its pool and its stores, and the store array it points to."""
@@ -98,16 +111,14 @@ def _pages_desc(table: DevicePageTable, kv: KVLayers, stores: Optional[Mapping[i
         raise ValueError(f"the pool's rows of {kv.row_len} values are no whole number of heads of {head_dim}")
     n = table.tier.numel()
     _require_dense(table.tier, "table.tier", torch.int8, (n,), device)
-    for name in ("layer", "token_start", "slot"):
-        _require_dense(getattr(table, name), f"table.{name}", torch.int32, (n,), device)
+    _require_dense(table.layer, "table.layer", torch.int32, (n,), device)
+    _require_dense(table.token_start, "table.token_start", torch.int32, (n,), device)
+    _require_dense(table.slot, "table.slot", torch.int32, (n,), device)
     if kv.k[0].device != device:
         raise ValueError(f"the KV pool is on {kv.k[0].device}, expected {device}")
     if tokens_per_page <= 0:
         raise ValueError("tokens_per_page must be positive")
-    descs = (_native.TierStoreDesc * NUM_TIERS)()
-    descs[0] = _native.TierStoreDesc(None, 0, 0, _native.PAGE_BF16, None, None)
-    for t in range(1, NUM_TIERS):
-        descs[t] = _native.TierStoreDesc(None, 0, 0, _native.PAGE_NONE, None, None)
+    descs = _StoreDescs.from_buffer_copy(_NO_STORES)
     cap = 0
     for t, s in (stores or {}).items():
         if not 0 < int(t) < NUM_TIERS:
