@@ -25,7 +25,7 @@ constexpr int kWorkersPerSm = 12;   // resident worker warps per SM
 constexpr uint32_t kPolls = 1u << 24;  // bounded mbarrier waits
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 256;
 
 struct AttnParams {
   // pages
@@ -61,6 +61,8 @@ struct AttnParams {
   float* part_o;      // [ranges + n_seqs][heads_q][D], each divided by its sum
   float* part_lse2;   // [ranges + n_seqs][heads_q]
   float* page_lse2;   // [n_seqs][max_pages][heads_q], with mass only
+  int32_t* first_range;  // [n_seqs][heads_kv]: the ranges that hold a list's first and last entry
+  int32_t* last_range;
   int32_t warp_smem;  // bytes of shared memory of a worker
   int32_t fp8_pages, int_pages;  // whether a store holds FP8, or INT8 or INT4 pages
   uint32_t* status;
@@ -1109,6 +1111,7 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
     }
   }
   __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up from here on
   if (warp == kWarpsA) {
     Producer<D>(p, hk, s_share[mine], ring, bars).run();
     return;
@@ -1165,49 +1168,42 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
       }
     }
     work.finish(int64_t(range + b) * p.heads_q + hq0, nq);
+    if (lane == 0) {
+      if (pos == before) p.first_range[int64_t(b) * p.heads_kv + hk] = range;
+      if (before + n <= end) p.last_range[int64_t(b) * p.heads_kv + hk] = range;
+    }
     before += n;
     pos = before;
   }
 }
 
-// log2-sum over the partials of (sequence b, query head hq): ranges r0 .. r1.
-__device__ __forceinline__ void join_range(const AttnParams& p, int b, int hk, int& r0, int& r1) {
-  const int before = lists_before(p, b, hk), n = list_len(p, b, hk);
-  int total = before + n;
-  const int lane = threadIdx.x & 31;
-  int rest = 0;
-  for (int i = b + 1 + lane; i < p.n_seqs; i += 32) rest += list_len(p, i, hk);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) rest += __shfl_xor_sync(0xFFFFFFFFu, rest, off);
-  total += rest;
-  const int len = range_len(p, total);
-  r0 = before / len;
-  r1 = n == 0 ? r0 - 1 : (before + n - 1) / len;
+// The ranges r0 .. r1 that hold pages of (sequence b, key head hk); none: r1 < r0.
+__device__ __forceinline__ void partials_of(const AttnParams& p, int b, int hk, int& r0, int& r1) {
+  const int64_t at = int64_t(b) * p.heads_kv + hk;
+  const bool any = list_len(p, b, hk) > 0;
+  r0 = min(max(p.first_range[at], 0), p.ranges - 1);
+  r1 = any ? min(max(p.last_range[at], r0), p.ranges - 1) : r0 - 1;
 }
-__device__ __forceinline__ float join_lse2(const AttnParams& p, int b, int hq, int r0, int r1) {  // warp-collective
-  const int lane = threadIdx.x & 31;
-  float m = -INFINITY, l = 0.0f;
-  for (int r = r0 + lane; r <= r1; r += 32) {
-    const float x = p.part_lse2[int64_t(r + b) * p.heads_q + hq];
-    const float mn = x > m || x != x ? x : m, ref = mn == -INFINITY ? 0.0f : mn;
-    l = l * exp2f(m - ref) + exp2f(x - ref);
-    m = mn;
-  }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const float m2 = __shfl_xor_sync(0xFFFFFFFFu, m, off), l2 = __shfl_xor_sync(0xFFFFFFFFu, l, off);
-    const float mn = m2 > m || m2 != m2 ? m2 : m, ref = mn == -INFINITY ? 0.0f : mn;
-    l = l * exp2f(m - ref) + l2 * exp2f(m2 - ref);
-    m = mn;
-  }
-  return (m == -INFINITY ? 0.0f : m) + log2f(l);  // no tokens: log2(0) = -inf
+// (m, l) <- the log2-sum of (m, l) and (m2, l2): m + log2 l; NaN stays.
+__device__ __forceinline__ void merge_lse2(float& m, float& l, float m2, float l2) {
+  const float top = m2 > m || m2 != m2 ? m2 : m, ref = top == -INFINITY ? 0.0f : top;
+  l = l * ex2(m - ref) + l2 * ex2(m2 - ref);
+  m = top;
 }
+__device__ __forceinline__ float lse2_of(float m, float l) { return (m == -INFINITY ? 0.0f : m) + log2f(l); }
 
-// Blocks 0 .. n_seqs * heads_q - 1: one result row each.  With mass, then
-// ceil(max_pages / kJoinThreads) blocks per sequence for its pages' mass.
+// Blocks 0 .. n_seqs * heads_q - 1: a result row each, its partials spread over
+// the warps and added through shared memory.  With mass, then blocks for
+// kMassPages pages of a sequence each: the total log2-sum of every head, then a
+// half warp per page over the heads.  Bound by the latency of three dependent
+// loads.
+constexpr int kMassPages = 64;
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const AttnParams p) {
-  const int tid = threadIdx.x;
+__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int kWarps = kJoinThreads / 32, N = D / 32;
+  extern __shared__ float s_join[];  // [kWarps][D], or [2][heads_q]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the partials are complete and visible
   const int64_t n_out = int64_t(p.n_seqs) * p.heads_q;
   if (blockIdx.x < n_out) {
     const int b = int(blockIdx.x / p.heads_q), hq = int(blockIdx.x % p.heads_q);
@@ -1216,38 +1212,85 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const AttnPar
       if (p.lengths[b] != seq_tokens(p, b) || n < 0 || n > p.max_selected) flag(p.status, ASHKV_FLAG_INDEX_RANGE);
     }
     int r0, r1;
-    join_range(p, b, hq / p.group, r0, r1);
-    const float lse2 = join_lse2(p, b, hq, r0, r1);
-    if (tid < D) {
-      float acc = 0.0f;
-      for (int r = r0; r <= r1; ++r) {
-        const int64_t at = int64_t(r + b) * p.heads_q + hq;
-        const float x = p.part_lse2[at];
-        if (x != -INFINITY) acc = fmaf(exp2f(x - lse2), p.part_o[at * D + tid], acc);
+    partials_of(p, b, hq / p.group, r0, r1);
+    const float* lse = p.part_lse2 + int64_t(b) * p.heads_q + hq;  // + r * heads_q
+    float m = -INFINITY, l = 0.0f;
+    for (int r = r0 + lane; r <= r1; r += 32) merge_lse2(m, l, lse[int64_t(r) * p.heads_q], 1.0f);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+      merge_lse2(m, l, __shfl_xor_sync(0xFFFFFFFFu, m, off), __shfl_xor_sync(0xFFFFFFFFu, l, off));
+    const float total = lse2_of(m, l);
+    float acc[N] = {};
+    const float* rows = p.part_o + (int64_t(b) * p.heads_q + hq) * D + lane * N;  // + r * heads_q * D
+#pragma unroll 4
+    for (int r = r0 + warp; r <= r1; r += kWarps) {
+      const float x = lse[int64_t(r) * p.heads_q];
+      float v[N];
+      if constexpr (N == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(rows + int64_t(r) * p.heads_q * D);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+      } else {
+        const float2 f = *reinterpret_cast<const float2*>(rows + int64_t(r) * p.heads_q * D);
+        v[0] = f.x; v[1] = f.y;
       }
-      p.out[int64_t(blockIdx.x) * D + tid] = f32_to_bf16(acc);
+      const float w = x == -INFINITY ? 0.0f : ex2(x - total);
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] = fmaf(w, v[k], acc[k]);
     }
-    if (tid == 0 && p.lse) p.lse[blockIdx.x] = lse2 * kLn2;
+#pragma unroll
+    for (int k = 0; k < N; ++k) s_join[warp * D + lane * N + k] = acc[k];
+    __syncthreads();
+    if (tid < D) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) sum += s_join[w * D + tid];
+      p.out[int64_t(blockIdx.x) * D + tid] = f32_to_bf16(sum);
+    }
+    if (tid == 0 && p.lse) p.lse[blockIdx.x] = total * kLn2;
     return;
   }
-  extern __shared__ float s_lse[];  // [heads_q]
+  const int per = (p.max_pages + kMassPages - 1) / kMassPages;
   const int64_t mb = int64_t(blockIdx.x) - n_out;
-  const int per = (p.max_pages + kJoinThreads - 1) / kJoinThreads;
-  const int b = int(mb / per), j = int(mb % per) * kJoinThreads + tid;
-  for (int hq = tid >> 5; hq < p.heads_q; hq += kJoinThreads / 32) {
-    int r0, r1;
-    join_range(p, b, hq / p.group, r0, r1);
-    const float lse2 = join_lse2(p, b, hq, r0, r1);
-    if ((tid & 31) == 0) s_lse[hq] = lse2;
+  const int b = int(mb / per), j0 = int(mb % per) * kMassPages;
+  const int pages = int((seq_tokens(p, b) + p.T - 1) / p.T), j1 = min(pages, j0 + kMassPages);
+  if (j0 >= j1) return;
+  float* s_total = s_join;
+  for (int h0 = 0; h0 < p.heads_q; h0 += 32) {  // 32 heads at a time, a warp's lanes; the warps share the partials
+    const int hq = h0 + lane;
+    float m = -INFINITY, l = 0.0f;
+    if (hq < p.heads_q) {
+      int r0, r1;
+      partials_of(p, b, hq / p.group, r0, r1);
+#pragma unroll 4
+      for (int r = r0 + warp; r <= r1; r += kWarps)
+        merge_lse2(m, l, p.part_lse2[int64_t(r + b) * p.heads_q + hq], 1.0f);
+    }
+    float* s_m = s_join + p.heads_q;
+    s_m[tid] = m;
+    s_m[kJoinThreads + tid] = l;
+    __syncthreads();
+    if (warp == 0 && hq < p.heads_q) {
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) merge_lse2(m, l, s_m[w * 32 + lane], s_m[kJoinThreads + w * 32 + lane]);
+      s_total[hq] = lse2_of(m, l);
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  if (int64_t(j) * p.T >= seq_tokens(p, b)) return;
-  const float* pl = p.page_lse2 + (int64_t(b) * p.max_pages + j) * p.heads_q;
-  float sum = 0.0f;
-  for (int h = 0; h < p.heads_q; ++h)
-    if (pl[h] != -INFINITY) sum += exp2f(pl[h] - s_lse[h]);
-  float* m = p.mass + int64_t(b) * p.mass_stride + j;
-  *m = fmaf(p.decay, *m, sum);
+  const int half = tid >> 4, sub = tid & 15;
+  for (int j = j0 + half; j - half < j1; j += kJoinThreads / 16) {
+    float sum = 0.0f;
+    if (j < j1) {
+      const float* pl = p.page_lse2 + (int64_t(b) * p.max_pages + j) * p.heads_q;
+      for (int h = sub; h < p.heads_q; h += 16)
+        if (pl[h] != -INFINITY) sum += ex2(pl[h] - s_total[h]);
+    }
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+    if (sub == 0 && j < j1) {
+      float* at = p.mass + int64_t(b) * p.mass_stride + j;
+      *at = fmaf(p.decay, *at, sum);
+    }
+  }
 }
 
 int ranges_for(int64_t n_seqs, int heads_kv, int q_chunks, int64_t pages_per_list) {
@@ -1314,9 +1357,25 @@ ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
     return ASHKV_LAUNCH_ERROR;
   }
   decode_partials_kernel<D, NT><<<unsigned((workers + kWarpsA - 1) / kWarpsA), kThreadsA, smem, st>>>(p);
+  const ashkv_status_t rc = check_launch("ashkv_decode_attention");
+  if (rc != ASHKV_OK) return rc;
   int64_t blocks = int64_t(p.n_seqs) * p.heads_q;
-  if (p.mass) blocks += int64_t(p.n_seqs) * ((p.max_pages + kJoinThreads - 1) / kJoinThreads);
-  decode_join_kernel<D><<<unsigned(blocks), kJoinThreads, p.mass ? size_t(p.heads_q) * 4 : 0, st>>>(p);
+  size_t join_smem = kJoinThreads / 32 * D * 4;
+  if (p.mass) {
+    blocks += int64_t(p.n_seqs) * ((p.max_pages + kMassPages - 1) / kMassPages);
+    join_smem = std::max(join_smem, size_t(p.heads_q + 2 * kJoinThreads) * 4);
+  }
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(unsigned(blocks));
+  config.blockDim = dim3(kJoinThreads);
+  config.dynamicSmemBytes = join_smem;
+  config.stream = st;
+  cudaLaunchAttribute overlap{};  // its launch overlaps the partials; it waits for them itself
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &overlap;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, decode_join_kernel<D>, static_cast<const AttnParams>(p));
   return check_launch("ashkv_decode_attention");
 }
 
@@ -1329,7 +1388,7 @@ extern "C" int64_t ashkv_decode_scratch_floats(int32_t n_seqs, int32_t heads_q, 
                                                int32_t pages_per_list, int32_t with_mass) {
   if (n_seqs < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv || head_dim <= 0 || pages_per_list < 0) return -1;
   const int64_t slots = int64_t(ranges_for(n_seqs, heads_kv, q_chunks_for(heads_q, heads_kv), pages_per_list)) + n_seqs;
-  int64_t n = slots * heads_q * (int64_t(head_dim) + 1);
+  int64_t n = slots * heads_q * (int64_t(head_dim) + 1) + 2 * int64_t(n_seqs) * heads_kv;
   if (with_mass) n += int64_t(n_seqs) * pages_per_list * heads_q;
   return n;
 }
@@ -1367,7 +1426,9 @@ extern "C" ashkv_status_t ashkv_decode_attention(
   const int64_t rows = (int64_t(p.ranges) + n_seqs) * heads_q;
   p.part_o = d_scratch;
   p.part_lse2 = p.part_o + rows * kv->head_dim;
-  p.page_lse2 = p.part_lse2 + rows;
+  p.first_range = reinterpret_cast<int32_t*>(p.part_lse2 + rows);
+  p.last_range = p.first_range + int64_t(n_seqs) * p.heads_kv;
+  p.page_lse2 = reinterpret_cast<float*>(p.last_range + int64_t(n_seqs) * p.heads_kv);
   for (int t = 1; t < kTiers; ++t) {
     p.fp8_pages |= p.store[t].format == ASHKV_PAGE_FP8;
     p.int_pages |= p.store[t].format == ASHKV_PAGE_INT8 || p.store[t].format == ASHKV_PAGE_INT4;
