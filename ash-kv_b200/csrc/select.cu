@@ -56,91 +56,90 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
   return uint32_t(a & 255) | (uint32_t(b & 255) << 8) | (uint32_t(c & 255) << 16) | (uint32_t(d & 255) << 24);
 }
 
-// A warp per (listed page, key head): lane l keeps the extremes of channels
-// l * D/32 .. over the page's tokens.  Bound by reading the keys once.
+__device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {  // passes over a NaN
+  uint32_t d;
+  asm("min.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// A thread per 8 channels of a listed page: a page's threads read whole rows, 16
+// bytes each, eight rows in flight, and keep the channels' extremes as bf16
+// pairs; the D / 8 threads of a head share its exponent.  Bound by reading the
+// keys once.
 template <int D>
 __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsParams p) {
-  constexpr int N = D / 32, W = N / 2;  // channels, 32-bit words per lane
+  constexpr int kHead = D / 8;  // threads of a head
   const int lane = threadIdx.x & 31;
   const int64_t n = p.count ? min(max(*p.count, 0), p.max_entries) : p.max_entries;
-  const int64_t stride = int64_t(gridDim.x) * (blockDim.x >> 5);
-  for (int64_t i = int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); i < n * p.heads; i += stride) {
-    const int64_t entry = i / p.heads;
-    const int h = int(i % p.heads);
-    const int32_t id = p.list[entry];
-    bool ok = id >= 0 && id < p.n_pages && p.tier[id] == 0;
-    int32_t l = 0, ts = 0;
+  const int chunks = p.heads * kHead;
+  const int64_t items = n * chunks, stride = int64_t(gridDim.x) * 256;
+  for (int64_t i0 = int64_t(blockIdx.x) * 256 + (threadIdx.x & ~31); i0 < items; i0 += stride) {  // warp-uniform
+    const int64_t i = i0 + lane, entry = i / chunks;
+    const int c = int(i - entry * chunks), h = c / kHead;
+    const bool on = i < items;  // a head's threads are all on or all off
+    const int32_t id = on ? p.list[entry] : -1;
+    bool ok = id >= 0 && id < p.n_pages;
+    int32_t tier = 0, l = 0, ts = 0;
+    int nt = p.T;
     if (ok) {
+      tier = p.tier[id];
       l = p.layer_id[id];
       ts = p.token_start[id];
-      ok = l >= 0 && l < p.n_layers && ts >= 0 && int64_t(ts) + p.T <= p.pool_tokens;
+      if (p.valid) nt = max(0, min(p.valid[entry], p.T));
     }
-    if (!ok) {
-      if (lane == 0) flag(p.status, ASHKV_FLAG_INDEX_RANGE);
-      continue;
-    }
-    const int nt = p.valid ? max(0, min(p.valid[entry], p.T)) : p.T;
-    const uint16_t* k = reinterpret_cast<const uint16_t*>(p.layer_k[l]) + int64_t(ts) * p.row_stride + h * D + lane * N;
-    float lo[N], hi[N];
+    ok = ok && tier == 0 && l >= 0 && l < p.n_layers && ts >= 0 && int64_t(ts) + p.T <= p.pool_tokens;
+    if (on && !ok && c == 0) flag(p.status, ASHKV_FLAG_INDEX_RANGE);
+    uint32_t lo[4], hi[4];
 #pragma unroll
-    for (int c = 0; c < N; ++c) { lo[c] = INFINITY; hi[c] = -INFINITY; }
-    auto take = [&](const uint32_t (&w)[W]) {
+    for (int k = 0; k < 4; ++k) { lo[k] = 0x7F807F80u; hi[k] = 0xFF80FF80u; }  // +inf, -inf
+    if (ok) {
+      const uint16_t* row = reinterpret_cast<const uint16_t*>(p.layer_k[l]) + int64_t(ts) * p.row_stride + c * 8;
+      auto take = [&](const uint4& v) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int c = 0; c < W; ++c) {  // fminf / fmaxf pass over a NaN
-        lo[2 * c] = fminf(lo[2 * c], bf16lo(w[c])); hi[2 * c] = fmaxf(hi[2 * c], bf16lo(w[c]));
-        lo[2 * c + 1] = fminf(lo[2 * c + 1], bf16hi(w[c])); hi[2 * c + 1] = fmaxf(hi[2 * c + 1], bf16hi(w[c]));
+        for (int k = 0; k < 4; ++k) { lo[k] = min_bf16x2(lo[k], w[k]); hi[k] = max_bf16x2(hi[k], w[k]); }
+      };
+      int t = 0;
+      for (; t + 8 <= nt; t += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = ld_nc_v4(row + (t + u) * p.row_stride);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) take(v[u]);
       }
-    };
-    auto load = [&](int t, uint32_t (&w)[W]) {
-      if constexpr (W == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(k + t * p.row_stride);
-        w[0] = v.x; w[1] = v.y;
-      } else {
-        w[0] = *reinterpret_cast<const uint32_t*>(k + t * p.row_stride);
-      }
-    };
-    int t = 0;
-    for (; t + 8 <= nt; t += 8) {
-      uint32_t w[8][W];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) load(t + u, w[u]);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) take(w[u]);
+      for (; t < nt; ++t) take(ld_nc_v4(row + t * p.row_stride));
     }
-    for (; t < nt; ++t) {
-      uint32_t w[W];
-      load(t, w);
-      take(w);
-    }
-    float amax = 0.0f;
+    float a[8], b[8], amax = 0.0f;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      const bool none = lo[c] > hi[c];  // no number in the channel
-      lo[c] = none ? 0.0f : fmaxf(fminf(lo[c], kBf16Max), -kBf16Max);
-      hi[c] = none ? 0.0f : fmaxf(fminf(hi[c], kBf16Max), -kBf16Max);
-      amax = fmaxf(amax, fmaxf(fabsf(lo[c]), fabsf(hi[c])));
+    for (int k = 0; k < 8; ++k) {
+      a[k] = k & 1 ? bf16hi(lo[k >> 1]) : bf16lo(lo[k >> 1]);
+      b[k] = k & 1 ? bf16hi(hi[k >> 1]) : bf16lo(hi[k >> 1]);
+      const bool none = a[k] > b[k];  // no number in the channel
+      a[k] = none ? 0.0f : fmaxf(fminf(a[k], kBf16Max), -kBf16Max);
+      b[k] = none ? 0.0f : fmaxf(fminf(b[k], kBf16Max), -kBf16Max);
+      amax = fmaxf(amax, fmaxf(fabsf(a[k]), fabsf(b[k])));
     }
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, off));
+    for (int off = kHead / 2; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, off));
+    if (!ok) continue;  // (the loop bound is the same for the whole warp)
     const int e = bound_exponent(amax);
-    // 2^-e, exact: e is in [-100, 122]
-    const float unit = __uint_as_float(uint32_t(127 - e) << 23);
-    int cl[4] = {0, 0, 0, 0}, ch[4] = {0, 0, 0, 0};
+    const float unit = __uint_as_float(uint32_t(127 - e) << 23);  // 2^-e, exact: e is in [-100, 122]
+    int cl[8], ch[8];
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
+    for (int k = 0; k < 8; ++k) {
       // a bound too small for fp32 in these units still rounds outwards
-      cl[c] = lo[c] < 0.0f ? min(int(floorf(lo[c] * unit)), -1) : int(floorf(lo[c] * unit));
-      ch[c] = hi[c] > 0.0f ? max(int(ceilf(hi[c] * unit)), 1) : int(ceilf(hi[c] * unit));
+      cl[k] = a[k] < 0.0f ? min(int(floorf(a[k] * unit)), -1) : int(floorf(a[k] * unit));
+      ch[k] = b[k] > 0.0f ? max(int(ceilf(b[k] * unit)), 1) : int(ceilf(b[k] * unit));
     }
-    int8_t* out = p.codes + (int64_t(id) * p.heads + h) * 2 * D + lane * N;
-    if constexpr (N == 4) {
-      *reinterpret_cast<uint32_t*>(out) = pack4(cl[0], cl[1], cl[2], cl[3]);
-      *reinterpret_cast<uint32_t*>(out + D) = pack4(ch[0], ch[1], ch[2], ch[3]);
-    } else {
-      *reinterpret_cast<uint16_t*>(out) = uint16_t(pack4(cl[0], cl[1], 0, 0));
-      *reinterpret_cast<uint16_t*>(out + D) = uint16_t(pack4(ch[0], ch[1], 0, 0));
-    }
-    if (lane == 0) p.exponents[int64_t(id) * p.heads + h] = int8_t(e);
+    int8_t* out = p.codes + (int64_t(id) * p.heads + h) * 2 * D + (c % kHead) * 8;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack4(cl[0], cl[1], cl[2], cl[3]), pack4(cl[4], cl[5], cl[6], cl[7]));
+    *reinterpret_cast<uint2*>(out + D) = make_uint2(pack4(ch[0], ch[1], ch[2], ch[3]), pack4(ch[4], ch[5], ch[6], ch[7]));
+    if (c % kHead == 0) p.exponents[int64_t(id) * p.heads + h] = int8_t(e);
   }
 }
 
@@ -169,66 +168,118 @@ __device__ __forceinline__ int pages_of(int32_t length, int max_pages, int T) {
 __device__ __forceinline__ float times_pow2(int dot, int x) { return scalbnf(float(dot), x); }
 
 constexpr int kScoreWarps = 8;
-constexpr int kScorePages = 64;  // pages of a CTA
+constexpr int kScorePages = 16;  // pages of a warp, in two halves of 8
 
-// A CTA per (kScorePages page positions, key head, sequence).  The group's
-// queries are quantised once into shared memory; a warp then takes a page at a
-// time, lane l the bytes 4l .. of lo or hi (D = 128: lanes cover lo, then hi).
+// D (16 x 8, int32) += A (16 x 32, int8, row) * B (32 x 8, int8, col): lane (g, t) holds
+// A rows g and g + 8 and B column g at k = 4t .. 4t + 3 and 16 more, D rows g and g
+// + 8 at columns 2t, 2t + 1.
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+// A CTA per (kScoreWarps * kScorePages page positions, key head, sequence).  The
+// group's queries are quantised into shared memory as A operands of 16 rows,
+// min(q8, 0) against the lower and max(q8, 0) against the upper bounds; the
+// bounds of 8 pages are a B operand straight from global memory, 16 bytes a load
+// (thread t takes chunk 4 j + t of a page, its words serving two products of 32).
+// Bound by reading the bounds once.
 template <int D>
 __global__ void __launch_bounds__(kScoreWarps * 32) select_scores_kernel(const ScoreParams p) {
-  constexpr int W = D / 4;  // 32-bit words of one bound
-  extern __shared__ uint32_t s_q[];  // [group][2][W]: min(q8, 0), max(q8, 0); then [group] exponents
+  constexpr int kChunks = 2 * D / 16;           // 16-byte chunks of a page's bounds
+  extern __shared__ __align__(16) uint8_t s_score[];  // [tiles of 16 queries][kChunks][2 products][8 rows][16 B], exponents
   const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
   const int n = pages_of(p.lengths[b], p.max_pages, p.T);
-  const int j0 = blockIdx.x * kScorePages;
-  if (j0 >= n) return;
-  int* s_e = reinterpret_cast<int*>(s_q + p.group * 2 * W);
-  for (int g = warp; g < p.group; g += kScoreWarps) {
-    const uint16_t* q = p.q + b * p.q_seq_stride + int64_t(h * p.group + g) * p.q_head_stride;
-    constexpr int N = D / 32;
+  const int j_cta = blockIdx.x * (kScoreWarps * kScorePages);
+  if (j_cta >= n) return;
+  const int tiles = (p.group + 15) / 16;
+  // page ids and bounds first: they do not depend on the queries
+  const int j0 = j_cta + warp * kScorePages;
+  int32_t id[2];
+  bool ok[2];
+  uint4 w[2][kChunks / 4];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int j = j0 + 8 * u + g;
+    id[u] = j < n ? p.page_ids[b * p.page_ids_stride + j] : -1;
+    ok[u] = id[u] >= 0 && id[u] < p.n_pages;
+    if (j < n && !ok[u] && t == 0) flag(p.status, ASHKV_FLAG_INDEX_RANGE);
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int8_t* c = p.codes + (int64_t(ok[u] ? id[u] : 0) * p.heads + h) * 2 * D + t * 16;
+#pragma unroll
+    for (int k = 0; k < kChunks / 4; ++k)
+      w[u][k] = ok[u] ? ld_nc_v4(c + 64 * k) : make_uint4(0, 0, 0, 0);
+  }
+  int e_mine[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) e_mine[u] = ok[u] ? p.exponents[int64_t(id[u]) * p.heads + h] : 0;
+  int* s_e = reinterpret_cast<int*>(s_score + size_t(tiles) * kChunks * 256);
+  for (int q = warp; q < tiles * 16; q += kScoreWarps) {
+    constexpr int N = D / 32;  // channels of a lane: lane * N ..
     float x[N], amax = 0.0f;
+    const uint16_t* src = p.q + b * p.q_seq_stride + int64_t(h * p.group + q) * p.q_head_stride + lane * N;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      x[c] = bf16_to_f32(q[lane * N + c]);
-      if (!(fabsf(x[c]) <= kBf16Max)) x[c] = 0.0f;
-      amax = fmaxf(amax, fabsf(x[c]));
+    for (int k = 0; k < N; ++k) {
+      x[k] = q < p.group ? bf16_to_f32(src[k]) : 0.0f;
+      if (!(fabsf(x[k]) <= kBf16Max)) x[k] = 0.0f;
+      amax = fmaxf(amax, fabsf(x[k]));
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, off));
+    amax = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(amax)));
     const int e = bound_exponent(amax);
     const float unit = __uint_as_float(uint32_t(127 - e) << 23);
-    int8_t* neg = reinterpret_cast<int8_t*>(s_q + g * 2 * W) + lane * N;
+    if (lane == 0) s_e[q] = e;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      const int v = __float2int_rn(x[c] * unit);
-      neg[c] = int8_t(min(v, 0));
-      neg[D + c] = int8_t(max(v, 0));
+    for (int k = 0; k < N; ++k) {
+      const int v = __float2int_rn(x[k] * unit);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // lower bounds, then upper
+        const int at = half * D + lane * N + k, chunk = at >> 4, word = (at >> 2) & 3;
+        // product word / 2 of the chunk; operand order: (row g, row g + 8) of its first, of its second word
+        s_score[((size_t(q >> 4) * kChunks + chunk) * 2 + (word >> 1)) * 128 + (q & 7) * 16 +
+                ((word & 1) * 2 + ((q >> 3) & 1)) * 4 + (at & 3)] = uint8_t(half ? max(v, 0) : min(v, 0));
+      }
     }
-    if (lane == 0) s_e[g] = e;
   }
   __syncthreads();
-  const int j1 = min(n, j0 + kScorePages);
-  for (int j = j0 + warp; j < j1; j += kScoreWarps) {
-    const int32_t id = p.page_ids[b * p.page_ids_stride + j];
-    float best = -INFINITY;
-    if (id >= 0 && id < p.n_pages) {
-      const uint32_t* c = reinterpret_cast<const uint32_t*>(p.codes + (int64_t(id) * p.heads + h) * 2 * D);
-      uint32_t w[2 * W / 32];
+  float best[2][2];  // [half][page 2t, 2t + 1]
 #pragma unroll
-      for (int k = 0; k < 2 * W / 32; ++k) w[k] = c[lane + 32 * k];
-      const int e = p.exponents[int64_t(id) * p.heads + h];
-      for (int g = 0; g < p.group; ++g) {
-        int dot = 0;
+  for (int u = 0; u < 2; ++u) best[u][0] = best[u][1] = -INFINITY;
+  for (int m = 0; m < tiles; ++m) {
+    int d[2][4] = {};
 #pragma unroll
-        for (int k = 0; k < 2 * W / 32; ++k) dot = __dp4a(int(w[k]), int(s_q[g * 2 * W + lane + 32 * k]), dot);
-        dot = __reduce_add_sync(0xFFFFFFFFu, dot);
-        best = fmaxf(best, times_pow2(dot, e + s_e[g]));
+    for (int k = 0; k < kChunks / 4; ++k) {
+      const uint4* a = reinterpret_cast<const uint4*>(s_score + (size_t(m) * kChunks + 4 * k + t) * 256) + g;
+      const uint4 a0 = a[0], a1 = a[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        mma_s8(d[u], a0, w[u][k].x, w[u][k].y);
+        mma_s8(d[u], a1, w[u][k].z, w[u][k].w);
       }
-    } else if (lane == 0) {
-      flag(p.status, ASHKV_FLAG_INDEX_RANGE);
     }
-    if (lane == 0) p.scores[(int64_t(b) * p.heads + h) * p.max_pages + j] = best;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {  // row g (+ 8), column 2t + (x & 1)
+        const int q = 16 * m + g + 8 * (x >> 1);
+        const int e = __shfl_sync(0xFFFFFFFFu, e_mine[u], 4 * (2 * t + (x & 1)));
+        if (q < p.group) best[u][x & 1] = fmaxf(best[u][x & 1], times_pow2(d[u][x], e + s_e[q]));
+      }
   }
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float v = best[u][x];
+      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
+      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));
+      v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 16));
+      const int j = j0 + 8 * u + 2 * t + x;
+      const bool exists = __shfl_sync(0xFFFFFFFFu, int(ok[u]), 4 * (2 * t + x));
+      if (g == 0 && j < n) p.scores[(int64_t(b) * p.heads + h) * p.max_pages + j] = exists ? v : -INFINITY;
+    }
 }
 
 // ---------------------------------------------------------------- keep the highest
@@ -241,97 +292,123 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 
 constexpr int kKeepThreads = 1024;
 
+constexpr int kKeepWarps = kKeepThreads / 32;
+constexpr int kBins = 2048, kDigit = 11;
+
 struct KeepShared {
-  uint32_t hist[256];
-  uint32_t warp_a[32], warp_b[32];
-  uint32_t prefix, need;
-  uint32_t base_eq, base_keep;
+  uint32_t hist[kBins];
+  uint32_t warp_a[kKeepWarps], warp_b[kKeepWarps];
+  uint32_t border, need, done;
 };
+
+// Sum over the CTA of what the threads before this one hold (and of all of it).
+__device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* s_warp, uint32_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t inc = v;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, inc, off);
+    if (lane >= off) inc += x;
+  }
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  uint32_t w = s_warp[lane], wi = w;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, wi, off);
+    if (lane >= off) wi += x;
+  }
+  total = __shfl_sync(0xFFFFFFFFu, wi, 31);
+  return __shfl_sync(0xFFFFFFFFu, wi - w, warp) + inc - v;
+}
 
 // One CTA decides for each position j of a row of n scores whether it is kept
 // -- the first `sink`, the last `recent`, and of the others the highest, of
 // equal ones the first, `budget` in all -- and calls emit(j, kept, rank) with
 // its rank among the kept (else among the dropped) in ascending order of j.
-// The border score is found by four rounds over 8 bits of the keys each
-// (a count per value of the digit among the keys that share the digits above).
+// The border score is found by up to three rounds over 11, 11 and 10 bits of
+// the keys (a count per value of the digit among the keys that share the digits
+// above), fewer where a digit's count ends exactly at the number still wanted.
+// For the ranks every warp owns a run of positions and counts it first, so one
+// scan over the warps serves the whole row.  Bound by the latency of its rounds.
 template <class Emit>
 __device__ void keep_highest(const float* __restrict__ score, int n, int budget, int sink, int recent, KeepShared& sm,
                              Emit emit) {
+  static_assert(kKeepWarps == 32, "scan_before takes 32 warps");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool all = n <= budget;
   const int lo = sink, hi = n - recent;  // the positions that compete
   uint32_t border = 0, need = all ? 0u : uint32_t(budget - sink - recent);
   const bool rank = !all && need > 0;
   if (rank) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) sm.hist[tid] = 0;
-      __syncthreads();
+    for (int i = tid; i < kBins; i += kKeepThreads) sm.hist[i] = 0;
+    __syncthreads();
+    for (int shift = 32 - kDigit;; shift = shift >= kDigit ? shift - kDigit : 0) {
+      // digit: bits [shift, shift + bits); the last round has the 10 lowest
+      const int bits = shift == 0 ? 32 - 2 * kDigit : kDigit;
+      const uint32_t mask = (1u << bits) - 1u;
       for (int j = lo + tid; j < hi; j += kKeepThreads) {
         const uint32_t k = order_key(score[j]);
-        if (shift == 24 || (k >> (shift + 8)) == (border >> (shift + 8))) atomicAdd(&sm.hist[(k >> shift) & 255u], 1u);
+        if (shift + bits == 32 || (k >> (shift + bits)) == (border >> (shift + bits)))
+          atomicAdd(&sm.hist[(k >> shift) & mask], 1u);
       }
       __syncthreads();
-      if (warp == 0) {  // the digit, from the top, at which the count reaches `need`
-        uint32_t v[8], sum = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          v[k] = sm.hist[255 - (lane * 8 + k)];
-          sum += v[k];
-        }
-        uint32_t inc = sum;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, inc, off);
-          if (lane >= off) inc += x;
-        }
-        uint32_t above = inc - sum;
-        if (above < need && inc >= need) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            if (above < need && above + v[k] >= need) {
-              sm.prefix = border | (uint32_t(255 - (lane * 8 + k)) << shift);
-              sm.need = need - above;
-              break;
-            }
-            above += v[k];
-          }
-        }
+      // two bins of a thread, from the top
+      const uint32_t d0 = kBins - 1 - 2 * tid, v0 = sm.hist[d0], v1 = sm.hist[d0 - 1];
+      uint32_t total;
+      const uint32_t above = scan_before(v0 + v1, sm.warp_a, total);
+      if (above < need && above + v0 + v1 >= need) {  // exactly one thread
+        const bool first = above + v0 >= need;
+        const uint32_t over = first ? above : above + v0, count = first ? v0 : v1;
+        sm.border = border | ((first ? d0 : d0 - 1) << shift);
+        sm.need = need - over;
+        sm.done = over + count == need;  // every key of this digit is wanted
       }
+      sm.hist[d0] = sm.hist[d0 - 1] = 0;
       __syncthreads();
-      border = sm.prefix;
+      border = sm.border;
       need = sm.need;
+      if (shift == 0) break;
+      if (sm.done) {  // keys from the border on are in, and no more than those
+        need = 0xFFFFFFFFu;
+        break;
+      }
     }
   }
-  if (tid == 0) sm.base_eq = sm.base_keep = 0;
-  __syncthreads();
-  for (int j0 = 0; j0 < n; j0 += kKeepThreads) {
-    const int j = j0 + tid;
-    const bool on = j < n, mid = on && !all && j >= lo && j < hi;
+  // kept: key > border, or the first `need` of key == border; all of key >= border where need is no limit
+  const int run = (n + kKeepThreads - 1) / kKeepThreads * 32, w0 = warp * run, w1 = min(n, w0 + run);
+  auto classify = [&](int j, bool& keep, bool& eq) {
+    const bool mid = !all && j >= lo && j < hi;
     const uint32_t k = mid && rank ? order_key(score[j]) : 0u;
-    const bool eq = mid && rank && k == border;
-    const unsigned me = __ballot_sync(0xFFFFFFFFu, eq);
-    if (lane == 0) sm.warp_a[warp] = __popc(me);
-    __syncthreads();
-    uint32_t before = sm.base_eq, total_eq = sm.base_eq;
-    for (int w = 0; w < kKeepThreads / 32; ++w) {
-      before += w < warp ? sm.warp_a[w] : 0u;
-      total_eq += sm.warp_a[w];
-    }
-    before += __popc(me & ((1u << lane) - 1u));
-    const bool keep = on && (!mid || (rank && (k > border || (eq && before < need))));
-    const unsigned mk = __ballot_sync(0xFFFFFFFFu, keep);
-    if (lane == 0) sm.warp_b[warp] = __popc(mk);
-    __syncthreads();
-    uint32_t kept = sm.base_keep, total_keep = sm.base_keep;
-    for (int w = 0; w < kKeepThreads / 32; ++w) {
-      kept += w < warp ? sm.warp_b[w] : 0u;
-      total_keep += sm.warp_b[w];
-    }
-    kept += __popc(mk & ((1u << lane) - 1u));
-    if (on) emit(j, keep, keep ? int(kept) : j - int(kept));
-    __syncthreads();
-    if (tid == 0) { sm.base_eq = total_eq; sm.base_keep = total_keep; }
-    __syncthreads();
+    eq = mid && rank && need != 0xFFFFFFFFu && k == border;
+    keep = !mid || (rank && (need == 0xFFFFFFFFu ? k >= border : k > border));
+  };
+  uint32_t n_keep = 0, n_eq = 0;
+  for (int j0 = w0; j0 < w1; j0 += 32) {
+    bool keep = false, eq = false;
+    if (j0 + lane < w1) classify(j0 + lane, keep, eq);
+    n_keep += __popc(__ballot_sync(0xFFFFFFFFu, keep));
+    n_eq += __popc(__ballot_sync(0xFFFFFFFFu, eq));
+  }
+  if (lane == 0) { sm.warp_a[warp] = n_keep; sm.warp_b[warp] = n_eq; }
+  __syncthreads();
+  uint32_t eq_before = 0, keep_before = 0;
+  for (int w = 0; w < warp; ++w) {  // the warps before: their certain ones, and of the border's what is still wanted
+    keep_before += sm.warp_a[w];
+    eq_before += sm.warp_b[w];
+  }
+  const uint32_t want = need == 0xFFFFFFFFu ? 0u : need;
+  for (int j0 = w0; j0 < w1; j0 += 32) {
+    const int j = j0 + lane;
+    bool keep = false, eq = false;
+    if (j < w1) classify(j, keep, eq);
+    const unsigned below = (1u << lane) - 1u, mk = __ballot_sync(0xFFFFFFFFu, keep), me = __ballot_sync(0xFFFFFFFFu, eq);
+    const uint32_t e = eq_before + __popc(me & below);
+    const uint32_t kept = keep_before + __popc(mk & below) + min(e, want);
+    if (eq) keep = e < want;
+    if (j < w1) emit(j, keep, keep ? int(kept) : j - int(kept));
+    keep_before += __popc(mk);
+    eq_before += __popc(me);
   }
 }
 
@@ -419,9 +496,9 @@ extern "C" ashkv_status_t ashkv_page_bounds(const ashkv_paged_kv_t* kv, const in
   BoundsParams p{kv->d_tier, kv->d_layer_id, kv->d_token_start, kv->n_pages, kv->d_layer_k, kv->pool_tokens,
                  kv->row_stride, kv->n_layers, kv->tokens_per_page, kv->heads_kv, d_list, d_count, max_entries, d_valid,
                  d_codes, d_exponents, d_status};
-  const int64_t warps = int64_t(max_entries) * p.heads;
+  const int64_t threads = int64_t(max_entries) * p.heads * (kv->head_dim / 8);
   const int sms = sm_count() > 0 ? sm_count() : 148;
-  const unsigned grid = unsigned(std::min<int64_t>((warps + 7) / 8, int64_t(sms) * 8));
+  const unsigned grid = unsigned(std::min<int64_t>((threads + 255) / 256, int64_t(sms) * 8));
   if (kv->head_dim == 64) page_bounds_kernel<64><<<grid, 256, 0, as_stream(stream)>>>(p);
   else page_bounds_kernel<128><<<grid, 256, 0, as_stream(stream)>>>(p);
   return check_launch(kName);
@@ -460,8 +537,9 @@ extern "C" ashkv_status_t ashkv_select_pages(const void* d_q, int64_t q_seq_stri
     ScoreParams p{static_cast<const uint16_t*>(d_q), q_seq_stride, q_head_stride, n_seqs, heads_q, heads_kv, group,
                   d_codes, d_exponents, n_pages, d_page_ids, page_ids_stride, max_pages, tokens_per_page, d_lengths,
                   d_scratch, d_status};
-    const dim3 grid(unsigned((max_pages + kScorePages - 1) / kScorePages), unsigned(heads_kv), unsigned(n_seqs));
-    const size_t smem = size_t(group) * (2 * head_dim + 4);
+    constexpr int kPages = kScoreWarps * kScorePages;
+    const dim3 grid(unsigned((max_pages + kPages - 1) / kPages), unsigned(heads_kv), unsigned(n_seqs));
+    const size_t smem = size_t((group + 15) / 16) * 16 * (2 * head_dim + 4);  // at most 128 queries: 33 KB
     if (head_dim == 64) select_scores_kernel<64><<<grid, kScoreWarps * 32, smem, st>>>(p);
     else select_scores_kernel<128><<<grid, kScoreWarps * 32, smem, st>>>(p);
     const ashkv_status_t rc = check_launch(kName);
