@@ -1074,6 +1074,7 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
   const int range = w / cells, cell = w % cells;
   const int hk = cell % p.heads_kv, q0 = (cell / p.heads_kv) * (8 * NT);
   const uint32_t ring = smem_u32(smem) + uint32_t(mine * p.warp_smem), bars = smem_u32(s_bars[mine]);
+  wait_for_previous();
   if (warp < kWarpsA) {
     Share sh{0, 0, 0, 0};
     if (range < p.ranges) {
@@ -1111,7 +1112,7 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
     }
   }
   __syncthreads();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up from here on
+  allow_next();
   if (warp == kWarpsA) {
     Producer<D>(p, hk, s_share[mine], ring, bars).run();
     return;
@@ -1203,7 +1204,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
   constexpr int kWarps = kJoinThreads / 32, N = D / 32;
   extern __shared__ float s_join[];  // [kWarps][D], or [2][heads_q]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the partials are complete and visible
+  wait_for_previous();  // the partials
   const int64_t n_out = int64_t(p.n_seqs) * p.heads_q;
   if (blockIdx.x < n_out) {
     const int b = int(blockIdx.x / p.heads_q), hq = int(blockIdx.x % p.heads_q);
@@ -1356,7 +1357,8 @@ ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
     set_error("ashkv_decode_attention (shared memory attribute)", e);
     return ASHKV_LAUNCH_ERROR;
   }
-  decode_partials_kernel<D, NT><<<unsigned((workers + kWarpsA - 1) / kWarpsA), kThreadsA, smem, st>>>(p);
+  launch_overlapped(decode_partials_kernel<D, NT>, dim3(unsigned((workers + kWarpsA - 1) / kWarpsA)), dim3(kThreadsA),
+                    size_t(smem), st, p);
   const ashkv_status_t rc = check_launch("ashkv_decode_attention");
   if (rc != ASHKV_OK) return rc;
   int64_t blocks = int64_t(p.n_seqs) * p.heads_q;
@@ -1365,17 +1367,7 @@ ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
     blocks += int64_t(p.n_seqs) * ((p.max_pages + kMassPages - 1) / kMassPages);
     join_smem = std::max(join_smem, size_t(p.heads_q + 2 * kJoinThreads) * 4);
   }
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(unsigned(blocks));
-  config.blockDim = dim3(kJoinThreads);
-  config.dynamicSmemBytes = join_smem;
-  config.stream = st;
-  cudaLaunchAttribute overlap{};  // its launch overlaps the partials; it waits for them itself
-  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  overlap.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &overlap;
-  config.numAttrs = 1;
-  cudaLaunchKernelEx(&config, decode_join_kernel<D>, static_cast<const AttnParams>(p));
+  launch_overlapped(decode_join_kernel<D>, dim3(unsigned(blocks)), dim3(kJoinThreads), join_smem, st, p);
   return check_launch("ashkv_decode_attention");
 }
 

@@ -24,6 +24,29 @@ inline bool aligned(const void* p, uintptr_t a) {
 
 int sm_count();
 
+// Launches a kernel whose set-up may overlap the kernel before it in the stream
+// (programmatic dependent launch).  Its first statement is wait_for_previous(),
+// which returns once that kernel has completed and its writes are visible, so
+// what it reads and writes is ordered as by a plain launch.
+template <class... Params, class... Args>
+cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                              Args&&... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &overlap;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+}
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// From here on (in every CTA) the next kernel may be set up.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // cuTensorMapEncodeTiled fetched once through the runtime's driver entry point
 // (no -lcuda); nullptr when unavailable.  Cast to PFN_cuTensorMapEncodeTiled_v12000.
 void* tensor_map_encoder();

@@ -75,6 +75,7 @@ template <int D>
 __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsParams p) {
   constexpr int kHead = D / 8;  // threads of a head
   const int lane = threadIdx.x & 31;
+  wait_for_previous();
   const int64_t n = p.count ? min(max(*p.count, 0), p.max_entries) : p.max_entries;
   const int chunks = p.heads * kHead;
   const int64_t items = n * chunks, stride = int64_t(gridDim.x) * 256;
@@ -188,8 +189,14 @@ template <int D>
 __global__ void __launch_bounds__(kScoreWarps * 32) select_scores_kernel(const ScoreParams p) {
   constexpr int kChunks = 2 * D / 16;           // 16-byte chunks of a page's bounds
   extern __shared__ __align__(16) uint8_t s_score[];  // [tiles of 16 queries][kChunks][2 products][8 rows][16 B], exponents
+  // Neighbouring chunks keep a row in different banks.
+  const auto operand_row = [](int tile, int chunk, int product, int row) {
+    return ((tile * kChunks + chunk) * 2 + product) * 128 + (row ^ ((2 * chunk + product) & 7)) * 16;
+  };
   const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
+  wait_for_previous();
+  allow_next();
   const int n = pages_of(p.lengths[b], p.max_pages, p.T);
   const int j_cta = blockIdx.x * (kScoreWarps * kScorePages);
   if (j_cta >= n) return;
@@ -231,16 +238,20 @@ __global__ void __launch_bounds__(kScoreWarps * 32) select_scores_kernel(const S
     const int e = bound_exponent(amax);
     const float unit = __uint_as_float(uint32_t(127 - e) << 23);
     if (lane == 0) s_e[q] = e;
+    uint32_t low = 0, high = 0;  // this lane's channels against the lower and the upper bounds
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int v = __float2int_rn(x[k] * unit);
+      low |= uint32_t(min(v, 0) & 255) << (8 * k);
+      high |= uint32_t(max(v, 0)) << (8 * k);
+    }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {  // lower bounds, then upper
-        const int at = half * D + lane * N + k, chunk = at >> 4, word = (at >> 2) & 3;
-        // product word / 2 of the chunk; operand order: (row g, row g + 8) of its first, of its second word
-        s_score[((size_t(q >> 4) * kChunks + chunk) * 2 + (word >> 1)) * 128 + (q & 7) * 16 +
-                ((word & 1) * 2 + ((q >> 3) & 1)) * 4 + (at & 3)] = uint8_t(half ? max(v, 0) : min(v, 0));
-      }
+    for (int half = 0; half < 2; ++half) {
+      const int at = half * D + lane * N, word = (at >> 2) & 3;
+      // operand word order: (row g, row g + 8) of the product's first, of its second word
+      uint8_t* to = s_score + operand_row(q >> 4, at >> 4, word >> 1, q & 7) + ((word & 1) * 2 + ((q >> 3) & 1)) * 4 + (at & 3);
+      if constexpr (N == 4) *reinterpret_cast<uint32_t*>(to) = half ? high : low;
+      else *reinterpret_cast<uint16_t*>(to) = uint16_t(half ? high : low);
     }
   }
   __syncthreads();
@@ -251,8 +262,8 @@ __global__ void __launch_bounds__(kScoreWarps * 32) select_scores_kernel(const S
     int d[2][4] = {};
 #pragma unroll
     for (int k = 0; k < kChunks / 4; ++k) {
-      const uint4* a = reinterpret_cast<const uint4*>(s_score + (size_t(m) * kChunks + 4 * k + t) * 256) + g;
-      const uint4 a0 = a[0], a1 = a[8];
+      const uint4 a0 = *reinterpret_cast<const uint4*>(s_score + operand_row(m, 4 * k + t, 0, g));
+      const uint4 a1 = *reinterpret_cast<const uint4*>(s_score + operand_row(m, 4 * k + t, 1, g));
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         mma_s8(d[u], a0, w[u][k].x, w[u][k].y);
@@ -329,9 +340,12 @@ __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* s_warp, ui
 // The border score is found by up to three rounds over 11, 11 and 10 bits of
 // the keys (a count per value of the digit among the keys that share the digits
 // above), fewer where a digit's count ends exactly at the number still wanted.
-// For the ranks every warp owns a run of positions and counts it first, so one
-// scan over the warps serves the whole row.  Bound by the latency of its rounds.
-template <class Emit>
+// Every warp owns a run of positions, 32 at a time; a row of up to 32 * KEYS per
+// warp keeps its keys in registers.  For the ranks each warp counts its run
+// first, so one scan over the warps serves the whole row.  Bound by the latency
+// of its rounds.
+constexpr int kCached = 8;
+template <bool CACHED, class Emit>
 __device__ void keep_highest(const float* __restrict__ score, int n, int budget, int sink, int recent, KeepShared& sm,
                              Emit emit) {
   static_assert(kKeepWarps == 32, "scan_before takes 32 warps");
@@ -339,19 +353,38 @@ __device__ void keep_highest(const float* __restrict__ score, int n, int budget,
   const bool all = n <= budget;
   const int lo = sink, hi = n - recent;  // the positions that compete
   uint32_t border = 0, need = all ? 0u : uint32_t(budget - sink - recent);
-  const bool rank = !all && need > 0;
-  if (rank) {
+  const int steps = (n + kKeepThreads - 1) / kKeepThreads, w0 = warp * steps * 32;
+  uint32_t cached[CACHED ? kCached : 1];
+  const auto key_at = [&](int s) { return order_key(score[w0 + 32 * s + lane]); };
+  const auto competes = [&](int s) {
+    const int j = w0 + 32 * s + lane;
+    return !all && j >= lo && j < hi;
+  };
+  const auto for_steps = [&](auto body) {
+    if constexpr (CACHED) {
+#pragma unroll
+      for (int s = 0; s < kCached; ++s)
+        if (s < steps) body(s, cached[s]);
+    } else {
+      for (int s = 0; s < steps; ++s) body(s, competes(s) ? key_at(s) : 0u);
+    }
+  };
+  if constexpr (CACHED) {
+#pragma unroll
+    for (int s = 0; s < kCached; ++s) cached[s] = s < steps && competes(s) ? key_at(s) : 0u;
+  }
+  // whether keys equal to the border are all in (then there are no more than wanted above and at it)
+  bool whole = false;
+  if (!all && need > 0) {
     for (int i = tid; i < kBins; i += kKeepThreads) sm.hist[i] = 0;
     __syncthreads();
     for (int shift = 32 - kDigit;; shift = shift >= kDigit ? shift - kDigit : 0) {
       // digit: bits [shift, shift + bits); the last round has the 10 lowest
       const int bits = shift == 0 ? 32 - 2 * kDigit : kDigit;
-      const uint32_t mask = (1u << bits) - 1u;
-      for (int j = lo + tid; j < hi; j += kKeepThreads) {
-        const uint32_t k = order_key(score[j]);
-        if (shift + bits == 32 || (k >> (shift + bits)) == (border >> (shift + bits)))
-          atomicAdd(&sm.hist[(k >> shift) & mask], 1u);
-      }
+      const uint32_t mask = (1u << bits) - 1u, above_bits = uint32_t(uint64_t(0xFFFFFFFFu) << (shift + bits));
+      for_steps([&](int s, uint32_t k) {
+        if (competes(s) && ((k ^ border) & above_bits) == 0) atomicAdd(&sm.hist[(k >> shift) & mask], 1u);
+      });
       __syncthreads();
       // two bins of a thread, from the top
       const uint32_t d0 = kBins - 1 - 2 * tid, v0 = sm.hist[d0], v1 = sm.hist[d0 - 1];
@@ -368,48 +401,50 @@ __device__ void keep_highest(const float* __restrict__ score, int n, int budget,
       __syncthreads();
       border = sm.border;
       need = sm.need;
-      if (shift == 0) break;
-      if (sm.done) {  // keys from the border on are in, and no more than those
-        need = 0xFFFFFFFFu;
-        break;
-      }
+      whole = sm.done;
+      if (shift == 0 || whole) break;
     }
+  } else {
+    border = 0xFFFFFFFFu;  // no competing key is kept
   }
-  // kept: key > border, or the first `need` of key == border; all of key >= border where need is no limit
-  const int run = (n + kKeepThreads - 1) / kKeepThreads * 32, w0 = warp * run, w1 = min(n, w0 + run);
-  auto classify = [&](int j, bool& keep, bool& eq) {
-    const bool mid = !all && j >= lo && j < hi;
-    const uint32_t k = mid && rank ? order_key(score[j]) : 0u;
-    eq = mid && rank && need != 0xFFFFFFFFu && k == border;
-    keep = !mid || (rank && (need == 0xFFFFFFFFu ? k >= border : k > border));
+  unsigned mk[CACHED ? kCached : 1], me[CACHED ? kCached : 1];
+  const auto votes = [&](int s, uint32_t k, unsigned& in, unsigned& at_border) {
+    const bool here = w0 + 32 * s + lane < n, mid = competes(s);
+    in = __ballot_sync(0xFFFFFFFFu, here && (!mid || (whole ? k >= border : k > border)));
+    at_border = __ballot_sync(0xFFFFFFFFu, here && mid && !whole && k == border);
   };
   uint32_t n_keep = 0, n_eq = 0;
-  for (int j0 = w0; j0 < w1; j0 += 32) {
-    bool keep = false, eq = false;
-    if (j0 + lane < w1) classify(j0 + lane, keep, eq);
-    n_keep += __popc(__ballot_sync(0xFFFFFFFFu, keep));
-    n_eq += __popc(__ballot_sync(0xFFFFFFFFu, eq));
-  }
+  for_steps([&](int s, uint32_t k) {
+    unsigned in, at_border;
+    votes(s, k, in, at_border);
+    if constexpr (CACHED) { mk[s] = in; me[s] = at_border; }
+    n_keep += __popc(in);
+    n_eq += __popc(at_border);
+  });
   if (lane == 0) { sm.warp_a[warp] = n_keep; sm.warp_b[warp] = n_eq; }
   __syncthreads();
-  uint32_t eq_before = 0, keep_before = 0;
-  for (int w = 0; w < warp; ++w) {  // the warps before: their certain ones, and of the border's what is still wanted
-    keep_before += sm.warp_a[w];
-    eq_before += sm.warp_b[w];
-  }
-  const uint32_t want = need == 0xFFFFFFFFu ? 0u : need;
-  for (int j0 = w0; j0 < w1; j0 += 32) {
-    const int j = j0 + lane;
-    bool keep = false, eq = false;
-    if (j < w1) classify(j, keep, eq);
-    const unsigned below = (1u << lane) - 1u, mk = __ballot_sync(0xFFFFFFFFu, keep), me = __ballot_sync(0xFFFFFFFFu, eq);
-    const uint32_t e = eq_before + __popc(me & below);
-    const uint32_t kept = keep_before + __popc(mk & below) + min(e, want);
-    if (eq) keep = e < want;
-    if (j < w1) emit(j, keep, keep ? int(kept) : j - int(kept));
-    keep_before += __popc(mk);
-    eq_before += __popc(me);
-  }
+  // the warps before: their certain ones, and the keys at the border, of which `need` are wanted
+  uint32_t keep_before = lane < warp ? sm.warp_a[lane] : 0u, eq_before = lane < warp ? sm.warp_b[lane] : 0u;
+  keep_before = __reduce_add_sync(0xFFFFFFFFu, keep_before);
+  eq_before = __reduce_add_sync(0xFFFFFFFFu, eq_before);
+  const unsigned below = (1u << lane) - 1u;
+  for_steps([&](int s, uint32_t k) {
+    unsigned in, at_border;
+    if constexpr (CACHED) { in = mk[s]; at_border = me[s]; }
+    else votes(s, k, in, at_border);
+    const uint32_t e = eq_before + __popc(at_border & below), kept = keep_before + __popc(in & below) + min(e, need);
+    const bool eq = (at_border >> lane) & 1u, keep = eq ? e < need : (in >> lane) & 1u;
+    const int j = w0 + 32 * s + lane;
+    if (j < n) emit(j, keep, keep ? int(kept) : j - int(kept));
+    keep_before += __popc(in);
+    eq_before += __popc(at_border);
+  });
+}
+template <class Emit>
+__device__ __forceinline__ void keep_highest_of(const float* score, int n, int budget, int sink, int recent,
+                                                KeepShared& sm, Emit emit) {
+  if (n <= kCached * kKeepThreads) keep_highest<true>(score, n, budget, sink, recent, sm, emit);
+  else keep_highest<false>(score, n, budget, sink, recent, sm, emit);
 }
 
 __global__ void __launch_bounds__(kKeepThreads) select_keep_kernel(const float* __restrict__ scores,
@@ -420,9 +455,11 @@ __global__ void __launch_bounds__(kKeepThreads) select_keep_kernel(const float* 
   __shared__ KeepShared sm;
   const int64_t row = blockIdx.x;
   const int b = int(row / heads);
+  wait_for_previous();
+  allow_next();
   const int n = pages_of(lengths[b], max_pages, T);
   int32_t* out = selected + row * budget;
-  keep_highest(scores + row * max_pages, n, budget, sink, recent, sm, [&](int j, bool kept, int at) {
+  keep_highest_of(scores + row * max_pages, n, budget, sink, recent, sm, [&](int j, bool kept, int at) {
     if (kept) out[at] = j;
   });
   const int kept = min(n, budget);
@@ -440,13 +477,14 @@ __global__ void __launch_bounds__(kKeepThreads) evict_kernel(
     int32_t* __restrict__ evicted, int32_t* __restrict__ evicted_count) {
   __shared__ KeepShared sm;
   const int64_t b = blockIdx.x;
+  wait_for_previous();
   const int n = pages_of(lengths[b], max_pages, T);
   const float* m = mass + b * mass_stride;
   const int32_t* ids = page_ids + b * page_ids_stride;
   int32_t* oi = out_ids + b * max_pages;
   float* om = out_mass + b * max_pages;
   int32_t* ev = evicted + b * max_pages;
-  keep_highest(m, n, budget, sink, recent, sm, [&](int j, bool kept, int at) {
+  keep_highest_of(m, n, budget, sink, recent, sm, [&](int j, bool kept, int at) {
     if (kept) {
       oi[at] = ids[j];
       om[at] = m[j];
@@ -499,8 +537,8 @@ extern "C" ashkv_status_t ashkv_page_bounds(const ashkv_paged_kv_t* kv, const in
   const int64_t threads = int64_t(max_entries) * p.heads * (kv->head_dim / 8);
   const int sms = sm_count() > 0 ? sm_count() : 148;
   const unsigned grid = unsigned(std::min<int64_t>((threads + 255) / 256, int64_t(sms) * 8));
-  if (kv->head_dim == 64) page_bounds_kernel<64><<<grid, 256, 0, as_stream(stream)>>>(p);
-  else page_bounds_kernel<128><<<grid, 256, 0, as_stream(stream)>>>(p);
+  launch_overlapped(kv->head_dim == 64 ? page_bounds_kernel<64> : page_bounds_kernel<128>, dim3(grid), dim3(256), 0,
+                    as_stream(stream), p);
   return check_launch(kName);
 }
 
@@ -540,14 +578,13 @@ extern "C" ashkv_status_t ashkv_select_pages(const void* d_q, int64_t q_seq_stri
     constexpr int kPages = kScoreWarps * kScorePages;
     const dim3 grid(unsigned((max_pages + kPages - 1) / kPages), unsigned(heads_kv), unsigned(n_seqs));
     const size_t smem = size_t((group + 15) / 16) * 16 * (2 * head_dim + 4);  // at most 128 queries: 33 KB
-    if (head_dim == 64) select_scores_kernel<64><<<grid, kScoreWarps * 32, smem, st>>>(p);
-    else select_scores_kernel<128><<<grid, kScoreWarps * 32, smem, st>>>(p);
+    launch_overlapped(head_dim == 64 ? select_scores_kernel<64> : select_scores_kernel<128>, grid, dim3(kScoreWarps * 32),
+                      smem, st, p);
     const ashkv_status_t rc = check_launch(kName);
     if (rc != ASHKV_OK) return rc;
   }
-  select_keep_kernel<<<unsigned(n_seqs * heads_kv), kKeepThreads, 0, st>>>(
-      d_scratch, d_lengths, heads_kv, max_pages, tokens_per_page, budget, sink, recent, d_selected, d_selected_count,
-      d_status);
+  launch_overlapped(select_keep_kernel, dim3(unsigned(n_seqs * heads_kv)), dim3(kKeepThreads), 0, st, d_scratch, d_lengths,
+                    heads_kv, max_pages, tokens_per_page, budget, sink, recent, d_selected, d_selected_count, d_status);
   return check_launch(kName);
 }
 
@@ -567,8 +604,8 @@ extern "C" ashkv_status_t ashkv_evict_pages(const float* d_page_mass, int64_t ma
       (max_pages > 0 && (!d_page_mass || !d_page_ids || !d_out_page_ids || !d_out_mass || !d_evicted)))
     return refuse(kName, "null device pointer");
   if (page_ids_stride < max_pages || mass_stride < max_pages) return refuse(kName, "row strides must hold max_pages entries");
-  evict_kernel<<<unsigned(n_seqs), kKeepThreads, 0, as_stream(stream)>>>(
-      d_page_mass, mass_stride, d_page_ids, page_ids_stride, d_lengths, max_pages, tokens_per_page, budget, sink,
-      recent, d_out_page_ids, d_out_mass, d_out_lengths, d_evicted, d_evicted_count);
+  launch_overlapped(evict_kernel, dim3(unsigned(n_seqs)), dim3(kKeepThreads), 0, as_stream(stream), d_page_mass, mass_stride,
+                    d_page_ids, page_ids_stride, d_lengths, max_pages, tokens_per_page, budget, sink, recent,
+                    d_out_page_ids, d_out_mass, d_out_lengths, d_evicted, d_evicted_count);
   return check_launch(kName);
 }
