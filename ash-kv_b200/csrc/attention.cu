@@ -203,6 +203,10 @@ __device__ __forceinline__ uint32_t v_off(uint32_t r, uint32_t c) {
   return q * RB + (c << 4);
 }
 
+// v_off(r + 8, c) - v_off(r, c) for r < 8.
+template <int RB>
+__host__ __device__ constexpr uint32_t v_off_8() { return RB >= 128 ? 8 * RB : 4 * RB; }
+
 // ---------------------------------------------------------------- the pages of a worker
 constexpr int kRing = 3;  // units in shared memory per worker: one in use, two on their way
 
@@ -401,11 +405,18 @@ struct Producer {
     const uint32_t r0 = uint32_t(sub) / LPR, c0 = uint32_t(sub) % LPR;
     src += r0 * step + c0 * 16u;
     if (rows >= 16) {
+      // the places of a chunk in four rows; they repeat with the rows (and, for wide rows, the chunks) behind
+      constexpr uint32_t kPeriod = 8 / RPI < 16 / RPI ? 8 / RPI : 16 / RPI;
+      uint32_t place[kPeriod];
+#pragma unroll
+      for (uint32_t j = 0; j < kPeriod; ++j)
+        place[j] = tile + (V ? v_off<RB>(r0 + RPI * j, c0) : k_off<RB>(r0 + RPI * j, c0));
+      constexpr uint32_t kBehind = V ? v_off_8<RB>() : 8 * RB;  // the same chunk 8 rows on
 #pragma unroll
       for (uint32_t j = 0; j < 16 / RPI; ++j) {
 #pragma unroll
         for (uint32_t c = 0; c < CPR; c += LPR)
-          cp_async16(tile + (V ? v_off<RB>(r0 + RPI * j, c0 + c) : k_off<RB>(r0 + RPI * j, c0 + c)), src + c * 16);
+          cp_async16(place[j % kPeriod] + j / kPeriod * kBehind + c * 16u, src + c * 16);
         src += RPI * step;
       }
       return;
@@ -424,6 +435,9 @@ struct Producer {
   __device__ void run() {
     open_segment();
     const uint32_t group = threadIdx.x & 24u;  // first lane of the worker's eight
+    const uint8_t *pk = nullptr, *pv = nullptr;  // the current page
+    uint32_t pm = 0;
+    int pp = 0;
     for (uint32_t sent = 0; __any_sync(0xFFFFFFFFu, active); ++sent) {
       const bool page_start = active && !second && t0 == 0;
       // two pages apart, a step for the next eight entries
@@ -431,12 +445,13 @@ struct Producer {
         if (i - batch0 == kLook) take_batch();
         look_up((i - batch0) >> 1);
       }
-      __syncwarp();
-      const int src = int(group) + ((i - batch0) & (kLook - 1));
-      const uint8_t* pk = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(k), src));
-      const uint8_t* pv = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(v), src));
-      const uint32_t pm = __shfl_sync(0xFFFFFFFFu, meta, src);
-      const int pp = __shfl_sync(0xFFFFFFFFu, pos, src);
+      if (__any_sync(0xFFFFFFFFu, page_start)) {
+        const int src = int(group) + ((i - batch0) & (kLook - 1));  // (inside a page: its own entry again)
+        pk = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(k), src));
+        pv = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(v), src));
+        pm = __shfl_sync(0xFFFFFFFFu, meta, src);
+        pp = __shfl_sync(0xFFFFFFFFu, pos, src);
+      }
       bool ok = true;
       if (active && sent >= kRing) ok = wait_bar(bars + (kRing + slot) * 8, phase ^ 1u);
       if (!__all_sync(0xFFFFFFFFu, ok)) {
@@ -473,9 +488,13 @@ struct Producer {
           if (format == ASHKV_PAGE_INT8) {
             // 8 words of K scales, 9 of V scales (all inside the slot: codes follow them)
             const uint8_t* vs = pv + ((T + uint32_t(t0)) * 2u & ~3u);
-            cp_async4(unit + Layout::kScales + sub * 4u, pv + t0 * 2 + sub * 4);
-            cp_async4(unit + Layout::kScales + 32u + sub * 4u, vs + sub * 4);
-            if (sub == 0) cp_async4(unit + Layout::kScales + 64u, vs + 32);
+            if (T % 8u == 0) {  // 16-byte chunks: two of either
+              if (sub < 4) cp_async16(unit + Layout::kScales + sub * 16u, (sub < 2 ? pv + t0 * 2 : vs - 32) + sub * 16);
+            } else {
+              cp_async4(unit + Layout::kScales + sub * 4u, pv + t0 * 2 + sub * 4);
+              cp_async4(unit + Layout::kScales + 32u + sub * 4u, vs + sub * 4);
+              if (sub == 0) cp_async4(unit + Layout::kScales + 64u, vs + 32);
+            }
           }
         }
         if (done) {
@@ -545,6 +564,7 @@ struct Producer {
 template <int D, int NT>
 struct Worker {
   static constexpr int MT = D / 16;  // channel tiles of 16
+  static constexpr float kUnit8 = 1.0f / 127.0f, kUnit4 = 1.0f / 7.0f;  // a code's value is code * scale * unit
   const AttnParams& p;
   float acc[NT][MT][4];              // [queries 8 n ..][channel tile]: rows g, g + 8, columns (queries) 2t, 2t + 1
   float m[NT], thr[NT], l[NT], ps[NT];  // of query 8 n + g; ps: the page's own sum
@@ -728,12 +748,13 @@ struct Worker {
       fresh = false;
     }
   }
-  // Weights times c and the scales w of the rows of this lane's tokens, as the fp16 operand of the
-  // product with V.
-  __device__ __forceinline__ void fp16_weights(const float (&s)[NT][4], const float (&w)[4], uint32_t (&b)[NT][2]) {
+  // Weights times the scales w of the rows of this lane's tokens and a unit (c times what the scales
+  // leave out), as the fp16 operand of the product with V.
+  static __device__ __forceinline__ void fp16_weights(const float (&s)[NT][4], const float (&w)[4], float unit,
+                                                      uint32_t (&b)[NT][2]) {
     float wc[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) wc[x] = w[x] * c;
+    for (int x = 0; x < 4; ++x) wc[x] = w[x] * unit;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       b[n][0] = f32x2_to_f16x2(s[n][0] * wc[0], s[n][1] * wc[1]);
@@ -850,37 +871,38 @@ struct Worker {
       return fmaf(float(a.d[0][h][j] * 256 + a.d[0][h][2 + j]), 256.0f, float(a.d[1][h][j] + a.d[2][h][2 + j]));
     return fmaf(float(a.d[0][h][2 * n + j] * 256 + a.d[1][h][2 * n + j]), 256.0f, float(a.d[2][h][2 * n + j]));
   }
-  // A tile's row scales of this lane's tokens 2t, 2t + 1, 2t + 8, 2t + 9; 0 for rows not in use.
-  __device__ __forceinline__ void zero_unused(float (&x)[4], int rows) const {
-    if (rows < 16) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (2 * t + (k & 1) + 8 * (k >> 1) >= rows) x[k] = 0.0f;
-    }
-  }
+  // A tile's row scales of this lane's tokens 2t, 2t + 1, 2t + 8, 2t + 9.
   static __device__ __forceinline__ void fp16_pairs(uint32_t a, uint32_t b, float (&x)[4]) {
-    x[0] = f16_to_f32(uint16_t(a)) * (1.0f / 127.0f); x[1] = f16_to_f32(uint16_t(a >> 16)) * (1.0f / 127.0f);
-    x[2] = f16_to_f32(uint16_t(b)) * (1.0f / 127.0f); x[3] = f16_to_f32(uint16_t(b >> 16)) * (1.0f / 127.0f);
+    x[0] = f16_to_f32(uint16_t(a)); x[1] = f16_to_f32(uint16_t(a >> 16));
+    x[2] = f16_to_f32(uint16_t(b)); x[3] = f16_to_f32(uint16_t(b >> 16));
   }
-  __device__ __forceinline__ void int8_scales(uint32_t at, int rows, float (&ks)[4], float (&vs)[4]) const {
-    fp16_pairs(lds32(at + 4 * t), lds32(at + 4 * t + 16), ks);
-    at += 32 + 4 * t;
+  __device__ __forceinline__ void int8_scales(uint32_t at, float (&ks)[4], float (&vs)[4]) const {
+    at += 4 * t;
+    fp16_pairs(lds32(at), lds32(at + 16), ks);
     if (odd_pages)  // the V rows start in the upper half of a word
-      fp16_pairs(__byte_perm(lds32(at), lds32(at + 4), 0x5432), __byte_perm(lds32(at + 16), lds32(at + 20), 0x5432), vs);
+      fp16_pairs(__byte_perm(lds32(at + 32), lds32(at + 36), 0x5432), __byte_perm(lds32(at + 48), lds32(at + 52), 0x5432), vs);
     else
-      fp16_pairs(lds32(at), lds32(at + 16), vs);
-    zero_unused(ks, rows);
-    zero_unused(vs, rows);
+      fp16_pairs(lds32(at + 32), lds32(at + 48), vs);
+  }
+  // Rows not in use weigh nothing: 0 for their scales.
+  template <int K>
+  __device__ __forceinline__ void zero_unused(float (&x)[K][4], int rows) const {
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      if (2 * t + (y & 1) + 8 * (y >> 1) >= rows)
+#pragma unroll
+        for (int k = 0; k < K; ++k) x[k][y] = 0.0f;
   }
 
   // A tile of a page of 8-bit codes, K then V.
   template <bool INT8>
   __device__ __forceinline__ void tile8(uint32_t tile, int rows) {
-    float s[NT][4], vs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+    float s[NT][4], vs[1][4] = {{1.0f, 1.0f, 1.0f, 1.0f}};
     if constexpr (INT8) {
       float ks[4];
-      int8_scales(tile + 16 * D * 2, rows, ks, vs);
-      fit_scale(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
+      int8_scales(tile + 16 * D * 2, ks, vs[0]);
+      if (rows < 16) zero_unused(vs, rows);
+      fit_scale(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[0][2], vs[0][3])) * kUnit8);
       Dots a;
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
@@ -890,7 +912,7 @@ struct Worker {
 #pragma unroll
       for (int x = 0; x < 4; ++x)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][x] = dot_value(a, n, x) * (qs_i[n] * ks[x]);
+        for (int n = 0; n < NT; ++n) s[n][x] = dot_value(a, n, x) * (qs_i[n] * kUnit8 * ks[x]);
     } else {
       fit_scale(1.0f);
       float d[2][4], e[2][4];
@@ -914,7 +936,7 @@ struct Worker {
     }
     weights(s, rows);
     uint32_t b[NT][2];
-    fp16_weights(s, vs, b);
+    fp16_weights(s, vs[0], INT8 ? c * kUnit8 : c, b);
     tile += 16 * D;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
@@ -951,32 +973,31 @@ struct Worker {
                       __byte_perm(e1, o1, 0x7362));
   }
 
-  __device__ __forceinline__ void int4_scales(uint32_t at, int rows, float (&x)[D / 64][4]) const {
+  __device__ __forceinline__ void int4_scales(uint32_t at, float (&x)[D / 64][4]) const {
     const uint2 a = lds64(at), b = lds64(at + 32);
     const uint32_t w[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       if constexpr (D == 128) {
-        x[0][y] = bf16lo(w[y]) * (1.0f / 7.0f);
-        x[1][y] = bf16hi(w[y]) * (1.0f / 7.0f);
+        x[0][y] = bf16lo(w[y]);
+        x[1][y] = bf16hi(w[y]);
       } else {
-        x[0][y] = (odd_head ? bf16hi(w[y]) : bf16lo(w[y])) * (1.0f / 7.0f);
+        x[0][y] = odd_head ? bf16hi(w[y]) : bf16lo(w[y]);
       }
     }
-#pragma unroll
-    for (int k = 0; k < D / 64; ++k) zero_unused(x[k], rows);
   }
 
   // A tile of an INT4 page (scales per 64 channels), K then V.
   __device__ __forceinline__ void tile4(uint32_t tile, int rows) {
     constexpr int K = D / 64;
     float ks[K][4], vs[K][4];
-    int4_scales(tile + 16 * D * 2 + 8 * t, rows, ks);
-    int4_scales(tile + 16 * D * 2 + 8 * t + 64, rows, vs);
+    int4_scales(tile + 16 * D * 2 + 8 * t, ks);
+    int4_scales(tile + 16 * D * 2 + 8 * t + 64, vs);
+    if (rows < 16) zero_unused(vs, rows);
     float top = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) top = fmaxf(top, fmaxf(fmaxf(vs[k][0], vs[k][1]), fmaxf(vs[k][2], vs[k][3])));
-    fit_scale(top);
+    fit_scale(top * kUnit4);
     float s[NT][4];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -995,13 +1016,13 @@ struct Worker {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int y = 0; y < 4; ++y) s[n][y] *= qs_i[n] * 0.0625f;
+      for (int y = 0; y < 4; ++y) s[n][y] *= qs_i[n] * (0.0625f * kUnit4);
     weights(s, rows);
     tile += 8 * D;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       uint32_t b[NT][2], v[4];
-      fp16_weights(s, vs[k], b);
+      fp16_weights(s, vs[k], c * kUnit4, b);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         v[j] = lds32(tile + v_off<D / 2>(2 * t + (j & 1) + 8 * (j >> 1), 2 * k + (g >> 2)) + (g & 3) * 4);
