@@ -302,7 +302,7 @@ struct Producer {
   const uint8_t *k, *v;
   uint32_t meta;
   int pos, batch0;
-  int n_pos, n_id, n_tier, n_layer, n_where;
+  int n_pos, n_id, n_tier, n_layer, n_start, n_slot;
   uint64_t n_k, n_v;
 
   __device__ __forceinline__ Producer(const AttnParams& p_, int hk_, const Share& s, uint32_t ring_, uint32_t bars_)
@@ -347,9 +347,8 @@ struct Producer {
       const bool ok = n_id >= 0 && n_id < p.n_pages;
       n_tier = ok ? p.tier[n_id] : -1;
       n_layer = ok ? p.layer_id[n_id] : 0;
-      n_where = ok ? p.token_start[n_id] : 0;
-      const int s = ok ? p.page_slot[n_id] : 0;
-      if (n_tier != 0) n_where = s;
+      n_start = ok ? p.token_start[n_id] : 0;
+      n_slot = ok ? p.page_slot[n_id] : 0;
     } else {
       const bool ok = n_tier == 0 && n_layer >= 0 && n_layer < p.n_layers;
       n_k = ok ? p.layer_k[n_layer] : 0;
@@ -363,6 +362,7 @@ struct Producer {
     meta = 0;
     pos = n_pos;
     if (batch0 + sub >= i1) return;
+    const int n_where = n_tier == 0 ? n_start : n_slot;
     bool ok = n_tier >= 0 && n_tier < kTiers && n_where >= 0;
     if (ok && n_tier == 0) {
       ok = n_layer >= 0 && n_layer < p.n_layers && int64_t(n_where) + p.T <= p.pool_tokens;
