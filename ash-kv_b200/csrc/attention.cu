@@ -203,23 +203,20 @@ __device__ __forceinline__ uint32_t v_off(uint32_t r, uint32_t c) {
   return q * RB + (c << 4);
 }
 
-// v_off(r + 8, c) - v_off(r, c) for r < 8.
-template <int RB>
-__host__ __device__ constexpr uint32_t v_off_8() { return RB >= 128 ? 8 * RB : 4 * RB; }
-
 // ---------------------------------------------------------------- the pages of a worker
 constexpr int kRing = 3;  // units in shared memory per worker: one in use, two on their way
 
 // A unit is 16 tokens of a page for one key head: the K or the V rows of a BF16
-// page (16 x D bf16), or the codes of both of a compressed page (K first), and
-// behind them the scales of those rows: INT8: fp16, K then V, the V rows from the
+// page (16 x D bf16), or the codes of both of a compressed page (K first), with
+// the scales of those rows beside them: INT8: fp16, K then V, the V rows from the
 // last 4-byte boundary on; INT4: a word per row, K then V (D = 64: the row's scale
 // for this head is the word's upper half for an odd head).  A dithered page, and
 // one to leave out, takes a unit that nothing is copied to.  A header says what
 // the unit is.
 template <int D>
-struct UnitLayout {
-  static constexpr int kScales = 16 * D * 2, kHeader = kScales + 128, kBytes = kHeader + 16;
+struct UnitLayout {  // the ring's data, scales and headers, one after the other
+  static constexpr uint32_t kData = 16 * D * 2, kScales = kRing * kData, kHeaders = kScales + kRing * 128,
+                            kBytes = kHeaders + kRing * 16;
 };
 struct Header {
   const uint8_t* slot;  // dithered pages
@@ -296,17 +293,17 @@ struct Producer {
   bool active;
   int t0;                 // first token of the next unit in its page
   bool second;            // BF16: the V rows are next
-  uint32_t unit, slot, phase;
+  uint32_t slot, phase;
   const uint32_t ring, bars;  // shared addresses: the units; full[kRing], empty[kRing]
   // entry batch0 + sub of the segment, and the one being looked up for the next batch
   const uint8_t *k, *v;
-  uint32_t meta;
-  int pos, batch0;
+  uint32_t meta;          // format | tokens in use << 8; no tokens: a page to leave out
+  int pos, batch0;        // position in the sequence
   int n_pos, n_id, n_tier, n_layer, n_start, n_slot;
   uint64_t n_k, n_v;
 
   __device__ __forceinline__ Producer(const AttnParams& p_, int hk_, const Share& s, uint32_t ring_, uint32_t bars_)
-      : p(p_), hk(hk_), sub(int(threadIdx.x & 7u)), unit(ring_), slot(0), phase(0), ring(ring_), bars(bars_) {
+      : p(p_), hk(hk_), sub(int(threadIdx.x & 7u)), slot(0), phase(0), ring(ring_), bars(bars_) {
     b = s.b; before = s.before; row_pos = s.pos; row_end = s.end;
     active = row_pos < row_end;
   }
@@ -405,18 +402,11 @@ struct Producer {
     const uint32_t r0 = uint32_t(sub) / LPR, c0 = uint32_t(sub) % LPR;
     src += r0 * step + c0 * 16u;
     if (rows >= 16) {
-      // the places of a chunk in four rows; they repeat with the rows (and, for wide rows, the chunks) behind
-      constexpr uint32_t kPeriod = 8 / RPI < 16 / RPI ? 8 / RPI : 16 / RPI;
-      uint32_t place[kPeriod];
-#pragma unroll
-      for (uint32_t j = 0; j < kPeriod; ++j)
-        place[j] = tile + (V ? v_off<RB>(r0 + RPI * j, c0) : k_off<RB>(r0 + RPI * j, c0));
-      constexpr uint32_t kBehind = V ? v_off_8<RB>() : 8 * RB;  // the same chunk 8 rows on
 #pragma unroll
       for (uint32_t j = 0; j < 16 / RPI; ++j) {
 #pragma unroll
         for (uint32_t c = 0; c < CPR; c += LPR)
-          cp_async16(place[j % kPeriod] + j / kPeriod * kBehind + c * 16u, src + c * 16);
+          cp_async16(tile + (V ? v_off<RB>(r0 + RPI * j, c0 + c) : k_off<RB>(r0 + RPI * j, c0 + c)), src + c * 16);
         src += RPI * step;
       }
       return;
@@ -456,10 +446,14 @@ struct Producer {
       if (active && sent >= kRing) ok = wait_bar(bars + (kRing + slot) * 8, phase ^ 1u);
       if (!__all_sync(0xFFFFFFFFu, ok)) {
         flag(p.status, ASHKV_FLAG_TIMEOUT);
+        for (uint32_t n = sent < kRing ? 0 : sent - kRing; n < sent && active; ++n)  // what is still on its way
+          wait_bar(bars + n % kRing * 8, n / kRing & 1u);
         break;
       }
       if (active) {
         const uint32_t format = pm & 0xFFu, T = uint32_t(p.T), row = uint32_t(p.row_len);
+        const uint32_t unit = ring + slot * Layout::kData, scales = ring + Layout::kScales + slot * 128;
+        const uint32_t full = bars + slot * 8;
         const int page_tokens = int(pm >> 8), left = page_tokens - t0;
         uint32_t h = format | uint32_t(max(0, min(left, 16))) << 8 | uint32_t(t0) << 16;
         bool done = true;  // with these tokens
@@ -471,29 +465,32 @@ struct Producer {
           if (second) h |= Header::kIsV;
           done = second;
           second = !second;
-        } else if (format == ASHKV_PAGE_INT4) {
-          const uint8_t* codes = pk + uint32_t(t0) * (row / 2);
-          copy_rows<D / 2, false>(codes, row / 2, left, unit);
-          copy_rows<D / 2, true>(codes + T * (row / 2), row / 2, left, unit + 8 * D);
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t r = sub + 8u * (j & 1u);
-            cp_async4(unit + Layout::kScales + (16u * (j >> 1) + r) * 4u,
-                      pv + (min(uint32_t(t0) + r, T - 1u) + (j >> 1) * T) * (row / 32u));
-          }
         } else if (format < ASHKV_PAGE_NBIT4) {
-          const uint8_t* codes = pk + uint32_t(t0) * row;
-          copy_rows<D, false>(codes, row, left, unit);
-          copy_rows<D, true>(codes + T * row, row, left, unit + 16 * D);
-          if (format == ASHKV_PAGE_INT8) {
+          const bool int4 = format == ASHKV_PAGE_INT4;
+          if (int4) {
+            const uint8_t* codes = pk + uint32_t(t0) * (row / 2);
+            copy_rows<D / 2, false>(codes, row / 2, left, unit);
+            copy_rows<D / 2, true>(codes + T * (row / 2), row / 2, left, unit + 8 * D);
+          } else {
+            const uint8_t* codes = pk + uint32_t(t0) * row;
+            copy_rows<D, false>(codes, row, left, unit);
+            copy_rows<D, true>(codes + T * row, row, left, unit + 16 * D);
+          }
+          if (int4) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+              const uint32_t r = sub + 8u * (j & 1u);
+              cp_async4(scales + (16u * (j >> 1) + r) * 4u, pv + (min(uint32_t(t0) + r, T - 1u) + (j >> 1) * T) * (row / 32u));
+            }
+          } else if (format == ASHKV_PAGE_INT8) {
             // 8 words of K scales, 9 of V scales (all inside the slot: codes follow them)
             const uint8_t* vs = pv + ((T + uint32_t(t0)) * 2u & ~3u);
             if (T % 8u == 0) {  // 16-byte chunks: two of either
-              if (sub < 4) cp_async16(unit + Layout::kScales + sub * 16u, (sub < 2 ? pv + t0 * 2 : vs - 32) + sub * 16);
+              if (sub < 4) cp_async16(scales + sub * 16u, (sub < 2 ? pv + t0 * 2 : vs - 32) + sub * 16);
             } else {
-              cp_async4(unit + Layout::kScales + sub * 4u, pv + t0 * 2 + sub * 4);
-              cp_async4(unit + Layout::kScales + 32u + sub * 4u, vs + sub * 4);
-              if (sub == 0) cp_async4(unit + Layout::kScales + 64u, vs + 32);
+              cp_async4(scales + sub * 4u, pv + t0 * 2 + sub * 4);
+              cp_async4(scales + 32u + sub * 4u, vs + sub * 4);
+              if (sub == 0) cp_async4(scales + 64u, vs + 32);
             }
           }
         }
@@ -505,19 +502,15 @@ struct Producer {
             if (++i == i1) h |= Header::kSegmentEnd;
           }
         }
-        const uint32_t full = bars + slot * 8;
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(full) : "memory");
         if (sub == 0) {
           const uint64_t a = reinterpret_cast<uint64_t>(pk);
-          sts128(unit + Layout::kHeader, make_uint4(uint32_t(a), uint32_t(a >> 32), h, uint32_t(pp)));
+          sts128(ring + Layout::kHeaders + slot * 16, make_uint4(uint32_t(a), uint32_t(a >> 32), h, uint32_t(pp)));
           asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(full) : "memory");
         }
         if (++slot == kRing) {
           slot = 0;
           phase ^= 1u;
-          unit = ring;
-        } else {
-          unit += Layout::kBytes;
         }
       }
       const bool ended = active && i == i1;
@@ -896,11 +889,11 @@ struct Worker {
 
   // A tile of a page of 8-bit codes, K then V.
   template <bool INT8>
-  __device__ __forceinline__ void tile8(uint32_t tile, int rows) {
+  __device__ __forceinline__ void tile8(uint32_t tile, uint32_t scales, int rows) {
     float s[NT][4], vs[1][4] = {{1.0f, 1.0f, 1.0f, 1.0f}};
     if constexpr (INT8) {
       float ks[4];
-      int8_scales(tile + 16 * D * 2, ks, vs[0]);
+      int8_scales(scales, ks, vs[0]);
       if (rows < 16) zero_unused(vs, rows);
       fit_scale(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[0][2], vs[0][3])) * kUnit8);
       Dots a;
@@ -988,11 +981,11 @@ struct Worker {
   }
 
   // A tile of an INT4 page (scales per 64 channels), K then V.
-  __device__ __forceinline__ void tile4(uint32_t tile, int rows) {
+  __device__ __forceinline__ void tile4(uint32_t tile, uint32_t scales, int rows) {
     constexpr int K = D / 64;
     float ks[K][4], vs[K][4];
-    int4_scales(tile + 16 * D * 2 + 8 * t, ks);
-    int4_scales(tile + 16 * D * 2 + 8 * t + 64, vs);
+    int4_scales(scales + 8 * t, ks);
+    int4_scales(scales + 8 * t + 64, vs);
     if (rows < 16) zero_unused(vs, rows);
     float top = 0.0f;
 #pragma unroll
@@ -1094,7 +1087,7 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
   const int w = int(blockIdx.x) * kWarpsA + mine;
   const int range = w / cells, cell = w % cells;
   const int hk = cell % p.heads_kv, q0 = (cell / p.heads_kv) * (8 * NT);
-  const uint32_t ring = smem_u32(smem) + uint32_t(mine * p.warp_smem), bars = smem_u32(s_bars[mine]);
+  const uint32_t ring = ((smem_u32(smem) + 1023u) & ~1023u) + uint32_t(mine * p.warp_smem), bars = smem_u32(s_bars[mine]);
   wait_for_previous();
   if (warp < kWarpsA) {
     Share sh{0, 0, 0, 0};
@@ -1138,11 +1131,11 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
     Producer<D>(p, hk, s_share[mine], ring, bars).run();
     return;
   }
-  Worker<D, NT> work(p, ring + kRing * Layout::kBytes, hk);
+  Worker<D, NT> work(p, ring + Layout::kBytes, hk);
   const int nq = min(8 * NT, p.group - q0), hq0 = hk * p.group + q0;
   int b = s_share[warp].b, before = s_share[warp].before, pos = s_share[warp].pos;
   const int end = s_share[warp].end;
-  uint32_t unit = ring, slot = 0, phase = 0;
+  uint32_t slot = 0, phase = 0;
   for (; pos < end; ++b) {
     const int n = list_len(p, b, hk);
     if (n == 0) continue;
@@ -1153,15 +1146,16 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
         flag(p.status, ASHKV_FLAG_TIMEOUT);
         return;
       }
-      const uint4 h4 = lds128(unit + Layout::kHeader);
+      const uint32_t unit = ring + slot * Layout::kData, scales = ring + Layout::kScales + slot * 128;
+      const uint4 h4 = lds128(ring + Layout::kHeaders + slot * 16);
       const Header h{reinterpret_cast<const uint8_t*>(uint64_t(h4.x) | uint64_t(h4.y) << 32), h4.z, int32_t(h4.w)};
       if (h.rows() == 0) {
       } else if (h.format() == ASHKV_PAGE_INT8) {
-        work.template tile8<true>(unit, h.rows());
+        work.template tile8<true>(unit, scales, h.rows());
       } else if (h.format() == ASHKV_PAGE_FP8) {
-        work.template tile8<false>(unit, h.rows());
+        work.template tile8<false>(unit, scales, h.rows());
       } else if (h.format() == ASHKV_PAGE_INT4) {
-        work.tile4(unit, h.rows());
+        work.tile4(unit, scales, h.rows());
       } else if (h.format() >= ASHKV_PAGE_NBIT4) {
         const int t0 = int(h.meta >> 20) * 16;
         for (int half = 0; half < 2; ++half) {
@@ -1184,9 +1178,6 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
       if (++slot == kRing) {
         slot = 0;
         phase ^= 1u;
-        unit = ring;
-      } else {
-        unit += Layout::kBytes;
       }
     }
     work.finish(int64_t(range + b) * p.heads_q + hq0, nq);
@@ -1371,8 +1362,9 @@ ashkv_status_t refuse(const char* what, const char* why) {
 template <int D, int NT>
 ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
   const int64_t workers = int64_t(p.ranges) * p.heads_kv * p.q_chunks;
-  p.warp_smem = kRing * UnitLayout<D>::kBytes + NT * 8 * D * (2 + (p.fp8_pages ? 2 : 0) + (p.int_pages ? 3 : 0));
-  const int smem = kWarpsA * p.warp_smem;
+  p.warp_smem = int(UnitLayout<D>::kBytes) + NT * 8 * D * (2 + (p.fp8_pages ? 2 : 0) + (p.int_pages ? 3 : 0));
+  p.warp_smem = (p.warp_smem + 1023) / 1024 * 1024;
+  const int smem = kWarpsA * p.warp_smem + 1024;
   const cudaError_t e = cudaFuncSetAttribute(decode_partials_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     set_error("ashkv_decode_attention (shared memory attribute)", e);
