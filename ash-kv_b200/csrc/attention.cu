@@ -166,6 +166,9 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" :: "r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(dst), "l"(src) : "memory");
 }
@@ -210,9 +213,10 @@ constexpr int kRing = 3;  // units in shared memory per worker: one in use, two 
 // page (16 x D bf16), or the codes of both of a compressed page (K first), with
 // the scales of those rows beside them: INT8: fp16, K then V, the V rows from the
 // last 4-byte boundary on; INT4: a word per row, K then V (D = 64: the row's scale
-// for this head is the word's upper half for an odd head).  A dithered page, and
-// one to leave out, takes a unit that nothing is copied to.  A header says what
-// the unit is.
+// for this head is the word's upper half for an odd head).  The K or the V rows of
+// a dithered page come as they are (see RawNbit) and are decoded to a BF16 unit
+// in place.  A page to leave out takes a unit that nothing is copied to.  A
+// header says what the unit is.
 template <int D>
 struct UnitLayout {  // the ring's data, scales and headers, one after the other
   static constexpr uint32_t kData = 16 * D * 2, kScales = kRing * kData, kHeaders = kScales + kRing * 128,
@@ -227,48 +231,71 @@ struct Header {
   __device__ __forceinline__ int rows() const { return int(meta >> 8) & 0xFF; }
 };
 
-// Decodes the K or V rows of a dithered page into a BF16 unit.
-  // (Out of line: a call costs little beside the decode, and the loop of the other formats stays short.)
+// A unit of a dithered page as copied: 16 rows of codes, their deltas (D / 32 of a
+// row), the slot's first 16 bytes (the number of outliers) and its first outliers.
 template <int D, int BITS>
-__device__ __noinline__ void stage_nbit(const uint8_t* slot, int T, int row_len, int cap, int hk, bool v, int t0, int rows,
-                                        uint32_t dst) {
-    const int lane = threadIdx.x & 31;
-    const int64_t E = 2 * int64_t(T) * row_len;
-    const uint16_t* delta = reinterpret_cast<const uint16_t*>(slot + nbit_delta_off());
-    const uint8_t* codes = slot + nbit_codes_off(E);
-    constexpr float half = float((1 << BITS) - 1) * 0.5f;
-    constexpr int GPR = D / 32, RB = D * 2;
-    const int row0 = (v ? T : 0) + t0;
+struct RawNbit {
+  static constexpr uint32_t kRow = D * BITS / 8, kDeltas = 16 * kRow, kDeltaRow = D / 16, kCount = kDeltas + 16 * kDeltaRow,
+                            kEntries = kCount + 16, kMaxEntries = 128;
+};
+// Decodes such a unit in place into the K or V rows (bf16) of a BF16 unit; slot: the page's.  A group
+// of 32 channels at a time and lane, all read before any is written; the outliers overwrite theirs.
+// (Out of line: a call costs little beside the decode, and the loop of the other formats stays short.)
+template <int D, int BITS>
+__device__ __noinline__ void decode_nbit(uint32_t unit, const uint8_t* slot, int T, int row_len, int cap, int hk, bool v,
+                                         int t0, int rows) {
+  using Raw = RawNbit<D, BITS>;
+  constexpr int GPR = D / 32, RB = D * 2, N = GPR / 2;
+  constexpr float half = float((1 << BITS) - 1) * 0.5f;
+  const int lane = threadIdx.x & 31;
+  GroupCodes<BITS> gc[N];
 #pragma unroll
-    for (int j = 0; j < GPR / 2; ++j) {
-      const int n = lane + 32 * j, r = n / GPR, k = n % GPR;
-      uint32_t o[16];
-      if (r < rows) {
-        GroupCodes<BITS> gc;
-        load_group<BITS>(delta, codes, (int64_t(row0 + r) * row_len + hk * D) / 32 + k, gc);
-        group_bf16<BITS>(gc, half, o);
-      } else {
-#pragma unroll
-        for (int c = 0; c < 16; ++c) o[c] = 0;
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        sts128(dst + (v ? v_off<RB>(r, 4 * k + c) : k_off<RB>(r, 4 * k + c)),
-               make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]));
+  for (int j = 0; j < N; ++j) {
+    const uint32_t n = lane + 32 * j, at = unit + n * (4 * BITS);  // group n % GPR of row n / GPR
+    if constexpr (BITS == 4) {
+      const uint4 x = lds128(at);
+      gc[j].w[0] = x.x; gc[j].w[1] = x.y; gc[j].w[2] = x.z; gc[j].w[3] = x.w;
+    } else {
+      const uint2 x = lds64(at);
+      gc[j].w[0] = x.x; gc[j].w[1] = x.y;
     }
-    __syncwarp();  // dense values first, then the outliers overwrite theirs
-    const uint32_t n_out = min(*reinterpret_cast<const uint32_t*>(slot), uint32_t(cap));
-    const uint32_t* ent = reinterpret_cast<const uint32_t*>(slot + nbit_entries_off(E, BITS));
-    for (uint32_t j = lane; j < n_out; j += 32) {
-      const uint32_t e = ent[j];
-      const uint32_t r = (e >> 16) / uint32_t(row_len) - uint32_t(row0);
-      const uint32_t c = (e >> 16) % uint32_t(row_len) - uint32_t(hk * D);
-      if (r < uint32_t(rows) && c < uint32_t(D)) {
-        const uint32_t at = dst + (v ? v_off<RB>(r, c >> 3) : k_off<RB>(r, c >> 3)) + (c & 7u) * 2u;
-        asm volatile("st.shared.u16 [%0], %1;" :: "r"(at), "h"(static_cast<uint16_t>(e)) : "memory");
-      }
+    uint16_t d;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(d) : "r"(unit + Raw::kDeltas + n * 2));
+    gc[j].delta = bf16_to_f32(d);
+  }
+  const uint32_t n_out = min(lds32(unit + Raw::kCount), uint32_t(cap));
+  uint32_t entry[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) entry[j] = lds32(unit + Raw::kEntries + (lane + 32 * j) * 4);
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const uint32_t n = lane + 32 * j, r = n / GPR, k = n % GPR;
+    uint32_t o[16];
+    group_bf16<BITS>(gc[j], half, o);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint4 x = int(r) < rows ? make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]) : make_uint4(0, 0, 0, 0);
+      sts128(unit + (v ? v_off<RB>(r, 4 * k + c) : k_off<RB>(r, 4 * k + c)), x);
     }
   }
+  __syncwarp();
+  const uint32_t row0 = uint32_t((v ? T : 0) + t0), shift = 31 - __clz(row_len);  // rows are powers of two
+  const auto put = [&](uint32_t e) {
+    const uint32_t r = (e >> 16 >> shift) - row0, c = ((e >> 16) & uint32_t(row_len - 1)) - uint32_t(hk * D);
+    if (r < uint32_t(rows) && c < uint32_t(D))
+      asm volatile("st.shared.u16 [%0], %1;" :: "r"(unit + (v ? v_off<RB>(r, c >> 3) : k_off<RB>(r, c >> 3)) + (c & 7u) * 2u),
+                   "h"(static_cast<uint16_t>(e)) : "memory");
+  };
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (lane + 32 * j < n_out) put(entry[j]);
+  if (n_out > Raw::kMaxEntries) {
+    const uint32_t* ent = reinterpret_cast<const uint32_t*>(slot + nbit_entries_off(2 * int64_t(T) * row_len, BITS));
+    for (uint32_t j = Raw::kMaxEntries + lane; j < n_out; j += 32) put(__ldg(ent + j));
+  }
+  __syncwarp();
+}
 
 // Where a worker's pages begin: sequence b, of whose list `before` entries of the row lie ahead.
 struct Share {
@@ -422,6 +449,34 @@ struct Producer {
     }
   }
 
+  // The rows, deltas and first outliers of a dithered page (slot pk) for a unit.
+  template <int BITS>
+  __device__ __forceinline__ void copy_nbit(const uint8_t* pk, int rows, uint32_t unit) const {
+    using Raw = RawNbit<D, BITS>;
+    const int64_t E = 2 * int64_t(p.T) * p.row_len;
+    const uint32_t row = uint32_t(p.row_len), row0 = uint32_t((second ? p.T : 0) + t0), last = uint32_t(min(rows, 16)) - 1u;
+    const uint8_t *codes = pk + nbit_codes_off(E), *deltas = pk + nbit_delta_off();
+    constexpr uint32_t CPR = Raw::kRow / 16;
+#pragma unroll
+    for (uint32_t j = 0; j < 2 * CPR; ++j) {  // (rows not in use: the last one again)
+      const uint32_t n = uint32_t(sub) + 8u * j, r = n / CPR, c = n % CPR;
+      cp_async16(unit + n * 16u, codes + ((row0 + min(r, last)) * row + hk * D) * BITS / 8u + c * 16u);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+      const uint32_t r = uint32_t(sub) + 8u * j;
+      const uint8_t* src = deltas + ((row0 + min(r, last)) * row + hk * D) / 16u;
+      if constexpr (D == 128) cp_async8(unit + Raw::kDeltas + r * 8u, src);
+      else cp_async4(unit + Raw::kDeltas + r * 4u, src);
+    }
+    if (sub == 0) cp_async16(unit + Raw::kCount, pk);
+    const uint8_t* entries = pk + nbit_entries_off(E, BITS);
+    const uint32_t bytes = uint32_t(min(p.outlier_cap, int(Raw::kMaxEntries))) * 4u;  // (slots end on 256 bytes)
+#pragma unroll
+    for (uint32_t o = 0; o < Raw::kMaxEntries * 4; o += 128)
+      if (o + uint32_t(sub) * 16u < bytes) cp_async16(unit + Raw::kEntries + o + uint32_t(sub) * 16u, entries + o + sub * 16);
+  }
+
   __device__ void run() {
     open_segment();
     const uint32_t group = threadIdx.x & 24u;  // first lane of the worker's eight
@@ -454,7 +509,7 @@ struct Producer {
         const uint32_t format = pm & 0xFFu, T = uint32_t(p.T), row = uint32_t(p.row_len);
         const uint32_t unit = ring + slot * Layout::kData, scales = ring + Layout::kScales + slot * 128;
         const uint32_t full = bars + slot * 8;
-        const int page_tokens = int(pm >> 8), left = page_tokens - t0;
+        const int left = int(pm >> 8) - t0;
         uint32_t h = format | uint32_t(max(0, min(left, 16))) << 8 | uint32_t(t0) << 16;
         bool done = true;  // with these tokens
         if (left <= 0) {
@@ -493,6 +548,13 @@ struct Producer {
               if (sub == 0) cp_async4(scales + 64u, vs + 32);
             }
           }
+        }
+        else {
+          if (format == ASHKV_PAGE_NBIT4) copy_nbit<4>(pk, left, unit);
+          else copy_nbit<2>(pk, left, unit);
+          if (second) h |= Header::kIsV;
+          done = second;
+          second = !second;
         }
         if (done) {
           t0 += 16;
@@ -1149,6 +1211,14 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
       const uint32_t unit = ring + slot * Layout::kData, scales = ring + Layout::kScales + slot * 128;
       const uint4 h4 = lds128(ring + Layout::kHeaders + slot * 16);
       const Header h{reinterpret_cast<const uint8_t*>(uint64_t(h4.x) | uint64_t(h4.y) << 32), h4.z, int32_t(h4.w)};
+      if (h.format() >= ASHKV_PAGE_NBIT4 && h.rows()) {
+        const int t0 = int(h.meta >> 20) * 16;
+        const bool is_v = h.meta & Header::kIsV;
+        if (h.format() == ASHKV_PAGE_NBIT4)
+          decode_nbit<D, 4>(unit, h.slot, p.T, p.row_len, p.outlier_cap, hk, is_v, t0, h.rows());
+        else
+          decode_nbit<D, 2>(unit, h.slot, p.T, p.row_len, p.outlier_cap, hk, is_v, t0, h.rows());
+      }
       if (h.rows() == 0) {
       } else if (h.format() == ASHKV_PAGE_INT8) {
         work.template tile8<true>(unit, scales, h.rows());
@@ -1156,16 +1226,6 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
         work.template tile8<false>(unit, scales, h.rows());
       } else if (h.format() == ASHKV_PAGE_INT4) {
         work.tile4(unit, scales, h.rows());
-      } else if (h.format() >= ASHKV_PAGE_NBIT4) {
-        const int t0 = int(h.meta >> 20) * 16;
-        for (int half = 0; half < 2; ++half) {
-          if (h.format() == ASHKV_PAGE_NBIT4) stage_nbit<D, 4>(h.slot, p.T, p.row_len, p.outlier_cap, hk, half, t0, h.rows(), unit);
-          else stage_nbit<D, 2>(h.slot, p.T, p.row_len, p.outlier_cap, hk, half, t0, h.rows(), unit);
-          __syncwarp();
-          if (half) work.bf16_values(unit, s);
-          else work.bf16_scores(unit, h.rows(), s);
-          __syncwarp();
-        }
       } else if (h.meta & Header::kIsV) {
         work.bf16_values(unit, s);
       } else {

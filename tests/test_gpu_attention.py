@@ -614,3 +614,11 @@ def test_refusals(cuda):
     no(ValueError, E, mass, ids, L, 2, sink=2, recent=1)
     no(ValueError, E, mass[:, :1], ids, L, 2)
     no(TypeError, E, mass.double(), ids, L, 2)
+
+
+@pytest.mark.parametrize("tiers,dim,heads", [("nbit4", 128, 8), ("nbit2", 64, 16)])
+def test_decode_many_outliers(cuda, tiers, dim, heads):
+    """Some pages of 65536 values hold more outliers than a unit carries."""
+    c, *_ = run_case(cuda, tiers, 32, heads, heads, dim, [70, 33], 7)
+    counts = [int(c.stores[TIER[f]].slot_view()[int(c.table.slot[i])][:4].view(torch.int32)) for i, f in enumerate(c.formats)]
+    assert 128 < max(counts) <= CAP
