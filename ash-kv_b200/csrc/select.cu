@@ -351,40 +351,47 @@ __device__ void keep_highest(const float* __restrict__ score, int n, int budget,
   static_assert(kKeepWarps == 32, "scan_before takes 32 warps");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool all = n <= budget;
-  const int lo = sink, hi = n - recent;  // the positions that compete
-  uint32_t border = 0, need = all ? 0u : uint32_t(budget - sink - recent);
-  const int steps = (n + kKeepThreads - 1) / kKeepThreads, w0 = warp * steps * 32;
+  const int lo = all ? n : sink, hi = all ? n : n - recent;  // the positions that compete
+  const int steps = (n + kKeepThreads - 1) / kKeepThreads, j_first = warp * steps * 32 + lane;
+  const auto competes = [&](int s) { return unsigned(j_first + 32 * s - lo) < unsigned(hi - lo); };
   uint32_t cached[CACHED ? kCached : 1];
-  const auto key_at = [&](int s) { return order_key(score[w0 + 32 * s + lane]); };
-  const auto competes = [&](int s) {
-    const int j = w0 + 32 * s + lane;
-    return !all && j >= lo && j < hi;
-  };
-  const auto for_steps = [&](auto body) {
-    if constexpr (CACHED) {
-#pragma unroll
-      for (int s = 0; s < kCached; ++s)
-        if (s < steps) body(s, cached[s]);
-    } else {
-      for (int s = 0; s < steps; ++s) body(s, competes(s) ? key_at(s) : 0u);
-    }
-  };
+  uint32_t alive = 0;  // bit s (CACHED): step s's position competes and shares the border's digits so far
   if constexpr (CACHED) {
 #pragma unroll
-    for (int s = 0; s < kCached; ++s) cached[s] = s < steps && competes(s) ? key_at(s) : 0u;
+    for (int s = 0; s < kCached; ++s) {
+      cached[s] = 0;
+      if (s < steps && competes(s)) {
+        cached[s] = order_key(score[j_first + 32 * s]);
+        alive |= 1u << s;
+      }
+    }
   }
+  const uint32_t competing = alive;
+  uint32_t border = 0xFFFFFFFFu, need = all ? 0u : uint32_t(budget - sink - recent);
   // whether keys equal to the border are all in (then there are no more than wanted above and at it)
   bool whole = false;
-  if (!all && need > 0) {
+  if (need > 0) {
+    border = 0;
     for (int i = tid; i < kBins; i += kKeepThreads) sm.hist[i] = 0;
     __syncthreads();
     for (int shift = 32 - kDigit;; shift = shift >= kDigit ? shift - kDigit : 0) {
       // digit: bits [shift, shift + bits); the last round has the 10 lowest
       const int bits = shift == 0 ? 32 - 2 * kDigit : kDigit;
-      const uint32_t mask = (1u << bits) - 1u, above_bits = uint32_t(uint64_t(0xFFFFFFFFu) << (shift + bits));
-      for_steps([&](int s, uint32_t k) {
-        if (competes(s) && ((k ^ border) & above_bits) == 0) atomicAdd(&sm.hist[(k >> shift) & mask], 1u);
-      });
+      const uint32_t mask = (1u << bits) - 1u;
+      if constexpr (CACHED) {
+        if (alive) {
+#pragma unroll
+          for (int s = 0; s < kCached; ++s)
+            if (alive >> s & 1u) atomicAdd(&sm.hist[cached[s] >> shift & mask], 1u);
+        }
+      } else {
+        const uint32_t above_bits = uint32_t(uint64_t(0xFFFFFFFFu) << (shift + bits));
+        for (int s = 0; s < steps; ++s) {
+          if (!competes(s)) continue;
+          const uint32_t k = order_key(score[j_first + 32 * s]);
+          if (((k ^ border) & above_bits) == 0) atomicAdd(&sm.hist[k >> shift & mask], 1u);
+        }
+      }
       __syncthreads();
       // two bins of a thread, from the top
       const uint32_t d0 = kBins - 1 - 2 * tid, v0 = sm.hist[d0], v1 = sm.hist[d0 - 1];
@@ -403,38 +410,58 @@ __device__ void keep_highest(const float* __restrict__ score, int n, int budget,
       need = sm.need;
       whole = sm.done;
       if (shift == 0 || whole) break;
+      if constexpr (CACHED) {
+        if (alive) {
+#pragma unroll
+          for (int s = 0; s < kCached; ++s)
+            if ((cached[s] ^ border) >> shift & mask) alive &= ~(1u << s);
+        }
+      }
     }
-  } else {
-    border = 0xFFFFFFFFu;  // no competing key is kept
   }
-  unsigned mk[CACHED ? kCached : 1], me[CACHED ? kCached : 1];
-  const auto votes = [&](int s, uint32_t k, unsigned& in, unsigned& at_border) {
-    const bool here = w0 + 32 * s + lane < n, mid = competes(s);
-    in = __ballot_sync(0xFFFFFFFFu, here && (!mid || (whole ? k >= border : k > border)));
-    at_border = __ballot_sync(0xFFFFFFFFu, here && mid && !whole && k == border);
+  // Kept for certain (`in`), and at the border, where `need` are still wanted.
+  const auto votes = [&](int s, unsigned& in, unsigned& at_border) {
+    const int j = j_first + 32 * s;
+    bool mid;
+    uint32_t k = 0;
+    if constexpr (CACHED) {
+      mid = competing >> s & 1u;
+      k = cached[s];
+    } else {
+      mid = competes(s);
+      if (mid) k = order_key(score[j]);
+    }
+    in = __ballot_sync(0xFFFFFFFFu, j < n && (!mid || (whole ? k >= border : k > border)));
+    at_border = __ballot_sync(0xFFFFFFFFu, mid && !whole && k == border);
+  };
+  const auto for_steps = [&](auto body) {
+    if constexpr (CACHED) {
+#pragma unroll
+      for (int s = 0; s < kCached; ++s)
+        if (s < steps) body(s);
+    } else {
+      for (int s = 0; s < steps; ++s) body(s);
+    }
   };
   uint32_t n_keep = 0, n_eq = 0;
-  for_steps([&](int s, uint32_t k) {
+  for_steps([&](int s) {
     unsigned in, at_border;
-    votes(s, k, in, at_border);
-    if constexpr (CACHED) { mk[s] = in; me[s] = at_border; }
+    votes(s, in, at_border);
     n_keep += __popc(in);
     n_eq += __popc(at_border);
   });
   if (lane == 0) { sm.warp_a[warp] = n_keep; sm.warp_b[warp] = n_eq; }
   __syncthreads();
-  // the warps before: their certain ones, and the keys at the border, of which `need` are wanted
   uint32_t keep_before = lane < warp ? sm.warp_a[lane] : 0u, eq_before = lane < warp ? sm.warp_b[lane] : 0u;
   keep_before = __reduce_add_sync(0xFFFFFFFFu, keep_before);
   eq_before = __reduce_add_sync(0xFFFFFFFFu, eq_before);
   const unsigned below = (1u << lane) - 1u;
-  for_steps([&](int s, uint32_t k) {
+  for_steps([&](int s) {
     unsigned in, at_border;
-    if constexpr (CACHED) { in = mk[s]; at_border = me[s]; }
-    else votes(s, k, in, at_border);
+    votes(s, in, at_border);
     const uint32_t e = eq_before + __popc(at_border & below), kept = keep_before + __popc(in & below) + min(e, need);
-    const bool eq = (at_border >> lane) & 1u, keep = eq ? e < need : (in >> lane) & 1u;
-    const int j = w0 + 32 * s + lane;
+    const bool eq = at_border >> lane & 1u, keep = eq ? e < need : in >> lane & 1u;
+    const int j = j_first + 32 * s;
     if (j < n) emit(j, keep, keep ? int(kept) : j - int(kept));
     keep_before += __popc(in);
     eq_before += __popc(at_border);
@@ -447,7 +474,7 @@ __device__ __forceinline__ void keep_highest_of(const float* score, int n, int b
   else keep_highest<false>(score, n, budget, sink, recent, sm, emit);
 }
 
-__global__ void __launch_bounds__(kKeepThreads) select_keep_kernel(const float* __restrict__ scores,
+__global__ void __launch_bounds__(kKeepThreads, 2) select_keep_kernel(const float* __restrict__ scores,
                                                                    const int32_t* __restrict__ lengths, int heads,
                                                                    int max_pages, int T, int budget, int sink,
                                                                    int recent, int32_t* __restrict__ selected,
@@ -470,7 +497,7 @@ __global__ void __launch_bounds__(kKeepThreads) select_keep_kernel(const float* 
   }
 }
 
-__global__ void __launch_bounds__(kKeepThreads) evict_kernel(
+__global__ void __launch_bounds__(kKeepThreads, 2) evict_kernel(
     const float* __restrict__ mass, int64_t mass_stride, const int32_t* __restrict__ page_ids, int64_t page_ids_stride,
     const int32_t* __restrict__ lengths, int max_pages, int T, int budget, int sink, int recent,
     int32_t* __restrict__ out_ids, float* __restrict__ out_mass, int32_t* __restrict__ out_lengths,
