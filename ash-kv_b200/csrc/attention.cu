@@ -5,8 +5,8 @@
 // 2^(s2[t] - M), s2 = s * log2(e), for any M; one pass over the pages keeps a
 // running M and the two sums.  The work is split over the length of the pages:
 // for each key head the pages of all sequences form one row, cut into equal
-// ranges, one warp each, so a batch of one long sequence and a ragged batch
-// fill the GPU alike.  A range that reaches into several sequences leaves one
+// ranges, one worker warp each, so a batch of one long sequence and a ragged
+// batch fill the GPU alike.  A range that reaches into several sequences leaves one
 // partial result per sequence (normalised, with its log2-sum); the join kernel
 // weighs the partials of each sequence by 2^(their log2-sum - the total).
 #include <algorithm>
@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kWarpsA = 4;          // worker warps of a CTA; a fifth warp feeds them
 constexpr int kThreadsA = (kWarpsA + 1) * 32;
-constexpr int kWorkersPerSm = 12;   // resident worker warps per SM
+constexpr int kWorkersPerSm = 12;   // resident worker warps per SM (8 where registers or shared memory leave two CTAs)
 constexpr uint32_t kPolls = 1u << 24;  // bounded mbarrier waits
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -684,7 +684,7 @@ struct Worker {
       const uint32_t k8 = uint32_t(lane * N) >> 3, w8 = (uint32_t(lane * N) & 7u) >> 1;
 #pragma unroll
       for (int k = 0; k < N; k += 2) sts32(qb + q_word(n, k8, w8 + k / 2, false), uint32_t(x[k]) | (uint32_t(x[k + 1]) << 16));
-      // the exponent of the largest value, kept where 2^+-(e + 23) are normal numbers
+      // the exponent of the largest value, kept where 2^+-(e + 22) are normal numbers
       const int e = min(100, max(-100, int(__float_as_uint(amax) >> 23) - 127));
       const float unit = __uint_as_float(uint32_t(127 + e) << 23), inv = __uint_as_float(uint32_t(127 - e) << 23);
       const bool mine = (n & 7) == g;
@@ -698,13 +698,13 @@ struct Worker {
           sts32(qh + q_word(n, k8, w8 + k / 2, true), f32x2_to_f16x2(bf16_to_f32(x[k]) * down, bf16_to_f32(x[k + 1]) * down));
       }
       if (p.int_pages) {
-        // whole numbers of 23 bits with sign, as digits of base 256 in [-128, 127]: exact down to
-        // 2^-15 of the largest value, off by at most 2^-24 of it below
-        if (mine) qs_i[half] = whole ? p.scale2 * unit * 0x1p-22f : NAN;
+        // whole numbers below 2^22 as digits of base 256 in [-128, 127] (the highest at most 64): exact
+        // down to 2^-14 of the largest value, off by at most 2^-22 of it below
+        if (mine) qs_i[half] = whole ? p.scale2 * unit * 0x1p-21f : NAN;
         uint32_t d[3] = {0, 0, 0};
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-          const int v = __float2int_rn(bf16_to_f32(x[k]) * (inv * 0x1p22f));
+          const int v = __float2int_rn(bf16_to_f32(x[k]) * (inv * 0x1p21f));
           const int v1 = (v + 128) >> 8, v2 = (v1 + 128) >> 8;
           d[0] |= uint32_t(v2 & 255) << (8 * k);
           d[1] |= uint32_t(v1 & 255) << (8 * k);
@@ -1287,18 +1287,8 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
     int r0, r1;
     partials_of(p, b, hq / p.group, r0, r1);
     const float* lse = p.part_lse2 + int64_t(b) * p.heads_q + hq;  // + r * heads_q
-    float m = -INFINITY, l = 0.0f;
-    for (int r = r0 + lane; r <= r1; r += 32) merge_lse2(m, l, lse[int64_t(r) * p.heads_q], 1.0f);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-      merge_lse2(m, l, __shfl_xor_sync(0xFFFFFFFFu, m, off), __shfl_xor_sync(0xFFFFFFFFu, l, off));
-    const float total = lse2_of(m, l);
-    float acc[N] = {};
     const float* rows = p.part_o + (int64_t(b) * p.heads_q + hq) * D + lane * N;  // + r * heads_q * D
-#pragma unroll 4
-    for (int r = r0 + warp; r <= r1; r += kWarps) {
-      const float x = lse[int64_t(r) * p.heads_q];
-      float v[N];
+    const auto load_row = [&](int r, float (&v)[N]) {
       if constexpr (N == 4) {
         const float4 f = *reinterpret_cast<const float4*>(rows + int64_t(r) * p.heads_q * D);
         v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
@@ -1306,9 +1296,30 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
         const float2 f = *reinterpret_cast<const float2*>(rows + int64_t(r) * p.heads_q * D);
         v[0] = f.x; v[1] = f.y;
       }
-      const float w = x == -INFINITY ? 0.0f : ex2(x - total);
+    };
+    // this warp's first two rows are on their way while the total is found
+    float v0[N] = {}, v1[N] = {};
+    if (r0 + warp <= r1) load_row(r0 + warp, v0);
+    if (r0 + warp + kWarps <= r1) load_row(r0 + warp + kWarps, v1);
+    float m = -INFINITY, l = 0.0f;
+    for (int r = r0 + lane; r <= r1; r += 32) merge_lse2(m, l, lse[int64_t(r) * p.heads_q], 1.0f);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+      merge_lse2(m, l, __shfl_xor_sync(0xFFFFFFFFu, m, off), __shfl_xor_sync(0xFFFFFFFFu, l, off));
+    const float total = lse2_of(m, l);
+    float acc[N] = {};
+    const auto add_row = [&](int r, const float (&v)[N]) {
+      const float x = lse[int64_t(r) * p.heads_q], w = x == -INFINITY ? 0.0f : ex2(x - total);
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] = fmaf(w, v[k], acc[k]);
+    };
+    if (r0 + warp <= r1) add_row(r0 + warp, v0);
+    if (r0 + warp + kWarps <= r1) add_row(r0 + warp + kWarps, v1);
+#pragma unroll 4
+    for (int r = r0 + warp + 2 * kWarps; r <= r1; r += kWarps) {
+      float v[N];
+      load_row(r, v);
+      add_row(r, v);
     }
 #pragma unroll
     for (int k = 0; k < N; ++k) s_join[warp * D + lane * N + k] = acc[k];
@@ -1366,9 +1377,10 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
   }
 }
 
-int ranges_for(int64_t n_seqs, int heads_kv, int q_chunks, int64_t pages_per_list) {
+// Ranges that fill the GPU once with `per_sm` workers on an SM.
+int ranges_for(int64_t n_seqs, int heads_kv, int q_chunks, int64_t pages_per_list, int per_sm) {
   const int sms = sm_count() > 0 ? sm_count() : 148;
-  const int64_t fit = std::max<int64_t>(1, int64_t(sms) * kWorkersPerSm / (int64_t(heads_kv) * q_chunks));
+  const int64_t fit = std::max<int64_t>(1, int64_t(sms) * per_sm / (int64_t(heads_kv) * q_chunks));
   return int(std::max<int64_t>(1, std::min<int64_t>(fit, n_seqs * pages_per_list)));
 }
 // Query heads of one worker: one or two column tiles.
@@ -1452,7 +1464,8 @@ using namespace ashkv;
 extern "C" int64_t ashkv_decode_scratch_floats(int32_t n_seqs, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
                                                int32_t pages_per_list, int32_t with_mass) {
   if (n_seqs < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv || head_dim <= 0 || pages_per_list < 0) return -1;
-  const int64_t slots = int64_t(ranges_for(n_seqs, heads_kv, q_chunks_for(heads_q, heads_kv), pages_per_list)) + n_seqs;
+  const int64_t slots = int64_t(ranges_for(n_seqs, heads_kv, q_chunks_for(heads_q, heads_kv), pages_per_list, kWorkersPerSm)) +
+                        n_seqs;
   int64_t n = slots * heads_q * (int64_t(head_dim) + 1) + 2 * int64_t(n_seqs) * heads_kv;
   if (with_mass) n += int64_t(n_seqs) * pages_per_list * heads_q;
   return n;
@@ -1487,17 +1500,18 @@ extern "C" ashkv_status_t ashkv_decode_attention(
   p.scale2 = scale * kLog2e;
   p.mass = d_page_mass; p.mass_stride = mass_stride; p.decay = decay;
   p.out = static_cast<uint16_t*>(d_out); p.lse = d_lse; p.status = d_status;
-  p.ranges = ranges_for(n_seqs, p.heads_kv, p.q_chunks, width);
+  for (int t = 1; t < kTiers; ++t) {
+    p.fp8_pages |= p.store[t].format == ASHKV_PAGE_FP8;
+    p.int_pages |= p.store[t].format == ASHKV_PAGE_INT8 || p.store[t].format == ASHKV_PAGE_INT4;
+  }
+  const bool two_ctas = worker_queries(p.group) == 16 || (p.fp8_pages && p.int_pages);
+  p.ranges = ranges_for(n_seqs, p.heads_kv, p.q_chunks, width, two_ctas ? 2 * kWarpsA : kWorkersPerSm);
   const int64_t rows = (int64_t(p.ranges) + n_seqs) * heads_q;
   p.part_o = d_scratch;
   p.part_lse2 = p.part_o + rows * kv->head_dim;
   p.first_range = reinterpret_cast<int32_t*>(p.part_lse2 + rows);
   p.last_range = p.first_range + int64_t(n_seqs) * p.heads_kv;
   p.page_lse2 = reinterpret_cast<float*>(p.last_range + int64_t(n_seqs) * p.heads_kv);
-  for (int t = 1; t < kTiers; ++t) {
-    p.fp8_pages |= p.store[t].format == ASHKV_PAGE_FP8;
-    p.int_pages |= p.store[t].format == ASHKV_PAGE_INT8 || p.store[t].format == ASHKV_PAGE_INT4;
-  }
   cudaStream_t st = as_stream(stream);
   if (worker_queries(p.group) == 8) return kv->head_dim == 64 ? launch_decode<64, 1>(p, st) : launch_decode<128, 1>(p, st);
   return kv->head_dim == 64 ? launch_decode<64, 2>(p, st) : launch_decode<128, 2>(p, st);

@@ -41,11 +41,12 @@ def decode_attention(q, lists, lengths, T, scale, page_mass=None, decay=1.0):
     """q float64 [n, heads_q, dim]; ``lists[b][hk]`` = [(position, (K, V)), ...] of key head hk.
 
     Returns arrays: out, lse, mass, and for tolerances ``reach`` = sum_t P |v| per result element,
-    ``size`` = max_t scale * sum |q||k| and ``largest`` = max |v| per query head (0 without tokens)."""
+    ``size`` = max_t scale * sum |q||k|, ``wide`` = max_t scale * max|q| sum |k| and ``largest`` =
+    max |v| per query head (0 without tokens)."""
     n, hq, d = q.shape
     hkv = len(lists[0])
     out, reach = np.zeros_like(q), np.zeros_like(q)
-    lse, size, largest = np.full((n, hq), -np.inf), np.zeros((n, hq)), np.zeros((n, hq))
+    lse, size, wide, largest = (np.full((n, hq), -np.inf), *(np.zeros((n, hq)) for _ in range(3)))
     mass = None if page_mass is None else page_mass.astype(np.float64).copy()
     for b in range(n):
         if mass is not None:
@@ -66,13 +67,14 @@ def decode_attention(q, lists, lengths, T, scale, page_mass=None, decay=1.0):
             p = p / p.sum() if p.sum() != 0 else p
             out[b, h], reach[b, h] = p @ V, p @ np.abs(V)
             size[b, h] = (abs(scale) * (np.abs(K) @ np.abs(q[b, h]))).max()
+            wide[b, h] = abs(scale) * np.abs(K).sum(-1).max() * np.abs(q[b, h]).max()
             largest[b, h] = np.abs(V).max()
             if mass is not None:
                 at = 0
                 for pos, k, _ in entries:
                     mass[b, pos] += p[at:at + len(k)].sum()
                     at += len(k)
-    return {"out": out, "lse": lse, "mass": mass, "reach": reach, "size": size, "largest": largest}
+    return {"out": out, "lse": lse, "mass": mass, "reach": reach, "size": size, "wide": wide, "largest": largest}
 
 
 def exponent(amax: float) -> int:

@@ -3,7 +3,9 @@
 Tolerances, from the arithmetic and not from runs.  With u = 2^-24:
   a score is an fp32 sum of dim exact products, scaled by a few factors:
       |ds| <= (dim + 16) * u * size,  size = max_t scale * sum_d |q_d k_d|, plus
-      4 u |s| for the scale and 2^-22 of a weight for exp2;
+      4 u |s| for the scale and 2^-22 of a weight for exp2; over INT8 and INT4 pages the
+      queries are whole numbers off by at most 2^-22 of their largest value, 4 u * wide,
+      wide = max_t scale * max|q| sum_d |k_d|;
   a weight is then off by a factor of at most 1 + dp, dp = 2 max|ds| + 2^-20;
   weights are rounded once before the product with V: 2^-11 (fp16) or, in two
       bf16 parts, 2^-16; the product accumulates in fp32 over the tokens;
@@ -95,7 +97,7 @@ def queries(n, hq, dim, seed, std=1.0):
 
 def check(got, lse, want, dim, n_tokens, mass=None, acc=None, decay=1.0):
     out = got.double().cpu().numpy()
-    ds = (dim + 20) * U * want["size"]
+    ds = (dim + 20) * U * want["size"] + 4 * U * want["wide"]
     dp = 2 * ds + 2.0 ** -20
     tol = 2.0 ** -8 * np.abs(want["out"]) + (2.0 ** -11 + 2 * dp + n_tokens * U)[..., None] * want["reach"]
     tol = tol + n_tokens * 2.0 ** -31 * want["largest"][..., None] + 1e-37
@@ -169,6 +171,28 @@ def test_decode_many_sequences_and_one_long(cuda, tiers):
 def test_decode_value_ranges(cuda, tiers, std):
     """Small values, and scores in the hundreds (one token takes the whole row)."""
     run_case(cuda, tiers, 16, 4, 2, 128, [100, 17], 6, std=std)
+
+
+@pytest.mark.parametrize("tiers", list(FORMATS))
+def test_decode_query_extremes(cuda, tiers):
+    """Largest significands (1.1111111b), negative ones, powers of two, a lone large channel, zeros."""
+    T, heads, dim = 16, 1, 128
+    c = Cache(cuda, [FORMATS[tiers][i % len(FORMATS[tiers])] for i in range(8)], T, heads, dim, 21)
+    ids = np.arange(8, dtype=np.int32).reshape(1, 8)
+    q = queries(1, 8, dim, 21)
+    q[0, 0, :7] = 255 / 128
+    q[0, 1, :7] = -255 / 128
+    q[0, 2, 5] = 255 / 128 * 4
+    q[0, 3, 9] = 255 / 128 * 64
+    q[0, 4, 9] = -512.0
+    q[0, 5] = 0.0
+    q[0, 6] = torch.where(torch.arange(dim) % 2 == 0, 255 / 128, -255 / 128)
+    q[0, 7] *= 2.0 ** -120
+    L = torch.tensor([120], dtype=torch.int32, device=cuda)
+    out, lse = A.decode_attention(q.to(cuda), c.table, c.kv, c.stores, torch.from_numpy(ids).to(cuda), L, scale=0.05,
+                                  return_lse=True)
+    want = O.decode_attention(q.double().numpy(), c.lists(ids, [120]), [120], T, 0.05)
+    check(out, lse, want, dim, 120)
 
 
 def test_decode_no_tokens_and_no_sequences(cuda):
@@ -622,3 +646,87 @@ def test_decode_many_outliers(cuda, tiers, dim, heads):
     c, *_ = run_case(cuda, tiers, 32, heads, heads, dim, [70, 33], 7)
     counts = [int(c.stores[TIER[f]].slot_view()[int(c.table.slot[i])][:4].view(torch.int32)) for i, f in enumerate(c.formats)]
     assert 128 < max(counts) <= CAP
+
+
+# ----------------------------------------------------------------------------- together
+def test_serving_loop(cuda):
+    """Pages are bounded while they are bf16, demoted by the migrator, attended with their mass,
+    evicted, attended again, and attended by selection: against float64 at every step."""
+    from ashkv.contracts.config import ASHKVConfig
+    from ashkv.runtime.batch import BatchMigrator
+    T, heads, dim, P, B = 16, 2, 128, 20, 3
+    row, n = heads * dim, 3 * 20
+    g = torch.Generator().manual_seed(70)
+    k = torch.randn(n * T, heads, dim, generator=g).bfloat16().to(cuda)
+    v = torch.randn(n * T, heads, dim, generator=g).bfloat16().to(cuda)
+    table = DevicePageTable.empty(n, cuda)
+    table.token_start.copy_(torch.randperm(n, generator=g).to(torch.int32) * T)
+    kv = KVLayers([k], [v])
+    stores = {1: TierStore(N.PAGE_INT8, n, cuda, T, row), 2: TierStore(N.PAGE_INT4, n, cuda, T, row)}
+    lengths = [P * T, 11 * T + 5, 1]
+    ids = torch.randperm(n, generator=g).to(torch.int32).view(B, P).to(cuda)
+    L = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    # bounds of every full page; they are of the keys as they were before the move
+    bounds = A.PageBounds.empty(n, heads, dim, cuda)
+    bounds.update(table, kv, ids.view(-1))
+    # two thirds of the pages leave the pool, half of those two tiers down; the last pages stay
+    mig = BatchMigrator(table, kv, stores, ASHKVConfig(), [(0, 1), (1, 0), (1, 2), (2, 1)], tokens_per_page=T)
+    last = {int(ids[b, (x - 1) // T]) for b, x in enumerate(lengths)}
+    move = torch.tensor([p for p in range(n) if p % 3 and p not in last], dtype=torch.int32, device=cuda)
+    for target, lst in ((1, move), (2, move[::2].contiguous())):
+        mig.migrate(lst, torch.tensor([lst.numel()], dtype=torch.int32, device=cuda),
+                    torch.full((n,), target, dtype=torch.int8, device=cuda))
+        assert (mig.status[:lst.numel()] == N.MIGRATE_OK).all()
+    pool = {p: 0 for p in range(n)}
+    for p in range(n):
+        t, s = int(table.tier[p]), int(table.slot[p])
+        if t == 0:
+            at = int(table.token_start[p])
+            data, fmt = np.concatenate([bits(k[at:at + T]).reshape(-1), bits(v[at:at + T]).reshape(-1)]), N.PAGE_BF16
+        else:
+            data, fmt = stores[t].slot_view()[s].cpu().numpy(), stores[t].format
+        pool[p] = O.page_values(fmt, data, T, heads, dim)
+    assert {int(t) for t in table.tier} == {0, 1, 2}
+    scale = dim ** -0.5
+    mass = torch.zeros(B, P, device=cuda)
+    acc = np.zeros((B, P))
+    for step in range(2):  # two steps' mass, the first decayed
+        q = queries(B, 8, dim, 71 + step, 2.0)
+        out, lse = A.decode_attention(q.to(cuda), table, kv, stores, ids, L, page_mass=mass, decay=0.5, return_lse=True)
+        lists = [[[(j, pool[int(ids[b, j])]) for j in range(-(-lengths[b] // T))]] * heads for b in range(B)]
+        want = O.decode_attention(q.double().numpy(), lists, lengths, T, scale, acc, 0.5)
+        check(out, lse, want, dim, P * T, mass, acc, 0.5)
+        acc = want["mass"]
+    kept = A.evict_pages(mass, ids, L, 8, sink=1, recent=2)
+    assert kept.n_evicted.tolist() == [P - 8, 12 - 8, 0] and kept.lengths.tolist() == [8 * T, 7 * T + 5, 1]
+    host = mass.cpu().numpy()
+    for b in range(B):
+        want_ids = [int(ids[b, j]) for j in O.keep_highest(host[b, :-(-lengths[b] // T)].astype(np.float64), 8, 1, 2)]
+        assert kept.page_ids[b, :len(want_ids)].tolist() == want_ids
+    lengths2 = kept.lengths.tolist()
+    lists = [[[(j, pool[int(kept.page_ids[b, j])]) for j in range(-(-lengths2[b] // T))]] * heads for b in range(B)]
+    acc = kept.page_mass.double().cpu().numpy()
+    out, lse = A.decode_attention(q.to(cuda), table, kv, stores, kept.page_ids, kept.lengths, page_mass=kept.page_mass,
+                                  decay=1.0, return_lse=True)
+    check(out, lse, O.decode_attention(q.double().numpy(), lists, lengths2, T, scale, acc, 1.0), dim, P * T,
+          kept.page_mass, acc, 1.0)
+    sel, cnt = A.select_pages(q.to(cuda), bounds, ids, L, 6, sink=1, recent=1)
+    check_selected(sel, cnt, select_want(q, bounds, ids.cpu().numpy(), lengths, T, 6, 1, 1))
+    out, lse = A.decode_attention(q.to(cuda), table, kv, stores, ids, L, selected=sel, selected_count=cnt, return_lse=True)
+    lists = [[[(j, pool[int(ids[b, j])]) for j in sel[b, h, :int(cnt[b, h])].tolist()] for h in range(heads)]
+             for b in range(B)]
+    check(out, lse, O.decode_attention(q.double().numpy(), lists, lengths, T, scale), dim, 6 * T)
+
+
+def test_results_do_not_depend_on_the_run(cuda):
+    """No sum's order depends on timing: the same call gives the same bits."""
+    c = Cache(cuda, [FORMATS["mixed"][i % 4] for i in range(64)], 16, 2, 128, 80)
+    ids = torch.randperm(64, generator=torch.Generator().manual_seed(2)).to(torch.int32).view(2, 32).to(cuda)
+    L = torch.tensor([512, 300], dtype=torch.int32, device=cuda)
+    q = queries(2, 8, 128, 80).to(cuda)
+    first = None
+    for _ in range(10):
+        mass = torch.zeros(2, 32, device=cuda)
+        got = (*A.decode_attention(q, c.table, c.kv, c.stores, ids, L, page_mass=mass, return_lse=True), mass)
+        first = first or got
+        assert all(torch.equal(x, y) for x, y in zip(got, first))
