@@ -56,22 +56,27 @@ def _refuse(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device
         raise ValueError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
 
 
-def _require_rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
-    """[rows, width], dense in its width, with any row stride that keeps rows apart."""
-    if not (t.is_cuda and t.dtype == dtype and t.shape == shape and t.device == device):
-        _refuse(t, name, dtype, shape, device)
-    if not t.is_contiguous():
-        if shape[1] > 1 and t.stride(1) != 1:
-            raise ValueError(f"{name} must be dense in its last dimension")
-        if shape[0] > 1 and t.stride(0) < shape[1]:
-            raise ValueError(f"{name} rows overlap")
-
-
 def _require_dense(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
-    if not (t.is_cuda and t.dtype == dtype and t.shape == shape and t.device == device):
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_cuda:
         _refuse(t, name, dtype, shape, device)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+def _require_rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> torch.Tensor:
+    """[rows, width], dense in its width, with any row stride that keeps rows apart (returned with a
+    stride of at least the width: a single row may carry any)."""
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_cuda:
+        _refuse(t, name, dtype, shape, device)
+    if t.is_contiguous():
+        return t if shape[0] != 1 or t.stride(0) >= shape[1] else t.view(-1).view(shape)
+    if shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} must be dense in its last dimension")
+    if t.stride(0) < shape[1]:
+        if shape[0] > 1:
+            raise ValueError(f"{name} rows overlap")
+        return t.as_strided(shape, (shape[1], 1))
+    return t
 
 
 def _require_query(q: torch.Tensor) -> None:
@@ -87,16 +92,11 @@ def _require_query(q: torch.Tensor) -> None:
         raise ValueError("q has no heads")
 
 
-def _require_lists(page_ids: torch.Tensor, lengths: torch.Tensor, n_seqs: int, device: torch.device) -> None:
+def _require_lists(page_ids: torch.Tensor, lengths: torch.Tensor, n_seqs: int, device: torch.device) -> torch.Tensor:
     if page_ids.dim() != 2:
         raise ValueError("page_ids must be [n_seqs, max_pages]")
-    _require_rows(page_ids, "page_ids", torch.int32, (n_seqs, page_ids.shape[1]), device)
     _require_dense(lengths, "lengths", torch.int32, (n_seqs,), device)
-
-
-def _row_stride(t: torch.Tensor) -> torch.Tensor:
-    """A single row may carry any stride: give it its width (what the kernels check)."""
-    return t if t.shape[0] != 1 or t.stride(0) >= t.shape[1] else t.as_strided(t.shape, (max(t.shape[1], 1), 1))
+    return _require_rows(page_ids, "page_ids", torch.int32, (n_seqs, page_ids.shape[1]), device)
 
 
 _StoreDescs = _native.TierStoreDesc * NUM_TIERS
@@ -166,7 +166,7 @@ def decode_attention(q: torch.Tensor, table: DevicePageTable, kv: KVLayers,
     _require_query(q)
     n_seqs, heads_q, d = q.shape
     dev = q.device
-    _require_lists(page_ids, lengths, n_seqs, dev)
+    page_ids = _require_lists(page_ids, lengths, n_seqs, dev)
     desc, keep = _pages_desc(table, kv, stores, d, tokens_per_page, dev)
     if heads_q % desc.heads_kv:
         raise ValueError(f"{heads_q} query heads are no multiple of {desc.heads_kv} key heads")
@@ -182,12 +182,11 @@ def decode_attention(q: torch.Tensor, table: DevicePageTable, kv: KVLayers,
         _require_dense(selected, "selected", torch.int32, (n_seqs, desc.heads_kv, width), dev)
         _require_dense(selected_count, "selected_count", torch.int32, (n_seqs, desc.heads_kv), dev)
     if page_mass is not None:
-        _require_rows(page_mass, "page_mass", torch.float32, tuple(page_ids.shape), dev)
-        page_mass = _row_stride(page_mass)
+        page_mass = _require_rows(page_mass, "page_mass", torch.float32, page_ids.shape, dev)
     if status is not None:
         _require_dense(status, "status", torch.int32, (1,), dev)
     if out is None:
-        out = torch.empty(n_seqs, heads_q, d, dtype=torch.bfloat16, device=dev)
+        out = q.new_empty((n_seqs, heads_q, d))
     else:
         _require_dense(out, "out", torch.bfloat16, (n_seqs, heads_q, d), dev)
     lse = torch.empty(n_seqs, heads_q, dtype=torch.float32, device=dev) if return_lse else None
@@ -196,7 +195,7 @@ def decode_attention(q: torch.Tensor, table: DevicePageTable, kv: KVLayers,
             scratch = torch.empty(_native.decode_scratch_floats(n_seqs, heads_q, desc.heads_kv, d, width,
                                                                 page_mass is not None),
                                   dtype=torch.float32, device=dev)
-            _native.decode_attention(desc, q, _row_stride(page_ids), lengths, selected, selected_count,
+            _native.decode_attention(desc, q, page_ids, lengths, selected, selected_count,
                                      1.0 / math.sqrt(d) if scale is None else float(scale), page_mass, float(decay),
                                      out, lse, scratch, status)
     return (out, lse) if return_lse else out
@@ -257,7 +256,7 @@ def select_pages(q: torch.Tensor, bounds: PageBounds, page_ids: torch.Tensor, le
     _require_query(q)
     n_seqs, heads_q, d = q.shape
     dev = q.device
-    _require_lists(page_ids, lengths, n_seqs, dev)
+    page_ids = _require_lists(page_ids, lengths, n_seqs, dev)
     heads_kv = bounds.codes.shape[1]
     if bounds.codes.device != dev:
         raise ValueError(f"the bounds are on {bounds.codes.device}, expected {dev}")
@@ -269,13 +268,12 @@ def select_pages(q: torch.Tensor, bounds: PageBounds, page_ids: torch.Tensor, le
         raise ValueError("tokens_per_page must be positive")
     if status is not None:
         _require_dense(status, "status", torch.int32, (1,), dev)
-    selected = torch.empty(n_seqs, heads_kv, budget, dtype=torch.int32, device=dev)
-    count = torch.empty(n_seqs, heads_kv, dtype=torch.int32, device=dev)
+    selected, count = page_ids.new_empty((n_seqs, heads_kv, budget)), page_ids.new_empty((n_seqs, heads_kv))
     if n_seqs:
         with _on(dev):
             scratch = torch.empty(_native.select_scratch_floats(n_seqs, heads_kv, page_ids.shape[1]),
                                   dtype=torch.float32, device=dev)
-            _native.select_pages(q, bounds.codes, bounds.exponents, _row_stride(page_ids), lengths, tokens_per_page,
+            _native.select_pages(q, bounds.codes, bounds.exponents, page_ids, lengths, tokens_per_page,
                                  budget, sink, recent, selected, count, scratch, status)
     return selected, count
 
@@ -302,18 +300,17 @@ def evict_pages(page_mass: torch.Tensor, page_ids: torch.Tensor, lengths: torch.
         raise ValueError("page_ids must be [n_seqs, max_pages]")
     n_seqs, width = page_ids.shape
     dev = page_ids.device
-    _require_lists(page_ids, lengths, n_seqs, dev)
-    _require_rows(page_mass, "page_mass", torch.float32, (n_seqs, width), dev)
+    page_ids = _require_lists(page_ids, lengths, n_seqs, dev)
+    page_mass = _require_rows(page_mass, "page_mass", torch.float32, (n_seqs, width), dev)
     if recent < 1 or sink < 0 or sink + recent > budget:
         raise ValueError("recent must be at least 1, sink not negative, and budget at least sink + recent")
     if tokens_per_page <= 0:
         raise ValueError("tokens_per_page must be positive")
-    new = lambda dt, *shape: torch.empty(*shape, dtype=dt, device=dev)  # noqa: E731
-    got = Eviction(new(torch.int32, n_seqs, width), new(torch.float32, n_seqs, width), new(torch.int32, n_seqs),
-                   new(torch.int32, n_seqs, width), new(torch.int32, n_seqs))
+    ids = page_ids.new_empty
+    got = Eviction(ids((n_seqs, width)), page_mass.new_empty((n_seqs, width)), ids(n_seqs), ids((n_seqs, width)), ids(n_seqs))
     if n_seqs:
         with _on(dev):
-            _native.evict_pages(_row_stride(page_mass), _row_stride(page_ids), lengths, tokens_per_page, budget, sink,
+            _native.evict_pages(page_mass, page_ids, lengths, tokens_per_page, budget, sink,
                                 recent, got.page_ids, got.page_mass, got.lengths, got.evicted, got.n_evicted)
     return got
 

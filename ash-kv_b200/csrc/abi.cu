@@ -1,4 +1,5 @@
 // Library-level entry points: version, status text, last CUDA error.
+#include <atomic>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -38,9 +39,12 @@ void* tensor_map_encoder() {
 }
 
 int sm_count() {
+  static std::atomic<int> known[64];  // per device, once asked
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 

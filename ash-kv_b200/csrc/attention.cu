@@ -10,6 +10,7 @@
 // partial result per sequence (normalised, with its log2-sum); the join kernel
 // weighs the partials of each sequence by 2^(their log2-sum - the total).
 #include <algorithm>
+#include <atomic>
 #include <cstdio>
 
 #include "common.cuh"
@@ -1437,7 +1438,16 @@ ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
   p.warp_smem = int(UnitLayout<D>::kBytes) + NT * 8 * D * (2 + (p.fp8_pages ? 2 : 0) + (p.int_pages ? 3 : 0));
   p.warp_smem = (p.warp_smem + 1023) / 1024 * 1024;
   const int smem = kWarpsA * p.warp_smem + 1024;
-  const cudaError_t e = cudaFuncSetAttribute(decode_partials_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // The attribute is the kernel's on a device and outlasts the call: asked for once with the most that
+  // any stores need.
+  static std::atomic<bool> allowed[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !allowed[dev].load(std::memory_order_acquire))) {
+    constexpr int kMost = kWarpsA * ((int(UnitLayout<D>::kBytes) + NT * 8 * D * 7 + 1023) / 1024 * 1024) + 1024;
+    e = cudaFuncSetAttribute(decode_partials_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (e == cudaSuccess && dev < 64) allowed[dev].store(true, std::memory_order_release);
+  }
   if (e != cudaSuccess) {
     set_error("ashkv_decode_attention (shared memory attribute)", e);
     return ASHKV_LAUNCH_ERROR;
