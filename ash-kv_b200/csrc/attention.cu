@@ -990,16 +990,23 @@ struct Worker {
 #pragma unroll
         for (int x = 0; x < 4; ++x) s[n][x] *= qs_h[n];
     }
+    tile += 16 * D;
+    // V's first 64 channels are on their way from shared memory while the scores become weights
+    const auto load_v = [&](int i, int k) {
+      return lds64(tile + v_off<D>(2 * t + (k & 1) + 8 * (k >> 1), 4 * i + (g >> 1)) + (g & 1) * 8);
+    };
+    uint2 raw[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) raw[k] = load_v(0, k);
     weights(s, rows);
     uint32_t b[NT][2];
     fp16_weights(s, vs[0], INT8 ? c * kUnit8 : c, b);
-    tile += 16 * D;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
       uint32_t v[4][2];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint2 x = lds64(tile + v_off<D>(2 * t + (k & 1) + 8 * (k >> 1), 4 * i + (g >> 1)) + (g & 1) * 8);
+        const uint2 x = i == 0 ? raw[k] : load_v(i, k);
         v[k][0] = INT8 ? x.x ^ 0x80808080u : x.x;
         v[k][1] = INT8 ? x.y ^ 0x80808080u : x.y;
       }
@@ -1073,15 +1080,20 @@ struct Worker {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int y = 0; y < 4; ++y) s[n][y] *= qs_i[n] * (0.0625f * kUnit4);
-    weights(s, rows);
     tile += 8 * D;
+    // V is on its way from shared memory while the scores become weights
+    uint32_t raw[K][4];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      uint32_t b[NT][2], v[4];
-      fp16_weights(s, vs[k], c * kUnit4, b);
+    for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        v[j] = lds32(tile + v_off<D / 2>(2 * t + (j & 1) + 8 * (j >> 1), 2 * k + (g >> 2)) + (g & 3) * 4);
+        raw[k][j] = lds32(tile + v_off<D / 2>(2 * t + (j & 1) + 8 * (j >> 1), 2 * k + (g >> 2)) + (g & 3) * 4);
+    weights(s, rows);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      uint32_t b[NT][2];
+      fp16_weights(s, vs[k], c * kUnit4, b);
+      const uint32_t (&v)[4] = raw[k];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // bytes 2h, 2h + 1 of both tokens: four channels
         uint32_t lo = __byte_perm(v[0], v[1], h ? 0x7632 : 0x5410), hi = __byte_perm(v[2], v[3], h ? 0x7632 : 0x5410);
