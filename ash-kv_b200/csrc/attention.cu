@@ -728,7 +728,7 @@ struct Worker {
 #pragma unroll
         for (int x = 0; x < 4; ++x) acc[n][k][x] = 0.0f;
     }
-    c = 0x1p-8f;  // weights reach 2^8: with bf16 pages alone the sums hold any mean of bf16 values
+    c = 0x1p-8f;  // weights reach 2^8: a sum of n bf16 values stays below n times the largest
     fresh = true;
     __syncwarp();
   }
@@ -795,8 +795,10 @@ struct Worker {
   __device__ __forceinline__ void fit_scale(float x) {
     if (!__any_sync(0xFFFFFFFFu, fresh || x * c > 128.0f)) return;
     const float top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, x > 0.0f ? __float_as_uint(x) : 0u));
-    if (top > 0x1p-100f && top < 0x1p100f) {  // c * top to [2^6, 2^7)
-      const float next = __uint_as_float(uint32_t(254 + 6 - int(__float_as_uint(top) >> 23)) << 23);
+    if (top > 0.0f && top < INFINITY) {  // c * top to [2^6, 2^7)
+      // (c stops at 2^60, where BF16 values up to 2^60 still fit beside it: scales below 2^-54 are off by up to 2^-85)
+      const int e = max(int(__float_as_uint(top) >> 23), 73);
+      const float next = __uint_as_float(uint32_t(254 + 6 - e) << 23);
       const float f = next / c;  // a power of two
 #pragma unroll
       for (int n = 0; n < NT; ++n) scale_acc(n, f, f);

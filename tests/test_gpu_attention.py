@@ -195,6 +195,25 @@ def test_decode_query_extremes(cuda, tiers):
     check(out, lse, want, dim, 120)
 
 
+@pytest.mark.parametrize("kinds,sizes", [
+    ([N.PAGE_INT4, N.PAGE_BF16, N.PAGE_INT4], [1e-7, 1e15, 1.0]), ([N.PAGE_BF16, N.PAGE_INT4, N.PAGE_BF16], [1.0, 1e-7, 1e12]),
+    ([N.PAGE_INT4] * 3, [3e35, 1e-7, 1e35]), ([N.PAGE_INT4, N.PAGE_FP8, N.PAGE_FP8], [1e-7, 1e2, 1.0]),
+    ([N.PAGE_INT8, N.PAGE_NBIT4], [1e-7, 1e15])])
+def test_decode_values_of_far_apart_sizes(cuda, kinds, sizes):
+    """Rows whose scales differ by many powers of two, the smallest first: no sum overflows."""
+    T, heads, dim = 16, 2, 128
+    g = torch.Generator().manual_seed(81)
+    pages = torch.randn(len(kinds), 2, T * heads * dim, generator=g)
+    pages[:, 1] *= torch.tensor(sizes)[:, None]
+    c = Cache(cuda, kinds, T, heads, dim, 81, pool_bits=bits(pages.reshape(len(kinds), -1).to(torch.bfloat16)))
+    ids, lengths = np.arange(len(kinds), dtype=np.int32)[None], [len(kinds) * T - 3]
+    q = queries(1, 8, dim, 81)
+    out, lse = A.decode_attention(q.to(cuda), c.table, c.kv, c.stores, torch.from_numpy(ids).to(cuda),
+                                  torch.tensor(lengths, dtype=torch.int32, device=cuda), return_lse=True)
+    want = O.decode_attention(q.double().numpy(), c.lists(ids, lengths), lengths, T, dim ** -0.5)
+    check(out, lse, want, dim, lengths[0])
+
+
 def test_decode_no_tokens_and_no_sequences(cuda):
     c = Cache(cuda, [N.PAGE_BF16] * 4, 16, 2, 64)
     ids = torch.arange(4, dtype=torch.int32, device=cuda).view(2, 2)
@@ -286,6 +305,8 @@ def test_decode_strides_shared_pages_and_out(cuda):
     want = O.decode_attention(q.double().cpu().numpy(), c.lists(ids.cpu().numpy(), L.cpu().numpy()), L.cpu().numpy(),
                               T, dim ** -0.5, np.zeros((3, 3)), 1.0)
     check(out, lse, want, dim, 49, mass[:, 4:7].contiguous(), np.zeros((3, 3)))
+    over = q.contiguous()  # the result in place of the query
+    assert torch.equal(A.decode_attention(over, c.table, c.kv, c.stores, ids[:, :3], L, out=over), out)
     swapped = q.transpose(0, 1).contiguous().transpose(0, 1)  # heads outermost
     assert torch.equal(A.decode_attention(swapped, c.table, c.kv, c.stores, ids[:, :3], L), out)
 
@@ -402,6 +423,42 @@ def test_decode_streams_and_graphs(cuda):
     L.fill_(60)
     graphs[0].replay()
     assert torch.equal(outs[0], A.decode_attention(qs[1], c.table, c.kv, c.stores, ids, L))
+
+
+def test_captured_fork_of_the_operators(cuda):
+    """Bounds on one stream of a capture and attention with its eviction on another, then a selection after both."""
+    T, heads, dim, P = 16, 2, 128, 12
+    c = Cache(cuda, [N.PAGE_BF16] * (2 * P), T, heads, dim, 82)
+    ids = torch.randperm(2 * P, generator=torch.Generator().manual_seed(2)).to(torch.int32).view(2, P).to(cuda)
+    L = torch.tensor([P * T, 100], dtype=torch.int32, device=cuda)
+    q = queries(2, 8, dim, 82).to(cuda)
+    mass, bounds = torch.zeros(2, P, device=cuda), A.PageBounds.empty(2 * P, heads, dim, cuda)
+    pages = ids.view(-1)
+
+    def step(side):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            bounds.update(c.table, c.kv, pages)
+        out = A.decode_attention(q, c.table, c.kv, None, ids, L, page_mass=mass)
+        kept = A.evict_pages(mass, ids, L, 6)
+        main.wait_stream(side)
+        sel, cnt = A.select_pages(q, bounds, ids, L, 4)
+        part = A.decode_attention(q, c.table, c.kv, None, ids, L, selected=sel, selected_count=cnt)
+        return [out, *kept, sel, cnt, part]
+
+    side = torch.cuda.Stream()
+    want = [t.clone() for t in step(side)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(side)
+    for _ in range(3):
+        mass.zero_()
+        bounds.codes.zero_(), bounds.exponents.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 # ----------------------------------------------------------------------------- bounds
@@ -555,6 +612,10 @@ def test_selected_attention(cuda):
                                   status=status)
     assert int(status) == N.FLAG_INDEX_RANGE
     check(out, lse, O.decode_attention(q.double().numpy(), lists, lengths, T, dim ** -0.5), dim, 12 * T)
+    sel[0, 0, :3] = torch.tensor([3, 0, 3])  # out of order, and a position twice: it counts twice
+    lists[0][0] = [(j, c.values[ids[0, j]]) for j in (3, 0, 3)]
+    out, lse = A.decode_attention(*args, selected=sel.to(cuda), selected_count=cnt.to(cuda), return_lse=True)
+    check(out, lse, O.decode_attention(q.double().numpy(), lists, lengths, T, dim ** -0.5), dim, 12 * T)
 
 
 # ----------------------------------------------------------------------------- eviction
@@ -621,11 +682,15 @@ def test_refusals(cuda):
     no(ValueError, D, q, c.table, c.kv, c.stores, ids.expand(2, 2), L.repeat(2),
        page_mass=mass.expand(2, 2))
     no(TypeError, D, q, c.table, c.kv, c.stores, ids, L, status=mass[0, :1])
+    no(ValueError, D, q, c.table, c.kv, c.stores, ids, L, tokens_per_page=2 ** 32 + 16)
     b = A.PageBounds.empty(2, 2, 64, cuda)
+    no(ValueError, b.update, c.table, c.kv, ids[0], tokens_per_page=2 ** 32 + 16)
     S = A.select_pages
     no(ValueError, S, q, b, ids, L, 0)
     no(ValueError, S, q, b, ids, L, 2, sink=2, recent=1)
     no(ValueError, S, q, b, ids, L, 2, sink=-1)
+    no(ValueError, S, q, b, ids, L, 2 ** 32 + 2)
+    no(ValueError, S, q, b, ids, L, 2, tokens_per_page=2 ** 32 + 16)
     no(ValueError, S, q[:, :3], b, ids, L, 2)
     no(ValueError, S, torch.zeros(1, 4, 128, dtype=torch.bfloat16, device=cuda), b, ids, L, 2)
     no(ValueError, A.PageBounds, b.codes[..., :32].contiguous(), b.exponents)
@@ -637,6 +702,8 @@ def test_refusals(cuda):
     no(ValueError, E, mass, ids, L, 2, recent=0)
     no(ValueError, E, mass, ids, L, 2, sink=2, recent=1)
     no(ValueError, E, mass[:, :1], ids, L, 2)
+    no(ValueError, E, mass, ids, L, 2 ** 32 + 2)
+    no(ValueError, E, mass, ids, L, 2, tokens_per_page=2 ** 32 + 16)
     no(TypeError, E, mass.double(), ids, L, 2)
 
 
