@@ -92,9 +92,19 @@ def _require_query(q: torch.Tensor) -> None:
         raise ValueError("q has no heads")
 
 
+_MOST = 2 ** 31 - 1  # the library takes sizes as int32
+
+
+def _require_tokens_per_page(n: int) -> None:
+    if not 0 < n <= _MOST:
+        raise ValueError("tokens_per_page must be positive and fit an int32")
+
+
 def _require_lists(page_ids: torch.Tensor, lengths: torch.Tensor, n_seqs: int, device: torch.device) -> torch.Tensor:
     if page_ids.dim() != 2:
         raise ValueError("page_ids must be [n_seqs, max_pages]")
+    if page_ids.shape[1] > _MOST or n_seqs > _MOST:
+        raise ValueError("page_ids is too large")
     _require_dense(lengths, "lengths", torch.int32, (n_seqs,), device)
     return _require_rows(page_ids, "page_ids", torch.int32, (n_seqs, page_ids.shape[1]), device)
 
@@ -116,8 +126,7 @@ def _pages_desc(table: DevicePageTable, kv: KVLayers, stores: Optional[Mapping[i
     _require_dense(table.slot, "table.slot", torch.int32, (n,), device)
     if kv.k[0].device != device:
         raise ValueError(f"the KV pool is on {kv.k[0].device}, expected {device}")
-    if tokens_per_page <= 0:
-        raise ValueError("tokens_per_page must be positive")
+    _require_tokens_per_page(tokens_per_page)
     descs = _StoreDescs.from_buffer_copy(_NO_STORES)
     cap = 0
     for t, s in (stores or {}).items():
@@ -230,6 +239,8 @@ class PageBounds:
         given): ``valid[i]`` tokens of page ``pages[i]``, all of them without ``valid``.  Other rows
         are left as they were.  A page listed twice must have one ``valid``."""
         dev = self.codes.device
+        if pages.numel() > _MOST:
+            raise ValueError("pages is too long")
         desc, keep = _pages_desc(table, kv, None, self.codes.shape[3], tokens_per_page, dev)
         if desc.heads_kv != self.codes.shape[1] or desc.n_pages != self.codes.shape[0]:
             raise ValueError("the bounds were made for another page table or another number of key heads")
@@ -262,10 +273,9 @@ def select_pages(q: torch.Tensor, bounds: PageBounds, page_ids: torch.Tensor, le
         raise ValueError(f"the bounds are on {bounds.codes.device}, expected {dev}")
     if bounds.codes.shape[3] != d or heads_kv == 0 or heads_q % heads_kv:
         raise ValueError("q and the bounds differ in head_dim, or the query heads are no multiple of the key heads")
-    if budget < 1 or sink < 0 or recent < 0 or sink + recent > budget:
-        raise ValueError("budget must be at least 1 and at least sink + recent, neither negative")
-    if tokens_per_page <= 0:
-        raise ValueError("tokens_per_page must be positive")
+    if budget < 1 or sink < 0 or recent < 0 or sink + recent > budget or budget > _MOST:
+        raise ValueError("budget must be at least 1, at least sink + recent (neither negative) and fit an int32")
+    _require_tokens_per_page(tokens_per_page)
     if status is not None:
         _require_dense(status, "status", torch.int32, (1,), dev)
     selected, count = page_ids.new_empty((n_seqs, heads_kv, budget)), page_ids.new_empty((n_seqs, heads_kv))
@@ -302,10 +312,9 @@ def evict_pages(page_mass: torch.Tensor, page_ids: torch.Tensor, lengths: torch.
     dev = page_ids.device
     page_ids = _require_lists(page_ids, lengths, n_seqs, dev)
     page_mass = _require_rows(page_mass, "page_mass", torch.float32, (n_seqs, width), dev)
-    if recent < 1 or sink < 0 or sink + recent > budget:
-        raise ValueError("recent must be at least 1, sink not negative, and budget at least sink + recent")
-    if tokens_per_page <= 0:
-        raise ValueError("tokens_per_page must be positive")
+    if recent < 1 or sink < 0 or sink + recent > budget or budget > _MOST:
+        raise ValueError("recent must be at least 1, sink not negative, budget at least sink + recent and fit an int32")
+    _require_tokens_per_page(tokens_per_page)
     ids = page_ids.new_empty
     got = Eviction(ids((n_seqs, width)), page_mass.new_empty((n_seqs, width)), ids(n_seqs), ids((n_seqs, width)), ids(n_seqs))
     if n_seqs:
