@@ -9,6 +9,20 @@
 // batch fill the GPU alike.  A range that reaches into several sequences leaves one
 // partial result per sequence (normalised, with its log2-sum); the join kernel
 // weighs the partials of each sequence by 2^(their log2-sum - the total).
+//
+// A step reads every page once and uses it for one group of query heads (8 of
+// them: 8 operations a byte of bf16, 32 of INT4), so HBM is the bound to aim for,
+// and products of 128 rows are not what is missing: the tensor pipe is 10 to 18 % busy with the 16 x 8 ones used here,
+// whose operands come from codes in registers.  Measured calls, both kernels:
+//   32 x 8192 tokens, 64 / 8 heads of 128:  bf16 185 us (5.8 TB/s, 88 % of a
+//     plain copy's rate), INT8 with page mass 142 us (3.8 TB/s; the copies alone
+//     run at 5.1, the rest is issue and latency)
+//   131071 INT4 tokens, 32 / 8 heads: 75 us (1.9 TB/s; 58 % of the issue slots
+//     are used, 48 % of the ALU's: two tokens' nibbles make one operand word)
+//   24 ragged sequences over bf16, INT8, INT4 and 2-bit pages: 82 us (the four
+//     formats' code does not fit the instruction cache together)
+//   64 sequences, 2 heads of 64, FP8: 32 us, of which about 7 pass before the
+//     first page arrives (lengths, ids, table, page: loads that wait for another)
 #include <algorithm>
 #include <atomic>
 #include <cstdio>
@@ -1151,6 +1165,14 @@ struct Worker {
   }
 };
 
+// Four workers and a producer, 128 registers a thread, three such CTAs on an SM
+// (two with NT = 2).  Why a producer: a worker that copies its own units spent
+// about 240 of 550 instructions for a page and head on look-ups and copies; here
+// eight lanes for each of four workers issue them once (INT8 135 -> 131 us, FP8 31 -> 23).  Why cp.async and
+// not tensor copies: a unit is 1 to 4 KB in runs of 64 to 256 bytes, and one lane
+// per worker issuing boxes measured 129 against 128 us (INT8) and 68 against 63
+// (131071 INT4 tokens).  A ring of three units leaves two on their way: 24 to an
+// SM, 48 to 96 KB, which covers a microsecond of HBM's full rate.
 template <int D, int NT>
 __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_kernel(const __grid_constant__ AttnParams p) {
   using Layout = UnitLayout<D>;
@@ -1284,7 +1306,8 @@ __device__ __forceinline__ float lse2_of(float m, float l) { return (m == -INFIN
 // the warps and added through shared memory.  With mass, then blocks for
 // kMassPages pages of a sequence each: the total log2-sum of every head, then a
 // half warp per page over the heads.  Bound by the latency of three dependent
-// loads.
+// loads; 5 to 10 us.  With 4 warps instead of 8 a call of 2048 rows of 8 partials
+// takes 183.8 instead of 186.5 us, one of 32 rows of 222 partials 84 instead of 77.
 constexpr int kMassPages = 64;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ AttnParams p) {
@@ -1398,7 +1421,10 @@ int ranges_for(int64_t n_seqs, int heads_kv, int q_chunks, int64_t pages_per_lis
   const int64_t fit = std::max<int64_t>(1, int64_t(sms) * per_sm / (int64_t(heads_kv) * q_chunks));
   return int(std::max<int64_t>(1, std::min<int64_t>(fit, n_seqs * pages_per_list)));
 }
-// Query heads of one worker: one or two column tiles.
+// Query heads of one worker: one or two column tiles.  Two read a page once for up to 16 heads of a
+// group but hold twice the sums, so 8 instead of 12 workers fit an SM.  16 x 8192 tokens, 8 key heads:
+// groups of 16 take 135 us (bf16), 114 (INT8), 115 (INT4) with two and 152, 128, 131 as two halves of
+// 8, groups of 10 bf16 125 and 150; groups of 8 take 106, 79, 78 with one and 122, 102, 103 with two.
 int worker_queries(int group) { return group <= 8 ? 8 : 16; }
 int q_chunks_for(int heads_q, int heads_kv) {
   const int group = heads_q / heads_kv, n = worker_queries(group);

@@ -500,12 +500,17 @@ ASHKV_API ashkv_status_t ashkv_page_features(const float* d_token_saliency, cons
  * K and V are the numbers the page's codes stand for: the bf16 values, INT8
  * code * scale / 127, INT4 (nibble - 8) * scale / 7, FP8 the e4m3 number,
  * none rounded to bf16, and for the dithered formats the bf16 values that
- * their decoder gives.  Sums and softmax statistics are fp32.  A sequence
- * without tokens gives 0 and -inf.  Tokens past the length are not used,
- * whatever their page holds.
+ * their decoder gives.  Sums and softmax statistics are fp32.  Over INT8 and
+ * INT4 pages a query enters as whole numbers, exact down to 2^-14 of its
+ * head's largest value and off by at most 2^-22 of that below; a query head
+ * with an element that is not finite gives NaN there.  A weight is rounded
+ * once (fp16 over codes, two bf16 parts over bf16 values).  A sequence without
+ * tokens gives 0 and -inf.  Tokens past the length are not used, whatever
+ * their page holds.
  *   d_selected (may be NULL): [n_seqs, heads_kv, max_selected] page positions;
  *   key head h then attends only positions d_selected[b,h,i], i <
- *   d_selected_count[b,h] (as ashkv_select_pages writes them).
+ *   d_selected_count[b,h] (as ashkv_select_pages writes them; any order, and a
+ *   position that stands there twice counts twice).
  *   d_page_mass (may be NULL, not with d_selected): fp32 [n_seqs, max_pages]
  *   with row stride mass_stride; for each page position j that holds tokens
  *   mass[b,j] = decay * mass[b,j] + sum over h and the page's tokens of P[h,t].
@@ -513,10 +518,11 @@ ASHKV_API ashkv_status_t ashkv_page_features(const float* d_token_saliency, cons
  * its table) is left out and sets ASHKV_FLAG_INDEX_RANGE in *d_status (if
  * given), as does a length or count beyond max_pages / max_selected, which is
  * cut there.  d_q: bf16 with unit element stride and the given strides (in
- * elements); d_out: contiguous bf16; d_lse (may be NULL): fp32 [n_seqs,
+ * elements); d_out: contiguous bf16, which may be d_q itself; d_lse (may be NULL): fp32 [n_seqs,
  * heads_q].  head_dim is 64 or 128; with stores, heads_kv * head_dim and
- * tokens_per_page have the limits of ashkv_migrate_pages.  n_seqs * heads_q
- * is at most 2^24.  d_scratch: ashkv_decode_scratch_floats(...) floats
+ * tokens_per_page have the limits of ashkv_migrate_pages.  A page's rows span
+ * less than 2^31 bytes, heads_q is at most 8192, n_seqs * heads_q at most
+ * 2^24.  d_scratch: ashkv_decode_scratch_floats(...) floats
  * (pages_per_list = max_selected with d_selected, else max_pages), 16-byte
  * aligned, used by this call alone until it has run.
  * ======================================================================== */
@@ -570,7 +576,8 @@ ASHKV_API ashkv_status_t ashkv_decode_attention(
  * and the highest scores up to `budget` (all pages where there are no more;
  * of equal scores the lower position), then -1, and their number to
  * d_selected_count.  A page id outside the bounds table scores -inf and sets
- * ASHKV_FLAG_INDEX_RANGE.  sink + recent <= budget, budget >= 1.
+ * ASHKV_FLAG_INDEX_RANGE.  sink + recent <= budget, budget >= 1; at most 128
+ * query heads to a key head, 65535 key heads and 65535 sequences.
  * d_scratch: ashkv_select_scratch_floats(...) floats.
  * ======================================================================== */
 ASHKV_API ashkv_status_t ashkv_page_bounds(const ashkv_paged_kv_t* kv, const int32_t* d_list, const int32_t* d_count,
