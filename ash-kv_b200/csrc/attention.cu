@@ -14,8 +14,8 @@
 // them: 8 operations a byte of bf16, 32 of INT4), so HBM is the bound to aim for,
 // and products of 128 rows are not what is missing: the tensor pipe is 10 to 18 % busy with the 16 x 8 ones used here,
 // whose operands come from codes in registers.  Measured calls, both kernels:
-//   32 x 8192 tokens, 64 / 8 heads of 128:  bf16 185 us (5.8 TB/s, 88 % of a
-//     plain copy's rate), INT8 with page mass 142 us (3.8 TB/s; the copies alone
+//   32 x 8192 tokens, 64 / 8 heads of 128:  bf16 184 us (5.8 TB/s, 89 % of a
+//     plain copy's rate), INT8 with page mass 137 us (3.9 TB/s; the copies alone
 //     run at 5.1, the rest is issue and latency)
 //   131071 INT4 tokens, 32 / 8 heads: 75 us (1.9 TB/s; 58 % of the issue slots
 //     are used, 48 % of the ALU's: two tokens' nibbles make one operand word)
@@ -1302,77 +1302,117 @@ __device__ __forceinline__ void merge_lse2(float& m, float& l, float m2, float l
 }
 __device__ __forceinline__ float lse2_of(float m, float l) { return (m == -INFINITY ? 0.0f : m) + log2f(l); }
 
-// Blocks 0 .. n_seqs * heads_q - 1: a result row each, its partials spread over
-// the warps and added through shared memory.  With mass, then blocks for
-// kMassPages pages of a sequence each: the total log2-sum of every head, then a
-// half warp per page over the heads.  Bound by the latency of three dependent
-// loads; 5 to 10 us.  With 4 warps instead of 8 a call of 2048 rows of 8 partials
-// takes 183.8 instead of 186.5 us, one of 32 rows of 222 partials 84 instead of 77.
-constexpr int kMassPages = 64;
-template <int D>
-__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int kWarps = kJoinThreads / 32, N = D / 32;
-  extern __shared__ float s_join[];  // [kWarps][D], or [2][heads_q]
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  wait_for_previous();  // the partials
-  const int64_t n_out = int64_t(p.n_seqs) * p.heads_q;
-  if (blockIdx.x < n_out) {
-    const int b = int(blockIdx.x / p.heads_q), hq = int(blockIdx.x % p.heads_q);
-    if (tid == 0 && hq % p.group == 0) {  // what list_len cut
-      const int32_t n = p.selected ? p.selected_count[int64_t(b) * p.heads_kv + hq / p.group] : 0;
-      if (p.lengths[b] != seq_tokens(p, b) || n < 0 || n > p.max_selected) flag(p.status, ASHKV_FLAG_INDEX_RANGE);
+constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kLongRow = 24;  // a row of more partials takes the block's warps together
+
+// A result row, its partials shared by W warps (this one is the first'th; with W = kJoinWarps the
+// block's, added through shared memory s_join [kJoinWarps][D]).
+template <int D, int W>
+__device__ __forceinline__ void join_row(const AttnParams& p, int64_t row, int first, int r0, int r1, float* s_join) {
+  static_assert(W == 1 || W == kJoinWarps, "a row has one warp or the block's");
+  constexpr int N = D / 32;               // channels of a lane
+  constexpr int kAhead = W == 1 ? 6 : 2;  // partials of a warp that are on their way while the total is found
+  const int lane = threadIdx.x & 31;
+  const int b = int(row / p.heads_q), hq = int(row % p.heads_q);
+  if (first == 0 && lane == 0 && hq % p.group == 0) {  // what list_len cut
+    const int32_t n = p.selected ? p.selected_count[int64_t(b) * p.heads_kv + hq / p.group] : 0;
+    if (p.lengths[b] != seq_tokens(p, b) || n < 0 || n > p.max_selected) flag(p.status, ASHKV_FLAG_INDEX_RANGE);
+  }
+  const float* lse = p.part_lse2 + int64_t(b) * p.heads_q + hq;  // + r * heads_q
+  const float* rows = p.part_o + (int64_t(b) * p.heads_q + hq) * D + lane * N;  // + r * heads_q * D
+  const auto load_row = [&](int r, float (&v)[N]) {
+    if constexpr (N == 4) {
+      const float4 f = *reinterpret_cast<const float4*>(rows + int64_t(r) * p.heads_q * D);
+      v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else {
+      const float2 f = *reinterpret_cast<const float2*>(rows + int64_t(r) * p.heads_q * D);
+      v[0] = f.x; v[1] = f.y;
     }
-    int r0, r1;
-    partials_of(p, b, hq / p.group, r0, r1);
-    const float* lse = p.part_lse2 + int64_t(b) * p.heads_q + hq;  // + r * heads_q
-    const float* rows = p.part_o + (int64_t(b) * p.heads_q + hq) * D + lane * N;  // + r * heads_q * D
-    const auto load_row = [&](int r, float (&v)[N]) {
-      if constexpr (N == 4) {
-        const float4 f = *reinterpret_cast<const float4*>(rows + int64_t(r) * p.heads_q * D);
-        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-      } else {
-        const float2 f = *reinterpret_cast<const float2*>(rows + int64_t(r) * p.heads_q * D);
-        v[0] = f.x; v[1] = f.y;
-      }
-    };
-    // this warp's first two rows are on their way while the total is found
-    float v0[N] = {}, v1[N] = {};
-    if (r0 + warp <= r1) load_row(r0 + warp, v0);
-    if (r0 + warp + kWarps <= r1) load_row(r0 + warp + kWarps, v1);
-    float m = -INFINITY, l = 0.0f;
-    for (int r = r0 + lane; r <= r1; r += 32) merge_lse2(m, l, lse[int64_t(r) * p.heads_q], 1.0f);
+  };
+  float ahead[kAhead][N] = {};
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-      merge_lse2(m, l, __shfl_xor_sync(0xFFFFFFFFu, m, off), __shfl_xor_sync(0xFFFFFFFFu, l, off));
-    const float total = lse2_of(m, l);
-    float acc[N] = {};
-    const auto add_row = [&](int r, const float (&v)[N]) {
-      const float x = lse[int64_t(r) * p.heads_q], w = x == -INFINITY ? 0.0f : ex2(x - total);
+  for (int k = 0; k < kAhead; ++k)
+    if (r0 + first + k * W <= r1) load_row(r0 + first + k * W, ahead[k]);
+  float m = -INFINITY, l = 0.0f;
+  for (int r = r0 + lane; r <= r1; r += 32) merge_lse2(m, l, lse[int64_t(r) * p.heads_q], 1.0f);
 #pragma unroll
-      for (int k = 0; k < N; ++k) acc[k] = fmaf(w, v[k], acc[k]);
-    };
-    if (r0 + warp <= r1) add_row(r0 + warp, v0);
-    if (r0 + warp + kWarps <= r1) add_row(r0 + warp + kWarps, v1);
+  for (int off = 16; off > 0; off >>= 1)
+    merge_lse2(m, l, __shfl_xor_sync(0xFFFFFFFFu, m, off), __shfl_xor_sync(0xFFFFFFFFu, l, off));
+  const float total = lse2_of(m, l);
+  float acc[N] = {};
+  const auto add_row = [&](int r, const float (&v)[N]) {
+    const float x = lse[int64_t(r) * p.heads_q], w = x == -INFINITY ? 0.0f : ex2(x - total);
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = fmaf(w, v[k], acc[k]);
+  };
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (r0 + first + k * W <= r1) add_row(r0 + first + k * W, ahead[k]);
 #pragma unroll 4
-    for (int r = r0 + warp + 2 * kWarps; r <= r1; r += kWarps) {
-      float v[N];
-      load_row(r, v);
-      add_row(r, v);
-    }
+  for (int r = r0 + first + kAhead * W; r <= r1; r += W) {
+    float v[N];
+    load_row(r, v);
+    add_row(r, v);
+  }
+  uint16_t* out = p.out + row * D;  // (any alignment of 2 bytes)
+  if constexpr (W == 1) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) s_join[warp * D + lane * N + k] = acc[k];
+    for (int k = 0; k < N; ++k) out[lane * N + k] = f32_to_bf16(acc[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) s_join[first * D + lane * N + k] = acc[k];
     __syncthreads();
-    if (tid < D) {
+    for (int ch = threadIdx.x; ch < D; ch += kJoinThreads) {
       float sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) sum += s_join[w * D + tid];
-      p.out[int64_t(blockIdx.x) * D + tid] = f32_to_bf16(sum);
+      for (int w = 0; w < W; ++w) sum += s_join[w * D + ch];
+      out[ch] = f32_to_bf16(sum);
     }
-    if (tid == 0 && p.lse) p.lse[blockIdx.x] = total * kLn2;
+  }
+  if (first == 0 && lane == 0 && p.lse) p.lse[row] = total * kLn2;
+}
+
+// The first blocks hold the result rows: W = kJoinWarps: a block for each; W = 1: a
+// warp for each, but for the rows of many partials (a long sequence among short
+// ones), which the block's warps then take together, one row after the other.
+// With mass, then blocks for kMassPages pages of a sequence each: the total
+// log2-sum of every head, then a half warp per page over the heads.  Bound by the
+// latency of three dependent loads; 4 to 10 us.
+constexpr int kMassPages = 64;
+template <int D, int W>
+__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int kWarps = kJoinWarps, kRows = kWarps / W;  // rows of a block
+  extern __shared__ float s_join[];  // [kWarps][D], or [heads_q] and [2][kJoinThreads]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  wait_for_previous();  // the partials
+  const int64_t n_out = int64_t(p.n_seqs) * p.heads_q, out_blocks = (n_out + kRows - 1) / kRows;
+  if (blockIdx.x < out_blocks) {
+    // a block's rows lie far apart, so that the heads of one long sequence are in as many blocks
+    const auto row_of = [&](int k) { return int64_t(blockIdx.x) + k * out_blocks; };
+    const auto partials = [&](int64_t row, int& r0, int& r1) {
+      partials_of(p, int(row / p.heads_q), int(row % p.heads_q) / p.group, r0, r1);
+    };
+    int r0 = 0, r1 = -1;
+    if constexpr (W == 1) {
+      const int64_t row = row_of(warp);
+      if (row < n_out) partials(row, r0, r1);
+      const bool split = r1 - r0 >= kLongRow;
+      if (row < n_out && !split) join_row<D, 1>(p, row, 0, r0, r1, s_join);
+      if (!__syncthreads_or(split)) return;
+      for (int k = 0; k < kRows && row_of(k) < n_out; ++k) {
+        partials(row_of(k), r0, r1);
+        if (r1 - r0 < kLongRow) continue;
+        join_row<D, kWarps>(p, row_of(k), warp, r0, r1, s_join);
+        __syncthreads();  // s_join is read before the next row's sums
+      }
+    } else {
+      partials(row_of(0), r0, r1);
+      join_row<D, kWarps>(p, row_of(0), warp, r0, r1, s_join);
+    }
     return;
   }
   const int per = (p.max_pages + kMassPages - 1) / kMassPages;
-  const int64_t mb = int64_t(blockIdx.x) - n_out;
+  const int64_t mb = int64_t(blockIdx.x) - out_blocks;
   const int b = int(mb / per), j0 = int(mb % per) * kMassPages;
   const int pages = int((seq_tokens(p, b) + p.T - 1) / p.T), j1 = min(pages, j0 + kMassPages);
   if (j0 >= j1) return;
@@ -1472,6 +1512,13 @@ ashkv_status_t refuse(const char* what, const char* why) {
   return ASHKV_BAD_ARGUMENT;
 }
 
+// Warps of a result row in the join.  One warp per row makes eight times fewer CTAs and needs no second
+// sum, eight read a row's partials at once.  Calls with one / eight warps, by partials to a row: 1.7 (128 x
+// 1024 bf16 tokens, 64 heads) 109 / 129 us; 3.5 (64 x 2048 INT8) 79 / 88; 7 (32 x 8192 bf16) 183 / 186; 9 (24 x
+// 8192 INT8) 103.8 / 104.4; 14 (16 x 8192 bf16) 106.6 / 105.3; 28 (8 x 8192) 68.9 / 65.7; 111 (2 x 8192) 41 / 33.
+// One sequence of 131072 among 31 of 30 tokens: 219 / 213 (230 if its rows had one warp each).
+int join_warps(const AttnParams& p) { return p.ranges <= int64_t(p.n_seqs) * 10 ? 1 : 8; }
+
 template <int D, int NT>
 ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
   const int64_t workers = int64_t(p.ranges) * p.heads_kv * p.q_chunks;
@@ -1496,13 +1543,16 @@ ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
                     size_t(smem), st, p);
   const ashkv_status_t rc = check_launch("ashkv_decode_attention");
   if (rc != ASHKV_OK) return rc;
-  int64_t blocks = int64_t(p.n_seqs) * p.heads_q;
+  const int64_t rows = int64_t(p.n_seqs) * p.heads_q;
+  const int w = join_warps(p), per_block = kJoinThreads / 32 / w;
+  int64_t blocks = (rows + per_block - 1) / per_block;
   size_t join_smem = kJoinThreads / 32 * D * 4;
   if (p.mass) {
     blocks += int64_t(p.n_seqs) * ((p.max_pages + kMassPages - 1) / kMassPages);
     join_smem = std::max(join_smem, size_t(p.heads_q + 2 * kJoinThreads) * 4);
   }
-  launch_overlapped(decode_join_kernel<D>, dim3(unsigned(blocks)), dim3(kJoinThreads), join_smem, st, p);
+  launch_overlapped(w == 1 ? decode_join_kernel<D, 1> : decode_join_kernel<D, 8>, dim3(unsigned(blocks)), dim3(kJoinThreads),
+                    join_smem, st, p);
   return check_launch("ashkv_decode_attention");
 }
 

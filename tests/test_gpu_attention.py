@@ -166,6 +166,21 @@ def test_decode_many_sequences_and_one_long(cuda, tiers):
     run_case(cuda, tiers, 16, 4, 2, 64, [4001], 5)
 
 
+def test_decode_one_long_sequence_among_short_ones(cuda):
+    """One row of many partial results beside rows of one or two."""
+    T, heads, dim, n = 16, 8, 64, 41
+    c = Cache(cuda, [N.PAGE_BF16] * 375, T, heads, dim, 83)
+    lengths = [(7 * i) % 40 for i in range(n)]
+    lengths[13] = 375 * T - 3
+    ids = np.stack([np.random.default_rng(b).permutation(375) for b in range(n)]).astype(np.int32)
+    q, acc = queries(n, 16, dim, 83), np.zeros((n, 375))
+    mass = torch.zeros(n, 375, device=cuda)
+    out, lse = A.decode_attention(q.to(cuda), c.table, c.kv, None, torch.from_numpy(ids).to(cuda),
+                                  torch.tensor(lengths, dtype=torch.int32, device=cuda), page_mass=mass, return_lse=True)
+    want = O.decode_attention(q.double().numpy(), c.lists(ids, lengths), lengths, T, dim ** -0.5, acc, 1.0)
+    check(out, lse, want, dim, max(lengths), mass, acc, 1.0)
+
+
 @pytest.mark.parametrize("tiers", ["bf16", "int8", "mixed"])
 @pytest.mark.parametrize("std", [1e-3, 30.0])
 def test_decode_value_ranges(cuda, tiers, std):
