@@ -57,7 +57,7 @@ def _refuse(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device
 
 
 def _require_dense(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_cuda:
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device.index:  # (-1 on the host)
         _refuse(t, name, dtype, shape, device)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -66,7 +66,7 @@ def _require_dense(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple,
 def _require_rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> torch.Tensor:
     """[rows, width], dense in its width, with any row stride that keeps rows apart (returned with a
     stride of at least the width: a single row may carry any)."""
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_cuda:
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device.index:  # (-1 on the host)
         _refuse(t, name, dtype, shape, device)
     if t.is_contiguous():
         return t if shape[0] != 1 or t.stride(0) >= shape[1] else t.view(-1).view(shape)

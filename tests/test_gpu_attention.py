@@ -166,6 +166,11 @@ def test_decode_many_sequences_and_one_long(cuda, tiers):
     run_case(cuda, tiers, 16, 4, 2, 64, [4001], 5)
 
 
+@pytest.mark.parametrize("T,lengths", [(1000, [2001, 999, 1]), (65536, [65541])])
+def test_decode_very_large_pages(cuda, T, lengths):
+    run_case(cuda, "bf16", T, 2, 1, 64, lengths, 84)
+
+
 def test_decode_one_long_sequence_among_short_ones(cuda):
     """One row of many partial results beside rows of one or two."""
     T, heads, dim, n = 16, 8, 64, 41
