@@ -257,9 +257,8 @@ def _inputs(case, seed):
 
 def prepare(case, seed):
     s = _inputs(case, seed)
-    if own:
-        s["library"] = _library()
-        s["handle"] = _handle(s) if case["kind"] != "evict" else None
+    if own and case["kind"] != "evict":
+        s["handle"] = _handle(s)
     return s
 
 
@@ -276,7 +275,7 @@ def _library():
 
 def _handle(s):
     """The page table, the pool, the stores and the bounds as a user's program keeps them."""
-    PageBounds = s["library"].PageBounds
+    PageBounds = _library().PageBounds
     from ashkv.runtime.batch import DevicePageTable, KVLayers, TierStore
     case, dev = s["case"], s["q"].device
     f = s["mass"].reshape(-1) if s["case"]["mass"] else s["zeros"].float()
@@ -473,7 +472,7 @@ def run(s):
     case = s["case"]
     if not own:
         return {"decode": _decode, "sparse": _sparse, "bounds": _bounds, "evict": _evict}[case["kind"]](s)
-    A = s["library"]
+    A = _library()
     if case["kind"] == "evict":
         got = A.evict_pages(s["mass"], s["page_ids"], s["lengths"], case["budget"], sink=case["sink"],
                             recent=case["recent"], tokens_per_page=T)
