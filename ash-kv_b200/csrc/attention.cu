@@ -307,7 +307,7 @@ __device__ __noinline__ void decode_nbit(uint32_t unit, const uint8_t* slot, int
     if (lane + 32 * j < n_out) put(entry[j]);
   if (n_out > Raw::kMaxEntries) {
     const uint32_t* ent = reinterpret_cast<const uint32_t*>(slot + nbit_entries_off(2 * int64_t(T) * row_len, BITS));
-    for (uint32_t j = Raw::kMaxEntries + lane; j < n_out; j += 32) put(__ldg(ent + j));
+    for (uint32_t j = Raw::kMaxEntries + lane; j < n_out; j += 32) put(ent[j]);
   }
   __syncwarp();
 }

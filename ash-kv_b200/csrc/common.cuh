@@ -27,7 +27,10 @@ int sm_count();
 // Launches a kernel whose set-up may overlap the kernel before it in the stream
 // (programmatic dependent launch).  Its first statement is wait_for_previous(),
 // which returns once that kernel has completed and its writes are visible, so
-// what it reads and writes is ordered as by a plain launch.
+// what it reads and writes is ordered as by a plain launch.  The kernel is
+// resident while its predecessor still writes, so it promises of nothing that it
+// reads that it does not change: no __restrict__ pointers, no ld.global.nc, no
+// __ldg (a read of that kind may also be moved above the wait).
 template <class... Params, class... Args>
 cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                               Args&&... args) {
@@ -110,6 +113,15 @@ __device__ __forceinline__ float f16_to_f32(uint16_t h) {
   return __half2float(__ushort_as_half(h));
 }
 
+// 16 bytes of data that an earlier kernel may have written while this one was resident (and
+// that this one does not write: volatile keeps it behind the wait, nothing else is ordered).
+__device__ __forceinline__ uint4 ld_v4(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
 // Streaming 16-byte load through the non-coherent path (data read once).
 __device__ __forceinline__ uint4 ld_nc_v4(const void* p) {
   uint4 r;

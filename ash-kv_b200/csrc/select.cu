@@ -110,11 +110,11 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsParams p) 
       for (; t + 8 <= nt; t += 8) {
         uint4 v[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = ld_nc_v4(row + (t + u) * p.row_stride);
+        for (int u = 0; u < 8; ++u) v[u] = ld_v4(row + (t + u) * p.row_stride);
 #pragma unroll
         for (int u = 0; u < 8; ++u) take(v[u]);
       }
-      for (; t < nt; ++t) take(ld_nc_v4(row + t * p.row_stride));
+      for (; t < nt; ++t) take(ld_v4(row + t * p.row_stride));
     }
     float a[8], b[8], amax = 0.0f;
 #pragma unroll
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32) select_scores_kernel(const S
     const int8_t* c = p.codes + (int64_t(ok[u] ? id[u] : 0) * p.heads + h) * 2 * D + t * 16;
 #pragma unroll
     for (int k = 0; k < kChunks / 4; ++k)
-      w[u][k] = ok[u] ? ld_nc_v4(c + 64 * k) : make_uint4(0, 0, 0, 0);
+      w[u][k] = ok[u] ? ld_v4(c + 64 * k) : make_uint4(0, 0, 0, 0);
   }
   int e_mine[2];
 #pragma unroll
@@ -353,7 +353,7 @@ __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* s_warp, ui
 // rows (evict) 32.2 and 34.8; the same at 2048.
 constexpr int kCached = 8;
 template <bool CACHED, class Emit>
-__device__ void keep_highest(const float* __restrict__ score, int n, int budget, int sink, int recent, KeepShared& sm,
+__device__ void keep_highest(const float* score, int n, int budget, int sink, int recent, KeepShared& sm,
                              Emit emit) {
   static_assert(kKeepWarps == 32, "scan_before takes 32 warps");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -481,11 +481,10 @@ __device__ __forceinline__ void keep_highest_of(const float* score, int n, int b
   else keep_highest<false>(score, n, budget, sink, recent, sm, emit);
 }
 
-__global__ void __launch_bounds__(kKeepThreads, 2) select_keep_kernel(const float* __restrict__ scores,
-                                                                   const int32_t* __restrict__ lengths, int heads,
-                                                                   int max_pages, int T, int budget, int sink,
-                                                                   int recent, int32_t* __restrict__ selected,
-                                                                   int32_t* __restrict__ count, uint32_t* status) {
+__global__ void __launch_bounds__(kKeepThreads, 2) select_keep_kernel(const float* scores, const int32_t* lengths,
+                                                                      int heads, int max_pages, int T, int budget,
+                                                                      int sink, int recent, int32_t* selected,
+                                                                      int32_t* count, uint32_t* status) {
   __shared__ KeepShared sm;
   const int64_t row = blockIdx.x;
   const int b = int(row / heads);
@@ -505,10 +504,9 @@ __global__ void __launch_bounds__(kKeepThreads, 2) select_keep_kernel(const floa
 }
 
 __global__ void __launch_bounds__(kKeepThreads, 2) evict_kernel(
-    const float* __restrict__ mass, int64_t mass_stride, const int32_t* __restrict__ page_ids, int64_t page_ids_stride,
-    const int32_t* __restrict__ lengths, int max_pages, int T, int budget, int sink, int recent,
-    int32_t* __restrict__ out_ids, float* __restrict__ out_mass, int32_t* __restrict__ out_lengths,
-    int32_t* __restrict__ evicted, int32_t* __restrict__ evicted_count) {
+    const float* mass, int64_t mass_stride, const int32_t* page_ids, int64_t page_ids_stride, const int32_t* lengths,
+    int max_pages, int T, int budget, int sink, int recent, int32_t* out_ids, float* out_mass, int32_t* out_lengths,
+    int32_t* evicted, int32_t* evicted_count) {
   __shared__ KeepShared sm;
   const int64_t b = blockIdx.x;
   wait_for_previous();
@@ -519,11 +517,13 @@ __global__ void __launch_bounds__(kKeepThreads, 2) evict_kernel(
   float* om = out_mass + b * max_pages;
   int32_t* ev = evicted + b * max_pages;
   keep_highest_of(m, n, budget, sink, recent, sm, [&](int j, bool kept, int at) {
+    const int32_t id = ids[j];  // both loads before a store that they might have to wait for
+    const float x = m[j];
     if (kept) {
-      oi[at] = ids[j];
-      om[at] = m[j];
+      oi[at] = id;
+      om[at] = x;
     } else {
-      ev[at] = ids[j];
+      ev[at] = id;
     }
   });
   const int kept = min(n, budget), gone = n - kept;

@@ -817,3 +817,44 @@ def test_results_do_not_depend_on_the_run(cuda):
         got = (*A.decode_attention(q, c.table, c.kv, c.stores, ids, L, page_mass=mass, return_lse=True), mass)
         first = first or got
         assert all(torch.equal(x, y) for x, y in zip(got, first))
+
+
+def test_inputs_written_by_the_kernel_before(cuda):
+    """Each call right behind the kernel that writes what it reads (lengths, mass, bounds, scores),
+    many times over, against the same calls with the device idle in between."""
+    T, heads, dim, P, B = 16, 2, 128, 600, 4
+    c = Cache(cuda, [N.PAGE_BF16] * 64, T, heads, dim, 90)
+    g = torch.Generator().manual_seed(90)
+    ids = torch.randint(0, 64, (B, P), generator=g).to(torch.int32).to(cuda)
+    q = queries(B, 8, dim, 90).to(cuda)
+    rounds = 12
+    lengths = torch.randint(1, P * T, (rounds, B), generator=g).to(torch.int32).to(cuda)
+    masses = torch.rand(rounds, B, P, generator=g).to(cuda)
+    lists = torch.stack([torch.randperm(64, generator=g) for _ in range(rounds)]).to(torch.int32).to(cuda)
+
+    def run(wait):
+        L, mass = torch.zeros(B, dtype=torch.int32, device=cuda), torch.zeros(B, P, device=cuda)
+        bounds, got = A.PageBounds.empty(64, heads, dim, cuda), []
+        pause = torch.cuda.synchronize if wait else (lambda: None)
+        for r in range(rounds):
+            L.copy_(lengths[r]), mass.copy_(masses[r])
+            pause()
+            got.append(tuple(A.evict_pages(mass, ids, L, 40)))
+            c.kv.k[0].neg_(), c.kv.k[1].neg_()
+            pause()
+            bounds.update(c.table, c.kv, lists[r])
+            pause()
+            sel, cnt = A.select_pages(q, bounds, ids, L, 33)
+            pause()
+            got.append((sel, cnt, A.decode_attention(q, c.table, c.kv, None, ids, L, selected=sel, selected_count=cnt)))
+            pause()
+            got.append((A.decode_attention(q, c.table, c.kv, None, ids, L, page_mass=mass), mass.clone()))
+            pause()
+            got.append(tuple(A.evict_pages(mass, ids, L, 40)))
+            pause()
+        torch.cuda.synchronize()
+        return got
+
+    want, got = run(True), run(False)  # an even number of sign changes: both start from the same keys
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))

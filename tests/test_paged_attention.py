@@ -3,6 +3,8 @@ host tensors, and the oracle's own consistency."""
 from __future__ import annotations
 
 import ctypes
+import re
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -145,3 +147,18 @@ def test_oracle_keeps_by_score_then_position():
     assert O.keep_highest(s, 5, 1, 1) == [0, 2, 3, 5, 6]
     assert O.keep_highest(s, 6, 1, 1) == [0, 1, 2, 3, 5, 6]
     assert O.keep_highest(s, 1, 0, 1) == [6]
+
+
+def test_overlapped_kernels_promise_nothing_of_what_they_read():
+    """A kernel launched by launch_overlapped is resident while its predecessor still writes: no
+    pointer of its file is __restrict__ and no load takes the path of data that never changes."""
+    csrc = Path(__file__).resolve().parent.parent / "ash-kv_b200" / "csrc"
+    seen = 0
+    for f in sorted(csrc.glob("*.cu")):
+        code = re.sub(r"//[^\n]*", "", f.read_text())
+        if "launch_overlapped(" not in code:
+            continue
+        seen += 1
+        for word in ("__restrict__", "ld_nc", "__ldg", "ld.global.nc"):
+            assert word not in code, f"{f.name}: {word}"
+    assert seen == 2
