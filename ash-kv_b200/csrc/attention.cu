@@ -41,6 +41,8 @@ constexpr uint32_t kPolls = 1u << 24;  // bounded mbarrier waits
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kJoinThreads = 256;
+// Entries of all lists of a call: what is added to a position (ranges, a batch looked up ahead) stays inside an int.
+constexpr int64_t kMostEntries = 0x7FFFFFFFLL - 65536;
 
 struct AttnParams {
   // pages
@@ -1583,7 +1585,7 @@ extern "C" ashkv_status_t ashkv_decode_attention(
     return refuse(kName, "negative size, or heads_q not a multiple of heads_kv");
   if (int64_t(n_seqs) * heads_q > (int64_t(1) << 24) || heads_q > 8192) return refuse(kName, "too many query rows");
   const int64_t width = d_selected ? max_selected : max_pages;
-  if (width < 0 || int64_t(n_seqs) * width > 0x7FFFFFFFLL || int64_t(n_seqs) * max_pages > 0x7FFFFFFFLL)
+  if (width < 0 || int64_t(n_seqs) * width > kMostEntries || int64_t(n_seqs) * max_pages > kMostEntries)
     return refuse(kName, "too many list entries");
   if (d_selected && (!d_selected_count || d_page_mass)) return refuse(kName, "d_selected needs its counts and takes no mass");
   if (n_seqs == 0) return ASHKV_OK;

@@ -522,7 +522,8 @@ ASHKV_API ashkv_status_t ashkv_page_features(const float* d_token_saliency, cons
  * heads_q].  head_dim is 64 or 128; with stores, heads_kv * head_dim and
  * tokens_per_page have the limits of ashkv_migrate_pages.  A page's rows span
  * less than 2^31 bytes, heads_q is at most 8192, n_seqs * heads_q at most
- * 2^24.  d_scratch: ashkv_decode_scratch_floats(...) floats
+ * 2^24, n_seqs * max_pages and n_seqs * max_selected at most 2^31 - 1 - 2^16.
+ * d_scratch: ashkv_decode_scratch_floats(...) floats
  * (pages_per_list = max_selected with d_selected, else max_pages), 16-byte
  * aligned, used by this call alone until it has run.
  * ======================================================================== */

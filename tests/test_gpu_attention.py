@@ -858,3 +858,22 @@ def test_inputs_written_by_the_kernel_before(cuda):
     want, got = run(True), run(False)  # an even number of sign changes: both start from the same keys
     for a, b in zip(want, got):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_decode_the_longest_list(cuda):
+    """2^31 - 1 - 2^16 pages of one token; all but the last entry weigh e^-64."""
+    most, dim = 2 ** 31 - 1 - 2 ** 16, 64
+    k, v = (torch.zeros(2, 1, dim, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    k[1], v[0] = 8.0, 1.0
+    v[1] = torch.arange(dim).to(v)
+    table = DevicePageTable.empty(2, cuda)
+    table.token_start[1] = 1
+    ids = torch.zeros(1, most, dtype=torch.int32, device=cuda)
+    ids[0, -1] = 1
+    L, status = torch.tensor([most], dtype=torch.int32, device=cuda), torch.zeros(1, dtype=torch.int32, device=cuda)
+    out, lse = A.decode_attention(torch.ones(1, 1, dim, dtype=torch.bfloat16, device=cuda), table, KVLayers([k], [v]),
+                                  None, ids, L, tokens_per_page=1, return_lse=True, status=status)
+    # the other entries weigh less than 2^31 e^-64 = 2^(31 - 92.33) < 2^-61 together, their values are at most 1, and
+    # v[1]'s whole numbers are bf16 numbers; lse: log2(e), ln 2 and two products are rounded
+    assert int(status) == 0 and ((out[0, 0].double() - v[1, 0].double()).abs() <= 2.0 ** -61).all()
+    assert abs(float(lse) - 64.0) <= 8 * U * 64.0

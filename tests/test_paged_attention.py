@@ -162,3 +162,12 @@ def test_overlapped_kernels_promise_nothing_of_what_they_read():
         for word in ("__restrict__", "ld_nc", "__ldg", "ld.global.nc"):
             assert word not in code, f"{f.name}: {word}"
     assert seen == 2
+
+
+def test_decode_refuses_lists_whose_positions_leave_an_int():
+    most = 2 ** 31 - 1 - 2 ** 16
+    for n, pages in ((1, 2 ** 31 - 1), (1, most + 1), (16, most // 16 + 1)):
+        assert decode(desc(), n=n, pages=pages, ids_stride=pages) == N.BAD_ARGUMENT
+        assert b"too many list entries" in N.lib().ashkv_last_error()
+        assert decode(desc(), n=n, sel=X, cnt=X, width=pages) == N.BAD_ARGUMENT
+        assert b"too many list entries" in N.lib().ashkv_last_error()
