@@ -146,6 +146,7 @@ __device__ __forceinline__ void mma16832(int (&d)[4], const uint4& a, uint32_t b
     ASHKV_MMA("m16n8k32.row.col.s32.s8.s8.s32", "{%0,%1,%2,%3}", : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -701,27 +702,31 @@ struct Worker {
       const uint32_t k8 = uint32_t(lane * N) >> 3, w8 = (uint32_t(lane * N) & 7u) >> 1;
 #pragma unroll
       for (int k = 0; k < N; k += 2) sts32(qb + q_word(n, k8, w8 + k / 2, false), uint32_t(x[k]) | (uint32_t(x[k + 1]) << 16));
-      // the exponent of the largest value, kept where 2^+-(e + 22) are normal numbers
-      const int e = min(100, max(-100, int(__float_as_uint(amax) >> 23) - 127));
-      const float unit = __uint_as_float(uint32_t(127 + e) << 23), inv = __uint_as_float(uint32_t(127 - e) << 23);
+      // the exponent e of the largest value; powers of two around it in two factors, as 2^+-(e + 21) may
+      // be no fp32 numbers.  The first takes the values to 2^(e / 2): exact, or nothing is left of values below
+      // 2^-126 of the largest.
+      const int e = max(int(__float_as_uint(amax) >> 23) - 127, -126), e1 = e >> 1, e2 = e - e1;
+      const float up = pow2(e1), down = pow2(-e1);
       const bool mine = (n & 7) == g;
       if (p.fp8_pages) {
         // the largest value to [2^14, 2^15): fp16 then keeps all 8 bits of every value down to
         // 2^-31 of it, exactly
-        if (mine) qs_h[half] = p.scale2 * unit * 0x1p-14f;
-        const float down = inv * 0x1p14f;
+        if (mine) qs_h[half] = p.scale2 * up * pow2(e2 - 14);
+        const float down2 = pow2(14 - e2);
 #pragma unroll
         for (int k = 0; k < N; k += 2)
-          sts32(qh + q_word(n, k8, w8 + k / 2, true), f32x2_to_f16x2(bf16_to_f32(x[k]) * down, bf16_to_f32(x[k + 1]) * down));
+          sts32(qh + q_word(n, k8, w8 + k / 2, true),
+                f32x2_to_f16x2(bf16_to_f32(x[k]) * down * down2, bf16_to_f32(x[k + 1]) * down * down2));
       }
       if (p.int_pages) {
         // whole numbers below 2^22 as digits of base 256 in [-128, 127] (the highest at most 64): exact
         // down to 2^-14 of the largest value, off by at most 2^-22 of it below
-        if (mine) qs_i[half] = whole ? p.scale2 * unit * 0x1p-21f : NAN;
+        if (mine) qs_i[half] = whole ? p.scale2 * up * pow2(e2 - 21) : NAN;
+        const float down2 = pow2(21 - e2);
         uint32_t d[3] = {0, 0, 0};
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-          const int v = __float2int_rn(bf16_to_f32(x[k]) * (inv * 0x1p21f));
+          const int v = __float2int_rn(bf16_to_f32(x[k]) * down * down2);
           const int v1 = (v + 128) >> 8, v2 = (v1 + 128) >> 8;
           d[0] |= uint32_t(v2 & 255) << (8 * k);
           d[1] |= uint32_t(v1 & 255) << (8 * k);

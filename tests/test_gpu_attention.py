@@ -877,3 +877,20 @@ def test_decode_the_longest_list(cuda):
     # v[1]'s whole numbers are bf16 numbers; lse: log2(e), ln 2 and two products are rounded
     assert int(status) == 0 and ((out[0, 0].double() - v[1, 0].double()).abs() <= 2.0 ** -61).all()
     assert abs(float(lse) - 64.0) <= 8 * U * 64.0
+
+
+@pytest.mark.parametrize("heads_q", [8, 12])
+@pytest.mark.parametrize("tiers,power", [(t, e) for t in FORMATS for e in (110, -110)] +
+                         [(t, e) for t in ("int8", "fp8", "int4") for e in (125, -125)])
+def test_decode_queries_of_any_size(cuda, tiers, power, heads_q):
+    """Queries near either end of bf16's range, brought back by the scale (bf16 keys stay where
+    an fp32 sum of products does not overflow)."""
+    T, heads, dim = 16, 1, 128
+    c = Cache(cuda, [FORMATS[tiers][i % len(FORMATS[tiers])] for i in range(8)], T, heads, dim, 91)
+    ids = np.arange(8, dtype=np.int32).reshape(1, 8)
+    q = queries(1, heads_q, dim, 91).float().mul(2.0 ** power).bfloat16()
+    assert torch.isfinite(q).all()
+    scale = 0.05 * 2.0 ** -power
+    out, lse = A.decode_attention(q.to(cuda), c.table, c.kv, c.stores, torch.from_numpy(ids).to(cuda),
+                                  torch.tensor([120], dtype=torch.int32, device=cuda), scale=scale, return_lse=True)
+    check(out, lse, O.decode_attention(q.double().numpy(), c.lists(ids, [120]), [120], T, scale), dim, 120)
