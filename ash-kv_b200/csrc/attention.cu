@@ -1095,14 +1095,11 @@ struct Worker {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          const float z = dot_value(a, n, y);
-          s[n][y] = k ? fmaf(z, ks[k][y], s[n][y]) : z * ks[k][y];
+          // (the factor of the query meets the scale first: a product of up to 2^35 and a scale above 2^93 would overflow)
+          const float z = dot_value(a, n, y), f = ks[k][y] * (qs_i[n] * (0.0625f * kUnit4));
+          s[n][y] = k ? fmaf(z, f, s[n][y]) : z * f;
         }
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int y = 0; y < 4; ++y) s[n][y] *= qs_i[n] * (0.0625f * kUnit4);
     tile += 8 * D;
     // V is on its way from shared memory while the scores become weights
     uint32_t raw[K][4];

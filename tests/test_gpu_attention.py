@@ -894,3 +894,19 @@ def test_decode_queries_of_any_size(cuda, tiers, power, heads_q):
     out, lse = A.decode_attention(q.to(cuda), c.table, c.kv, c.stores, torch.from_numpy(ids).to(cuda),
                                   torch.tensor([120], dtype=torch.int32, device=cuda), scale=scale, return_lse=True)
     check(out, lse, O.decode_attention(q.double().numpy(), c.lists(ids, [120]), [120], T, scale), dim, 120)
+
+
+@pytest.mark.parametrize("heads_q", [8, 12])
+@pytest.mark.parametrize("kinds", [[N.PAGE_INT4] * 3, [N.PAGE_INT4, N.PAGE_BF16, N.PAGE_NBIT2], [N.PAGE_NBIT4] * 2])
+def test_decode_large_keys(cuda, kinds, heads_q):
+    """Keys around 2^97, brought back by the scale."""
+    T, heads, dim, scale = 16, 1, 128, 0.5 * 2.0 ** -97
+    g = torch.Generator().manual_seed(92)
+    pages = torch.randn(len(kinds), 2, T * heads * dim, generator=g)
+    pages[:, 0] *= 2.0 ** 97
+    c = Cache(cuda, kinds, T, heads, dim, 92, pool_bits=bits(pages.reshape(len(kinds), -1).to(torch.bfloat16)))
+    ids, lengths = np.arange(len(kinds), dtype=np.int32)[None], [len(kinds) * T - 3]
+    q = queries(1, heads_q, dim, 92)
+    out, lse = A.decode_attention(q.to(cuda), c.table, c.kv, c.stores, torch.from_numpy(ids).to(cuda),
+                                  torch.tensor(lengths, dtype=torch.int32, device=cuda), scale=scale, return_lse=True)
+    check(out, lse, O.decode_attention(q.double().numpy(), c.lists(ids, lengths), lengths, T, scale), dim, lengths[0])
