@@ -817,8 +817,10 @@ struct Worker {
     if (!__any_sync(0xFFFFFFFFu, fresh || x * c > 128.0f)) return;
     const float top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, x > 0.0f ? __float_as_uint(x) : 0u));
     if (top > 0.0f && top < INFINITY) {  // c * top to [2^6, 2^7)
-      // (c stops at 2^60, where BF16 values up to 2^60 still fit beside it: scales below 2^-54 are off by up to 2^-85)
-      const int e = max(int(__float_as_uint(top) >> 23), 73);
+      // (c stops at 2^37, which the smallest scales that the codecs write need, 1e-8 and the least fp16 above 0, so
+      // that n weights of up to 2^8 have room beside it for BF16 values up to 2^83 / n; a scale below that is off by
+      // up to 2^-62 a token)
+      const int e = max(int(__float_as_uint(top) >> 23), 96);
       const float next = __uint_as_float(uint32_t(254 + 6 - e) << 23);
       const float f = next / c;  // a power of two
 #pragma unroll

@@ -504,8 +504,12 @@ ASHKV_API ashkv_status_t ashkv_page_features(const float* d_token_saliency, cons
  * INT4 pages a query enters as whole numbers, exact down to 2^-14 of its
  * head's largest value and off by at most 2^-22 of that below; a query head
  * with an element that is not finite gives NaN there.  A weight is rounded
- * once (fp16 over codes, two bf16 parts over bf16 values).  A sequence without
- * tokens gives 0 and -inf.  Tokens past the length are not used, whatever
+ * once (fp16 over codes, two bf16 parts over bf16 values).  Values are summed
+ * before they are divided by the sum of the weights, which n values of up to
+ * 2^127 / n pass; in a list that also has INT8, FP8 or INT4 pages bf16 and
+ * dithered values up to 2^83 / n do, larger ones may overflow.  A V scale there
+ * that is smaller than the codecs write (below 1e-8) is off by up to 2^-62 a
+ * token.  A sequence without tokens gives 0 and -inf.  Tokens past the length are not used, whatever
  * their page holds.
  *   d_selected (may be NULL): [n_seqs, heads_kv, max_selected] page positions;
  *   key head h then attends only positions d_selected[b,h,i], i <

@@ -910,3 +910,59 @@ def test_decode_large_keys(cuda, kinds, heads_q):
     out, lse = A.decode_attention(q.to(cuda), c.table, c.kv, c.stores, torch.from_numpy(ids).to(cuda),
                                   torch.tensor(lengths, dtype=torch.int32, device=cuda), scale=scale, return_lse=True)
     check(out, lse, O.decode_attention(q.double().numpy(), c.lists(ids, lengths), lengths, T, scale), dim, lengths[0])
+
+
+def run_shared(dev, c, heads_q, lengths, seed, ids=None, decay=0.75, scale=None):
+    """Sequences over few pages that they share, so many list entries that a worker has several to
+    attend one after the other (at most 12 workers on each of 148 SMs for all key heads)."""
+    P = max(-(-x // c.T) for x in lengths)
+    entries, workers = sum(-(-x // c.T) for x in lengths), 12 * torch.cuda.get_device_properties(dev).multi_processor_count
+    assert entries >= 3 * (workers // c.heads)
+    g = np.random.default_rng(seed)
+    if ids is None:
+        ids = g.integers(0, len(c.formats), (len(lengths), P)).astype(np.int32)
+    q, acc = queries(len(lengths), heads_q, c.dim, seed), g.random((len(lengths), P), dtype=np.float32)
+    mass, status = torch.from_numpy(acc.copy()).to(dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    scale = c.dim ** -0.5 if scale is None else scale
+    out, lse = A.decode_attention(q.to(dev), c.table, c.kv, c.stores, torch.from_numpy(ids).to(dev),
+                                  torch.tensor(lengths, dtype=torch.int32, device=dev), tokens_per_page=c.T, scale=scale,
+                                  page_mass=mass, decay=decay, return_lse=True, status=status)
+    assert int(status) == 0
+    want = O.decode_attention(q.double().numpy(), c.lists(ids, lengths), lengths, c.T, scale, acc, decay)
+    check(out, lse, want, c.dim, max(lengths) + 1, mass, acc, decay)
+
+
+def far_apart(dev, kinds, sizes):
+    T, heads, dim = 16, 16, 128
+    g = torch.Generator().manual_seed(93)
+    pages = torch.randn(len(kinds), 2, T * heads * dim, generator=g)
+    pages[:, 1] *= torch.tensor(sizes)[:, None]
+    return Cache(dev, kinds, T, heads, dim, 93, pool_bits=bits(pages.reshape(len(kinds), -1).to(torch.bfloat16)))
+
+
+@pytest.mark.parametrize("group", [1, 12])
+@pytest.mark.parametrize("kinds,sizes", [
+    ([N.PAGE_BF16, N.PAGE_INT4], [2.0 ** 70, 2.0 ** -40]), ([N.PAGE_INT8, N.PAGE_NBIT4], [1e-5, 2.0 ** 70]),
+    ([N.PAGE_NBIT2, N.PAGE_INT8, N.PAGE_BF16], [2.0 ** 70, 1e-5, 1.0]),
+    ([N.PAGE_INT4, N.PAGE_BF16, N.PAGE_INT4], [1e-8, 2.0 ** 62, 2.0 ** 100]),
+    ([N.PAGE_INT4, N.PAGE_BF16, N.PAGE_INT4], [1e-7, 1e15, 1.0]), ([N.PAGE_INT4] * 3, [3e35, 1e-7, 1e35]),
+    ([N.PAGE_INT4, N.PAGE_FP8, N.PAGE_FP8], [1e-7, 1e2, 1.0]), ([N.PAGE_BF16] * 2, [2.0 ** 100, 2.0 ** -60])])
+def test_decode_values_of_far_apart_sizes_of_one_worker(cuda, kinds, sizes, group):
+    """The power of two that small scales need leaves room for the values of other pages, before and behind them."""
+    c = far_apart(cuda, kinds, sizes)
+    ids = (np.arange(36 * 10) % len(kinds)).astype(np.int32).reshape(36, 10)
+    run_shared(cuda, c, 16 * group, [157] * 36, 93, ids)
+
+
+@pytest.mark.parametrize("group", [1, 12])
+@pytest.mark.parametrize("first", [0, 1])
+def test_decode_scales_smaller_than_a_codec_writes(cuda, first, group):
+    """INT4 V scales of 2^-60 beside bf16 values of 2^70."""
+    T, heads, dim = 16, 16, 128
+    c = far_apart(cuda, [N.PAGE_INT4, N.PAGE_BF16], [1.0, 2.0 ** 70])
+    slot = c.stores[TIER[N.PAGE_INT4]].slot_view()[int(c.table.slot[0])]
+    row = heads * dim
+    slot[T * row // 32:2 * T * row // 32].view(torch.bfloat16).fill_(2.0 ** -60)
+    c.values[0] = O.page_values(N.PAGE_INT4, slot.cpu().numpy(), T, heads, dim)
+    ids = ((first + np.arange(36 * 10)) % 2).astype(np.int32).reshape(36, 10)
+    run_shared(cuda, c, heads * group, [157] * 36, 94, ids)
