@@ -157,6 +157,11 @@ __device__ __forceinline__ uint32_t f32x2_to_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+__device__ __forceinline__ uint32_t f32x2_to_bf16x2_down(float lo, float hi) {  // toward zero
+  uint32_t r;
+  asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 __device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -885,7 +890,8 @@ struct Worker {
     weights(s, rows);
   }
   // Adds a tile of BF16 values: the weights in two bf16 parts (8 + 8 bits), as a single one would
-  // cost as much accuracy as the rounding of the result.
+  // cost as much accuracy as the rounding of the result.  Both parts of a weight are above 0 (the lower one
+  // at least 2^-17 of it), so that an infinite value stays what it is.
   __device__ __forceinline__ void bf16_values(uint32_t tile, const float (&s)[NT][4]) {
     uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
@@ -893,8 +899,8 @@ struct Worker {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float x0 = s[n][2 * h] * c, x1 = s[n][2 * h + 1] * c;
-        hi[n][h] = f32x2_to_bf16x2(x0, x1);
-        lo[n][h] = f32x2_to_bf16x2(x0 - bf16lo(hi[n][h]), x1 - bf16hi(hi[n][h]));
+        hi[n][h] = f32x2_to_bf16x2_down(x0, x1);
+        lo[n][h] = f32x2_to_bf16x2(fmaxf(x0 - bf16lo(hi[n][h]), x0 * 0x1p-17f), fmaxf(x1 - bf16hi(hi[n][h]), x1 * 0x1p-17f));
       }
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {

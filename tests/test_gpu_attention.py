@@ -966,3 +966,25 @@ def test_decode_scales_smaller_than_a_codec_writes(cuda, first, group):
     c.values[0] = O.page_values(N.PAGE_INT4, slot.cpu().numpy(), T, heads, dim)
     ids = ((first + np.arange(36 * 10)) % 2).astype(np.int32).reshape(36, 10)
     run_shared(cuda, c, heads * group, [157] * 36, 94, ids)
+
+
+@pytest.mark.parametrize("heads_q", [2, 12])
+@pytest.mark.parametrize("at", [0, 3, 21])
+def test_decode_an_infinite_value_stays_infinite(cuda, at, heads_q):
+    """... in its channel; beside one of the other sign it gives NaN."""
+    c = Cache(cuda, [N.PAGE_BF16] * 2, 16, 1, 64, 8)
+    ids = torch.arange(2, dtype=torch.int32, device=cuda).view(1, 2)
+    L = torch.tensor([30], dtype=torch.int32, device=cuda)
+    q = queries(1, heads_q, 64, 8).to(cuda)
+    where = [(c.kv.v[int(c.table.layer[p])], int(c.table.token_start[p])) for p in range(2)]
+    want = A.decode_attention(q, c.table, c.kv, None, ids, L)
+    v, s = where[at // 16]
+    v[s + at % 16, 0, 5], v[s + at % 16, 0, 9] = float("inf"), -float("inf")
+    out = A.decode_attention(q, c.table, c.kv, None, ids, L)
+    assert (out[..., 5] == float("inf")).all() and (out[..., 9] == -float("inf")).all()
+    rest = [d for d in range(64) if d not in (5, 9)]
+    assert torch.equal(out[..., rest], want[..., rest])
+    v, s = where[0]
+    v[s + 7, 0, 5] = -float("inf")
+    out = A.decode_attention(q, c.table, c.kv, None, ids, L)
+    assert torch.isnan(out[..., 5]).all() and (out[..., 9] == -float("inf")).all()
