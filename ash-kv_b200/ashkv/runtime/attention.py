@@ -119,6 +119,9 @@ def _pages_desc(table: DevicePageTable, kv: KVLayers, stores: Optional[Mapping[i
     """The ashkv_paged_kv_t of a table, its pool and its stores, and the store array it points to."""
     if kv.row_len % head_dim:
         raise ValueError(f"the pool's rows of {kv.row_len} values are no whole number of heads of {head_dim}")
+    pool = kv.k[0].shape
+    if len(pool) > 2 and pool[-1] != head_dim:
+        raise ValueError(f"the pool's heads have {pool[-1]} channels, not {head_dim}")
     n = table.tier.numel()
     _require_dense(table.tier, "table.tier", torch.int8, (n,), device)
     _require_dense(table.layer, "table.layer", torch.int32, (n,), device)

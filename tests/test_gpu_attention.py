@@ -988,3 +988,15 @@ def test_decode_an_infinite_value_stays_infinite(cuda, at, heads_q):
     v[s + 7, 0, 5] = -float("inf")
     out = A.decode_attention(q, c.table, c.kv, None, ids, L)
     assert torch.isnan(out[..., 5]).all() and (out[..., 9] == -float("inf")).all()
+
+
+def test_refuses_heads_of_another_size_than_the_pools(cuda):
+    c = Cache(cuda, [N.PAGE_BF16], 16, 2, 128, 61)
+    ids, L = torch.zeros(1, 1, dtype=torch.int32, device=cuda), torch.tensor([16], dtype=torch.int32, device=cuda)
+    with pytest.raises(ValueError, match="128 channels"):
+        A.decode_attention(queries(1, 4, 64, 61).to(cuda), c.table, c.kv, None, ids, L)
+    with pytest.raises(ValueError, match="128 channels"):
+        A.PageBounds.empty(1, 4, 64, cuda).update(c.table, c.kv, ids[0])
+    flat = KVLayers([k.view(k.shape[0], -1) for k in c.kv.k], [v.view(v.shape[0], -1) for v in c.kv.v])  # rows as one
+    q = queries(1, 4, 128, 61).to(cuda)
+    assert torch.equal(A.decode_attention(q, c.table, flat, None, ids, L), A.decode_attention(q, c.table, c.kv, None, ids, L))
