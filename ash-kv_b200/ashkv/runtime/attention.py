@@ -137,6 +137,10 @@ def _pages_desc(table: DevicePageTable, kv: KVLayers, stores: Optional[Mapping[i
             raise ValueError(f"tier {t} cannot have a store")
         if s.data.device != device:
             raise ValueError(f"the store of tier {t} is on {s.data.device}, expected {device}")
+        if s.tokens_per_page != tokens_per_page or s.row_len != kv.row_len:
+            raise _native.KernelError("tier store", _native.BAD_ARGUMENT,
+                                      f"the store of tier {t} was laid out for pages of {s.tokens_per_page} x {s.row_len}, "
+                                      f"not {tokens_per_page} x {kv.row_len}")
         if s.data.numel() * s.data.element_size() < s.n_slots * s.slot_bytes:
             raise ValueError(f"the store of tier {t} holds fewer than its {s.n_slots} slots")
         descs[int(t)] = s.desc()

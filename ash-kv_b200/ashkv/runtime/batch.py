@@ -125,6 +125,7 @@ class TierStore(SlotArena):
         super().__init__(n_slots, need, device)
         self.format = fmt
         self.outlier_cap = outlier_cap
+        self.tokens_per_page, self.row_len = tokens_per_page, row_len
 
     def desc(self) -> "_native.TierStoreDesc":
         return _native.TierStoreDesc(self.data.data_ptr(), self.slot_bytes, self.n_slots, self.format,

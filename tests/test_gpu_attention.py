@@ -1000,3 +1000,16 @@ def test_refuses_heads_of_another_size_than_the_pools(cuda):
     flat = KVLayers([k.view(k.shape[0], -1) for k in c.kv.k], [v.view(v.shape[0], -1) for v in c.kv.v])  # rows as one
     q = queries(1, 4, 128, 61).to(cuda)
     assert torch.equal(A.decode_attention(q, c.table, flat, None, ids, L), A.decode_attention(q, c.table, c.kv, None, ids, L))
+
+
+def test_refuses_stores_of_other_pages(cuda):
+    """Slots are laid out for one page size; a smaller page fits, but is not what they hold."""
+    c = Cache(cuda, [N.PAGE_BF16, N.PAGE_INT8], 16, 2, 128, 62)
+    ids, L = torch.zeros(1, 2, dtype=torch.int32, device=cuda), torch.tensor([8], dtype=torch.int32, device=cuda)
+    q = queries(1, 4, 128, 62).to(cuda)
+    A.decode_attention(q, c.table, c.kv, c.stores, ids, L)
+    with pytest.raises(N.KernelError, match="laid out for pages of 16 x 256"):
+        A.decode_attention(q, c.table, c.kv, c.stores, ids, L, tokens_per_page=8)
+    wide = {1: TierStore(N.PAGE_INT8, 2, cuda, 16, 512)}
+    with pytest.raises(N.KernelError, match="laid out for pages of 16 x 512"):
+        A.decode_attention(q, c.table, c.kv, wide, ids, L)
