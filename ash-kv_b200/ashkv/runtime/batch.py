@@ -143,6 +143,8 @@ class KVLayers:
         for t in self.k + self.v:
             if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.shape != t0.shape or not t.is_cuda:
                 raise ValueError("K/V layers must be contiguous CUDA bf16 tensors of one shape")
+            if t.device != t0.device:
+                raise ValueError(f"K/V layers must be on one device, got {t.device} and {t0.device}")
             if t.data_ptr() % 16:
                 raise ValueError("K/V layer tensors must be 16-byte aligned")
         self.row_len = int(np.prod(t0.shape[1:]))

@@ -171,3 +171,23 @@ def test_decode_refuses_lists_whose_positions_leave_an_int():
         assert b"too many list entries" in N.lib().ashkv_last_error()
         assert decode(desc(), n=n, sel=X, cnt=X, width=pages) == N.BAD_ARGUMENT
         assert b"too many list entries" in N.lib().ashkv_last_error()
+
+
+def test_layers_of_two_devices_are_refused():
+    """The kernels follow every layer's address on the device of the first."""
+    class Layer:
+        dtype, shape, is_cuda = torch.bfloat16, torch.Size([32, 2, 64]), True
+
+        def __init__(self, device):
+            self.device = torch.device(device)
+
+        def is_contiguous(self):
+            return True
+
+        def data_ptr(self):
+            return 256
+
+    from ashkv.runtime.batch import KVLayers
+    for k, v in ((["cuda:0", "cuda:1"], ["cuda:0"] * 2), (["cuda:0"] * 2, ["cuda:0", "cuda:1"]), (["cuda:0"], ["cuda:1"])):
+        with pytest.raises(ValueError, match="one device"):
+            KVLayers([Layer(d) for d in k], [Layer(d) for d in v])
