@@ -1013,3 +1013,126 @@ def test_refuses_stores_of_other_pages(cuda):
     wide = {1: TierStore(N.PAGE_INT8, 2, cuda, 16, 512)}
     with pytest.raises(N.KernelError, match="laid out for pages of 16 x 512"):
         A.decode_attention(q, c.table, c.kv, wide, ids, L)
+
+
+# ----------------------------------------------------------------------------- every instance of the kernels
+STORES = {**FORMATS, "fp8+int4": [N.PAGE_FP8, N.PAGE_INT4]}  # the last: queries in all three forms at once
+
+
+@pytest.mark.parametrize("tiers", list(STORES))
+@pytest.mark.parametrize("dim,heads", [(64, 2), (64, 8), (128, 1), (128, 2)])
+@pytest.mark.parametrize("group", [9, 20])
+def test_decode_groups_of_all_formats(cuda, tiers, dim, heads, group, monkeypatch):
+    monkeypatch.setitem(FORMATS, tiers, STORES[tiers])
+    run_case(cuda, tiers, 16, heads * group, heads, dim, [50, 131], 100)
+
+
+@pytest.mark.parametrize("dim,heads,group", [(64, 1, 12), (64, 3, 9), (128, 5, 11)])
+def test_decode_odd_numbers_of_heads(cuda, dim, heads, group):
+    run_case(cuda, "bf16", 16, heads * group, heads, dim, [50, 131], 101)
+
+
+@pytest.mark.parametrize("tiers", list(STORES))
+@pytest.mark.parametrize("T", [1, 19])
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 3), (64, 10), (128, 12)])
+def test_decode_compressed_pages_of_an_odd_number_of_tokens(cuda, tiers, T, dim, group, monkeypatch):
+    monkeypatch.setitem(FORMATS, tiers, STORES[tiers])
+    heads = 512 // dim
+    run_case(cuda, tiers, T, heads * group, heads, dim, [T, 3 * T - 1, 4 * T + 1, 1], 102)
+
+
+@pytest.mark.parametrize("tiers", list(STORES))
+@pytest.mark.parametrize("T,dim,group", [(16, 128, 1), (16, 64, 12), (5, 128, 9), (8, 64, 2), (16, 128, 8)])
+def test_decode_several_pages_to_a_worker(cuda, tiers, T, dim, group):
+    """Workers that attend many pages of several sequences, some of them empty."""
+    heads = 2048 // dim
+    kinds = STORES[tiers]
+    c = Cache(cuda, [kinds[i % len(kinds)] for i in range(12)], T, heads, dim, 103)
+    run_shared(cuda, c, heads * group, [0 if i % 7 == 3 else 1 + (53 * i) % (40 * T) for i in range(30)], 103)
+
+
+@pytest.mark.parametrize("tiers", ["bf16", "mixed", "fp8+int4"])
+@pytest.mark.parametrize("dim,group", [(64, 3), (128, 12)])
+def test_decode_selected_several_pages_to_a_worker(cuda, tiers, dim, group):
+    T, heads, P, B = 16, 1024 // dim, 60, 24
+    kinds = STORES[tiers]
+    c = Cache(cuda, [kinds[i % len(kinds)] for i in range(12)], T, heads, dim, 104)
+    g = np.random.default_rng(104)
+    ids = g.integers(0, 12, (B, P)).astype(np.int32)
+    lengths = [int(x) for x in g.integers(1, P * T, B)]
+    lengths[5] = 0
+    sel, cnt = np.full((B, heads, 40), -1, np.int32), np.zeros((B, heads), np.int32)
+    rows = {}
+    for b in range(B):
+        for h in range(heads):
+            pages = -(-lengths[b] // T)
+            k = int(g.integers(0, min(40, pages) + 1))
+            rows[b, h] = sorted(g.permutation(pages)[:k].tolist())
+            sel[b, h, :k], cnt[b, h] = rows[b, h], k
+    q, status = queries(B, heads * group, dim, 104), torch.zeros(1, dtype=torch.int32, device=cuda)
+    out, lse = A.decode_attention(q.to(cuda), c.table, c.kv, c.stores, torch.from_numpy(ids).to(cuda),
+                                  torch.tensor(lengths, dtype=torch.int32, device=cuda), selected=torch.from_numpy(sel).to(cuda),
+                                  selected_count=torch.from_numpy(cnt).to(cuda), return_lse=True, status=status)
+    assert int(status) == 0
+    lists = [[[(j, c.values[ids[b, j]]) for j in rows[b, h]] for h in range(heads)] for b in range(B)]
+    check(out, lse, O.decode_attention(q.double().numpy(), lists, lengths, T, dim ** -0.5), dim, 40 * T)
+
+
+@pytest.mark.parametrize("pages", [8191, 8192, 8193, 20001])
+@pytest.mark.parametrize("budget,sink,recent", [(1, 0, 1), (300, 2, 5), (8192, 1, 1), (20000, 0, 0)])
+def test_select_rows_around_and_beyond_8192(cuda, pages, budget, sink, recent):
+    """Rows whose keys do not fit the registers of a CTA are read anew in each round."""
+    T, n, heads = 16, 700, 2
+    g = torch.Generator().manual_seed(105)
+    b = A.PageBounds.empty(n, heads, 64, cuda)
+    b.codes.copy_(torch.randint(-127, 128, b.codes.shape, generator=g).sort(2).values.to(torch.int8))
+    b.exponents.copy_(torch.randint(-2, 2, (n, heads), generator=g).to(torch.int8))
+    ids = torch.randint(0, n, (2, pages), generator=g).to(torch.int32)  # every page about thirty times: ties
+    lengths = [pages * T - 3, (pages // 2) * T]
+    q = queries(2, 4, 64, 105)
+    sel, cnt = A.select_pages(q.to(cuda), b, ids.to(cuda), torch.tensor(lengths, dtype=torch.int32, device=cuda), budget,
+                              sink=sink, recent=recent)
+    check_selected(sel, cnt, select_want(q, b, ids.numpy(), lengths, T, budget, sink, recent))
+
+
+@pytest.mark.parametrize("pages", [8192, 8193, 20001])
+@pytest.mark.parametrize("budget,sink,recent", [(1, 0, 1), (700, 3, 8), (8192, 1, 1), (20000, 5, 2)])
+def test_evict_rows_around_and_beyond_8192(cuda, pages, budget, sink, recent):
+    T = 16
+    g = torch.Generator().manual_seed(106)
+    mass = torch.rand(4, pages, generator=g)
+    mass[1, ::2] = 0.25  # ties
+    mass[2, 3::5] = float("nan")
+    mass[2, 4::50], mass[2, 8::50], mass[2, 9::50] = -0.0, -1.0, float("inf")
+    mass[3] = 0.0
+    ids = torch.randint(0, 1 << 30, (4, pages), generator=g).to(torch.int32)
+    lengths = [pages * T, pages * T - 5, (pages - 1) * T + 1, (pages // 2) * T]
+    got = A.evict_pages(mass.to(cuda), ids.to(cuda), torch.tensor(lengths, dtype=torch.int32, device=cuda), budget, sink=sink,
+                        recent=recent)
+    for b, n in enumerate(lengths):
+        used = -(-n // T)
+        keep = O.keep_highest(mass[b, :used].double().numpy(), budget, sink, recent)
+        gone = np.setdiff1d(np.arange(used), keep)
+        assert np.array_equal(got.page_ids[b, :len(keep)].cpu().numpy(), ids[b, keep].numpy())
+        assert np.array_equal(got.page_mass[b, :len(keep)].cpu().numpy(), mass[b, keep].numpy(), equal_nan=True)
+        assert (got.page_ids[b, len(keep):] == -1).all() and (got.page_mass[b, len(keep):] == 0).all()
+        assert np.array_equal(got.evicted[b, :len(gone)].cpu().numpy(), ids[b, gone].numpy())
+        assert (got.evicted[b, len(gone):] == -1).all()
+        assert int(got.n_evicted[b]) == len(gone) and int(got.lengths[b]) == n - T * len(gone)
+
+
+def test_refuses_rows_that_overlap(cuda):
+    """Sequences whose ids or masses share memory: two blocks would update one mass."""
+    c = Cache(cuda, [N.PAGE_BF16, N.PAGE_BF16], 16, 2, 64, 60)
+    ids = torch.zeros(2, 2, dtype=torch.int32, device=cuda)
+    L, q, mass = torch.full((2,), 16, dtype=torch.int32, device=cuda), queries(2, 4, 64, 60).to(cuda), torch.zeros(2, 2, device=cuda)
+    bounds = A.PageBounds.empty(2, 2, 64, cuda)
+    for call in (lambda i, m: A.decode_attention(q, c.table, c.kv, c.stores, i, L, page_mass=m),
+                 lambda i, m: A.evict_pages(m, i, L, 2)):
+        call(ids, mass)
+        for i, m in ((ids[:1].expand(2, 2), mass), (ids, mass[:1].expand(2, 2)),
+                     (ids, torch.zeros(3, device=cuda).as_strided((2, 2), (1, 1)))):
+            with pytest.raises(ValueError, match="rows overlap"):
+                call(i, m)
+    with pytest.raises(ValueError, match="rows overlap"):
+        A.select_pages(q, bounds, ids[:1].expand(2, 2), L, 2)
