@@ -169,7 +169,9 @@ def decode_attention(q: torch.Tensor, table: DevicePageTable, kv: KVLayers,
     compressed tier to its store, as for :class:`~ashkv.runtime.batch.BatchMigrator`.  ``scale``
     defaults to 1/sqrt(head_dim).  Returns the bf16 result [n_seqs, heads_q, head_dim]
     (``out``, if given), with ``return_lse`` also the fp32 log of the sum of exponentials
-    [n_seqs, heads_q].  A sequence of length 0 gives zeros and -inf.
+    [n_seqs, heads_q].  A sequence of length 0 gives zeros and -inf.  The lists hold up to
+    2^31 - 1 - 2^16 entries together.  A store must have been made for pages of
+    ``tokens_per_page`` tokens of the pool's rows.
 
     Compressed codes count as the numbers they stand for (a decode's rounding to bf16 is left
     out; dithered pages count as the bf16 values of their decoder).
@@ -310,8 +312,8 @@ def evict_pages(page_mass: torch.Tensor, page_ids: torch.Tensor, lengths: torch.
 
     ``page_mass`` is what :func:`decode_attention` keeps.  The first ``sink`` and the last
     ``recent`` (at least the page being filled) pages stay, and of the others those of greatest
-    mass (of equal mass the lower position, NaN counts as the least).  The inputs are not
-    changed; the pages that leave are listed, their slots and pool rows stay the caller's to
+    mass (of equal mass the lower position, NaN counts as the least).  A length beyond
+    ``max_pages`` pages is cut there; a negative one is none.  The inputs are not changed; the pages that leave are listed, their slots and pool rows stay the caller's to
     give back (another sequence may share them)."""
     if page_ids.dim() != 2:
         raise ValueError("page_ids must be [n_seqs, max_pages]")

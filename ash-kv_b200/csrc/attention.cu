@@ -672,10 +672,9 @@ struct Worker {
   // Digits.  Channels 16 k .. 16 k + 15 (words of four) serve two products of 32 channels.  NT = 1: the
   // two higher digits as the two halves of the rows, two operands; the lowest like 16-bit words above.
   // NT = 2: two operands for each digit.
-  static constexpr uint32_t kLowDigit = 8 * D * 2;
   static __device__ __forceinline__ uint32_t digit_chunk(uint32_t row, uint32_t chunk) { return row * (D * 2) + ((chunk ^ (row & 1u)) << 4); }
   static __device__ __forceinline__ uint32_t low_chunk(uint32_t row, uint32_t chunk) {
-    return kLowDigit + row * D + (((chunk ^ ((row & 1u) << 2)) & (D / 16 - 1)) << 4);
+    return 8 * D * 2 + row * D + (((chunk ^ ((row & 1u) << 2)) & (D / 16 - 1)) << 4);
   }
   static __device__ __forceinline__ uint32_t digit_word(uint32_t digit, uint32_t n, uint32_t k, uint32_t w) {  // digit 0: the highest
     if constexpr (NT == 1) {

@@ -344,13 +344,13 @@ __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* s_warp, ui
 // above), fewer where a digit's count ends exactly at the number still wanted.
 // Every warp owns a run of positions, 32 at a time.  For the ranks each warp counts
 // its run first, so one scan over the warps serves the whole row.  Bound by the
-// latency of its rounds: 256 of 8192 pages for 8 rows 15 us on 8 SMs, 1024 of
-// up to 8192 for 256 rows (eviction) 28 us.  Digits taken of the distance from the
+// latency of its rounds: 128 of 8192 pages for 8 rows 15 us on 8 SMs, 1024 of
+// up to 8192 for 256 rows (eviction) 24 us.  Digits taken of the distance from the
 // lowest key, which spread over more bins, cost the reduction what they save.
 //   CACHED: rows of up to kCached * kKeepThreads positions keep their keys in
 // registers, longer ones read them anew in each round.  At 8192 positions: 8 rows
-// (select, with its attention) 39.9 us and 41.3 read anew, 64 rows 102 and 99, 256
-// rows (evict) 32.2 and 34.8; the same at 2048.
+// (select, with its attention) 39.4 us and 41.4 read anew, 64 rows 100 and 104, 256
+// rows (evict) 28.5 and 30.8; the same at 2048.
 constexpr int kCached = 8;
 template <bool CACHED, class Emit>
 __device__ void keep_highest(const float* score, int n, int budget, int sink, int recent, KeepShared& sm,

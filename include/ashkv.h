@@ -576,7 +576,7 @@ ASHKV_API ashkv_status_t ashkv_decode_attention(
  *   score[b, head, j] = max over the head's query heads of
  *        2^(f + e) * sum_d max(q8[d] * lo[d], q8[d] * hi[d])      (lo <= hi)
  * -- whole numbers times a power of two, so the scores, and with them the
- * selection, are exact -- and writes to d_selected[b, head, 0 .. budget) the
+ * selection, are exact (as far as a score is a normal fp32 number) -- and writes to d_selected[b, head, 0 .. budget) the
  * positions, ascending, of the first `sink` pages, the last `recent` pages
  * and the highest scores up to `budget` (all pages where there are no more;
  * of equal scores the lower position), then -1, and their number to
