@@ -317,7 +317,7 @@ def _handle(s):
     package = str(Path(__file__).resolve().parent.parent / "ash-kv_b200")  # (a folder of the repository, not on the path)
     if package not in sys.path:
         sys.path.insert(0, package)
-    from ashkv import runtime
+    from ashkv.runtime import attention, cache
     from ashkv.runtime.batch import DevicePageTable, KVLayers, TierStore
     case, f = s["case"], s["zeros"].float()
     table = DevicePageTable(f, f, f, f, s["tier"], s["zeros"], s["zeros"], s["start"], s["slot"])
@@ -327,7 +327,7 @@ def _handle(s):
                           CAP if fmt in (NBIT4, NBIT2) else 0)
         store.data = data.view(-1)
         stores[TIER_OF[fmt]] = store
-    return runtime, table, KVLayers([s["k"]], [s["v"]]), stores
+    return attention, cache, table, KVLayers([s["k"]], [s["v"]]), stores
 
 
 # ----------------------------------------------------------------------------- plain forms
@@ -465,22 +465,22 @@ def run(s):
     case = s["case"]
     if not own:
         return {"store": _store, "load": _load, "prompt": _prompt, "step": _step}[case["kind"]](s)
-    R, table, kv, stores = s["handle"]
+    A, C, table, kv, stores = s["handle"]
     T, hq, hkv = case["page"], case["heads_q"], case["heads_kv"]
     window = case["window"] or None
     if case["kind"] == "step":
         mass = s["mass"].clone() if case["mass"] else None  # the program's running mass, kept for the next pass
-        out, lse = R.decode_attention(s["qkv"][:, :hq], table, kv, stores, s["page_ids"], s["lengths"], tokens_per_page=T,
+        out, lse = A.decode_attention(s["qkv"][:, :hq], table, kv, stores, s["page_ids"], s["lengths"], tokens_per_page=T,
                                       window=window, sinks=case["sinks"], page_mass=mass, decay=DECAY, return_lse=True)
         return {"out": out, "lse": lse} | ({"mass": mass} if case["mass"] else {})
     if case["kind"] == "prompt":
-        out, lse = R.prompt_attention(s["qkv"][:, :hq], table, kv, stores, s["page_ids"], s["lengths"], s["starts"],
+        out, lse = A.prompt_attention(s["qkv"][:, :hq], table, kv, stores, s["page_ids"], s["lengths"], s["starts"],
                                       tokens_per_page=T, window=window, sinks=case["sinks"], return_lse=True)
         return {"out": out, "lse": lse}
     if case["kind"] == "store":
-        R.write_kv(s["qkv"][:, hq:hq + hkv], s["qkv"][:, hq + hkv:], table, kv, stores, s["page_ids"], s["lengths"],
+        C.write_kv(s["qkv"][:, hq:hq + hkv], s["qkv"][:, hq + hkv:], table, kv, stores, s["page_ids"], s["lengths"],
                    s["starts"], tokens_per_page=T)
-    k, v = R.read_kv(table, kv, stores, s["page_ids"], s["lengths"], s["starts"], s["N"], tokens_per_page=T)
+    k, v = C.read_kv(table, kv, stores, s["page_ids"], s["lengths"], s["starts"], s["N"], tokens_per_page=T)
     return {"k": k, "v": v}
 
 
