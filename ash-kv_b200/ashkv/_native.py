@@ -79,6 +79,10 @@ SIGNATURES: dict[str, tuple] = {
     "ashkv_decode_scratch_floats": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
     "ashkv_decode_attention": (_I32, [_P, _P, _I64, _I64, _I32, _I32, _P, _I64, _I32, _P, _P, _P, _I32, _F32, _P,
                                       _I64, _F32, _P, _P, _P, _P, _P]),
+    "ashkv_decode_attention_window": (_I32, [_P, _P, _I64, _I64, _I32, _I32, _P, _I64, _I32, _P, _I32, _I32, _F32, _P,
+                                             _I64, _F32, _P, _P, _P, _P, _P]),
+    "ashkv_write_kv": (_I32, [_P, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I32, _P, _P, _I32, _P, _P]),
+    "ashkv_read_kv": (_I32, [_P, _P, _I64, _I32, _P, _P, _I32, _I64, _P, _P, _P, _P]),
     "ashkv_page_bounds": (_I32, [_P, _P, _P, _I32, _P, _P, _P, _P, _P]),
     "ashkv_select_scratch_floats": (_I64, [_I32, _I32, _I32]),
     "ashkv_select_pages": (_I32, [_P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _I64, _P, _I64, _I32, _P, _I32,
@@ -583,6 +587,35 @@ def decode_attention(desc: PagedKVDesc, q: torch.Tensor, page_ids: torch.Tensor,
         0 if selected is None else selected.shape[2], scale, _ptr(page_mass),
         0 if page_mass is None else page_mass.stride(0), decay, out.data_ptr(), _ptr(lse), scratch.data_ptr(),
         _ptr(status), raw_stream(q)), "decode_attention")
+
+
+def decode_attention_window(desc: PagedKVDesc, q: torch.Tensor, page_ids: torch.Tensor, lengths: torch.Tensor,
+                            window: int, sinks: int, scale: float, page_mass: Optional[torch.Tensor], decay: float,
+                            out: torch.Tensor, lse: Optional[torch.Tensor], scratch: torch.Tensor,
+                            status: Optional[torch.Tensor]) -> None:
+    n_seqs, heads_q = q.shape[0], q.shape[1]
+    _check_text(lib().ashkv_decode_attention_window(
+        ctypes.addressof(desc), q.data_ptr(), q.stride(0), q.stride(1), n_seqs, heads_q, page_ids.data_ptr(),
+        page_ids.stride(0), page_ids.shape[1], lengths.data_ptr(), window, sinks, scale, _ptr(page_mass),
+        0 if page_mass is None else page_mass.stride(0), decay, out.data_ptr(), _ptr(lse), scratch.data_ptr(),
+        _ptr(status), raw_stream(q)), "decode_attention")
+
+
+def write_kv(desc: PagedKVDesc, k: torch.Tensor, v: torch.Tensor, page_ids: torch.Tensor, lengths: torch.Tensor,
+             starts: torch.Tensor, status: Optional[torch.Tensor]) -> None:
+    """Rows k, v [n, heads, dim] bf16 (unit inner stride) -> the pages of ``desc``."""
+    _check_text(lib().ashkv_write_kv(
+        ctypes.addressof(desc), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), k.shape[0],
+        page_ids.data_ptr(), page_ids.stride(0), page_ids.shape[1], lengths.data_ptr(), starts.data_ptr(),
+        lengths.shape[0], _ptr(status), raw_stream(k)), "write_kv")
+
+
+def read_kv(desc: PagedKVDesc, page_ids: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, k: torch.Tensor,
+            v: torch.Tensor, status: Optional[torch.Tensor]) -> None:
+    _check_text(lib().ashkv_read_kv(
+        ctypes.addressof(desc), page_ids.data_ptr(), page_ids.stride(0), page_ids.shape[1], lengths.data_ptr(),
+        starts.data_ptr(), lengths.shape[0], k.shape[0], k.data_ptr(), v.data_ptr(), _ptr(status), raw_stream(k)),
+        "read_kv")
 
 
 def page_bounds(desc: PagedKVDesc, pages: torch.Tensor, count: Optional[torch.Tensor], valid: Optional[torch.Tensor],

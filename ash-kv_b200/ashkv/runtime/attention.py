@@ -95,6 +95,15 @@ def _require_query(q: torch.Tensor) -> None:
 _MOST = 2 ** 31 - 1  # the library takes sizes as int32
 
 
+def _require_window(window: Optional[int], sinks: int) -> None:
+    if window is not None and not 0 < window <= _MOST:
+        raise ValueError("window must be at least 1 and fit an int32")
+    if not 0 <= sinks <= _MOST:
+        raise ValueError("sinks must not be negative and fit an int32")
+    if window is None and sinks:
+        raise ValueError("sinks need a window")
+
+
 def _require_tokens_per_page(n: int) -> None:
     if not 0 < n <= _MOST:
         raise ValueError("tokens_per_page must be positive and fit an int32")
@@ -160,7 +169,7 @@ def decode_attention(q: torch.Tensor, table: DevicePageTable, kv: KVLayers,
                      tokens_per_page: int = 16, scale: Optional[float] = None,
                      selected: Optional[torch.Tensor] = None, selected_count: Optional[torch.Tensor] = None,
                      page_mass: Optional[torch.Tensor] = None, decay: float = 1.0,
-                     out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                     window: Optional[int] = None, sinks: int = 0, out: Optional[torch.Tensor] = None, return_lse: bool = False,
                      status: Optional[torch.Tensor] = None):
     """Attention of one new token per sequence over its pages, whatever tier holds them.
 
@@ -180,8 +189,13 @@ def decode_attention(q: torch.Tensor, table: DevicePageTable, kv: KVLayers,
     restricts each key head to those page positions (see :func:`select_pages`).  ``page_mass``
     fp32 [n_seqs, max_pages] is updated in place: for each position j that holds tokens,
     ``page_mass[b, j] = decay * page_mass[b, j] +`` the attention weight of page j summed over
-    heads and tokens; it cannot be combined with ``selected``."""
+    heads and tokens; it cannot be combined with ``selected``.
+
+    With ``window`` only the newest ``window`` tokens and the first ``sinks`` are attended, and
+    only their pages are looked up and read (the list's other entries may be anything);
+    ``selected`` has first and last pages of its own and takes no window."""
     _require_query(q)
+    _require_window(window, sinks)
     n_seqs, heads_q, d = q.shape
     dev = q.device
     page_ids = _require_lists(page_ids, lengths, n_seqs, dev)
@@ -194,6 +208,8 @@ def decode_attention(q: torch.Tensor, table: DevicePageTable, kv: KVLayers,
     if selected is not None:
         if page_mass is not None:
             raise ValueError("page_mass cannot be combined with selected")
+        if window is not None:
+            raise ValueError("a window cannot be combined with selected")
         if selected.dim() != 3 or selected.shape[2] == 0:
             raise ValueError("selected must be [n_seqs, heads_kv, width] with a width of at least 1")
         width = selected.shape[2]
@@ -213,9 +229,13 @@ def decode_attention(q: torch.Tensor, table: DevicePageTable, kv: KVLayers,
             scratch = torch.empty(_native.decode_scratch_floats(n_seqs, heads_q, desc.heads_kv, d, width,
                                                                 page_mass is not None),
                                   dtype=torch.float32, device=dev)
-            _native.decode_attention(desc, q, page_ids, lengths, selected, selected_count,
-                                     1.0 / math.sqrt(d) if scale is None else float(scale), page_mass, float(decay),
-                                     out, lse, scratch, status)
+            scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+            if window is None:
+                _native.decode_attention(desc, q, page_ids, lengths, selected, selected_count, scale, page_mass,
+                                         float(decay), out, lse, scratch, status)
+            else:
+                _native.decode_attention_window(desc, q, page_ids, lengths, window, sinks, scale, page_mass,
+                                                float(decay), out, lse, scratch, status)
     return (out, lse) if return_lse else out
 
 

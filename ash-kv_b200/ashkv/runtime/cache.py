@@ -1,0 +1,114 @@
+"""Tokens into tiered pages and back.
+
+The reference encodes a page once it is complete in the KV pool and promotes it before it is
+used (ashkv/runtime/migrate.py:35-191).  Here the tokens that a model has just computed go
+straight into the pages they belong to, in the format of each page's tier, and the tokens of any
+pages can be had as dense rows:
+
+* :func:`write_kv`: new keys and values are quantised as they are written;
+* :func:`read_kv`: the bf16 values that the pages of a sequence decode to.
+
+Sequences are rows of ``page_ids`` with their ``lengths``, as for
+:func:`~ashkv.runtime.attention.decode_attention`.  ``starts`` (int32 [n_seqs + 1], ascending) says
+whose the rows of a call are: rows ``starts[b] .. starts[b + 1] - 1`` are the newest tokens of
+sequence b, the last of them token ``lengths[b] - 1``; rows of no sequence (behind the last one, in
+a padded batch) are left alone.  All calls run on the current stream of the tensors' device, never
+wait for the device, and can be captured in a CUDA graph.
+"""
+from __future__ import annotations
+
+from typing import Mapping, Optional
+
+import torch
+
+from .. import _native
+from .attention import _on, _pages_desc, _refuse, _require_dense, _require_lists
+from .batch import DevicePageTable, KVLayers, TierStore
+
+
+def _row_shape(kv: KVLayers) -> tuple[int, int]:
+    """Heads and channels of the pool's rows; one head where they are flat."""
+    pool = kv.k[0].shape
+    dim = pool[-1] if len(pool) > 2 else kv.row_len
+    return kv.row_len // max(dim, 1), dim
+
+
+def _require_starts(starts: torch.Tensor, n_seqs: int, device: torch.device) -> None:
+    _require_dense(starts, "starts", torch.int32, (n_seqs + 1,), device)
+
+
+def _new_rows(x: torch.Tensor, name: str, heads: int, dim: int) -> torch.Tensor:
+    if not x.is_cuda or x.dtype != torch.bfloat16:
+        _refuse(x, name, torch.bfloat16, x.shape, x.device)
+    if x.dim() == 2 and x.shape[1] == heads * dim and (x.stride(1) == 1 or x.shape[1] == 1):
+        x = x.unflatten(1, (heads, dim))
+    if x.dim() != 3 or x.shape[1:] != (heads, dim):
+        raise ValueError(f"{name} must be [n_rows, {heads}, {dim}] or [n_rows, {heads * dim}]")
+    if x.stride(2) != 1 and dim > 1:
+        raise ValueError(f"{name} must be dense in its last dimension")
+    return x
+
+
+def write_kv(k: torch.Tensor, v: torch.Tensor, table: DevicePageTable, kv: KVLayers,
+             stores: Optional[Mapping[int, TierStore]], page_ids: torch.Tensor, lengths: torch.Tensor,
+             starts: torch.Tensor, *, tokens_per_page: int = 16, status: Optional[torch.Tensor] = None) -> None:
+    """Quantise the keys and values of new tokens into the pages they belong to.
+
+    ``k`` and ``v`` are bf16 [n_rows, heads_kv, head_dim] (any strides with a dense last dimension, so
+    slices of a fused projection will do); ``lengths`` count the new tokens already.  A page in the
+    BF16 tier takes the row as it is, an INT8 page its codes and per-token scale, an FP8 page its
+    codes, an INT4 page its groups' scales and codes: the bytes that a migration of the complete page
+    would write.  A page must have its slot (``table.slot``) before it is written to.  Tokens of pages
+    that do not exist are left out and set ``_native.FLAG_INDEX_RANGE`` in ``status`` (int32 [1], if
+    given), as are those of dithered pages, which are coded as a whole.  Two rows must not be the same
+    token."""
+    heads, dim = _row_shape(kv)
+    k, v = _new_rows(k, "k", heads, dim), _new_rows(v, "v", heads, dim)
+    dev = k.device
+    if v.device != dev or v.shape[0] != k.shape[0]:
+        raise ValueError("k and v must have as many rows, on one device")
+    n_seqs = lengths.numel()
+    page_ids = _require_lists(page_ids, lengths, n_seqs, dev)
+    _require_starts(starts, n_seqs, dev)
+    desc, keep = _pages_desc(table, kv, stores, dim, tokens_per_page, dev)
+    if status is not None:
+        _require_dense(status, "status", torch.int32, (1,), dev)
+    if n_seqs and k.shape[0]:
+        with _on(dev):
+            _native.write_kv(desc, k, v, page_ids, lengths, starts, status)
+
+
+def read_kv(table: DevicePageTable, kv: KVLayers, stores: Optional[Mapping[int, TierStore]], page_ids: torch.Tensor,
+            lengths: torch.Tensor, starts: torch.Tensor, n_rows: int, *, tokens_per_page: int = 16,
+            out: Optional[tuple[torch.Tensor, torch.Tensor]] = None, status: Optional[torch.Tensor] = None):
+    """The keys and values of the newest tokens of each sequence as dense bf16 rows.
+
+    Returns (k, v), each [n_rows] rows shaped as the pool's (``out``, if given): the values that a
+    promotion of the tokens' pages would write, whatever tier holds them.  ``n_rows`` is what the host
+    knows ``starts[-1]`` to be, or more (those rows are left as they were).  Tokens whose page does not
+    exist are zeros and set ``_native.FLAG_INDEX_RANGE`` in ``status``."""
+    heads, dim = _row_shape(kv)
+    dev = page_ids.device
+    n_seqs = lengths.numel()
+    page_ids = _require_lists(page_ids, lengths, n_seqs, dev)
+    _require_starts(starts, n_seqs, dev)
+    desc, keep = _pages_desc(table, kv, stores, dim, tokens_per_page, dev)
+    if status is not None:
+        _require_dense(status, "status", torch.int32, (1,), dev)
+    if n_rows < 0:
+        raise ValueError("n_rows must not be negative")
+    shape = (n_rows, *kv.k[0].shape[1:])
+    if out is None:
+        out = kv.k[0].new_empty(shape), kv.k[0].new_empty(shape)
+    else:
+        for name, x in zip(("out[0]", "out[1]"), out):
+            _require_dense(x, name, torch.bfloat16, shape, dev)
+            if x.data_ptr() % 16:
+                raise ValueError(f"{name} must be 16-byte aligned")
+    if n_seqs and n_rows:
+        with _on(dev):
+            _native.read_kv(desc, page_ids, lengths, starts, out[0], out[1], status)
+    return out
+
+
+__all__ = ["write_kv", "read_kv"]

@@ -25,11 +25,11 @@
 //     first page arrives (lengths, ids, table, page: loads that wait for another)
 #include <algorithm>
 #include <atomic>
-#include <cstdio>
+#include <type_traits>
 
 #include "common.cuh"
 #include "nbit_group.cuh"
-#include "page_layout.cuh"
+#include "paged_kv.cuh"
 
 namespace ashkv {
 namespace {
@@ -41,8 +41,6 @@ constexpr uint32_t kPolls = 1u << 24;  // bounded mbarrier waits
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kJoinThreads = 256;
-// Entries of all lists of a call: what is added to a position (ranges, a batch looked up ahead) stays inside an int.
-constexpr int64_t kMostEntries = 0x7FFFFFFFLL - 65536;
 
 struct AttnParams {
   // pages
@@ -83,28 +81,49 @@ struct AttnParams {
   int32_t warp_smem;  // bytes of shared memory of a worker
   int32_t fp8_pages, int_pages;  // whether a store holds FP8, or INT8 or INT4 pages
   uint32_t* status;
+  int32_t window, sinks;  // kernels with WIN: tokens of the sliding window (at least 1), first tokens that stay visible
 };
-
-__device__ __forceinline__ void flag(uint32_t* status, uint32_t f) {
-  if (status) atomicOr(status, f);
-}
 
 // Tokens of sequence b that its page list can hold.
 __device__ __forceinline__ int64_t seq_tokens(const AttnParams& p, int b) {
   const int64_t len = p.lengths[b], most = int64_t(p.max_pages) * p.T;
   return len < 0 ? 0 : (len > most ? most : len);
 }
+// With a window a sequence's list has its first `sinks` pages (those of the tokens that stay visible) and,
+// `skip` pages later, those from the window's first token on.
+struct Span {
+  int sinks, skip, entries;
+  __device__ __forceinline__ int position(int e) const { return e < sinks ? e : e + skip; }
+};
+__device__ __forceinline__ Span span_of(const AttnParams& p, int64_t tokens) {
+  Span s;
+  const int pages = int((tokens + p.T - 1) / p.T);
+  s.sinks = int((min(int64_t(p.sinks), tokens) + p.T - 1) / p.T);
+  s.skip = max(0, int(max(int64_t(0), tokens - p.window) / p.T) - s.sinks);
+  s.entries = pages - s.skip;
+  return s;
+}
+// Which of the 16 tokens from `first` on the newest of `tokens` tokens sees.
+__device__ __forceinline__ uint32_t seen_of(const AttnParams& p, int64_t tokens, int64_t first) {
+  const int sinks = int(max(int64_t(0), min(int64_t(16), p.sinks - first)));
+  const int old = int(max(int64_t(0), min(int64_t(16), tokens - p.window - first)));
+  return ((1u << sinks) - 1u) | (0xFFFFu & ~((1u << old) - 1u));
+}
+
 // Entries of the list that key head hk of sequence b attends.
+template <bool WIN>
 __device__ __forceinline__ int list_len(const AttnParams& p, int b, int hk) {
+  if constexpr (WIN) return span_of(p, seq_tokens(p, b)).entries;
   if (p.selected) return max(0, min(p.selected_count[int64_t(b) * p.heads_kv + hk], p.max_selected));
   return int((seq_tokens(p, b) + p.T - 1) / p.T);
 }
 
 // Pages of key head hk's lists before sequence b (warp-collective; b <= n_seqs).
+template <bool WIN>
 __device__ int lists_before(const AttnParams& p, int b, int hk) {
   const int lane = threadIdx.x & 31;
   int sum = 0;
-  for (int i = lane; i < b; i += 32) sum += list_len(p, i, hk);
+  for (int i = lane; i < b; i += 32) sum += list_len<WIN>(p, i, hk);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
   return sum;
@@ -261,12 +280,13 @@ struct RawNbit {
   static constexpr uint32_t kRow = D * BITS / 8, kDeltas = 16 * kRow, kDeltaRow = D / 16, kCount = kDeltas + 16 * kDeltaRow,
                             kEntries = kCount + 16, kMaxEntries = 128;
 };
-// Decodes such a unit in place into the K or V rows (bf16) of a BF16 unit; slot: the page's.  A group
+// Decodes such a unit in place into the K or V rows (bf16) of a BF16 unit; slot: the page's; seen: a bit for
+// each row, the others become zeros.  A group
 // of 32 channels at a time and lane, all read before any is written; the outliers overwrite theirs.
 // (Out of line: a call costs little beside the decode, and the loop of the other formats stays short.)
 template <int D, int BITS>
 __device__ __noinline__ void decode_nbit(uint32_t unit, const uint8_t* slot, int T, int row_len, int cap, int hk, bool v,
-                                         int t0, int rows) {
+                                         int t0, uint32_t seen) {
   using Raw = RawNbit<D, BITS>;
   constexpr int GPR = D / 32, RB = D * 2, N = GPR / 2;
   constexpr float half = float((1 << BITS) - 1) * 0.5f;
@@ -298,7 +318,7 @@ __device__ __noinline__ void decode_nbit(uint32_t unit, const uint8_t* slot, int
     group_bf16<BITS>(gc[j], half, o);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const uint4 x = int(r) < rows ? make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]) : make_uint4(0, 0, 0, 0);
+      const uint4 x = seen >> r & 1u ? make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]) : make_uint4(0, 0, 0, 0);
       sts128(unit + (v ? v_off<RB>(r, 4 * k + c) : k_off<RB>(r, 4 * k + c)), x);
     }
   }
@@ -306,7 +326,7 @@ __device__ __noinline__ void decode_nbit(uint32_t unit, const uint8_t* slot, int
   const uint32_t row0 = uint32_t((v ? T : 0) + t0), shift = 31 - __clz(row_len);  // rows are powers of two
   const auto put = [&](uint32_t e) {
     const uint32_t r = (e >> 16 >> shift) - row0, c = ((e >> 16) & uint32_t(row_len - 1)) - uint32_t(hk * D);
-    if (r < uint32_t(rows) && c < uint32_t(D))
+    if (r < 16u && (seen >> r & 1u) && c < uint32_t(D))
       asm volatile("st.shared.u16 [%0], %1;" :: "r"(unit + (v ? v_off<RB>(r, c >> 3) : k_off<RB>(r, c >> 3)) + (c & 7u) * 2u),
                    "h"(static_cast<uint16_t>(e)) : "memory");
   };
@@ -331,7 +351,7 @@ struct Share {
 // are looked up eight at a time, a lane each, in four steps two pages apart
 // (position, page id, page-table columns, layer address), so that no step waits
 // for the loads of the one before it.
-template <int D>
+template <int D, bool WIN>
 struct Producer {
   using Layout = UnitLayout<D>;
   static constexpr int kLook = 8;
@@ -339,6 +359,7 @@ struct Producer {
   const int hk, sub;      // this lane's worker's key head; lane within the worker's eight
   int b, i, i0, i1;       // its sequence, next list entry, the segment's entries
   int64_t tokens;
+  Span span;              // (WIN)
   int row_pos, row_end, before;
   bool active;
   int t0;                 // first token of the next unit in its page
@@ -362,7 +383,7 @@ struct Producer {
   __device__ void open_segment() {
     int n = 0;
     for (; active; ++b) {
-      n = list_len(p, b, hk);
+      n = list_len<WIN>(p, b, hk);
       if (before + n > row_pos) break;
       before += n;
     }
@@ -370,6 +391,7 @@ struct Producer {
       i0 = i = row_pos - before;
       i1 = min(n, row_end - before);
       tokens = seq_tokens(p, b);
+      if constexpr (WIN) span = span_of(p, tokens);
     } else {
       i0 = i = i1 = 0;
       tokens = 0;
@@ -385,7 +407,8 @@ struct Producer {
     const int e = batch0 + kLook + sub;
     const bool mine = e < i1;
     if (step == 0) {
-      n_pos = mine && p.selected ? p.selected[(int64_t(b) * p.heads_kv + hk) * p.max_selected + e] : e;
+      if constexpr (WIN) n_pos = mine ? span.position(e) : e;
+      else n_pos = mine && p.selected ? p.selected[(int64_t(b) * p.heads_kv + hk) * p.max_selected + e] : e;
     } else if (step == 1) {
       const bool ok = mine && n_pos >= 0 && int64_t(n_pos) * p.T < tokens;
       n_id = ok ? p.page_ids[int64_t(b) * p.page_ids_stride + n_pos] : -1;
@@ -444,14 +467,14 @@ struct Producer {
   }
 
   // 16 rows of RB bytes, `step` bytes apart from src on, into a tile by the worker's eight lanes;
-  // rows behind `rows` become zeros.
+  // rows behind `rows` and those without a bit in `seen` become zeros.
   template <int RB, bool V>
-  __device__ __forceinline__ void copy_rows(const uint8_t* src, uint32_t step, int rows, uint32_t tile) const {
+  __device__ __forceinline__ void copy_rows(const uint8_t* src, uint32_t step, int rows, uint32_t seen, uint32_t tile) const {
     constexpr uint32_t CPR = RB / 16;                     // chunks of a row
     constexpr uint32_t LPR = CPR < 8 ? CPR : 8, RPI = 8 / LPR;  // lanes of a row, rows of one instruction
     const uint32_t r0 = uint32_t(sub) / LPR, c0 = uint32_t(sub) % LPR;
     src += r0 * step + c0 * 16u;
-    if (rows >= 16) {
+    if (rows >= 16 && (!WIN || seen == 0xFFFFu)) {
 #pragma unroll
       for (uint32_t j = 0; j < 16 / RPI; ++j) {
 #pragma unroll
@@ -464,7 +487,7 @@ struct Producer {
 #pragma unroll 1
     for (uint32_t j = 0; j < 16 / RPI; ++j) {
       const uint32_t r = r0 + RPI * j;
-      const bool real = r < uint32_t(rows);
+      const bool real = r < uint32_t(rows) && (!WIN || (seen >> r & 1u));
 #pragma unroll
       for (uint32_t c = 0; c < CPR; c += LPR)
         cp_async16_or_zero(tile + (V ? v_off<RB>(r, c0 + c) : k_off<RB>(r, c0 + c)),
@@ -535,11 +558,12 @@ struct Producer {
         const int left = int(pm >> 8) - t0;
         uint32_t h = format | uint32_t(max(0, min(left, 16))) << 8 | uint32_t(t0) << 16;
         bool done = true;  // with these tokens
+        const uint32_t seen = WIN ? seen_of(p, tokens, int64_t(pp) * p.T + t0) : 0xFFFFu;
         if (left <= 0) {
         } else if (format == ASHKV_PAGE_BF16) {
           const uint32_t step = uint32_t(p.row_stride) * 2u;
-          if (second) copy_rows<D * 2, true>(pv + uint32_t(t0) * step, step, left, unit);
-          else copy_rows<D * 2, false>(pk + uint32_t(t0) * step, step, left, unit);
+          if (second) copy_rows<D * 2, true>(pv + uint32_t(t0) * step, step, left, seen, unit);
+          else copy_rows<D * 2, false>(pk + uint32_t(t0) * step, step, left, seen, unit);
           if (second) h |= Header::kIsV;
           done = second;
           second = !second;
@@ -547,12 +571,12 @@ struct Producer {
           const bool int4 = format == ASHKV_PAGE_INT4;
           if (int4) {
             const uint8_t* codes = pk + uint32_t(t0) * (row / 2);
-            copy_rows<D / 2, false>(codes, row / 2, left, unit);
-            copy_rows<D / 2, true>(codes + T * (row / 2), row / 2, left, unit + 8 * D);
+            copy_rows<D / 2, false>(codes, row / 2, left, seen, unit);
+            copy_rows<D / 2, true>(codes + T * (row / 2), row / 2, left, seen, unit + 8 * D);
           } else {
             const uint8_t* codes = pk + uint32_t(t0) * row;
-            copy_rows<D, false>(codes, row, left, unit);
-            copy_rows<D, true>(codes + T * row, row, left, unit + 16 * D);
+            copy_rows<D, false>(codes, row, left, seen, unit);
+            copy_rows<D, true>(codes + T * row, row, left, seen, unit + 16 * D);
           }
           if (int4) {
 #pragma unroll
@@ -639,7 +663,8 @@ struct Producer {
 // keeps weight * scale inside the fp16 range: c * (largest scale so far) lies in
 // [2^6, 2^7], a weight below 2^8, so the operand stays below 2^15 and is off by at
 // most 2^-25 / c where fp16 runs out of digits, 2^-31 of a largest value.
-template <int D, int NT>
+// `rows` of a unit: how many of its first rows count, or with WIN a bit for each row that does.
+template <int D, int NT, bool WIN>
 struct Worker {
   static constexpr int MT = D / 16;  // channel tiles of 16
   static constexpr float kUnit8 = 1.0f / 127.0f, kUnit4 = 1.0f / 7.0f;  // a code's value is code * scale * unit
@@ -776,13 +801,15 @@ struct Worker {
   }
 
   // log2 scores of tokens 2t, 2t + 1, 2t + 8, 2t + 9 -> weights 2^(s - m), added up.
+  static __device__ __forceinline__ bool all_count(int rows) { return WIN ? rows == 0xFFFF : rows >= 16; }
+  static __device__ __forceinline__ bool counts(int r, int rows) { return WIN ? (rows >> r & 1) != 0 : r < rows; }
   __device__ __forceinline__ void weights(float (&s)[NT][4], int rows) {
-    if (rows < 16) {
+    if (!all_count(rows)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          if (2 * t + (x & 1) + 8 * (x >> 1) >= rows) s[n][x] = -INFINITY;
+          if (!counts(2 * t + (x & 1) + 8 * (x >> 1), rows)) s[n][x] = -INFINITY;
     }
     bool over = false;
     float top[NT];
@@ -975,7 +1002,7 @@ struct Worker {
   __device__ __forceinline__ void zero_unused(float (&x)[K][4], int rows) const {
 #pragma unroll
     for (int y = 0; y < 4; ++y)
-      if (2 * t + (y & 1) + 8 * (y >> 1) >= rows)
+      if (!counts(2 * t + (y & 1) + 8 * (y >> 1), rows))
 #pragma unroll
         for (int k = 0; k < K; ++k) x[k][y] = 0.0f;
   }
@@ -987,7 +1014,7 @@ struct Worker {
     if constexpr (INT8) {
       float ks[4];
       int8_scales(scales, ks, vs[0]);
-      if (rows < 16) zero_unused(vs, rows);
+      if (!all_count(rows)) zero_unused(vs, rows);
       fit_scale(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[0][2], vs[0][3])) * kUnit8);
       Dots a;
 #pragma unroll
@@ -1086,7 +1113,7 @@ struct Worker {
     float ks[K][4], vs[K][4];
     int4_scales(scales + 8 * t, ks);
     int4_scales(scales + 8 * t + 64, vs);
-    if (rows < 16) zero_unused(vs, rows);
+    if (!all_count(rows)) zero_unused(vs, rows);
     float top = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) top = fmaxf(top, fmaxf(fmaxf(vs[k][0], vs[k][1]), fmaxf(vs[k][2], vs[k][3])));
@@ -1184,7 +1211,7 @@ struct Worker {
 // per worker issuing boxes measured 129 against 128 us (INT8) and 68 against 63
 // (131071 INT4 tokens).  A ring of three units leaves two on their way: 24 to an
 // SM, 48 to 96 KB, which covers a microsecond of HBM's full rate.
-template <int D, int NT>
+template <int D, int NT, bool WIN>
 __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_kernel(const __grid_constant__ AttnParams p) {
   using Layout = UnitLayout<D>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -1202,13 +1229,13 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
   if (warp < kWarpsA) {
     Share sh{0, 0, 0, 0};
     if (range < p.ranges) {
-      const int total = lists_before(p, p.n_seqs, hk), len = range_len(p, total);
+      const int total = lists_before<WIN>(p, p.n_seqs, hk), len = range_len(p, total);
       const int64_t at = int64_t(range) * len;
       sh.pos = int(min(at, int64_t(total)));
       sh.end = int(min(at + len, int64_t(total)));
       if (sh.pos < sh.end) {  // the sequence that the range starts in
         for (int b0 = 0;; b0 += 32) {
-          const int n = b0 + lane < p.n_seqs ? list_len(p, b0 + lane, hk) : 0;
+          const int n = b0 + lane < p.n_seqs ? list_len<WIN>(p, b0 + lane, hk) : 0;
           int upto = n;
 #pragma unroll
           for (int off = 1; off < 32; off <<= 1) {
@@ -1238,46 +1265,50 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
   __syncthreads();
   allow_next();
   if (warp == kWarpsA) {
-    Producer<D>(p, hk, s_share[mine], ring, bars).run();
+    Producer<D, WIN>(p, hk, s_share[mine], ring, bars).run();
     return;
   }
-  Worker<D, NT> work(p, ring + Layout::kBytes, hk);
+  Worker<D, NT, WIN> work(p, ring + Layout::kBytes, hk);
   const int nq = min(8 * NT, p.group - q0), hq0 = hk * p.group + q0;
   int b = s_share[warp].b, before = s_share[warp].before, pos = s_share[warp].pos;
   const int end = s_share[warp].end;
   uint32_t slot = 0, phase = 0;
   for (; pos < end; ++b) {
-    const int n = list_len(p, b, hk);
+    const int n = list_len<WIN>(p, b, hk);
     if (n == 0) continue;
+    const int64_t tokens = WIN ? seq_tokens(p, b) : 0;
     work.start(b, hq0, nq);
     float s[NT][4];  // weights of a BF16 tile between its K and its V unit
     for (bool last = false; !last;) {
-      if (!Producer<D>::wait_bar(bars + slot * 8, phase)) {
+      if (!Producer<D, WIN>::wait_bar(bars + slot * 8, phase)) {
         flag(p.status, ASHKV_FLAG_TIMEOUT);
         return;
       }
       const uint32_t unit = ring + slot * Layout::kData, scales = ring + Layout::kScales + slot * 128;
       const uint4 h4 = lds128(ring + Layout::kHeaders + slot * 16);
       const Header h{reinterpret_cast<const uint8_t*>(uint64_t(h4.x) | uint64_t(h4.y) << 32), h4.z, int32_t(h4.w)};
-      if (h.format() >= ASHKV_PAGE_NBIT4 && h.rows()) {
-        const int t0 = int(h.meta >> 20) * 16;
+      const int t0 = int(h.meta >> 20) * 16;
+      const uint32_t first_rows = (1u << h.rows()) - 1u;
+      const uint32_t seen = WIN ? first_rows & seen_of(p, tokens, int64_t(h.pos) * p.T + t0) : first_rows;
+      const int rows = WIN ? int(seen) : h.rows();
+      if (h.format() >= ASHKV_PAGE_NBIT4 && rows) {
         const bool is_v = h.meta & Header::kIsV;
         if (h.format() == ASHKV_PAGE_NBIT4)
-          decode_nbit<D, 4>(unit, h.slot, p.T, p.row_len, p.outlier_cap, hk, is_v, t0, h.rows());
+          decode_nbit<D, 4>(unit, h.slot, p.T, p.row_len, p.outlier_cap, hk, is_v, t0, seen);
         else
-          decode_nbit<D, 2>(unit, h.slot, p.T, p.row_len, p.outlier_cap, hk, is_v, t0, h.rows());
+          decode_nbit<D, 2>(unit, h.slot, p.T, p.row_len, p.outlier_cap, hk, is_v, t0, seen);
       }
-      if (h.rows() == 0) {
+      if (rows == 0) {
       } else if (h.format() == ASHKV_PAGE_INT8) {
-        work.template tile8<true>(unit, scales, h.rows());
+        work.template tile8<true>(unit, scales, rows);
       } else if (h.format() == ASHKV_PAGE_FP8) {
-        work.template tile8<false>(unit, scales, h.rows());
+        work.template tile8<false>(unit, scales, rows);
       } else if (h.format() == ASHKV_PAGE_INT4) {
-        work.tile4(unit, scales, h.rows());
+        work.tile4(unit, scales, rows);
       } else if (h.meta & Header::kIsV) {
         work.bf16_values(unit, s);
       } else {
-        work.bf16_scores(unit, h.rows(), s);
+        work.bf16_scores(unit, rows, s);
       }
       if (p.mass && (h.meta & Header::kPageEnd) && h.rows()) work.page_sum(b, h.pos, hq0, nq);
       last = h.meta & Header::kSegmentEnd;
@@ -1299,9 +1330,10 @@ __global__ void __launch_bounds__(kThreadsA, NT == 1 ? 3 : 2) decode_partials_ke
 }
 
 // The ranges r0 .. r1 that hold pages of (sequence b, key head hk); none: r1 < r0.
+template <bool WIN>
 __device__ __forceinline__ void partials_of(const AttnParams& p, int b, int hk, int& r0, int& r1) {
   const int64_t at = int64_t(b) * p.heads_kv + hk;
-  const bool any = list_len(p, b, hk) > 0;
+  const bool any = list_len<WIN>(p, b, hk) > 0;
   r0 = min(max(p.first_range[at], 0), p.ranges - 1);
   r1 = any ? min(max(p.last_range[at], r0), p.ranges - 1) : r0 - 1;
 }
@@ -1390,7 +1422,7 @@ __device__ __forceinline__ void join_row(const AttnParams& p, int64_t row, int f
 // log2-sum of every head, then a half warp per page over the heads.  Bound by the
 // latency of three dependent loads; 4 to 10 us.
 constexpr int kMassPages = 64;
-template <int D, int W>
+template <int D, int W, bool WIN>
 __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ AttnParams p) {
   constexpr int kWarps = kJoinWarps, kRows = kWarps / W;  // rows of a block
   extern __shared__ float s_join[];  // [kWarps][D], or [heads_q] and [2][kJoinThreads]
@@ -1401,7 +1433,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
     // a block's rows lie far apart, so that the heads of one long sequence are in as many blocks
     const auto row_of = [&](int k) { return int64_t(blockIdx.x) + k * out_blocks; };
     const auto partials = [&](int64_t row, int& r0, int& r1) {
-      partials_of(p, int(row / p.heads_q), int(row % p.heads_q) / p.group, r0, r1);
+      partials_of<WIN>(p, int(row / p.heads_q), int(row % p.heads_q) / p.group, r0, r1);
     };
     int r0 = 0, r1 = -1;
     if constexpr (W == 1) {
@@ -1433,7 +1465,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
     float m = -INFINITY, l = 0.0f;
     if (hq < p.heads_q) {
       int r0, r1;
-      partials_of(p, b, hq / p.group, r0, r1);
+      partials_of<WIN>(p, b, hq / p.group, r0, r1);
 #pragma unroll 4
       for (int r = r0 + warp; r <= r1; r += kWarps)
         merge_lse2(m, l, p.part_lse2[int64_t(r + b) * p.heads_q + hq], 1.0f);
@@ -1450,9 +1482,11 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
     __syncthreads();
   }
   const int half = tid >> 4, sub = tid & 15;
+  Span span;
+  if constexpr (WIN) span = span_of(p, seq_tokens(p, b));
   for (int j = j0 + half; j - half < j1; j += kJoinThreads / 16) {
     float sum = 0.0f;
-    if (j < j1) {
+    if (j < j1 && (!WIN || j < span.sinks || j >= span.sinks + span.skip)) {  // (pages that nobody sees draw nothing)
       const float* pl = p.page_lse2 + (int64_t(b) * p.max_pages + j) * p.heads_q;
       for (int h = sub; h < p.heads_q; h += 16)
         if (pl[h] != -INFINITY) sum += ex2(pl[h] - s_total[h]);
@@ -1482,47 +1516,6 @@ int q_chunks_for(int heads_q, int heads_kv) {
   return (group + n - 1) / n;
 }
 
-bool row_ok(int64_t row) { return row == 128 || row == 256 || row == 512 || row == 1024 || row == 2048; }
-
-// The page description of a call; the message of what is wrong with it, or nullptr.
-const char* copy_pages(const ashkv_paged_kv_t* kv, AttnParams& p) {
-  if (!kv) return "null page description";
-  if (kv->head_dim != 64 && kv->head_dim != 128) return "head_dim must be 64 or 128";
-  if (kv->heads_kv <= 0 || kv->tokens_per_page <= 0 || kv->n_layers <= 0 || kv->n_pages < 0 || kv->pool_tokens < 0 ||
-      kv->outlier_cap < 0 || kv->tokens_per_page > 65536 || kv->heads_kv > 65536)
-    return "heads_kv, tokens_per_page and n_layers must be positive, sizes not negative";
-  const int64_t row = int64_t(kv->heads_kv) * kv->head_dim;
-  if (row > 0x7FFFFFFF || kv->row_stride > 0x3FFFFFFF || kv->tokens_per_page * kv->row_stride > 0x3FFFFFFF)
-    return "a page must span less than 2^31 bytes";
-  if (kv->row_stride < row || kv->row_stride % 8) return "row_stride must be a multiple of 8 and at least heads_kv * head_dim";
-  if (!kv->d_tier || !kv->d_layer_id || !kv->d_token_start || !kv->d_page_slot || !kv->d_layer_k || !kv->d_layer_v)
-    return "null device pointer";
-  if (!copy_stores(kv->stores, p.store, true)) return "bad tier store table (store 0 must be the BF16 pool)";
-  bool any = false;
-  for (int t = 1; t < kTiers; ++t) {
-    if (p.store[t].format == ASHKV_PAGE_NONE) continue;
-    any = true;
-    if (p.store[t].slot_bytes < ashkv_page_slot_bytes(p.store[t].format, kv->tokens_per_page, int32_t(row), kv->outlier_cap))
-      return "a tier store's slots are smaller than its format needs";
-  }
-  const int64_t E = 2 * int64_t(kv->tokens_per_page) * row;
-  if (any && (!row_ok(row) || E % 1024 || E > 65536))
-    return "with stores heads_kv * head_dim must be 128, 256, 512, 1024 or 2048 and a page a multiple of 1024 and at "
-           "most 65536 elements";
-  p.tier = kv->d_tier; p.layer_id = kv->d_layer_id; p.token_start = kv->d_token_start; p.page_slot = kv->d_page_slot;
-  p.n_pages = kv->n_pages; p.layer_k = kv->d_layer_k; p.layer_v = kv->d_layer_v;
-  p.pool_tokens = kv->pool_tokens; p.row_stride = kv->row_stride; p.n_layers = kv->n_layers;
-  p.T = kv->tokens_per_page; p.row_len = int32_t(row); p.outlier_cap = kv->outlier_cap; p.heads_kv = kv->heads_kv;
-  return nullptr;
-}
-
-ashkv_status_t refuse(const char* what, const char* why) {
-  char text[256];
-  snprintf(text, sizeof text, "%s: %s", what, why);
-  set_message(text);
-  return ASHKV_BAD_ARGUMENT;
-}
-
 // Warps of a result row in the join.  One warp per row makes eight times fewer CTAs and needs no second
 // sum, eight read a row's partials at once.  Calls with one / eight warps, by partials to a row: 1.7 (128 x
 // 1024 bf16 tokens, 64 heads) 109 / 129 us; 3.5 (64 x 2048 INT8) 79 / 88; 7 (32 x 8192 bf16) 183 / 186; 9 (24 x
@@ -1530,7 +1523,7 @@ ashkv_status_t refuse(const char* what, const char* why) {
 // One sequence of 131072 among 31 of 30 tokens: 219 / 213 (230 if its rows had one warp each).
 int join_warps(const AttnParams& p) { return p.ranges <= int64_t(p.n_seqs) * 10 ? 1 : 8; }
 
-template <int D, int NT>
+template <int D, int NT, bool WIN>
 ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
   const int64_t workers = int64_t(p.ranges) * p.heads_kv * p.q_chunks;
   p.warp_smem = int(UnitLayout<D>::kBytes) + NT * 8 * D * (2 + (p.fp8_pages ? 2 : 0) + (p.int_pages ? 3 : 0));
@@ -1543,14 +1536,14 @@ ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !allowed[dev].load(std::memory_order_acquire))) {
     constexpr int kMost = kWarpsA * ((int(UnitLayout<D>::kBytes) + NT * 8 * D * 7 + 1023) / 1024 * 1024) + 1024;
-    e = cudaFuncSetAttribute(decode_partials_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    e = cudaFuncSetAttribute(decode_partials_kernel<D, NT, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (e == cudaSuccess && dev < 64) allowed[dev].store(true, std::memory_order_release);
   }
   if (e != cudaSuccess) {
     set_error("ashkv_decode_attention (shared memory attribute)", e);
     return ASHKV_LAUNCH_ERROR;
   }
-  launch_overlapped(decode_partials_kernel<D, NT>, dim3(unsigned((workers + kWarpsA - 1) / kWarpsA)), dim3(kThreadsA),
+  launch_overlapped(decode_partials_kernel<D, NT, WIN>, dim3(unsigned((workers + kWarpsA - 1) / kWarpsA)), dim3(kThreadsA),
                     size_t(smem), st, p);
   const ashkv_status_t rc = check_launch("ashkv_decode_attention");
   if (rc != ASHKV_OK) return rc;
@@ -1562,7 +1555,7 @@ ashkv_status_t launch_decode(AttnParams& p, cudaStream_t st) {
     blocks += int64_t(p.n_seqs) * ((p.max_pages + kMassPages - 1) / kMassPages);
     join_smem = std::max(join_smem, size_t(p.heads_q + 2 * kJoinThreads) * 4);
   }
-  launch_overlapped(w == 1 ? decode_join_kernel<D, 1> : decode_join_kernel<D, 8>, dim3(unsigned(blocks)), dim3(kJoinThreads),
+  launch_overlapped(w == 1 ? decode_join_kernel<D, 1, WIN> : decode_join_kernel<D, 8, WIN>, dim3(unsigned(blocks)), dim3(kJoinThreads),
                     join_smem, st, p);
   return check_launch("ashkv_decode_attention");
 }
@@ -1582,12 +1575,12 @@ extern "C" int64_t ashkv_decode_scratch_floats(int32_t n_seqs, int32_t heads_q, 
   return n;
 }
 
-extern "C" ashkv_status_t ashkv_decode_attention(
+static ashkv_status_t decode_call(
+    const char* kName, int32_t window, int32_t sinks,
     const ashkv_paged_kv_t* kv, const void* d_q, int64_t q_seq_stride, int64_t q_head_stride, int32_t n_seqs,
     int32_t heads_q, const int32_t* d_page_ids, int64_t page_ids_stride, int32_t max_pages, const int32_t* d_lengths,
     const int32_t* d_selected, const int32_t* d_selected_count, int32_t max_selected, float scale, float* d_page_mass,
     int64_t mass_stride, float decay, void* d_out, float* d_lse, float* d_scratch, uint32_t* d_status, void* stream) {
-  constexpr const char* kName = "ashkv_decode_attention";
   AttnParams p{};
   if (const char* why = copy_pages(kv, p)) return refuse(kName, why);
   if (n_seqs < 0 || max_pages < 0 || heads_q <= 0 || heads_q % p.heads_kv)
@@ -1596,6 +1589,7 @@ extern "C" ashkv_status_t ashkv_decode_attention(
   const int64_t width = d_selected ? max_selected : max_pages;
   if (width < 0 || int64_t(n_seqs) * width > kMostEntries || int64_t(n_seqs) * max_pages > kMostEntries)
     return refuse(kName, "too many list entries");
+  if (window < 0 || sinks < 0) return refuse(kName, "window must be at least 1, sinks not negative");
   if (d_selected && (!d_selected_count || d_page_mass)) return refuse(kName, "d_selected needs its counts and takes no mass");
   if (n_seqs == 0) return ASHKV_OK;
   if (!d_q || (!d_page_ids && max_pages > 0) || !d_lengths || !d_out || !d_scratch || !aligned(d_scratch, 16))
@@ -1616,7 +1610,12 @@ extern "C" ashkv_status_t ashkv_decode_attention(
     p.int_pages |= p.store[t].format == ASHKV_PAGE_INT8 || p.store[t].format == ASHKV_PAGE_INT4;
   }
   const bool two_ctas = worker_queries(p.group) == 16 || (p.fp8_pages && p.int_pages);
-  p.ranges = ranges_for(n_seqs, p.heads_kv, p.q_chunks, width, two_ctas ? 2 * kWarpsA : kWorkersPerSm);
+  p.window = window;
+  p.sinks = sinks;
+  // entries of the longest list (at most max_pages, for which the scratch is asked for)
+  const int64_t entries =
+      window ? std::min<int64_t>(width, (int64_t(sinks) + p.T - 1) / p.T + (int64_t(window) + p.T - 1) / p.T + 1) : width;
+  p.ranges = ranges_for(n_seqs, p.heads_kv, p.q_chunks, entries, two_ctas ? 2 * kWarpsA : kWorkersPerSm);
   const int64_t rows = (int64_t(p.ranges) + n_seqs) * heads_q;
   p.part_o = d_scratch;
   p.part_lse2 = p.part_o + rows * kv->head_dim;
@@ -1624,6 +1623,32 @@ extern "C" ashkv_status_t ashkv_decode_attention(
   p.last_range = p.first_range + int64_t(n_seqs) * p.heads_kv;
   p.page_lse2 = reinterpret_cast<float*>(p.last_range + int64_t(n_seqs) * p.heads_kv);
   cudaStream_t st = as_stream(stream);
-  if (worker_queries(p.group) == 8) return kv->head_dim == 64 ? launch_decode<64, 1>(p, st) : launch_decode<128, 1>(p, st);
-  return kv->head_dim == 64 ? launch_decode<64, 2>(p, st) : launch_decode<128, 2>(p, st);
+  const auto launch = [&](auto win) {
+    constexpr bool WIN = decltype(win)::value;
+    if (worker_queries(p.group) == 8) return kv->head_dim == 64 ? launch_decode<64, 1, WIN>(p, st) : launch_decode<128, 1, WIN>(p, st);
+    return kv->head_dim == 64 ? launch_decode<64, 2, WIN>(p, st) : launch_decode<128, 2, WIN>(p, st);
+  };
+  return window ? launch(std::true_type()) : launch(std::false_type());
+}
+
+extern "C" ashkv_status_t ashkv_decode_attention(
+    const ashkv_paged_kv_t* kv, const void* d_q, int64_t q_seq_stride, int64_t q_head_stride, int32_t n_seqs,
+    int32_t heads_q, const int32_t* d_page_ids, int64_t page_ids_stride, int32_t max_pages, const int32_t* d_lengths,
+    const int32_t* d_selected, const int32_t* d_selected_count, int32_t max_selected, float scale, float* d_page_mass,
+    int64_t mass_stride, float decay, void* d_out, float* d_lse, float* d_scratch, uint32_t* d_status, void* stream) {
+  return decode_call("ashkv_decode_attention", 0, 0, kv, d_q, q_seq_stride, q_head_stride, n_seqs, heads_q, d_page_ids,
+                     page_ids_stride, max_pages, d_lengths, d_selected, d_selected_count, max_selected, scale, d_page_mass,
+                     mass_stride, decay, d_out, d_lse, d_scratch, d_status, stream);
+}
+
+extern "C" ashkv_status_t ashkv_decode_attention_window(
+    const ashkv_paged_kv_t* kv, const void* d_q, int64_t q_seq_stride, int64_t q_head_stride, int32_t n_seqs,
+    int32_t heads_q, const int32_t* d_page_ids, int64_t page_ids_stride, int32_t max_pages, const int32_t* d_lengths,
+    int32_t window, int32_t sinks, float scale, float* d_page_mass, int64_t mass_stride, float decay, void* d_out,
+    float* d_lse, float* d_scratch, uint32_t* d_status, void* stream) {
+  constexpr const char* kName = "ashkv_decode_attention_window";
+  if (window < 1) return refuse(kName, "window must be at least 1");
+  return decode_call(kName, window, sinks, kv, d_q, q_seq_stride, q_head_stride, n_seqs, heads_q, d_page_ids, page_ids_stride,
+                     max_pages, d_lengths, nullptr, nullptr, 0, scale, d_page_mass, mass_stride, decay, d_out, d_lse,
+                     d_scratch, d_status, stream);
 }

@@ -1,0 +1,343 @@
+// New tokens into tiered pages, and tokens of tiered pages into dense rows (ashkv_write_kv,
+// ashkv_read_kv).
+//
+// Writing quantises a token where its page lies: with x the token's K or V row (row_len values),
+//   BF16 the row itself;  INT8: scale = fp16(max(max |x|, 1e-8)), codes as the INT8 codec's;
+//   FP8: e4m3 codes;      INT4: a scale and nibbles for every 64 values, as INT4Codec's,
+// the same bytes that a migration of the finished page writes.  Reading decodes them as a
+// promotion does.  A row of either is independent of its neighbours, so a warp takes a token: it
+// finds the sequence of its row (32 starts at a time), the page, its table columns and address,
+// a chain of loads that the loads of a written token's rows do not wait for, then encodes or
+// decodes K and V in chunks of eight values a lane.
+#include <algorithm>
+
+#include "common.cuh"
+#include "page_codec.cuh"
+#include "paged_kv.cuh"
+
+namespace ashkv {
+namespace {
+
+constexpr int kThreadsC = 256;
+
+struct WriteParams {
+  PagedKV kv;
+  PageLists lists;
+  int64_t n_rows;
+  const uint16_t *k, *v;  // with their strides in elements
+  int64_t k_row, k_head, v_row, v_head;
+  int32_t head_dim;
+  bool wide;  // 16-byte loads
+};
+struct ReadParams {
+  PagedKV kv;
+  PageLists lists;
+  int64_t n_rows;
+  uint16_t *k, *v;  // [n_rows, row_len]
+};
+
+// Eight values of a row at column c (a chunk never crosses a head).
+__device__ __forceinline__ uint4 load_chunk(const uint16_t* row, int64_t head_stride, int head_dim, int c, bool wide) {
+  const uint16_t* at = row + int64_t(c / head_dim) * head_stride + c % head_dim;
+  if (wide) return ld_v4(at);
+  uint16_t x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = at[j];
+  return make_uint4(x[0] | uint32_t(x[1]) << 16, x[2] | uint32_t(x[3]) << 16, x[4] | uint32_t(x[5]) << 16, x[6] | uint32_t(x[7]) << 16);
+}
+
+// The place of row i's token (warp-collective): its page, and its token there.  False: no such row or page.
+__device__ __forceinline__ bool token_of(const PagedKV& kv, const PageLists& l, int64_t i, Place& at, int& t, bool& row_of_none) {
+  const int b = sequence_of(l, i);
+  row_of_none = b < 0;
+  if (b < 0) return false;
+  const int64_t pos = int64_t(l.lengths[b]) - (int64_t(l.starts[b + 1]) - i);
+  at.format = -1;
+  if (pos >= 0) {
+    const int64_t j = pos / kv.T;
+    t = int(pos - j * kv.T);
+    if (j < l.max_pages) at = place_of(kv, l.page_ids[int64_t(b) * l.page_ids_stride + j]);
+  }
+  if (at.format >= 0) return true;
+  if ((threadIdx.x & 31) == 0) flag(l.status, ASHKV_FLAG_INDEX_RANGE);
+  return false;
+}
+
+// Rows of ROW values by TEAM lanes, N chunks a lane (chunk j * TEAM + the lane's place).  With 16
+// lanes to a row a warp holds K and V side by side, else one after the other.
+template <int ROW>
+struct RowShape {
+  static constexpr int kTeam = ROW >= 256 ? 32 : ROW / 8, kChunks = ROW / 8 / kTeam, kPasses = kTeam == 32 ? 2 : 1;
+  static_assert(ROW % 128 == 0, "a team of 16 or 32 lanes");
+};
+
+// A row (r of the page's 2 T) in registers -> the slot.
+template <int ROW>
+__device__ __forceinline__ void encode_row(const PagedKV& p, const Place& at, int r, int lin, const uint32_t (&w)[RowShape<ROW>::kChunks * 4]) {
+  constexpr int TEAM = RowShape<ROW>::kTeam, N = RowShape<ROW>::kChunks;
+  if (at.format == ASHKV_PAGE_BF16) {
+    const bool v = r >= p.T;
+    uint4* to = reinterpret_cast<uint4*>((v ? at.v : at.k) + int64_t(v ? r - p.T : r) * p.row_stride * 2);
+#pragma unroll
+    for (int c = 0; c < N; ++c) to[c * TEAM + lin] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+  } else if (at.format == ASHKV_PAGE_INT8) {
+    const float am = fmaxf(team_absmax_bf16<TEAM>(w), 1e-8f);
+    if (lin == 0) reinterpret_cast<uint16_t*>(at.k)[r] = f32_to_f16(am);
+    const Int8Div d = int8_div(am);
+    uint2* to = reinterpret_cast<uint2*>(at.k + int8_codes_offset(p.T) + int64_t(r) * ROW);
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      to[c * TEAM + lin] = make_uint2(int8_codes4_bf16(w[4 * c], w[4 * c + 1], d), int8_codes4_bf16(w[4 * c + 2], w[4 * c + 3], d));
+  } else if (at.format == ASHKV_PAGE_FP8) {
+    uint2* to = reinterpret_cast<uint2*>(at.k + int64_t(r) * ROW);
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      to[c * TEAM + lin] = make_uint2(fp8x2_from_bf16x2(w[4 * c]) | (fp8x2_from_bf16x2(w[4 * c + 1]) << 16),
+                                      fp8x2_from_bf16x2(w[4 * c + 2]) | (fp8x2_from_bf16x2(w[4 * c + 3]) << 16));
+  } else {  // INT4: a group of 64 values is eight chunks, the chunks of eight neighbouring lanes
+    const int64_t E = 2 * int64_t(p.T) * ROW;
+    uint16_t* scales = reinterpret_cast<uint16_t*>(at.k) + int64_t(r) * (ROW / 64);
+    uint32_t* to = reinterpret_cast<uint32_t*>(at.k + E / 32 + int64_t(r) * (ROW / 2));
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      float x[8];
+      unpack_chunk(make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]), x);
+      float m = chunk_max(0.0f, x);
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
+      const float am = group_max_finish(m);
+      if (lin % 8 == 0) scales[(c * TEAM + lin) / 8] = static_cast<uint16_t>(bf16_cpu(am));
+      to[c * TEAM + lin] = pack_chunk(x, group_div(am));
+    }
+  }
+}
+
+// Bound by HBM (reads 4 bytes, writes 1 to 4 a pair of values) and, for few rows, by the chain of loads
+// that finds a page.
+template <int ROW>
+__global__ void __launch_bounds__(kThreadsC) write_kv_kernel(const __grid_constant__ WriteParams p) {
+  constexpr int TEAM = RowShape<ROW>::kTeam, N = RowShape<ROW>::kChunks, PASSES = RowShape<ROW>::kPasses;
+  const int lane = threadIdx.x & 31, lin = lane % TEAM;
+  const int64_t i = int64_t(blockIdx.x) * (kThreadsC / 32) + (threadIdx.x >> 5);
+  wait_for_previous();
+  allow_next();
+  if (i >= p.n_rows) return;
+  uint32_t w[PASSES][4 * N];
+#pragma unroll
+  for (int half = 0; half < PASSES; ++half) {
+    const bool v = PASSES == 2 ? half : lane >= TEAM;
+    const uint16_t* row = v ? p.v + i * p.v_row : p.k + i * p.k_row;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const uint4 x = load_chunk(row, v ? p.v_head : p.k_head, p.head_dim, (c * TEAM + lin) * 8, p.wide);
+      w[half][4 * c] = x.x; w[half][4 * c + 1] = x.y; w[half][4 * c + 2] = x.z; w[half][4 * c + 3] = x.w;
+    }
+  }
+  Place at;
+  int t;
+  bool none;
+  if (!token_of(p.kv, p.lists, i, at, t, none)) return;
+  if (at.format >= ASHKV_PAGE_NBIT4) {  // a dithered page is coded as a whole
+    if (lane == 0) flag(p.lists.status, ASHKV_FLAG_INDEX_RANGE);
+    return;
+  }
+#pragma unroll
+  for (int half = 0; half < PASSES; ++half)
+    encode_row<ROW>(p.kv, at, t + ((PASSES == 2 ? half : lane >= TEAM) ? p.kv.T : 0), lin, w[half]);
+}
+
+// Rows of any multiple of eight values, without stores: copies into the pool.
+__global__ void __launch_bounds__(kThreadsC) write_pool_kernel(const __grid_constant__ WriteParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t i = int64_t(blockIdx.x) * (kThreadsC / 32) + (threadIdx.x >> 5);
+  wait_for_previous();
+  allow_next();
+  if (i >= p.n_rows) return;
+  Place at;
+  int t;
+  bool none;
+  if (!token_of(p.kv, p.lists, i, at, t, none)) return;
+  const int64_t off = int64_t(t) * p.kv.row_stride * 2;
+  for (int half = 0; half < 2; ++half) {
+    const uint16_t* row = half ? p.v + i * p.v_row : p.k + i * p.k_row;
+    uint4* to = reinterpret_cast<uint4*>((half ? at.v : at.k) + off);
+#pragma unroll 4
+    for (int c = lane; c < p.kv.row_len / 8; c += 32)
+      to[c] = load_chunk(row, half ? p.v_head : p.k_head, p.head_dim, c * 8, p.wide);
+  }
+}
+
+// The outliers of row r of a dithered page over its decoded values (by the warp that wrote those).
+template <int BITS>
+__device__ __forceinline__ void overlay_row(const PagedKV& p, const uint8_t* slot, int64_t E, int r, uint16_t* out) {
+  const uint32_t n = min(*reinterpret_cast<const uint32_t*>(slot), uint32_t(p.outlier_cap));
+  const uint32_t* entries = reinterpret_cast<const uint32_t*>(slot + nbit_entries_off(E, BITS));
+  const uint32_t first = uint32_t(r) * uint32_t(p.row_len);
+  for (uint32_t j = threadIdx.x & 31; j < n; j += 32) {
+    const uint32_t e = entries[j], c = (e >> 16) - first;
+    if (c < uint32_t(p.row_len)) out[c] = uint16_t(e);
+  }
+}
+
+template <int ROW>
+__global__ void __launch_bounds__(kThreadsC) read_kv_kernel(const __grid_constant__ ReadParams p) {
+  constexpr int TEAM = RowShape<ROW>::kTeam, N = RowShape<ROW>::kChunks, PASSES = RowShape<ROW>::kPasses;
+  const int lane = threadIdx.x & 31, lin = lane % TEAM;
+  const int64_t i = int64_t(blockIdx.x) * (kThreadsC / 32) + (threadIdx.x >> 5);
+  wait_for_previous();
+  allow_next();
+  if (i >= p.n_rows) return;
+  Place at;
+  int t;
+  bool none;
+  const bool real = token_of(p.kv, p.lists, i, at, t, none);
+  if (none) return;
+  const PagedKV& kv = p.kv;
+  const int T = kv.T;
+  const int64_t E = 2 * int64_t(T) * ROW;
+  uint4 x[PASSES][N];
+  const auto row_of = [&](int half) { return t + ((PASSES == 2 ? half != 0 : lane >= TEAM) ? T : 0); };
+  const auto each = [&](auto decode) {  // decode(row of the page, chunk)
+#pragma unroll
+    for (int half = 0; half < PASSES; ++half)
+#pragma unroll
+      for (int c = 0; c < N; ++c) x[half][c] = decode(row_of(half), c * TEAM + lin);
+  };
+  if (!real) {
+    each([&](int, int) { return make_uint4(0, 0, 0, 0); });
+  } else if (at.format == ASHKV_PAGE_BF16) {
+    each([&](int r, int c) {
+      const bool v = r >= T;
+      return ld_v4((v ? at.v : at.k) + (int64_t(v ? r - T : r) * kv.row_stride + c * 8) * 2);
+    });
+  } else if (at.format == ASHKV_PAGE_INT8) {
+    const uint8_t* codes = at.k + int8_codes_offset(T);
+    uint2 q[PASSES][N];
+    float s[PASSES];
+#pragma unroll
+    for (int half = 0; half < PASSES; ++half) {
+      s[half] = f16_to_f32(reinterpret_cast<const uint16_t*>(at.k)[row_of(half)]);
+#pragma unroll
+      for (int c = 0; c < N; ++c) q[half][c] = *reinterpret_cast<const uint2*>(codes + int64_t(row_of(half)) * ROW + (c * TEAM + lin) * 8);
+    }
+#pragma unroll
+    for (int half = 0; half < PASSES; ++half)
+#pragma unroll
+      for (int c = 0; c < N; ++c) x[half][c] = int8_dec8(q[half][c], s[half]);
+  } else if (at.format == ASHKV_PAGE_FP8) {
+    each([&](int r, int c) { return fp8_dec8(*reinterpret_cast<const uint2*>(at.k + int64_t(r) * ROW + c * 8)); });
+  } else if (at.format == ASHKV_PAGE_INT4) {
+    each([&](int r, int c) {
+      return int4_dec8(*reinterpret_cast<const uint32_t*>(at.k + E / 32 + int64_t(r) * (ROW / 2) + c * 4),
+                       reinterpret_cast<const uint16_t*>(at.k)[r * (ROW / 64) + c / 8]);
+    });
+  } else if (at.format == ASHKV_PAGE_NBIT4) {
+    each([&](int r, int c) {
+      const int64_t g = int64_t(r) * (ROW / 8) + c;  // chunk of the page
+      return nbit_dec8<4>(*reinterpret_cast<const uint32_t*>(at.k + nbit_codes_off(E) + g * 4),
+                          reinterpret_cast<const uint16_t*>(at.k + nbit_delta_off())[g / 4]);
+    });
+  } else {
+    each([&](int r, int c) {
+      const int64_t g = int64_t(r) * (ROW / 8) + c;
+      return nbit_dec8<2>(*reinterpret_cast<const uint16_t*>(at.k + nbit_codes_off(E) + g * 2),
+                          reinterpret_cast<const uint16_t*>(at.k + nbit_delta_off())[g / 4]);
+    });
+  }
+#pragma unroll
+  for (int half = 0; half < PASSES; ++half) {
+    uint16_t* out = (PASSES == 2 ? half != 0 : lane >= TEAM) ? p.v + i * ROW : p.k + i * ROW;
+#pragma unroll
+    for (int c = 0; c < N; ++c) st_cs_v4(out + (c * TEAM + lin) * 8, x[half][c]);
+  }
+  if (real && at.format >= ASHKV_PAGE_NBIT4) {
+    __syncwarp();  // the decoded values lie under the outliers
+    for (int half = 0; half < 2; ++half) {
+      uint16_t* out = half ? p.v + i * ROW : p.k + i * ROW;
+      if (at.format == ASHKV_PAGE_NBIT4) overlay_row<4>(kv, at.k, E, t + half * T, out);
+      else overlay_row<2>(kv, at.k, E, t + half * T, out);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kThreadsC) read_pool_kernel(const __grid_constant__ ReadParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t i = int64_t(blockIdx.x) * (kThreadsC / 32) + (threadIdx.x >> 5);
+  wait_for_previous();
+  allow_next();
+  if (i >= p.n_rows) return;
+  Place at;
+  int t;
+  bool none;
+  const bool real = token_of(p.kv, p.lists, i, at, t, none);
+  if (none) return;
+  for (int half = 0; half < 2; ++half) {
+    const uint8_t* from = (half ? at.v : at.k) + (real ? int64_t(t) * p.kv.row_stride * 2 : 0);
+    uint16_t* out = (half ? p.v : p.k) + i * p.kv.row_len;
+#pragma unroll 4
+    for (int c = lane; c < p.kv.row_len / 8; c += 32)
+      st_cs_v4(out + c * 8, real ? ld_v4(from + c * 16) : make_uint4(0, 0, 0, 0));
+  }
+}
+
+int64_t blocks_of(int64_t n_rows) { return (n_rows + kThreadsC / 32 - 1) / (kThreadsC / 32); }
+
+}  // namespace
+}  // namespace ashkv
+
+using namespace ashkv;
+
+extern "C" ashkv_status_t ashkv_write_kv(const ashkv_paged_kv_t* kv, const void* d_k, int64_t k_row_stride,
+                                         int64_t k_head_stride, const void* d_v, int64_t v_row_stride,
+                                         int64_t v_head_stride, int64_t n_rows, const int32_t* d_page_ids,
+                                         int64_t page_ids_stride, int32_t max_pages, const int32_t* d_lengths,
+                                         const int32_t* d_starts, int32_t n_seqs, uint32_t* d_status, void* stream) {
+  constexpr const char* kName = "ashkv_write_kv";
+  WriteParams p{};
+  if (const char* why = copy_pages(kv, p.kv, true)) return refuse(kName, why);
+  if (const char* why = copy_lists(d_page_ids, page_ids_stride, max_pages, d_lengths, d_starts, n_seqs, n_rows, d_status, p.lists))
+    return refuse(kName, why);
+  if (n_rows == 0 || n_seqs == 0) return ASHKV_OK;
+  if (!d_k || !d_v || !aligned(d_k, 2) || !aligned(d_v, 2)) return refuse(kName, "null or misaligned device pointer");
+  p.n_rows = n_rows;
+  p.k = static_cast<const uint16_t*>(d_k); p.v = static_cast<const uint16_t*>(d_v);
+  p.k_row = k_row_stride; p.k_head = k_head_stride; p.v_row = v_row_stride; p.v_head = v_head_stride;
+  p.head_dim = kv->head_dim;
+  p.wide = aligned(d_k, 16) && aligned(d_v, 16) && k_row_stride % 8 == 0 && v_row_stride % 8 == 0 && k_head_stride % 8 == 0 &&
+           v_head_stride % 8 == 0;
+  void (*kernel)(WriteParams) = write_pool_kernel;
+  switch (p.kv.row_len) {
+    case 128: kernel = write_kv_kernel<128>; break;
+    case 256: kernel = write_kv_kernel<256>; break;
+    case 512: kernel = write_kv_kernel<512>; break;
+    case 1024: kernel = write_kv_kernel<1024>; break;
+    case 2048: kernel = write_kv_kernel<2048>; break;
+  }
+  launch_paged(kernel, blocks_of(n_rows), kThreadsC, 0, stream, p);
+  return check_launch(kName);
+}
+
+extern "C" ashkv_status_t ashkv_read_kv(const ashkv_paged_kv_t* kv, const int32_t* d_page_ids, int64_t page_ids_stride,
+                                        int32_t max_pages, const int32_t* d_lengths, const int32_t* d_starts,
+                                        int32_t n_seqs, int64_t n_rows, void* d_k, void* d_v, uint32_t* d_status,
+                                        void* stream) {
+  constexpr const char* kName = "ashkv_read_kv";
+  ReadParams p{};
+  if (const char* why = copy_pages(kv, p.kv, true)) return refuse(kName, why);
+  if (const char* why = copy_lists(d_page_ids, page_ids_stride, max_pages, d_lengths, d_starts, n_seqs, n_rows, d_status, p.lists))
+    return refuse(kName, why);
+  if (n_rows == 0 || n_seqs == 0) return ASHKV_OK;
+  if (!d_k || !d_v || !aligned(d_k, 16) || !aligned(d_v, 16)) return refuse(kName, "null or misaligned device pointer");
+  p.n_rows = n_rows;
+  p.k = static_cast<uint16_t*>(d_k); p.v = static_cast<uint16_t*>(d_v);
+  void (*kernel)(ReadParams) = read_pool_kernel;
+  switch (p.kv.row_len) {
+    case 128: kernel = read_kv_kernel<128>; break;
+    case 256: kernel = read_kv_kernel<256>; break;
+    case 512: kernel = read_kv_kernel<512>; break;
+    case 1024: kernel = read_kv_kernel<1024>; break;
+    case 2048: kernel = read_kv_kernel<2048>; break;
+  }
+  launch_paged(kernel, blocks_of(n_rows), kThreadsC, 0, stream, p);
+  return check_launch(kName);
+}

@@ -44,6 +44,7 @@
 #include "fp8_conv.cuh"
 #include "int4_group.cuh"
 #include "nbit_group.cuh"
+#include "page_codec.cuh"
 #include "page_layout.cuh"
 
 namespace ashkv {
@@ -147,41 +148,6 @@ __device__ __forceinline__ uint2 ld_nc_v2(const void* p) {
   uint2 r;
   asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
   return r;
-}
-
-// ---------------------------------------------------------------- 8-element decoders
-// Eight INT8 codes with scale s -> eight bf16 (the reference decode).
-__device__ __forceinline__ uint4 int8_dec8(uint2 cw, float s) {
-  const Recip y = make_recip(127.0f);
-  const f2 YHI = pk2(y.hi, y.hi), YLO = pk2(y.lo, y.lo), S = pk2(s, s);
-  const bool fast = int8_dec_fast(s);
-  const uint32_t ww[2] = {cw.x, cw.y};
-  uint32_t o[4];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    f2 F0, F1;
-    int8x4_to_f2(ww[h], F0, F1);
-    if (fast) {
-      o[2 * h] = f32x2_to_bf16x2_pk(div2_short(mul2(F0, S), YHI, YLO));
-      o[2 * h + 1] = f32x2_to_bf16x2_pk(div2_short(mul2(F1, S), YHI, YLO));
-    } else {
-      float a, b;
-      upk2(F0, a, b);
-      o[2 * h] = f32x2_to_bf16x2(__fdiv_rn(__fmul_rn(a, s), 127.0f), __fdiv_rn(__fmul_rn(b, s), 127.0f));
-      upk2(F1, a, b);
-      o[2 * h + 1] = f32x2_to_bf16x2(__fdiv_rn(__fmul_rn(a, s), 127.0f), __fdiv_rn(__fmul_rn(b, s), 127.0f));
-    }
-  }
-  return make_uint4(o[0], o[1], o[2], o[3]);
-}
-__device__ __forceinline__ uint4 fp8_dec8(uint2 c) {
-  return make_uint4(bf16x2_from_fp8x2(c.x & 0xFFFFu), bf16x2_from_fp8x2(c.x >> 16),
-                    bf16x2_from_fp8x2(c.y & 0xFFFFu), bf16x2_from_fp8x2(c.y >> 16));
-}
-__device__ __forceinline__ uint4 int4_dec8(uint32_t c, uint16_t scale) {
-  uint32_t o[4];
-  unpack_nibbles8(c, bf16_to_f32(scale), o);
-  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // ---------------------------------------------------------------- decoders (slot -> staging)
@@ -475,31 +441,13 @@ __device__ void pool_from_nbit(const MigParams& p, const Entry& en, const uint8_
 // outliers in a sorted list; `first[g]` is the first list entry of group g or
 // later (built once per page), so a chunk finds its outliers in a few steps.
 
-// Eight codes of a dithered group (chunk c of group g) -> eight bf16, as group_bf16 decodes them.
+// Chunk k (eight codes of a dithered group) -> eight bf16, as group_bf16 decodes them.
 template <int BITS>
 __device__ __forceinline__ uint4 nbit_chunk(const uint8_t* raw, int64_t E, int k) {
-  constexpr float half = float((1 << BITS) - 1) * 0.5f;
-  const int g = k >> 2, c = k & 3;
-  const float delta = bf16_to_f32(reinterpret_cast<const uint16_t*>(raw + nbit_delta_off())[g]);
-  const f2 DEL = pk2(delta, delta), NH = pk2(-half, -half), N23 = pk2(-8388608.0f, -8388608.0f);
-  auto pair = [&](float a, float b) { return f32x2_to_bf16x2_pk(mul2(add2(add2(pk2(a, b), N23), NH), DEL)); };
-  const uint8_t* codes = raw + nbit_codes_off(E) + int64_t(g) * (4 * BITS);
-  uint32_t o[4];
-  if constexpr (BITS == 4) {  // word c: elements 8c .. 8c+7, byte j = (elem 2j) << 4 | elem 2j+1
-    const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[c];
-    const uint32_t hi = (w >> 4) & 0x0F0F0F0Fu, lo = w & 0x0F0F0F0Fu;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = pair(code_plus_2p23(hi, j), code_plus_2p23(lo, j));
-  } else {  // bytes 2c, 2c+1 of the group: four codes each, the first in the top bits
-    const uint32_t w = reinterpret_cast<const uint16_t*>(codes)[c];
-    const uint32_t c0 = (w >> 6) & 0x0303u, c1 = (w >> 4) & 0x0303u, c2 = (w >> 2) & 0x0303u, c3 = w & 0x0303u;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      o[2 * j] = pair(code_plus_2p23(c0, j), code_plus_2p23(c1, j));
-      o[2 * j + 1] = pair(code_plus_2p23(c2, j), code_plus_2p23(c3, j));
-    }
-  }
-  return make_uint4(o[0], o[1], o[2], o[3]);
+  const uint16_t delta = reinterpret_cast<const uint16_t*>(raw + nbit_delta_off())[k >> 2];
+  const uint8_t* codes = raw + nbit_codes_off(E) + int64_t(k) * BITS;
+  const uint32_t w = BITS == 4 ? *reinterpret_cast<const uint32_t*>(codes) : *reinterpret_cast<const uint16_t*>(codes);
+  return nbit_dec8<BITS>(w, delta);
 }
 
 // first[g] = index of the first outlier entry whose element lies in group g or

@@ -558,6 +558,50 @@ ASHKV_API ashkv_status_t ashkv_decode_attention(
     int64_t mass_stride, float decay, void* d_out, float* d_lse, float* d_scratch, uint32_t* d_status, void* stream);
 
 /* ========================================================================
+ * The same with a sliding window: token t counts only if t >= d_lengths[b] -
+ * window or t < sinks (the first tokens stay visible); window is at least 1.
+ * Pages without such a token are neither looked up nor read; their page mass
+ * is only decayed.
+ * ======================================================================== */
+ASHKV_API ashkv_status_t ashkv_decode_attention_window(
+    const ashkv_paged_kv_t* kv, const void* d_q, int64_t q_seq_stride, int64_t q_head_stride, int32_t n_seqs,
+    int32_t heads_q, const int32_t* d_page_ids, int64_t page_ids_stride, int32_t max_pages, const int32_t* d_lengths,
+    int32_t window, int32_t sinks, float scale, float* d_page_mass, int64_t mass_stride, float decay, void* d_out,
+    float* d_lse, float* d_scratch, uint32_t* d_status, void* stream);
+
+/* ========================================================================
+ * New tokens into tiered pages, and tokens of tiered pages into dense rows.
+ * No counterpart in the reference, which encodes pages that are complete in
+ * the pool (ashkv/runtime/migrate.py:35-191).  d_starts [n_seqs + 1] ascends:
+ * rows d_starts[b] <= i < d_starts[b + 1] belong to sequence b, whose newest
+ * tokens they are: row i is token d_lengths[b] - (d_starts[b + 1] - i).  Rows
+ * of no sequence are left alone.
+ *
+ * ashkv_write_kv writes row i of d_k and d_v (bf16, element (i, head, c) at
+ * i * row_stride + head * head_stride + c) into the token's page in the
+ * format of the page's tier: bf16 pool rows, INT8 codes with the row's scale,
+ * FP8 codes, INT4 codes with their groups' scales -- the bytes that
+ * ashkv_migrate_pages writes for the same values.  A row of a page that does
+ * not exist or is dithered (that is coded as a whole) is left out and sets
+ * ASHKV_FLAG_INDEX_RANGE.  Two rows of a call must not be the same token.
+ * ashkv_read_kv writes the bf16 values that the token's page decodes to (as a
+ * promotion would) to row i of d_k and d_v [n_rows, heads_kv * head_dim],
+ * 16-byte aligned; zeros, and ASHKV_FLAG_INDEX_RANGE, where there is no page.
+ * head_dim may be any multiple of 8 in both; the pages have the other limits
+ * of ashkv_decode_attention, n_rows and n_seqs * max_pages at most 2^31 - 1 -
+ * 2^16.
+ * ======================================================================== */
+ASHKV_API ashkv_status_t ashkv_write_kv(const ashkv_paged_kv_t* kv, const void* d_k, int64_t k_row_stride,
+                                        int64_t k_head_stride, const void* d_v, int64_t v_row_stride,
+                                        int64_t v_head_stride, int64_t n_rows, const int32_t* d_page_ids,
+                                        int64_t page_ids_stride, int32_t max_pages, const int32_t* d_lengths,
+                                        const int32_t* d_starts, int32_t n_seqs, uint32_t* d_status, void* stream);
+ASHKV_API ashkv_status_t ashkv_read_kv(const ashkv_paged_kv_t* kv, const int32_t* d_page_ids, int64_t page_ids_stride,
+                                       int32_t max_pages, const int32_t* d_lengths, const int32_t* d_starts,
+                                       int32_t n_seqs, int64_t n_rows, void* d_k, void* d_v, uint32_t* d_status,
+                                       void* stream);
+
+/* ========================================================================
  * Page selection by key bounds.  No counterpart in the reference.
  * ashkv_page_bounds writes, for each entry i < (d_count ? min(*d_count,
  * max_entries) : max_entries) of d_list (page p in the BF16 tier, its first
