@@ -244,7 +244,7 @@ def test_read(cuda, tiers, heads, dim):
 def test_read_page_sizes(cuda, tiers, T):
     lengths, new = [1, T, T + 1, 3 * T - 1], [1, T, 1, 2 * T]
     kinds = FORMATS[tiers]
-    c = Cache(cuda, [kinds[i % len(kinds)] for i in range(12)], T, 4, 64, 7)
+    c = Cache(cuda, [kinds[i % len(kinds)] for i in range(12)], T, 8, 64, 7)
     ids = np.random.default_rng(7).permutation(12).astype(np.int32).reshape(4, 3)
     k, v = C.read_kv(c.table, c.kv, c.stores, i32(ids, cuda), i32(lengths, cuda), i32(starts_of(new), cuda), sum(new),
                      tokens_per_page=T)

@@ -87,7 +87,7 @@ def test_borders(cuda, tiers, window, sinks):
     run(cuda, FORMATS[tiers], 16, 4, 2, 128, [0, 1, 15, 16, 17, 31, 32, 33, 47, 48, 49, 64, 150], window, sinks, 2)
 
 
-@pytest.mark.parametrize("T,tiers", [(1, "bf16"), (5, "bf16"), (24, "bf16"), (1000, "bf16"), (8, "mixed"), (19, "int8"),
+@pytest.mark.parametrize("T,tiers", [(1, "bf16"), (5, "bf16"), (24, "bf16"), (1000, "bf16"), (8, "mixed"), (18, "int8"),
                                      (20, "int4"), (40, "mixed8"), (64, "int8"), (64, "nbit4")])
 @pytest.mark.parametrize("window,sinks", [(3, 0), (33, 2), (70, 50)])
 def test_page_sizes(cuda, T, tiers, window, sinks):
