@@ -83,6 +83,9 @@ SIGNATURES: dict[str, tuple] = {
                                              _I64, _F32, _P, _P, _P, _P, _P]),
     "ashkv_write_kv": (_I32, [_P, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I32, _P, _P, _I32, _P, _P]),
     "ashkv_read_kv": (_I32, [_P, _P, _I64, _I32, _P, _P, _I32, _I64, _P, _P, _P, _P]),
+    "ashkv_prompt_scratch_floats": (_I64, [_I64, _I32, _I32, _I32, _I32]),
+    "ashkv_prompt_attention": (_I32, [_P, _P, _I64, _I64, _I64, _I32, _P, _I64, _I32, _P, _P, _I32, _I32, _I32, _F32, _P,
+                                      _P, _P, _P, _P]),
     "ashkv_page_bounds": (_I32, [_P, _P, _P, _I32, _P, _P, _P, _P, _P]),
     "ashkv_select_scratch_floats": (_I64, [_I32, _I32, _I32]),
     "ashkv_select_pages": (_I32, [_P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _I64, _P, _I64, _I32, _P, _I32,
@@ -616,6 +619,20 @@ def read_kv(desc: PagedKVDesc, page_ids: torch.Tensor, lengths: torch.Tensor, st
         ctypes.addressof(desc), page_ids.data_ptr(), page_ids.stride(0), page_ids.shape[1], lengths.data_ptr(),
         starts.data_ptr(), lengths.shape[0], k.shape[0], k.data_ptr(), v.data_ptr(), _ptr(status), raw_stream(k)),
         "read_kv")
+
+
+def prompt_scratch_floats(n_rows: int, n_seqs: int, heads_q: int, heads_kv: int, head_dim: int) -> int:
+    return int(lib().ashkv_prompt_scratch_floats(n_rows, n_seqs, heads_q, heads_kv, head_dim))
+
+
+def prompt_attention(desc: PagedKVDesc, q: torch.Tensor, page_ids: torch.Tensor, lengths: torch.Tensor,
+                     starts: torch.Tensor, window: int, sinks: int, scale: float, out: torch.Tensor,
+                     lse: Optional[torch.Tensor], scratch: torch.Tensor, status: Optional[torch.Tensor]) -> None:
+    """q [n_rows, heads_q, head_dim] bf16 (unit inner stride) over the pages of ``desc`` -> out, lse; window 0: none."""
+    _check_text(lib().ashkv_prompt_attention(
+        ctypes.addressof(desc), q.data_ptr(), q.stride(0), q.stride(1), q.shape[0], q.shape[1], page_ids.data_ptr(),
+        page_ids.stride(0), page_ids.shape[1], lengths.data_ptr(), starts.data_ptr(), lengths.shape[0], window, sinks,
+        scale, out.data_ptr(), _ptr(lse), scratch.data_ptr(), _ptr(status), raw_stream(q)), "prompt_attention")
 
 
 def page_bounds(desc: PagedKVDesc, pages: torch.Tensor, count: Optional[torch.Tensor], valid: Optional[torch.Tensor],

@@ -118,6 +118,10 @@ def _require_lists(page_ids: torch.Tensor, lengths: torch.Tensor, n_seqs: int, d
     return _require_rows(page_ids, "page_ids", torch.int32, (n_seqs, page_ids.shape[1]), device)
 
 
+def _require_starts(starts: torch.Tensor, n_seqs: int, device: torch.device) -> None:
+    _require_dense(starts, "starts", torch.int32, (n_seqs + 1,), device)
+
+
 _StoreDescs = _native.TierStoreDesc * NUM_TIERS
 _NO_STORES = bytes(_StoreDescs(*(_native.TierStoreDesc(
     None, 0, 0, _native.PAGE_NONE if t else _native.PAGE_BF16, None, None) for t in range(NUM_TIERS))))
@@ -239,6 +243,53 @@ def decode_attention(q: torch.Tensor, table: DevicePageTable, kv: KVLayers,
     return (out, lse) if return_lse else out
 
 
+def prompt_attention(q: torch.Tensor, table: DevicePageTable, kv: KVLayers,
+                     stores: Optional[Mapping[int, TierStore]], page_ids: torch.Tensor, lengths: torch.Tensor,
+                     starts: torch.Tensor, *, tokens_per_page: int = 16, scale: Optional[float] = None,
+                     window: Optional[int] = None, sinks: int = 0, out: Optional[torch.Tensor] = None,
+                     return_lse: bool = False, status: Optional[torch.Tensor] = None):
+    """Causal attention of the new tokens of each sequence (a prompt, a chunk of one, drafted tokens).
+
+    ``q`` is bf16 [n_rows, heads_q, head_dim] (any strides with a dense last dimension); rows
+    ``starts[b] .. starts[b + 1] - 1`` (int32 [n_seqs + 1], ascending) are the newest tokens of sequence
+    b, whose ``lengths`` count them and whose pages hold their keys and values already (see
+    :func:`~ashkv.runtime.cache.write_kv`).  The query at position p attends the tokens up to p; with
+    ``window`` only the newest ``window`` of them and the first ``sinks``, and pages that no query of a
+    sequence sees are not looked up.  Pages of any tier are read where they lie; compressed ones count
+    as the bf16 values that they decode to (what :func:`~ashkv.runtime.cache.read_kv` gives).  Returns
+    the bf16 result [n_rows, heads_q, head_dim] (``out``, if given: contiguous, 16-byte aligned, not
+    ``q``), with ``return_lse`` also the fp32 log of the sum of exponentials [n_rows, heads_q].  A query
+    without tokens gives zeros and -inf.  Rows of no sequence are left as they were."""
+    _require_query(q)
+    _require_window(window, sinks)
+    n_rows, heads_q, d = q.shape
+    dev = q.device
+    n_seqs = lengths.numel()
+    page_ids = _require_lists(page_ids, lengths, n_seqs, dev)
+    _require_starts(starts, n_seqs, dev)
+    desc, keep = _pages_desc(table, kv, stores, d, tokens_per_page, dev)
+    if heads_q % desc.heads_kv:
+        raise ValueError(f"{heads_q} query heads are no multiple of {desc.heads_kv} key heads")
+    if status is not None:
+        _require_dense(status, "status", torch.int32, (1,), dev)
+    if out is None:
+        out = q.new_empty(n_rows, heads_q, d)
+    else:
+        _require_dense(out, "out", torch.bfloat16, (n_rows, heads_q, d), dev)
+        if out.data_ptr() % 16:
+            raise ValueError("out must be 16-byte aligned")
+        if out.data_ptr() == q.data_ptr() and n_rows:
+            raise ValueError("out must not be q")
+    lse = torch.empty(n_rows, heads_q, dtype=torch.float32, device=dev) if return_lse else None
+    if n_seqs and n_rows:
+        with _on(dev):
+            scratch = torch.empty(_native.prompt_scratch_floats(n_rows, n_seqs, heads_q, desc.heads_kv, d),
+                                  dtype=torch.float32, device=dev)
+            _native.prompt_attention(desc, q, page_ids, lengths, starts, window or 0, sinks,
+                                     1.0 / math.sqrt(d) if scale is None else float(scale), out, lse, scratch, status)
+    return (out, lse) if return_lse else out
+
+
 class PageBounds:
     """Int8 bounds of the keys of each page of a table, per key head.
 
@@ -353,4 +404,4 @@ def evict_pages(page_mass: torch.Tensor, page_ids: torch.Tensor, lengths: torch.
     return got
 
 
-__all__ = ["decode_attention", "PageBounds", "select_pages", "Eviction", "evict_pages"]
+__all__ = ["decode_attention", "prompt_attention", "PageBounds", "select_pages", "Eviction", "evict_pages"]

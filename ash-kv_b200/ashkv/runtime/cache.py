@@ -22,7 +22,7 @@ from typing import Mapping, Optional
 import torch
 
 from .. import _native
-from .attention import _on, _pages_desc, _refuse, _require_dense, _require_lists
+from .attention import _on, _pages_desc, _refuse, _require_dense, _require_lists, _require_starts
 from .batch import DevicePageTable, KVLayers, TierStore
 
 
@@ -31,10 +31,6 @@ def _row_shape(kv: KVLayers) -> tuple[int, int]:
     pool = kv.k[0].shape
     dim = pool[-1] if len(pool) > 2 else kv.row_len
     return kv.row_len // max(dim, 1), dim
-
-
-def _require_starts(starts: torch.Tensor, n_seqs: int, device: torch.device) -> None:
-    _require_dense(starts, "starts", torch.int32, (n_seqs + 1,), device)
 
 
 def _new_rows(x: torch.Tensor, name: str, heads: int, dim: int) -> torch.Tensor:

@@ -30,6 +30,7 @@
 #include <cudaTypedefs.h>
 
 #include "common.cuh"
+#include "tensor_core.cuh"
 
 namespace ashkv {
 namespace {
@@ -44,53 +45,6 @@ constexpr int kSB = 4;                       // B tile stages
 constexpr int kAcc = 4;                      // 128-column fp32 accumulators
 constexpr uint32_t kAccCols = 128 * kAcc;    // the whole TMEM of the SM: one CTA per SM
 
-// ---------------------------------------------------------------- tcgen05 / TMA wrappers
-__device__ __forceinline__ void tmem_alloc(uint32_t* smem_dst, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-               :: "r"(smem_u32(smem_dst)), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(taddr), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// D[tmem] (+)= A * B^T, A: M x K and B: N x K, both K-major bf16 in shared memory.
-__device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                          uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-               :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate),
-                  "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
-}
-// Arrive on `bar` once every MMA this thread issued so far has completed.
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-               :: "r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-               : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// Shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row atoms of
-// 128 bytes stacked every 1024 bytes (stride byte offset), sm_100 version 1.
-__device__ __forceinline__ uint64_t sw128_kmajor_desc(uint32_t smem_addr) {
-  uint64_t d = uint64_t((smem_addr >> 4) & 0x3FFFu);  // start address (16-byte units)
-  d |= uint64_t(1) << 16;                              // leading byte offset: unused for swizzled K-major
-  d |= uint64_t(1024 >> 4) << 32;                      // stride byte offset
-  d |= uint64_t(1) << 46;                              // descriptor version
-  d |= uint64_t(2) << 61;                              // SWIZZLE_128B
-  return d;
-}
 // Instruction descriptor: kind::f16, A = B = bf16, D = f32, both K-major, M = N = 128.
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t(kTile) >> 3) << 17) |
                             ((uint32_t(kTile) >> 4) << 24);
@@ -102,17 +56,6 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, ui
       :: "r"(smem_u32(smem_dst)), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 // Two 2^x on an fp32 pair.
 __device__ __forceinline__ f2 ex2_2(f2 x) {
   float a, b;
@@ -169,10 +112,6 @@ __device__ __forceinline__ void init_bars(PassBars& br) {
 #pragma unroll
   for (int i = 0; i < kAcc; ++i) { mbar_init(&br.full[i], 1); mbar_init(&br.empty[i], kEpiWarps); }
   mbar_init_fence();
-}
-
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(smem_u32(bar)) : "memory");
 }
 
 // The pipelined loop shared by both passes.  A (the CTA's fixed tile) is

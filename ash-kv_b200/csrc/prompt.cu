@@ -1,0 +1,1103 @@
+// Attention of the new tokens of each sequence (prompts, chunks of them, drafted tokens) over paged KV whose
+// pages may be in any tier (ashkv_prompt_attention).
+//
+// With p the position of a query and t <= p, and with a window t > p - window or t < sinks,
+//   s[t] = scale * q . K[t],  out = sum_t 2^(s2[t] - M) V[t] / sum_t 2^(s2[t] - M),  s2 = s * log2(e),
+// for any M: one pass over the keys keeps a running M and the two sums.  Compressed pages count as
+// the bf16 values that they decode to, so both products run on tcgen05 with bf16 operands and fp32 sums
+// in TMEM; a weight is rounded to bf16 once (by 2^-8 of it at most, as the result is), the sum of the weights
+// takes them unrounded.
+//
+// Rows: the (token, query head) pairs of a key head, token by token; an item is 256 of them, two
+// tiles of 128 that share the key tiles of 128 tokens.  A plan kernel lists the items, cuts those of
+// more key tiles than a CTA's share into pieces, and sorts them by length; the CTAs of the main
+// kernel, one to an SM, take them in turn; a join kernel weighs the partial results of cut items.
+//
+// A CTA: two softmax warpgroups, a tile each, a thread to a row (its 128 scores come from TMEM as
+// registers and go back as bf16 weights over the scores' columns); four warps that bring K and V tiles
+// into shared memory, decoding them where a page is compressed; three warps that look the pages
+// up; one that issues the products.  While one tile's scores become weights the tensor cores work
+// on the other's.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "common.cuh"
+#include "page_codec.cuh"
+#include "paged_kv.cuh"
+#include "tensor_core.cuh"
+
+namespace ashkv {
+namespace {
+
+constexpr float kLog2eP = 1.4426950408889634f;
+constexpr float kLn2P = 0.6931471805599453f;
+constexpr int kTileRows = 128, kItemRows = 256, kTileKeys = 128;
+constexpr int kThreadsP = 512, kPlanThreads = 1024, kJoinThreadsP = 256;
+constexpr int kLoaders = 128, kLookWarps = 3, kLook = 6;  // threads that load, warps that look up, tiles looked up ahead
+constexpr uint32_t kPollsP = 1u << 24;                    // bounded waits
+constexpr int kBins = 64;
+constexpr uint32_t kNoPage = 0xFFu;
+
+// A run of an item's key tiles [begin, end): tile index i stands for tile i of the sequence below ts, else i - ts + tw.
+struct __align__(16) Piece {
+  int32_t seq, row0, rows, first;  // rows row0 .. of the sequence's, whose first token is row `first` of q
+  int32_t pos0, begin, end, part;  // position of that token; part: its partial result, or -1
+  int32_t ts, tw, lo, kmax;        // tokens that some row sees: below sinks, or lo .., up to kmax
+};
+struct __align__(16) Split {  // an item cut into pieces
+  int32_t row0, rows, first, part, parts, pad[3];
+};
+
+struct PromptParams {
+  PagedKV kv;
+  PageLists lists;
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  int32_t n_rows, heads_q, group;
+  bool q_wide;
+  float scale2;      // |scale| * log2(e)
+  uint32_t negate;   // of the instruction descriptor, for a negative scale
+  int32_t window, sinks;  // window 0: none
+  uint16_t* out;
+  float* lse;
+  // scratch
+  int32_t* counts;  // pieces, splits
+  int32_t* prefix;  // [n_seqs + 1] items before a sequence
+  Piece* pieces;
+  Split* splits;
+  int32_t max_pieces, max_parts;  // (per key head)
+  int32_t share;                  // pieces to aim for over all key heads
+  float* part_o;     // [max_parts * heads_kv][part_rows][D], each divided by its sum
+  float* part_lse2;  // [max_parts * heads_kv][part_rows]
+  int32_t part_rows;
+};
+
+// ---------------------------------------------------------------- plan
+struct Item {
+  int first, row0, rows, pos0, n, ts, tw, lo, kmax;
+};
+__device__ __forceinline__ int seq_rows(const PromptParams& p, int b, int& first) {
+  const int s0 = max(0, min(p.lists.starts[b], p.n_rows)), s1 = max(s0, min(p.lists.starts[b + 1], p.n_rows));
+  first = s0;
+  return (s1 - s0) * p.group;
+}
+__device__ Item item_of(const PromptParams& p, int b, int m) {
+  Item it;
+  const int rows = seq_rows(p, b, it.first);
+  it.row0 = m * kItemRows;
+  it.rows = min(kItemRows, rows - it.row0);
+  const int64_t cap = int64_t(p.lists.max_pages) * p.kv.T;
+  const int64_t pos0 = max(int64_t(-(1 << 30)), int64_t(p.lists.lengths[b]) - (int64_t(p.lists.starts[b + 1]) - it.first));
+  const int64_t pa = pos0 + it.row0 / p.group, pb = pos0 + (it.row0 + it.rows - 1) / p.group;
+  const int64_t kmax = min(pb, cap - 1), lo = p.window ? max(int64_t(0), pa - p.window + 1) : 0;
+  it.pos0 = int(pos0);
+  it.kmax = int(max(kmax, int64_t(-1)));
+  it.lo = int(min(lo, int64_t(0x7FFFFFFF)));
+  it.ts = it.tw = it.n = 0;
+  if (kmax >= 0) {
+    const int te = int(kmax / kTileKeys) + 1;
+    it.ts = p.window ? int((min(int64_t(p.sinks), kmax + 1) + kTileKeys - 1) / kTileKeys) : 0;
+    it.tw = max(it.lo / kTileKeys, it.ts);
+    it.n = it.ts + max(0, te - it.tw);
+  }
+  return it;
+}
+__device__ __forceinline__ int seq_of_item(const int32_t* prefix, int n_seqs, int idx) {
+  int lo = 0, hi = n_seqs;  // the last b with prefix[b] <= idx
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (prefix[mid] <= idx) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// One CTA.  Counts the items of each sequence, then their key tiles; cuts what is longer than a CTA's share;
+// writes the pieces, the longest first (64 bins of lengths).
+__global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_constant__ PromptParams p, int least) {
+  __shared__ int s_warp[32], s_base, s_longest, s_parts, s_splits;
+  __shared__ unsigned long long s_tiles;
+  __shared__ int s_bin[kBins];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) { s_base = 0; s_longest = 1; s_parts = 0; s_splits = 0; s_tiles = 0; }
+  if (tid < kBins) s_bin[tid] = 0;
+  wait_for_previous();
+  allow_next();
+  __syncthreads();
+  const int n_seqs = p.lists.n_seqs;
+  bool bad = false;
+  for (int b0 = 0; b0 < n_seqs; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int first = 0, n = 0;
+    if (b < n_seqs) {
+      n = (seq_rows(p, b, first) + kItemRows - 1) / kItemRows;
+      const int64_t len = p.lists.lengths[b];
+      const int s0 = p.lists.starts[b], s1 = p.lists.starts[b + 1];
+      bad |= s0 < 0 || s1 < s0 || s1 > p.n_rows;
+      if (len < 0 || len > int64_t(p.lists.max_pages) * p.kv.T || int64_t(s1) - s0 > len) flag(p.lists.status, ASHKV_FLAG_INDEX_RANGE);
+    }
+    int upto = n;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int x = __shfl_up_sync(0xFFFFFFFFu, upto, off);
+      if (lane >= off) upto += x;
+    }
+    if (lane == 31) s_warp[warp] = upto;
+    __syncthreads();
+    if (warp == 0) {
+      int w = s_warp[lane];
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int x = __shfl_up_sync(0xFFFFFFFFu, w, off);
+        if (lane >= off) w += x;
+      }
+      s_warp[lane] = w;
+    }
+    __syncthreads();
+    const int before = s_base + (warp ? s_warp[warp - 1] : 0) + upto - n;
+    if (b < n_seqs) p.prefix[b] = before;
+    __syncthreads();
+    if (tid == 0) s_base += s_warp[31];
+    __syncthreads();
+  }
+  const int items = s_base;
+  if (tid == 0) p.prefix[n_seqs] = items;
+  if (__syncthreads_or(bad)) {  // rows that two sequences claim: nothing is computed
+    if (tid == 0) {
+      p.counts[0] = p.counts[1] = 0;
+      flag(p.lists.status, ASHKV_FLAG_INDEX_RANGE);
+    }
+    return;
+  }
+  const auto item = [&](int i, int& b) {
+    b = seq_of_item(p.prefix, n_seqs, i);
+    return item_of(p, b, i - p.prefix[b]);
+  };
+  unsigned long long tiles = 0;
+  int longest = 1, b;
+  for (int i = tid; i < items; i += kPlanThreads) {
+    const Item it = item(i, b);
+    tiles += it.n;
+    longest = max(longest, it.n);
+  }
+  atomicAdd(&s_tiles, tiles);
+  atomicMax(&s_longest, longest);
+  __syncthreads();
+  const unsigned long long all = s_tiles * p.kv.heads_kv;
+  const int share = int(min((unsigned long long)0x40000000, max((unsigned long long)least, (all + p.share - 1) / p.share)));
+  const int top = min(share, s_longest);
+  const auto parts_of = [&](int n) { return n > share ? (n + share - 1) / share : 1; };
+  const auto bin_of = [&](int len) { return int(int64_t(top - len) * kBins / (top + 1)); };
+  for (int i = tid; i < items; i += kPlanThreads) {
+    const Item it = item(i, b);
+    const int parts = parts_of(it.n);
+    for (int k = 0; k < parts; ++k)
+      atomicAdd(&s_bin[bin_of(int(int64_t(it.n) * (k + 1) / parts - int64_t(it.n) * k / parts))], 1);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int sum = 0;
+    for (int k = 0; k < kBins; ++k) {
+      const int n = s_bin[k];
+      s_bin[k] = sum;
+      sum += n;
+    }
+    p.counts[0] = min(sum, p.max_pieces);
+  }
+  __syncthreads();
+  for (int i = tid; i < items; i += kPlanThreads) {
+    const Item it = item(i, b);
+    int parts = parts_of(it.n), part = -1;
+    if (parts > 1) {
+      part = atomicAdd(&s_parts, parts);
+      const int at = atomicAdd(&s_splits, 1);
+      if (at < p.max_parts) p.splits[at] = Split{it.row0, it.rows, it.first, part, parts, {0, 0, 0}};
+    }
+    for (int k = 0; k < parts; ++k) {
+      const int begin = int(int64_t(it.n) * k / parts), end = int(int64_t(it.n) * (k + 1) / parts);
+      const int at = atomicAdd(&s_bin[bin_of(end - begin)], 1);
+      if (at < p.max_pieces)
+        p.pieces[at] = Piece{b, it.row0, it.rows, it.first, it.pos0, begin, end, parts > 1 ? part + k : -1, it.ts, it.tw, it.lo, it.kmax};
+    }
+  }
+  __syncthreads();
+  if (tid == 0) p.counts[1] = s_splits;
+}
+
+// ---------------------------------------------------------------- main
+// Shared memory: the queries (two tiles), kStages key or value tiles (K, V, K, V ..), and where pages may be
+// compressed kRaw half tiles' codes on their way, with a word of scales for each 16 of them.  A tile is
+// 128 rows of D bf16 in runs of 64 (128 bytes, swizzled).  kAhead half tiles are under way while one is finished.
+template <int D, bool RAW>
+struct Shape {
+  static constexpr int kUnitsRow = D / 16, kRowsPass = kLoaders / kUnitsRow, kPasses = kTileKeys / kRowsPass;  // (with RAW)
+  static constexpr uint32_t kHalf = kTileRows * 128, kTile = kHalf * (D / 64);
+  static constexpr int kStages = RAW ? (D == 64 ? 6 : 3) : (D == 64 ? 8 : 4);
+  static constexpr int kAhead = kStages - 2;
+  static constexpr int kRaw = RAW ? kAhead + 1 : 0;
+  static constexpr uint32_t kUnits = kTileKeys * D / 16;  // 16 codes each
+  static constexpr uint32_t kBytes = 2 * kTile + kStages * kTile + kRaw * kUnits * 20 + 1024;
+};
+
+struct __align__(16) TileInfo {
+  uint64_t k[kTileKeys], v[kTileKeys];  // BF16 rows: of the head's first channel; else the slot
+  uint32_t meta[kTileKeys];             // format | token in its page << 8
+  uint32_t seen[4];                     // a bit for each token that exists
+  int32_t first;                        // position of the tile's first token
+  int32_t edge;                         // some row does not see some token of the tile
+  int32_t odd;                          // and one of its values is not finite
+  int32_t pad;
+};
+struct PromptBars {
+  uint64_t q_full, q_empty, full[8], empty[8], info_full[kLook], info_empty[kLook], s_full[2], p_ready[2], drained;
+};
+
+struct Shared {
+  PromptBars bars;
+  TileInfo info[kLook];
+  uint32_t tmem;
+  volatile int failed;
+};
+
+__device__ __forceinline__ bool wait_p(Shared& sm, uint64_t* bar, uint32_t parity) {
+  for (uint32_t n = 0; n < kPollsP; ++n) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((n & 255u) == 255u && sm.failed) return false;
+  }
+  sm.failed = 1;
+  return false;
+}
+
+__device__ __forceinline__ bool wait_warp(Shared& sm, uint64_t* bar, uint32_t parity) {  // all lanes, with one answer
+  return __all_sync(0xFFFFFFFFu, wait_p(sm, bar, parity));
+}
+
+// The works of a CTA: piece w / heads_kv for key head w % heads_kv; neighbours in turn, there and back, so that
+// CTA sums of the sorted lengths come out alike.
+__device__ __forceinline__ int64_t work_of(int k) {
+  return int64_t(k) * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+__device__ __forceinline__ Piece load_piece(const PromptParams& p, int64_t w, int& head) {
+  const int64_t i = w / p.kv.heads_kv;
+  head = int(w - i * p.kv.heads_kv);
+  const uint4* at = reinterpret_cast<const uint4*>(p.pieces + i);
+  const uint4 a = ld_v4(at), b = ld_v4(at + 1), c = ld_v4(at + 2);
+  return Piece{int(a.x), int(a.y), int(a.z), int(a.w), int(b.x), int(b.y), int(b.z), int(b.w), int(c.x), int(c.y), int(c.z), int(c.w)};
+}
+__device__ __forceinline__ int tile_of(const Piece& pc, int i) { return i < pc.ts ? i : i - pc.ts + pc.tw; }
+
+// ---- pages: three warps, a tile in turn each
+template <int D>
+__device__ void look_up(const PromptParams& p, Shared& sm, int64_t works, int which) {
+  const int lane = threadIdx.x & 31;
+  int n = 0;  // tiles of the CTA so far
+  for (int k = 0; work_of(k) < works; ++k) {
+    int head;
+    const Piece pc = load_piece(p, work_of(k), head);
+    const int64_t pa = int64_t(pc.pos0) + pc.row0 / p.group, pb = int64_t(pc.pos0) + (pc.row0 + pc.rows - 1) / p.group;
+    const int32_t* ids = p.lists.page_ids + int64_t(pc.seq) * p.lists.page_ids_stride;
+    for (int i = pc.begin; i < pc.end; ++i, ++n) {
+      if (n % kLookWarps != which) continue;
+      const int first = tile_of(pc, i) * kTileKeys;
+      TileInfo& t = sm.info[n % kLook];
+      // four neighbouring tokens a lane; one look-up where they share a page
+      Place at[4];
+      int tok[4];
+      bool need[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t pos = int64_t(first) + 4 * lane + u;
+        need[u] = pos <= pc.kmax && (pos < p.sinks || pos >= pc.lo || !p.window);
+      }
+      const bool shared_page = p.kv.T % 4 == 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t pos = int64_t(first) + 4 * lane + u;
+        if (u > 0 && shared_page) {
+          at[u] = at[0];
+          tok[u] = tok[0] + u;
+          continue;
+        }
+        const bool any = shared_page ? need[0] || need[1] || need[2] || need[3] : need[u];
+        const int64_t j = pos / p.kv.T;
+        tok[u] = int(pos - j * p.kv.T);
+        at[u] = Place{-1, nullptr, nullptr};
+        if (any) at[u] = place_of(p.kv, ids[j]);
+        if (any && at[u].format < 0) flag(p.lists.status, ASHKV_FLAG_INDEX_RANGE);
+      }
+      if (n >= kLook && !wait_warp(sm, &sm.bars.info_empty[n % kLook], (n / kLook - 1) & 1)) return;
+      uint32_t bits = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int e = 4 * lane + u;
+        const bool ok = need[u] && at[u].format >= 0;
+        if (ok) bits |= 1u << u;
+        const int64_t off = ok && at[u].format == ASHKV_PAGE_BF16 ? (tok[u] * p.kv.row_stride + head * D) * 2 : 0;
+        const uint64_t none = reinterpret_cast<uint64_t>(p.pieces);  // (an aligned address; nothing is read there)
+        t.k[e] = ok ? reinterpret_cast<uint64_t>(at[u].k) + off : none;
+        t.v[e] = ok ? reinterpret_cast<uint64_t>(at[u].v) + off : none;
+        t.meta[e] = (ok ? uint32_t(at[u].format) : kNoPage) | uint32_t(tok[u]) << 8;
+      }
+      bits <<= 4 * (lane & 7);  // eight lanes make a word
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) bits |= __shfl_xor_sync(0xFFFFFFFFu, bits, off);
+      if ((lane & 7) == 0) t.seen[lane >> 3] = bits;
+      if (lane == 0) {
+        t.first = first;
+        const int64_t last = int64_t(first) + kTileKeys - 1;
+        t.edge = !(last <= pa && (!p.window || first > pb - p.window || last < p.sinks));
+        t.odd = 0;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.bars.info_full[n % kLook]);
+    }
+  }
+}
+
+// ---- loads: four warps
+// A row of a half tile, `unit`: 16 of its channels.  Where their two chunks of 16 bytes go.
+__device__ __forceinline__ uint32_t chunk_at(uint32_t row, uint32_t chunk) {
+  return (chunk >> 3) * (kTileRows * 128) + row * 128 + (((chunk & 7u) ^ (row & 7u)) << 4);
+}
+__device__ __forceinline__ void sts128p(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, uint64_t src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, int bytes) {
+  if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" :: "r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ bool not_finite(uint4 x) {
+  const uint32_t m = max_u16x2(max_u16x2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu), max_u16x2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
+  return (m & 0xFFFFu) >= 0x7F80u || (m >> 16) >= 0x7F80u;
+}
+
+// The outliers of row pr of a dithered page over its decoded values (row r of a half tile), by the lanes that wrote those.
+template <int D, int BITS>
+__device__ __noinline__ void overlay(const uint8_t* slot, uint32_t T, uint32_t row, uint32_t cap, uint32_t pr, uint32_t r,
+                                     uint32_t u, uint32_t to, uint32_t head) {
+  const uint32_t n = min(*reinterpret_cast<const uint32_t*>(slot), cap);
+  const uint32_t* entries = reinterpret_cast<const uint32_t*>(slot + nbit_entries_off(2 * int64_t(T) * row, BITS));
+  const uint32_t e0 = pr * row + head * D;
+  for (uint32_t j = u; j < n; j += D / 16) {
+    const uint32_t x = entries[j], c = (x >> 16) - e0;
+    if (c < uint32_t(D))
+      asm volatile("st.shared.u16 [%0], %1;" :: "r"(to + chunk_at(r, c >> 3) + (c & 7u) * 2u), "h"(uint16_t(x)) : "memory");
+  }
+}
+
+template <int D, bool RAW>
+struct Loader {
+  using S = Shape<D, RAW>;
+  const PromptParams& p;
+  Shared& sm;
+  const int tid;
+  const uint32_t q_at, stages, raw, words;
+  const int64_t works;
+  // the half tile to issue next: of work ik, tile ii; in: tiles issued before
+  int ik = 0, ii = 0, iend = 0, ihead = 0, in = 0, ih = 0;
+  bool iv = false, more = true;
+
+  __device__ __forceinline__ Loader(const PromptParams& p_, Shared& sm_, uint32_t base, int64_t works_)
+      : p(p_), sm(sm_), tid(threadIdx.x & (kLoaders - 1)), q_at(base), stages(base + 2 * S::kTile),
+        raw(stages + S::kStages * S::kTile), words(raw + S::kRaw * S::kUnits * 16), works(works_) {
+    open(0);
+  }
+  __device__ __forceinline__ void open(int k) {  // the first work from k on that has tiles
+    for (ik = k;; ++ik) {
+      more = work_of(ik) < works;
+      if (!more) return;
+      const Piece pc = load_piece(p, work_of(ik), ihead);
+      ii = pc.begin;
+      iend = pc.end;
+      if (ii < iend) return;
+    }
+  }
+
+  __device__ __forceinline__ bool issue() {
+    if (more) {
+      TileInfo& t = sm.info[in % kLook];
+      if (!iv && !wait_warp(sm, &sm.bars.info_full[in % kLook], (in / kLook) & 1)) return false;
+      const int st = ih % S::kStages;
+      if (ih >= S::kStages && !wait_warp(sm, &sm.bars.empty[st], (ih / S::kStages - 1) & 1)) return false;
+      const uint32_t to = stages + uint32_t(st) * S::kTile;
+      const uint64_t* rows = iv ? t.v : t.k;
+      if constexpr (!RAW) {
+        constexpr int CPR = D / 8, RPP = kLoaders / CPR;
+        const uint32_t c = uint32_t(tid) % CPR, r0 = uint32_t(tid) / CPR;
+#pragma unroll 8
+        for (uint32_t k = 0; k < kTileKeys / RPP; ++k) {
+          const uint32_t r = r0 + RPP * k;
+          cp_async16_zfill(to + chunk_at(r, c), rows[r] + c * 16, (t.meta[r] & 0xFFu) != kNoPage);
+        }
+      } else {
+        const uint32_t u = uint32_t(tid) % S::kUnitsRow, r0 = uint32_t(tid) / S::kUnitsRow;
+        const uint32_t slot = uint32_t(ih) % S::kRaw * S::kUnits;
+#pragma unroll 2
+        for (uint32_t k = 0; k < S::kPasses; ++k) {
+          const uint32_t r = r0 + S::kRowsPass * k, meta = t.meta[r], fmt = meta & 0xFFu;
+          const uint64_t base = rows[r];
+          if (fmt == ASHKV_PAGE_BF16) {  // (chunks u and u + D / 16: neighbouring lanes, neighbouring chunks)
+            cp_async16_zfill(to + chunk_at(r, u), base + u * 16, true);
+            cp_async16_zfill(to + chunk_at(r, u + D / 16), base + (u + D / 16) * 16, true);
+          } else if (fmt != kNoPage) {
+            const uint8_t* s = reinterpret_cast<const uint8_t*>(base);
+            const uint32_t T = uint32_t(p.kv.T), row = uint32_t(p.kv.row_len), E = 2 * T * row;
+            const uint32_t pr = (meta >> 8) + (iv ? T : 0), e = pr * row + uint32_t(ihead) * D + 16 * u;
+            const uint32_t d = raw + (slot + r * S::kUnitsRow + u) * 16, w = words + (slot + r * S::kUnitsRow + u) * 4;
+            if (fmt == ASHKV_PAGE_INT8) {
+              cp_async16(d, s + uint32_t(int8_codes_offset(T)) + e);
+              cp_async_small(w, s + (2 * pr & ~3u), 4);
+            } else if (fmt == ASHKV_PAGE_FP8) {
+              cp_async16(d, s + e);
+            } else if (fmt == ASHKV_PAGE_INT4) {
+              cp_async_small(d, s + E / 32 + e / 2, 8);
+              cp_async_small(w, s + (e / 64 * 2 & ~3u), 4);
+            } else if (fmt == ASHKV_PAGE_NBIT4) {
+              cp_async_small(d, s + nbit_codes_off(E) + e / 2, 8);
+              cp_async_small(w, s + nbit_delta_off() + (e / 32 * 2 & ~3u), 4);
+            } else {
+              cp_async_small(d, s + nbit_codes_off(E) + e / 4, 4);
+              cp_async_small(w, s + nbit_delta_off() + (e / 32 * 2 & ~3u), 4);
+            }
+          }
+        }
+      }
+      ++ih;
+      iv = !iv;
+      if (!iv) {
+        ++in;
+        if (++ii == iend) open(ik + 1);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    return true;
+  }
+
+  // The bf16 values of a unit of a compressed page.
+  __device__ __forceinline__ void decode(uint32_t fmt, uint32_t d, uint32_t word, uint32_t pr, uint32_t e, uint4& x, uint4& y) const {
+    if (fmt == ASHKV_PAGE_INT8) {
+      const uint4 c = lds128(d);
+      const float s = f16_to_f32(uint16_t(pr & 1u ? word >> 16 : word));
+      x = int8_dec8(make_uint2(c.x, c.y), s);
+      y = int8_dec8(make_uint2(c.z, c.w), s);
+    } else if (fmt == ASHKV_PAGE_FP8) {
+      const uint4 c = lds128(d);
+      x = fp8_dec8(make_uint2(c.x, c.y));
+      y = fp8_dec8(make_uint2(c.z, c.w));
+    } else {
+      uint2 c;
+      asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(c.x), "=r"(c.y) : "r"(d));
+      if (fmt == ASHKV_PAGE_INT4) {
+        const uint16_t s = uint16_t(e / 64 & 1u ? word >> 16 : word);
+        x = int4_dec8(c.x, s);
+        y = int4_dec8(c.y, s);
+        return;
+      }
+      const uint16_t s = uint16_t(e / 32 & 1u ? word >> 16 : word);
+      if (fmt == ASHKV_PAGE_NBIT4) {
+        x = nbit_dec8<4>(c.x, s);
+        y = nbit_dec8<4>(c.y, s);
+      } else {
+        x = nbit_dec8<2>(c.x & 0xFFFFu, s);
+        y = nbit_dec8<2>(c.x >> 16, s);
+      }
+    }
+  }
+
+  // Half tile h (of tile n, key head `head`) has arrived: decodes what is compressed, and hands it over.
+  __device__ __forceinline__ void finish(int h, int n, int head, bool v) {
+    const uint32_t st = uint32_t(h) % S::kStages, to = stages + st * S::kTile;
+    TileInfo& t = sm.info[n % kLook];
+    const bool look = v && t.edge;
+    bool odd = false;
+    if constexpr (RAW) {
+      const uint32_t u = uint32_t(tid) % S::kUnitsRow, r0 = uint32_t(tid) / S::kUnitsRow;
+      const uint32_t slot = uint32_t(h) % S::kRaw * S::kUnits;
+      bool dithered = false;
+#pragma unroll 2
+      for (uint32_t k = 0; k < S::kPasses; ++k) {
+        const uint32_t r = r0 + S::kRowsPass * k, meta = t.meta[r], fmt = meta & 0xFFu;
+        uint4 x = make_uint4(0, 0, 0, 0), y = x;
+        if (fmt == ASHKV_PAGE_BF16) {
+          if (look) odd |= not_finite(lds128(to + chunk_at(r, u))) || not_finite(lds128(to + chunk_at(r, u + D / 16)));
+          continue;
+        }
+        if (fmt != kNoPage) {
+          const uint32_t pr = (meta >> 8) + (v ? uint32_t(p.kv.T) : 0), e = pr * uint32_t(p.kv.row_len) + uint32_t(head) * D + 16 * u;
+          uint32_t word;
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(word) : "r"(words + (slot + r * S::kUnitsRow + u) * 4));
+          decode(fmt, raw + (slot + r * S::kUnitsRow + u) * 16, word, pr, e, x, y);
+          dithered |= fmt >= ASHKV_PAGE_NBIT4;
+          if (look) odd |= not_finite(x) || not_finite(y);
+        }
+        // lanes of the upper half of a row store their odd chunk first: eight lanes, eight banks of 16 bytes
+        const bool swap = u >= 4;
+        sts128p(to + chunk_at(r, 2 * u + swap), swap ? y : x);
+        sts128p(to + chunk_at(r, 2 * u + !swap), swap ? x : y);
+      }
+      if (__any_sync(0xFFFFFFFFu, dithered)) {
+        __syncwarp();
+        for (uint32_t k = 0; k < S::kPasses; ++k) {
+          const uint32_t r = r0 + S::kRowsPass * k, meta = t.meta[r], fmt = meta & 0xFFu;
+          const uint8_t* s = reinterpret_cast<const uint8_t*>(v ? t.v[r] : t.k[r]);
+          const uint32_t pr = (meta >> 8) + (v ? uint32_t(p.kv.T) : 0);
+          const uint32_t T = uint32_t(p.kv.T), row = uint32_t(p.kv.row_len), cap = uint32_t(p.kv.outlier_cap);
+          if (fmt == ASHKV_PAGE_NBIT4) overlay<D, 4>(s, T, row, cap, pr, r, u, to, uint32_t(head));
+          else if (fmt == ASHKV_PAGE_NBIT2) overlay<D, 2>(s, T, row, cap, pr, r, u, to, uint32_t(head));
+        }
+        __syncwarp();
+        if (look)  // (outliers may be infinite too)
+          for (uint32_t k = 0; k < S::kPasses; ++k) {
+            const uint32_t r = r0 + S::kRowsPass * k;
+            odd |= not_finite(lds128(to + chunk_at(r, 2 * u))) || not_finite(lds128(to + chunk_at(r, 2 * u + 1)));
+          }
+      }
+    } else if (look) {
+      constexpr int CPR = D / 8, RPP = kLoaders / CPR;
+      const uint32_t c = uint32_t(tid) % CPR, r0 = uint32_t(tid) / CPR;
+      for (uint32_t k = 0; k < kTileKeys / RPP; ++k) odd |= not_finite(lds128(to + chunk_at(r0 + RPP * k, c)));
+    }
+    if (odd) *const_cast<volatile int32_t*>(&t.odd) = 1;
+    fence_proxy_async_smem();
+    mbar_arrive(&sm.bars.full[st]);
+  }
+
+  __device__ __forceinline__ void load_queries(const Piece& pc, int head) {
+    constexpr int CPR = D / 8, RPP = kLoaders / CPR;
+    const uint32_t c = uint32_t(tid) % CPR, r0 = uint32_t(tid) / CPR;
+    const int rows = pc.rows > kTileRows ? kItemRows : kTileRows;
+    for (int r = int(r0); r < rows; r += RPP) {
+      const int pair = pc.row0 + r, token = pair / p.group;
+      const uint16_t* src = p.q + (int64_t(pc.first) + token) * p.q_row + int64_t(head * p.group + pair - token * p.group) * p.q_head + c * 8;
+      const uint32_t to = q_at + uint32_t(r / kTileRows) * S::kTile + chunk_at(uint32_t(r % kTileRows), c);
+      const bool real = r < pc.rows;
+      if (p.q_wide) {
+        cp_async16_zfill(to, real ? reinterpret_cast<uint64_t>(src) : reinterpret_cast<uint64_t>(p.pieces), real);
+      } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (real)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = src[2 * j] | uint32_t(src[2 * j + 1]) << 16;
+        sts128p(to, make_uint4(w[0], w[1], w[2], w[3]));
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  __device__ void run() {
+    int h = 0, n = 0, q_loads = 0;
+    bool ok = true;
+    for (int k = 0; k < S::kAhead && ok; ++k) ok = issue();
+    for (int k = 0; ok && work_of(k) < works; ++k) {
+      int head;
+      const Piece pc = load_piece(p, work_of(k), head);
+      if (pc.begin >= pc.end) continue;
+      if (q_loads > 0 && !(ok = wait_warp(sm, &sm.bars.q_empty, (q_loads - 1) & 1))) break;
+      ++q_loads;
+      load_queries(pc, head);
+      cp_async_wait_all();
+      fence_proxy_async_smem();
+      mbar_arrive(&sm.bars.q_full);
+      for (int i = pc.begin; ok && i < pc.end; ++i, ++n)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          if (!(ok = issue())) break;
+          asm volatile("cp.async.wait_group %0;" :: "n"(S::kAhead) : "memory");
+          finish(h++, n, head, v != 0);
+        }
+    }
+    cp_async_wait_all();
+  }
+};
+
+// ---- products: one thread
+template <int D, bool RAW>
+__device__ void issue_products(const PromptParams& p, Shared& sm, uint32_t base, int64_t works) {
+  using S = Shape<D, RAW>;
+  const uint32_t q_at = base, stages = base + 2 * S::kTile, tmem = sm.tmem;
+  constexpr uint32_t kScores = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kTileKeys >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
+  constexpr uint32_t kValues = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
+  const uint32_t scores_desc = kScores | p.negate;
+  int n = 0, items = 0, ready[2] = {0, 0};
+  bool ok = true;
+  for (int k = 0; ok && work_of(k) < works; ++k) {
+    int head;
+    const Piece pc = load_piece(p, work_of(k), head);
+    const int tiles = pc.end - pc.begin, two = pc.rows > kTileRows ? 2 : 1;
+    if (tiles <= 0) continue;
+    if (!(ok = wait_p(sm, &sm.bars.q_full, items++ & 1))) break;
+    bool odd = false;
+    for (int i = 0; ok && i <= tiles; ++i) {
+      const int hk = 2 * (n + i), hv = hk - 1;  // K of tile i, V of the one before
+      for (int g = 0; g < two; ++g) {
+        const uint32_t s = tmem + uint32_t(g) * 128, o = tmem + 256 + uint32_t(g) * 128;
+        if (i > 0) {
+          if (g == 0) {
+            if (!(ok = wait_p(sm, &sm.bars.full[hv % S::kStages], (hv / S::kStages) & 1))) break;
+            odd = *const_cast<volatile int32_t*>(&sm.info[(n + i - 1) % kLook].odd);
+          }
+          if (!(ok = wait_p(sm, &sm.bars.p_ready[g], ready[g]++ & 1))) break;
+          tc_fence_after();
+          if (!odd) {
+            const uint32_t v = stages + uint32_t(hv % S::kStages) * S::kTile;
+#pragma unroll
+            for (int j = 0; j < kTileKeys / 16; ++j)
+              umma_bf16_ts(o, s + j * 8, sw128_mnmajor_desc(v + j * 2048, S::kHalf), kValues, i > 1 || j > 0);
+          }
+          if (i == tiles) umma_commit(&sm.bars.s_full[g]);
+        }
+        if (i < tiles) {
+          if (g == 0 && !(ok = wait_p(sm, &sm.bars.full[hk % S::kStages], (hk / S::kStages) & 1))) break;
+          tc_fence_after();
+          const uint32_t q = q_at + uint32_t(g) * S::kTile, kt = stages + uint32_t(hk % S::kStages) * S::kTile;
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              umma_bf16(s, sw128_kmajor_desc(q + c * S::kHalf + j * 32), sw128_kmajor_desc(kt + c * S::kHalf + j * 32),
+                        scores_desc, (c | j) != 0);
+          umma_commit(&sm.bars.s_full[g]);
+        }
+      }
+      if (!ok) break;
+      if (i > 0) {
+        umma_commit(&sm.bars.empty[hv % S::kStages]);
+        umma_commit(&sm.bars.info_empty[(n + i - 1) % kLook]);
+      }
+      if (i < tiles) umma_commit(&sm.bars.empty[hk % S::kStages]);
+      if (i == tiles - 1) umma_commit(&sm.bars.q_empty);
+    }
+    n += tiles;
+  }
+  umma_commit(&sm.bars.drained);  // every product is done before TMEM and shared memory are given up
+  for (uint32_t t = 0; t < kPollsP && !mbar_try_wait(&sm.bars.drained, 0); ++t) {}
+}
+
+// ---- softmax: a warpgroup to a tile, a thread to a row
+// O (+)= P V for a tile whose V has values that are not finite, for rows that may not see them: weights of 0 take nothing.
+// The weights are in the scores' columns as fp32.
+template <int D>
+__device__ __noinline__ void add_values_by_row(uint32_t s, uint32_t o, uint32_t v, bool first) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < D; c0 += 32) {
+    float acc[32];
+    if (first) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) acc[c] = 0.0f;
+    } else {
+      tmem_ld32(o + c0, acc);
+      tmem_ld_wait();
+      tmem_ld_done(acc);
+    }
+#pragma unroll 1
+    for (int j0 = 0; j0 < kTileKeys; j0 += 32) {
+      float w[32];
+      tmem_ld32(s + j0, w);
+      tmem_ld_wait();
+      tmem_ld_done(w);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        if (w[j] == 0.0f) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint4 x = lds128(v + chunk_at(uint32_t(j0 + j), uint32_t(c0 / 8 + k)));
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            acc[8 * k + 2 * y] = fmaf(w[j], bf16lo(xs[y]), acc[8 * k + 2 * y]);
+            acc[8 * k + 2 * y + 1] = fmaf(w[j], bf16hi(xs[y]), acc[8 * k + 2 * y + 1]);
+          }
+        }
+      }
+      __syncwarp();
+    }
+    uint32_t r[32];
+#pragma unroll
+    for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(acc[c]);
+    tmem_st32(o + c0, r);
+  }
+  tmem_st_wait();
+}
+
+// The tokens of 32 from `first` on that a query at pos sees.
+__device__ __forceinline__ uint32_t low_bits(int64_t n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t seen_by(const PromptParams& p, int64_t first, int64_t pos) {
+  uint32_t m = low_bits(pos + 1 - first);
+  if (p.window) m &= ~low_bits(pos - p.window + 1 - first) | low_bits(p.sinks - first);
+  return m;
+}
+
+template <int D, bool RAW>
+__device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, int64_t works, int g) {
+  using S = Shape<D, RAW>;
+  const int lane = threadIdx.x & 31, r = int(threadIdx.x & 127);
+  const uint32_t lanes = uint32_t(r & 96) << 16;
+  const uint32_t s = sm.tmem + uint32_t(g) * 128 + lanes, o = sm.tmem + 256 + uint32_t(g) * 128 + lanes;
+  const float scale2 = p.scale2;
+  int n = 0, seen_scores = 0;
+  for (int k = 0; work_of(k) < works; ++k) {
+    int head;
+    const Piece pc = load_piece(p, work_of(k), head);
+    const int tiles = pc.end - pc.begin;
+    if (g == 1 && pc.rows <= kTileRows) {
+      n += tiles;
+      continue;
+    }
+    const int at = g * kTileRows + r;
+    const bool mine = at < pc.rows;
+    const int pair = pc.row0 + min(at, pc.rows - 1), token = pair / p.group, hq = head * p.group + pair - token * p.group;
+    const int64_t pos = int64_t(pc.pos0) + token;
+    float m = -INFINITY, l = 0.0f;
+    for (int i = 0; i < tiles; ++i, ++n) {
+      if (!wait_warp(sm, &sm.bars.s_full[g], seen_scores++ & 1)) return;
+      tc_fence_after();
+      const TileInfo& t = sm.info[n % kLook];
+      const int64_t first = t.first;
+      float v[4][32];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) tmem_ld32(s + q * 32, v[q]);
+      const uint4 real = *reinterpret_cast<const uint4*>(t.seen);
+      const bool all = first + kTileKeys - 1 <= pos && (real.x & real.y & real.z & real.w) == 0xFFFFFFFFu &&
+                       (!p.window || first > pos - p.window || first + kTileKeys - 1 < p.sinks);
+      tmem_ld_wait();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) tmem_ld_done(v[q]);
+      const bool plain = __all_sync(0xFFFFFFFFu, all);
+      float top;
+      if (plain) {
+        float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            m0 = max3f(m0, v[q][j], v[q][j + 1]);
+            m1 = max3f(m1, v[q][j + 2], v[q][j + 3]);
+          }
+        top = fmaxf(m0, m1) * scale2;
+      } else {
+        const uint32_t bits[4] = {real.x & seen_by(p, first, pos), real.y & seen_by(p, first + 32, pos),
+                                  real.z & seen_by(p, first + 64, pos), real.w & seen_by(p, first + 96, pos)};
+        top = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            v[q][j] = (bits[q] >> j) & 1u ? v[q][j] * scale2 : -INFINITY;
+            top = fmaxf(top, v[q][j]);
+          }
+      }
+      // the reference follows the running maximum only when that lies more than 2^8 above it
+      const bool over = top > m + 8.0f || (m == -INFINITY && top > m);
+      const float f = over ? ex2(m - top) : 1.0f;  // (0 at first)
+      if (over) {
+        m = top;
+        l *= f;
+      }
+      if (i > 0 && __any_sync(0xFFFFFFFFu, over)) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float x[32];
+          tmem_ld32(o + c, x);
+          tmem_ld_wait();
+          tmem_ld_done(x);
+          uint32_t y[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(x[j] * f);
+          tmem_st32(o + c, y);
+        }
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+      const f2 SC = plain ? pk2(scale2, scale2) : pk2(1.0f, 1.0f), NM = pk2(-ref, -ref);
+      f2 sum0 = pk2(0.0f, 0.0f), sum1 = sum0;
+      bool odd = false;
+      if (t.edge) {  // does V hold values that some rows must not see?
+        const int hv = 2 * n + 1;
+        if (!wait_warp(sm, &sm.bars.full[hv % S::kStages], (hv / S::kStages) & 1)) return;
+        odd = *const_cast<const volatile int32_t*>(&t.odd);
+      }
+      if (odd) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t w[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float x = ex2(plain ? fmaf(v[q][j], scale2, -ref) : v[q][j] - ref);
+            l += x;
+            w[j] = __float_as_uint(x);
+          }
+          tmem_st32(s + q * 32, w);
+        }
+        tmem_st_wait();
+        add_values_by_row<D>(s, o, base + 2 * S::kTile + uint32_t((2 * n + 1) % S::kStages) * S::kTile, i == 0);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          uint32_t w[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float a = v[q + (j >> 4)][2 * (j & 15)], b = v[q + (j >> 4)][2 * (j & 15) + 1];
+            float x, y;
+            upk2(fma2(pk2(a, b), SC, NM), x, y);
+            x = ex2(x);
+            y = ex2(y);
+            if (j & 1) sum1 = add2(sum1, pk2(x, y));
+            else sum0 = add2(sum0, pk2(x, y));
+            w[j] = f32x2_to_bf16x2(x, y);
+          }
+          tmem_st32(s + (q >> 1) * 32, w);
+        }
+        tmem_st_wait();
+      }
+      float a, b;
+      upk2(add2(sum0, sum1), a, b);
+      l += a + b;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.bars.p_ready[g]);
+    }
+    if (tiles > 0) {
+      if (!wait_warp(sm, &sm.bars.s_full[g], seen_scores++ & 1)) return;
+      tc_fence_after();
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
+    const int64_t row = (int64_t(pc.first) + token) * p.heads_q + hq;
+    const int64_t part = (int64_t(pc.part) * p.kv.heads_kv + head) * p.part_rows + at;
+    if (mine) {
+      if (pc.part >= 0) p.part_lse2[part] = lse2;
+      else if (p.lse) p.lse[row] = lse2 * kLn2P;
+    }
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+      float x[32];
+      if (tiles > 0) {
+        tmem_ld32(o + c, x);
+        tmem_ld_wait();
+        tmem_ld_done(x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) x[j] = inv == 0.0f ? 0.0f : x[j] * inv;
+      if (!mine) {
+      } else if (pc.part >= 0) {
+        float4* to = reinterpret_cast<float4*>(p.part_o + part * D + c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) to[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+      } else {
+        uint4* to = reinterpret_cast<uint4*>(p.out + row * D + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          to[j] = make_uint4(f32x2_to_bf16x2(x[8 * j], x[8 * j + 1]), f32x2_to_bf16x2(x[8 * j + 2], x[8 * j + 3]),
+                             f32x2_to_bf16x2(x[8 * j + 4], x[8 * j + 5]), f32x2_to_bf16x2(x[8 * j + 6], x[8 * j + 7]));
+      }
+      __syncwarp();
+    }
+    tc_fence_before();  // (O is free for the next item once its first weights are ready)
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
+
+// 512 threads of 128 registers at launch; 176 for the softmax warpgroups, 80 for the others (together as many).
+template <int D, bool RAW>
+__global__ void __launch_bounds__(kThreadsP, 1) prompt_kernel(const __grid_constant__ PromptParams p) {
+  extern __shared__ uint8_t smem[];
+  __shared__ Shared sm;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
+  if (threadIdx.x == 0) {
+    PromptBars& b = sm.bars;
+    mbar_init(&b.q_full, kLoaders);
+    mbar_init(&b.q_empty, 1);
+    for (int i = 0; i < 8; ++i) { mbar_init(&b.full[i], kLoaders); mbar_init(&b.empty[i], 1); }
+    for (int i = 0; i < kLook; ++i) { mbar_init(&b.info_full[i], 1); mbar_init(&b.info_empty[i], 1); }
+    for (int g = 0; g < 2; ++g) { mbar_init(&b.s_full[g], 1); mbar_init(&b.p_ready[g], 4); }
+    mbar_init(&b.drained, 1);
+    mbar_init_fence();
+    sm.failed = 0;
+  }
+  if (warp == 12) tmem_alloc(&sm.tmem, 512);
+  tc_fence_before();
+  wait_for_previous();
+  __syncthreads();
+  tc_fence_after();
+  allow_next();
+  const int64_t works = int64_t(*const_cast<const volatile int32_t*>(p.counts)) * p.kv.heads_kv;
+  if (warp < 8) {
+    more_registers<176>();
+    softmax_rows<D, RAW>(p, sm, base, works, warp >> 2);
+  } else {
+    fewer_registers<80>();
+    if (warp < 12) Loader<D, RAW>(p, sm, base, works).run();
+    else if (warp > 12) look_up<D>(p, sm, works, warp - 13);
+    else if (lane == 0) issue_products<D, RAW>(p, sm, base, works);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x == 0 && sm.failed) flag(p.lists.status, ASHKV_FLAG_TIMEOUT);
+  if (warp == 12) {
+    tmem_dealloc(sm.tmem, 512);
+    tmem_relinquish();
+  }
+}
+
+// ---------------------------------------------------------------- join
+// A warp to a row of a cut item: its partial results weighed by 2^(their log2-sum - the total), in their order.
+template <int D>
+__global__ void __launch_bounds__(kJoinThreadsP) prompt_join_kernel(const __grid_constant__ PromptParams p) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x & 31;
+  wait_for_previous();
+  allow_next();
+  const int64_t rows = int64_t(p.counts[1]) * p.kv.heads_kv * p.part_rows;
+  for (int64_t w = int64_t(blockIdx.x) * (kJoinThreadsP / 32) + (threadIdx.x >> 5); w < rows;
+       w += int64_t(gridDim.x) * (kJoinThreadsP / 32)) {
+    const int at = int(w % p.part_rows), head = int(w / p.part_rows % p.kv.heads_kv);
+    const Split sp = p.splits[w / p.part_rows / p.kv.heads_kv];
+    if (at >= sp.rows) continue;
+    const int64_t step = int64_t(p.kv.heads_kv) * p.part_rows, first = (int64_t(sp.part) * p.kv.heads_kv + head) * p.part_rows + at;
+    float top = -INFINITY;
+    bool bad = false;
+    for (int k = lane; k < sp.parts; k += 32) {
+      const float x = p.part_lse2[first + k * step];
+      bad |= x != x;
+      top = fmaxf(top, x);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+    bad = __any_sync(0xFFFFFFFFu, bad);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, acc[N] = {};
+#pragma unroll 4
+    for (int k = 0; k < sp.parts; ++k) {
+      const float x = p.part_lse2[first + k * step];
+      const float* o = p.part_o + (first + k * step) * D + lane * N;
+      float v[N];
+      if constexpr (N == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(o);
+        v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(o);
+        v[0] = y.x; v[1] = y.y;
+      }
+      if (x == -INFINITY) continue;
+      const float f = ex2(x - ref);
+      sum += f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] = fmaf(f, v[j], acc[j]);
+    }
+    const float inv = sum == 0.0f && !bad ? 0.0f : 1.0f / sum;
+    const int pair = sp.row0 + at, token = pair / p.group;
+    const int64_t row = (int64_t(sp.first) + token) * p.heads_q + head * p.group + pair - token * p.group;
+    uint32_t* out = reinterpret_cast<uint32_t*>(p.out + row * D + lane * N);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) out[j / 2] = f32x2_to_bf16x2(acc[j] * inv, acc[j + 1] * inv);
+    if (lane == 0 && p.lse) p.lse[row] = sum == 0.0f && !bad ? -INFINITY : (ref + log2f(sum)) * kLn2P;
+  }
+}
+
+// ---------------------------------------------------------------- host
+// Key tiles of a piece at least, and pieces to aim for.
+constexpr int kLeastTiles = 4;
+struct Sizes {
+  int64_t items, pieces, parts, part_rows, prefix;
+  int share;
+  int64_t ints() const { return 8 + (prefix + 3) / 4 * 4 + pieces * int64_t(sizeof(Piece) / 4) + parts * int64_t(sizeof(Split) / 4); }
+  int64_t floats(int heads_kv, int D) const { return (ints() + 31) / 32 * 32 + parts * heads_kv * part_rows * (int64_t(D) + 1) + 32; }
+};
+Sizes sizes_of(int64_t n_rows, int64_t n_seqs, int heads_q, int heads_kv) {
+  Sizes s;
+  const int sms = sm_count() > 0 ? sm_count() : 148, group = heads_q / heads_kv;
+  s.items = n_rows * group / kItemRows + n_seqs;
+  s.part_rows = std::min<int64_t>(kItemRows, std::max<int64_t>(1, n_rows * group));
+  s.share = sms;
+  // an item of n tiles is cut where n exceeds a share: into at most 2 n / share pieces, share >= all tiles / s.share
+  s.parts = std::min<int64_t>(2 * int64_t(s.share) / heads_kv + 2, 2 * int64_t(s.share) + 2);
+  s.pieces = s.items + s.parts;
+  s.prefix = n_seqs + 1;
+  return s;
+}
+
+template <int D, bool RAW>
+ashkv_status_t launch_prompt(const PromptParams& p, int sms, void* stream) {
+  constexpr const char* kName = "ashkv_prompt_attention";
+  // the attribute is the kernel's on a device and outlasts the call
+  static std::atomic<bool> allowed[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !allowed[dev].load(std::memory_order_acquire))) {
+    e = cudaFuncSetAttribute(prompt_kernel<D, RAW>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<D, RAW>::kBytes));
+    if (e == cudaSuccess && dev < 64) allowed[dev].store(true, std::memory_order_release);
+  }
+  if (e != cudaSuccess) {
+    set_error("ashkv_prompt_attention (shared memory attribute)", e);
+    return ASHKV_LAUNCH_ERROR;
+  }
+  launch_paged(prompt_plan_kernel, 1, kPlanThreads, 0, stream, p, kLeastTiles);
+  launch_paged(prompt_kernel<D, RAW>, sms, kThreadsP, Shape<D, RAW>::kBytes, stream, p);
+  const ashkv_status_t rc = check_launch(kName);
+  if (rc != ASHKV_OK) return rc;
+  launch_paged(prompt_join_kernel<D>, 4 * sms, kJoinThreadsP, 0, stream, p);
+  return check_launch(kName);
+}
+
+}  // namespace
+}  // namespace ashkv
+
+using namespace ashkv;
+
+extern "C" int64_t ashkv_prompt_scratch_floats(int64_t n_rows, int32_t n_seqs, int32_t heads_q, int32_t heads_kv,
+                                               int32_t head_dim) {
+  if (n_rows < 0 || n_seqs < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv || head_dim <= 0) return -1;
+  return sizes_of(n_rows, n_seqs, heads_q, heads_kv).floats(heads_kv, head_dim);
+}
+
+extern "C" ashkv_status_t ashkv_prompt_attention(
+    const ashkv_paged_kv_t* kv, const void* d_q, int64_t q_row_stride, int64_t q_head_stride, int64_t n_rows, int32_t heads_q,
+    const int32_t* d_page_ids, int64_t page_ids_stride, int32_t max_pages, const int32_t* d_lengths, const int32_t* d_starts,
+    int32_t n_seqs, int32_t window, int32_t sinks, float scale, void* d_out, float* d_lse, float* d_scratch,
+    uint32_t* d_status, void* stream) {
+  constexpr const char* kName = "ashkv_prompt_attention";
+  PromptParams p{};
+  if (const char* why = copy_pages(kv, p.kv)) return refuse(kName, why);
+  if (const char* why = copy_lists(d_page_ids, page_ids_stride, max_pages, d_lengths, d_starts, n_seqs, n_rows, d_status, p.lists))
+    return refuse(kName, why);
+  if (heads_q <= 0 || heads_q % p.kv.heads_kv || heads_q > 8192) return refuse(kName, "heads_q must be a multiple of heads_kv, at most 8192");
+  if (n_rows * heads_q > (int64_t(1) << 30)) return refuse(kName, "too many query rows");
+  if (window < 0 || sinks < 0 || (sinks && !window)) return refuse(kName, "window and sinks must not be negative, sinks need a window");
+  if (n_rows == 0 || n_seqs == 0) return ASHKV_OK;
+  if (!d_q || !d_out || !d_scratch || !aligned(d_q, 2) || !aligned(d_out, 16) || !aligned(d_scratch, 16))
+    return refuse(kName, "null or misaligned device pointer");
+  p.q = static_cast<const uint16_t*>(d_q);
+  p.q_row = q_row_stride; p.q_head = q_head_stride;
+  p.q_wide = aligned(d_q, 16) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0;
+  p.n_rows = int32_t(n_rows); p.heads_q = heads_q; p.group = heads_q / p.kv.heads_kv;
+  p.negate = scale < 0.0f ? 1u << 13 : 0u;
+  p.scale2 = (scale < 0.0f ? -scale : scale) * kLog2eP;
+  p.window = window; p.sinks = sinks;
+  p.out = static_cast<uint16_t*>(d_out); p.lse = d_lse;
+  const Sizes s = sizes_of(n_rows, n_seqs, heads_q, p.kv.heads_kv);
+  p.counts = reinterpret_cast<int32_t*>(d_scratch);
+  p.prefix = p.counts + 8;
+  p.pieces = reinterpret_cast<Piece*>(p.prefix + (s.prefix + 3) / 4 * 4);
+  p.splits = reinterpret_cast<Split*>(p.pieces + s.pieces);
+  p.max_pieces = int32_t(s.pieces); p.max_parts = int32_t(s.parts); p.share = s.share; p.part_rows = int32_t(s.part_rows);
+  p.part_o = d_scratch + (s.ints() + 31) / 32 * 32;
+  p.part_lse2 = p.part_o + s.parts * p.kv.heads_kv * s.part_rows * kv->head_dim;
+  bool stores = false;
+  for (int t = 1; t < kTiers; ++t) stores |= p.kv.store[t].format != ASHKV_PAGE_NONE;
+  const int sms = sm_count() > 0 ? sm_count() : 148;
+  if (kv->head_dim == 64) return stores ? launch_prompt<64, true>(p, sms, stream) : launch_prompt<64, false>(p, sms, stream);
+  return stores ? launch_prompt<128, true>(p, sms, stream) : launch_prompt<128, false>(p, sms, stream);
+}

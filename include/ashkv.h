@@ -602,6 +602,40 @@ ASHKV_API ashkv_status_t ashkv_read_kv(const ashkv_paged_kv_t* kv, const int32_t
                                        void* stream);
 
 /* ========================================================================
+ * Attention of the new tokens of each sequence (a prompt, a chunk of one,
+ * drafted tokens) over tiered, paged KV.  No counterpart in the reference.
+ * Rows and sequences are those of ashkv_write_kv, with n_rows rows of
+ * heads_q query heads; the pages hold the new tokens' K and V already.  For
+ * row i of sequence b, p = d_lengths[b] - (d_starts[b + 1] - i) and query
+ * head h (key head h / (heads_q / heads_kv)), over the tokens t <= p, with
+ * window > 0 only those with t > p - window or t < sinks:
+ *   s[t] = scale * q[i,h] . K[t],  out[i,h] = sum_t softmax(s)[t] V[t] (bf16),
+ *   lse[i,h] = log sum_t exp s[t].
+ * Compressed pages count as the bf16 values that they decode to (what
+ * ashkv_read_kv gives).  Sums and softmax statistics are fp32; a weight is
+ * rounded to bf16 once for the product with V, the sum of the weights takes
+ * them unrounded; weights reach 2^8, so values of up to 2^119 / n are summed
+ * without overflow.  What a row must not see does not change its result,
+ * whatever it holds.  A row without tokens gives 0 and -inf; rows of no
+ * sequence are left alone.  Tokens of pages that do not exist are left out
+ * and set ASHKV_FLAG_INDEX_RANGE in *d_status (if given), as do lengths that
+ * the lists cannot hold or that the new tokens exceed; starts that do not
+ * ascend within [0, n_rows] set it and nothing is computed.  d_q has unit
+ * element stride; d_out is contiguous bf16, 16-byte aligned, and must not
+ * overlap d_q; d_lse (may be NULL): fp32 [n_rows, heads_q].  n_rows * heads_q
+ * is at most 2^30; other limits are those of ashkv_decode_attention.
+ * d_scratch: ashkv_prompt_scratch_floats(...) floats, 16-byte aligned, used
+ * by this call alone until it has run.
+ * ======================================================================== */
+ASHKV_API int64_t ashkv_prompt_scratch_floats(int64_t n_rows, int32_t n_seqs, int32_t heads_q, int32_t heads_kv,
+                                              int32_t head_dim);
+ASHKV_API ashkv_status_t ashkv_prompt_attention(
+    const ashkv_paged_kv_t* kv, const void* d_q, int64_t q_row_stride, int64_t q_head_stride, int64_t n_rows,
+    int32_t heads_q, const int32_t* d_page_ids, int64_t page_ids_stride, int32_t max_pages, const int32_t* d_lengths,
+    const int32_t* d_starts, int32_t n_seqs, int32_t window, int32_t sinks, float scale, void* d_out, float* d_lse,
+    float* d_scratch, uint32_t* d_status, void* stream);
+
+/* ========================================================================
  * Page selection by key bounds.  No counterpart in the reference.
  * ashkv_page_bounds writes, for each entry i < (d_count ? min(*d_count,
  * max_entries) : max_entries) of d_list (page p in the BF16 tier, its first
