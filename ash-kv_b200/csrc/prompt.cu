@@ -614,84 +614,167 @@ struct Loader {
   }
 };
 
-// ---- products: one thread
+// ---- products: a warp, whose elected lane issues them
 template <int D, bool RAW>
 __device__ void issue_products(const PromptParams& p, Shared& sm, uint32_t base, int64_t works) {
   using S = Shape<D, RAW>;
-  const uint32_t q_at = base, stages = base + 2 * S::kTile, tmem = sm.tmem;
   constexpr uint32_t kScores = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kTileKeys >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
   constexpr uint32_t kValues = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
-  const uint32_t scores_desc = kScores | p.negate;
+  const uint32_t scores_desc = kScores | p.negate, tmem = sm.tmem;
+  // descriptors of the first query tile and of stage 0 as K and as V; an address further on is added in units of 16 bytes
+  const uint64_t q_desc = sw128_kmajor_desc(base), k_desc = sw128_kmajor_desc(base + 2 * S::kTile);
+  const uint64_t v_desc = sw128_mnmajor_desc(base + 2 * S::kTile, S::kHalf);
   int n = 0, items = 0, ready[2] = {0, 0};
   bool ok = true;
+  const auto scores = [&](int g, uint32_t stage) {
+    const uint64_t q = q_desc + (uint32_t(g) * S::kTile >> 4), k = k_desc + (stage * S::kTile >> 4);
+    if (elect_one()) {
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          umma_bf16(tmem + uint32_t(g) * 128, q + ((c * S::kHalf + j * 32) >> 4), k + ((c * S::kHalf + j * 32) >> 4), scores_desc, (c | j) != 0);
+      umma_commit(&sm.bars.s_full[g]);
+    }
+    __syncwarp();
+  };
+  const auto values = [&](int g, uint32_t stage, bool more) {
+    const uint64_t v = v_desc + (stage * S::kTile >> 4);
+    const uint32_t s = tmem + uint32_t(g) * 128, o = tmem + 256 + uint32_t(g) * 128;
+    if (elect_one()) {
+      umma_bf16_ts(o, s, v, kValues, more);
+#pragma unroll
+      for (int j = 1; j < kTileKeys / 16; ++j) umma_bf16_ts(o, s + j * 8, v + (j * 2048 >> 4), kValues, 1);
+    }
+    __syncwarp();
+  };
+  const auto commit = [&](uint64_t* bar) {
+    if (elect_one()) umma_commit(bar);
+    __syncwarp();
+  };
   for (int k = 0; ok && work_of(k) < works; ++k) {
     int head;
     const Piece pc = load_piece(p, work_of(k), head);
-    const int tiles = pc.end - pc.begin, two = pc.rows > kTileRows ? 2 : 1;
+    const int tiles = __shfl_sync(0xFFFFFFFFu, pc.end - pc.begin, 0);  // (uniform for the compiler too)
+    const int two = __shfl_sync(0xFFFFFFFFu, pc.rows > kTileRows ? 2 : 1, 0);
     if (tiles <= 0) continue;
-    if (!(ok = wait_p(sm, &sm.bars.q_full, items++ & 1))) break;
+    if (!(ok = wait_warp(sm, &sm.bars.q_full, items++ & 1))) break;
     bool odd = false;
     for (int i = 0; ok && i <= tiles; ++i) {
       const int hk = 2 * (n + i), hv = hk - 1;  // K of tile i, V of the one before
-      for (int g = 0; g < two; ++g) {
-        const uint32_t s = tmem + uint32_t(g) * 128, o = tmem + 256 + uint32_t(g) * 128;
+      const uint32_t sk = uint32_t(hk) % S::kStages, sv = uint32_t(hv) % S::kStages;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (g == two) break;
         if (i > 0) {
           if (g == 0) {
-            if (!(ok = wait_p(sm, &sm.bars.full[hv % S::kStages], (hv / S::kStages) & 1))) break;
-            odd = *const_cast<volatile int32_t*>(&sm.info[(n + i - 1) % kLook].odd);
+            if (!(ok = wait_warp(sm, &sm.bars.full[sv], (hv / S::kStages) & 1))) break;
+            odd = __any_sync(0xFFFFFFFFu, *const_cast<volatile int32_t*>(&sm.info[(n + i - 1) % kLook].odd));
           }
-          if (!(ok = wait_p(sm, &sm.bars.p_ready[g], ready[g]++ & 1))) break;
+          if (!(ok = wait_warp(sm, &sm.bars.p_ready[g], ready[g]++ & 1))) break;
           tc_fence_after();
-          if (!odd) {
-            const uint32_t v = stages + uint32_t(hv % S::kStages) * S::kTile;
-#pragma unroll
-            for (int j = 0; j < kTileKeys / 16; ++j)
-              umma_bf16_ts(o, s + j * 8, sw128_mnmajor_desc(v + j * 2048, S::kHalf), kValues, i > 1 || j > 0);
-          }
-          if (i == tiles) umma_commit(&sm.bars.s_full[g]);
+          if (!odd) values(g, sv, i > 1);
+          if (i == tiles) commit(&sm.bars.s_full[g]);
         }
         if (i < tiles) {
-          if (g == 0 && !(ok = wait_p(sm, &sm.bars.full[hk % S::kStages], (hk / S::kStages) & 1))) break;
+          if (g == 0 && !(ok = wait_warp(sm, &sm.bars.full[sk], (hk / S::kStages) & 1))) break;
           tc_fence_after();
-          const uint32_t q = q_at + uint32_t(g) * S::kTile, kt = stages + uint32_t(hk % S::kStages) * S::kTile;
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              umma_bf16(s, sw128_kmajor_desc(q + c * S::kHalf + j * 32), sw128_kmajor_desc(kt + c * S::kHalf + j * 32),
-                        scores_desc, (c | j) != 0);
-          umma_commit(&sm.bars.s_full[g]);
+          scores(g, sk);
         }
       }
       if (!ok) break;
       if (i > 0) {
-        umma_commit(&sm.bars.empty[hv % S::kStages]);
-        umma_commit(&sm.bars.info_empty[(n + i - 1) % kLook]);
+        commit(&sm.bars.empty[sv]);
+        commit(&sm.bars.info_empty[(n + i - 1) % kLook]);
       }
-      if (i < tiles) umma_commit(&sm.bars.empty[hk % S::kStages]);
-      if (i == tiles - 1) umma_commit(&sm.bars.q_empty);
+      if (i < tiles) commit(&sm.bars.empty[sk]);
+      if (i == tiles - 1) commit(&sm.bars.q_empty);
     }
     n += tiles;
   }
-  umma_commit(&sm.bars.drained);  // every product is done before TMEM and shared memory are given up
-  for (uint32_t t = 0; t < kPollsP && !mbar_try_wait(&sm.bars.drained, 0); ++t) {}
+  commit(&sm.bars.drained);  // every product is done before TMEM and shared memory are given up
+  for (uint32_t t = 0; t < kPollsP && !__all_sync(0xFFFFFFFFu, mbar_try_wait(&sm.bars.drained, 0)); ++t) {}
 }
 
 // ---- softmax: a warpgroup to a tile, a thread to a row
-// O (+)= P V for a tile whose V has values that are not finite, for rows that may not see them: weights of 0 take nothing.
-// The weights are in the scores' columns as fp32.
+// The tokens of 32 from first on that a query at first + ahead sees.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t seen_by(const PromptParams& p, int first, int ahead) {
+  uint32_t m = low_bits(ahead + 1);
+  if (p.window) m &= ~low_bits(ahead + 1 - p.window) | low_bits(p.sinks - first);
+  return m;
+}
+// The reference of the weights follows the running maximum only when that lies more than 2^8 above it: what the sums so far
+// are to be multiplied by.
+__device__ __forceinline__ float follow(float top, float& m, float& l) {
+  if (!(top > m + 8.0f) && !(m == -INFINITY && top > m)) return 1.0f;
+  const float f = ex2(m - top);  // (0 at first)
+  m = top;
+  l *= f;
+  return f;
+}
 template <int D>
-__device__ __noinline__ void add_values_by_row(uint32_t s, uint32_t o, uint32_t v, bool first) {
+__device__ __forceinline__ void scale_sums(uint32_t o, float f) {
+#pragma unroll 1
+  for (int c = 0; c < D; c += 32) {
+    float x[32];
+    tmem_ld32(o + c, x);
+    tmem_ld_wait();
+    tmem_ld_done(x);
+    uint32_t y[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(x[j] * f);
+    tmem_st32(o + c, y);
+  }
+}
+
+// A tile whose V has values that are not finite, for rows that may not see them: O (+)= P V row by row, where
+// weights of 0 take nothing.  Scores, then weights, stay in their columns as fp32.
+template <int D>
+__device__ __noinline__ void tile_by_row(uint32_t s, uint32_t o, uint32_t v, uint4 bits, float scale2, bool started, float& m, float& l) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t seen = q == 0 ? bits.x : q == 1 ? bits.y : q == 2 ? bits.z : bits.w;
+    float x[32];
+    tmem_ld32(s + q * 32, x);
+    tmem_ld_wait();
+    tmem_ld_done(x);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) top = fmaxf(top, seen >> j & 1u ? x[j] * scale2 : -INFINITY);
+  }
+  const float f = follow(top, m, l), ref = m == -INFINITY ? 0.0f : m;
+  if (started && __any_sync(0xFFFFFFFFu, f != 1.0f)) {
+    scale_sums<D>(o, f);
+    tmem_st_wait();
+  }
+#pragma unroll 1
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t seen = q == 0 ? bits.x : q == 1 ? bits.y : q == 2 ? bits.z : bits.w;
+    float x[32];
+    tmem_ld32(s + q * 32, x);
+    tmem_ld_wait();
+    tmem_ld_done(x);
+    uint32_t w[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const float y = seen >> j & 1u ? ex2(fmaf(x[j], scale2, -ref)) : 0.0f;
+      l += y;
+      w[j] = __float_as_uint(y);
+    }
+    tmem_st32(s + q * 32, w);
+  }
+  tmem_st_wait();
 #pragma unroll 1
   for (int c0 = 0; c0 < D; c0 += 32) {
     float acc[32];
-    if (first) {
-#pragma unroll
-      for (int c = 0; c < 32; ++c) acc[c] = 0.0f;
-    } else {
+    if (started) {
       tmem_ld32(o + c0, acc);
       tmem_ld_wait();
       tmem_ld_done(acc);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) acc[c] = 0.0f;
     }
 #pragma unroll 1
     for (int j0 = 0; j0 < kTileKeys; j0 += 32) {
@@ -720,128 +803,79 @@ __device__ __noinline__ void add_values_by_row(uint32_t s, uint32_t o, uint32_t 
     for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(acc[c]);
     tmem_st32(o + c0, r);
   }
-  tmem_st_wait();
-}
-
-// The tokens of 32 from `first` on that a query at pos sees.
-__device__ __forceinline__ uint32_t low_bits(int64_t n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
-__device__ __forceinline__ uint32_t seen_by(const PromptParams& p, int64_t first, int64_t pos) {
-  uint32_t m = low_bits(pos + 1 - first);
-  if (p.window) m &= ~low_bits(pos - p.window + 1 - first) | low_bits(p.sinks - first);
-  return m;
 }
 
 template <int D, bool RAW>
 __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, int64_t works, int g) {
   using S = Shape<D, RAW>;
-  const int lane = threadIdx.x & 31, r = int(threadIdx.x & 127);
-  const uint32_t lanes = uint32_t(r & 96) << 16;
+  const int lane = threadIdx.x & 31, at = int(threadIdx.x & 255);  // the row of the item
+  const uint32_t lanes = uint32_t(at & 96) << 16;
   const uint32_t s = sm.tmem + uint32_t(g) * 128 + lanes, o = sm.tmem + 256 + uint32_t(g) * 128 + lanes;
   const float scale2 = p.scale2;
-  int n = 0, seen_scores = 0;
+  int n = 0, phase = 0;  // tiles of the CTA and scores of this tile so far
   for (int k = 0; work_of(k) < works; ++k) {
-    int head;
-    const Piece pc = load_piece(p, work_of(k), head);
-    const int tiles = pc.end - pc.begin;
-    if (g == 1 && pc.rows <= kTileRows) {
-      n += tiles;
-      continue;
+    int tiles, pos;
+    {
+      int head;
+      const Piece pc = load_piece(p, work_of(k), head);
+      tiles = pc.end - pc.begin;
+      if (g == 1 && pc.rows <= kTileRows) {
+        n += tiles;
+        continue;
+      }
+      pos = pc.pos0 + (pc.row0 + min(at, pc.rows - 1)) / p.group;
     }
-    const int at = g * kTileRows + r;
-    const bool mine = at < pc.rows;
-    const int pair = pc.row0 + min(at, pc.rows - 1), token = pair / p.group, hq = head * p.group + pair - token * p.group;
-    const int64_t pos = int64_t(pc.pos0) + token;
     float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
     for (int i = 0; i < tiles; ++i, ++n) {
-      if (!wait_warp(sm, &sm.bars.s_full[g], seen_scores++ & 1)) return;
+      if (!wait_warp(sm, &sm.bars.s_full[g], phase++ & 1)) return;
       tc_fence_after();
       const TileInfo& t = sm.info[n % kLook];
-      const int64_t first = t.first;
-      float v[4][32];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tmem_ld32(s + q * 32, v[q]);
+      const int first = t.first, ahead = pos - first;  // (tokens that the row sees of this tile end here)
       const uint4 real = *reinterpret_cast<const uint4*>(t.seen);
-      const bool all = first + kTileKeys - 1 <= pos && (real.x & real.y & real.z & real.w) == 0xFFFFFFFFu &&
-                       (!p.window || first > pos - p.window || first + kTileKeys - 1 < p.sinks);
-      tmem_ld_wait();
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tmem_ld_done(v[q]);
-      const bool plain = __all_sync(0xFFFFFFFFu, all);
-      float top;
-      if (plain) {
-        float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            m0 = max3f(m0, v[q][j], v[q][j + 1]);
-            m1 = max3f(m1, v[q][j + 2], v[q][j + 3]);
-          }
-        top = fmaxf(m0, m1) * scale2;
-      } else {
-        const uint32_t bits[4] = {real.x & seen_by(p, first, pos), real.y & seen_by(p, first + 32, pos),
-                                  real.z & seen_by(p, first + 64, pos), real.w & seen_by(p, first + 96, pos)};
-        top = -INFINITY;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            v[q][j] = (bits[q] >> j) & 1u ? v[q][j] * scale2 : -INFINITY;
-            top = fmaxf(top, v[q][j]);
-          }
-      }
-      // the reference follows the running maximum only when that lies more than 2^8 above it
-      const bool over = top > m + 8.0f || (m == -INFINITY && top > m);
-      const float f = over ? ex2(m - top) : 1.0f;  // (0 at first)
-      if (over) {
-        m = top;
-        l *= f;
-      }
-      if (i > 0 && __any_sync(0xFFFFFFFFu, over)) {
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          float x[32];
-          tmem_ld32(o + c, x);
-          tmem_ld_wait();
-          tmem_ld_done(x);
-          uint32_t y[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(x[j] * f);
-          tmem_st32(o + c, y);
-        }
-      }
-      const float ref = m == -INFINITY ? 0.0f : m;
-      const f2 SC = plain ? pk2(scale2, scale2) : pk2(1.0f, 1.0f), NM = pk2(-ref, -ref);
-      f2 sum0 = pk2(0.0f, 0.0f), sum1 = sum0;
+      const bool edge = t.edge != 0;
       bool odd = false;
-      if (t.edge) {  // does V hold values that some rows must not see?
+      if (edge) {  // does V hold values that some rows must not see?
         const int hv = 2 * n + 1;
         if (!wait_warp(sm, &sm.bars.full[hv % S::kStages], (hv / S::kStages) & 1)) return;
         odd = *const_cast<const volatile int32_t*>(&t.odd);
       }
       if (odd) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t w[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float x = ex2(plain ? fmaf(v[q][j], scale2, -ref) : v[q][j] - ref);
-            l += x;
-            w[j] = __float_as_uint(x);
-          }
-          tmem_st32(s + q * 32, w);
-        }
-        tmem_st_wait();
-        add_values_by_row<D>(s, o, base + 2 * S::kTile + uint32_t((2 * n + 1) % S::kStages) * S::kTile, i == 0);
+        const uint4 bits = make_uint4(real.x & seen_by(p, first, ahead), real.y & seen_by(p, first + 32, ahead - 32),
+                                      real.z & seen_by(p, first + 64, ahead - 64), real.w & seen_by(p, first + 96, ahead - 96));
+        tile_by_row<D>(s, o, base + 2 * S::kTile + uint32_t((2 * n + 1) % S::kStages) * S::kTile, bits, scale2, i > 0, m, l);
       } else {
+        float v[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32(s + q * 32, v[q]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld_done(v[q]);
+        if (edge || (real.x & real.y & real.z & real.w) != 0xFFFFFFFFu) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t bits = (q == 0 ? real.x : q == 1 ? real.y : q == 2 ? real.z : real.w) & seen_by(p, first + 32 * q, ahead - 32 * q);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[q][j] = bits >> j & 1u ? v[q][j] : -INFINITY;
+          }
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 32; j += 2)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) top[q] = max3f(top[q], v[q][j], v[q][j + 1]);
+        const float f = follow(fmaxf(max3f(top[0], top[1], top[2]), top[3]) * scale2, m, l);
+        if (i > 0 && __any_sync(0xFFFFFFFFu, f != 1.0f)) scale_sums<D>(o, f);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        const f2 SC = pk2(scale2, scale2), NM = pk2(-ref, -ref);
+        f2 sum0 = pk2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll
         for (int q = 0; q < 4; q += 2) {
           uint32_t w[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const float a = v[q + (j >> 4)][2 * (j & 15)], b = v[q + (j >> 4)][2 * (j & 15) + 1];
             float x, y;
-            upk2(fma2(pk2(a, b), SC, NM), x, y);
+            upk2(fma2(pk2(v[q + (j >> 4)][2 * (j & 15)], v[q + (j >> 4)][2 * (j & 15) + 1]), SC, NM), x, y);
             x = ex2(x);
             y = ex2(y);
             if (j & 1) sum1 = add2(sum1, pk2(x, y));
@@ -850,19 +884,23 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
           }
           tmem_st32(s + (q >> 1) * 32, w);
         }
-        tmem_st_wait();
+        float a, b;
+        upk2(add2(sum0, sum1), a, b);
+        l += a + b;
       }
-      float a, b;
-      upk2(add2(sum0, sum1), a, b);
-      l += a + b;
+      tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.bars.p_ready[g]);
     }
     if (tiles > 0) {
-      if (!wait_warp(sm, &sm.bars.s_full[g], seen_scores++ & 1)) return;
+      if (!wait_warp(sm, &sm.bars.s_full[g], phase++ & 1)) return;
       tc_fence_after();
     }
+    int head;
+    const Piece pc = load_piece(p, work_of(k), head);
+    const bool mine = at < pc.rows;
+    const int pair = pc.row0 + min(at, pc.rows - 1), token = pair / p.group, hq = head * p.group + pair - token * p.group;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
     const int64_t row = (int64_t(pc.first) + token) * p.heads_q + hq;
@@ -912,7 +950,7 @@ template <int D, bool RAW>
 __global__ void __launch_bounds__(kThreadsP, 1) prompt_kernel(const __grid_constant__ PromptParams p) {
   extern __shared__ uint8_t smem[];
   __shared__ Shared sm;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);
   const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
   if (threadIdx.x == 0) {
     PromptBars& b = sm.bars;
@@ -939,7 +977,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) prompt_kernel(const __grid_const
     fewer_registers<80>();
     if (warp < 12) Loader<D, RAW>(p, sm, base, works).run();
     else if (warp > 12) look_up<D>(p, sm, works, warp - 13);
-    else if (lane == 0) issue_products<D, RAW>(p, sm, base, works);
+    else issue_products<D, RAW>(p, sm, base, works);
   }
   __syncwarp();
   tc_fence_before();
@@ -1085,6 +1123,7 @@ extern "C" ashkv_status_t ashkv_prompt_attention(
   p.n_rows = int32_t(n_rows); p.heads_q = heads_q; p.group = heads_q / p.kv.heads_kv;
   p.negate = scale < 0.0f ? 1u << 13 : 0u;
   p.scale2 = (scale < 0.0f ? -scale : scale) * kLog2eP;
+  if (p.scale2 == 0.0f) p.scale2 = 0x1p-126f;  // (a score of -infinity stays one)
   p.window = window; p.sinks = sinks;
   p.out = static_cast<uint16_t*>(d_out); p.lse = d_lse;
   const Sizes s = sizes_of(n_rows, n_seqs, heads_q, p.kv.heads_kv);
