@@ -34,10 +34,12 @@ constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kLn2P = 0.6931471805599453f;
 constexpr int kTileRows = 128, kItemRows = 256, kTileKeys = 128;
 constexpr int kThreadsP = 512, kPlanThreads = 1024, kJoinThreadsP = 256;
-constexpr int kLoaders = 128, kLookWarps = 3, kLook = 6;  // threads that load, warps that look up, tiles looked up ahead
+constexpr int kDecoders = 128;  // threads that decode
+constexpr int kLook = 4;        // tiles looked up ahead
 constexpr uint32_t kPollsP = 1u << 24;                    // bounded waits
 constexpr int kBins = 64;
 constexpr uint32_t kNoPage = 0xFFu;
+constexpr int kMixed = 0x100, kMixedBf16 = 0x101;
 
 // A run of an item's key tiles [begin, end): tile index i stands for tile i of the sequence below ts, else i - ts + tw.
 struct __align__(16) Piece {
@@ -227,17 +229,16 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_
 
 // ---------------------------------------------------------------- main
 // Shared memory: the queries (two tiles), kStages key or value tiles (K, V, K, V ..), and where pages may be
-// compressed kRaw half tiles' codes on their way, with a word of scales for each 16 of them.  A tile is
-// 128 rows of D bf16 in runs of 64 (128 bytes, swizzled).  kAhead half tiles are under way while one is finished.
+// compressed kRaw half tiles' codes on their way, with eight bytes of scales for each row.  A tile is 128 rows of
+// D bf16 in runs of 64 (128 bytes, swizzled).
 template <int D, bool RAW>
 struct Shape {
-  static constexpr int kUnitsRow = D / 16, kRowsPass = kLoaders / kUnitsRow, kPasses = kTileKeys / kRowsPass;  // (with RAW)
   static constexpr uint32_t kHalf = kTileRows * 128, kTile = kHalf * (D / 64);
   static constexpr int kStages = RAW ? (D == 64 ? 6 : 3) : (D == 64 ? 8 : 4);
-  static constexpr int kAhead = kStages - 2;
-  static constexpr int kRaw = RAW ? kAhead + 1 : 0;
-  static constexpr uint32_t kUnits = kTileKeys * D / 16;  // 16 codes each
-  static constexpr uint32_t kBytes = 2 * kTile + kStages * kTile + kRaw * kUnits * 20 + 1024;
+  static constexpr int kRaw = RAW ? (D == 64 ? 6 : 3) : 0;
+  static constexpr int kFetchers = RAW ? 2 : 4;  // warps, a tile in turn each
+  static constexpr uint32_t kCodes = kTileKeys * D, kRawBytes = kCodes + kTileKeys * 8;
+  static constexpr uint32_t kBytes = 2 * kTile + kStages * kTile + kRaw * kRawBytes + 1024;
 };
 
 struct __align__(16) TileInfo {
@@ -247,10 +248,10 @@ struct __align__(16) TileInfo {
   int32_t first;                        // position of the tile's first token
   int32_t edge;                         // some row does not see some token of the tile
   int32_t odd;                          // and one of its values is not finite
-  int32_t pad;
+  int32_t kind;                         // the format of all its rows, or kMixed, kMixedBf16 if BF16 rows are among them
 };
 struct PromptBars {
-  uint64_t q_full, q_empty, full[8], empty[8], info_full[kLook], info_empty[kLook], s_full[2], p_ready[2], drained;
+  uint64_t q_full, q_empty, full[8], empty[8], raw_full[8], raw_empty[8], info_empty[kLook], s_full[2], p_ready[2], drained;
 };
 
 struct Shared {
@@ -287,76 +288,8 @@ __device__ __forceinline__ Piece load_piece(const PromptParams& p, int64_t w, in
 }
 __device__ __forceinline__ int tile_of(const Piece& pc, int i) { return i < pc.ts ? i : i - pc.ts + pc.tw; }
 
-// ---- pages: three warps, a tile in turn each
-template <int D>
-__device__ void look_up(const PromptParams& p, Shared& sm, int64_t works, int which) {
-  const int lane = threadIdx.x & 31;
-  int n = 0;  // tiles of the CTA so far
-  for (int k = 0; work_of(k) < works; ++k) {
-    int head;
-    const Piece pc = load_piece(p, work_of(k), head);
-    const int64_t pa = int64_t(pc.pos0) + pc.row0 / p.group, pb = int64_t(pc.pos0) + (pc.row0 + pc.rows - 1) / p.group;
-    const int32_t* ids = p.lists.page_ids + int64_t(pc.seq) * p.lists.page_ids_stride;
-    for (int i = pc.begin; i < pc.end; ++i, ++n) {
-      if (n % kLookWarps != which) continue;
-      const int first = tile_of(pc, i) * kTileKeys;
-      TileInfo& t = sm.info[n % kLook];
-      // four neighbouring tokens a lane; one look-up where they share a page
-      Place at[4];
-      int tok[4];
-      bool need[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t pos = int64_t(first) + 4 * lane + u;
-        need[u] = pos <= pc.kmax && (pos < p.sinks || pos >= pc.lo || !p.window);
-      }
-      const bool shared_page = p.kv.T % 4 == 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t pos = int64_t(first) + 4 * lane + u;
-        if (u > 0 && shared_page) {
-          at[u] = at[0];
-          tok[u] = tok[0] + u;
-          continue;
-        }
-        const bool any = shared_page ? need[0] || need[1] || need[2] || need[3] : need[u];
-        const int64_t j = pos / p.kv.T;
-        tok[u] = int(pos - j * p.kv.T);
-        at[u] = Place{-1, nullptr, nullptr};
-        if (any) at[u] = place_of(p.kv, ids[j]);
-        if (any && at[u].format < 0) flag(p.lists.status, ASHKV_FLAG_INDEX_RANGE);
-      }
-      if (n >= kLook && !wait_warp(sm, &sm.bars.info_empty[n % kLook], (n / kLook - 1) & 1)) return;
-      uint32_t bits = 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int e = 4 * lane + u;
-        const bool ok = need[u] && at[u].format >= 0;
-        if (ok) bits |= 1u << u;
-        const int64_t off = ok && at[u].format == ASHKV_PAGE_BF16 ? (tok[u] * p.kv.row_stride + head * D) * 2 : 0;
-        const uint64_t none = reinterpret_cast<uint64_t>(p.pieces);  // (an aligned address; nothing is read there)
-        t.k[e] = ok ? reinterpret_cast<uint64_t>(at[u].k) + off : none;
-        t.v[e] = ok ? reinterpret_cast<uint64_t>(at[u].v) + off : none;
-        t.meta[e] = (ok ? uint32_t(at[u].format) : kNoPage) | uint32_t(tok[u]) << 8;
-      }
-      bits <<= 4 * (lane & 7);  // eight lanes make a word
-#pragma unroll
-      for (int off = 1; off < 8; off <<= 1) bits |= __shfl_xor_sync(0xFFFFFFFFu, bits, off);
-      if ((lane & 7) == 0) t.seen[lane >> 3] = bits;
-      if (lane == 0) {
-        t.first = first;
-        const int64_t last = int64_t(first) + kTileKeys - 1;
-        t.edge = !(last <= pa && (!p.window || first > pb - p.window || last < p.sinks));
-        t.odd = 0;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.bars.info_full[n % kLook]);
-    }
-  }
-}
-
-// ---- loads: four warps
-// A row of a half tile, `unit`: 16 of its channels.  Where their two chunks of 16 bytes go.
+// ---- keys and values
+// Chunk `chunk` (16 bytes) of a row of a tile.
 __device__ __forceinline__ uint32_t chunk_at(uint32_t row, uint32_t chunk) {
   return (chunk >> 3) * (kTileRows * 128) + row * 128 + (((chunk & 7u) ^ (row & 7u)) << 4);
 }
@@ -366,13 +299,258 @@ __device__ __forceinline__ void sts128p(uint32_t a, uint4 v) {
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, uint64_t src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, int bytes) {
-  if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" :: "r"(dst), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(dst), "l"(src) : "memory");
+template <int BYTES>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" :: "r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+// An arrival of this lane once its copies so far have landed.
+__device__ __forceinline__ void arrive_with_copies(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ bool not_finite(uint4 x) {
   const uint32_t m = max_u16x2(max_u16x2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu), max_u16x2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
   return (m & 0xFFFFu) >= 0x7F80u || (m >> 16) >= 0x7F80u;
+}
+
+// The codes and scales of row r (a page's row pr, key head `head`) of a compressed page -> a raw half tile.
+template <int D>
+__device__ __forceinline__ void copy_row(const PromptParams& p, uint32_t fmt, const uint8_t* s, uint32_t pr, uint32_t head, uint32_t codes,
+                                         uint32_t scales, uint32_t lane, uint32_t lanes) {
+  const uint32_t T = uint32_t(p.kv.T), row = uint32_t(p.kv.row_len), E = 2 * T * row, e = pr * row + head * D;
+  const uint8_t *from, *scale;
+  uint32_t bytes = D;
+  if (fmt == ASHKV_PAGE_INT8) {
+    from = s + uint32_t(int8_codes_offset(int(T))) + e;
+    scale = s + (2 * pr & ~3u);
+  } else if (fmt == ASHKV_PAGE_FP8) {
+    from = scale = s + e;
+  } else if (fmt == ASHKV_PAGE_INT4) {
+    from = s + E / 32 + e / 2;
+    scale = s + (e / 64 * 2 & ~3u);
+    bytes = D / 2;
+  } else {
+    const uint32_t bits = fmt == ASHKV_PAGE_NBIT4 ? 4 : 2;
+    from = s + nbit_codes_off(E) + e * bits / 8;
+    scale = s + nbit_delta_off() + e / 32 * 2;
+    bytes = D * bits / 8;
+  }
+  for (uint32_t c = lane; c < bytes / 16; c += lanes) cp_async16(codes + c * 16, from + c * 16);
+  if (lane == 0) {
+    if (D == 128 && fmt >= ASHKV_PAGE_NBIT4) cp_async_small<8>(scales, scale);
+    else cp_async_small<4>(scales, scale);
+  }
+}
+
+// Looks up the pages of its tiles, describes them in TileInfo and sends their copies on their way: BF16 rows to
+// their places where all pages are, codes to the raw half tiles where pages may be compressed.
+template <int D, bool RAW>
+__device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, int64_t works, int which) {
+  using S = Shape<D, RAW>;
+  const int lane = threadIdx.x & 31;
+  const uint32_t stages = base + 2 * S::kTile, raw = stages + S::kStages * S::kTile;
+  int n = 0;  // tiles of the CTA so far
+  for (int k = 0; work_of(k) < works; ++k) {
+    int head;
+    const Piece pc = load_piece(p, work_of(k), head);
+    const int pa = pc.pos0 + pc.row0 / p.group, pb = pc.pos0 + (pc.row0 + pc.rows - 1) / p.group;
+    const int32_t* ids = p.lists.page_ids + int64_t(pc.seq) * p.lists.page_ids_stride;
+    for (int i = pc.begin; i < pc.end; ++i, ++n) {
+      if (n % S::kFetchers != which) continue;
+      const int first = tile_of(pc, i) * kTileKeys;
+      TileInfo& t = sm.info[n % kLook];
+      // four neighbouring tokens a lane; one look-up where they share a page
+      Place at[4];
+      int tok[4];
+      bool need[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int pos = first + 4 * lane + u;  // (kmax + 127 at most; wrapped: negative)
+        need[u] = pos >= 0 && pos <= pc.kmax && (pos < p.sinks || pos >= pc.lo || !p.window);
+      }
+      const bool shared_page = p.kv.T % 4 == 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t pos = uint32_t(first + 4 * lane + u);
+        if (u > 0 && shared_page) {
+          at[u] = at[0];
+          tok[u] = tok[0] + u;
+          continue;
+        }
+        const bool any = shared_page ? need[0] || need[1] || need[2] || need[3] : need[u];
+        const uint32_t j = pos / uint32_t(p.kv.T);
+        tok[u] = int(pos - j * uint32_t(p.kv.T));
+        at[u] = Place{-1, nullptr, nullptr};
+        if (any) at[u] = place_of(p.kv, ids[j]);
+        if (any && at[u].format < 0) flag(p.lists.status, ASHKV_FLAG_INDEX_RANGE);
+      }
+      if (n >= kLook && !wait_warp(sm, &sm.bars.info_empty[n % kLook], (n / kLook - 1) & 1)) {
+            cp_async_wait_all();
+            return;
+          }
+      uint32_t bits = 0;
+      int kind = need[0] ? at[0].format : -1;
+      bool bf16 = false;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int e = 4 * lane + u;
+        const bool ok = need[u] && at[u].format >= 0;
+        if (ok) bits |= 1u << u;
+        if (!ok || at[u].format != kind) kind = kMixed;
+        bf16 |= ok && at[u].format == ASHKV_PAGE_BF16;
+        const int64_t off = ok && at[u].format == ASHKV_PAGE_BF16 ? (tok[u] * p.kv.row_stride + head * D) * 2 : 0;
+        const uint64_t none = reinterpret_cast<uint64_t>(p.pieces);  // (an aligned address; nothing is read there)
+        t.k[e] = ok ? reinterpret_cast<uint64_t>(at[u].k) + off : none;
+        t.v[e] = ok ? reinterpret_cast<uint64_t>(at[u].v) + off : none;
+        t.meta[e] = (ok ? uint32_t(at[u].format) : kNoPage) | uint32_t(tok[u]) << 8;
+      }
+      if (!__all_sync(0xFFFFFFFFu, kind == __shfl_sync(0xFFFFFFFFu, kind, 0))) kind = kMixed;
+      if (__any_sync(0xFFFFFFFFu, bf16) && kind == kMixed) kind = kMixedBf16;
+      bits <<= 4 * (lane & 7);  // eight lanes make a word
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) bits |= __shfl_xor_sync(0xFFFFFFFFu, bits, off);
+      if ((lane & 7) == 0) t.seen[lane >> 3] = bits;
+      const int64_t last = int64_t(first) + kTileKeys - 1;
+      const bool edge = !(last <= pa && (!p.window || int64_t(first) > int64_t(pb) - p.window || last < p.sinks));
+      if (lane == 0) {
+        t.first = first;
+        t.edge = edge;
+        t.odd = 0;
+        t.kind = kind;
+      }
+      __syncwarp();
+#pragma unroll 1
+      for (int v = 0; v < 2; ++v) {
+        const int h = 2 * n + v;
+        const uint64_t* rows = v ? t.v : t.k;
+        if constexpr (!RAW) {
+          constexpr uint32_t CPR = D / 8, RPI = 32 / CPR;  // chunks of a row, rows of one instruction
+          const int st = h % S::kStages;
+          const uint32_t to = stages + uint32_t(st) * S::kTile, c = uint32_t(lane) % CPR, r0 = uint32_t(lane) / CPR;
+          if (h >= S::kStages && !wait_warp(sm, &sm.bars.empty[st], (h / S::kStages - 1) & 1)) {
+            cp_async_wait_all();
+            return;
+          }
+#pragma unroll 8
+          for (uint32_t j = 0; j < kTileKeys / RPI; ++j) {
+            const uint32_t r = r0 + RPI * j;
+            cp_async16_zfill(to + chunk_at(r, c), rows[r] + c * 16, (t.meta[r] & 0xFFu) != kNoPage);
+          }
+          if (v && edge) {
+            cp_async_wait_all();
+            bool odd = false;
+            for (uint32_t j = 0; j < kTileKeys / RPI; ++j) odd |= not_finite(lds128(to + chunk_at(r0 + RPI * j, c)));
+            if (odd) *const_cast<volatile int32_t*>(&t.odd) = 1;
+            __syncwarp();
+          }
+          arrive_with_copies(&sm.bars.full[st]);
+          if (lane == 0) mbar_arrive(&sm.bars.full[st]);  // (what the lanes wrote themselves)
+        } else {
+          constexpr uint32_t L = D / 16;  // lanes of a row
+          const int slot = h % S::kRaw;
+          const uint32_t codes = raw + uint32_t(slot) * S::kRawBytes, scales = codes + S::kCodes;
+          if (h >= S::kRaw && !wait_warp(sm, &sm.bars.raw_empty[slot], (h / S::kRaw - 1) & 1)) {
+            cp_async_wait_all();
+            return;
+          }
+#pragma unroll 4
+          for (uint32_t r = uint32_t(lane) / L; r < kTileKeys; r += 32 / L) {
+            const uint32_t meta = t.meta[r], fmt = meta & 0xFFu;
+            if (fmt != kNoPage && fmt != ASHKV_PAGE_BF16)
+              copy_row<D>(p, fmt, reinterpret_cast<const uint8_t*>(rows[r]), (meta >> 8) + (v ? uint32_t(p.kv.T) : 0), uint32_t(head),
+                          codes + r * D, scales + r * 8, uint32_t(lane) % L, L);
+          }
+          arrive_with_copies(&sm.bars.raw_full[slot]);
+          if (lane == 0) mbar_arrive(&sm.bars.raw_full[slot]);
+        }
+      }
+    }
+  }
+  cp_async_wait_all();
+}
+
+// ---- decoding
+// Sixteen INT8 codes with scale s -> sixteen bf16, as int8_dec8 rounds them.  code * s / 127 = code * (H + L) with
+// H = RN(s / 127) and L what that leaves out, so the first step of div_short serves without the product code * s.
+__device__ __forceinline__ void int8_dec16(uint4 c, float s, uint4& x, uint4& y) {
+  if (!int8_dec_fast(s)) {
+    x = int8_dec8(make_uint2(c.x, c.y), s);
+    y = int8_dec8(make_uint2(c.z, c.w), s);
+    return;
+  }
+  const Recip d = make_recip(127.0f);
+  const float h = __fmul_rn(s, d.hi), l = __fmaf_rn(s, d.lo, __fmaf_rn(s, d.hi, -h));
+  const f2 H = pk2(h, h), L = pk2(l, l);
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    f2 a, b;
+    int8x4_to_f2(w[k], a, b);
+    o[2 * k] = f32x2_to_bf16x2_pk(fma2(a, H, mul2(a, L)));
+    o[2 * k + 1] = f32x2_to_bf16x2_pk(fma2(b, H, mul2(b, L)));
+  }
+  x = make_uint4(o[0], o[1], o[2], o[3]);
+  y = make_uint4(o[4], o[5], o[6], o[7]);
+}
+// Sixteen INT4 codes, likewise.
+__device__ __forceinline__ void int4_dec16(uint2 c, uint16_t scale, uint4& x, uint4& y) {
+  const float s = bf16_to_f32(scale);
+  if (!(s >= 0x1p-90f && s <= 0x1p+90f)) {
+    x = int4_dec8(c.x, scale);
+    y = int4_dec8(c.y, scale);
+    return;
+  }
+  const Recip d = make_recip(7.0f);
+  const float h = __fmul_rn(s, d.hi), l = __fmaf_rn(s, d.lo, __fmaf_rn(s, d.hi, -h));
+  const f2 H = pk2(h, h), L = pk2(l, l), bias = pk2(-8388616.0f, -8388616.0f);
+  uint32_t o[8];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t w = k ? c.y : c.x, hi = (w >> 4) & 0x0F0F0F0Fu, lo = w & 0x0F0F0F0Fu;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f2 a = add2(pk2(code_plus_2p23(hi, j), code_plus_2p23(lo, j)), bias);
+      o[4 * k + j] = f32x2_to_bf16x2_pk(fma2(a, H, mul2(a, L)));
+    }
+  }
+  x = make_uint4(o[0], o[1], o[2], o[3]);
+  y = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// Unit u (16 channels) of a row: its codes at `codes`, its scales at `scales`, row pr of the page, key head `head`.
+template <int D>
+__device__ __forceinline__ void decode_unit(uint32_t fmt, uint32_t codes, uint32_t scales, uint32_t u, uint32_t pr, uint32_t head, uint4& x,
+                                            uint4& y) {
+  const auto half = [&](uint32_t at) {
+    uint16_t s;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(s) : "r"(at));
+    return s;
+  };
+  const auto two = [&](uint32_t at) {
+    uint2 c;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(c.x), "=r"(c.y) : "r"(at));
+    return c;
+  };
+  if (fmt == ASHKV_PAGE_INT8) {
+    int8_dec16(lds128(codes + 16 * u), f16_to_f32(half(scales + (pr & 1u) * 2)), x, y);
+  } else if (fmt == ASHKV_PAGE_FP8) {
+    const uint4 c = lds128(codes + 16 * u);
+    x = fp8_dec8(make_uint2(c.x, c.y));
+    y = fp8_dec8(make_uint2(c.z, c.w));
+  } else if (fmt == ASHKV_PAGE_INT4) {
+    int4_dec16(two(codes + 8 * u), half(scales + (D == 128 ? u / 4 : head & 1u) * 2), x, y);
+  } else if (fmt == ASHKV_PAGE_NBIT4) {
+    const uint2 c = two(codes + 8 * u);
+    const uint16_t d = half(scales + u / 2 * 2);
+    x = nbit_dec8<4>(c.x, d);
+    y = nbit_dec8<4>(c.y, d);
+  } else {
+    uint32_t c;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(c) : "r"(codes + 4 * u));
+    const uint16_t d = half(scales + u / 2 * 2);
+    x = nbit_dec8<2>(c & 0xFFFFu, d);
+    y = nbit_dec8<2>(c >> 16, d);
+  }
 }
 
 // The outliers of row pr of a dithered page over its decoded values (row r of a half tile), by the lanes that wrote those.
@@ -389,191 +567,167 @@ __device__ __noinline__ void overlay(const uint8_t* slot, uint32_t T, uint32_t r
   }
 }
 
-template <int D, bool RAW>
-struct Loader {
-  using S = Shape<D, RAW>;
-  const PromptParams& p;
-  Shared& sm;
-  const int tid;
-  const uint32_t q_at, stages, raw, words;
-  const int64_t works;
-  // the half tile to issue next: of work ik, tile ii; in: tiles issued before
-  int ik = 0, ii = 0, iend = 0, ihead = 0, in = 0, ih = 0;
-  bool iv = false, more = true;
-
-  __device__ __forceinline__ Loader(const PromptParams& p_, Shared& sm_, uint32_t base, int64_t works_)
-      : p(p_), sm(sm_), tid(threadIdx.x & (kLoaders - 1)), q_at(base), stages(base + 2 * S::kTile),
-        raw(stages + S::kStages * S::kTile), words(raw + S::kRaw * S::kUnits * 16), works(works_) {
-    open(0);
-  }
-  __device__ __forceinline__ void open(int k) {  // the first work from k on that has tiles
-    for (ik = k;; ++ik) {
-      more = work_of(ik) < works;
-      if (!more) return;
-      const Piece pc = load_piece(p, work_of(ik), ihead);
-      ii = pc.begin;
-      iend = pc.end;
-      if (ii < iend) return;
-    }
-  }
-
-  __device__ __forceinline__ bool issue() {
-    if (more) {
-      TileInfo& t = sm.info[in % kLook];
-      if (!iv && !wait_warp(sm, &sm.bars.info_full[in % kLook], (in / kLook) & 1)) return false;
-      const int st = ih % S::kStages;
-      if (ih >= S::kStages && !wait_warp(sm, &sm.bars.empty[st], (ih / S::kStages - 1) & 1)) return false;
+// Raw half tiles -> key and value tiles.  D / 16 lanes to a row, 16 channels each; BF16 rows among compressed ones are copied
+// a half tile ahead.
+template <int D>
+__device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, int64_t works) {
+  using S = Shape<D, true>;
+  constexpr uint32_t L = D / 16, kStep = kDecoders / L, kPasses = kTileKeys / kStep;
+  const int tid = threadIdx.x & (kDecoders - 1);
+  const uint32_t u = uint32_t(tid) % L, r0 = uint32_t(tid) / L;
+  const uint32_t stages = base + 2 * S::kTile, raw = stages + S::kStages * S::kTile;
+  const uint32_t T = uint32_t(p.kv.T);
+  int copied = 0;  // half tiles whose BF16 rows are on their way
+  // Half tile h: waits for its description and its place, and copies its BF16 rows.
+  const auto open = [&](int h) {
+    const int st = h % S::kStages, slot = h % S::kRaw;
+    if (!wait_warp(sm, &sm.bars.raw_full[slot], (h / S::kRaw) & 1)) return false;
+    if (h >= S::kStages && !wait_warp(sm, &sm.bars.empty[st], (h / S::kStages - 1) & 1)) return false;
+    const TileInfo& t = sm.info[h / 2 % kLook];
+    if (t.kind == kMixedBf16 || t.kind == ASHKV_PAGE_BF16) {
+      const uint64_t* rows = h & 1 ? t.v : t.k;
       const uint32_t to = stages + uint32_t(st) * S::kTile;
-      const uint64_t* rows = iv ? t.v : t.k;
-      if constexpr (!RAW) {
-        constexpr int CPR = D / 8, RPP = kLoaders / CPR;
-        const uint32_t c = uint32_t(tid) % CPR, r0 = uint32_t(tid) / CPR;
-#pragma unroll 8
-        for (uint32_t k = 0; k < kTileKeys / RPP; ++k) {
-          const uint32_t r = r0 + RPP * k;
-          cp_async16_zfill(to + chunk_at(r, c), rows[r] + c * 16, (t.meta[r] & 0xFFu) != kNoPage);
+#pragma unroll 4
+      for (uint32_t k = 0; k < kPasses; ++k) {
+        const uint32_t r = r0 + kStep * k;
+        if ((t.meta[r] & 0xFFu) == ASHKV_PAGE_BF16) {  // (chunks u and u + D / 16: neighbouring lanes, neighbouring chunks)
+          cp_async16_zfill(to + chunk_at(r, u), rows[r] + u * 16, true);
+          cp_async16_zfill(to + chunk_at(r, u + L), rows[r] + (u + L) * 16, true);
         }
-      } else {
-        const uint32_t u = uint32_t(tid) % S::kUnitsRow, r0 = uint32_t(tid) / S::kUnitsRow;
-        const uint32_t slot = uint32_t(ih) % S::kRaw * S::kUnits;
-#pragma unroll 2
-        for (uint32_t k = 0; k < S::kPasses; ++k) {
-          const uint32_t r = r0 + S::kRowsPass * k, meta = t.meta[r], fmt = meta & 0xFFu;
-          const uint64_t base = rows[r];
-          if (fmt == ASHKV_PAGE_BF16) {  // (chunks u and u + D / 16: neighbouring lanes, neighbouring chunks)
-            cp_async16_zfill(to + chunk_at(r, u), base + u * 16, true);
-            cp_async16_zfill(to + chunk_at(r, u + D / 16), base + (u + D / 16) * 16, true);
-          } else if (fmt != kNoPage) {
-            const uint8_t* s = reinterpret_cast<const uint8_t*>(base);
-            const uint32_t T = uint32_t(p.kv.T), row = uint32_t(p.kv.row_len), E = 2 * T * row;
-            const uint32_t pr = (meta >> 8) + (iv ? T : 0), e = pr * row + uint32_t(ihead) * D + 16 * u;
-            const uint32_t d = raw + (slot + r * S::kUnitsRow + u) * 16, w = words + (slot + r * S::kUnitsRow + u) * 4;
-            if (fmt == ASHKV_PAGE_INT8) {
-              cp_async16(d, s + uint32_t(int8_codes_offset(T)) + e);
-              cp_async_small(w, s + (2 * pr & ~3u), 4);
-            } else if (fmt == ASHKV_PAGE_FP8) {
-              cp_async16(d, s + e);
-            } else if (fmt == ASHKV_PAGE_INT4) {
-              cp_async_small(d, s + E / 32 + e / 2, 8);
-              cp_async_small(w, s + (e / 64 * 2 & ~3u), 4);
-            } else if (fmt == ASHKV_PAGE_NBIT4) {
-              cp_async_small(d, s + nbit_codes_off(E) + e / 2, 8);
-              cp_async_small(w, s + nbit_delta_off() + (e / 32 * 2 & ~3u), 4);
-            } else {
-              cp_async_small(d, s + nbit_codes_off(E) + e / 4, 4);
-              cp_async_small(w, s + nbit_delta_off() + (e / 32 * 2 & ~3u), 4);
-            }
-          }
-        }
-      }
-      ++ih;
-      iv = !iv;
-      if (!iv) {
-        ++in;
-        if (++ii == iend) open(ik + 1);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     return true;
+  };
+  int total = 0;
+  for (int k = 0; work_of(k) < works; ++k) {
+    int head;
+    const Piece pc = load_piece(p, work_of(k), head);
+    total += max(0, pc.end - pc.begin);
   }
-
-  // The bf16 values of a unit of a compressed page.
-  __device__ __forceinline__ void decode(uint32_t fmt, uint32_t d, uint32_t word, uint32_t pr, uint32_t e, uint4& x, uint4& y) const {
-    if (fmt == ASHKV_PAGE_INT8) {
-      const uint4 c = lds128(d);
-      const float s = f16_to_f32(uint16_t(pr & 1u ? word >> 16 : word));
-      x = int8_dec8(make_uint2(c.x, c.y), s);
-      y = int8_dec8(make_uint2(c.z, c.w), s);
-    } else if (fmt == ASHKV_PAGE_FP8) {
-      const uint4 c = lds128(d);
-      x = fp8_dec8(make_uint2(c.x, c.y));
-      y = fp8_dec8(make_uint2(c.z, c.w));
-    } else {
-      uint2 c;
-      asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(c.x), "=r"(c.y) : "r"(d));
-      if (fmt == ASHKV_PAGE_INT4) {
-        const uint16_t s = uint16_t(e / 64 & 1u ? word >> 16 : word);
-        x = int4_dec8(c.x, s);
-        y = int4_dec8(c.y, s);
-        return;
-      }
-      const uint16_t s = uint16_t(e / 32 & 1u ? word >> 16 : word);
-      if (fmt == ASHKV_PAGE_NBIT4) {
-        x = nbit_dec8<4>(c.x, s);
-        y = nbit_dec8<4>(c.y, s);
-      } else {
-        x = nbit_dec8<2>(c.x & 0xFFFFu, s);
-        y = nbit_dec8<2>(c.x >> 16, s);
-      }
-    }
-  }
-
-  // Half tile h (of tile n, key head `head`) has arrived: decodes what is compressed, and hands it over.
-  __device__ __forceinline__ void finish(int h, int n, int head, bool v) {
-    const uint32_t st = uint32_t(h) % S::kStages, to = stages + st * S::kTile;
-    TileInfo& t = sm.info[n % kLook];
-    const bool look = v && t.edge;
-    bool odd = false;
-    if constexpr (RAW) {
-      const uint32_t u = uint32_t(tid) % S::kUnitsRow, r0 = uint32_t(tid) / S::kUnitsRow;
-      const uint32_t slot = uint32_t(h) % S::kRaw * S::kUnits;
-      bool dithered = false;
-#pragma unroll 2
-      for (uint32_t k = 0; k < S::kPasses; ++k) {
-        const uint32_t r = r0 + S::kRowsPass * k, meta = t.meta[r], fmt = meta & 0xFFu;
-        uint4 x = make_uint4(0, 0, 0, 0), y = x;
-        if (fmt == ASHKV_PAGE_BF16) {
-          if (look) odd |= not_finite(lds128(to + chunk_at(r, u))) || not_finite(lds128(to + chunk_at(r, u + D / 16)));
-          continue;
-        }
-        if (fmt != kNoPage) {
-          const uint32_t pr = (meta >> 8) + (v ? uint32_t(p.kv.T) : 0), e = pr * uint32_t(p.kv.row_len) + uint32_t(head) * D + 16 * u;
-          uint32_t word;
-          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(word) : "r"(words + (slot + r * S::kUnitsRow + u) * 4));
-          decode(fmt, raw + (slot + r * S::kUnitsRow + u) * 16, word, pr, e, x, y);
-          dithered |= fmt >= ASHKV_PAGE_NBIT4;
-          if (look) odd |= not_finite(x) || not_finite(y);
-        }
-        // lanes of the upper half of a row store their odd chunk first: eight lanes, eight banks of 16 bytes
-        const bool swap = u >= 4;
-        sts128p(to + chunk_at(r, 2 * u + swap), swap ? y : x);
-        sts128p(to + chunk_at(r, 2 * u + !swap), swap ? x : y);
-      }
-      if (__any_sync(0xFFFFFFFFu, dithered)) {
-        __syncwarp();
-        for (uint32_t k = 0; k < S::kPasses; ++k) {
-          const uint32_t r = r0 + S::kRowsPass * k, meta = t.meta[r], fmt = meta & 0xFFu;
-          const uint8_t* s = reinterpret_cast<const uint8_t*>(v ? t.v[r] : t.k[r]);
-          const uint32_t pr = (meta >> 8) + (v ? uint32_t(p.kv.T) : 0);
-          const uint32_t T = uint32_t(p.kv.T), row = uint32_t(p.kv.row_len), cap = uint32_t(p.kv.outlier_cap);
-          if (fmt == ASHKV_PAGE_NBIT4) overlay<D, 4>(s, T, row, cap, pr, r, u, to, uint32_t(head));
-          else if (fmt == ASHKV_PAGE_NBIT2) overlay<D, 2>(s, T, row, cap, pr, r, u, to, uint32_t(head));
-        }
-        __syncwarp();
-        if (look)  // (outliers may be infinite too)
-          for (uint32_t k = 0; k < S::kPasses; ++k) {
-            const uint32_t r = r0 + S::kRowsPass * k;
-            odd |= not_finite(lds128(to + chunk_at(r, 2 * u))) || not_finite(lds128(to + chunk_at(r, 2 * u + 1)));
+  int n = 0;
+  for (int k = 0; work_of(k) < works; ++k) {
+    int head;
+    const Piece pc = load_piece(p, work_of(k), head);
+    for (int i = pc.begin; i < pc.end; ++i, ++n)
+#pragma unroll 1
+      for (int v = 0; v < 2; ++v) {
+        const int h = 2 * n + v, st = h % S::kStages, slot = h % S::kRaw;
+        if (copied == h) {
+          if (!open(h)) {
+            cp_async_wait_all();
+            return;
           }
+          ++copied;
+        }
+        TileInfo& t = sm.info[n % kLook];
+        const int kind = t.kind;
+        // (BF16 rows: the next half tile's as well, if it is near)
+        bool ahead = false;
+        if ((kind == kMixedBf16 || kind == ASHKV_PAGE_BF16) && copied < 2 * total) {
+          if (!open(h + 1)) {
+            cp_async_wait_all();
+            return;
+          }
+          ++copied;
+          ahead = true;
+        }
+        const uint32_t to = stages + uint32_t(st) * S::kTile, codes = raw + uint32_t(slot) * S::kRawBytes, scales = codes + S::kCodes;
+        const bool look = v && t.edge;
+        bool odd = false;
+        const auto put = [&](uint32_t r, uint4 x, uint4 y) {
+          if (look) odd |= not_finite(x) || not_finite(y);
+          // lanes of the upper half of a row store their odd chunk first: eight lanes, eight banks of 16 bytes
+          const bool swap = u >= 4;
+          sts128p(to + chunk_at(r, 2 * u + swap), swap ? y : x);
+          sts128p(to + chunk_at(r, 2 * u + !swap), swap ? x : y);
+        };
+        const auto page_row = [&](uint32_t r) { return (t.meta[r] >> 8) + (v ? T : 0u); };
+        const auto all_rows = [&](auto format) {
+          constexpr uint32_t F = decltype(format)::value;
+#pragma unroll 4
+          for (uint32_t j = 0; j < kPasses; ++j) {
+            const uint32_t r = r0 + kStep * j;
+            uint4 x, y;
+            decode_unit<D>(F, codes + r * D, scales + r * 8, u, F == ASHKV_PAGE_INT8 ? page_row(r) : 0u, uint32_t(head), x, y);
+            put(r, x, y);
+          }
+        };
+        if (kind == ASHKV_PAGE_INT8) {
+          all_rows(std::integral_constant<uint32_t, ASHKV_PAGE_INT8>());
+        } else if (kind == ASHKV_PAGE_FP8) {
+          all_rows(std::integral_constant<uint32_t, ASHKV_PAGE_FP8>());
+        } else if (kind == ASHKV_PAGE_INT4) {
+          all_rows(std::integral_constant<uint32_t, ASHKV_PAGE_INT4>());
+        } else if (kind != ASHKV_PAGE_BF16) {
+          bool dithered = false;
+#pragma unroll 1
+          for (uint32_t j = 0; j < kPasses; ++j) {
+            const uint32_t r = r0 + kStep * j, fmt = t.meta[r] & 0xFFu;
+            if (fmt == ASHKV_PAGE_BF16) continue;
+            uint4 x = make_uint4(0, 0, 0, 0), y = x;
+            if (fmt != kNoPage) decode_unit<D>(fmt, codes + r * D, scales + r * 8, u, page_row(r), uint32_t(head), x, y);
+            dithered |= fmt != kNoPage && fmt >= ASHKV_PAGE_NBIT4;
+            put(r, x, y);
+          }
+          if (__any_sync(0xFFFFFFFFu, dithered)) {
+            __syncwarp();
+            for (uint32_t j = 0; j < kPasses; ++j) {
+              const uint32_t r = r0 + kStep * j, fmt = t.meta[r] & 0xFFu;
+              const uint8_t* s = reinterpret_cast<const uint8_t*>(v ? t.v[r] : t.k[r]);
+              const uint32_t row = uint32_t(p.kv.row_len), cap = uint32_t(p.kv.outlier_cap);
+              if (fmt == ASHKV_PAGE_NBIT4) overlay<D, 4>(s, T, row, cap, page_row(r), r, u, to, uint32_t(head));
+              else if (fmt == ASHKV_PAGE_NBIT2) overlay<D, 2>(s, T, row, cap, page_row(r), r, u, to, uint32_t(head));
+            }
+            __syncwarp();
+            if (look)  // (outliers may be infinite too)
+              for (uint32_t j = 0; j < kPasses; ++j) {
+                const uint32_t r = r0 + kStep * j;
+                if ((t.meta[r] & 0xFFu) != ASHKV_PAGE_BF16)
+                  odd |= not_finite(lds128(to + chunk_at(r, 2 * u))) || not_finite(lds128(to + chunk_at(r, 2 * u + 1)));
+              }
+          }
+        }
+        if (kind == kMixedBf16 || kind == ASHKV_PAGE_BF16) {
+          if (ahead) asm volatile("cp.async.wait_group 1;" ::: "memory");
+          else cp_async_wait_all();
+          if (look)
+            for (uint32_t j = 0; j < kPasses; ++j) {
+              const uint32_t r = r0 + kStep * j;
+              if ((t.meta[r] & 0xFFu) == ASHKV_PAGE_BF16)
+                odd |= not_finite(lds128(to + chunk_at(r, u))) || not_finite(lds128(to + chunk_at(r, u + L)));
+            }
+        }
+        if (odd) *const_cast<volatile int32_t*>(&t.odd) = 1;
+        fence_proxy_async_smem();
+        mbar_arrive(&sm.bars.full[st]);
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&sm.bars.raw_empty[slot]);
       }
-    } else if (look) {
-      constexpr int CPR = D / 8, RPP = kLoaders / CPR;
-      const uint32_t c = uint32_t(tid) % CPR, r0 = uint32_t(tid) / CPR;
-      for (uint32_t k = 0; k < kTileKeys / RPP; ++k) odd |= not_finite(lds128(to + chunk_at(r0 + RPP * k, c)));
-    }
-    if (odd) *const_cast<volatile int32_t*>(&t.odd) = 1;
-    fence_proxy_async_smem();
-    mbar_arrive(&sm.bars.full[st]);
   }
+  cp_async_wait_all();
+}
 
-  __device__ __forceinline__ void load_queries(const Piece& pc, int head) {
-    constexpr int CPR = D / 8, RPP = kLoaders / CPR;
-    const uint32_t c = uint32_t(tid) % CPR, r0 = uint32_t(tid) / CPR;
+// ---- queries: a warp
+template <int D, bool RAW>
+__device__ void load_queries(const PromptParams& p, Shared& sm, uint32_t base, int64_t works) {
+  using S = Shape<D, RAW>;
+  constexpr uint32_t CPR = D / 8, RPI = 32 / CPR;
+  const int lane = threadIdx.x & 31;
+  const uint32_t c = uint32_t(lane) % CPR, r0 = uint32_t(lane) / CPR;
+  int loads = 0;
+  for (int k = 0; work_of(k) < works; ++k) {
+    int head;
+    const Piece pc = load_piece(p, work_of(k), head);
+    if (pc.begin >= pc.end) continue;
+    if (loads > 0 && !wait_warp(sm, &sm.bars.q_empty, (loads - 1) & 1)) break;
+    ++loads;
     const int rows = pc.rows > kTileRows ? kItemRows : kTileRows;
-    for (int r = int(r0); r < rows; r += RPP) {
+#pragma unroll 4
+    for (int r = int(r0); r < rows; r += RPI) {
       const int pair = pc.row0 + r, token = pair / p.group;
       const uint16_t* src = p.q + (int64_t(pc.first) + token) * p.q_row + int64_t(head * p.group + pair - token * p.group) * p.q_head + c * 8;
-      const uint32_t to = q_at + uint32_t(r / kTileRows) * S::kTile + chunk_at(uint32_t(r % kTileRows), c);
+      const uint32_t to = base + uint32_t(r / kTileRows) * S::kTile + chunk_at(uint32_t(r % kTileRows), c);
       const bool real = r < pc.rows;
       if (p.q_wide) {
         cp_async16_zfill(to, real ? reinterpret_cast<uint64_t>(src) : reinterpret_cast<uint64_t>(p.pieces), real);
@@ -585,34 +739,11 @@ struct Loader {
         sts128p(to, make_uint4(w[0], w[1], w[2], w[3]));
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
-
-  __device__ void run() {
-    int h = 0, n = 0, q_loads = 0;
-    bool ok = true;
-    for (int k = 0; k < S::kAhead && ok; ++k) ok = issue();
-    for (int k = 0; ok && work_of(k) < works; ++k) {
-      int head;
-      const Piece pc = load_piece(p, work_of(k), head);
-      if (pc.begin >= pc.end) continue;
-      if (q_loads > 0 && !(ok = wait_warp(sm, &sm.bars.q_empty, (q_loads - 1) & 1))) break;
-      ++q_loads;
-      load_queries(pc, head);
-      cp_async_wait_all();
-      fence_proxy_async_smem();
-      mbar_arrive(&sm.bars.q_full);
-      for (int i = pc.begin; ok && i < pc.end; ++i, ++n)
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          if (!(ok = issue())) break;
-          asm volatile("cp.async.wait_group %0;" :: "n"(S::kAhead) : "memory");
-          finish(h++, n, head, v != 0);
-        }
-    }
     cp_async_wait_all();
+    fence_proxy_async_smem();
+    mbar_arrive(&sm.bars.q_full);
   }
-};
+}
 
 // ---- products: a warp, whose elected lane issues them
 template <int D, bool RAW>
@@ -672,12 +803,14 @@ __device__ void issue_products(const PromptParams& p, Shared& sm, uint32_t base,
             odd = __any_sync(0xFFFFFFFFu, *const_cast<volatile int32_t*>(&sm.info[(n + i - 1) % kLook].odd));
           }
           if (!(ok = wait_warp(sm, &sm.bars.p_ready[g], ready[g]++ & 1))) break;
+          fence_proxy_async_smem();  // (copies that landed without a thread to fence them)
           tc_fence_after();
           if (!odd) values(g, sv, i > 1);
           if (i == tiles) commit(&sm.bars.s_full[g]);
         }
         if (i < tiles) {
           if (g == 0 && !(ok = wait_warp(sm, &sm.bars.full[sk], (hk / S::kStages) & 1))) break;
+          fence_proxy_async_smem();
           tc_fence_after();
           scores(g, sk);
         }
@@ -954,10 +1087,15 @@ __global__ void __launch_bounds__(kThreadsP, 1) prompt_kernel(const __grid_const
   const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
   if (threadIdx.x == 0) {
     PromptBars& b = sm.bars;
-    mbar_init(&b.q_full, kLoaders);
+    mbar_init(&b.q_full, 32);
     mbar_init(&b.q_empty, 1);
-    for (int i = 0; i < 8; ++i) { mbar_init(&b.full[i], kLoaders); mbar_init(&b.empty[i], 1); }
-    for (int i = 0; i < kLook; ++i) { mbar_init(&b.info_full[i], 1); mbar_init(&b.info_empty[i], 1); }
+    for (int i = 0; i < 8; ++i) {
+      mbar_init(&b.full[i], RAW ? kDecoders : 33);  // (the lanes' copies, and what they wrote)
+      mbar_init(&b.empty[i], 1);
+      mbar_init(&b.raw_full[i], 33);
+      mbar_init(&b.raw_empty[i], kDecoders / 32);
+    }
+    for (int i = 0; i < kLook; ++i) mbar_init(&b.info_empty[i], 1);
     for (int g = 0; g < 2; ++g) { mbar_init(&b.s_full[g], 1); mbar_init(&b.p_ready[g], 4); }
     mbar_init(&b.drained, 1);
     mbar_init_fence();
@@ -975,9 +1113,14 @@ __global__ void __launch_bounds__(kThreadsP, 1) prompt_kernel(const __grid_const
     softmax_rows<D, RAW>(p, sm, base, works, warp >> 2);
   } else {
     fewer_registers<80>();
-    if (warp < 12) Loader<D, RAW>(p, sm, base, works).run();
-    else if (warp > 12) look_up<D>(p, sm, works, warp - 13);
-    else issue_products<D, RAW>(p, sm, base, works);
+    if (warp == 12) issue_products<D, RAW>(p, sm, base, works);
+    else if (warp == 13) load_queries<D, RAW>(p, sm, base, works);
+    else if constexpr (RAW) {
+      if (warp < 12) decode_tiles<D>(p, sm, base, works);
+      else fetch_tiles<D, RAW>(p, sm, base, works, warp - 14);
+    } else if (warp < 12) {
+      fetch_tiles<D, RAW>(p, sm, base, works, warp - 8);
+    }
   }
   __syncwarp();
   tc_fence_before();
