@@ -83,7 +83,7 @@ SIGNATURES: dict[str, tuple] = {
                                              _I64, _F32, _P, _P, _P, _P, _P]),
     "ashkv_write_kv": (_I32, [_P, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I32, _P, _P, _I32, _P, _P]),
     "ashkv_read_kv": (_I32, [_P, _P, _I64, _I32, _P, _P, _I32, _I64, _P, _P, _P, _P]),
-    "ashkv_prompt_scratch_floats": (_I64, [_I64, _I32, _I32, _I32, _I32]),
+    "ashkv_prompt_scratch_floats": (_I64, [_I64, _I32, _I32, _I32, _I32, _I32]),
     "ashkv_prompt_attention": (_I32, [_P, _P, _I64, _I64, _I64, _I32, _P, _I64, _I32, _P, _P, _I32, _I32, _I32, _F32, _P,
                                       _P, _P, _P, _P]),
     "ashkv_page_bounds": (_I32, [_P, _P, _P, _I32, _P, _P, _P, _P, _P]),
@@ -621,8 +621,8 @@ def read_kv(desc: PagedKVDesc, page_ids: torch.Tensor, lengths: torch.Tensor, st
         "read_kv")
 
 
-def prompt_scratch_floats(n_rows: int, n_seqs: int, heads_q: int, heads_kv: int, head_dim: int) -> int:
-    return int(lib().ashkv_prompt_scratch_floats(n_rows, n_seqs, heads_q, heads_kv, head_dim))
+def prompt_scratch_floats(n_rows: int, n_seqs: int, heads_q: int, heads_kv: int, head_dim: int, n_layers: int) -> int:
+    return int(lib().ashkv_prompt_scratch_floats(n_rows, n_seqs, heads_q, heads_kv, head_dim, n_layers))
 
 
 def prompt_attention(desc: PagedKVDesc, q: torch.Tensor, page_ids: torch.Tensor, lengths: torch.Tensor,

@@ -283,7 +283,7 @@ def prompt_attention(q: torch.Tensor, table: DevicePageTable, kv: KVLayers,
     lse = torch.empty(n_rows, heads_q, dtype=torch.float32, device=dev) if return_lse else None
     if n_seqs and n_rows:
         with _on(dev):
-            scratch = torch.empty(_native.prompt_scratch_floats(n_rows, n_seqs, heads_q, desc.heads_kv, d),
+            scratch = torch.empty(_native.prompt_scratch_floats(n_rows, n_seqs, heads_q, desc.heads_kv, d, kv.n_layers),
                                   dtype=torch.float32, device=dev)
             _native.prompt_attention(desc, q, page_ids, lengths, starts, window or 0, sinks,
                                      1.0 / math.sqrt(d) if scale is None else float(scale), out, lse, scratch, status)

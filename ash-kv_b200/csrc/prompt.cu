@@ -18,6 +18,9 @@
 // into shared memory, decoding them where a page is compressed; three warps that look the pages
 // up; one that issues the products.  While one tile's scores become weights the tensor cores work
 // on the other's.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -33,7 +36,7 @@ namespace {
 constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kLn2P = 0.6931471805599453f;
 constexpr int kTileRows = 128, kItemRows = 256, kTileKeys = 128;
-constexpr int kThreadsP = 512, kPlanThreads = 1024, kJoinThreadsP = 256;
+constexpr int kPlanThreads = 1024, kJoinThreadsP = 256;
 constexpr int kDecoders = 128;  // threads that decode
 constexpr int kLook = 4;        // tiles looked up ahead
 constexpr uint32_t kPollsP = 1u << 24;                    // bounded waits
@@ -73,6 +76,8 @@ struct PromptParams {
   float* part_o;     // [max_parts * heads_kv][part_rows][D], each divided by its sum
   float* part_lse2;  // [max_parts * heads_kv][part_rows]
   int32_t part_rows;
+  uint8_t* maps;     // [n_layers][K, V] maps of 128 bytes for tensor copies
+  int32_t box_rows;  // of a copy: the largest power of two, up to 128, of which a page is a multiple; 0: no tensor copies
 };
 
 // ---------------------------------------------------------------- plan
@@ -117,7 +122,9 @@ __device__ __forceinline__ int seq_of_item(const int32_t* prefix, int n_seqs, in
 
 // One CTA.  Counts the items of each sequence, then their key tiles; cuts what is longer than a CTA's share;
 // writes the pieces, the longest first (64 bins of lengths).
-__global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_constant__ PromptParams p, int least) {
+// And the maps of the layers' pools, from one that the host has made but for the address.
+__global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_constant__ PromptParams p,
+                                                                   const __grid_constant__ CUtensorMap pool, int least) {
   __shared__ int s_warp[32], s_base, s_longest, s_parts, s_splits;
   __shared__ unsigned long long s_tiles;
   __shared__ int s_bin[kBins];
@@ -127,6 +134,16 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_
   wait_for_previous();
   allow_next();
   __syncthreads();
+  if (p.box_rows) {
+    for (int i = tid; i < 2 * p.kv.n_layers; i += kPlanThreads) {
+      uint4* to = reinterpret_cast<uint4*>(p.maps + int64_t(i) * 128);
+      const uint4* from = reinterpret_cast<const uint4*>(&pool);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) to[k] = from[k];
+      set_map_address(to, (i & 1 ? p.kv.layer_v : p.kv.layer_k)[i >> 1]);
+    }
+    release_map();
+  }
   const int n_seqs = p.lists.n_seqs;
   bool bad = false;
   for (int b0 = 0; b0 < n_seqs; b0 += kPlanThreads) {
@@ -228,15 +245,22 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_
 }
 
 // ---------------------------------------------------------------- main
-// Shared memory: the queries (two tiles), kStages key or value tiles (K, V, K, V ..), and where pages may be
-// compressed kRaw half tiles' codes on their way, with eight bytes of scales for each row.  A tile is 128 rows of
-// D bf16 in runs of 64 (128 bytes, swizzled).
+// Shared memory: the queries (two tiles), kStages key or value tiles (K, V, K, V ..), and with RAW kRaw half tiles' codes
+// on their way, with eight bytes of scales for each row.  A tile is 128 rows of D bf16 in runs of 64 (128 bytes,
+// swizzled).  RAW: pages may be compressed, or of a size that tensor copies cannot place; else all tiles come by tensor copies.
+// Warps: eight for the softmax, one that issues the products, one that loads queries; then RAW: two that fetch, a tile in
+// turn each, and four that decode; else one that fetches and one that checks values.  Registers: what the softmax warps
+// take more than the launch gives, the others take less.
 template <int D, bool RAW>
 struct Shape {
   static constexpr uint32_t kHalf = kTileRows * 128, kTile = kHalf * (D / 64);
   static constexpr int kStages = RAW ? (D == 64 ? 6 : 3) : (D == 64 ? 8 : 4);
   static constexpr int kRaw = RAW ? (D == 64 ? 6 : 3) : 0;
-  static constexpr int kFetchers = RAW ? 2 : 4;  // warps, a tile in turn each
+  static constexpr int kFetchers = RAW ? 2 : 1;
+  static constexpr int kThreads = RAW ? 512 : 384, kSoftmaxRegs = RAW ? 176 : 200, kOtherRegs = RAW ? 80 : 104;
+  // (A wait for a phase is sound only where the phase before is known to be over: with two fetchers in turn, from three raw
+  // half tiles on.)
+  static_assert(!RAW || kRaw >= kFetchers + 1);
   static constexpr uint32_t kCodes = kTileKeys * D, kRawBytes = kCodes + kTileKeys * 8;
   static constexpr uint32_t kBytes = 2 * kTile + kStages * kTile + kRaw * kRawBytes + 1024;
 };
@@ -251,7 +275,7 @@ struct __align__(16) TileInfo {
   int32_t kind;                         // the format of all its rows, or kMixed, kMixedBf16 if BF16 rows are among them
 };
 struct PromptBars {
-  uint64_t q_full, q_empty, full[8], empty[8], raw_full[8], raw_empty[8], info_empty[kLook], s_full[2], p_ready[2], drained;
+  uint64_t q_full, q_empty, full[8], empty[8], raw_full[8], raw_empty[8], info_empty[kLook], checked[kLook], s_full[2], p_ready[2], drained;
 };
 
 struct Shared {
@@ -312,61 +336,194 @@ __device__ __forceinline__ bool not_finite(uint4 x) {
   return (m & 0xFFFFu) >= 0x7F80u || (m >> 16) >= 0x7F80u;
 }
 
-// The codes and scales of row r (a page's row pr, key head `head`) of a compressed page -> a raw half tile.
+// A tensor copy by a map in global memory, to a shared address.
+__device__ __forceinline__ void tma_load_2d_at(uint32_t to, const void* map, uint64_t* bar, int32_t x, int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      :: "r"(to), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+
+// Where the codes and scales of a row (row pr of a compressed page, key head `head`) are, and the bytes of its codes.
+struct RowBytes {
+  const uint8_t *codes, *scales;
+  uint32_t bytes;
+};
 template <int D>
-__device__ __forceinline__ void copy_row(const PromptParams& p, uint32_t fmt, const uint8_t* s, uint32_t pr, uint32_t head, uint32_t codes,
-                                         uint32_t scales, uint32_t lane, uint32_t lanes) {
+__device__ __forceinline__ RowBytes row_bytes(const PromptParams& p, uint32_t fmt, const uint8_t* s, uint32_t pr, uint32_t head) {
   const uint32_t T = uint32_t(p.kv.T), row = uint32_t(p.kv.row_len), E = 2 * T * row, e = pr * row + head * D;
-  const uint8_t *from, *scale;
-  uint32_t bytes = D;
-  if (fmt == ASHKV_PAGE_INT8) {
-    from = s + uint32_t(int8_codes_offset(int(T))) + e;
-    scale = s + (2 * pr & ~3u);
-  } else if (fmt == ASHKV_PAGE_FP8) {
-    from = scale = s + e;
-  } else if (fmt == ASHKV_PAGE_INT4) {
-    from = s + E / 32 + e / 2;
-    scale = s + (e / 64 * 2 & ~3u);
-    bytes = D / 2;
-  } else {
-    const uint32_t bits = fmt == ASHKV_PAGE_NBIT4 ? 4 : 2;
-    from = s + nbit_codes_off(E) + e * bits / 8;
-    scale = s + nbit_delta_off() + e / 32 * 2;
-    bytes = D * bits / 8;
-  }
-  for (uint32_t c = lane; c < bytes / 16; c += lanes) cp_async16(codes + c * 16, from + c * 16);
-  if (lane == 0) {
-    if (D == 128 && fmt >= ASHKV_PAGE_NBIT4) cp_async_small<8>(scales, scale);
-    else cp_async_small<4>(scales, scale);
+  if (fmt == ASHKV_PAGE_INT8) return {s + uint32_t(int8_codes_offset(int(T))) + e, s + (2 * pr & ~3u), D};
+  if (fmt == ASHKV_PAGE_FP8) return {s + e, s + e, D};
+  if (fmt == ASHKV_PAGE_INT4) return {s + E / 32 + e / 2, s + (e / 64 * 2 & ~3u), D / 2};
+  const uint32_t bits = fmt == ASHKV_PAGE_NBIT4 ? 4 : 2;
+  return {s + nbit_codes_off(E) + e * bits / 8, s + nbit_delta_off() + e / 32 * 2, D * bits / 8};
+}
+
+// The tokens of 32 from first on that some row of a piece sees.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t needed_of(const PromptParams& p, const Piece& pc, int first) {
+  uint32_t m = low_bits(pc.kmax + 1 - first);
+  if (p.window) m &= ~low_bits(pc.lo - first) | low_bits(p.sinks - first);
+  return m;
+}
+// Whether some row of a piece does not see some token of the tile from `first` on.
+__device__ __forceinline__ bool edge_of(const PromptParams& p, const Piece& pc, int first) {
+  const int64_t pa = int64_t(pc.pos0) + pc.row0 / p.group, pb = int64_t(pc.pos0) + (pc.row0 + pc.rows - 1) / p.group;
+  const int64_t last = int64_t(first) + kTileKeys - 1;
+  return !(last <= pa && (!p.window || first > pb - p.window || last < p.sinks));
+}
+
+// All pages in the pool, of a multiple of eight tokens: tensor copies of boxes of 64 channels.  A lane a box; what
+// it has to look up is on its way while the tiles before are sent: the page ids of the tile after next, the table's
+// columns of the next.  Boxes that nobody needs, or whose page does not exist, come from behind the pool's end: zeros.
+template <int D>
+__device__ void fetch_boxes(const PromptParams& p, Shared& sm, uint32_t base, int64_t works) {
+  using S = Shape<D, false>;
+  const int lane = threadIdx.x & 31;
+  const int box = p.box_rows, boxes = kTileKeys / box, group = lane % boxes, half = lane / boxes;  // (of 64 channels)
+  const bool active = half < D / 64;
+  const uint32_t stages = base + 2 * S::kTile;
+  const int end = int(p.kv.pool_tokens);
+  struct Tile {
+    int first, head, off, id, tier, layer, start;  // off: of the box in its page
+    uint32_t needed;                               // lanes 0 .. 3: a bit for each token
+    bool real, edge, wanted;
+  };
+  // a walk over the CTA's tiles
+  int wk = 0, wi = 0, whead = 0;
+  Piece wp{};
+  bool more = true;
+  const auto open = [&](int k) {
+    for (wk = k;; ++wk) {
+      more = work_of(wk) < works;
+      if (!more) return;
+      wp = load_piece(p, work_of(wk), whead);
+      wi = wp.begin;
+      if (wi < wp.end) return;
+    }
+  };
+  const auto next_ids = [&](Tile& x) {
+    x.real = more;
+    if (!more) return;
+    x.first = tile_of(wp, wi) * kTileKeys;
+    x.head = whead;
+    x.needed = lane < 4 ? needed_of(p, wp, x.first + 32 * lane) : 0u;
+    x.edge = edge_of(p, wp, x.first);
+    const uint32_t pos = uint32_t(x.first + group * box), j = pos / uint32_t(p.kv.T);
+    x.off = int(pos - j * uint32_t(p.kv.T));
+    const int last = int(pos) + box - 1;
+    x.wanted = active && int(pos) >= 0 && int(pos) <= wp.kmax && (!p.window || last >= wp.lo || int(pos) < p.sinks);
+    x.id = -1;
+    if (x.wanted) x.id = p.lists.page_ids[int64_t(wp.seq) * p.lists.page_ids_stride + j];
+    if (++wi == wp.end) open(wk + 1);
+  };
+  const auto next_columns = [&](Tile& x) {
+    x.tier = -1;
+    if (x.real && x.id >= 0 && x.id < p.kv.n_pages) {
+      x.tier = p.kv.tier[x.id];
+      x.layer = p.kv.layer_id[x.id];
+      x.start = p.kv.token_start[x.id];
+    }
+  };
+  open(0);
+  Tile a, b, c;  // two tiles ahead, one ahead, the one that is sent
+  next_ids(c);
+  next_columns(c);
+  next_ids(b);
+  int map_of = -1;
+  const auto landed = [&](int sent) {  // (for a call that gives up: the copies on their way)
+    for (int h = max(0, sent - S::kStages); h < sent; ++h)
+      for (uint32_t k = 0; k < kPollsP && !mbar_try_wait(&sm.bars.full[h % S::kStages], (h / S::kStages) & 1); ++k) {}
+  };
+  for (int n = 0; c.real; ++n) {
+    next_columns(b);
+    next_ids(a);
+    const bool ok = c.wanted && c.tier == 0 && c.layer >= 0 && c.layer < p.kv.n_layers && c.start >= 0 &&
+                    int64_t(c.start) + p.kv.T <= p.kv.pool_tokens;
+    if (c.wanted && !ok) flag(p.lists.status, ASHKV_FLAG_INDEX_RANGE);
+    const uint32_t there = __ballot_sync(0xFFFFFFFFu, ok);  // a bit for each box, in its lower `boxes`
+    TileInfo& t = sm.info[n % kLook];
+    if (n >= kLook && !wait_warp(sm, &sm.bars.info_empty[n % kLook], (n / kLook - 1) & 1)) return landed(2 * n);
+    if (lane < 4) {
+      uint32_t real = 0;
+      if (box >= 32) real = there >> (32 * lane / box) & 1u ? 0xFFFFFFFFu : 0u;
+      else
+        for (int k = 0; k < 32 / box; ++k)
+          if (there >> (32 * lane / box + k) & 1u) real |= ((1u << box) - 1u) << (k * box);
+      t.seen[lane] = c.needed & real;
+    }
+    if (lane == 0) {
+      t.first = c.first;
+      t.edge = c.edge;
+      t.odd = 0;
+    }
+    const int layer = ok ? c.layer : 0, y = ok ? c.start + c.off : end;
+    const uint8_t* map = p.maps + int64_t(layer) * 256;
+    if (layer != map_of) {
+      acquire_map(map);
+      acquire_map(map + 128);
+      map_of = layer;
+    }
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const int h = 2 * n + v, st = h % S::kStages;
+      if (h >= S::kStages && !wait_warp(sm, &sm.bars.empty[st], (h / S::kStages - 1) & 1)) return landed(h);
+      if (lane == 0) mbar_arrive_expect_tx(&sm.bars.full[st], S::kTile);
+      __syncwarp();
+      if (active)
+        tma_load_2d_at(stages + uint32_t(st) * S::kTile + uint32_t(half) * S::kHalf + uint32_t(group * box) * 128, map + v * 128,
+                       &sm.bars.full[st], c.head * D + half * 64, y);
+    }
+    c = b;
+    b = a;
   }
 }
 
-// Looks up the pages of its tiles, describes them in TileInfo and sends their copies on their way: BF16 rows to
-// their places where all pages are, codes to the raw half tiles where pages may be compressed.
-template <int D, bool RAW>
-__device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, int64_t works, int which) {
-  using S = Shape<D, RAW>;
+// Whether V has values that are not finite where some row must not see them, for each of the CTA's tiles in turn.
+template <int D>
+__device__ void check_values(const PromptParams& p, Shared& sm, uint32_t base, int64_t works) {
+  using S = Shape<D, false>;
   const int lane = threadIdx.x & 31;
-  const uint32_t stages = base + 2 * S::kTile, raw = stages + S::kStages * S::kTile;
+  int n = 0;
+  for (int k = 0; work_of(k) < works; ++k) {
+    int head;
+    const Piece pc = load_piece(p, work_of(k), head);
+    for (int i = pc.begin; i < pc.end; ++i, ++n) {
+      const int h = 2 * n + 1, st = h % S::kStages;
+      if (!wait_warp(sm, &sm.bars.full[st], (h / S::kStages) & 1)) return;
+      TileInfo& t = sm.info[n % kLook];
+      if (t.edge) {
+        bool odd = false;
+        const uint32_t at = base + 2 * S::kTile + uint32_t(st) * S::kTile + uint32_t(lane) * 16;
+#pragma unroll 8
+        for (uint32_t x = 0; x < S::kTile; x += 512) odd |= not_finite(lds128(at + x));
+        odd = __any_sync(0xFFFFFFFFu, odd);
+        if (odd && lane == 0) *const_cast<volatile int32_t*>(&t.odd) = 1;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.bars.checked[n % kLook]);
+    }
+  }
+}
+
+// Looks up the pages of its tiles, describes them in TileInfo and sends the codes of their rows on their way.
+template <int D>
+__device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, int64_t works, int which) {
+  using S = Shape<D, true>;
+  const int lane = threadIdx.x & 31;
+  const uint32_t raw = base + 2 * S::kTile + S::kStages * S::kTile;
   int n = 0;  // tiles of the CTA so far
   for (int k = 0; work_of(k) < works; ++k) {
     int head;
     const Piece pc = load_piece(p, work_of(k), head);
-    const int pa = pc.pos0 + pc.row0 / p.group, pb = pc.pos0 + (pc.row0 + pc.rows - 1) / p.group;
     const int32_t* ids = p.lists.page_ids + int64_t(pc.seq) * p.lists.page_ids_stride;
     for (int i = pc.begin; i < pc.end; ++i, ++n) {
       if (n % S::kFetchers != which) continue;
       const int first = tile_of(pc, i) * kTileKeys;
       TileInfo& t = sm.info[n % kLook];
       // four neighbouring tokens a lane; one look-up where they share a page
+      const uint32_t needed = needed_of(p, pc, first + 4 * lane) & 15u;
       Place at[4];
       int tok[4];
-      bool need[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int pos = first + 4 * lane + u;  // (kmax + 127 at most; wrapped: negative)
-        need[u] = pos >= 0 && pos <= pc.kmax && (pos < p.sinks || pos >= pc.lo || !p.window);
-      }
       const bool shared_page = p.kv.T % 4 == 0;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -376,7 +533,7 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
           tok[u] = tok[0] + u;
           continue;
         }
-        const bool any = shared_page ? need[0] || need[1] || need[2] || need[3] : need[u];
+        const bool any = shared_page ? needed != 0 : (needed >> u & 1u) != 0;
         const uint32_t j = pos / uint32_t(p.kv.T);
         tok[u] = int(pos - j * uint32_t(p.kv.T));
         at[u] = Place{-1, nullptr, nullptr};
@@ -384,16 +541,16 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
         if (any && at[u].format < 0) flag(p.lists.status, ASHKV_FLAG_INDEX_RANGE);
       }
       if (n >= kLook && !wait_warp(sm, &sm.bars.info_empty[n % kLook], (n / kLook - 1) & 1)) {
-            cp_async_wait_all();
-            return;
-          }
+        cp_async_wait_all();
+        return;
+      }
       uint32_t bits = 0;
-      int kind = need[0] ? at[0].format : -1;
+      int kind = needed & 1u ? at[0].format : -1;
       bool bf16 = false;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int e = 4 * lane + u;
-        const bool ok = need[u] && at[u].format >= 0;
+        const bool ok = (needed >> u & 1u) && at[u].format >= 0;
         if (ok) bits |= 1u << u;
         if (!ok || at[u].format != kind) kind = kMixed;
         bf16 |= ok && at[u].format == ASHKV_PAGE_BF16;
@@ -409,59 +566,46 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
 #pragma unroll
       for (int off = 1; off < 8; off <<= 1) bits |= __shfl_xor_sync(0xFFFFFFFFu, bits, off);
       if ((lane & 7) == 0) t.seen[lane >> 3] = bits;
-      const int64_t last = int64_t(first) + kTileKeys - 1;
-      const bool edge = !(last <= pa && (!p.window || int64_t(first) > int64_t(pb) - p.window || last < p.sinks));
       if (lane == 0) {
         t.first = first;
-        t.edge = edge;
+        t.edge = edge_of(p, pc, first);
         t.odd = 0;
         t.kind = kind;
       }
       __syncwarp();
 #pragma unroll 1
       for (int v = 0; v < 2; ++v) {
-        const int h = 2 * n + v;
+        constexpr uint32_t L = D / 16, B = 4;  // lanes of a row; passes that wait for their descriptions together
+        const int h = 2 * n + v, slot = h % S::kRaw;
         const uint64_t* rows = v ? t.v : t.k;
-        if constexpr (!RAW) {
-          constexpr uint32_t CPR = D / 8, RPI = 32 / CPR;  // chunks of a row, rows of one instruction
-          const int st = h % S::kStages;
-          const uint32_t to = stages + uint32_t(st) * S::kTile, c = uint32_t(lane) % CPR, r0 = uint32_t(lane) / CPR;
-          if (h >= S::kStages && !wait_warp(sm, &sm.bars.empty[st], (h / S::kStages - 1) & 1)) {
-            cp_async_wait_all();
-            return;
-          }
-#pragma unroll 8
-          for (uint32_t j = 0; j < kTileKeys / RPI; ++j) {
-            const uint32_t r = r0 + RPI * j;
-            cp_async16_zfill(to + chunk_at(r, c), rows[r] + c * 16, (t.meta[r] & 0xFFu) != kNoPage);
-          }
-          if (v && edge) {
-            cp_async_wait_all();
-            bool odd = false;
-            for (uint32_t j = 0; j < kTileKeys / RPI; ++j) odd |= not_finite(lds128(to + chunk_at(r0 + RPI * j, c)));
-            if (odd) *const_cast<volatile int32_t*>(&t.odd) = 1;
-            __syncwarp();
-          }
-          arrive_with_copies(&sm.bars.full[st]);
-          if (lane == 0) mbar_arrive(&sm.bars.full[st]);  // (what the lanes wrote themselves)
-        } else {
-          constexpr uint32_t L = D / 16;  // lanes of a row
-          const int slot = h % S::kRaw;
-          const uint32_t codes = raw + uint32_t(slot) * S::kRawBytes, scales = codes + S::kCodes;
-          if (h >= S::kRaw && !wait_warp(sm, &sm.bars.raw_empty[slot], (h / S::kRaw - 1) & 1)) {
-            cp_async_wait_all();
-            return;
-          }
-#pragma unroll 4
-          for (uint32_t r = uint32_t(lane) / L; r < kTileKeys; r += 32 / L) {
-            const uint32_t meta = t.meta[r], fmt = meta & 0xFFu;
-            if (fmt != kNoPage && fmt != ASHKV_PAGE_BF16)
-              copy_row<D>(p, fmt, reinterpret_cast<const uint8_t*>(rows[r]), (meta >> 8) + (v ? uint32_t(p.kv.T) : 0), uint32_t(head),
-                          codes + r * D, scales + r * 8, uint32_t(lane) % L, L);
-          }
-          arrive_with_copies(&sm.bars.raw_full[slot]);
-          if (lane == 0) mbar_arrive(&sm.bars.raw_full[slot]);
+        const uint32_t codes = raw + uint32_t(slot) * S::kRawBytes, scales = codes + S::kCodes, l = uint32_t(lane) % L;
+        if (h >= S::kRaw && !wait_warp(sm, &sm.bars.raw_empty[slot], (h / S::kRaw - 1) & 1)) {
+          cp_async_wait_all();
+          return;
         }
+#pragma unroll 1
+        for (uint32_t r = uint32_t(lane) / L; r < kTileKeys; r += 32 / L * B) {
+          RowBytes from[B];
+          uint32_t fmt[B];
+#pragma unroll
+          for (uint32_t x = 0; x < B; ++x) {
+            const uint32_t e = r + 32 / L * x, meta = t.meta[e];
+            fmt[x] = meta & 0xFFu;
+            from[x] = row_bytes<D>(p, fmt[x], reinterpret_cast<const uint8_t*>(rows[e]), (meta >> 8) + (v ? uint32_t(p.kv.T) : 0), uint32_t(head));
+            if (fmt[x] == kNoPage || fmt[x] == ASHKV_PAGE_BF16) from[x].bytes = 0;
+          }
+#pragma unroll
+          for (uint32_t x = 0; x < B; ++x) {
+            const uint32_t e = r + 32 / L * x;
+            if (l * 16 < from[x].bytes) cp_async16(codes + e * D + l * 16, from[x].codes + l * 16);
+            if (l == 0 && from[x].bytes) {
+              if (D == 128 && fmt[x] >= ASHKV_PAGE_NBIT4) cp_async_small<8>(scales + e * 8, from[x].scales);
+              else cp_async_small<4>(scales + e * 8, from[x].scales);
+            }
+          }
+        }
+        arrive_with_copies(&sm.bars.raw_full[slot]);
+        if (lane == 0) mbar_arrive(&sm.bars.raw_full[slot]);  // (what the lanes wrote themselves)
       }
     }
   }
@@ -517,39 +661,43 @@ __device__ __forceinline__ void int4_dec16(uint2 c, uint16_t scale, uint4& x, ui
   y = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
-// Unit u (16 channels) of a row: its codes at `codes`, its scales at `scales`, row pr of the page, key head `head`.
+// Unit u (16 channels) of a row: its codes and scale, from shared memory ..
+struct Unit {
+  uint4 codes;
+  uint16_t scale;
+};
 template <int D>
-__device__ __forceinline__ void decode_unit(uint32_t fmt, uint32_t codes, uint32_t scales, uint32_t u, uint32_t pr, uint32_t head, uint4& x,
-                                            uint4& y) {
-  const auto half = [&](uint32_t at) {
-    uint16_t s;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(s) : "r"(at));
-    return s;
-  };
-  const auto two = [&](uint32_t at) {
-    uint2 c;
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(c.x), "=r"(c.y) : "r"(at));
-    return c;
-  };
-  if (fmt == ASHKV_PAGE_INT8) {
-    int8_dec16(lds128(codes + 16 * u), f16_to_f32(half(scales + (pr & 1u) * 2)), x, y);
-  } else if (fmt == ASHKV_PAGE_FP8) {
-    const uint4 c = lds128(codes + 16 * u);
-    x = fp8_dec8(make_uint2(c.x, c.y));
-    y = fp8_dec8(make_uint2(c.z, c.w));
-  } else if (fmt == ASHKV_PAGE_INT4) {
-    int4_dec16(two(codes + 8 * u), half(scales + (D == 128 ? u / 4 : head & 1u) * 2), x, y);
-  } else if (fmt == ASHKV_PAGE_NBIT4) {
-    const uint2 c = two(codes + 8 * u);
-    const uint16_t d = half(scales + u / 2 * 2);
-    x = nbit_dec8<4>(c.x, d);
-    y = nbit_dec8<4>(c.y, d);
+__device__ __forceinline__ Unit load_unit(uint32_t fmt, uint32_t codes, uint32_t scales, uint32_t u, uint32_t pr, uint32_t head) {
+  Unit x;
+  uint32_t at = scales;
+  if (fmt == ASHKV_PAGE_INT8 || fmt == ASHKV_PAGE_FP8) {
+    x.codes = lds128(codes + 16 * u);
+    at += (pr & 1u) * 2;
+  } else if (fmt == ASHKV_PAGE_INT4 || fmt == ASHKV_PAGE_NBIT4) {
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x.codes.x), "=r"(x.codes.y) : "r"(codes + 8 * u));
+    at += fmt == ASHKV_PAGE_INT4 ? (D == 128 ? u / 4 : head & 1u) * 2 : u / 2 * 2;
   } else {
-    uint32_t c;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(c) : "r"(codes + 4 * u));
-    const uint16_t d = half(scales + u / 2 * 2);
-    x = nbit_dec8<2>(c & 0xFFFFu, d);
-    y = nbit_dec8<2>(c >> 16, d);
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x.codes.x) : "r"(codes + 4 * u));
+    at += u / 2 * 2;
+  }
+  if (fmt != ASHKV_PAGE_FP8) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x.scale) : "r"(at));
+  return x;
+}
+// .. and its values.
+__device__ __forceinline__ void decode_unit(uint32_t fmt, const Unit& n, uint4& x, uint4& y) {
+  if (fmt == ASHKV_PAGE_INT8) {
+    int8_dec16(n.codes, f16_to_f32(n.scale), x, y);
+  } else if (fmt == ASHKV_PAGE_FP8) {
+    x = fp8_dec8(make_uint2(n.codes.x, n.codes.y));
+    y = fp8_dec8(make_uint2(n.codes.z, n.codes.w));
+  } else if (fmt == ASHKV_PAGE_INT4) {
+    int4_dec16(make_uint2(n.codes.x, n.codes.y), n.scale, x, y);
+  } else if (fmt == ASHKV_PAGE_NBIT4) {
+    x = nbit_dec8<4>(n.codes.x, n.scale);
+    y = nbit_dec8<4>(n.codes.y, n.scale);
+  } else {
+    x = nbit_dec8<2>(n.codes.x & 0xFFFFu, n.scale);
+    y = nbit_dec8<2>(n.codes.x >> 16, n.scale);
   }
 }
 
@@ -645,12 +793,21 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
         const auto page_row = [&](uint32_t r) { return (t.meta[r] >> 8) + (v ? T : 0u); };
         const auto all_rows = [&](auto format) {
           constexpr uint32_t F = decltype(format)::value;
-#pragma unroll 4
-          for (uint32_t j = 0; j < kPasses; ++j) {
-            const uint32_t r = r0 + kStep * j;
-            uint4 x, y;
-            decode_unit<D>(F, codes + r * D, scales + r * 8, u, F == ASHKV_PAGE_INT8 ? page_row(r) : 0u, uint32_t(head), x, y);
-            put(r, x, y);
+          constexpr uint32_t B = 4;  // units that are on their way from shared memory together
+#pragma unroll 1
+          for (uint32_t j = 0; j < kPasses; j += B) {
+            Unit n[B];
+#pragma unroll
+            for (uint32_t b = 0; b < B; ++b) {
+              const uint32_t r = r0 + kStep * (j + b);
+              n[b] = load_unit<D>(F, codes + r * D, scales + r * 8, u, F == ASHKV_PAGE_INT8 ? page_row(r) : 0u, uint32_t(head));
+            }
+#pragma unroll
+            for (uint32_t b = 0; b < B; ++b) {
+              uint4 x, y;
+              decode_unit(F, n[b], x, y);
+              put(r0 + kStep * (j + b), x, y);
+            }
           }
         };
         if (kind == ASHKV_PAGE_INT8) {
@@ -666,7 +823,7 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
             const uint32_t r = r0 + kStep * j, fmt = t.meta[r] & 0xFFu;
             if (fmt == ASHKV_PAGE_BF16) continue;
             uint4 x = make_uint4(0, 0, 0, 0), y = x;
-            if (fmt != kNoPage) decode_unit<D>(fmt, codes + r * D, scales + r * 8, u, page_row(r), uint32_t(head), x, y);
+            if (fmt != kNoPage) decode_unit(fmt, load_unit<D>(fmt, codes + r * D, scales + r * 8, u, page_row(r), uint32_t(head)), x, y);
             dithered |= fmt != kNoPage && fmt >= ASHKV_PAGE_NBIT4;
             put(r, x, y);
           }
@@ -800,17 +957,16 @@ __device__ void issue_products(const PromptParams& p, Shared& sm, uint32_t base,
         if (i > 0) {
           if (g == 0) {
             if (!(ok = wait_warp(sm, &sm.bars.full[sv], (hv / S::kStages) & 1))) break;
+            if (!RAW && !(ok = wait_warp(sm, &sm.bars.checked[(n + i - 1) % kLook], ((n + i - 1) / kLook) & 1))) break;
             odd = __any_sync(0xFFFFFFFFu, *const_cast<volatile int32_t*>(&sm.info[(n + i - 1) % kLook].odd));
           }
           if (!(ok = wait_warp(sm, &sm.bars.p_ready[g], ready[g]++ & 1))) break;
-          fence_proxy_async_smem();  // (copies that landed without a thread to fence them)
           tc_fence_after();
           if (!odd) values(g, sv, i > 1);
           if (i == tiles) commit(&sm.bars.s_full[g]);
         }
         if (i < tiles) {
           if (g == 0 && !(ok = wait_warp(sm, &sm.bars.full[sk], (hk / S::kStages) & 1))) break;
-          fence_proxy_async_smem();
           tc_fence_after();
           scores(g, sk);
         }
@@ -831,7 +987,6 @@ __device__ void issue_products(const PromptParams& p, Shared& sm, uint32_t base,
 
 // ---- softmax: a warpgroup to a tile, a thread to a row
 // The tokens of 32 from first on that a query at first + ahead sees.
-__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 __device__ __forceinline__ uint32_t seen_by(const PromptParams& p, int first, int ahead) {
   uint32_t m = low_bits(ahead + 1);
   if (p.window) m &= ~low_bits(ahead + 1 - p.window) | low_bits(p.sinks - first);
@@ -970,7 +1125,8 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
       bool odd = false;
       if (edge) {  // does V hold values that some rows must not see?
         const int hv = 2 * n + 1;
-        if (!wait_warp(sm, &sm.bars.full[hv % S::kStages], (hv / S::kStages) & 1)) return;
+        uint64_t* known = RAW ? &sm.bars.full[hv % S::kStages] : &sm.bars.checked[n % kLook];
+        if (!wait_warp(sm, known, (RAW ? hv / S::kStages : n / kLook) & 1)) return;
         odd = *const_cast<const volatile int32_t*>(&t.odd);
       }
       if (odd) {
@@ -1078,9 +1234,8 @@ __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.
 template <int N>
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
 
-// 512 threads of 128 registers at launch; 176 for the softmax warpgroups, 80 for the others (together as many).
 template <int D, bool RAW>
-__global__ void __launch_bounds__(kThreadsP, 1) prompt_kernel(const __grid_constant__ PromptParams p) {
+__global__ void __launch_bounds__(Shape<D, RAW>::kThreads, 1) prompt_kernel(const __grid_constant__ PromptParams p) {
   extern __shared__ uint8_t smem[];
   __shared__ Shared sm;
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);
@@ -1090,18 +1245,18 @@ __global__ void __launch_bounds__(kThreadsP, 1) prompt_kernel(const __grid_const
     mbar_init(&b.q_full, 32);
     mbar_init(&b.q_empty, 1);
     for (int i = 0; i < 8; ++i) {
-      mbar_init(&b.full[i], RAW ? kDecoders : 33);  // (the lanes' copies, and what they wrote)
+      mbar_init(&b.full[i], RAW ? kDecoders : 1);
       mbar_init(&b.empty[i], 1);
-      mbar_init(&b.raw_full[i], 33);
+      mbar_init(&b.raw_full[i], 33);  // (the lanes' copies, and what they wrote)
       mbar_init(&b.raw_empty[i], kDecoders / 32);
     }
-    for (int i = 0; i < kLook; ++i) mbar_init(&b.info_empty[i], 1);
+    for (int i = 0; i < kLook; ++i) { mbar_init(&b.info_empty[i], 1); mbar_init(&b.checked[i], 1); }
     for (int g = 0; g < 2; ++g) { mbar_init(&b.s_full[g], 1); mbar_init(&b.p_ready[g], 4); }
     mbar_init(&b.drained, 1);
     mbar_init_fence();
     sm.failed = 0;
   }
-  if (warp == 12) tmem_alloc(&sm.tmem, 512);
+  if (warp == 8) tmem_alloc(&sm.tmem, 512);
   tc_fence_before();
   wait_for_previous();
   __syncthreads();
@@ -1109,17 +1264,19 @@ __global__ void __launch_bounds__(kThreadsP, 1) prompt_kernel(const __grid_const
   allow_next();
   const int64_t works = int64_t(*const_cast<const volatile int32_t*>(p.counts)) * p.kv.heads_kv;
   if (warp < 8) {
-    more_registers<176>();
+    more_registers<Shape<D, RAW>::kSoftmaxRegs>();
     softmax_rows<D, RAW>(p, sm, base, works, warp >> 2);
   } else {
-    fewer_registers<80>();
-    if (warp == 12) issue_products<D, RAW>(p, sm, base, works);
-    else if (warp == 13) load_queries<D, RAW>(p, sm, base, works);
+    fewer_registers<Shape<D, RAW>::kOtherRegs>();
+    if (warp == 8) issue_products<D, RAW>(p, sm, base, works);
+    else if (warp == 9) load_queries<D, RAW>(p, sm, base, works);
     else if constexpr (RAW) {
-      if (warp < 12) decode_tiles<D>(p, sm, base, works);
-      else fetch_tiles<D, RAW>(p, sm, base, works, warp - 14);
-    } else if (warp < 12) {
-      fetch_tiles<D, RAW>(p, sm, base, works, warp - 8);
+      if (warp < 12) fetch_tiles<D>(p, sm, base, works, warp - 10);
+      else decode_tiles<D>(p, sm, base, works);
+    } else if (warp == 10) {
+      fetch_boxes<D>(p, sm, base, works);
+    } else {
+      check_values<D>(p, sm, base, works);
     }
   }
   __syncwarp();
@@ -1127,7 +1284,7 @@ __global__ void __launch_bounds__(kThreadsP, 1) prompt_kernel(const __grid_const
   __syncthreads();
   tc_fence_after();
   if (threadIdx.x == 0 && sm.failed) flag(p.lists.status, ASHKV_FLAG_TIMEOUT);
-  if (warp == 12) {
+  if (warp == 8) {
     tmem_dealloc(sm.tmem, 512);
     tmem_relinquish();
   }
@@ -1192,12 +1349,15 @@ __global__ void __launch_bounds__(kJoinThreadsP) prompt_join_kernel(const __grid
 // Key tiles of a piece at least, and pieces to aim for.
 constexpr int kLeastTiles = 4;
 struct Sizes {
-  int64_t items, pieces, parts, part_rows, prefix;
+  int64_t items, pieces, parts, part_rows, prefix, maps;
   int share;
+  // [counts][prefix][pieces][splits], then [maps] and [partial results] on lines of 128 bytes
   int64_t ints() const { return 8 + (prefix + 3) / 4 * 4 + pieces * int64_t(sizeof(Piece) / 4) + parts * int64_t(sizeof(Split) / 4); }
-  int64_t floats(int heads_kv, int D) const { return (ints() + 31) / 32 * 32 + parts * heads_kv * part_rows * (int64_t(D) + 1) + 32; }
+  int64_t floats(int heads_kv, int D) const {
+    return (ints() + 31) / 32 * 32 + 32 * maps + parts * heads_kv * part_rows * (int64_t(D) + 1) + 64;
+  }
 };
-Sizes sizes_of(int64_t n_rows, int64_t n_seqs, int heads_q, int heads_kv) {
+Sizes sizes_of(int64_t n_rows, int64_t n_seqs, int heads_q, int heads_kv, int n_layers) {
   Sizes s;
   const int sms = sm_count() > 0 ? sm_count() : 148, group = heads_q / heads_kv;
   s.items = n_rows * group / kItemRows + n_seqs;
@@ -1207,11 +1367,22 @@ Sizes sizes_of(int64_t n_rows, int64_t n_seqs, int heads_q, int heads_kv) {
   s.parts = std::min<int64_t>(2 * int64_t(s.share) / heads_kv + 2, 2 * int64_t(s.share) + 2);
   s.pieces = s.items + s.parts;
   s.prefix = n_seqs + 1;
+  s.maps = 2 * int64_t(n_layers);
   return s;
 }
 
+// A map of a layer's pool [pool_tokens, row_len], boxes of `rows` x 64, but for its address (`any`: an aligned one).
+bool pool_map(CUtensorMap& map, void* any, const PagedKV& kv, int rows) {
+  auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
+  if (!fn) return false;
+  cuuint64_t dims[2] = {cuuint64_t(kv.row_len), cuuint64_t(kv.pool_tokens)}, strides[1] = {cuuint64_t(kv.row_stride) * 2};
+  cuuint32_t box[2] = {64, cuuint32_t(rows)}, steps[2] = {1, 1};
+  return fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, any, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, bool RAW>
-ashkv_status_t launch_prompt(const PromptParams& p, int sms, void* stream) {
+ashkv_status_t launch_prompt(const PromptParams& p, const CUtensorMap& pool, int sms, void* stream) {
   constexpr const char* kName = "ashkv_prompt_attention";
   // the attribute is the kernel's on a device and outlasts the call
   static std::atomic<bool> allowed[64];
@@ -1225,8 +1396,8 @@ ashkv_status_t launch_prompt(const PromptParams& p, int sms, void* stream) {
     set_error("ashkv_prompt_attention (shared memory attribute)", e);
     return ASHKV_LAUNCH_ERROR;
   }
-  launch_paged(prompt_plan_kernel, 1, kPlanThreads, 0, stream, p, kLeastTiles);
-  launch_paged(prompt_kernel<D, RAW>, sms, kThreadsP, Shape<D, RAW>::kBytes, stream, p);
+  launch_paged(prompt_plan_kernel, 1, kPlanThreads, 0, stream, p, pool, kLeastTiles);
+  launch_paged(prompt_kernel<D, RAW>, sms, Shape<D, RAW>::kThreads, Shape<D, RAW>::kBytes, stream, p);
   const ashkv_status_t rc = check_launch(kName);
   if (rc != ASHKV_OK) return rc;
   launch_paged(prompt_join_kernel<D>, 4 * sms, kJoinThreadsP, 0, stream, p);
@@ -1239,9 +1410,9 @@ ashkv_status_t launch_prompt(const PromptParams& p, int sms, void* stream) {
 using namespace ashkv;
 
 extern "C" int64_t ashkv_prompt_scratch_floats(int64_t n_rows, int32_t n_seqs, int32_t heads_q, int32_t heads_kv,
-                                               int32_t head_dim) {
-  if (n_rows < 0 || n_seqs < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv || head_dim <= 0) return -1;
-  return sizes_of(n_rows, n_seqs, heads_q, heads_kv).floats(heads_kv, head_dim);
+                                               int32_t head_dim, int32_t n_layers) {
+  if (n_rows < 0 || n_seqs < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv || head_dim <= 0 || n_layers <= 0) return -1;
+  return sizes_of(n_rows, n_seqs, heads_q, heads_kv, n_layers).floats(heads_kv, head_dim);
 }
 
 extern "C" ashkv_status_t ashkv_prompt_attention(
@@ -1269,17 +1440,27 @@ extern "C" ashkv_status_t ashkv_prompt_attention(
   if (p.scale2 == 0.0f) p.scale2 = 0x1p-126f;  // (a score of -infinity stays one)
   p.window = window; p.sinks = sinks;
   p.out = static_cast<uint16_t*>(d_out); p.lse = d_lse;
-  const Sizes s = sizes_of(n_rows, n_seqs, heads_q, p.kv.heads_kv);
+  const Sizes s = sizes_of(n_rows, n_seqs, heads_q, p.kv.heads_kv, p.kv.n_layers);
   p.counts = reinterpret_cast<int32_t*>(d_scratch);
   p.prefix = p.counts + 8;
   p.pieces = reinterpret_cast<Piece*>(p.prefix + (s.prefix + 3) / 4 * 4);
   p.splits = reinterpret_cast<Split*>(p.pieces + s.pieces);
   p.max_pieces = int32_t(s.pieces); p.max_parts = int32_t(s.parts); p.share = s.share; p.part_rows = int32_t(s.part_rows);
-  p.part_o = d_scratch + (s.ints() + 31) / 32 * 32;
+  // (the scratch is aligned to 16 bytes, maps to 128)
+  p.maps = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(d_scratch + s.ints()) + 127) & ~uintptr_t(127));
+  p.part_o = reinterpret_cast<float*>(p.maps) + 32 * s.maps;
   p.part_lse2 = p.part_o + s.parts * p.kv.heads_kv * s.part_rows * kv->head_dim;
   bool stores = false;
   for (int t = 1; t < kTiers; ++t) stores |= p.kv.store[t].format != ASHKV_PAGE_NONE;
   const int sms = sm_count() > 0 ? sm_count() : 148;
-  if (kv->head_dim == 64) return stores ? launch_prompt<64, true>(p, sms, stream) : launch_prompt<64, false>(p, sms, stream);
-  return stores ? launch_prompt<128, true>(p, sms, stream) : launch_prompt<128, false>(p, sms, stream);
+  // Tensor copies where every page is in the pool and a box of eight rows or more, which a swizzled tile can take, never
+  // crosses a page.  The whole prompt of 8192 tokens, 32 / 8 heads of 128: see the numbers at the kernel.
+  CUtensorMap pool{};
+  if (!stores && p.kv.T % 8 == 0 && p.kv.pool_tokens > 0 && p.kv.pool_tokens < 0x7FFFFFFF) {
+    p.box_rows = 8;
+    while (p.box_rows < kTileKeys && p.kv.T % (2 * p.box_rows) == 0) p.box_rows *= 2;
+    if (!pool_map(pool, d_scratch, p.kv, p.box_rows)) p.box_rows = 0;
+  }
+  if (kv->head_dim == 64) return p.box_rows ? launch_prompt<64, false>(p, pool, sms, stream) : launch_prompt<64, true>(p, pool, sms, stream);
+  return p.box_rows ? launch_prompt<128, false>(p, pool, sms, stream) : launch_prompt<128, true>(p, pool, sms, stream);
 }

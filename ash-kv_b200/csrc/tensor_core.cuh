@@ -78,6 +78,14 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
   return one != 0;
 }
+// Maps for tensor copies in global memory: the base address of a copy of a map is set by the device, and read by copies after a fence.
+__device__ __forceinline__ void set_map_address(void* map, uint64_t address) {
+  asm volatile("tensormap.replace.tile.global_address.global.b1024.b64 [%0], %1;" :: "l"(map), "l"(address) : "memory");
+}
+__device__ __forceinline__ void release_map() { asm volatile("fence.proxy.tensormap::generic.release.gpu;" ::: "memory"); }
+__device__ __forceinline__ void acquire_map(const void* map) {
+  asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" :: "l"(map) : "memory");
+}
 // 32 columns of the warp's lanes.
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"

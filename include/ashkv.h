@@ -628,7 +628,7 @@ ASHKV_API ashkv_status_t ashkv_read_kv(const ashkv_paged_kv_t* kv, const int32_t
  * by this call alone until it has run.
  * ======================================================================== */
 ASHKV_API int64_t ashkv_prompt_scratch_floats(int64_t n_rows, int32_t n_seqs, int32_t heads_q, int32_t heads_kv,
-                                              int32_t head_dim);
+                                              int32_t head_dim, int32_t n_layers);
 ASHKV_API ashkv_status_t ashkv_prompt_attention(
     const ashkv_paged_kv_t* kv, const void* d_q, int64_t q_row_stride, int64_t q_head_stride, int64_t n_rows,
     int32_t heads_q, const int32_t* d_page_ids, int64_t page_ids_stride, int32_t max_pages, const int32_t* d_lengths,
