@@ -54,8 +54,21 @@ struct __align__(16) Split {  // an item cut into pieces
   int32_t row0, rows, first, part, parts, pad[3];
 };
 
+// Quotients of numbers below 2^31 by a divisor of the call: n * m >> 31 + l with m = floor(2^(31 + l) / d) + 1, l = ceil(log2
+// d) (Granlund and Montgomery).
+struct Quotient {
+  uint32_t m, s;
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return uint32_t((uint64_t(n) * m) >> 31 >> s); }
+};
+Quotient quotient(uint32_t d) {
+  uint32_t l = 0;
+  while ((uint64_t(1) << l) < d) ++l;
+  return Quotient{uint32_t((uint64_t(1) << (31 + l)) / d + 1), l};
+}
+
 struct PromptParams {
   PagedKV kv;
+  Quotient by_page;  // by tokens_per_page
   PageLists lists;
   const uint16_t* q;
   int64_t q_row, q_head;
@@ -295,7 +308,7 @@ __device__ __forceinline__ bool wait_p(Shared& sm, uint64_t* bar, uint32_t parit
 }
 
 __device__ __forceinline__ bool wait_warp(Shared& sm, uint64_t* bar, uint32_t parity) {  // all lanes, with one answer
-  return __all_sync(0xFFFFFFFFu, wait_p(sm, bar, parity));
+  return __all_sync(0xFFFFFFFFu, wait_p(sm, bar, parity));  // (one lane asking for its warp measured 1.7 times as slow)
 }
 
 // The works of a CTA: piece w / heads_kv for key head w % heads_kv; neighbours in turn, there and back, so that
@@ -365,22 +378,21 @@ __device__ __forceinline__ uint32_t needed_of(const PromptParams& p, const Piece
   if (p.window) m &= ~low_bits(pc.lo - first) | low_bits(p.sinks - first);
   return m;
 }
-// Whether some row of a piece does not see some token of the tile from `first` on.
-__device__ __forceinline__ bool edge_of(const PromptParams& p, const Piece& pc, int first) {
-  const int64_t pa = int64_t(pc.pos0) + pc.row0 / p.group, pb = int64_t(pc.pos0) + (pc.row0 + pc.rows - 1) / p.group;
+// Whether some row of a piece, whose rows are at pa .. pb, does not see some token of the tile from `first` on.
+__device__ __forceinline__ bool edge_of(const PromptParams& p, int64_t pa, int64_t pb, int first) {
   const int64_t last = int64_t(first) + kTileKeys - 1;
   return !(last <= pa && (!p.window || first > pb - p.window || last < p.sinks));
 }
 
-// All pages in the pool, of a multiple of eight tokens: tensor copies of boxes of 64 channels.  A lane a box; what
+// All pages in the pool, of a multiple of eight tokens: tensor copies of boxes of 64 channels.  A lane a box's rows; what
 // it has to look up is on its way while the tiles before are sent: the page ids of the tile after next, the table's
 // columns of the next.  Boxes that nobody needs, or whose page does not exist, come from behind the pool's end: zeros.
 template <int D>
 __device__ void fetch_boxes(const PromptParams& p, Shared& sm, uint32_t base, int64_t works) {
   using S = Shape<D, false>;
   const int lane = threadIdx.x & 31;
-  const int box = p.box_rows, boxes = kTileKeys / box, group = lane % boxes, half = lane / boxes;  // (of 64 channels)
-  const bool active = half < D / 64;
+  const int box = p.box_rows, boxes = kTileKeys / box, group = lane;
+  const bool active = lane < boxes;
   const uint32_t stages = base + 2 * S::kTile;
   const int end = int(p.kv.pool_tokens);
   struct Tile {
@@ -389,7 +401,7 @@ __device__ void fetch_boxes(const PromptParams& p, Shared& sm, uint32_t base, in
     bool real, edge, wanted;
   };
   // a walk over the CTA's tiles
-  int wk = 0, wi = 0, whead = 0;
+  int wk = 0, wi = 0, whead = 0, wa = 0, wb = 0;
   Piece wp{};
   bool more = true;
   const auto open = [&](int k) {
@@ -398,6 +410,8 @@ __device__ void fetch_boxes(const PromptParams& p, Shared& sm, uint32_t base, in
       if (!more) return;
       wp = load_piece(p, work_of(wk), whead);
       wi = wp.begin;
+      wa = wp.pos0 + wp.row0 / p.group;
+      wb = wp.pos0 + (wp.row0 + wp.rows - 1) / p.group;
       if (wi < wp.end) return;
     }
   };
@@ -407,8 +421,8 @@ __device__ void fetch_boxes(const PromptParams& p, Shared& sm, uint32_t base, in
     x.first = tile_of(wp, wi) * kTileKeys;
     x.head = whead;
     x.needed = lane < 4 ? needed_of(p, wp, x.first + 32 * lane) : 0u;
-    x.edge = edge_of(p, wp, x.first);
-    const uint32_t pos = uint32_t(x.first + group * box), j = pos / uint32_t(p.kv.T);
+    x.edge = edge_of(p, wa, wb, x.first);
+    const uint32_t pos = uint32_t(x.first + group * box), j = p.by_page.of(pos);
     x.off = int(pos - j * uint32_t(p.kv.T));
     const int last = int(pos) + box - 1;
     x.wanted = active && int(pos) >= 0 && int(pos) <= wp.kmax && (!p.window || last >= wp.lo || int(pos) < p.sinks);
@@ -440,7 +454,7 @@ __device__ void fetch_boxes(const PromptParams& p, Shared& sm, uint32_t base, in
     const bool ok = c.wanted && c.tier == 0 && c.layer >= 0 && c.layer < p.kv.n_layers && c.start >= 0 &&
                     int64_t(c.start) + p.kv.T <= p.kv.pool_tokens;
     if (c.wanted && !ok) flag(p.lists.status, ASHKV_FLAG_INDEX_RANGE);
-    const uint32_t there = __ballot_sync(0xFFFFFFFFu, ok);  // a bit for each box, in its lower `boxes`
+    const uint32_t there = __ballot_sync(0xFFFFFFFFu, ok);  // a bit for each box
     TileInfo& t = sm.info[n % kLook];
     if (n >= kLook && !wait_warp(sm, &sm.bars.info_empty[n % kLook], (n / kLook - 1) & 1)) return landed(2 * n);
     if (lane < 4) {
@@ -457,10 +471,9 @@ __device__ void fetch_boxes(const PromptParams& p, Shared& sm, uint32_t base, in
       t.odd = 0;
     }
     const int layer = ok ? c.layer : 0, y = ok ? c.start + c.off : end;
-    const uint8_t* map = p.maps + int64_t(layer) * 256;
     if (layer != map_of) {
-      acquire_map(map);
-      acquire_map(map + 128);
+      acquire_map(p.maps + int64_t(layer) * 256);
+      acquire_map(p.maps + int64_t(layer) * 256 + 128);
       map_of = layer;
     }
 #pragma unroll
@@ -469,9 +482,19 @@ __device__ void fetch_boxes(const PromptParams& p, Shared& sm, uint32_t base, in
       if (h >= S::kStages && !wait_warp(sm, &sm.bars.empty[st], (h / S::kStages - 1) & 1)) return landed(h);
       if (lane == 0) mbar_arrive_expect_tx(&sm.bars.full[st], S::kTile);
       __syncwarp();
-      if (active)
-        tma_load_2d_at(stages + uint32_t(st) * S::kTile + uint32_t(half) * S::kHalf + uint32_t(group * box) * 128, map + v * 128,
-                       &sm.bars.full[st], c.head * D + half * 64, y);
+      const uint32_t to = stages + uint32_t(st) * S::kTile;
+#pragma unroll 4
+      for (int g = 0; g < boxes; ++g) {  // (one lane, uniform operands: a copy a lane took three times as long to issue)
+        const int64_t at = __shfl_sync(0xFFFFFFFFu, layer, g);
+        const int row = __shfl_sync(0xFFFFFFFFu, y, g), x = __shfl_sync(0xFFFFFFFFu, c.head, 0) * D;
+        if (elect_one()) {
+#pragma unroll
+          for (int half = 0; half < D / 64; ++half)
+            tma_load_2d_at(to + uint32_t(half) * S::kHalf + uint32_t(g * box) * 128, p.maps + at * 256 + v * 128, &sm.bars.full[st],
+                           x + half * 64, row);
+        }
+        __syncwarp();
+      }
     }
     c = b;
     b = a;
@@ -516,6 +539,7 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
     int head;
     const Piece pc = load_piece(p, work_of(k), head);
     const int32_t* ids = p.lists.page_ids + int64_t(pc.seq) * p.lists.page_ids_stride;
+    const int pa = pc.pos0 + pc.row0 / p.group, pb = pc.pos0 + (pc.row0 + pc.rows - 1) / p.group;
     for (int i = pc.begin; i < pc.end; ++i, ++n) {
       if (n % S::kFetchers != which) continue;
       const int first = tile_of(pc, i) * kTileKeys;
@@ -534,7 +558,7 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
           continue;
         }
         const bool any = shared_page ? needed != 0 : (needed >> u & 1u) != 0;
-        const uint32_t j = pos / uint32_t(p.kv.T);
+        const uint32_t j = p.by_page.of(pos);
         tok[u] = int(pos - j * uint32_t(p.kv.T));
         at[u] = Place{-1, nullptr, nullptr};
         if (any) at[u] = place_of(p.kv, ids[j]);
@@ -568,7 +592,7 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
       if ((lane & 7) == 0) t.seen[lane >> 3] = bits;
       if (lane == 0) {
         t.first = first;
-        t.edge = edge_of(p, pc, first);
+        t.edge = edge_of(p, pa, pb, first);
         t.odd = 0;
         t.kind = kind;
       }
@@ -947,26 +971,27 @@ __device__ void issue_products(const PromptParams& p, Shared& sm, uint32_t base,
     const int two = __shfl_sync(0xFFFFFFFFu, pc.rows > kTileRows ? 2 : 1, 0);
     if (tiles <= 0) continue;
     if (!(ok = wait_warp(sm, &sm.bars.q_full, items++ & 1))) break;
-    bool odd = false;
     for (int i = 0; ok && i <= tiles; ++i) {
       const int hk = 2 * (n + i), hv = hk - 1;  // K of tile i, V of the one before
       const uint32_t sk = uint32_t(hk) % S::kStages, sv = uint32_t(hv) % S::kStages;
+      // (keys and values first: they are mostly there, and the weights are what the products wait for)
+      bool odd = false;
+      if (i > 0) {
+        if (!(ok = wait_warp(sm, &sm.bars.full[sv], (hv / S::kStages) & 1))) break;
+        if (!RAW && !(ok = wait_warp(sm, &sm.bars.checked[(n + i - 1) % kLook], ((n + i - 1) / kLook) & 1))) break;
+        odd = __any_sync(0xFFFFFFFFu, *const_cast<volatile int32_t*>(&sm.info[(n + i - 1) % kLook].odd));
+      }
+      if (i < tiles && !(ok = wait_warp(sm, &sm.bars.full[sk], (hk / S::kStages) & 1))) break;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         if (g == two) break;
         if (i > 0) {
-          if (g == 0) {
-            if (!(ok = wait_warp(sm, &sm.bars.full[sv], (hv / S::kStages) & 1))) break;
-            if (!RAW && !(ok = wait_warp(sm, &sm.bars.checked[(n + i - 1) % kLook], ((n + i - 1) / kLook) & 1))) break;
-            odd = __any_sync(0xFFFFFFFFu, *const_cast<volatile int32_t*>(&sm.info[(n + i - 1) % kLook].odd));
-          }
           if (!(ok = wait_warp(sm, &sm.bars.p_ready[g], ready[g]++ & 1))) break;
           tc_fence_after();
           if (!odd) values(g, sv, i > 1);
           if (i == tiles) commit(&sm.bars.s_full[g]);
         }
         if (i < tiles) {
-          if (g == 0 && !(ok = wait_warp(sm, &sm.bars.full[sk], (hk / S::kStages) & 1))) break;
           tc_fence_after();
           scores(g, sk);
         }
@@ -1439,6 +1464,7 @@ extern "C" ashkv_status_t ashkv_prompt_attention(
   p.scale2 = (scale < 0.0f ? -scale : scale) * kLog2eP;
   if (p.scale2 == 0.0f) p.scale2 = 0x1p-126f;  // (a score of -infinity stays one)
   p.window = window; p.sinks = sinks;
+  p.by_page = quotient(uint32_t(p.kv.T));
   p.out = static_cast<uint16_t*>(d_out); p.lse = d_lse;
   const Sizes s = sizes_of(n_rows, n_seqs, heads_q, p.kv.heads_kv, p.kv.n_layers);
   p.counts = reinterpret_cast<int32_t*>(d_scratch);
