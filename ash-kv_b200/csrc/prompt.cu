@@ -279,8 +279,9 @@ struct Shape {
 };
 
 struct __align__(16) TileInfo {
-  uint64_t k[kTileKeys], v[kTileKeys];  // BF16 rows: of the head's first channel; else the slot
-  uint32_t meta[kTileKeys];             // format | token in its page << 8
+  uint64_t row[2][kTileKeys];           // (K, V) the head's channels: BF16 values or codes
+  uint32_t scale[2][kTileKeys];         // the word of the row's scales, so many bytes before its codes
+  uint32_t meta[kTileKeys];             // format | chunks of 16 bytes of its codes << 8 | token in its page << 16
   uint32_t seen[4];                     // a bit for each token that exists
   int32_t first;                        // position of the tile's first token
   int32_t edge;                         // some row does not see some token of the tile
@@ -356,19 +357,29 @@ __device__ __forceinline__ void tma_load_2d_at(uint32_t to, const void* map, uin
       :: "r"(to), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
 }
 
-// Where the codes and scales of a row (row pr of a compressed page, key head `head`) are, and the bytes of its codes.
+// Where the codes of a row (row pr of a compressed page at s, key head `head`) are, and how far before them the word (of
+// dithered pages: the eight bytes, with D = 128) of its scales.
 struct RowBytes {
-  const uint8_t *codes, *scales;
-  uint32_t bytes;
+  const uint8_t* codes;
+  uint32_t scale;
 };
 template <int D>
-__device__ __forceinline__ RowBytes row_bytes(const PromptParams& p, uint32_t fmt, const uint8_t* s, uint32_t pr, uint32_t head) {
-  const uint32_t T = uint32_t(p.kv.T), row = uint32_t(p.kv.row_len), E = 2 * T * row, e = pr * row + head * D;
-  if (fmt == ASHKV_PAGE_INT8) return {s + uint32_t(int8_codes_offset(int(T))) + e, s + (2 * pr & ~3u), D};
-  if (fmt == ASHKV_PAGE_FP8) return {s + e, s + e, D};
-  if (fmt == ASHKV_PAGE_INT4) return {s + E / 32 + e / 2, s + (e / 64 * 2 & ~3u), D / 2};
-  const uint32_t bits = fmt == ASHKV_PAGE_NBIT4 ? 4 : 2;
-  return {s + nbit_codes_off(E) + e * bits / 8, s + nbit_delta_off() + e / 32 * 2, D * bits / 8};
+__device__ __forceinline__ RowBytes row_bytes(uint32_t fmt, const uint8_t* s, uint32_t T, uint32_t row, uint32_t pr, uint32_t head) {
+  const uint32_t E = 2 * T * row, e = pr * row + head * D;
+  uint32_t codes, scale;
+  if (fmt == ASHKV_PAGE_INT8) {
+    codes = uint32_t(int8_codes_offset(int(T))) + e;
+    scale = 2 * pr & ~3u;
+  } else if (fmt == ASHKV_PAGE_FP8) {
+    codes = scale = e;
+  } else if (fmt == ASHKV_PAGE_INT4) {
+    codes = E / 32 + e / 2;
+    scale = e / 64 * 2 & ~3u;
+  } else {
+    codes = uint32_t(nbit_codes_off(E)) + (fmt == ASHKV_PAGE_NBIT4 ? e / 2 : e / 4);
+    scale = uint32_t(nbit_delta_off()) + e / 32 * 2;
+  }
+  return {s + codes, codes - scale};
 }
 
 // The tokens of 32 from first on that some row of a piece sees.
@@ -578,11 +589,21 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
         if (ok) bits |= 1u << u;
         if (!ok || at[u].format != kind) kind = kMixed;
         bf16 |= ok && at[u].format == ASHKV_PAGE_BF16;
-        const int64_t off = ok && at[u].format == ASHKV_PAGE_BF16 ? (tok[u] * p.kv.row_stride + head * D) * 2 : 0;
-        const uint64_t none = reinterpret_cast<uint64_t>(p.pieces);  // (an aligned address; nothing is read there)
-        t.k[e] = ok ? reinterpret_cast<uint64_t>(at[u].k) + off : none;
-        t.v[e] = ok ? reinterpret_cast<uint64_t>(at[u].v) + off : none;
-        t.meta[e] = (ok ? uint32_t(at[u].format) : kNoPage) | uint32_t(tok[u]) << 8;
+        const uint32_t fmt = ok ? uint32_t(at[u].format) : kNoPage;
+        const uint32_t chunks = fmt == ASHKV_PAGE_INT8 || fmt == ASHKV_PAGE_FP8 ? D / 16 : fmt == ASHKV_PAGE_INT4 || fmt == ASHKV_PAGE_NBIT4 ? D / 32 : fmt == ASHKV_PAGE_NBIT2 ? D / 64 : 0;
+        t.meta[e] = fmt | chunks << 8 | uint32_t(tok[u]) << 16;
+        if (fmt == ASHKV_PAGE_BF16) {
+          const int64_t off = (tok[u] * p.kv.row_stride + head * D) * 2;
+          t.row[0][e] = reinterpret_cast<uint64_t>(at[u].k) + off;
+          t.row[1][e] = reinterpret_cast<uint64_t>(at[u].v) + off;
+        } else if (ok) {
+#pragma unroll
+          for (uint32_t v = 0; v < 2; ++v) {
+            const RowBytes x = row_bytes<D>(fmt, at[u].k, uint32_t(p.kv.T), uint32_t(p.kv.row_len), uint32_t(tok[u]) + v * uint32_t(p.kv.T), uint32_t(head));
+            t.row[v][e] = reinterpret_cast<uint64_t>(x.codes);
+            t.scale[v][e] = x.scale;
+          }
+        }
       }
       if (!__all_sync(0xFFFFFFFFu, kind == __shfl_sync(0xFFFFFFFFu, kind, 0))) kind = kMixed;
       if (__any_sync(0xFFFFFFFFu, bf16) && kind == kMixed) kind = kMixedBf16;
@@ -599,9 +620,8 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
       __syncwarp();
 #pragma unroll 1
       for (int v = 0; v < 2; ++v) {
-        constexpr uint32_t L = D / 16, B = 4;  // lanes of a row; passes that wait for their descriptions together
+        constexpr uint32_t L = D / 16, B = 8;  // lanes of a row; passes that wait for their descriptions together
         const int h = 2 * n + v, slot = h % S::kRaw;
-        const uint64_t* rows = v ? t.v : t.k;
         const uint32_t codes = raw + uint32_t(slot) * S::kRawBytes, scales = codes + S::kCodes, l = uint32_t(lane) % L;
         if (h >= S::kRaw && !wait_warp(sm, &sm.bars.raw_empty[slot], (h / S::kRaw - 1) & 1)) {
           cp_async_wait_all();
@@ -609,24 +629,26 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
         }
 #pragma unroll 1
         for (uint32_t r = uint32_t(lane) / L; r < kTileKeys; r += 32 / L * B) {
-          RowBytes from[B];
-          uint32_t fmt[B];
-#pragma unroll
-          for (uint32_t x = 0; x < B; ++x) {
-            const uint32_t e = r + 32 / L * x, meta = t.meta[e];
-            fmt[x] = meta & 0xFFu;
-            from[x] = row_bytes<D>(p, fmt[x], reinterpret_cast<const uint8_t*>(rows[e]), (meta >> 8) + (v ? uint32_t(p.kv.T) : 0), uint32_t(head));
-            if (fmt[x] == kNoPage || fmt[x] == ASHKV_PAGE_BF16) from[x].bytes = 0;
-          }
+          uint64_t from[B];
+          uint32_t chunks[B];
 #pragma unroll
           for (uint32_t x = 0; x < B; ++x) {
             const uint32_t e = r + 32 / L * x;
-            if (l * 16 < from[x].bytes) cp_async16(codes + e * D + l * 16, from[x].codes + l * 16);
-            if (l == 0 && from[x].bytes) {
-              if (D == 128 && fmt[x] >= ASHKV_PAGE_NBIT4) cp_async_small<8>(scales + e * 8, from[x].scales);
-              else cp_async_small<4>(scales + e * 8, from[x].scales);
-            }
+            from[x] = t.row[v][e];
+            chunks[x] = t.meta[e] >> 8 & 0xFFu;
           }
+#pragma unroll
+          for (uint32_t x = 0; x < B; ++x)
+            if (l < chunks[x]) cp_async16(codes + (r + 32 / L * x) * D + l * 16, reinterpret_cast<const void*>(from[x] + l * 16));
+        }
+        // the scales, a row a lane
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x) {
+          const uint32_t e = uint32_t(lane) + 32 * x, meta = t.meta[e];
+          if (!(meta >> 8 & 0xFFu)) continue;
+          const void* from = reinterpret_cast<const void*>(t.row[v][e] - t.scale[v][e]);
+          if (D == 128 && (meta & 0xFFu) >= ASHKV_PAGE_NBIT4) cp_async_small<8>(scales + e * 8, from);
+          else cp_async_small<4>(scales + e * 8, from);
         }
         arrive_with_copies(&sm.bars.raw_full[slot]);
         if (lane == 0) mbar_arrive(&sm.bars.raw_full[slot]);  // (what the lanes wrote themselves)
@@ -645,7 +667,7 @@ __device__ __forceinline__ void int8_dec16(uint4 c, float s, uint4& x, uint4& y)
     y = int8_dec8(make_uint2(c.z, c.w), s);
     return;
   }
-  const Recip d = make_recip(127.0f);
+  const Recip d{0x1.020408p-7f, 0x1.020408p-35f};  // make_recip(127)
   const float h = __fmul_rn(s, d.hi), l = __fmaf_rn(s, d.lo, __fmaf_rn(s, d.hi, -h));
   const f2 H = pk2(h, h), L = pk2(l, l);
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
@@ -668,7 +690,7 @@ __device__ __forceinline__ void int4_dec16(uint2 c, uint16_t scale, uint4& x, ui
     y = int4_dec8(c.y, scale);
     return;
   }
-  const Recip d = make_recip(7.0f);
+  const Recip d{0x1.24924ap-3f, -0x1.b6db7p-28f};  // make_recip(7)
   const float h = __fmul_rn(s, d.hi), l = __fmaf_rn(s, d.lo, __fmaf_rn(s, d.hi, -h));
   const f2 H = pk2(h, h), L = pk2(l, l), bias = pk2(-8388616.0f, -8388616.0f);
   uint32_t o[8];
@@ -757,7 +779,7 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
     if (h >= S::kStages && !wait_warp(sm, &sm.bars.empty[st], (h / S::kStages - 1) & 1)) return false;
     const TileInfo& t = sm.info[h / 2 % kLook];
     if (t.kind == kMixedBf16 || t.kind == ASHKV_PAGE_BF16) {
-      const uint64_t* rows = h & 1 ? t.v : t.k;
+      const uint64_t* rows = t.row[h & 1];
       const uint32_t to = stages + uint32_t(st) * S::kTile;
 #pragma unroll 4
       for (uint32_t k = 0; k < kPasses; ++k) {
@@ -814,7 +836,7 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
           sts128p(to + chunk_at(r, 2 * u + swap), swap ? y : x);
           sts128p(to + chunk_at(r, 2 * u + !swap), swap ? x : y);
         };
-        const auto page_row = [&](uint32_t r) { return (t.meta[r] >> 8) + (v ? T : 0u); };
+        const auto page_row = [&](uint32_t r) { return (t.meta[r] >> 16) + (v ? T : 0u); };
         const auto all_rows = [&](auto format) {
           constexpr uint32_t F = decltype(format)::value;
           constexpr uint32_t B = 4;  // units that are on their way from shared memory together
@@ -855,10 +877,12 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
             __syncwarp();
             for (uint32_t j = 0; j < kPasses; ++j) {
               const uint32_t r = r0 + kStep * j, fmt = t.meta[r] & 0xFFu;
-              const uint8_t* s = reinterpret_cast<const uint8_t*>(v ? t.v[r] : t.k[r]);
-              const uint32_t row = uint32_t(p.kv.row_len), cap = uint32_t(p.kv.outlier_cap);
-              if (fmt == ASHKV_PAGE_NBIT4) overlay<D, 4>(s, T, row, cap, page_row(r), r, u, to, uint32_t(head));
-              else if (fmt == ASHKV_PAGE_NBIT2) overlay<D, 2>(s, T, row, cap, page_row(r), r, u, to, uint32_t(head));
+              if (fmt == kNoPage || fmt < ASHKV_PAGE_NBIT4) continue;
+              const uint32_t row = uint32_t(p.kv.row_len), cap = uint32_t(p.kv.outlier_cap), e = page_row(r) * row + uint32_t(head) * D;
+              const bool four = fmt == ASHKV_PAGE_NBIT4;
+              const uint8_t* s = reinterpret_cast<const uint8_t*>(t.row[v][r]) - nbit_codes_off(2 * T * row) - (four ? e / 2 : e / 4);
+              if (four) overlay<D, 4>(s, T, row, cap, page_row(r), r, u, to, uint32_t(head));
+              else overlay<D, 2>(s, T, row, cap, page_row(r), r, u, to, uint32_t(head));
             }
             __syncwarp();
             if (look)  // (outliers may be infinite too)
