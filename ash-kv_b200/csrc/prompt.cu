@@ -37,7 +37,7 @@ constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kLn2P = 0.6931471805599453f;
 constexpr int kTileRows = 128, kItemRows = 256, kTileKeys = 128;
 constexpr int kPlanThreads = 1024, kJoinThreadsP = 256;
-constexpr int kDecoders = 128;  // threads that decode
+constexpr int kDecoders = 256;  // threads that decode
 constexpr int kLook = 4;        // tiles looked up ahead
 constexpr uint32_t kPollsP = 1u << 24;                    // bounded waits
 constexpr int kBins = 64;
@@ -262,15 +262,15 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_
 // on their way, with eight bytes of scales for each row.  A tile is 128 rows of D bf16 in runs of 64 (128 bytes,
 // swizzled).  RAW: pages may be compressed, or of a size that tensor copies cannot place; else all tiles come by tensor copies.
 // Warps: eight for the softmax, one that issues the products, one that loads queries; then RAW: two that fetch, a tile in
-// turn each, and four that decode; else one that fetches and one that checks values.  Registers: what the softmax warps
-// take more than the launch gives, the others take less.
+// turn each, and eight that decode; else one that fetches and one that checks values.
 template <int D, bool RAW>
 struct Shape {
   static constexpr uint32_t kHalf = kTileRows * 128, kTile = kHalf * (D / 64);
   static constexpr int kStages = RAW ? (D == 64 ? 6 : 3) : (D == 64 ? 8 : 4);
   static constexpr int kRaw = RAW ? (D == 64 ? 6 : 3) : 0;
   static constexpr int kFetchers = RAW ? 2 : 1;
-  static constexpr int kThreads = RAW ? 512 : 384, kSoftmaxRegs = RAW ? 176 : 200, kOtherRegs = RAW ? 80 : 104;
+  static constexpr int kThreads = RAW ? 640 : 384;
+  static constexpr int kCols = RAW ? 1 : 2;  // 32 scores each that a softmax thread reads at a time
   // (A wait for a phase is sound only where the phase before is known to be over: with two fetchers in turn, from three raw
   // half tiles on.)
   static_assert(!RAW || kRaw >= kFetchers + 1);
@@ -280,7 +280,6 @@ struct Shape {
 
 struct __align__(16) TileInfo {
   uint64_t row[2][kTileKeys];           // (K, V) the head's channels: BF16 values or codes
-  uint32_t scale[2][kTileKeys];         // the word of the row's scales, so many bytes before its codes
   uint32_t meta[kTileKeys];             // format | chunks of 16 bytes of its codes << 8 | token in its page << 16
   uint32_t seen[4];                     // a bit for each token that exists
   int32_t first;                        // position of the tile's first token
@@ -357,29 +356,18 @@ __device__ __forceinline__ void tma_load_2d_at(uint32_t to, const void* map, uin
       :: "r"(to), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
 }
 
-// Where the codes of a row (row pr of a compressed page at s, key head `head`) are, and how far before them the word (of
-// dithered pages: the eight bytes, with D = 128) of its scales.
+// Where in its slot the codes of a row (row pr of a compressed page, key head `head`) are, and the word (of dithered
+// pages: the eight bytes, with D = 128) of its scales.
 struct RowBytes {
-  const uint8_t* codes;
-  uint32_t scale;
+  uint32_t codes, scales;
 };
 template <int D>
-__device__ __forceinline__ RowBytes row_bytes(uint32_t fmt, const uint8_t* s, uint32_t T, uint32_t row, uint32_t pr, uint32_t head) {
+__device__ __forceinline__ RowBytes row_bytes(uint32_t fmt, uint32_t T, uint32_t row, uint32_t pr, uint32_t head) {
   const uint32_t E = 2 * T * row, e = pr * row + head * D;
-  uint32_t codes, scale;
-  if (fmt == ASHKV_PAGE_INT8) {
-    codes = uint32_t(int8_codes_offset(int(T))) + e;
-    scale = 2 * pr & ~3u;
-  } else if (fmt == ASHKV_PAGE_FP8) {
-    codes = scale = e;
-  } else if (fmt == ASHKV_PAGE_INT4) {
-    codes = E / 32 + e / 2;
-    scale = e / 64 * 2 & ~3u;
-  } else {
-    codes = uint32_t(nbit_codes_off(E)) + (fmt == ASHKV_PAGE_NBIT4 ? e / 2 : e / 4);
-    scale = uint32_t(nbit_delta_off()) + e / 32 * 2;
-  }
-  return {s + codes, codes - scale};
+  if (fmt == ASHKV_PAGE_INT8) return {uint32_t(int8_codes_offset(int(T))) + e, 2 * pr & ~3u};
+  if (fmt == ASHKV_PAGE_FP8) return {e, e};
+  if (fmt == ASHKV_PAGE_INT4) return {E / 32 + e / 2, e / 64 * 2 & ~3u};
+  return {uint32_t(nbit_codes_off(E)) + (fmt == ASHKV_PAGE_NBIT4 ? e / 2 : e / 4), uint32_t(nbit_delta_off()) + e / 32 * 2};
 }
 
 // The tokens of 32 from first on that some row of a piece sees.
@@ -599,9 +587,8 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
         } else if (ok) {
 #pragma unroll
           for (uint32_t v = 0; v < 2; ++v) {
-            const RowBytes x = row_bytes<D>(fmt, at[u].k, uint32_t(p.kv.T), uint32_t(p.kv.row_len), uint32_t(tok[u]) + v * uint32_t(p.kv.T), uint32_t(head));
-            t.row[v][e] = reinterpret_cast<uint64_t>(x.codes);
-            t.scale[v][e] = x.scale;
+            const RowBytes x = row_bytes<D>(fmt, uint32_t(p.kv.T), uint32_t(p.kv.row_len), uint32_t(tok[u]) + v * uint32_t(p.kv.T), uint32_t(head));
+            t.row[v][e] = reinterpret_cast<uint64_t>(at[u].k) + x.codes;
           }
         }
       }
@@ -646,7 +633,8 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
         for (uint32_t x = 0; x < 4; ++x) {
           const uint32_t e = uint32_t(lane) + 32 * x, meta = t.meta[e];
           if (!(meta >> 8 & 0xFFu)) continue;
-          const void* from = reinterpret_cast<const void*>(t.row[v][e] - t.scale[v][e]);
+          const RowBytes at = row_bytes<D>(meta & 0xFFu, uint32_t(p.kv.T), uint32_t(p.kv.row_len), (meta >> 16) + v * uint32_t(p.kv.T), uint32_t(head));
+          const void* from = reinterpret_cast<const void*>(t.row[v][e] - at.codes + at.scales);
           if (D == 128 && (meta & 0xFFu) >= ASHKV_PAGE_NBIT4) cp_async_small<8>(scales + e * 8, from);
           else cp_async_small<4>(scales + e * 8, from);
         }
@@ -831,29 +819,18 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
         bool odd = false;
         const auto put = [&](uint32_t r, uint4 x, uint4 y) {
           if (look) odd |= not_finite(x) || not_finite(y);
-          // lanes of the upper half of a row store their odd chunk first: eight lanes, eight banks of 16 bytes
-          const bool swap = u >= 4;
-          sts128p(to + chunk_at(r, 2 * u + swap), swap ? y : x);
-          sts128p(to + chunk_at(r, 2 * u + !swap), swap ? x : y);
+          sts128p(to + chunk_at(r, 2 * u), x);
+          sts128p(to + chunk_at(r, 2 * u + 1), y);
         };
         const auto page_row = [&](uint32_t r) { return (t.meta[r] >> 16) + (v ? T : 0u); };
         const auto all_rows = [&](auto format) {
           constexpr uint32_t F = decltype(format)::value;
-          constexpr uint32_t B = 4;  // units that are on their way from shared memory together
 #pragma unroll 1
-          for (uint32_t j = 0; j < kPasses; j += B) {
-            Unit n[B];
-#pragma unroll
-            for (uint32_t b = 0; b < B; ++b) {
-              const uint32_t r = r0 + kStep * (j + b);
-              n[b] = load_unit<D>(F, codes + r * D, scales + r * 8, u, F == ASHKV_PAGE_INT8 ? page_row(r) : 0u, uint32_t(head));
-            }
-#pragma unroll
-            for (uint32_t b = 0; b < B; ++b) {
-              uint4 x, y;
-              decode_unit(F, n[b], x, y);
-              put(r0 + kStep * (j + b), x, y);
-            }
+          for (uint32_t j = 0; j < kPasses; ++j) {  // (rolled: four units at a time took 1.2 times as long, out of the instruction caches)
+            const uint32_t r = r0 + kStep * j;
+            uint4 x, y;
+            decode_unit(F, load_unit<D>(F, codes + r * D, scales + r * 8, u, F == ASHKV_PAGE_INT8 ? page_row(r) : 0u, uint32_t(head)), x, y);
+            put(r, x, y);
           }
         };
         if (kind == ASHKV_PAGE_INT8) {
@@ -878,10 +855,9 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
             for (uint32_t j = 0; j < kPasses; ++j) {
               const uint32_t r = r0 + kStep * j, fmt = t.meta[r] & 0xFFu;
               if (fmt == kNoPage || fmt < ASHKV_PAGE_NBIT4) continue;
-              const uint32_t row = uint32_t(p.kv.row_len), cap = uint32_t(p.kv.outlier_cap), e = page_row(r) * row + uint32_t(head) * D;
-              const bool four = fmt == ASHKV_PAGE_NBIT4;
-              const uint8_t* s = reinterpret_cast<const uint8_t*>(t.row[v][r]) - nbit_codes_off(2 * T * row) - (four ? e / 2 : e / 4);
-              if (four) overlay<D, 4>(s, T, row, cap, page_row(r), r, u, to, uint32_t(head));
+              const uint32_t row = uint32_t(p.kv.row_len), cap = uint32_t(p.kv.outlier_cap);
+              const uint8_t* s = reinterpret_cast<const uint8_t*>(t.row[v][r]) - row_bytes<D>(fmt, T, row, page_row(r), uint32_t(head)).codes;
+              if (fmt == ASHKV_PAGE_NBIT4) overlay<D, 4>(s, T, row, cap, page_row(r), r, u, to, uint32_t(head));
               else overlay<D, 2>(s, T, row, cap, page_row(r), r, u, to, uint32_t(head));
             }
             __syncwarp();
@@ -1145,6 +1121,7 @@ __device__ __noinline__ void tile_by_row(uint32_t s, uint32_t o, uint32_t v, uin
 template <int D, bool RAW>
 __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, int64_t works, int g) {
   using S = Shape<D, RAW>;
+  constexpr int kCols = S::kCols;
   const int lane = threadIdx.x & 31, at = int(threadIdx.x & 255);  // the row of the item
   const uint32_t lanes = uint32_t(at & 96) << 16;
   const uint32_t s = sm.tmem + uint32_t(g) * 128 + lanes, o = sm.tmem + 256 + uint32_t(g) * 128 + lanes;
@@ -1183,44 +1160,63 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
                                       real.z & seen_by(p, first + 64, ahead - 64), real.w & seen_by(p, first + 96, ahead - 96));
         tile_by_row<D>(s, o, base + 2 * S::kTile + uint32_t((2 * n + 1) % S::kStages) * S::kTile, bits, scale2, i > 0, m, l);
       } else {
-        float v[4][32];
+        // 32 kCols scores at a time, read twice: a loop of a few instructions stays in the instruction caches beside
+        // the other warps' code, 128 scores in registers, unrolled, do not
+        const bool hidden = edge || (real.x & real.y & real.z & real.w) != 0xFFFFFFFFu;
+        const auto load = [&](int q, float (&v)[kCols][32]) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32(s + q * 32, v[q]);
-        tmem_ld_wait();
+          for (int k = 0; k < kCols; ++k) tmem_ld32(s + (q + k) * 32, v[k]);
+          tmem_ld_wait();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld_done(v[q]);
-        if (edge || (real.x & real.y & real.z & real.w) != 0xFFFFFFFFu) {
+          for (int k = 0; k < kCols; ++k) tmem_ld_done(v[k]);
+          if (hidden) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t bits = (q == 0 ? real.x : q == 1 ? real.y : q == 2 ? real.z : real.w) & seen_by(p, first + 32 * q, ahead - 32 * q);
+            for (int k = 0; k < kCols; ++k) {
+              const uint32_t bits = t.seen[q + k] & seen_by(p, first + 32 * (q + k), ahead - 32 * (q + k));
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[q][j] = bits >> j & 1u ? v[q][j] : -INFINITY;
+              for (int j = 0; j < 32; ++j) v[k][j] = bits >> j & 1u ? v[k][j] : -INFINITY;
+            }
           }
+        };
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int q = 0; q < 4; q += kCols) {
+          float v[kCols][32];
+          load(q, v);
+          float x[2] = {top, -INFINITY};
+#pragma unroll
+          for (int k = 0; k < kCols; ++k)
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              x[0] = max3f(x[0], v[k][j], v[k][j + 1]);
+              x[1] = max3f(x[1], v[k][j + 2], v[k][j + 3]);
+            }
+          top = fmaxf(x[0], x[1]);
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int j = 0; j < 32; j += 2)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) top[q] = max3f(top[q], v[q][j], v[q][j + 1]);
-        const float f = follow(fmaxf(max3f(top[0], top[1], top[2]), top[3]) * scale2, m, l);
+        const float f = follow(top * scale2, m, l);
         if (i > 0 && __any_sync(0xFFFFFFFFu, f != 1.0f)) scale_sums<D>(o, f);
         const float ref = m == -INFINITY ? 0.0f : m;
         const f2 SC = pk2(scale2, scale2), NM = pk2(-ref, -ref);
         f2 sum0 = pk2(0.0f, 0.0f), sum1 = sum0;
+#pragma unroll 1
+        for (int q = 0; q < 4; q += kCols) {
+          float v[kCols][32];
+          load(q, v);
 #pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-          uint32_t w[32];
+          for (int k = 0; k < kCols; ++k) {
+            uint32_t w[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float x, y;
-            upk2(fma2(pk2(v[q + (j >> 4)][2 * (j & 15)], v[q + (j >> 4)][2 * (j & 15) + 1]), SC, NM), x, y);
-            x = ex2(x);
-            y = ex2(y);
-            if (j & 1) sum1 = add2(sum1, pk2(x, y));
-            else sum0 = add2(sum0, pk2(x, y));
-            w[j] = f32x2_to_bf16x2(x, y);
+            for (int j = 0; j < 16; ++j) {
+              float x, y;
+              upk2(fma2(pk2(v[k][2 * j], v[k][2 * j + 1]), SC, NM), x, y);
+              x = ex2(x);
+              y = ex2(y);
+              if (j & 1) sum1 = add2(sum1, pk2(x, y));
+              else sum0 = add2(sum0, pk2(x, y));
+              w[j] = f32x2_to_bf16x2(x, y);
+            }
+            tmem_st16(s + (q + k) * 16, w);
           }
-          tmem_st32(s + (q >> 1) * 32, w);
         }
         float a, b;
         upk2(add2(sum0, sum1), a, b);
@@ -1278,11 +1274,6 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
   }
 }
 
-template <int N>
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
-template <int N>
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
-
 template <int D, bool RAW>
 __global__ void __launch_bounds__(Shape<D, RAW>::kThreads, 1) prompt_kernel(const __grid_constant__ PromptParams p) {
   extern __shared__ uint8_t smem[];
@@ -1312,21 +1303,16 @@ __global__ void __launch_bounds__(Shape<D, RAW>::kThreads, 1) prompt_kernel(cons
   tc_fence_after();
   allow_next();
   const int64_t works = int64_t(*const_cast<const volatile int32_t*>(p.counts)) * p.kv.heads_kv;
-  if (warp < 8) {
-    more_registers<Shape<D, RAW>::kSoftmaxRegs>();
-    softmax_rows<D, RAW>(p, sm, base, works, warp >> 2);
+  if (warp < 8) softmax_rows<D, RAW>(p, sm, base, works, warp >> 2);
+  else if (warp == 8) issue_products<D, RAW>(p, sm, base, works);
+  else if (warp == 9) load_queries<D, RAW>(p, sm, base, works);
+  else if constexpr (RAW) {
+    if (warp < 12) fetch_tiles<D>(p, sm, base, works, warp - 10);
+    else decode_tiles<D>(p, sm, base, works);
+  } else if (warp == 10) {
+    fetch_boxes<D>(p, sm, base, works);
   } else {
-    fewer_registers<Shape<D, RAW>::kOtherRegs>();
-    if (warp == 8) issue_products<D, RAW>(p, sm, base, works);
-    else if (warp == 9) load_queries<D, RAW>(p, sm, base, works);
-    else if constexpr (RAW) {
-      if (warp < 12) fetch_tiles<D>(p, sm, base, works, warp - 10);
-      else decode_tiles<D>(p, sm, base, works);
-    } else if (warp == 10) {
-      fetch_boxes<D>(p, sm, base, works);
-    } else {
-      check_values<D>(p, sm, base, works);
-    }
+    check_values<D>(p, sm, base, works);
   }
   __syncwarp();
   tc_fence_before();
