@@ -270,7 +270,12 @@ struct Shape {
   static constexpr int kRaw = RAW ? (D == 64 ? 6 : 3) : 0;
   static constexpr int kFetchers = RAW ? 2 : 1;
   static constexpr int kThreads = RAW ? 640 : 384;
-  static constexpr int kCols = RAW ? 1 : 2;  // 32 scores each that a softmax thread reads at a time
+  // Scores that a softmax thread reads at a time, in units of 32: all four, which it then keeps, or one at a time and twice.
+  // Beside warps that decode, the short loop stays in the instruction caches and the long one does not (INT8: 920 and 1100
+  // us); alone the long one is faster (606 and 636).
+  static constexpr int kCols = RAW ? 1 : 4;
+  // Registers without RAW: what the softmax warps take more than the launch gives, the others take less.
+  static constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
   // (A wait for a phase is sound only where the phase before is known to be over: with two fetchers in turn, from three raw
   // half tiles on.)
   static_assert(!RAW || kRaw >= kFetchers + 1);
@@ -936,7 +941,8 @@ __device__ void issue_products(const PromptParams& p, Shared& sm, uint32_t base,
   // descriptors of the first query tile and of stage 0 as K and as V; an address further on is added in units of 16 bytes
   const uint64_t q_desc = sw128_kmajor_desc(base), k_desc = sw128_kmajor_desc(base + 2 * S::kTile);
   const uint64_t v_desc = sw128_mnmajor_desc(base + 2 * S::kTile, S::kHalf);
-  int n = 0, items = 0, ready[2] = {0, 0};
+  int n = 0, items = 0;
+  uint32_t ready = 0;  // a bit for each tile
   bool ok = true;
   const auto scores = [&](int g, uint32_t stage) {
     const uint64_t q = q_desc + (uint32_t(g) * S::kTile >> 4), k = k_desc + (stage * S::kTile >> 4);
@@ -982,11 +988,11 @@ __device__ void issue_products(const PromptParams& p, Shared& sm, uint32_t base,
         odd = __any_sync(0xFFFFFFFFu, *const_cast<volatile int32_t*>(&sm.info[(n + i - 1) % kLook].odd));
       }
       if (i < tiles && !(ok = wait_warp(sm, &sm.bars.full[sk], (hk / S::kStages) & 1))) break;
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (g == two) break;
+#pragma unroll 1
+      for (int g = 0; g < two; ++g) {
         if (i > 0) {
-          if (!(ok = wait_warp(sm, &sm.bars.p_ready[g], ready[g]++ & 1))) break;
+          if (!(ok = wait_warp(sm, &sm.bars.p_ready[g], ready >> g & 1))) break;
+          ready ^= 1u << g;
           tc_fence_after();
           if (!odd) values(g, sv, i > 1);
           if (i == tiles) commit(&sm.bars.s_full[g]);
@@ -1160,8 +1166,6 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
                                       real.z & seen_by(p, first + 64, ahead - 64), real.w & seen_by(p, first + 96, ahead - 96));
         tile_by_row<D>(s, o, base + 2 * S::kTile + uint32_t((2 * n + 1) % S::kStages) * S::kTile, bits, scale2, i > 0, m, l);
       } else {
-        // 32 kCols scores at a time, read twice: a loop of a few instructions stays in the instruction caches beside
-        // the other warps' code, 128 scores in registers, unrolled, do not
         const bool hidden = edge || (real.x & real.y & real.z & real.w) != 0xFFFFFFFFu;
         const auto load = [&](int q, float (&v)[kCols][32]) {
 #pragma unroll
@@ -1178,10 +1182,9 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
             }
           }
         };
-        float top = -INFINITY;
+        float v[kCols][32], top = -INFINITY;
 #pragma unroll 1
         for (int q = 0; q < 4; q += kCols) {
-          float v[kCols][32];
           load(q, v);
           float x[2] = {top, -INFINITY};
 #pragma unroll
@@ -1200,8 +1203,7 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
         f2 sum0 = pk2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll 1
         for (int q = 0; q < 4; q += kCols) {
-          float v[kCols][32];
-          load(q, v);
+          if constexpr (kCols < 4) load(q, v);
 #pragma unroll
           for (int k = 0; k < kCols; ++k) {
             uint32_t w[16];
@@ -1274,6 +1276,11 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
   }
 }
 
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
+
 template <int D, bool RAW>
 __global__ void __launch_bounds__(Shape<D, RAW>::kThreads, 1) prompt_kernel(const __grid_constant__ PromptParams p) {
   extern __shared__ uint8_t smem[];
@@ -1303,6 +1310,10 @@ __global__ void __launch_bounds__(Shape<D, RAW>::kThreads, 1) prompt_kernel(cons
   tc_fence_after();
   allow_next();
   const int64_t works = int64_t(*const_cast<const volatile int32_t*>(p.counts)) * p.kv.heads_kv;
+  if constexpr (!RAW) {
+    if (warp < 8) more_registers<Shape<D, RAW>::kSoftmaxRegs>();
+    else fewer_registers<Shape<D, RAW>::kOtherRegs>();
+  }
   if (warp < 8) softmax_rows<D, RAW>(p, sm, base, works, warp >> 2);
   else if (warp == 8) issue_products<D, RAW>(p, sm, base, works);
   else if (warp == 9) load_queries<D, RAW>(p, sm, base, works);
