@@ -125,15 +125,22 @@ __device__ __forceinline__ int sequence_of(const PageLists& l, int64_t i) {
   return -1;
 }
 
+// What the table says of a page; of no such page, tier -1.
+struct Entry {
+  int32_t tier, layer, start, slot;
+};
+__device__ __forceinline__ Entry entry_of(const PagedKV& p, int32_t id) {
+  if (id < 0 || id >= p.n_pages) return Entry{-1, 0, 0, 0};
+  return Entry{p.tier[id], p.layer_id[id], p.token_start[id], p.page_slot[id]};
+}
 // Where a page lies: its format, and its first K and V row in the pool or (k) its slot.  No such page: -1.
 struct Place {
   int32_t format;
   uint8_t *k, *v;
 };
-__device__ __forceinline__ Place place_of(const PagedKV& p, int32_t id) {
+__device__ __forceinline__ Place place_of(const PagedKV& p, const Entry& e) {
   Place at{-1, nullptr, nullptr};
-  if (id < 0 || id >= p.n_pages) return at;
-  const int tier = p.tier[id], layer = p.layer_id[id], start = p.token_start[id], slot = p.page_slot[id];
+  const auto [tier, layer, start, slot] = e;
   if (tier == 0) {
     if (layer < 0 || layer >= p.n_layers || start < 0 || int64_t(start) + p.T > p.pool_tokens) return at;
     at.format = ASHKV_PAGE_BF16;
@@ -147,6 +154,7 @@ __device__ __forceinline__ Place place_of(const PagedKV& p, int32_t id) {
   }
   return at;
 }
+__device__ __forceinline__ Place place_of(const PagedKV& p, int32_t id) { return place_of(p, entry_of(p, id)); }
 
 }  // namespace
 }  // namespace ashkv

@@ -304,6 +304,7 @@ struct Shared {
 };
 
 __device__ __forceinline__ bool wait_p(Shared& sm, uint64_t* bar, uint32_t parity) {
+#pragma unroll 1  // (unrolled, the many waits made the kernel 3 % slower)
   for (uint32_t n = 0; n < kPollsP; ++n) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((n & 255u) == 255u && sm.failed) return false;
@@ -321,12 +322,16 @@ __device__ __forceinline__ bool wait_warp(Shared& sm, uint64_t* bar, uint32_t pa
 __device__ __forceinline__ int64_t work_of(int k) {
   return int64_t(k) * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
+// A value that all lanes hold, for the compiler one of the warp too: what it takes for a thread's own makes of every branch
+// that depends on it one that could diverge, with collective instructions behind it.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xFFFFFFFFu, x, 0); }
 __device__ __forceinline__ Piece load_piece(const PromptParams& p, int64_t w, int& head) {
   const int64_t i = w / p.kv.heads_kv;
   head = int(w - i * p.kv.heads_kv);
   const uint4* at = reinterpret_cast<const uint4*>(p.pieces + i);
   const uint4 a = ld_v4(at), b = ld_v4(at + 1), c = ld_v4(at + 2);
-  return Piece{int(a.x), int(a.y), int(a.z), int(a.w), int(b.x), int(b.y), int(b.z), int(b.w), int(c.x), int(c.y), int(c.z), int(c.w)};
+  return Piece{uniform(a.x), uniform(a.y), uniform(a.z), uniform(a.w), uniform(b.x), uniform(b.y),
+               uniform(b.z), uniform(b.w), uniform(c.x), uniform(c.y), uniform(c.z), uniform(c.w)};
 }
 __device__ __forceinline__ int tile_of(const Piece& pc, int i) { return i < pc.ts ? i : i - pc.ts + pc.tw; }
 
@@ -518,7 +523,7 @@ __device__ void check_values(const PromptParams& p, Shared& sm, uint32_t base, i
       const int h = 2 * n + 1, st = h % S::kStages;
       if (!wait_warp(sm, &sm.bars.full[st], (h / S::kStages) & 1)) return;
       TileInfo& t = sm.info[n % kLook];
-      if (t.edge) {
+      if (uniform(t.edge)) {
         bool odd = false;
         const uint32_t at = base + 2 * S::kTile + uint32_t(st) * S::kTile + uint32_t(lane) * 16;
 #pragma unroll 8
@@ -675,68 +680,85 @@ __device__ __forceinline__ void int8_dec16(uint4 c, float s, uint4& x, uint4& y)
   x = make_uint4(o[0], o[1], o[2], o[3]);
   y = make_uint4(o[4], o[5], o[6], o[7]);
 }
-// Sixteen INT4 codes, likewise.
-__device__ __forceinline__ void int4_dec16(uint2 c, uint16_t scale, uint4& x, uint4& y) {
+// Eight INT4 codes, likewise.
+__device__ __forceinline__ uint4 int4_dec8_short(uint32_t w, uint16_t scale) {
   const float s = bf16_to_f32(scale);
-  if (!(s >= 0x1p-90f && s <= 0x1p+90f)) {
-    x = int4_dec8(c.x, scale);
-    y = int4_dec8(c.y, scale);
-    return;
-  }
+  if (!(s >= 0x1p-90f && s <= 0x1p+90f)) return int4_dec8(w, scale);
   const Recip d{0x1.24924ap-3f, -0x1.b6db7p-28f};  // make_recip(7)
   const float h = __fmul_rn(s, d.hi), l = __fmaf_rn(s, d.lo, __fmaf_rn(s, d.hi, -h));
   const f2 H = pk2(h, h), L = pk2(l, l), bias = pk2(-8388616.0f, -8388616.0f);
-  uint32_t o[8];
+  uint32_t o[4];
+  const uint32_t hi = (w >> 4) & 0x0F0F0F0Fu, lo = w & 0x0F0F0F0Fu;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const uint32_t w = k ? c.y : c.x, hi = (w >> 4) & 0x0F0F0F0Fu, lo = w & 0x0F0F0F0Fu;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f2 a = add2(pk2(code_plus_2p23(hi, j), code_plus_2p23(lo, j)), bias);
-      o[4 * k + j] = f32x2_to_bf16x2_pk(fma2(a, H, mul2(a, L)));
-    }
+  for (int j = 0; j < 4; ++j) {
+    const f2 a = add2(pk2(code_plus_2p23(hi, j), code_plus_2p23(lo, j)), bias);
+    o[j] = f32x2_to_bf16x2_pk(fma2(a, H, mul2(a, L)));
   }
-  x = make_uint4(o[0], o[1], o[2], o[3]);
-  y = make_uint4(o[4], o[5], o[6], o[7]);
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// Unit u (16 channels) of a row: its codes and scale, from shared memory ..
+// Unit u of a row, channels 8 u .. and D / 2 + 8 u .. (so that eight lanes' stores meet no bank twice: 16 neighbouring channels
+// a lane took twice the cycles of the banks): its codes and scales, from shared memory ..
 struct Unit {
-  uint4 codes;
-  uint16_t scale;
+  uint2 a, b;
+  uint16_t s, t;
 };
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+  uint2 x;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(at));
+  return x;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+  uint32_t x;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at));
+  return x;
+}
+__device__ __forceinline__ uint16_t lds16(uint32_t at) {
+  uint16_t x;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at));
+  return x;
+}
 template <int D>
 __device__ __forceinline__ Unit load_unit(uint32_t fmt, uint32_t codes, uint32_t scales, uint32_t u, uint32_t pr, uint32_t head) {
   Unit x;
-  uint32_t at = scales;
   if (fmt == ASHKV_PAGE_INT8 || fmt == ASHKV_PAGE_FP8) {
-    x.codes = lds128(codes + 16 * u);
-    at += (pr & 1u) * 2;
-  } else if (fmt == ASHKV_PAGE_INT4 || fmt == ASHKV_PAGE_NBIT4) {
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x.codes.x), "=r"(x.codes.y) : "r"(codes + 8 * u));
-    at += fmt == ASHKV_PAGE_INT4 ? (D == 128 ? u / 4 : head & 1u) * 2 : u / 2 * 2;
+    x.a = lds64(codes + 8 * u);
+    x.b = lds64(codes + D / 2 + 8 * u);
+    if (fmt == ASHKV_PAGE_INT8) x.s = lds16(scales + (pr & 1u) * 2);
+  } else if (fmt == ASHKV_PAGE_INT4) {
+    x.a.x = lds32(codes + 4 * u);
+    x.b.x = lds32(codes + D / 4 + 4 * u);
+    x.s = lds16(scales + (D == 128 ? 0 : head & 1u) * 2);
+    x.t = D == 128 ? lds16(scales + 2) : x.s;
   } else {
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x.codes.x) : "r"(codes + 4 * u));
-    at += u / 2 * 2;
+    if (fmt == ASHKV_PAGE_NBIT4) {
+      x.a.x = lds32(codes + 4 * u);
+      x.b.x = lds32(codes + D / 4 + 4 * u);
+    } else {
+      x.a.x = lds16(codes + 2 * u);
+      x.b.x = lds16(codes + D / 8 + 2 * u);
+    }
+    x.s = lds16(scales + u / 4 * 2);
+    x.t = lds16(scales + (u + D / 16) / 4 * 2);
   }
-  if (fmt != ASHKV_PAGE_FP8) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x.scale) : "r"(at));
   return x;
 }
 // .. and its values.
 __device__ __forceinline__ void decode_unit(uint32_t fmt, const Unit& n, uint4& x, uint4& y) {
   if (fmt == ASHKV_PAGE_INT8) {
-    int8_dec16(n.codes, f16_to_f32(n.scale), x, y);
+    int8_dec16(make_uint4(n.a.x, n.a.y, n.b.x, n.b.y), f16_to_f32(n.s), x, y);
   } else if (fmt == ASHKV_PAGE_FP8) {
-    x = fp8_dec8(make_uint2(n.codes.x, n.codes.y));
-    y = fp8_dec8(make_uint2(n.codes.z, n.codes.w));
+    x = fp8_dec8(n.a);
+    y = fp8_dec8(n.b);
   } else if (fmt == ASHKV_PAGE_INT4) {
-    int4_dec16(make_uint2(n.codes.x, n.codes.y), n.scale, x, y);
+    x = int4_dec8_short(n.a.x, n.s);
+    y = int4_dec8_short(n.b.x, n.t);
   } else if (fmt == ASHKV_PAGE_NBIT4) {
-    x = nbit_dec8<4>(n.codes.x, n.scale);
-    y = nbit_dec8<4>(n.codes.y, n.scale);
+    x = nbit_dec8<4>(n.a.x, n.s);
+    y = nbit_dec8<4>(n.b.x, n.t);
   } else {
-    x = nbit_dec8<2>(n.codes.x & 0xFFFFu, n.scale);
-    y = nbit_dec8<2>(n.codes.x >> 16, n.scale);
+    x = nbit_dec8<2>(n.a.x, n.s);
+    y = nbit_dec8<2>(n.b.x, n.t);
   }
 }
 
@@ -754,7 +776,7 @@ __device__ __noinline__ void overlay(const uint8_t* slot, uint32_t T, uint32_t r
   }
 }
 
-// Raw half tiles -> key and value tiles.  D / 16 lanes to a row, 16 channels each; BF16 rows among compressed ones are copied
+// Raw half tiles -> key and value tiles.  D / 16 lanes to a row, two chunks of 8 channels each; BF16 rows among compressed ones are copied
 // a half tile ahead.
 template <int D>
 __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, int64_t works) {
@@ -771,7 +793,8 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
     if (!wait_warp(sm, &sm.bars.raw_full[slot], (h / S::kRaw) & 1)) return false;
     if (h >= S::kStages && !wait_warp(sm, &sm.bars.empty[st], (h / S::kStages - 1) & 1)) return false;
     const TileInfo& t = sm.info[h / 2 % kLook];
-    if (t.kind == kMixedBf16 || t.kind == ASHKV_PAGE_BF16) {
+    const int kind = uniform(t.kind);
+    if (kind == kMixedBf16 || kind == ASHKV_PAGE_BF16) {
       const uint64_t* rows = t.row[h & 1];
       const uint32_t to = stages + uint32_t(st) * S::kTile;
 #pragma unroll 4
@@ -808,7 +831,7 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
           ++copied;
         }
         TileInfo& t = sm.info[n % kLook];
-        const int kind = t.kind;
+        const int kind = uniform(t.kind);
         // (BF16 rows: the next half tile's as well, if it is near)
         bool ahead = false;
         if ((kind == kMixedBf16 || kind == ASHKV_PAGE_BF16) && copied < 2 * total) {
@@ -820,12 +843,12 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
           ahead = true;
         }
         const uint32_t to = stages + uint32_t(st) * S::kTile, codes = raw + uint32_t(slot) * S::kRawBytes, scales = codes + S::kCodes;
-        const bool look = v && t.edge;
+        const bool look = v && uniform(t.edge);
         bool odd = false;
         const auto put = [&](uint32_t r, uint4 x, uint4 y) {
           if (look) odd |= not_finite(x) || not_finite(y);
-          sts128p(to + chunk_at(r, 2 * u), x);
-          sts128p(to + chunk_at(r, 2 * u + 1), y);
+          sts128p(to + chunk_at(r, u), x);
+          sts128p(to + chunk_at(r, u + L), y);
         };
         const auto page_row = [&](uint32_t r) { return (t.meta[r] >> 16) + (v ? T : 0u); };
         const auto all_rows = [&](auto format) {
@@ -870,7 +893,7 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
               for (uint32_t j = 0; j < kPasses; ++j) {
                 const uint32_t r = r0 + kStep * j;
                 if ((t.meta[r] & 0xFFu) != ASHKV_PAGE_BF16)
-                  odd |= not_finite(lds128(to + chunk_at(r, 2 * u))) || not_finite(lds128(to + chunk_at(r, 2 * u + 1)));
+                  odd |= not_finite(lds128(to + chunk_at(r, u))) || not_finite(lds128(to + chunk_at(r, u + L)));
               }
           }
         }
@@ -937,7 +960,7 @@ __device__ void issue_products(const PromptParams& p, Shared& sm, uint32_t base,
   using S = Shape<D, RAW>;
   constexpr uint32_t kScores = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kTileKeys >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
   constexpr uint32_t kValues = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
-  const uint32_t scores_desc = kScores | p.negate, tmem = sm.tmem;
+  const uint32_t scores_desc = kScores | p.negate, tmem = uniform(sm.tmem);
   // descriptors of the first query tile and of stage 0 as K and as V; an address further on is added in units of 16 bytes
   const uint64_t q_desc = sw128_kmajor_desc(base), k_desc = sw128_kmajor_desc(base + 2 * S::kTile);
   const uint64_t v_desc = sw128_mnmajor_desc(base + 2 * S::kTile, S::kHalf);
@@ -973,8 +996,7 @@ __device__ void issue_products(const PromptParams& p, Shared& sm, uint32_t base,
   for (int k = 0; ok && work_of(k) < works; ++k) {
     int head;
     const Piece pc = load_piece(p, work_of(k), head);
-    const int tiles = __shfl_sync(0xFFFFFFFFu, pc.end - pc.begin, 0);  // (uniform for the compiler too)
-    const int two = __shfl_sync(0xFFFFFFFFu, pc.rows > kTileRows ? 2 : 1, 0);
+    const int tiles = pc.end - pc.begin, two = pc.rows > kTileRows ? 2 : 1;
     if (tiles <= 0) continue;
     if (!(ok = wait_warp(sm, &sm.bars.q_full, items++ & 1))) break;
     for (int i = 0; ok && i <= tiles; ++i) {
@@ -1130,11 +1152,11 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
   constexpr int kCols = S::kCols;
   const int lane = threadIdx.x & 31, at = int(threadIdx.x & 255);  // the row of the item
   const uint32_t lanes = uint32_t(at & 96) << 16;
-  const uint32_t s = sm.tmem + uint32_t(g) * 128 + lanes, o = sm.tmem + 256 + uint32_t(g) * 128 + lanes;
+  const uint32_t tmem = uniform(sm.tmem), s = tmem + uint32_t(g) * 128 + lanes, o = tmem + 256 + uint32_t(g) * 128 + lanes;
   const float scale2 = p.scale2;
   int n = 0, phase = 0;  // tiles of the CTA and scores of this tile so far
   for (int k = 0; work_of(k) < works; ++k) {
-    int tiles, pos;
+    int tiles, pos, quarters = 4;  // 0: no row is the warp's, and nobody reads what its lanes of TMEM hold
     {
       int head;
       const Piece pc = load_piece(p, work_of(k), head);
@@ -1144,6 +1166,7 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
         continue;
       }
       pos = pc.pos0 + (pc.row0 + min(at, pc.rows - 1)) / p.group;
+      if (RAW && uniform(at) >= pc.rows) quarters = 0;
     }
     float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
@@ -1153,20 +1176,20 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
       const TileInfo& t = sm.info[n % kLook];
       const int first = t.first, ahead = pos - first;  // (tokens that the row sees of this tile end here)
       const uint4 real = *reinterpret_cast<const uint4*>(t.seen);
-      const bool edge = t.edge != 0;
+      const bool edge = uniform(t.edge) != 0;
       bool odd = false;
       if (edge) {  // does V hold values that some rows must not see?
         const int hv = 2 * n + 1;
         uint64_t* known = RAW ? &sm.bars.full[hv % S::kStages] : &sm.bars.checked[n % kLook];
         if (!wait_warp(sm, known, (RAW ? hv / S::kStages : n / kLook) & 1)) return;
-        odd = *const_cast<const volatile int32_t*>(&t.odd);
+        odd = uniform(*const_cast<const volatile int32_t*>(&t.odd)) != 0;
       }
       if (odd) {
         const uint4 bits = make_uint4(real.x & seen_by(p, first, ahead), real.y & seen_by(p, first + 32, ahead - 32),
                                       real.z & seen_by(p, first + 64, ahead - 64), real.w & seen_by(p, first + 96, ahead - 96));
         tile_by_row<D>(s, o, base + 2 * S::kTile + uint32_t((2 * n + 1) % S::kStages) * S::kTile, bits, scale2, i > 0, m, l);
       } else {
-        const bool hidden = edge || (real.x & real.y & real.z & real.w) != 0xFFFFFFFFu;
+        const bool hidden = edge || uniform(real.x & real.y & real.z & real.w) != -1;
         const auto load = [&](int q, float (&v)[kCols][32]) {
 #pragma unroll
           for (int k = 0; k < kCols; ++k) tmem_ld32(s + (q + k) * 32, v[k]);
@@ -1184,7 +1207,7 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
         };
         float v[kCols][32], top = -INFINITY;
 #pragma unroll 1
-        for (int q = 0; q < 4; q += kCols) {
+        for (int q = 0; q < quarters; q += kCols) {
           load(q, v);
           float x[2] = {top, -INFINITY};
 #pragma unroll
@@ -1202,7 +1225,7 @@ __device__ void softmax_rows(const PromptParams& p, Shared& sm, uint32_t base, i
         const f2 SC = pk2(scale2, scale2), NM = pk2(-ref, -ref);
         f2 sum0 = pk2(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll 1
-        for (int q = 0; q < 4; q += kCols) {
+        for (int q = 0; q < quarters; q += kCols) {
           if constexpr (kCols < 4) load(q, v);
 #pragma unroll
           for (int k = 0; k < kCols; ++k) {
@@ -1309,7 +1332,7 @@ __global__ void __launch_bounds__(Shape<D, RAW>::kThreads, 1) prompt_kernel(cons
   __syncthreads();
   tc_fence_after();
   allow_next();
-  const int64_t works = int64_t(*const_cast<const volatile int32_t*>(p.counts)) * p.kv.heads_kv;
+  const int64_t works = int64_t(uniform(*const_cast<const volatile int32_t*>(p.counts))) * p.kv.heads_kv;
   if constexpr (!RAW) {
     if (warp < 8) more_registers<Shape<D, RAW>::kSoftmaxRegs>();
     else fewer_registers<Shape<D, RAW>::kOtherRegs>();
@@ -1408,7 +1431,10 @@ Sizes sizes_of(int64_t n_rows, int64_t n_seqs, int heads_q, int heads_kv, int n_
   const int sms = sm_count() > 0 ? sm_count() : 148, group = heads_q / heads_kv;
   s.items = n_rows * group / kItemRows + n_seqs;
   s.part_rows = std::min<int64_t>(kItemRows, std::max<int64_t>(1, n_rows * group));
-  s.share = sms;
+  // Works that would leave the CTAs a fifth of their time idle are cut, into four for each CTA; else a piece more costs more
+  // (the queries come anew: 3 us) than it evens out (272 works: 370 us, cut into 1300: 396).
+  const int64_t works = s.items * heads_kv;
+  s.share = (works + sms - 1) / sms * sms * 4 > works * 5 ? 4 * sms : sms;
   // an item of n tiles is cut where n exceeds a share: into at most 2 n / share pieces, share >= all tiles / s.share
   s.parts = std::min<int64_t>(2 * int64_t(s.share) / heads_kv + 2, 2 * int64_t(s.share) + 2);
   s.pieces = s.items + s.parts;
