@@ -40,7 +40,7 @@ constexpr int kPlanThreads = 1024, kJoinThreadsP = 256;
 constexpr int kDecoders = 256;  // threads that decode
 constexpr int kLook = 4;        // tiles looked up ahead
 constexpr uint32_t kPollsP = 1u << 24;                    // bounded waits
-constexpr int kBins = 64;
+constexpr int kBins = 64;  // (two to a lane)
 constexpr uint32_t kNoPage = 0xFFu;
 constexpr int kMixed = 0x100, kMixedBf16 = 0x101;
 
@@ -74,6 +74,7 @@ struct PromptParams {
   int64_t q_row, q_head;
   int32_t n_rows, heads_q, group;
   bool q_wide;
+  bool q_boxes;      // a tile's queries are a box: tensor copies by a map of [n_rows][heads_q][D]
   float scale2;      // |scale| * log2(e)
   uint32_t negate;   // of the instruction descriptor, for a negative scale
   int32_t window, sinks;  // window 0: none
@@ -228,14 +229,17 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_
       atomicAdd(&s_bin[bin_of(int(int64_t(it.n) * (k + 1) / parts - int64_t(it.n) * k / parts))], 1);
   }
   __syncthreads();
-  if (tid == 0) {
-    int sum = 0;
-    for (int k = 0; k < kBins; ++k) {
-      const int n = s_bin[k];
-      s_bin[k] = sum;
-      sum += n;
+  if (warp == 0) {  // where each bin begins, two bins a lane
+    const int x = s_bin[2 * lane], y = s_bin[2 * lane + 1];
+    int upto = x + y;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int z = __shfl_up_sync(0xFFFFFFFFu, upto, off);
+      if (lane >= off) upto += z;
     }
-    p.counts[0] = min(sum, p.max_pieces);
+    s_bin[2 * lane] = upto - x - y;
+    s_bin[2 * lane + 1] = upto - y;
+    if (lane == 31) p.counts[0] = min(upto, p.max_pieces);
   }
   __syncthreads();
   for (int i = tid; i < items; i += kPlanThreads) {
@@ -364,6 +368,12 @@ __device__ __forceinline__ void tma_load_2d_at(uint32_t to, const void* map, uin
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
       :: "r"(to), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_at(uint32_t to, const void* map, uint64_t* bar, int32_t x, int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      :: "r"(to), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
 }
 
 // Where in its slot the codes of a row (row pr of a compressed page, key head `head`) are, and the word (of dithered
@@ -919,7 +929,7 @@ __device__ void decode_tiles(const PromptParams& p, Shared& sm, uint32_t base, i
 
 // ---- queries: a warp
 template <int D, bool RAW>
-__device__ void load_queries(const PromptParams& p, Shared& sm, uint32_t base, int64_t works) {
+__device__ void load_queries(const PromptParams& p, const CUtensorMap* map, Shared& sm, uint32_t base, int64_t works) {
   using S = Shape<D, RAW>;
   constexpr uint32_t CPR = D / 8, RPI = 32 / CPR;
   const int lane = threadIdx.x & 31;
@@ -932,26 +942,44 @@ __device__ void load_queries(const PromptParams& p, Shared& sm, uint32_t base, i
     if (loads > 0 && !wait_warp(sm, &sm.bars.q_empty, (loads - 1) & 1)) break;
     ++loads;
     const int rows = pc.rows > kTileRows ? kItemRows : kTileRows;
-#pragma unroll 4
-    for (int r = int(r0); r < rows; r += RPI) {
-      const int pair = pc.row0 + r, token = pair / p.group;
-      const uint16_t* src = p.q + (int64_t(pc.first) + token) * p.q_row + int64_t(head * p.group + pair - token * p.group) * p.q_head + c * 8;
-      const uint32_t to = base + uint32_t(r / kTileRows) * S::kTile + chunk_at(uint32_t(r % kTileRows), c);
-      const bool real = r < pc.rows;
-      if (p.q_wide) {
-        cp_async16_zfill(to, real ? reinterpret_cast<uint64_t>(src) : reinterpret_cast<uint64_t>(p.pieces), real);
-      } else {
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (real)
+    if (p.q_boxes) {  // (rows behind the sequence's are another's, which nobody reads)
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&sm.bars.q_full, uint32_t(rows / kTileRows) * S::kTile);
+        for (int g = 0; g < rows / kTileRows; ++g)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = src[2 * j] | uint32_t(src[2 * j + 1]) << 16;
-        sts128p(to, make_uint4(w[0], w[1], w[2], w[3]));
+          for (int half = 0; half < D / 64; ++half)
+            tma_load_3d_at(base + uint32_t(g) * S::kTile + uint32_t(half) * S::kHalf, map, &sm.bars.q_full, half * 64, head * p.group,
+                           pc.first + (pc.row0 + g * kTileRows) / p.group);
+      }
+      __syncwarp();
+      continue;
+    }
+    for (int block = 0; block < rows; block += 32) {
+      const int pair = pc.row0 + block + lane, token = pair / p.group;
+      const int64_t mine = (int64_t(pc.first) + token) * p.q_row + int64_t(head * p.group + pair - token * p.group) * p.q_head;
+#pragma unroll 4
+      for (int r = int(r0); r < 32; r += RPI) {
+        const uint16_t* src = p.q + __shfl_sync(0xFFFFFFFFu, mine, r) + c * 8;
+        const uint32_t to = base + uint32_t(block / kTileRows) * S::kTile + chunk_at(uint32_t((block + r) % kTileRows), c);
+        const bool real = block + r < pc.rows;
+        if (p.q_wide) {
+          cp_async16_zfill(to, real ? reinterpret_cast<uint64_t>(src) : reinterpret_cast<uint64_t>(p.pieces), real);
+        } else {
+          uint32_t w[4] = {0, 0, 0, 0};
+          if (real)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = src[2 * j] | uint32_t(src[2 * j + 1]) << 16;
+          sts128p(to, make_uint4(w[0], w[1], w[2], w[3]));
+        }
       }
     }
     cp_async_wait_all();
     fence_proxy_async_smem();
     mbar_arrive(&sm.bars.q_full);
   }
+  // (for a call that gives up: the copies on their way)
+  if (p.q_boxes && loads > 0)
+    for (uint32_t k = 0; k < kPollsP && !__all_sync(0xFFFFFFFFu, mbar_try_wait(&sm.bars.q_full, (loads - 1) & 1)); ++k) {}
 }
 
 // ---- products: a warp, whose elected lane issues them
@@ -1305,14 +1333,15 @@ template <int N>
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
 
 template <int D, bool RAW>
-__global__ void __launch_bounds__(Shape<D, RAW>::kThreads, 1) prompt_kernel(const __grid_constant__ PromptParams p) {
+__global__ void __launch_bounds__(Shape<D, RAW>::kThreads, 1) prompt_kernel(const __grid_constant__ PromptParams p,
+                                                                               const __grid_constant__ CUtensorMap queries) {
   extern __shared__ uint8_t smem[];
   __shared__ Shared sm;
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);
   const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
   if (threadIdx.x == 0) {
     PromptBars& b = sm.bars;
-    mbar_init(&b.q_full, 32);
+    mbar_init(&b.q_full, p.q_boxes ? 1 : 32);
     mbar_init(&b.q_empty, 1);
     for (int i = 0; i < 8; ++i) {
       mbar_init(&b.full[i], RAW ? kDecoders : 1);
@@ -1339,7 +1368,7 @@ __global__ void __launch_bounds__(Shape<D, RAW>::kThreads, 1) prompt_kernel(cons
   }
   if (warp < 8) softmax_rows<D, RAW>(p, sm, base, works, warp >> 2);
   else if (warp == 8) issue_products<D, RAW>(p, sm, base, works);
-  else if (warp == 9) load_queries<D, RAW>(p, sm, base, works);
+  else if (warp == 9) load_queries<D, RAW>(p, &queries, sm, base, works);
   else if constexpr (RAW) {
     if (warp < 12) fetch_tiles<D>(p, sm, base, works, warp - 10);
     else decode_tiles<D>(p, sm, base, works);
@@ -1453,8 +1482,19 @@ bool pool_map(CUtensorMap& map, void* any, const PagedKV& kv, int rows) {
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// And one of the queries [n_rows][heads_q][D], boxes of a tile's tokens x the query heads of a key head x 64.
+bool query_map(CUtensorMap& map, const void* q, const PromptParams& p, int D) {
+  auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
+  if (!fn) return false;
+  cuuint64_t dims[3] = {cuuint64_t(D), cuuint64_t(p.heads_q), cuuint64_t(p.n_rows)};
+  cuuint64_t strides[2] = {cuuint64_t(p.q_head) * 2, cuuint64_t(p.q_row) * 2};
+  cuuint32_t box[3] = {64, cuuint32_t(p.group), cuuint32_t(kTileRows / p.group)}, steps[3] = {1, 1, 1};
+  return fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, bool RAW>
-ashkv_status_t launch_prompt(const PromptParams& p, const CUtensorMap& pool, int sms, void* stream) {
+ashkv_status_t launch_prompt(const PromptParams& p, const CUtensorMap& pool, const CUtensorMap& queries, int sms, void* stream) {
   constexpr const char* kName = "ashkv_prompt_attention";
   // the attribute is the kernel's on a device and outlasts the call
   static std::atomic<bool> allowed[64];
@@ -1469,7 +1509,7 @@ ashkv_status_t launch_prompt(const PromptParams& p, const CUtensorMap& pool, int
     return ASHKV_LAUNCH_ERROR;
   }
   launch_paged(prompt_plan_kernel, 1, kPlanThreads, 0, stream, p, pool, kLeastTiles);
-  launch_paged(prompt_kernel<D, RAW>, sms, Shape<D, RAW>::kThreads, Shape<D, RAW>::kBytes, stream, p);
+  launch_paged(prompt_kernel<D, RAW>, sms, Shape<D, RAW>::kThreads, Shape<D, RAW>::kBytes, stream, p, queries);
   const ashkv_status_t rc = check_launch(kName);
   if (rc != ASHKV_OK) return rc;
   launch_paged(prompt_join_kernel<D>, 4 * sms, kJoinThreadsP, 0, stream, p);
@@ -1534,6 +1574,8 @@ extern "C" ashkv_status_t ashkv_prompt_attention(
     while (p.box_rows < kTileKeys && p.kv.T % (2 * p.box_rows) == 0) p.box_rows *= 2;
     if (!pool_map(pool, d_scratch, p.kv, p.box_rows)) p.box_rows = 0;
   }
-  if (kv->head_dim == 64) return p.box_rows ? launch_prompt<64, false>(p, pool, sms, stream) : launch_prompt<64, true>(p, pool, sms, stream);
-  return p.box_rows ? launch_prompt<128, false>(p, pool, sms, stream) : launch_prompt<128, true>(p, pool, sms, stream);
+  CUtensorMap queries{};
+  p.q_boxes = p.q_wide && kTileRows % p.group == 0 && q_row_stride > 0 && q_head_stride > 0 && query_map(queries, d_q, p, kv->head_dim);
+  if (kv->head_dim == 64) return p.box_rows ? launch_prompt<64, false>(p, pool, queries, sms, stream) : launch_prompt<64, true>(p, pool, queries, sms, stream);
+  return p.box_rows ? launch_prompt<128, false>(p, pool, queries, sms, stream) : launch_prompt<128, true>(p, pool, queries, sms, stream);
 }
