@@ -82,7 +82,7 @@ struct PromptParams {
   float* lse;
   // scratch
   int32_t* counts;  // pieces, splits
-  int32_t* prefix;  // [n_seqs + 1] items before a sequence
+  int32_t* prefix;  // [n_seqs + 1] items before a sequence, where there are more of these than the plan holds itself
   Piece* pieces;
   Split* splits;
   int32_t max_pieces, max_parts;  // (per key head)
@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_
   __shared__ int s_warp[32], s_base, s_longest, s_parts, s_splits;
   __shared__ unsigned long long s_tiles;
   __shared__ int s_bin[kBins];
+  __shared__ int32_t s_prefix[kPlanThreads + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) { s_base = 0; s_longest = 1; s_parts = 0; s_splits = 0; s_tiles = 0; }
   if (tid < kBins) s_bin[tid] = 0;
@@ -159,6 +160,7 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_
     release_map();
   }
   const int n_seqs = p.lists.n_seqs;
+  int32_t* prefix = n_seqs <= kPlanThreads ? s_prefix : p.prefix;  // items before a sequence
   bool bad = false;
   for (int b0 = 0; b0 < n_seqs; b0 += kPlanThreads) {
     const int b = b0 + tid;
@@ -189,13 +191,13 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_
     }
     __syncthreads();
     const int before = s_base + (warp ? s_warp[warp - 1] : 0) + upto - n;
-    if (b < n_seqs) p.prefix[b] = before;
+    if (b < n_seqs) prefix[b] = before;
     __syncthreads();
     if (tid == 0) s_base += s_warp[31];
     __syncthreads();
   }
   const int items = s_base;
-  if (tid == 0) p.prefix[n_seqs] = items;
+  if (tid == 0) prefix[n_seqs] = items;
   if (__syncthreads_or(bad)) {  // rows that two sequences claim: nothing is computed
     if (tid == 0) {
       p.counts[0] = p.counts[1] = 0;
@@ -203,19 +205,31 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_
     }
     return;
   }
-  const auto item = [&](int i, int& b) {
-    b = seq_of_item(p.prefix, n_seqs, i);
-    return item_of(p, b, i - p.prefix[b]);
+  const auto find = [&](int i, int& b) {
+    b = seq_of_item(prefix, n_seqs, i);
+    return item_of(p, b, i - prefix[b]);
   };
   unsigned long long tiles = 0;
-  int longest = 1, b;
+  int longest = 1, b, own_b = 0;
+  Item own{};  // a thread's first is kept
+  if (tid < items) own = find(tid, own_b);
+  const auto item = [&](int i, int& b) {
+    if (i != tid) return find(i, b);
+    b = own_b;
+    return own;
+  };
   for (int i = tid; i < items; i += kPlanThreads) {
     const Item it = item(i, b);
     tiles += it.n;
     longest = max(longest, it.n);
   }
-  atomicAdd(&s_tiles, tiles);
-  atomicMax(&s_longest, longest);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) tiles += __shfl_xor_sync(0xFFFFFFFFu, tiles, off);
+  longest = __reduce_max_sync(0xFFFFFFFFu, longest);
+  if (lane == 0 && tiles) {
+    atomicAdd(&s_tiles, tiles);
+    atomicMax(&s_longest, longest);
+  }
   __syncthreads();
   const unsigned long long all = s_tiles * p.kv.heads_kv;
   const int share = int(min((unsigned long long)0x40000000, max((unsigned long long)least, (all + p.share - 1) / p.share)));
@@ -1512,6 +1526,7 @@ ashkv_status_t launch_prompt(const PromptParams& p, const CUtensorMap& pool, con
   launch_paged(prompt_kernel<D, RAW>, sms, Shape<D, RAW>::kThreads, Shape<D, RAW>::kBytes, stream, p, queries);
   const ashkv_status_t rc = check_launch(kName);
   if (rc != ASHKV_OK) return rc;
+  if (int64_t(p.lists.max_pages) * p.kv.T <= kLeastTiles * kTileKeys) return ASHKV_OK;  // nothing is long enough to be cut
   launch_paged(prompt_join_kernel<D>, 4 * sms, kJoinThreadsP, 0, stream, p);
   return check_launch(kName);
 }
