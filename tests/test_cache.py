@@ -1,4 +1,4 @@
-"""Writing and reading tiered pages, and windows, without a GPU: refused arguments at the C boundary,
+"""Writing, reading and attending tiered pages, without a GPU: refused arguments at the C boundary,
 and the sources' promises."""
 from __future__ import annotations
 
@@ -68,6 +68,39 @@ def test_window_refusals():
     assert decode(n=0, q=None) == N.OK
 
 
+def test_prompt_refusals():
+    def prompt(**change):
+        a = dict(q=X, qs=1024, qh=128, n=3, hq=8, ids=X, ids_stride=4, pages=4, lengths=X, starts=X, seqs=1, window=0, sinks=0,
+                 scale=1.0, out=X, lse=None, scratch=X, status=None, stream=None)
+        kv = change.pop("kv", desc())
+        a.update(change)
+        return N.lib().ashkv_prompt_attention(None if kv is None else ctypes.addressof(kv), *a.values())
+
+    assert prompt(kv=None) == N.BAD_ARGUMENT
+    for bad in (dict(head_dim=32), dict(head_dim=96), dict(heads_kv=0), dict(tokens_per_page=0), dict(row_stride=248), dict(d_tier=None)):
+        assert prompt(kv=desc(**bad)) == N.BAD_ARGUMENT, bad
+    for bad in (dict(hq=0), dict(hq=7), dict(hq=16384), dict(n=-1), dict(n=2 ** 28), dict(seqs=-1), dict(pages=-1), dict(ids_stride=3),
+                dict(window=-1), dict(sinks=-1, window=1), dict(sinks=1), dict(q=None), dict(out=None), dict(scratch=None),
+                dict(q=ctypes.c_void_p(257)), dict(out=ctypes.c_void_p(264)), dict(scratch=ctypes.c_void_p(260)),
+                dict(lengths=None), dict(starts=None), dict(ids=None)):
+        assert prompt(**bad) == N.BAD_ARGUMENT, bad
+        assert b"ashkv_prompt_attention" in N.lib().ashkv_last_error()
+    assert prompt(n=0, q=None, out=None, scratch=None) == N.OK and prompt(seqs=0, lengths=None, starts=None) == N.OK
+
+
+def test_prompt_scratch():
+    size = N.lib().ashkv_prompt_scratch_floats
+    for bad in ((-1, 1, 8, 2, 128, 1), (1, -1, 8, 2, 128, 1), (1, 1, 0, 2, 128, 1), (1, 1, 8, 0, 128, 1), (1, 1, 7, 2, 128, 1),
+                (1, 1, 8, 2, 0, 1), (1, 1, 8, 2, 128, 0)):
+        assert size(*bad) == -1, bad
+    # a row of results in fp32 and its sum for each place that a cut item can have, of at most 256 rows
+    assert 0 < size(1, 1, 8, 2, 128, 1) < 2 ** 20
+    assert size(8192, 1, 32, 8, 128, 1) < 2 ** 25
+    assert size(300, 1, 8, 2, 128, 1) < 2 ** 27
+    for n in (1, 40, 8192, 1 << 20):  # more of anything needs no less within a rule of cutting
+        assert size(n, 2, 8, 2, 128, 1) <= size(n, 2, 8, 2, 128, 9)
+
+
 def test_kernels_over_page_lists_promise_nothing_of_what_they_read():
     """launch_paged overlaps a kernel with the one before it, as launch_overlapped does: the same rules."""
     csrc = Path(__file__).resolve().parent.parent / "ash-kv_b200" / "csrc"
@@ -79,4 +112,4 @@ def test_kernels_over_page_lists_promise_nothing_of_what_they_read():
         seen.append(f.name)
         for word in ("__restrict__", "ld_nc", "__ldg", "ld.global.nc"):
             assert word not in code, f"{f.name}: {word}"
-    assert "cache.cu" in seen
+    assert {"cache.cu", "prompt.cu"} <= set(seen)
