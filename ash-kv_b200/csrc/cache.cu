@@ -10,6 +10,7 @@
 // a chain of loads that the loads of a written token's rows do not wait for, then encodes or
 // decodes K and V in chunks of eight values a lane.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "page_codec.cuh"
@@ -46,21 +47,32 @@ __device__ __forceinline__ uint4 load_chunk(const uint16_t* row, int64_t head_st
   return make_uint4(x[0] | uint32_t(x[1]) << 16, x[2] | uint32_t(x[3]) << 16, x[4] | uint32_t(x[5]) << 16, x[6] | uint32_t(x[7]) << 16);
 }
 
-// The place of row i's token (warp-collective): its page, and its token there.  False: no such row or page.
-__device__ __forceinline__ bool token_of(const PagedKV& kv, const PageLists& l, int64_t i, Place& at, int& t, bool& row_of_none) {
+// The place of a row's token: its page, and its token there.  `real`: there are such; `none`: the row is of no sequence.
+struct Token {
+  Place at{-1, nullptr, nullptr};
+  int t = 0;
+  bool real = false, none = true;
+  int64_t end = 0;  // of the sequence's rows
+};
+// That of row i (warp-collective), after that of the row before or none.
+__device__ __forceinline__ void go_to(Token& x, const PagedKV& kv, const PageLists& l, int64_t i) {
+  if (x.real && i < x.end && x.t + 1 < kv.T) {
+    ++x.t;
+    return;
+  }
+  x = Token{};
   const int b = sequence_of(l, i);
-  row_of_none = b < 0;
-  if (b < 0) return false;
-  const int64_t pos = int64_t(l.lengths[b]) - (int64_t(l.starts[b + 1]) - i);
-  at.format = -1;
+  if (b < 0) return;
+  x.none = false;
+  x.end = l.starts[b + 1];
+  const int64_t pos = int64_t(l.lengths[b]) - (x.end - i);
   if (pos >= 0) {
     const int64_t j = pos / kv.T;
-    t = int(pos - j * kv.T);
-    if (j < l.max_pages) at = place_of(kv, l.page_ids[int64_t(b) * l.page_ids_stride + j]);
+    x.t = int(pos - j * kv.T);
+    if (j < l.max_pages) x.at = place_of(kv, l.page_ids[int64_t(b) * l.page_ids_stride + j]);
   }
-  if (at.format >= 0) return true;
-  if ((threadIdx.x & 31) == 0) flag(l.status, ASHKV_FLAG_INDEX_RANGE);
-  return false;
+  x.real = x.at.format >= 0;
+  if (!x.real && (threadIdx.x & 31) == 0) flag(l.status, ASHKV_FLAG_INDEX_RANGE);
 }
 
 // Rows of ROW values by TEAM lanes, N chunks a lane (chunk j * TEAM + the lane's place).  With 16
@@ -113,37 +125,46 @@ __device__ __forceinline__ void encode_row(const PagedKV& p, const Place& at, in
 }
 
 // Bound by HBM (reads 4 bytes, writes 1 to 4 a pair of values) and, for few rows, by the chain of loads
-// that finds a page.
-template <int ROW>
+// that finds a page.  A warp takes R rows: one where these are few, four neighbours, which mostly share a page and its look-up,
+// where they fill the device all the same.
+template <int ROW, int R>
 __global__ void __launch_bounds__(kThreadsC) write_kv_kernel(const __grid_constant__ WriteParams p) {
   constexpr int TEAM = RowShape<ROW>::kTeam, N = RowShape<ROW>::kChunks, PASSES = RowShape<ROW>::kPasses;
   const int lane = threadIdx.x & 31, lin = lane % TEAM;
-  const int64_t i = int64_t(blockIdx.x) * (kThreadsC / 32) + (threadIdx.x >> 5);
+  const int64_t first = (int64_t(blockIdx.x) * (kThreadsC / 32) + (threadIdx.x >> 5)) * R;
   wait_for_previous();
   allow_next();
-  if (i >= p.n_rows) return;
-  uint32_t w[PASSES][4 * N];
+  if (first >= p.n_rows) return;
+  uint32_t w[R][PASSES][4 * N];
+  const auto load = [&](int64_t i, uint32_t (&to)[PASSES][4 * N]) {
 #pragma unroll
-  for (int half = 0; half < PASSES; ++half) {
-    const bool v = PASSES == 2 ? half : lane >= TEAM;
-    const uint16_t* row = v ? p.v + i * p.v_row : p.k + i * p.k_row;
+    for (int half = 0; half < PASSES; ++half) {
+      const bool v = PASSES == 2 ? half : lane >= TEAM;
+      const uint16_t* row = v ? p.v + i * p.v_row : p.k + i * p.k_row;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      const uint4 x = load_chunk(row, v ? p.v_head : p.k_head, p.head_dim, (c * TEAM + lin) * 8, p.wide);
-      w[half][4 * c] = x.x; w[half][4 * c + 1] = x.y; w[half][4 * c + 2] = x.z; w[half][4 * c + 3] = x.w;
+      for (int c = 0; c < N; ++c) {
+        const uint4 x = load_chunk(row, v ? p.v_head : p.k_head, p.head_dim, (c * TEAM + lin) * 8, p.wide);
+        to[half][4 * c] = x.x; to[half][4 * c + 1] = x.y; to[half][4 * c + 2] = x.z; to[half][4 * c + 3] = x.w;
+      }
     }
-  }
-  Place at;
-  int t;
-  bool none;
-  if (!token_of(p.kv, p.lists, i, at, t, none)) return;
-  if (at.format >= ASHKV_PAGE_NBIT4) {  // a dithered page is coded as a whole
-    if (lane == 0) flag(p.lists.status, ASHKV_FLAG_INDEX_RANGE);
-    return;
-  }
+  };
 #pragma unroll
-  for (int half = 0; half < PASSES; ++half)
-    encode_row<ROW>(p.kv, at, t + ((PASSES == 2 ? half : lane >= TEAM) ? p.kv.T : 0), lin, w[half]);
+  for (int r = 0; r < R; ++r)
+    if (first + r < p.n_rows) load(first + r, w[r]);
+  Token x;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (first + r >= p.n_rows) return;
+    go_to(x, p.kv, p.lists, first + r);
+    if (!x.real) continue;
+    if (x.at.format >= ASHKV_PAGE_NBIT4) {  // a dithered page is coded as a whole
+      if (lane == 0) flag(p.lists.status, ASHKV_FLAG_INDEX_RANGE);
+      continue;
+    }
+#pragma unroll
+    for (int half = 0; half < PASSES; ++half)
+      encode_row<ROW>(p.kv, x.at, x.t + ((PASSES == 2 ? half : lane >= TEAM) ? p.kv.T : 0), lin, w[r][half]);
+  }
 }
 
 // Rows of any multiple of eight values, without stores: copies into the pool.
@@ -153,14 +174,13 @@ __global__ void __launch_bounds__(kThreadsC) write_pool_kernel(const __grid_cons
   wait_for_previous();
   allow_next();
   if (i >= p.n_rows) return;
-  Place at;
-  int t;
-  bool none;
-  if (!token_of(p.kv, p.lists, i, at, t, none)) return;
-  const int64_t off = int64_t(t) * p.kv.row_stride * 2;
+  Token x;
+  go_to(x, p.kv, p.lists, i);
+  if (!x.real) return;
+  const int64_t off = int64_t(x.t) * p.kv.row_stride * 2;
   for (int half = 0; half < 2; ++half) {
     const uint16_t* row = half ? p.v + i * p.v_row : p.k + i * p.k_row;
-    uint4* to = reinterpret_cast<uint4*>((half ? at.v : at.k) + off);
+    uint4* to = reinterpret_cast<uint4*>((half ? x.at.v : x.at.k) + off);
 #pragma unroll 4
     for (int c = lane; c < p.kv.row_len / 8; c += 32)
       to[c] = load_chunk(row, half ? p.v_head : p.k_head, p.head_dim, c * 8, p.wide);
@@ -179,83 +199,87 @@ __device__ __forceinline__ void overlay_row(const PagedKV& p, const uint8_t* slo
   }
 }
 
-template <int ROW>
+// Bound as writing is, but that a row's loads wait for its look-up.
+template <int ROW, int R>
 __global__ void __launch_bounds__(kThreadsC) read_kv_kernel(const __grid_constant__ ReadParams p) {
   constexpr int TEAM = RowShape<ROW>::kTeam, N = RowShape<ROW>::kChunks, PASSES = RowShape<ROW>::kPasses;
   const int lane = threadIdx.x & 31, lin = lane % TEAM;
-  const int64_t i = int64_t(blockIdx.x) * (kThreadsC / 32) + (threadIdx.x >> 5);
+  const int64_t first = (int64_t(blockIdx.x) * (kThreadsC / 32) + (threadIdx.x >> 5)) * R;
   wait_for_previous();
   allow_next();
-  if (i >= p.n_rows) return;
-  Place at;
-  int t;
-  bool none;
-  const bool real = token_of(p.kv, p.lists, i, at, t, none);
-  if (none) return;
-  const PagedKV& kv = p.kv;
-  const int T = kv.T;
-  const int64_t E = 2 * int64_t(T) * ROW;
-  uint4 x[PASSES][N];
-  const auto row_of = [&](int half) { return t + ((PASSES == 2 ? half != 0 : lane >= TEAM) ? T : 0); };
-  const auto each = [&](auto decode) {  // decode(row of the page, chunk)
+  Token token;
+#pragma unroll 1
+  for (int64_t i = first; i < min(first + R, p.n_rows); ++i) {
+    go_to(token, p.kv, p.lists, i);
+    if (token.none) continue;
+    const Place at = token.at;
+    const int t = token.t;
+    const bool real = token.real;
+    const PagedKV& kv = p.kv;
+    const int T = kv.T;
+    const int64_t E = 2 * int64_t(T) * ROW;
+    uint4 x[PASSES][N];
+    const auto row_of = [&](int half) { return t + ((PASSES == 2 ? half != 0 : lane >= TEAM) ? T : 0); };
+    const auto each = [&](auto decode) {  // decode(row of the page, chunk)
 #pragma unroll
-    for (int half = 0; half < PASSES; ++half)
+      for (int half = 0; half < PASSES; ++half)
 #pragma unroll
-      for (int c = 0; c < N; ++c) x[half][c] = decode(row_of(half), c * TEAM + lin);
-  };
-  if (!real) {
-    each([&](int, int) { return make_uint4(0, 0, 0, 0); });
-  } else if (at.format == ASHKV_PAGE_BF16) {
-    each([&](int r, int c) {
-      const bool v = r >= T;
-      return ld_v4((v ? at.v : at.k) + (int64_t(v ? r - T : r) * kv.row_stride + c * 8) * 2);
-    });
-  } else if (at.format == ASHKV_PAGE_INT8) {
-    const uint8_t* codes = at.k + int8_codes_offset(T);
-    uint2 q[PASSES][N];
-    float s[PASSES];
+        for (int c = 0; c < N; ++c) x[half][c] = decode(row_of(half), c * TEAM + lin);
+    };
+    if (!real) {
+      each([&](int, int) { return make_uint4(0, 0, 0, 0); });
+    } else if (at.format == ASHKV_PAGE_BF16) {
+      each([&](int r, int c) {
+        const bool v = r >= T;
+        return ld_v4((v ? at.v : at.k) + (int64_t(v ? r - T : r) * kv.row_stride + c * 8) * 2);
+      });
+    } else if (at.format == ASHKV_PAGE_INT8) {
+      const uint8_t* codes = at.k + int8_codes_offset(T);
+      uint2 q[PASSES][N];
+      float s[PASSES];
 #pragma unroll
-    for (int half = 0; half < PASSES; ++half) {
-      s[half] = f16_to_f32(reinterpret_cast<const uint16_t*>(at.k)[row_of(half)]);
+      for (int half = 0; half < PASSES; ++half) {
+        s[half] = f16_to_f32(reinterpret_cast<const uint16_t*>(at.k)[row_of(half)]);
 #pragma unroll
-      for (int c = 0; c < N; ++c) q[half][c] = *reinterpret_cast<const uint2*>(codes + int64_t(row_of(half)) * ROW + (c * TEAM + lin) * 8);
+        for (int c = 0; c < N; ++c) q[half][c] = *reinterpret_cast<const uint2*>(codes + int64_t(row_of(half)) * ROW + (c * TEAM + lin) * 8);
+      }
+#pragma unroll
+      for (int half = 0; half < PASSES; ++half)
+#pragma unroll
+        for (int c = 0; c < N; ++c) x[half][c] = int8_dec8(q[half][c], s[half]);
+    } else if (at.format == ASHKV_PAGE_FP8) {
+      each([&](int r, int c) { return fp8_dec8(*reinterpret_cast<const uint2*>(at.k + int64_t(r) * ROW + c * 8)); });
+    } else if (at.format == ASHKV_PAGE_INT4) {
+      each([&](int r, int c) {
+        return int4_dec8(*reinterpret_cast<const uint32_t*>(at.k + E / 32 + int64_t(r) * (ROW / 2) + c * 4),
+                         reinterpret_cast<const uint16_t*>(at.k)[r * (ROW / 64) + c / 8]);
+      });
+    } else if (at.format == ASHKV_PAGE_NBIT4) {
+      each([&](int r, int c) {
+        const int64_t g = int64_t(r) * (ROW / 8) + c;  // chunk of the page
+        return nbit_dec8<4>(*reinterpret_cast<const uint32_t*>(at.k + nbit_codes_off(E) + g * 4),
+                            reinterpret_cast<const uint16_t*>(at.k + nbit_delta_off())[g / 4]);
+      });
+    } else {
+      each([&](int r, int c) {
+        const int64_t g = int64_t(r) * (ROW / 8) + c;
+        return nbit_dec8<2>(*reinterpret_cast<const uint16_t*>(at.k + nbit_codes_off(E) + g * 2),
+                            reinterpret_cast<const uint16_t*>(at.k + nbit_delta_off())[g / 4]);
+      });
     }
 #pragma unroll
-    for (int half = 0; half < PASSES; ++half)
+    for (int half = 0; half < PASSES; ++half) {
+      uint16_t* out = (PASSES == 2 ? half != 0 : lane >= TEAM) ? p.v + i * ROW : p.k + i * ROW;
 #pragma unroll
-      for (int c = 0; c < N; ++c) x[half][c] = int8_dec8(q[half][c], s[half]);
-  } else if (at.format == ASHKV_PAGE_FP8) {
-    each([&](int r, int c) { return fp8_dec8(*reinterpret_cast<const uint2*>(at.k + int64_t(r) * ROW + c * 8)); });
-  } else if (at.format == ASHKV_PAGE_INT4) {
-    each([&](int r, int c) {
-      return int4_dec8(*reinterpret_cast<const uint32_t*>(at.k + E / 32 + int64_t(r) * (ROW / 2) + c * 4),
-                       reinterpret_cast<const uint16_t*>(at.k)[r * (ROW / 64) + c / 8]);
-    });
-  } else if (at.format == ASHKV_PAGE_NBIT4) {
-    each([&](int r, int c) {
-      const int64_t g = int64_t(r) * (ROW / 8) + c;  // chunk of the page
-      return nbit_dec8<4>(*reinterpret_cast<const uint32_t*>(at.k + nbit_codes_off(E) + g * 4),
-                          reinterpret_cast<const uint16_t*>(at.k + nbit_delta_off())[g / 4]);
-    });
-  } else {
-    each([&](int r, int c) {
-      const int64_t g = int64_t(r) * (ROW / 8) + c;
-      return nbit_dec8<2>(*reinterpret_cast<const uint16_t*>(at.k + nbit_codes_off(E) + g * 2),
-                          reinterpret_cast<const uint16_t*>(at.k + nbit_delta_off())[g / 4]);
-    });
-  }
-#pragma unroll
-  for (int half = 0; half < PASSES; ++half) {
-    uint16_t* out = (PASSES == 2 ? half != 0 : lane >= TEAM) ? p.v + i * ROW : p.k + i * ROW;
-#pragma unroll
-    for (int c = 0; c < N; ++c) st_cs_v4(out + (c * TEAM + lin) * 8, x[half][c]);
-  }
-  if (real && at.format >= ASHKV_PAGE_NBIT4) {
-    __syncwarp();  // the decoded values lie under the outliers
-    for (int half = 0; half < 2; ++half) {
-      uint16_t* out = half ? p.v + i * ROW : p.k + i * ROW;
-      if (at.format == ASHKV_PAGE_NBIT4) overlay_row<4>(kv, at.k, E, t + half * T, out);
-      else overlay_row<2>(kv, at.k, E, t + half * T, out);
+      for (int c = 0; c < N; ++c) st_cs_v4(out + (c * TEAM + lin) * 8, x[half][c]);
+    }
+    if (real && at.format >= ASHKV_PAGE_NBIT4) {
+      __syncwarp();  // the decoded values lie under the outliers
+      for (int half = 0; half < 2; ++half) {
+        uint16_t* out = half ? p.v + i * ROW : p.k + i * ROW;
+        if (at.format == ASHKV_PAGE_NBIT4) overlay_row<4>(kv, at.k, E, t + half * T, out);
+        else overlay_row<2>(kv, at.k, E, t + half * T, out);
+      }
     }
   }
 }
@@ -266,13 +290,12 @@ __global__ void __launch_bounds__(kThreadsC) read_pool_kernel(const __grid_const
   wait_for_previous();
   allow_next();
   if (i >= p.n_rows) return;
-  Place at;
-  int t;
-  bool none;
-  const bool real = token_of(p.kv, p.lists, i, at, t, none);
-  if (none) return;
+  Token x;
+  go_to(x, p.kv, p.lists, i);
+  if (x.none) return;
+  const bool real = x.real;
   for (int half = 0; half < 2; ++half) {
-    const uint8_t* from = (half ? at.v : at.k) + (real ? int64_t(t) * p.kv.row_stride * 2 : 0);
+    const uint8_t* from = (half ? x.at.v : x.at.k) + (real ? int64_t(x.t) * p.kv.row_stride * 2 : 0);
     uint16_t* out = (half ? p.v : p.k) + i * p.kv.row_len;
 #pragma unroll 4
     for (int c = lane; c < p.kv.row_len / 8; c += 32)
@@ -280,7 +303,25 @@ __global__ void __launch_bounds__(kThreadsC) read_pool_kernel(const __grid_const
   }
 }
 
-int64_t blocks_of(int64_t n_rows) { return (n_rows + kThreadsC / 32 - 1) / (kThreadsC / 32); }
+// Calls use with the kernels' row length that is `row`, if there is one.
+template <typename F>
+void by_row(int64_t row, F use) {
+  switch (row) {
+    case 128: use(std::integral_constant<int, 128>()); break;
+    case 256: use(std::integral_constant<int, 256>()); break;
+    case 512: use(std::integral_constant<int, 512>()); break;
+    case 1024: use(std::integral_constant<int, 1024>()); break;
+    case 2048: use(std::integral_constant<int, 2048>()); break;
+  }
+}
+// Rows of a warp where there are many: four short ones, whose look-ups take longer than their bytes.  262144 rows in us, one and
+// four to a warp: written 128 (FP8) 158 and 111, 256 (INT8) 246 and 219, 512 (INT8) 350 and 410; read 128 76 and 62, 256 113
+// and 99, 512 163 and 148; 131072 of 1024 read 177 and 190.
+template <int ROW>
+constexpr int kWriteRows = ROW <= 256 ? 4 : 1;
+template <int ROW>
+constexpr int kReadRows = ROW <= 512 ? 4 : 1;
+int64_t blocks_of(int64_t n_rows, int64_t rows) { return (n_rows + kThreadsC / 32 * rows - 1) / (kThreadsC / 32 * rows); }
 
 }  // namespace
 }  // namespace ashkv
@@ -306,14 +347,13 @@ extern "C" ashkv_status_t ashkv_write_kv(const ashkv_paged_kv_t* kv, const void*
   p.wide = aligned(d_k, 16) && aligned(d_v, 16) && k_row_stride % 8 == 0 && v_row_stride % 8 == 0 && k_head_stride % 8 == 0 &&
            v_head_stride % 8 == 0;
   void (*kernel)(WriteParams) = write_pool_kernel;
-  switch (p.kv.row_len) {
-    case 128: kernel = write_kv_kernel<128>; break;
-    case 256: kernel = write_kv_kernel<256>; break;
-    case 512: kernel = write_kv_kernel<512>; break;
-    case 1024: kernel = write_kv_kernel<1024>; break;
-    case 2048: kernel = write_kv_kernel<2048>; break;
-  }
-  launch_paged(kernel, blocks_of(n_rows), kThreadsC, 0, stream, p);
+  const bool many = n_rows >= int64_t(sm_count() > 0 ? sm_count() : 148) * 64 * 4;  // (64 warps to an SM)
+  int rows = 1;
+  by_row(p.kv.row_len, [&](auto row) {
+    kernel = many ? write_kv_kernel<row(), kWriteRows<row()>> : write_kv_kernel<row(), 1>;
+    rows = many ? kWriteRows<row()> : 1;
+  });
+  launch_paged(kernel, blocks_of(n_rows, rows), kThreadsC, 0, stream, p);
   return check_launch(kName);
 }
 
@@ -331,13 +371,12 @@ extern "C" ashkv_status_t ashkv_read_kv(const ashkv_paged_kv_t* kv, const int32_
   p.n_rows = n_rows;
   p.k = static_cast<uint16_t*>(d_k); p.v = static_cast<uint16_t*>(d_v);
   void (*kernel)(ReadParams) = read_pool_kernel;
-  switch (p.kv.row_len) {
-    case 128: kernel = read_kv_kernel<128>; break;
-    case 256: kernel = read_kv_kernel<256>; break;
-    case 512: kernel = read_kv_kernel<512>; break;
-    case 1024: kernel = read_kv_kernel<1024>; break;
-    case 2048: kernel = read_kv_kernel<2048>; break;
-  }
-  launch_paged(kernel, blocks_of(n_rows), kThreadsC, 0, stream, p);
+  const bool many = n_rows >= int64_t(sm_count() > 0 ? sm_count() : 148) * 64 * 4;  // (64 warps to an SM)
+  int rows = 1;
+  by_row(p.kv.row_len, [&](auto row) {
+    kernel = many ? read_kv_kernel<row(), kReadRows<row()>> : read_kv_kernel<row(), 1>;
+    rows = many ? kReadRows<row()> : 1;
+  });
+  launch_paged(kernel, blocks_of(n_rows, rows), kThreadsC, 0, stream, p);
   return check_launch(kName);
 }

@@ -151,6 +151,69 @@ def test_write_many_sequences(cuda):
     write_case(cuda, WRITES["int8"], 16, 2, 64, [m + i % 20 for i, m in enumerate(new)], new, 4)
 
 
+@pytest.mark.parametrize("heads,dim,T", [(2, 64, 8), (4, 64, 16), (4, 128, 4)])
+def test_many_rows(cuda, heads, dim, T):
+    """Enough rows that a warp takes several: they may cross pages and sequences, follow a page that does not exist, and end early."""
+    lengths, seqs = 20000 + 3, 2
+    P = -(-lengths // T)
+    n = 64  # (each stands in many places of the lists)
+    c = Cache(cuda, FORMATS["mixed"] * (n // 4), T, heads, dim, 20)
+    g = np.random.default_rng(20)
+    ids = g.integers(0, n, (seqs, P)).astype(np.int32)
+    ids[1, 5::7] = n + 3
+    new = [20001, 19990]
+    args = (c.table, c.kv, c.stores, i32(ids, cuda), i32([lengths, lengths - 2], cuda), i32(starts_of(new) + 1, cuda), sum(new) + 5)
+    out = tuple(torch.full((args[-1], heads, dim), 5.0, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    C.read_kv(*args, tokens_per_page=T, out=out, status=status)
+    assert int(status) & N.FLAG_INDEX_RANGE
+    pages = np.zeros((n + 4, 2, T, heads * dim), np.uint16)
+    for i in range(n):
+        pages[i] = page_bits_of(c, i)
+    for side in range(2):
+        got = bits(out[side]).reshape(-1, heads * dim)
+        assert (bits(out[side][:1]) == 0x40A0).all() and (got[1 + sum(new):] == 0x40A0).all()
+        at = 1
+        for b, (length, m) in enumerate(zip((lengths, lengths - 2), new)):
+            pos = np.arange(length - m, length)
+            want = pages[np.minimum(ids[b, pos // T], n + 3), side, pos % T]
+            assert np.array_equal(got[at:at + m], want)
+            at += m
+
+
+@pytest.mark.parametrize("heads,dim,T,tiers", [(2, 64, 8, "bf16"), (2, 64, 16, "int8"), (4, 64, 16, "int4"), (4, 64, 4, "fp8")])
+def test_write_many_rows(cuda, heads, dim, T, tiers):
+    """As many rows written, each to a place of its own, as a few at a time write them."""
+    seqs, length = 5, 8001
+    P = -(-length // T)
+    caches = []
+    n = seqs * length
+    k, v = new_rows(n, heads, dim, cuda, 21)
+    ids = i32(np.random.default_rng(21).permutation(seqs * P).reshape(seqs, P), cuda)
+    row = heads * dim
+    fmt = FORMATS[tiers][0]
+    for step in (n, 8001):
+        z = torch.zeros(seqs * P, device=cuda)
+        tier = torch.full((seqs * P,), TIER.get(fmt, 0), dtype=torch.int8, device=cuda)
+        own = torch.arange(seqs * P, dtype=torch.int32, device=cuda)
+        table = DevicePageTable(z, z, z, z, tier, torch.zeros_like(own), torch.zeros_like(own), own * T, own)
+        pool = [torch.zeros(seqs * P * T, heads, dim, dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+        stores = {} if fmt == N.PAGE_BF16 else {TIER[fmt]: TierStore(fmt, seqs * P, cuda, T, row)}
+        for s in stores.values():
+            s.data.zero_()
+        kv = KVLayers(pool[:1], pool[1:])
+        for b in range(0, n, step):
+            m = min(step, n - b)
+            one = slice(b // length, (b + m) // length)
+            C.write_kv(k[b:b + m], v[b:b + m], table, kv, stores, ids[one].contiguous(), i32([length] * (m // length), cuda),
+                       i32(starts_of([length] * (m // length)), cuda), tokens_per_page=T)
+        caches.append((pool, [s.data for s in stores.values()]))
+    (pool, data), (pool1, data1) = caches
+    for a, b in zip(pool + data, pool1 + data1):
+        assert torch.equal(a, b)
+    assert any(bool((x != 0).any()) for x in pool + data)
+
+
 @pytest.mark.parametrize("heads,dim", [(3, 40), (5, 64), (1, 8), (1, 3000)])
 def test_rows_of_any_size_in_the_pool(cuda, heads, dim):
     dev, T, n = cuda, 4, 40
