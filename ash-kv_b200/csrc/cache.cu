@@ -199,9 +199,10 @@ __device__ __forceinline__ void overlay_row(const PagedKV& p, const uint8_t* slo
   }
 }
 
-// Bound as writing is, but that a row's loads wait for its look-up.
+// Bound as writing is, but that a row's loads wait for its look-up: warps in flight count, so long rows are kept to the registers of
+// five blocks to an SM (131072 rows of 1024, mixed formats: 178 -> 166 us, 4.8 TB/s; with six, which spill, the same).
 template <int ROW, int R>
-__global__ void __launch_bounds__(kThreadsC) read_kv_kernel(const __grid_constant__ ReadParams p) {
+__global__ void __launch_bounds__(kThreadsC, ROW >= 512 ? 5 : 1) read_kv_kernel(const __grid_constant__ ReadParams p) {
   constexpr int TEAM = RowShape<ROW>::kTeam, N = RowShape<ROW>::kChunks, PASSES = RowShape<ROW>::kPasses;
   const int lane = threadIdx.x & 31, lin = lane % TEAM;
   const int64_t first = (int64_t(blockIdx.x) * (kThreadsC / 32) + (threadIdx.x >> 5)) * R;
