@@ -9,15 +9,25 @@
 // takes them unrounded.
 //
 // Rows: the (token, query head) pairs of a key head, token by token; an item is 256 of them, two
-// tiles of 128 that share the key tiles of 128 tokens.  A plan kernel lists the items, cuts those of
-// more key tiles than a CTA's share into pieces, and sorts them by length; the CTAs of the main
-// kernel, one to an SM, take them in turn; a join kernel weighs the partial results of cut items.
+// tiles of 128 that share the key tiles of 128 tokens.  A plan kernel lists the items, cuts long ones
+// into pieces where the items alone would leave CTAs idle, and sorts them by length; the CTAs of the
+// main kernel, one to an SM, take them in turn; a join kernel weighs the partial results of cut items.
+// No result depends on the order in which the plan's atomics hand out places.
 //
-// A CTA: two softmax warpgroups, a tile each, a thread to a row (its 128 scores come from TMEM as
-// registers and go back as bf16 weights over the scores' columns); four warps that bring K and V tiles
-// into shared memory, decoding them where a page is compressed; three warps that look the pages
-// up; one that issues the products.  While one tile's scores become weights the tensor cores work
-// on the other's.
+// A CTA: two softmax warpgroups, a tile of rows each, a thread to a row (its scores come from TMEM
+// and go back as bf16 weights over the scores' columns, where the second product reads them); a warp
+// that issues the products; one that loads queries.  While one tile's scores become weights the tensor cores work on
+// the other's.  Where all pages are in the pool a warp sends tensor copies of 64 channels x a page's tokens
+// and another looks for values that are not finite where they must not be seen; where pages are compressed, or no box of
+// a page fits the tile, two warps look pages up and copy codes, and eight decode them into the tiles.
+//
+// What bounds it.  A tile pair costs the tensor cores 16.8 MFLOP, 1.5 us at the rate that a large matrix product
+// reaches, and the special function units 32768 exponentials, 1.1 us; the pair takes 2.2 us: the chain
+// scores -> weights -> product of one tile of rows does not quite fit beside the other's.  Figures (B200, graph replays,
+// 32 query heads over 8 of 128): 8192 rows of one prompt 488 us, 0.68 of that rate (tensor pipe busy 54 % of the cycles
+// under a profiler's clocks); 40 rows over 300 tokens 21 us, of which the plan takes 7; 4 x 2048 rows of 64 heads over INT8
+// pages, window 4096, 675 us (decoding beside the softmax: issue slots and instruction caches); 32 x 5 rows over 8192
+// tokens of FP8 351 us, of bf16 254 (128 rows are computed for 20).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -86,7 +96,7 @@ struct PromptParams {
   Piece* pieces;
   Split* splits;
   int32_t max_pieces, max_parts;  // (per key head)
-  int32_t share;                  // pieces to aim for over all key heads
+  int32_t share;                  // pieces to aim for over all key heads, at most
   float* part_o;     // [max_parts * heads_kv][part_rows][D], each divided by its sum
   float* part_lse2;  // [max_parts * heads_kv][part_rows]
   int32_t part_rows;
@@ -134,7 +144,7 @@ __device__ __forceinline__ int seq_of_item(const int32_t* prefix, int n_seqs, in
   return lo;
 }
 
-// One CTA.  Counts the items of each sequence, then their key tiles; cuts what is longer than a CTA's share;
+// One CTA.  Counts the items of each sequence, then their key tiles; cuts them by their part of the pieces to aim for;
 // writes the pieces, the longest first (64 bins of lengths).
 // And the maps of the layers' pools, from one that the host has made but for the address.
 __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_constant__ PromptParams p,
@@ -232,10 +242,11 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const __grid_
   }
   __syncthreads();
   const unsigned long long all = s_tiles * p.kv.heads_kv;
-  const int share = int(min((unsigned long long)0x40000000, max((unsigned long long)least, (all + p.share - 1) / p.share)));
-  const int top = min(share, s_longest);
-  const auto parts_of = [&](int n) { return n > share ? (n + share - 1) / share : 1; };
-  const auto bin_of = [&](int len) { return int(int64_t(top - len) * kBins / (top + 1)); };
+  // An item of n tiles: as many pieces as its part of p.share, rounded down, so that all together are no more than that.
+  const auto parts_of = [&](int n) { return n < 2 * least ? 1 : max(1, min(n / least, int(uint64_t(n) * p.share / all))); };
+  // (no piece is longer than two shares, or than two of the least)
+  const int top = int(min((unsigned long long)s_longest, max(2 * all / p.share + 2, 2ull * least)));
+  const auto bin_of = [&](int len) { return max(0, int(int64_t(top - len) * kBins / (top + 1))); };
   for (int i = tid; i < items; i += kPlanThreads) {
     const Item it = item(i, b);
     const int parts = parts_of(it.n);
@@ -290,7 +301,7 @@ struct Shape {
   static constexpr int kThreads = RAW ? 640 : 384;
   // Scores that a softmax thread reads at a time, in units of 32: all four, which it then keeps, or one at a time and twice.
   // Beside warps that decode, the short loop stays in the instruction caches and the long one does not (INT8: 920 and 1100
-  // us); alone the long one is faster (606 and 636).
+  // us); alone the long one is faster (606 and 636; each measured before queries came by tensor copies).
   static constexpr int kCols = RAW ? 1 : 4;
   // Registers without RAW: what the softmax warps take more than the launch gives, the others take less.
   static constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
@@ -1474,12 +1485,17 @@ Sizes sizes_of(int64_t n_rows, int64_t n_seqs, int heads_q, int heads_kv, int n_
   const int sms = sm_count() > 0 ? sm_count() : 148, group = heads_q / heads_kv;
   s.items = n_rows * group / kItemRows + n_seqs;
   s.part_rows = std::min<int64_t>(kItemRows, std::max<int64_t>(1, n_rows * group));
-  // Works that would leave the CTAs a fifth of their time idle are cut, into four for each CTA; else a piece more costs more
-  // (the queries come anew: 3 us) than it evens out (272 works: 370 us, cut into 1300: 396).
-  const int64_t works = s.items * heads_kv;
-  s.share = (works + sms - 1) / sms * sms * 4 > works * 5 ? 4 * sms : sms;
-  // an item of n tiles is cut where n exceeds a share: into at most 2 n / share pieces, share >= all tiles / s.share
-  s.parts = std::min<int64_t>(2 * int64_t(s.share) / heads_kv + 2, 2 * int64_t(s.share) + 2);
+  // A few pieces to a CTA, as few as fill the CTAs to 17 / 20 if the items are of one length: a piece more costs the queries anew,
+  // some 3 us (1 x 8 rows over 32768 tokens, 18 pieces of each key head's item 62 us, 64 pieces 108).
+  const int64_t works = std::max<int64_t>(1, s.items * heads_kv);
+  int64_t best = 0;
+  for (int k = 1; k <= 8; ++k) {
+    const int64_t cut = std::max<int64_t>(1, int64_t(k) * sms / works), waves = (works * cut + sms - 1) / sms;
+    const int64_t filled = works * cut * 1024 / (waves * sms);
+    if (filled > best) best = filled, s.share = k * sms;
+    if (best * 20 >= 17 * 1024) break;
+  }
+  s.parts = s.share / heads_kv + 1;
   s.pieces = s.items + s.parts;
   s.prefix = n_seqs + 1;
   s.maps = 2 * int64_t(n_layers);
@@ -1582,7 +1598,8 @@ extern "C" ashkv_status_t ashkv_prompt_attention(
   for (int t = 1; t < kTiers; ++t) stores |= p.kv.store[t].format != ASHKV_PAGE_NONE;
   const int sms = sm_count() > 0 ? sm_count() : 148;
   // Tensor copies where every page is in the pool and a box of eight rows or more, which a swizzled tile can take, never
-  // crosses a page.  The whole prompt of 8192 tokens, 32 / 8 heads of 128: see the numbers at the kernel.
+  // crosses a page.  One prompt of 8192 rows, 32 / 8 heads of 128: 488 us; by
+  // the warps that decode, which copy such rows too, 1100 before their loops were shortened.
   CUtensorMap pool{};
   if (!stores && p.kv.T % 8 == 0 && p.kv.pool_tokens > 0 && p.kv.pool_tokens < 0x7FFFFFFF) {
     p.box_rows = 8;
