@@ -468,8 +468,8 @@ __device__ void fetch_boxes(const PromptParams& p, Shared& sm, uint32_t base, in
     x.edge = edge_of(p, wa, wb, x.first);
     const uint32_t pos = uint32_t(x.first + group * box), j = p.by_page.of(pos);
     x.off = int(pos - j * uint32_t(p.kv.T));
-    const int last = int(pos) + box - 1;
-    x.wanted = active && int(pos) >= 0 && int(pos) <= wp.kmax && (!p.window || last >= wp.lo || int(pos) < p.sinks);
+    const uint32_t last = pos + uint32_t(box) - 1;
+    x.wanted = active && int(pos) >= 0 && int(pos) <= wp.kmax && (!p.window || last >= uint32_t(wp.lo) || int(pos) < p.sinks);
     x.id = -1;
     if (x.wanted) x.id = p.lists.page_ids[int64_t(wp.seq) * p.lists.page_ids_stride + j];
     if (++wi == wp.end) open(wk + 1);
@@ -515,10 +515,13 @@ __device__ void fetch_boxes(const PromptParams& p, Shared& sm, uint32_t base, in
       t.odd = 0;
     }
     const int layer = ok ? c.layer : 0, y = ok ? c.start + c.off : end;
-    if (layer != map_of) {
-      acquire_map(p.maps + int64_t(layer) * 256);
-      acquire_map(p.maps + int64_t(layer) * 256 + 128);
-      map_of = layer;
+    if (__any_sync(0xFFFFFFFFu, active && layer != map_of)) {
+#pragma unroll 1
+      for (int g = 0; g < boxes; ++g) {  // (every map by every lane: whichever issues the copies has to have done it)
+        map_of = __shfl_sync(0xFFFFFFFFu, layer, g);
+        acquire_map(p.maps + int64_t(map_of) * 256);
+        acquire_map(p.maps + int64_t(map_of) * 256 + 128);
+      }
     }
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
@@ -1598,8 +1601,8 @@ extern "C" ashkv_status_t ashkv_prompt_attention(
   for (int t = 1; t < kTiers; ++t) stores |= p.kv.store[t].format != ASHKV_PAGE_NONE;
   const int sms = sm_count() > 0 ? sm_count() : 148;
   // Tensor copies where every page is in the pool and a box of eight rows or more, which a swizzled tile can take, never
-  // crosses a page.  One prompt of 8192 rows, 32 / 8 heads of 128: 488 us; by
-  // the warps that decode, which copy such rows too, 1100 before their loops were shortened.
+  // crosses a page.  One prompt of 8192 rows, 32 / 8 heads of 128: 484 us; by
+  // the warps that decode, which copy such rows too, 705 (32 x 5 rows over 8192 tokens 254 and 301).
   CUtensorMap pool{};
   if (!stores && p.kv.T % 8 == 0 && p.kv.pool_tokens > 0 && p.kv.pool_tokens < 0x7FFFFFFF) {
     p.box_rows = 8;
