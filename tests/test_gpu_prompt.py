@@ -367,6 +367,34 @@ def test_odd_starts_and_lengths(cuda):
     check(out[:5], call([0, 20], [0, 0, 5])[1][:5], want, 128, 20)
 
 
+@pytest.mark.parametrize("tiers", list(FORMATS))
+@pytest.mark.parametrize("std", [2.0 ** -12, 1.0, 300.0])
+@pytest.mark.parametrize("T", [16, 4])
+def test_a_token_that_sees_itself_alone_gives_its_values(cuda, tiers, std, T):
+    """A weight of one: the decoded bf16 values, bit by bit what a dense read gives."""
+    n = 64
+    c = Cache(cuda, [FORMATS[tiers][i % len(FORMATS[tiers])] for i in range(n)], T, 4, 128, 27, std=std)
+    ids = i32(np.random.default_rng(27).permutation(n)[None], cuda)
+    args = (c.table, c.kv, c.stores, ids, i32([n * T], cuda), i32([0, n * T], cuda))
+    out = A.prompt_attention(rows_of(n * T, 8, 128, 27, cuda), *args, tokens_per_page=T, window=1, scale=2.0 ** -12)
+    keys, values = C.read_kv(*args, n * T, tokens_per_page=T)
+    finite = torch.isfinite(keys).all(-1) & torch.isfinite(values).all(-1)  # (FP8 pages hold NaN for values beyond 448)
+    assert finite.any() or std > 1
+    for h in range(8):
+        ok = finite[:, h // 2]
+        assert torch.equal(out[ok, h], values[ok, h // 2])
+
+
+@pytest.mark.parametrize("std,scale", [(2.0 ** 90, 2.0 ** -95), (2.0 ** -100, 1.0), (2.0 ** -60, 2.0 ** 55)])
+def test_value_ranges(cuda, std, scale):
+    c = Cache(cuda, [N.PAGE_BF16] * 20, 16, 2, 128, 28, std=std)
+    ids = np.arange(20, dtype=np.int32)[None]
+    q = rows_of(300, 8, 128, 28, cuda)
+    out, lse = A.prompt_attention(q, c.table, c.kv, None, i32(ids, cuda), i32([311], cuda), i32([0, 300], cuda), scale=scale,
+                                  return_lse=True)
+    check(out, lse, reference(c, ids, q.double().cpu().numpy(), [311], [300], scale=scale), 128, 312)
+
+
 def test_pages_shared_and_listed_twice(cuda):
     c = Cache(cuda, FORMATS["mixed"] * 2, 16, 2, 128, 17)
     ids = np.array([[3, 1, 3, 3, 0], [1, 1, 3, 2, 2]], np.int32)
