@@ -1545,7 +1545,7 @@ ashkv_status_t launch_prompt(const PromptParams& p, const CUtensorMap& pool, con
   launch_paged(prompt_kernel<D, RAW>, sms, Shape<D, RAW>::kThreads, Shape<D, RAW>::kBytes, stream, p, queries);
   const ashkv_status_t rc = check_launch(kName);
   if (rc != ASHKV_OK) return rc;
-  if (int64_t(p.lists.max_pages) * p.kv.T <= kLeastTiles * kTileKeys) return ASHKV_OK;  // nothing is long enough to be cut
+  if (int64_t(p.lists.max_pages) * p.kv.T <= (2 * kLeastTiles - 1) * kTileKeys) return ASHKV_OK;  // nothing is long enough to be cut
   launch_paged(prompt_join_kernel<D>, 4 * sms, kJoinThreadsP, 0, stream, p);
   return check_launch(kName);
 }

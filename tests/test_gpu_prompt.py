@@ -201,6 +201,11 @@ def test_long_contexts(cuda, tiers, lengths, new, window, sinks):
     run(cuda, FORMATS[tiers], 16, 8, 2, 128, lengths, new, 7, window, sinks)
 
 
+@pytest.mark.parametrize("pages", [55, 56, 57, 63, 64, 65])
+def test_around_the_first_cut(cuda, pages):
+    run(cuda, FORMATS["bf16"], 16, 8, 2, 128, [16 * pages, 16 * pages - 15], [3, 20], 29)
+
+
 @pytest.mark.parametrize("tiers", ["bf16", "int4"])
 @pytest.mark.parametrize("shift", [1, 4, 8])
 def test_query_alignment(cuda, tiers, shift):
@@ -216,6 +221,9 @@ def test_query_strides_and_out(cuda):
     assert A.prompt_attention(by_head, *args, out=to) is to and torch.equal(to, out)
     one = q[:, :1].expand(-1, 8, -1)  # a stride of zero
     assert torch.equal(A.prompt_attention(one, *args), A.prompt_attention(one.contiguous(), *args))
+    padded = torch.full((2, 19), 2 ** 30, dtype=torch.int32, device=cuda)
+    padded[:, 5:5 + ids.shape[1]] = args[3]
+    assert torch.equal(A.prompt_attention(q, *args[:3], padded[:, 5:5 + ids.shape[1]], *args[4:]), out)
     wide = torch.empty(83, 8, 192, dtype=torch.bfloat16, device=cuda)[..., :64].copy_(q)
     assert torch.equal(A.prompt_attention(wide, *args), out)
 
