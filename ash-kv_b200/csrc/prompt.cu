@@ -25,9 +25,10 @@
 // reaches, and the special function units 32768 exponentials, 1.1 us; the pair takes 2.2 us: the chain
 // scores -> weights -> product of one tile of rows does not quite fit beside the other's.  Figures (B200, graph replays,
 // 32 query heads over 8 of 128): 8192 rows of one prompt 488 us, 0.68 of that rate (tensor pipe busy 54 % of the cycles
-// under a profiler's clocks); 40 rows over 300 tokens 21 us, of which the plan takes 7; 4 x 2048 rows of 64 heads over INT8
-// pages, window 4096, 675 us (decoding beside the softmax: issue slots and instruction caches); 32 x 5 rows over 8192
-// tokens of FP8 351 us, of bf16 254 (128 rows are computed for 20).
+// under a profiler's clocks); 40 rows over 300 tokens 23 us, of which the plan takes 7; 4 x 2048 rows of 64 heads over INT8
+// pages, window 4096, 674 us (531 without the decoding's arithmetic, 541 without the softmax's, 426 without both: hand-overs
+// between the roles and the fetching warps' own instructions); 32 x 5 rows over 8192 tokens of FP8 322 us, of bf16 254
+// (128 rows are computed for 20).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -676,11 +677,11 @@ __device__ void fetch_tiles(const PromptParams& p, Shared& sm, uint32_t base, in
           for (uint32_t x = 0; x < B; ++x)
             if (l < chunks[x]) cp_async16(codes + (r + 32 / L * x) * D + l * 16, reinterpret_cast<const void*>(from[x] + l * 16));
         }
-        // the scales, a row a lane
+        // the scales, a row a lane (FP8 has none: 32 x 5 rows over 8192 tokens took 350 us when they were copied all the same, 322 now)
 #pragma unroll
         for (uint32_t x = 0; x < 4; ++x) {
           const uint32_t e = uint32_t(lane) + 32 * x, meta = t.meta[e];
-          if (!(meta >> 8 & 0xFFu)) continue;
+          if (!(meta >> 8 & 0xFFu) || (meta & 0xFFu) == ASHKV_PAGE_FP8) continue;
           const RowBytes at = row_bytes<D>(meta & 0xFFu, uint32_t(p.kv.T), uint32_t(p.kv.row_len), (meta >> 16) + v * uint32_t(p.kv.T), uint32_t(head));
           const void* from = reinterpret_cast<const void*>(t.row[v][e] - at.codes + at.scales);
           if (D == 128 && (meta & 0xFFu) >= ASHKV_PAGE_NBIT4) cp_async_small<8>(scales + e * 8, from);
